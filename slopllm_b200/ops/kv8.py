@@ -1,0 +1,277 @@
+"""An 8-bit paged key/value cache for grouped-query attention: norm, rotation and quantised write, reading back, attention of prompts and of
+single tokens.  It takes the place of the bf16 cache of `ops/dense.py` at half of its bytes (`--kv-dtype e4m3`).
+
+A token's row of one key head is `hd` e4m3 codes and one exponent byte b, for keys and for values; value = code * 2^(b - 127).  The exponent
+is the smallest between -60 and 60 with which the largest finite magnitude of the row is at most 448; larger values saturate, and a value that
+is not finite is the NaN code.  Codes lie at [slot, head, :] with slot = page * page_size + offset, exponent bytes at [page, head, 0 (keys) or
+1 (values), offset].
+
+CUDA tensors run `csrc/kv8.cu` and `csrc/kv8_attn.cu` (prompts: the tcgen05 kernel of `csrc/prefill_attn.cu` over rows read back, which bf16 holds
+exactly); CPU tensors run the fp32 definition below.
+"""
+from __future__ import annotations
+
+import ctypes as C
+from dataclasses import dataclass
+from typing import Optional, Tuple
+
+import torch
+
+from . import reference as R
+from .dense import AttnParams, _slots
+from .rotary import RotaryTable
+
+LOW, HIGH, BIAS = -60, 60, 127         # limits of the exponent, and what is added to it in its byte
+UNPACK_BUDGET_BYTES = 1 << 30          # transient bf16 rows of a prompt step; more sequences go in groups
+
+
+def _native():
+    from . import native as N
+    return N
+
+
+class _Pages(C.Structure):
+    _fields_ = [("page_table", C.c_void_p), ("pt_stride", C.c_int), ("pt_rows", C.c_int), ("pt_width", C.c_int), ("page_size", C.c_int),
+                ("num_slots", C.c_int), ("guard", C.c_void_p)]
+
+
+class Kv8StoreParams(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("ldq", C.c_int), ("k", C.c_void_p), ("ldk", C.c_int), ("v", C.c_void_p), ("ldv", C.c_int),
+                ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("freq", C.c_void_p), ("gain", C.c_float), ("rot_dims", C.c_int),
+                ("positions", C.c_void_p), ("batch_idx", C.c_void_p), ("pages", _Pages), ("n_heads", C.c_int), ("n_kv", C.c_int),
+                ("hd", C.c_int), ("q_stride", C.c_int), ("eps", C.c_float), ("q_out", C.c_void_p), ("k_codes", C.c_void_p),
+                ("v_codes", C.c_void_p), ("exps", C.c_void_p)]
+
+
+class _Rows(C.Structure):
+    _fields_ = [("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("exps", C.c_void_p), ("pages", _Pages), ("n_kv", C.c_int), ("hd", C.c_int)]
+
+
+class Kv8ReadParams(C.Structure):
+    _fields_ = [("c", _Rows), ("ranges", C.c_void_p), ("rows", C.c_int), ("k", C.c_void_p), ("v", C.c_void_p)]
+
+
+class Kv8UnpackParams(C.Structure):
+    _fields_ = [("c", _Rows), ("qo_indptr", C.c_void_p), ("positions", C.c_void_p), ("batch_idx", C.c_void_p), ("per_seq", C.c_int),
+                ("k", C.c_void_p), ("v", C.c_void_p), ("table", C.c_void_p), ("rows_out", C.c_void_p), ("positions_out", C.c_void_p)]
+
+
+class Kv8DecodeParams(C.Structure):
+    _fields_ = [("q", C.c_void_p), ("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("exps", C.c_void_p), ("positions", C.c_void_p),
+                ("batch_idx", C.c_void_p), ("pages", _Pages), ("n_heads", C.c_int), ("n_kv", C.c_int), ("hd", C.c_int), ("scale", C.c_float),
+                ("out", C.c_void_p)]
+
+
+@dataclass
+class Kv8Cache:
+    """One layer's cache.  `k`, `v`: uint8 [slots, n_kv, hd] e4m3 codes; `exps`: uint8 [pages, n_kv, 2, page_size]."""
+
+    k: torch.Tensor
+    v: torch.Tensor
+    exps: torch.Tensor
+
+    def __post_init__(self):
+        slots, n_kv, hd = self.k.shape
+        pages, heads, two, page_size = self.exps.shape
+        if self.v.shape != self.k.shape or (pages * page_size, heads, two) != (slots, n_kv, 2):
+            raise ValueError(f"codes {tuple(self.k.shape)} and {tuple(self.v.shape)} do not go with exponents {tuple(self.exps.shape)}")
+        if hd % 16 or not 16 <= hd <= 256 or page_size % 16 or not page_size:
+            raise ValueError(f"heads of {hd} values in pages of {page_size} tokens: the 8-bit cache takes multiples of 16, heads of up to 256")
+        for x in (self.k, self.v, self.exps):
+            if x.dtype != torch.uint8 or not x.is_contiguous() or x.device != self.k.device:
+                raise ValueError("the tensors of an 8-bit cache are contiguous, of type uint8 and on one device")
+        if (self.k.data_ptr() | self.v.data_ptr() | self.exps.data_ptr()) % 16:
+            raise ValueError("the tensors of an 8-bit cache start at multiples of 16 bytes")
+
+    @property
+    def page_size(self) -> int:
+        return self.exps.shape[3]
+
+    @staticmethod
+    def allocate(num_pages: int, page_size: int, n_kv: int, hd: int, device) -> "Kv8Cache":
+        codes = lambda: torch.zeros(num_pages * page_size, n_kv, hd, dtype=torch.uint8, device=device)
+        return Kv8Cache(codes(), codes(), torch.zeros(num_pages, n_kv, 2, page_size, dtype=torch.uint8, device=device))
+
+
+def _check_step(x: torch.Tensor, cache: Kv8Cache, *tables: torch.Tensor) -> None:
+    """Tables of a step are int32 on the device of `x` and the cache, with values side by side."""
+    for t in tables:
+        if t.dtype != torch.int32 or t.device != x.device or (t.shape[-1] > 1 and t.stride(-1) != 1):
+            raise ValueError("positions, rows, ranges and page tables are int32, on the device of the data, with values side by side")
+    if cache.k.device != x.device:
+        raise ValueError(f"data on {x.device}, cache on {cache.k.device}")
+
+
+def _pages(cache: Kv8Cache, page_table: torch.Tensor) -> _Pages:
+    from . import tcgen05
+    rows, width = page_table.shape
+    return _Pages(page_table.data_ptr(), page_table.stride(0), rows, width, cache.exps.shape[3], cache.k.shape[0],
+                  tcgen05.error_flag(cache.k.device).data_ptr() + 16)
+
+
+def _rows(cache: Kv8Cache, page_table: torch.Tensor) -> _Rows:
+    return _Rows(cache.k.data_ptr(), cache.v.data_ptr(), cache.exps.data_ptr(), _pages(cache, page_table), cache.k.shape[1], cache.k.shape[2])
+
+
+def _call(x: torch.Tensor, name: str, *args) -> None:
+    """A kernel call on the stream and device of `x`."""
+    N = _native()
+    if x.get_device() == torch.cuda.current_device():
+        N.call(name, *args, N.stream())
+    else:
+        with torch.cuda.device(x.device):
+            N.call(name, *args, N.stream())
+
+
+# ---- the format ----------------------------------------------------------------------------------------------------------------------
+
+def kv8_quantize(x: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """fp32 rows [..., hd] -> (e4m3 codes, exponent bytes [...]), both uint8 (the definition)."""
+    x = torch.where(x.isfinite(), x, torch.full_like(x, float("nan")))
+    m, e = torch.frexp(x.nan_to_num(0.0).abs().amax(-1))
+    e = torch.where(m == 0, torch.full_like(e, LOW), (e - 9 + (m > 0.875)).clamp(LOW, HIGH))
+    codes = torch.ldexp(x, -e[..., None]).clamp(-448.0, 448.0).to(torch.float8_e4m3fn).view(torch.uint8)
+    return codes, (e + BIAS).to(torch.uint8)
+
+
+def kv8_values(codes: torch.Tensor, exps: torch.Tensor) -> torch.Tensor:
+    """The fp32 values of codes [..., hd] with exponent bytes [...]."""
+    return torch.ldexp(codes.view(torch.float8_e4m3fn).to(torch.float32), (exps.to(torch.int32) - BIAS)[..., None])
+
+
+def _cached(cache: Kv8Cache, slots: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """fp32 keys and values [n, n_kv, hd] of slots."""
+    e = cache.exps[slots // cache.page_size, :, :, slots % cache.page_size]
+    return kv8_values(cache.k[slots], e[..., 0]), kv8_values(cache.v[slots], e[..., 1])
+
+
+# ---- operators -----------------------------------------------------------------------------------------------------------------------
+
+def kv8_store(q, k, v, q_norm, k_norm, rot: RotaryTable, positions, batch_idx, page_table, cache: Kv8Cache, n_heads: int, eps: float,
+              q_stride: Optional[int] = None) -> torch.Tensor:
+    """:func:`~slopllm_b200.ops.dense.qk_norm_rope_cache` for the 8-bit cache: per-head RMS norm (weights [hd], or None) and rotation of the first
+    `rot.dims` values of queries and keys; key and value rows go into their places quantised.  q [T, n_heads * q_stride] (head h starts at
+    h * q_stride), k / v [T, n_kv * hd], bf16 on a GPU with rows of any stride.  Everything is fp32 between the rows and the one rounding of a
+    result (angles: position * frequency in 64 bits).  A token whose position is negative leaves the cache as it is.  Returns
+    the queries [T, n_heads, hd]."""
+    T, (_, n_kv, hd) = q.shape[0], cache.k.shape
+    q_stride = hd if q_stride is None else q_stride
+    if q.shape[1] != n_heads * q_stride or q_stride < hd or k.shape != (T, n_kv * hd) or v.shape != k.shape:
+        raise ValueError(f"projections {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)} for {n_heads} heads over {n_kv} of {hd} values")
+    if rot.dims > hd or rot.freq.numel() != rot.dims // 2 or rot.dims % 2:
+        raise ValueError(f"{rot.dims} rotated values with {rot.freq.numel()} frequencies in heads of {hd}")
+    if positions.shape != (T,) or batch_idx.shape != (T,):
+        raise ValueError(f"{T} tokens with positions {tuple(positions.shape)} and rows {tuple(batch_idx.shape)}")
+    _check_step(q, cache, positions, batch_idx, page_table)
+    if q.is_cuda:
+        for x in (q, k, v, q_norm, k_norm):
+            if x is not None and (x.dtype != torch.bfloat16 or x.device != q.device or x.stride(-1) != 1):
+                raise ValueError("projection rows and norm weights are bf16, on one device, with values side by side")
+        if rot.freq.dtype != torch.float32 or rot.freq.device != q.device or not rot.freq.is_contiguous():
+            raise ValueError("frequencies are fp32, contiguous and on the device of the data")
+        N = _native()
+        out = torch.empty(T, n_heads, hd, dtype=torch.bfloat16, device=q.device)
+        p = Kv8StoreParams(q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), N.ptr(q_norm), N.ptr(k_norm),
+                           rot.freq.data_ptr(), rot.gain, rot.dims, positions.data_ptr(), batch_idx.data_ptr(), _pages(cache, page_table),
+                           n_heads, n_kv, hd, q_stride, eps, out.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.exps.data_ptr())
+        _call(q, "sl_kv8_store", C.byref(p), T)
+        return out
+
+    def turned(x, w):
+        x = x.to(torch.float32)
+        if w is not None:
+            x = R.rmsnorm(x, w, eps)
+        half, ang = rot.dims // 2, (positions.double()[:, None] * rot.freq.double())[:, None]
+        cos, sin = (ang.cos() * rot.gain).float(), (ang.sin() * rot.gain).float()
+        a, b = x[..., :half], x[..., half:rot.dims]
+        return torch.cat([a * cos - b * sin, b * cos + a * sin, x[..., rot.dims:]], -1)
+
+    on = positions >= 0
+    slots = _slots(positions[on], batch_idx[on], page_table, cache.page_size)
+    for which, (codes, x) in enumerate(((cache.k, turned(k.reshape(T, n_kv, hd), k_norm)), (cache.v, v.reshape(T, n_kv, hd).to(torch.float32)))):
+        c, e = kv8_quantize(x[on])
+        codes[slots] = c
+        cache.exps[slots // cache.page_size, :, which, slots % cache.page_size] = e
+    return turned(q.reshape(T, n_heads, q_stride)[..., :hd], q_norm).to(q.dtype)
+
+
+def kv8_read(cache: Kv8Cache, ranges: torch.Tensor, rows: int, longest: int, page_table: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Cached keys and values [rows, n_kv, hd] in bf16, which holds them exactly.  `ranges` int32 [R, 4]: page-table row, first position, number
+    of tokens (at most `longest`), first row of the result; rows in no range are not written."""
+    if ranges.dim() != 2 or ranges.shape[1] != 4 or not ranges.is_contiguous():
+        raise ValueError(f"ranges are [R, 4] and contiguous, not {tuple(ranges.shape)}")
+    _check_step(ranges, cache, ranges, page_table)
+    _, n_kv, hd = cache.k.shape
+    k, v = (torch.empty(rows, n_kv, hd, dtype=torch.bfloat16, device=cache.k.device) for _ in range(2))
+    if ranges.is_cuda:
+        p = Kv8ReadParams(_rows(cache, page_table), ranges.data_ptr(), rows, k.data_ptr(), v.data_ptr())
+        _call(k, "sl_kv8_read", C.byref(p), ranges.shape[0], longest)
+        return k, v
+    for b, first, n, row in ranges.tolist():
+        pos = torch.arange(first, first + n)
+        kv = _cached(cache, _slots(pos, torch.full_like(pos, b), page_table, cache.page_size))
+        k[row:row + n], v[row:row + n] = kv
+    return k, v
+
+
+def kv8_attention(q, cache: Kv8Cache, positions, batch_idx, page_table, sm_scale: float, qo_indptr: Optional[torch.Tensor] = None, max_q: int = 0,
+                  max_kv_len: int = 0) -> torch.Tensor:
+    """:func:`~slopllm_b200.ops.dense.paged_attention` over the 8-bit cache: causal attention of each query token (position positions[t],
+    page-table row batch_idx[t]) over the keys 0..position of its sequence.  q [T, n_heads, hd], bf16 on a GPU -> [T, n_heads, hd].  With
+    `qo_indptr` ([B + 1], contiguous token ranges of the sequences, at most `max_q` tokens and `max_kv_len` keys each; 0: not known) heads have 64
+    or 128 values on a GPU; without it a row may have no keys (position -1), and is zero."""
+    T, n_heads, hd = q.shape
+    _, n_kv, width = cache.k.shape
+    if hd != width or n_heads % n_kv:
+        raise ValueError(f"{n_heads} query heads of {hd} values over {n_kv} key heads of {width}")
+    if positions.shape != (T,) or batch_idx.shape != (T,):
+        raise ValueError(f"{T} tokens with positions {tuple(positions.shape)} and rows {tuple(batch_idx.shape)}")
+    _check_step(q, cache, positions, batch_idx, page_table, *(() if qo_indptr is None else (qo_indptr,)))
+    if not q.is_cuda:
+        out = torch.zeros(T, n_heads, hd, dtype=torch.float32)
+        for t in range(T):
+            n = int(positions[t]) + 1
+            kp = torch.arange(n)
+            if n:
+                k, v = _cached(cache, _slots(kp, torch.full_like(kp, int(batch_idx[t])), page_table, cache.page_size))
+                out[t] = R.dense_attention(q[t:t + 1], k, v, sm_scale, causal_offset=n - 1)[0]
+        return out.to(q.dtype)
+    if q.dtype != torch.bfloat16:
+        raise ValueError(f"queries of type {q.dtype}: the kernels take bf16")
+    if not q.is_contiguous() or q.data_ptr() % 16:
+        q = q.clone(memory_format=torch.contiguous_format)
+    out = torch.empty(T, n_heads, hd, dtype=torch.bfloat16, device=q.device)
+    if T == 0:
+        return out
+    if qo_indptr is None:
+        p = Kv8DecodeParams(q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.exps.data_ptr(), positions.data_ptr(), batch_idx.data_ptr(),
+                            _pages(cache, page_table), n_heads, n_kv, hd, sm_scale, out.data_ptr())
+        _call(q, "sl_kv8_decode", C.byref(p), T)
+        return out
+    if hd not in (64, 128):
+        raise ValueError(f"heads of {hd} values: attention of prompts takes 64 or 128")
+    _prompts(q, cache, positions, batch_idx, page_table, sm_scale, qo_indptr, max_q or T, max_kv_len, out)
+    return out
+
+
+def _prompts(q, cache, positions, batch_idx, page_table, sm_scale, qo_indptr, max_q, max_kv_len, out) -> None:
+    """Histories are read back into bf16 pages of 64 tokens, over which the prompt kernel attends.  Done once per key head and token, that
+    costs less than codes that every block of the kernel (query heads x 128 queries) turns into an operand anew."""
+    from . import tcgen05
+    T, n_heads, hd = q.shape
+    n_kv, B, dev = cache.k.shape[1], qo_indptr.numel() - 1, q.device
+    most = page_table.shape[1] * cache.page_size
+    per_seq = max(1, -(-min(max_kv_len or most, most) // 64))
+    group = max(1, min(B, UNPACK_BUDGET_BYTES // (per_seq * 64 * n_kv * hd * 4)))
+    k, v = (torch.empty(group * per_seq * 64, n_kv, hd, dtype=torch.bfloat16, device=dev) for _ in range(2))
+    ints = torch.empty(group * per_seq + 2 * T, dtype=torch.int32, device=dev)
+    table, rows_out, positions_out = ints.data_ptr(), ints.data_ptr() + 4 * group * per_seq, ints.data_ptr() + 4 * (group * per_seq + T)
+    rows = _rows(cache, page_table)
+    for s in range(0, B, group):
+        n, ends = min(group, B - s), qo_indptr.data_ptr() + 4 * s
+        up = Kv8UnpackParams(rows, ends, positions.data_ptr(), batch_idx.data_ptr(), per_seq, k.data_ptr(), v.data_ptr(), table, rows_out, positions_out)
+        _call(q, "sl_kv8_unpack", C.byref(up), n)
+        p = AttnParams(q=q.data_ptr(), k_cache=k.data_ptr(), v_cache=v.data_ptr(), positions=positions_out, batch_idx=rows_out, page_table=table,
+                       pt_stride=per_seq, page_size=64, qo_indptr=ends, n_heads=n_heads, n_kv=n_kv, hd=hd, sm_scale=sm_scale, out=out.data_ptr(), T=T,
+                       num_slots=k.shape[0], max_keys=max_kv_len, err=tcgen05.error_flag(dev).data_ptr())
+        _call(q, "sl_paged_attn_prefill", C.byref(p), n, int(max_q))
