@@ -1,7 +1,23 @@
-// Attention of one new token per sequence over the 8-bit key/value cache (kv8.cuh).
+// Attention of one new token per sequence over the 8-bit key/value cache (kv8.cuh): every cached byte is read once, so what counts is bytes in
+// flight and few instructions a byte.
 //
-//  * kv8_rows_kernel: one query head and token a block, on the CUDA cores.
+// All histories are cut into tiles of 64 keys of one key head (and of up to 8 or 16 of its query heads); the tiles of the whole batch, one
+// history behind the other, are dealt out to the blocks in equal shares, so that a batch of ragged histories, one long history and many short ones
+// fill the device alike.  A history that lies in several shares leaves a partial result in each, which kv8_merge_kernel joins.
+//
+// kv8_decode_kernel: a fetching warp brings tiles (TMA, swizzled) and their exponent bytes through a ring of stages, also across the ends of
+// histories; four warps take 16 keys of a tile each, with softmax states of their own and no barrier before a history's end.
+//
+//   S^T = K Q^T      keys are the 16-row operand: a lane's 16 bytes of two keys are four steps of the product as they lie, since any order
+//                    of the summed dims will do that the queries follow
+//   O^T += V^T P^T   a lane's 16 bytes of four keys, two keys' bytes interleaved, are the operand of 8 products: its rows are those dims
+//
+// e4m3 codes become fp16 exactly (mma.sync f16, fp32 sums); the queries are fp16 times a power of two per head, which loses less than 2^-24 of
+// the largest value.  The keys' scales go onto the scores.  The values' scales go into the weights: the reference of a row is the maximum of
+// score + exponent (in powers of two), so weights times scales are at most 1, and the denominator takes the scale out again.  Weights are two fp16
+// terms (21 bits).
 #include "kv8.cuh"
+#include "tcgen05.cuh"
 
 namespace {
 
@@ -13,64 +29,509 @@ struct Kv8DecodeParams {
     int n_heads, n_kv, hd;
     float scale;
     bf16* out;                           // [T, n_heads, hd]
+    float *o_part, *lse_part;            // [blocks, 2, rows, width], [blocks, 2, rows]
+    int T;
+    int* err;                            // error word of bounded waits
 };
 
-constexpr int KT = 64;
+constexpr int KT = 64, WARPS = 4, THREADS = WARPS * 32 + 32, MAX_T = 1024;
 
-// grid (heads, T), block 128
-__global__ void __launch_bounds__(128) kv8_rows_kernel(Kv8DecodeParams p) {
+__device__ __forceinline__ uint32_t transposed8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ void mma_f16_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+// Four e4m3 codes -> fp16 pairs (bytes 0 and 1, bytes 2 and 3).
+__device__ __forceinline__ void e4m3x4_to_f16(uint32_t w, uint32_t& lo, uint32_t& hi) {
+    asm("{ .reg .b16 a, b; mov.b32 {a, b}, %2; cvt.rn.f16x2.e4m3x2 %0, a; cvt.rn.f16x2.e4m3x2 %1, b; }" : "=r"(lo), "=r"(hi) : "r"(w));
+}
+__device__ __forceinline__ uint32_t f2_to_f16x2(float a, float b) {
+    const __half2 h = __floats2half2_rn(a, b);
+    return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// The batch's tiles, numbered token by token, key head (and group of query heads) by key head, tile by tile.
+struct Tiles {
+    const int* before;                   // [T + 1] tiles of one key head in front of a token
+    int T, items;                        // key heads x groups of query heads
+    int blocks;                          // that get a share
+
+    __device__ __forceinline__ long long total() const { return (long long)before[T] * items; }
+    __device__ __forceinline__ long long begin(int b) const { return total() * b / blocks; }
+    struct Place { int t, item, tile, n; };          // n: tiles of the item
+    __device__ __forceinline__ Place at(long long w) const {
+        const int x = (int)(w / items);
+        int lo = 0, hi = T;                          // the last token with before <= x (tokens without tiles lie in front of it)
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (before[mid] <= x) lo = mid;
+            else hi = mid;
+        }
+        const int n = before[lo + 1] - before[lo], off = (int)(w - (long long)before[lo] * items);
+        return {lo, off / n, off % n, n};
+    }
+};
+
+// Fills `before` (shared, T + 1) and returns the numbering; all threads of the block.
+__device__ __forceinline__ Tiles number_tiles(int* before, const int* positions, int T, int items, int blocks, int per_block) {
+    for (int t = threadIdx.x; t < T; t += blockDim.x) before[t + 1] = positions[t] < 0 ? 0 : positions[t] / KT + 1;
+    if (threadIdx.x == 0) before[0] = 0;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        int sum = 0;
+        for (int t0 = 1; t0 <= T; t0 += 32) {
+            const int t = t0 + threadIdx.x;
+            int x = t <= T ? before[t] : 0;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, x, o);
+                if ((int)threadIdx.x >= o) x += y;
+            }
+            if (t <= T) before[t] = sum + x;
+            sum += __shfl_sync(0xffffffffu, x, 31);
+        }
+    }
+    __syncthreads();
+    Tiles tl{before, T, items, 1};
+    tl.blocks = (int)max(1ll, min((long long)blocks, (tl.total() + per_block - 1) / per_block));
+    return tl;
+}
+
+template <int D, int NG>
+struct Cfg {
+    static constexpr int ROW = D < 128 ? D : 128, HALVES = D / ROW;      // bytes of a row in one box, boxes
+    static constexpr int STAGES = D == 64 ? 6 : D == 128 ? 3 : 2, HG = 8 * NG, LO = D + 4;
+    static constexpr int CODES = KT * D, STAGE = 2 * CODES;              // keys, values
+    static constexpr int EXPS = STAGES * STAGE;                          // 64 bytes of the keys, 64 of the values
+    static constexpr int JOIN = EXPS + STAGES * 2 * KT;                  // fp32 [WARPS][HG][LO], then [2][WARPS][HG]
+    static constexpr int BEFORE = JOIN + (WARPS * HG * LO + 2 * WARPS * HG) * 4;
+    static constexpr int BARS = (BEFORE + (MAX_T + 1) * 4 + 7) / 8 * 8;
+    static constexpr int TOTAL = BARS + 2 * STAGES * 8;
+    static constexpr int PER_SM = D == 128 && NG == 1 ? 3 : D == 64 && NG == 1 ? 3 : 2;
+    static constexpr int CHUNK = D < 128 ? 8 : 16;                       // neighbouring dims of a lane
+};
+
+// grid: blocks of the device, block 160
+template <int D, int NG>
+__global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                                               Kv8DecodeParams p, int box, int per_block) {
+    using M = Cfg<D, NG>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
+    uint64_t *full = reinterpret_cast<uint64_t*>(smem + M::BARS), *free_ = full + M::STAGES;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    if (tid == 0) {
+        for (int i = 0; i < M::STAGES; ++i) {
+            tc::mbar_init(full + i, 1);
+            tc::mbar_init(free_ + i, WARPS);
+        }
+        tc::mbar_fence_init();
+    }
     pdl_grid_sync();
-    __shared__ float q[256], sc[KT], vs[KT], scratch[33];
-    __shared__ int slots[KT];
-    const int h = blockIdx.x, t = blockIdx.y, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, hkv = h / (p.n_heads / p.n_kv);
-    const size_t at = ((size_t)t * p.n_heads + h) * p.hd, row = (size_t)p.n_kv * p.hd;
-    for (int d = tid; d < p.hd; d += 128) q[d] = __bfloat162float(p.q[at + d]);
-    const int n = p.positions[t] + 1, b = p.batch_idx[t];
-    float m = -INFINITY, l = 0.f, o[2] = {0.f, 0.f};
-    for (int k0 = 0; k0 < n; k0 += KT) {
-        const int nk = min(KT, n - k0);
-        __syncthreads();
-        if (tid < nk) {
-            const int s = kv8_slot(p.pages, 32, b, k0 + tid);
-            slots[tid] = s;
-            vs[tid] = s < 0 ? 0.f : __uint_as_float((uint32_t)p.exps[kv8_exp_at(p.pages, p.n_kv, s, hkv) + p.pages.page_size] << 23);
+    const int group = p.n_heads / p.n_kv, hg = (group + M::HG - 1) / M::HG;
+    const Tiles tiles = number_tiles(reinterpret_cast<int*>(smem + M::BEFORE), p.positions, p.T, p.n_kv * hg, gridDim.x, per_block);
+    for (int t = blockIdx.x; t < p.T; t += gridDim.x)
+        if (p.positions[t] < 0)
+            for (int i = tid; i < p.n_heads * p.hd / 2; i += THREADS) reinterpret_cast<uint32_t*>(p.out + (size_t)t * p.n_heads * p.hd)[i] = 0u;
+    if (blockIdx.x >= tiles.blocks) return;
+    const long long w0 = tiles.begin(blockIdx.x), w1 = tiles.begin(blockIdx.x + 1);
+    if (w0 >= w1) return;
+
+    if (warp == WARPS) {
+        // ---- fetching: a lane looks up the place of one box of a tile ahead ----
+        const int subs = KT / box, batch = 32 / subs;
+        const bool one = p.pages.page_size == box;               // a box's exponent bytes of keys and values are neighbours
+        auto look = [&](long long w, int& row, int& head) {
+            row = -2;                                            // nothing to fetch
+            head = 0;
+            if (w >= w1) return;
+            const Tiles::Place at = tiles.at(w);
+            const int key = at.tile * KT + lane % subs * box;
+            head = at.item / hg;
+            if (key <= p.positions[at.t]) row = kv8_slot(p.pages, 32, p.batch_idx[at.t], key);
+        };
+        int row, head, nrow, nhead, issued = 0;
+        bool ok = true;
+        look(w0 + lane / subs, nrow, nhead);
+        for (long long w = w0; w < w1 && ok; w += batch) {
+            row = nrow;
+            head = nhead;
+            look(w + batch + lane / subs, nrow, nhead);
+            const int n = (int)min((long long)batch, w1 - w);
+            for (int i = 0; i < n; ++i, ++issued) {
+                const int st = issued % M::STAGES;
+                if (issued >= M::STAGES && !tc::mbar_wait_warp(free_ + st, (uint32_t)(issued / M::STAGES + 1) & 1)) { ok = false; break; }
+                const uint32_t there = __ballot_sync(0xffffffffu, row > -2 && lane / subs == i);
+                if (lane == 0) tc::mbar_expect_tx(full + st, __popc(there) * box * (2 * D + 2));
+                uint8_t* codes = smem + st * M::STAGE;
+                uint8_t* exps = smem + M::EXPS + st * 2 * KT;
+                for (int u = 0; u < subs; ++u) {
+                    const int r = __shfl_sync(0xffffffffu, row, i * subs + u), h = __shfl_sync(0xffffffffu, head, i * subs + u);
+                    if (r > -2 && lane == 0) {
+#pragma unroll
+                        for (int x = 0; x < M::HALVES; ++x) {    // (a page that is not there: rows in front of the tensor read as zeros)
+                            tc::tma_load_3d(codes + x * KT * M::ROW + u * box * M::ROW, &map_k, full + st, x * 128, h, r < 0 ? -KT : r);
+                            tc::tma_load_3d(codes + M::CODES + x * KT * M::ROW + u * box * M::ROW, &map_v, full + st, x * 128, h, r < 0 ? -KT : r);
+                        }
+                        const uint8_t* e = p.exps + kv8_exp_at(p.pages, p.n_kv, max(r, 0), h);
+                        if (one && box == KT) {
+                            tc::bulk_load_1d(exps, e, 2 * KT, full + st);
+                        } else {
+                            tc::bulk_load_1d(exps + u * box, e, box, full + st);
+                            tc::bulk_load_1d(exps + KT + u * box, e + p.pages.page_size, box, full + st);
+                        }
+                    }
+                }
+                __syncwarp();
+            }
         }
-        __syncthreads();
-        for (int k = warp; k < nk; k += 4) {
-            const int s = slots[k];
-            float a = 0.f;
-            if (s >= 0)
-                for (int d = lane; d < p.hd; d += 32) a += q[d] * e4m3_to_float(p.k_codes[(size_t)s * row + (size_t)hkv * p.hd + d]);
-            a = warp_sum(a);
-            if (lane == 0) sc[k] = s < 0 ? 0.f : a * __uint_as_float((uint32_t)p.exps[kv8_exp_at(p.pages, p.n_kv, s, hkv)] << 23) * p.scale;
-        }
-        __syncthreads();
-        const float top = fmaxf(m, block_max(tid < nk ? sc[tid] : -FLT_MAX, scratch));
-        const float e = tid < nk ? expf(sc[tid] - top) : 0.f, f = m == -INFINITY ? 0.f : expf(m - top);
-        l = l * f + block_sum(e, scratch);
-        m = top;
-        if (tid < nk) sc[tid] = e * vs[tid];
-        __syncthreads();
-        for (int i = 0; i < 2; ++i) {
-            const int d = tid + i * 128;
-            if (d >= p.hd) break;
-            float a = o[i] * f;
-            for (int k = 0; k < nk; ++k)
-                if (slots[k] >= 0) a += sc[k] * e4m3_to_float(p.v_codes[(size_t)slots[k] * row + (size_t)hkv * p.hd + d]);
-            o[i] = a;
-        }
+        // nothing is in flight when the block ends, also where a wait ran out
+        for (int j = max(0, issued - M::STAGES); j < issued; ++j) ok &= tc::mbar_wait_warp(full + j % M::STAGES, (uint32_t)(j / M::STAGES) & 1);
+        if (!ok && lane == 0) atomicExch(p.err, 50);
+        return;
     }
-    for (int i = 0; i < 2; ++i) {
-        const int d = tid + i * 128;
-        if (d < p.hd) p.out[at + d] = __float2bfloat16(n > 0 ? o[i] / l : 0.f);
+
+    // ---- products: 16 keys of every tile ----
+    const int g = lane >> 2, c4 = lane & 3, k0 = warp * 16;
+    float* const so = reinterpret_cast<float*>(smem + M::JOIN);
+    float* const sm = so + WARPS * M::HG * M::LO;                    // references, then sums
+    constexpr int MT = D / 16, CH = D < 128 ? 1 : D / 64;            // 16-dim rows of products, 16-byte pieces of a key row a lane reads
+    // places of a lane's pieces in a tile
+    const int ks = D < 128 ? (k0 + g) * 64 + ((c4 ^ (g >> 1 & 3)) << 4) : (k0 + g) * 128;
+    int st = 0;
+    uint32_t phase = 0;
+    bool ok = true;
+    for (long long w = w0; w < w1;) {
+        const Tiles::Place at = tiles.at(w);
+        const int count = (int)min((long long)(at.n - at.tile), w1 - w), t = at.t, hkv = at.item / hg, r_lo = at.item % hg * M::HG;
+        const int nr = min(M::HG, group - r_lo), h0 = hkv * group + r_lo, keys = p.positions[t] + 1;
+        // queries as fp16 times 2^-eq: a lane holds head g's dims of its pieces, in the order of the pieces' bytes
+        uint32_t q[NG][CH * 4][2];
+        float qf[NG][2];                                             // factors on the scores of heads 2 c4 and 2 c4 + 1
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+            const bf16* src = p.q + ((size_t)t * p.n_heads + h0 + n * 8 + g) * p.hd;
+            uint4 raw[CH][2];
+            float top = 0.f;
+#pragma unroll
+            for (int j = 0; j < CH; ++j) {
+                const int d = D < 128 ? c4 * 16 : (j >> 1) * 128 + (2 * c4 + (j & 1)) * 16;
+                raw[j][0] = raw[j][1] = make_uint4(0u, 0u, 0u, 0u);
+                if (n * 8 + g < nr && d < p.hd) {
+                    raw[j][0] = *reinterpret_cast<const uint4*>(src + d);
+                    raw[j][1] = *reinterpret_cast<const uint4*>(src + d + 8);
+                }
+                const uint32_t* u = reinterpret_cast<const uint32_t*>(raw[j]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float2 f = bf162_to_f2(u[i]);
+                    top = fmaxf(top, fmaxf(fabsf(f.x), fabsf(f.y)));
+                }
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            const int eq = max(-100, (int)(__float_as_uint(top) >> 23) - 127 - 13);          // the largest value: 2^13 to 2^14
+            const float down = __uint_as_float((uint32_t)(127 - eq) << 23);
+            const float f = __uint_as_float((uint32_t)(127 + eq) << 23) * (p.scale * 1.4426950408889634f);
+            qf[n][0] = __shfl_sync(0xffffffffu, f, c4 * 8);
+            qf[n][1] = __shfl_sync(0xffffffffu, f, c4 * 8 + 4);
+#pragma unroll
+            for (int j = 0; j < CH; ++j) {
+                const uint32_t* u = reinterpret_cast<const uint32_t*>(raw[j]);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float2 x = bf162_to_f2(u[i]);
+                    q[n][j * 4 + i / 2][i & 1] = f2_to_f16x2(x.x * down, x.y * down);
+                }
+            }
+        }
+        float m[NG][2], l[NG][2], acc[NG][MT][4];                    // heads 2 c4 and 2 c4 + 1
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+            m[n][0] = m[n][1] = -INFINITY;
+            l[n][0] = l[n][1] = 0.f;
+#pragma unroll
+            for (int i = 0; i < MT; ++i) acc[n][i][0] = acc[n][i][1] = acc[n][i][2] = acc[n][i][3] = 0.f;
+        }
+        for (int j = at.tile; j < at.tile + count; ++j) {
+            if (ok) ok = tc::mbar_wait_warp(full + st, phase);
+            const uint8_t *kt = smem + st * M::STAGE, *vt = kt + M::CODES, *exps = smem + M::EXPS + st * 2 * KT;
+            const int nk = keys - j * KT - k0;                       // of this warp's 16
+            if (nk > 0) {
+                float s[NG][4];
+#pragma unroll
+                for (int n = 0; n < NG; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+#pragma unroll
+                for (int x = 0; x < CH; ++x) {
+                    const uint8_t* a0 = kt + (D < 128 ? ks : (x >> 1) * KT * 128 + ks + (((2 * c4 + (x & 1)) ^ g) << 4));
+                    const uint4 u0 = *reinterpret_cast<const uint4*>(a0), u1 = *reinterpret_cast<const uint4*>(a0 + 8 * M::ROW);
+                    const uint32_t w0_[4] = {u0.x, u0.y, u0.z, u0.w}, w1_[4] = {u1.x, u1.y, u1.z, u1.w};
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        uint32_t a[4];
+                        e4m3x4_to_f16(w0_[i], a[0], a[2]);
+                        e4m3x4_to_f16(w1_[i], a[1], a[3]);
+#pragma unroll
+                        for (int n = 0; n < NG; ++n) mma_f16_16816(s[n], a, q[n][x * 4 + i][0], q[n][x * 4 + i][1]);
+                    }
+                }
+                // exponents of keys g and g + 8 (a key that is not seen: any)
+                float kf[2], ev[2], back[2];
+#pragma unroll
+                for (int u = 0; u < 2; ++u) {
+                    const bool seen = g + u * 8 < nk;
+                    const int eb = seen ? exps[k0 + g + u * 8] : KV8_BIAS, vb = seen ? exps[KT + k0 + g + u * 8] : KV8_BIAS;
+                    kf[u] = __uint_as_float((uint32_t)eb << 23);
+                    ev[u] = (float)(vb - KV8_BIAS);
+                    back[u] = __uint_as_float((uint32_t)(2 * KV8_BIAS - vb) << 23);
+                }
+                uint32_t ph[NG][2], pl[NG][2];                       // weights times scales as two terms: head g, keys 2 c4 .. and 8 + 2 c4 ..
+#pragma unroll
+                for (int n = 0; n < NG; ++n) {
+                    float x[4], top[2];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) x[i] = g + (i >> 1) * 8 < nk ? fmaf(s[n][i] * kf[i >> 1], qf[n][i & 1], ev[i >> 1]) : -INFINITY;
+#pragma unroll
+                    for (int u = 0; u < 2; ++u) {
+                        top[u] = fmaxf(x[u], x[2 + u]);
+#pragma unroll
+                        for (int o = 4; o < 32; o <<= 1) top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], o));
+                    }
+                    if (__any_sync(0xffffffffu, top[0] > m[n][0] || top[1] > m[n][1])) {
+                        float f[2];
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            top[u] = fmaxf(top[u], m[n][u]);
+                            f[u] = m[n][u] == -INFINITY ? 0.f : exp2f(m[n][u] - top[u]);
+                            m[n][u] = top[u];
+                            l[n][u] *= f[u];
+                        }
+#pragma unroll
+                        for (int i = 0; i < MT; ++i) { acc[n][i][0] *= f[0]; acc[n][i][1] *= f[1]; acc[n][i][2] *= f[0]; acc[n][i][3] *= f[1]; }
+                    }
+#pragma unroll
+                    for (int r = 0; r < 2; ++r) {
+                        const float e0 = exp2f(x[r * 2] - m[n][0]), e1 = exp2f(x[r * 2 + 1] - m[n][1]);
+                        l[n][0] = fmaf(e0, back[r], l[n][0]);
+                        l[n][1] = fmaf(e1, back[r], l[n][1]);
+                        const __half2 hi = __floats2half2_rn(e0, e1);
+                        const float2 hf = __half22float2(hi);
+                        ph[n][r] = transposed8x8(*reinterpret_cast<const uint32_t*>(&hi));
+                        pl[n][r] = transposed8x8(f2_to_f16x2(e0 - hf.x, e1 - hf.y));
+                    }
+                }
+                // four keys of a lane's dims: 2 c4, 2 c4 + 1 and 8 on (values of keys that are not seen may be anything: they count as 0)
+                const bool whole = nk >= 16;
+#pragma unroll
+                for (int x = 0; x < M::HALVES; ++x) {
+                    uint32_t v[4][M::CHUNK / 4];
+#pragma unroll
+                    for (int u = 0; u < 4; ++u) {
+                        const int r = 2 * c4 + (u & 1) + (u >> 1) * 8;
+                        const bool seen = whole || r < nk;
+                        if (D < 128) {
+                            const uint2 y = *reinterpret_cast<const uint2*>(vt + (k0 + r) * 64 + (((g >> 1) ^ c4) << 4) + (g & 1) * 8);
+                            v[u][0] = seen ? y.x : 0u;
+                            v[u][1] = seen ? y.y : 0u;
+                        } else {
+                            const uint4 y = *reinterpret_cast<const uint4*>(vt + x * KT * 128 + (k0 + r) * 128 + ((g ^ (2 * c4 + (u & 1))) << 4));
+                            v[u][0] = seen ? y.x : 0u;
+                            v[u][1] = seen ? y.y : 0u;
+                            v[u][M::CHUNK / 4 - 2] = seen ? y.z : 0u;
+                            v[u][M::CHUNK / 4 - 1] = seen ? y.w : 0u;
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < M::CHUNK / 4; ++i)
+#pragma unroll
+                        for (int u = 0; u < 2; ++u) {
+                            uint32_t a[4];
+                            e4m3x4_to_f16(__byte_perm(v[0][i], v[1][i], u ? 0x7362 : 0x5140), a[0], a[1]);
+                            e4m3x4_to_f16(__byte_perm(v[2][i], v[3][i], u ? 0x7362 : 0x5140), a[2], a[3]);
+#pragma unroll
+                            for (int n = 0; n < NG; ++n) {
+                                mma_f16_16816(acc[n][x * 8 + i * 2 + u], a, ph[n][0], ph[n][1]);
+                                mma_f16_16816(acc[n][x * 8 + i * 2 + u], a, pl[n][0], pl[n][1]);
+                            }
+                        }
+                }
+            }
+            __syncwarp();
+            if (lane == 0) tc::mbar_arrive(free_ + st);
+            if (++st == M::STAGES) { st = 0; phase ^= 1u; }
+        }
+        // ---- join the warps ----
+#pragma unroll
+        for (int n = 0; n < NG; ++n)
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+#pragma unroll
+                for (int o = 4; o < 32; o <<= 1) l[n][u] += __shfl_xor_sync(0xffffffffu, l[n][u], o);
+                const int r = n * 8 + c4 * 2 + u;
+                if (g == 0) { sm[warp * M::HG + r] = m[n][u]; sm[(WARPS + warp) * M::HG + r] = l[n][u]; }
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {                       // a chunk's pairs are turned by its number, for the banks
+                    const int d = (i >> (M::CHUNK == 16 ? 3 : 2)) * 128 + g * M::CHUNK + ((i * 2 + g * 2) & (M::CHUNK - 1));
+                    *reinterpret_cast<float2*>(so + (warp * M::HG + r) * M::LO + d) = make_float2(acc[n][i][u], acc[n][i][2 + u]);
+                }
+            }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        const bool whole = count == at.n;
+        const size_t part = (size_t)blockIdx.x * 2 + (at.tile == 0 ? 1 : 0);
+        for (int i = tid; i < nr * (D / 2); i += WARPS * 32) {
+            const int r = i / (D / 2), d = i % (D / 2) * 2, ch = d / M::CHUNK, x = ch * M::CHUNK + ((d + (ch & 7) * 2) & (M::CHUNK - 1));
+            float top = sm[r], den = 0.f, a = 0.f, b = 0.f;
+#pragma unroll
+            for (int y = 1; y < WARPS; ++y) top = fmaxf(top, sm[y * M::HG + r]);
+#pragma unroll
+            for (int y = 0; y < WARPS; ++y) {
+                const float ref = sm[y * M::HG + r], f = ref == -INFINITY ? 0.f : exp2f(ref - top);
+                const float2 o = *reinterpret_cast<const float2*>(so + (y * M::HG + r) * M::LO + x);
+                den += f * sm[(WARPS + y) * M::HG + r];
+                a += f * o.x;
+                b += f * o.y;
+            }
+            a /= den;
+            b /= den;
+            if (whole) {
+                if (d < p.hd) *reinterpret_cast<uint32_t*>(p.out + ((size_t)t * p.n_heads + h0 + r) * p.hd + d) = f2_to_bf162(a, b);
+            } else {
+                *reinterpret_cast<float2*>(p.o_part + (part * M::HG + r) * D + d) = make_float2(a, b);
+                if (d == 0) p.lse_part[part * M::HG + r] = top + log2f(den);
+            }
+        }
+        asm volatile("bar.sync 1, 128;" ::: "memory");
+        w += count;
     }
+    if (!ok && lane == 0) atomicExch(p.err, 51);
+}
+
+// Joins the partial results of the histories that lie in several shares.  Block (b, row): the history that share b + 1 begins inside of, if no share
+// in front of it does; rows are its query heads.  A history's first part is its block's second partial result, the others are their blocks' first.
+// block 512: 4 neighbouring values a thread, D / 4 threads a part
+template <int D, int HG>
+__global__ void __launch_bounds__(512) kv8_merge_kernel(Kv8DecodeParams p, int blocks, int per_block) {
+    constexpr int LANES = D / 4, PARTS = 512 / LANES;
+    __shared__ int before[MAX_T + 1];
+    __shared__ float4 sums[512];
+    __shared__ float scratch[33];
+    pdl_grid_sync();
+    const int group = p.n_heads / p.n_kv, hg = (group + HG - 1) / HG, tid = threadIdx.x, b = blockIdx.x + 1, r = blockIdx.y;
+    const Tiles tiles = number_tiles(before, p.positions, p.T, p.n_kv * hg, blocks, per_block);
+    if (b >= tiles.blocks) return;
+    const long long w = tiles.begin(b);
+    const Tiles::Place at = tiles.at(w);
+    const long long first = w - at.tile, last = first + at.n - 1;
+    const int hkv = at.item / hg, r_lo = at.item % hg * HG;
+    if (at.tile == 0 || tiles.begin(b - 1) > first || r >= min(HG, group - r_lo)) return;
+    const int end = (int)(((last + 1) * tiles.blocks - 1) / tiles.total()), n = end - b + 2;       // parts
+    auto part = [&](int i) { return ((size_t)(b - 1 + i) * 2 + (i == 0 ? 1 : 0)) * HG + r; };
+    float top = -INFINITY;
+    for (int i = tid; i < n; i += 512) top = fmaxf(top, p.lse_part[part(i)]);
+    top = block_max(top == -INFINITY ? -FLT_MAX : top, scratch);
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    float den = 0.f;
+#pragma unroll 4
+    for (int i = tid / LANES; i < n; i += PARTS) {
+        const float f = exp2f(p.lse_part[part(i)] - top);
+        const float4 v = *reinterpret_cast<const float4*>(p.o_part + part(i) * D + tid % LANES * 4);
+        den += f;
+        o.x += f * v.x;
+        o.y += f * v.y;
+        o.z += f * v.z;
+        o.w += f * v.w;
+    }
+    __shared__ float dens[PARTS];
+    sums[tid] = o;
+    if (tid % LANES == 0) dens[tid / LANES] = den;
+    __syncthreads();
+    if (tid >= LANES || tid * 4 >= p.hd) return;
+    den = dens[0];
+#pragma unroll
+    for (int i = 1; i < PARTS; ++i) {
+        const float4 v = sums[i * LANES + tid];
+        o.x += v.x;
+        o.y += v.y;
+        o.z += v.z;
+        o.w += v.w;
+        den += dens[i];
+    }
+    *reinterpret_cast<uint2*>(p.out + ((size_t)at.t * p.n_heads + hkv * group + r_lo + r) * p.hd + tid * 4) =
+        make_uint2(f2_to_bf162(o.x / den, o.y / den), f2_to_bf162(o.z / den, o.w / den));
+}
+
+// Codes as [slots, heads, hd]; boxes of `rows` slots of one head, min(width, 128) bytes wide (what lies behind the head's last byte reads as zero).
+int map_codes(CUtensorMap* map, const void* codes, const Kv8DecodeParams* p, int width, int rows) {
+    PFN_encodeTiled enc = get_encode_tiled();
+    if (enc == nullptr) return -100;
+    cuuint64_t dims[3] = {(cuuint64_t)p->hd, (cuuint64_t)p->n_kv, (cuuint64_t)p->pages.num_slots}, strides[2] = {(cuuint64_t)p->hd, (cuuint64_t)p->n_kv * p->hd};
+    cuuint32_t box[3] = {(cuuint32_t)(width < 128 ? width : 128), 1, (cuuint32_t)rows}, steps[3] = {1, 1, 1};
+    return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(codes), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
+               width < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -102;
+}
+
+// width of the heads in the kernels, tiles of 8 query heads
+struct Shape { int width, tiles; };
+Shape shape_of(int n_heads, int n_kv, int hd) { return {hd <= 64 ? 64 : hd <= 128 ? 128 : 256, hd <= 128 && n_heads / n_kv > 8 ? 2 : 1}; }
+
+template <int D, int NG>
+int launch(const Kv8DecodeParams* all, int T, int blocks, cudaStream_t s) {
+    using M = Cfg<D, NG>;
+    constexpr int smem = M::TOTAL + 1024;
+    static_assert(M::PER_SM * (smem + 1024) <= 228 * 1024, "blocks per SM");
+    static SmemOptIn opt_in;
+    const int box = all->pages.page_size % 64 == 0 ? 64 : all->pages.page_size % 32 == 0 ? 32 : 16, per_block = 1;
+    CUtensorMap mk, mv;
+    int rc = map_codes(&mk, all->k_codes, all, D, box);
+    if (rc == 0) rc = map_codes(&mv, all->v_codes, all, D, box);
+    if (rc == 0) rc = opt_in((const void*)kv8_decode_kernel<D, NG>, smem);
+    if (rc != 0) return rc;
+    for (int t = 0; t < T; t += MAX_T) {
+        Kv8DecodeParams p = *all;
+        const size_t row = (size_t)p.n_heads * p.hd;
+        p.T = T - t < MAX_T ? T - t : MAX_T;
+        p.q += t * row;
+        p.out += t * row;
+        p.positions += t;
+        p.batch_idx += t;
+        sl_launch(kv8_decode_kernel<D, NG>, blocks, THREADS, smem, s, mk, mv, p, box, per_block);
+        if (blocks > 1) sl_launch(kv8_merge_kernel<D, 8 * NG>, dim3(blocks - 1, 8 * NG < p.n_heads / p.n_kv ? 8 * NG : p.n_heads / p.n_kv), 512, 0, s, p, blocks, per_block);
+        rc = SL_LAUNCH_CHECK();
+        if (rc != 0) return rc;
+    }
+    return 0;
 }
 
 }  // namespace
 
-SL_API int sl_kv8_decode(const Kv8DecodeParams* p, int T, cudaStream_t s) {
+// Blocks that attention of these sizes is dealt out to, and what a partial result takes: 2 `rows` x `width` sums (and as many / `width` references) a block.
+SL_API int sl_kv8_decode_plan(int n_heads, int n_kv, int hd, int* blocks, int* rows, int* width) {
+    if (hd < 16 || hd > 256 || hd % 16 != 0 || n_kv < 1 || n_heads < n_kv || n_heads % n_kv != 0) return -1;
+    int device = 0, sms = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
+    if (e != cudaSuccess) return (int)e;
+    const Shape sh = shape_of(n_heads, n_kv, hd);
+    *blocks = sms * (sh.width <= 128 && sh.tiles == 1 ? 3 : 2);
+    *rows = 8 * sh.tiles;
+    *width = sh.width;
+    return 0;
+}
+
+// out = attention of T tokens; `blocks`: of sl_kv8_decode_plan.
+SL_API int sl_kv8_decode(const Kv8DecodeParams* p, int T, int blocks, cudaStream_t s) {
     if (T == 0) return 0;
-    if (p->hd < 16 || p->hd > 256 || p->hd % 16 != 0 || p->n_kv < 1 || p->n_heads % p->n_kv != 0 || T > 65535 || p->pages.page_size < 1) return -1;
-    sl_launch(kv8_rows_kernel, dim3(p->n_heads, T), 128, 0, s, *p);
-    return SL_LAUNCH_CHECK();
+    if (p->hd < 16 || p->hd > 256 || p->hd % 16 != 0 || p->n_kv < 1 || p->n_heads % p->n_kv != 0 || blocks < 1) return -1;
+    if (p->pages.page_size < 16 || p->pages.page_size % 16 != 0 || p->o_part == nullptr || p->lse_part == nullptr) return -1;
+    if ((((uintptr_t)p->q | (uintptr_t)p->k_codes | (uintptr_t)p->v_codes | (uintptr_t)p->exps | (uintptr_t)p->out | (uintptr_t)p->o_part) & 15) != 0) return -1;
+    const Shape sh = shape_of(p->n_heads, p->n_kv, p->hd);
+    if (sh.width == 64) return sh.tiles == 2 ? launch<64, 2>(p, T, blocks, s) : launch<64, 1>(p, T, blocks, s);
+    if (sh.width == 128) return sh.tiles == 2 ? launch<128, 2>(p, T, blocks, s) : launch<128, 1>(p, T, blocks, s);
+    return launch<256, 1>(p, T, blocks, s);
 }

@@ -13,6 +13,7 @@ from __future__ import annotations
 
 import ctypes as C
 from dataclasses import dataclass
+from functools import lru_cache
 from typing import Optional, Tuple
 
 import torch
@@ -59,7 +60,7 @@ class Kv8UnpackParams(C.Structure):
 class Kv8DecodeParams(C.Structure):
     _fields_ = [("q", C.c_void_p), ("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("exps", C.c_void_p), ("positions", C.c_void_p),
                 ("batch_idx", C.c_void_p), ("pages", _Pages), ("n_heads", C.c_int), ("n_kv", C.c_int), ("hd", C.c_int), ("scale", C.c_float),
-                ("out", C.c_void_p)]
+                ("out", C.c_void_p), ("o_part", C.c_void_p), ("lse_part", C.c_void_p), ("T", C.c_int), ("err", C.c_void_p)]
 
 
 @dataclass
@@ -244,14 +245,29 @@ def kv8_attention(q, cache: Kv8Cache, positions, batch_idx, page_table, sm_scale
     if T == 0:
         return out
     if qo_indptr is None:
+        from . import tcgen05
+        blocks, rows, wide = _decode_plan(q.get_device(), n_heads, n_kv, hd)
+        part = torch.empty(blocks * 2 * rows * (wide + 1), dtype=torch.float32, device=q.device)
         p = Kv8DecodeParams(q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.exps.data_ptr(), positions.data_ptr(), batch_idx.data_ptr(),
-                            _pages(cache, page_table), n_heads, n_kv, hd, sm_scale, out.data_ptr())
-        _call(q, "sl_kv8_decode", C.byref(p), T)
+                            _pages(cache, page_table), n_heads, n_kv, hd, sm_scale, out.data_ptr(), part.data_ptr(),
+                            part.data_ptr() + blocks * 2 * rows * wide * 4, 0, tcgen05.error_flag(q.device).data_ptr())
+        _call(q, "sl_kv8_decode", C.byref(p), T, blocks)
         return out
     if hd not in (64, 128):
         raise ValueError(f"heads of {hd} values: attention of prompts takes 64 or 128")
     _prompts(q, cache, positions, batch_idx, page_table, sm_scale, qo_indptr, max_q or T, max_kv_len, out)
     return out
+
+
+@lru_cache(maxsize=None)
+def _decode_plan(device: int, n_heads: int, n_kv: int, hd: int) -> Tuple[int, int, int]:
+    """(blocks, rows and width of a partial result) of the decode kernel on a device."""
+    N = _native()
+    out = (C.c_int * 3)()
+    at = C.addressof(out)
+    with torch.cuda.device(device):
+        N.check(N.fn("sl_kv8_decode_plan")(n_heads, n_kv, hd, at, at + 4, at + 8), "sl_kv8_decode_plan")
+    return tuple(out)
 
 
 def _prompts(q, cache, positions, batch_idx, page_table, sm_scale, qo_indptr, max_q, max_kv_len, out) -> None:
