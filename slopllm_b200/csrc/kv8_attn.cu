@@ -6,7 +6,8 @@
 // fill the device alike.  A history that lies in several shares leaves a partial result in each, which kv8_merge_kernel joins.
 //
 // kv8_decode_kernel: a fetching warp brings tiles (TMA, swizzled) and their exponent bytes through a ring of stages, also across the ends of
-// histories; four warps take 16 keys of a tile each, with softmax states of their own and no barrier before a history's end.
+// histories; two pairs of warps take tiles in turn, a warp 32 keys of one, with softmax states of their own and no barrier before a history's
+// end.
 //
 //   S^T = K Q^T      keys are the 16-row operand: a lane's 16 bytes of two keys are four steps of the product as they lie, since any order
 //                    of the summed dims will do that the queries follow
@@ -14,7 +15,7 @@
 //
 // e4m3 codes become fp16 exactly (mma.sync f16, fp32 sums); the queries are fp16 times a power of two per head, which loses less than 2^-24 of
 // the largest value.  The keys' scales go onto the scores.  The values' scales go into the weights: the reference of a row is the maximum of
-// score + exponent (in powers of two), so weights times scales are at most 1, and the denominator takes the scale out again.  Weights are two fp16
+// score + exponent (in powers of two), so weights times scales stay within fp16, and the denominator takes the scale out again.  Weights are two fp16
 // terms (21 bits).
 #include "kv8.cuh"
 #include "tcgen05.cuh"
@@ -35,6 +36,15 @@ struct Kv8DecodeParams {
 };
 
 constexpr int KT = 64, WARPS = 4, THREADS = WARPS * 32 + 32, MAX_T = 1024;
+// A row's reference is raised when a weight would be above 2^(TOP + RAISE); weights reach down to 2^-126 beside 2^TOP, so that two rows whose
+// scales are the format's limits apart (2^120) are told apart by weights down to 2^-14 of the largest.
+constexpr float TOP = 8.f, RAISE = 7.f;
+
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 __device__ __forceinline__ uint32_t transposed8x8(uint32_t x) {
     uint32_t y;
@@ -105,14 +115,15 @@ __device__ __forceinline__ Tiles number_tiles(int* before, const int* positions,
 template <int D, int NG>
 struct Cfg {
     static constexpr int ROW = D < 128 ? D : 128, HALVES = D / ROW;      // bytes of a row in one box, boxes
-    static constexpr int STAGES = D == 64 ? 6 : D == 128 ? 3 : 2, HG = 8 * NG, LO = D + 4;
+    static constexpr int STAGES = D == 64 ? 6 : D == 128 ? 4 : 2, HG = 8 * NG, LO = D + 4;
     static constexpr int CODES = KT * D, STAGE = 2 * CODES;              // keys, values
     static constexpr int EXPS = STAGES * STAGE;                          // 64 bytes of the keys, 64 of the values
     static constexpr int JOIN = EXPS + STAGES * 2 * KT;                  // fp32 [WARPS][HG][LO], then [2][WARPS][HG]
     static constexpr int BEFORE = JOIN + (WARPS * HG * LO + 2 * WARPS * HG) * 4;
     static constexpr int BARS = (BEFORE + (MAX_T + 1) * 4 + 7) / 8 * 8;
     static constexpr int TOTAL = BARS + 2 * STAGES * 8;
-    static constexpr int PER_SM = D == 128 && NG == 1 ? 3 : D == 64 && NG == 1 ? 3 : 2;
+    static constexpr int PER_SM = D == 64 && NG == 1 ? 3 : 2;
+    static_assert(STAGES % 2 == 0, "a stage belongs to one pair of warps: a barrier is never two phases ahead of who waits for it");
     static constexpr int CHUNK = D < 128 ? 8 : 16;                       // neighbouring dims of a lane
 };
 
@@ -128,7 +139,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
     if (tid == 0) {
         for (int i = 0; i < M::STAGES; ++i) {
             tc::mbar_init(full + i, 1);
-            tc::mbar_init(free_ + i, WARPS);
+            tc::mbar_init(free_ + i, 2);
         }
         tc::mbar_fence_init();
     }
@@ -196,14 +207,14 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
         return;
     }
 
-    // ---- products: 16 keys of every tile ----
-    const int g = lane >> 2, c4 = lane & 3, k0 = warp * 16;
+    // ---- products: a pair of warps takes every other tile, a warp 32 of its keys ----
+    const int g = lane >> 2, c4 = lane & 3, k0 = (warp & 1) * 32;
     float* const so = reinterpret_cast<float*>(smem + M::JOIN);
     float* const sm = so + WARPS * M::HG * M::LO;                    // references, then sums
     constexpr int MT = D / 16, CH = D < 128 ? 1 : D / 64;            // 16-dim rows of products, 16-byte pieces of a key row a lane reads
     // places of a lane's pieces in a tile
     const int ks = D < 128 ? (k0 + g) * 64 + ((c4 ^ (g >> 1 & 3)) << 4) : (k0 + g) * 128;
-    int st = 0;
+    int st = 0, turn = warp >> 1;                                    // 0: this pair's tile
     uint32_t phase = 0;
     bool ok = true;
     for (long long w = w0; w < w1;) {
@@ -259,111 +270,127 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
             for (int i = 0; i < MT; ++i) acc[n][i][0] = acc[n][i][1] = acc[n][i][2] = acc[n][i][3] = 0.f;
         }
         for (int j = at.tile; j < at.tile + count; ++j) {
-            if (ok) ok = tc::mbar_wait_warp(full + st, phase);
-            const uint8_t *kt = smem + st * M::STAGE, *vt = kt + M::CODES, *exps = smem + M::EXPS + st * 2 * KT;
-            const int nk = keys - j * KT - k0;                       // of this warp's 16
+            const int stage = st;
+            const uint32_t par = phase;
+            if (++st == M::STAGES) { st = 0; phase ^= 1u; }
+            turn ^= 1;
+            if (turn == 0) continue;
+            if (ok) ok = tc::mbar_wait_warp(full + stage, par);
+            const uint8_t *kt = smem + stage * M::STAGE, *vt = kt + M::CODES, *exps = smem + M::EXPS + stage * 2 * KT + k0;
+            const int nk = keys - j * KT - k0;                       // of this warp's 32
             if (nk > 0) {
-                float s[NG][4];
+                const bool whole = nk >= 32;
+                float s[NG][2][4];                                   // keys g and g + 8 of 16, heads 2 c4 and 2 c4 + 1
 #pragma unroll
-                for (int n = 0; n < NG; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+                for (int n = 0; n < NG; ++n)
 #pragma unroll
-                for (int x = 0; x < CH; ++x) {
-                    const uint8_t* a0 = kt + (D < 128 ? ks : (x >> 1) * KT * 128 + ks + (((2 * c4 + (x & 1)) ^ g) << 4));
-                    const uint4 u0 = *reinterpret_cast<const uint4*>(a0), u1 = *reinterpret_cast<const uint4*>(a0 + 8 * M::ROW);
-                    const uint32_t w0_[4] = {u0.x, u0.y, u0.z, u0.w}, w1_[4] = {u1.x, u1.y, u1.z, u1.w};
+                    for (int y = 0; y < 2; ++y) s[n][y][0] = s[n][y][1] = s[n][y][2] = s[n][y][3] = 0.f;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        uint32_t a[4];
-                        e4m3x4_to_f16(w0_[i], a[0], a[2]);
-                        e4m3x4_to_f16(w1_[i], a[1], a[3]);
+                for (int x = 0; x < CH; ++x)
 #pragma unroll
-                        for (int n = 0; n < NG; ++n) mma_f16_16816(s[n], a, q[n][x * 4 + i][0], q[n][x * 4 + i][1]);
+                    for (int y = 0; y < 2; ++y) {
+                        const uint8_t* a0 = kt + (D < 128 ? ks : (x >> 1) * KT * 128 + ks + (((2 * c4 + (x & 1)) ^ g) << 4)) + y * 16 * M::ROW;
+                        const uint4 u0 = *reinterpret_cast<const uint4*>(a0), u1 = *reinterpret_cast<const uint4*>(a0 + 8 * M::ROW);
+                        const uint32_t r0[4] = {u0.x, u0.y, u0.z, u0.w}, r1[4] = {u1.x, u1.y, u1.z, u1.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            uint32_t a[4];
+                            e4m3x4_to_f16(r0[i], a[0], a[2]);
+                            e4m3x4_to_f16(r1[i], a[1], a[3]);
+#pragma unroll
+                            for (int n = 0; n < NG; ++n) mma_f16_16816(s[n][y], a, q[n][x * 4 + i][0], q[n][x * 4 + i][1]);
+                        }
                     }
-                }
-                // exponents of keys g and g + 8 (a key that is not seen: any)
-                float kf[2], ev[2], back[2];
+                // exponents of keys g, g + 8, g + 16, g + 24 (of a key that is not seen: any)
+                float kf[4], ev[4], back[4];
 #pragma unroll
-                for (int u = 0; u < 2; ++u) {
-                    const bool seen = g + u * 8 < nk;
-                    const int eb = seen ? exps[k0 + g + u * 8] : KV8_BIAS, vb = seen ? exps[KT + k0 + g + u * 8] : KV8_BIAS;
+                for (int u = 0; u < 4; ++u) {
+                    int eb = exps[g + u * 8], vb = exps[KT + g + u * 8];
+                    if (!whole && g + u * 8 >= nk) eb = vb = KV8_BIAS;
                     kf[u] = __uint_as_float((uint32_t)eb << 23);
                     ev[u] = (float)(vb - KV8_BIAS);
                     back[u] = __uint_as_float((uint32_t)(2 * KV8_BIAS - vb) << 23);
                 }
-                uint32_t ph[NG][2], pl[NG][2];                       // weights times scales as two terms: head g, keys 2 c4 .. and 8 + 2 c4 ..
+                uint32_t ph[NG][4], pl[NG][4];                       // weights times scales as two terms: head g, keys 2 c4 .. of every 8
 #pragma unroll
                 for (int n = 0; n < NG; ++n) {
-                    float x[4], top[2];
+                    float x[4][2], top[2];
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) x[i] = g + (i >> 1) * 8 < nk ? fmaf(s[n][i] * kf[i >> 1], qf[n][i & 1], ev[i >> 1]) : -INFINITY;
+                    for (int u = 0; u < 4; ++u)
 #pragma unroll
-                    for (int u = 0; u < 2; ++u) {
-                        top[u] = fmaxf(x[u], x[2 + u]);
+                        for (int h = 0; h < 2; ++h) {
+                            x[u][h] = fmaf(s[n][u >> 1][(u & 1) * 2 + h] * kf[u], qf[n][h], ev[u]);
+                            if (!whole && g + u * 8 >= nk) x[u][h] = -INFINITY;
+                        }
 #pragma unroll
-                        for (int o = 4; o < 32; o <<= 1) top[u] = fmaxf(top[u], __shfl_xor_sync(0xffffffffu, top[u], o));
+                    for (int h = 0; h < 2; ++h) {
+                        top[h] = fmaxf(fmaxf(x[0][h], x[1][h]), fmaxf(x[2][h], x[3][h]));
+#pragma unroll
+                        for (int o = 4; o < 32; o <<= 1) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], o));
                     }
-                    if (__any_sync(0xffffffffu, top[0] > m[n][0] || top[1] > m[n][1])) {
+                    if (__any_sync(0xffffffffu, top[0] > m[n][0] + RAISE || top[1] > m[n][1] + RAISE)) {
                         float f[2];
 #pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            top[u] = fmaxf(top[u], m[n][u]);
-                            f[u] = m[n][u] == -INFINITY ? 0.f : exp2f(m[n][u] - top[u]);
-                            m[n][u] = top[u];
-                            l[n][u] *= f[u];
+                        for (int h = 0; h < 2; ++h) {
+                            top[h] = fmaxf(top[h], m[n][h]);
+                            f[h] = m[n][h] == -INFINITY ? 0.f : ex2(m[n][h] - top[h]);
+                            m[n][h] = top[h];
+                            l[n][h] *= f[h];
                         }
 #pragma unroll
                         for (int i = 0; i < MT; ++i) { acc[n][i][0] *= f[0]; acc[n][i][1] *= f[1]; acc[n][i][2] *= f[0]; acc[n][i][3] *= f[1]; }
                     }
 #pragma unroll
-                    for (int r = 0; r < 2; ++r) {
-                        const float e0 = exp2f(x[r * 2] - m[n][0]), e1 = exp2f(x[r * 2 + 1] - m[n][1]);
-                        l[n][0] = fmaf(e0, back[r], l[n][0]);
-                        l[n][1] = fmaf(e1, back[r], l[n][1]);
+                    for (int u = 0; u < 4; ++u) {
+                        const float e0 = ex2(x[u][0] - (m[n][0] - TOP)), e1 = ex2(x[u][1] - (m[n][1] - TOP));
+                        l[n][0] = fmaf(e0, back[u], l[n][0]);
+                        l[n][1] = fmaf(e1, back[u], l[n][1]);
                         const __half2 hi = __floats2half2_rn(e0, e1);
                         const float2 hf = __half22float2(hi);
-                        ph[n][r] = transposed8x8(*reinterpret_cast<const uint32_t*>(&hi));
-                        pl[n][r] = transposed8x8(f2_to_f16x2(e0 - hf.x, e1 - hf.y));
+                        ph[n][u] = transposed8x8(*reinterpret_cast<const uint32_t*>(&hi));
+                        pl[n][u] = transposed8x8(f2_to_f16x2(e0 - hf.x, e1 - hf.y));
                     }
                 }
-                // four keys of a lane's dims: 2 c4, 2 c4 + 1 and 8 on (values of keys that are not seen may be anything: they count as 0)
-                const bool whole = nk >= 16;
+                // a lane's dims of keys 2 c4, 2 c4 + 1 and 8 on, of each 16 (values of keys that are not seen may be anything: they count as 0)
 #pragma unroll
-                for (int x = 0; x < M::HALVES; ++x) {
-                    uint32_t v[4][M::CHUNK / 4];
+                for (int x = 0; x < M::HALVES; ++x)
 #pragma unroll
-                    for (int u = 0; u < 4; ++u) {
-                        const int r = 2 * c4 + (u & 1) + (u >> 1) * 8;
-                        const bool seen = whole || r < nk;
-                        if (D < 128) {
-                            const uint2 y = *reinterpret_cast<const uint2*>(vt + (k0 + r) * 64 + (((g >> 1) ^ c4) << 4) + (g & 1) * 8);
-                            v[u][0] = seen ? y.x : 0u;
-                            v[u][1] = seen ? y.y : 0u;
-                        } else {
-                            const uint4 y = *reinterpret_cast<const uint4*>(vt + x * KT * 128 + (k0 + r) * 128 + ((g ^ (2 * c4 + (u & 1))) << 4));
-                            v[u][0] = seen ? y.x : 0u;
-                            v[u][1] = seen ? y.y : 0u;
-                            v[u][M::CHUNK / 4 - 2] = seen ? y.z : 0u;
-                            v[u][M::CHUNK / 4 - 1] = seen ? y.w : 0u;
-                        }
-                    }
+                    for (int y = 0; y < 2; ++y) {
+                        uint32_t v[4][M::CHUNK / 4];
 #pragma unroll
-                    for (int i = 0; i < M::CHUNK / 4; ++i)
-#pragma unroll
-                        for (int u = 0; u < 2; ++u) {
-                            uint32_t a[4];
-                            e4m3x4_to_f16(__byte_perm(v[0][i], v[1][i], u ? 0x7362 : 0x5140), a[0], a[1]);
-                            e4m3x4_to_f16(__byte_perm(v[2][i], v[3][i], u ? 0x7362 : 0x5140), a[2], a[3]);
-#pragma unroll
-                            for (int n = 0; n < NG; ++n) {
-                                mma_f16_16816(acc[n][x * 8 + i * 2 + u], a, ph[n][0], ph[n][1]);
-                                mma_f16_16816(acc[n][x * 8 + i * 2 + u], a, pl[n][0], pl[n][1]);
+                        for (int u = 0; u < 4; ++u) {
+                            const int r = y * 16 + 2 * c4 + (u & 1) + (u >> 1) * 8;
+                            if (D < 128) {
+                                *reinterpret_cast<uint2*>(v[u]) = *reinterpret_cast<const uint2*>(vt + (k0 + r) * 64 + (((g >> 1) ^ c4) << 4) + (g & 1) * 8);
+                            } else {
+                                *reinterpret_cast<uint4*>(v[u]) =
+                                    *reinterpret_cast<const uint4*>(vt + x * KT * 128 + (k0 + r) * 128 + ((g ^ (2 * c4 + (u & 1))) << 4));
                             }
                         }
-                }
+                        if (!whole) {
+#pragma unroll
+                            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                                for (int i = 0; i < M::CHUNK / 4; ++i)
+                                    if (y * 16 + 2 * c4 + (u & 1) + (u >> 1) * 8 >= nk) v[u][i] = 0u;
+                        }
+#pragma unroll
+                        for (int i = 0; i < M::CHUNK / 4; ++i)
+#pragma unroll
+                            for (int u = 0; u < 2; ++u) {
+                                uint32_t a[4];
+                                e4m3x4_to_f16(__byte_perm(v[0][i], v[1][i], u ? 0x7362 : 0x5140), a[0], a[1]);
+                                e4m3x4_to_f16(__byte_perm(v[2][i], v[3][i], u ? 0x7362 : 0x5140), a[2], a[3]);
+#pragma unroll
+                                for (int n = 0; n < NG; ++n) {
+                                    mma_f16_16816(acc[n][x * 8 + i * 2 + u], a, ph[n][y * 2], ph[n][y * 2 + 1]);
+                                    mma_f16_16816(acc[n][x * 8 + i * 2 + u], a, pl[n][y * 2], pl[n][y * 2 + 1]);
+                                }
+                            }
+                    }
             }
             __syncwarp();
-            if (lane == 0) tc::mbar_arrive(free_ + st);
-            if (++st == M::STAGES) { st = 0; phase ^= 1u; }
+            if (lane == 0) tc::mbar_arrive(free_ + stage);
         }
         // ---- join the warps ----
 #pragma unroll
@@ -390,7 +417,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
             for (int y = 1; y < WARPS; ++y) top = fmaxf(top, sm[y * M::HG + r]);
 #pragma unroll
             for (int y = 0; y < WARPS; ++y) {
-                const float ref = sm[y * M::HG + r], f = ref == -INFINITY ? 0.f : exp2f(ref - top);
+                const float ref = sm[y * M::HG + r], f = ref == -INFINITY ? 0.f : ex2(ref - top);
                 const float2 o = *reinterpret_cast<const float2*>(so + (y * M::HG + r) * M::LO + x);
                 den += f * sm[(WARPS + y) * M::HG + r];
                 a += f * o.x;
@@ -411,58 +438,82 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
     if (!ok && lane == 0) atomicExch(p.err, 51);
 }
 
-// Joins the partial results of the histories that lie in several shares.  Block (b, row): the history that share b + 1 begins inside of, if no share
-// in front of it does; rows are its query heads.  A history's first part is its block's second partial result, the others are their blocks' first.
-// block 512: 4 neighbouring values a thread, D / 4 threads a part
-template <int D, int HG>
+// Joins the partial results of histories that lie in several shares: the first part is its block's second partial result, the others are their
+// blocks' first.  Block (i, y): the i-th history (ALL), or the one that share i + 1 begins inside of, if no share in front of it does; rows y * R ..
+// of its query heads.  A thread has 4 neighbouring values, D / 4 threads a row and 512 / (D / 4) / R of the parts in turn.
+template <int D, int HG, int R, bool ALL>
 __global__ void __launch_bounds__(512) kv8_merge_kernel(Kv8DecodeParams p, int blocks, int per_block) {
-    constexpr int LANES = D / 4, PARTS = 512 / LANES;
+    constexpr int LANES = D / 4, TURNS = 512 / LANES / R, AHEAD = 4;
     __shared__ int before[MAX_T + 1];
     __shared__ float4 sums[512];
-    __shared__ float scratch[33];
+    __shared__ float2 state[512 / LANES];            // reference and denominator
     pdl_grid_sync();
-    const int group = p.n_heads / p.n_kv, hg = (group + HG - 1) / HG, tid = threadIdx.x, b = blockIdx.x + 1, r = blockIdx.y;
+    const int group = p.n_heads / p.n_kv, hg = (group + HG - 1) / HG, tid = threadIdx.x;
     const Tiles tiles = number_tiles(before, p.positions, p.T, p.n_kv * hg, blocks, per_block);
-    if (b >= tiles.blocks) return;
-    const long long w = tiles.begin(b);
+    long long w;
+    if (ALL) {
+        const int t = blockIdx.x / tiles.items;
+        w = (long long)before[t] * tiles.items + (long long)(blockIdx.x % tiles.items) * (before[t + 1] - before[t]);
+        if (before[t + 1] == before[t]) return;
+    } else {
+        if ((int)blockIdx.x + 1 >= tiles.blocks) return;
+        w = tiles.begin(blockIdx.x + 1);
+    }
     const Tiles::Place at = tiles.at(w);
-    const long long first = w - at.tile, last = first + at.n - 1;
-    const int hkv = at.item / hg, r_lo = at.item % hg * HG;
-    if (at.tile == 0 || tiles.begin(b - 1) > first || r >= min(HG, group - r_lo)) return;
-    const int end = (int)(((last + 1) * tiles.blocks - 1) / tiles.total()), n = end - b + 2;       // parts
-    auto part = [&](int i) { return ((size_t)(b - 1 + i) * 2 + (i == 0 ? 1 : 0)) * HG + r; };
-    float top = -INFINITY;
-    for (int i = tid; i < n; i += 512) top = fmaxf(top, p.lse_part[part(i)]);
-    top = block_max(top == -INFINITY ? -FLT_MAX : top, scratch);
+    const long long first = w - at.tile, total = tiles.total();
+    const int b0 = (int)(((first + 1) * tiles.blocks - 1) / total), b1 = (int)(((first + at.n) * tiles.blocks - 1) / total), n = b1 - b0 + 1;
+    if (n == 1 || (!ALL && (at.tile == 0 || b0 != (int)blockIdx.x))) return;
+    const int hkv = at.item / hg, r_lo = at.item % hg * HG, part_row = tid / LANES, r = blockIdx.y * R + part_row % R, d = tid % LANES * 4;
+    const bool on = r < min(HG, group - r_lo);
+    float top = -INFINITY, den = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    float den = 0.f;
-#pragma unroll 4
-    for (int i = tid / LANES; i < n; i += PARTS) {
-        const float f = exp2f(p.lse_part[part(i)] - top);
-        const float4 v = *reinterpret_cast<const float4*>(p.o_part + part(i) * D + tid % LANES * 4);
-        den += f;
-        o.x += f * v.x;
-        o.y += f * v.y;
-        o.z += f * v.z;
-        o.w += f * v.w;
-    }
-    __shared__ float dens[PARTS];
-    sums[tid] = o;
-    if (tid % LANES == 0) dens[tid / LANES] = den;
-    __syncthreads();
-    if (tid >= LANES || tid * 4 >= p.hd) return;
-    den = dens[0];
+    for (int i0 = part_row / R; i0 < n; i0 += TURNS * AHEAD) {
+        float lse[AHEAD];
+        float4 v[AHEAD];
 #pragma unroll
-    for (int i = 1; i < PARTS; ++i) {
-        const float4 v = sums[i * LANES + tid];
-        o.x += v.x;
-        o.y += v.y;
-        o.z += v.z;
-        o.w += v.w;
-        den += dens[i];
+        for (int u = 0; u < AHEAD; ++u) {
+            const int i = i0 + u * TURNS;
+            const bool there = on && i < n;
+            const size_t part = ((size_t)(b0 + i) * 2 + (i == 0 ? 1 : 0)) * HG + r;
+            lse[u] = there ? p.lse_part[part] : -INFINITY;
+            v[u] = there ? *reinterpret_cast<const float4*>(p.o_part + part * D + d) : make_float4(0.f, 0.f, 0.f, 0.f);
+        }
+        float up = top;
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) up = fmaxf(up, lse[u]);
+        const float f = top == -INFINITY ? 0.f : exp2f(top - up);
+        den *= f;
+        o.x *= f; o.y *= f; o.z *= f; o.w *= f;
+        top = up;
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const float e = lse[u] == -INFINITY ? 0.f : exp2f(lse[u] - top);
+            den += e;
+            o.x += e * v[u].x; o.y += e * v[u].y; o.z += e * v[u].z; o.w += e * v[u].w;
+        }
     }
-    *reinterpret_cast<uint2*>(p.out + ((size_t)at.t * p.n_heads + hkv * group + r_lo + r) * p.hd + tid * 4) =
-        make_uint2(f2_to_bf162(o.x / den, o.y / den), f2_to_bf162(o.z / den, o.w / den));
+    if (TURNS > 1) {
+        sums[tid] = o;
+        if (tid % LANES == 0) state[part_row] = make_float2(top, den);
+        __syncthreads();
+        if (part_row >= R) return;
+        float up = top;
+#pragma unroll
+        for (int i = 1; i < TURNS; ++i) up = fmaxf(up, state[part_row + i * R].x);
+        den = 0.f;
+        o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int i = 0; i < TURNS; ++i) {
+            const float2 s = state[part_row + i * R];
+            const float4 v = sums[tid + i * R * LANES];
+            const float e = s.x == -INFINITY ? 0.f : exp2f(s.x - up);
+            den += e * s.y;
+            o.x += e * v.x; o.y += e * v.y; o.z += e * v.z; o.w += e * v.w;
+        }
+    }
+    if (on && d < p.hd)
+        *reinterpret_cast<uint2*>(p.out + ((size_t)at.t * p.n_heads + hkv * group + r_lo + r) * p.hd + d) =
+            make_uint2(f2_to_bf162(o.x / den, o.y / den), f2_to_bf162(o.z / den, o.w / den));
 }
 
 // Codes as [slots, heads, hd]; boxes of `rows` slots of one head, min(width, 128) bytes wide (what lies behind the head's last byte reads as zero).
@@ -472,7 +523,7 @@ int map_codes(CUtensorMap* map, const void* codes, const Kv8DecodeParams* p, int
     cuuint64_t dims[3] = {(cuuint64_t)p->hd, (cuuint64_t)p->n_kv, (cuuint64_t)p->pages.num_slots}, strides[2] = {(cuuint64_t)p->hd, (cuuint64_t)p->n_kv * p->hd};
     cuuint32_t box[3] = {(cuuint32_t)(width < 128 ? width : 128), 1, (cuuint32_t)rows}, steps[3] = {1, 1, 1};
     return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(codes), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               width < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+               width < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, width < 128 ? CU_TENSOR_MAP_L2_PROMOTION_L2_64B : CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -102;
 }
 
@@ -501,7 +552,10 @@ int launch(const Kv8DecodeParams* all, int T, int blocks, cudaStream_t s) {
         p.positions += t;
         p.batch_idx += t;
         sl_launch(kv8_decode_kernel<D, NG>, blocks, THREADS, smem, s, mk, mv, p, box, per_block);
-        if (blocks > 1) sl_launch(kv8_merge_kernel<D, 8 * NG>, dim3(blocks - 1, 8 * NG < p.n_heads / p.n_kv ? 8 * NG : p.n_heads / p.n_kv), 512, 0, s, p, blocks, per_block);
+        // few histories have many parts each: a block a query head; many have few: a block for all of a share's border
+        const int group = p.n_heads / p.n_kv, items = p.T * p.n_kv * ((group + M::HG - 1) / M::HG);
+        if (blocks > 1 && items < blocks) sl_launch(kv8_merge_kernel<D, M::HG, 1, true>, dim3(items, M::HG < group ? M::HG : group), 512, 0, s, p, blocks, per_block);
+        else if (blocks > 1) sl_launch(kv8_merge_kernel<D, M::HG, M::HG, false>, blocks - 1, 512, 0, s, p, blocks, per_block);
         rc = SL_LAUNCH_CHECK();
         if (rc != 0) return rc;
     }
@@ -518,7 +572,7 @@ SL_API int sl_kv8_decode_plan(int n_heads, int n_kv, int hd, int* blocks, int* r
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
     if (e != cudaSuccess) return (int)e;
     const Shape sh = shape_of(n_heads, n_kv, hd);
-    *blocks = sms * (sh.width <= 128 && sh.tiles == 1 ? 3 : 2);
+    *blocks = sms * (sh.width == 64 && sh.tiles == 1 ? 3 : 2);
     *rows = 8 * sh.tiles;
     *width = sh.width;
     return 0;
