@@ -15,8 +15,10 @@
 //
 // e4m3 codes become fp16 exactly (mma.sync f16, fp32 sums); the queries are fp16 times a power of two per head, which loses less than 2^-24 of
 // the largest value.  The keys' scales go onto the scores.  The values' scales go into the weights: the reference of a row is the maximum of
-// score + exponent (in powers of two), so weights times scales stay within fp16, and the denominator takes the scale out again.  Weights are two fp16
-// terms (21 bits).
+// score + exponent (in powers of two), so weights times scales stay within fp16, and the denominator takes the scale out again.  Weights are
+// one fp16 term for the products (2^-12 of a weight at most, an eighth of the output's rounding to bf16) and fp32 for the denominator.
+#include <type_traits>
+
 #include "kv8.cuh"
 #include "tcgen05.cuh"
 
@@ -36,8 +38,9 @@ struct Kv8DecodeParams {
 };
 
 constexpr int KT = 64, WARPS = 4, THREADS = WARPS * 32 + 32, MAX_T = 1024;
-// A row's reference is raised when a weight would be above 2^(TOP + RAISE); weights reach down to 2^-126 beside 2^TOP, so that two rows whose
-// scales are the format's limits apart (2^120) are told apart by weights down to 2^-14 of the largest.
+// Weights are 2^(score + exponent of the value's scale - reference).  A row's reference is raised to 2^TOP below the largest when one would be above
+// 2^(TOP + RAISE), which fp16 holds; fp32 weights reach down to 2^-126, so that two rows whose scales are the format's limits apart (2^120) are told
+// apart by weights down to 2^-14 of the largest.
 constexpr float TOP = 8.f, RAISE = 7.f;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -172,9 +175,9 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
         for (long long w = w0; w < w1 && ok; w += batch) {
             row = nrow;
             head = nhead;
-            look(w + batch + lane / subs, nrow, nhead);
             const int n = (int)min((long long)batch, w1 - w);
             for (int i = 0; i < n; ++i, ++issued) {
+                if (i == min(n - 1, M::STAGES)) look(w + batch + lane / subs, nrow, nhead);      // (some microseconds; the ring is full)
                 const int st = issued % M::STAGES;
                 if (issued >= M::STAGES && !tc::mbar_wait_warp(free_ + st, (uint32_t)(issued / M::STAGES + 1) & 1)) { ok = false; break; }
                 const uint32_t there = __ballot_sync(0xffffffffu, row > -2 && lane / subs == i);
@@ -264,11 +267,12 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
         float m[NG][2], l[NG][2], acc[NG][MT][4];                    // heads 2 c4 and 2 c4 + 1
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
-            m[n][0] = m[n][1] = -INFINITY;
+            m[n][0] = m[n][1] = 0.f;
             l[n][0] = l[n][1] = 0.f;
 #pragma unroll
             for (int i = 0; i < MT; ++i) acc[n][i][0] = acc[n][i][1] = acc[n][i][2] = acc[n][i][3] = 0.f;
         }
+        bool fresh = true;                                           // no reference yet
         for (int j = at.tile; j < at.tile + count; ++j) {
             const int stage = st;
             const uint32_t par = phase;
@@ -278,8 +282,8 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
             if (ok) ok = tc::mbar_wait_warp(full + stage, par);
             const uint8_t *kt = smem + stage * M::STAGE, *vt = kt + M::CODES, *exps = smem + M::EXPS + stage * 2 * KT + k0;
             const int nk = keys - j * KT - k0;                       // of this warp's 32
-            if (nk > 0) {
-                const bool whole = nk >= 32;
+            auto tile = [&](auto all_seen) {
+                constexpr bool WHOLE = decltype(all_seen)::value;
                 float s[NG][2][4];                                   // keys g and g + 8 of 16, heads 2 c4 and 2 c4 + 1
 #pragma unroll
                 for (int n = 0; n < NG; ++n)
@@ -305,50 +309,46 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
                 float kf[4], ev[4], back[4];
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    int eb = exps[g + u * 8], vb = exps[KT + g + u * 8];
-                    if (!whole && g + u * 8 >= nk) eb = vb = KV8_BIAS;
-                    kf[u] = __uint_as_float((uint32_t)eb << 23);
-                    ev[u] = (float)(vb - KV8_BIAS);
-                    back[u] = __uint_as_float((uint32_t)(2 * KV8_BIAS - vb) << 23);
+                    uint32_t eb = exps[g + u * 8], vb = exps[KT + g + u * 8];
+                    if (!WHOLE && g + u * 8 >= nk) eb = vb = KV8_BIAS;
+                    kf[u] = __uint_as_float(eb << 23);
+                    ev[u] = __uint_as_float(0x4b000000u | vb) - (8388608.f + KV8_BIAS);
+                    back[u] = __uint_as_float((2 * KV8_BIAS - vb) << 23);
                 }
-                uint32_t ph[NG][4], pl[NG][4];                       // weights times scales as two terms: head g, keys 2 c4 .. of every 8
+                uint32_t pw[NG][4];                                  // weights times scales: head g, keys 2 c4 and 2 c4 + 1 of every 8
 #pragma unroll
                 for (int n = 0; n < NG; ++n) {
-                    float x[4][2], top[2];
+                    float x[4][2];                                   // log2 of the weights
 #pragma unroll
                     for (int u = 0; u < 4; ++u)
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            x[u][h] = fmaf(s[n][u >> 1][(u & 1) * 2 + h] * kf[u], qf[n][h], ev[u]);
-                            if (!whole && g + u * 8 >= nk) x[u][h] = -INFINITY;
+                            x[u][h] = fmaf(s[n][u >> 1][(u & 1) * 2 + h] * kf[u], qf[n][h], ev[u] - m[n][h]);
+                            if (!WHOLE && g + u * 8 >= nk) x[u][h] = -INFINITY;
                         }
+                    float top[2];
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        top[h] = fmaxf(fmaxf(x[0][h], x[1][h]), fmaxf(x[2][h], x[3][h]));
-#pragma unroll
-                        for (int o = 4; o < 32; o <<= 1) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], o));
-                    }
-                    if (__any_sync(0xffffffffu, top[0] > m[n][0] + RAISE || top[1] > m[n][1] + RAISE)) {
-                        float f[2];
+                    for (int h = 0; h < 2; ++h) top[h] = fmaxf(fmaxf(x[0][h], x[1][h]), fmaxf(x[2][h], x[3][h]));
+                    if (fresh || __any_sync(0xffffffffu, fmaxf(top[0], top[1]) > TOP + RAISE)) {
 #pragma unroll
                         for (int h = 0; h < 2; ++h) {
-                            top[h] = fmaxf(top[h], m[n][h]);
-                            f[h] = m[n][h] == -INFINITY ? 0.f : ex2(m[n][h] - top[h]);
-                            m[n][h] = top[h];
-                            l[n][h] *= f[h];
-                        }
 #pragma unroll
-                        for (int i = 0; i < MT; ++i) { acc[n][i][0] *= f[0]; acc[n][i][1] *= f[1]; acc[n][i][2] *= f[0]; acc[n][i][3] *= f[1]; }
+                            for (int o = 4; o < 32; o <<= 1) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], o));
+                            const float up = fresh ? top[h] - TOP : fmaxf(top[h] - TOP, 0.f), f = fresh ? 1.f : ex2(-up);
+                            m[n][h] += up;
+                            l[n][h] *= f;
+#pragma unroll
+                            for (int u = 0; u < 4; ++u) x[u][h] -= up;
+#pragma unroll
+                            for (int i = 0; i < MT; ++i) { acc[n][i][h] *= f; acc[n][i][2 + h] *= f; }
+                        }
                     }
 #pragma unroll
                     for (int u = 0; u < 4; ++u) {
-                        const float e0 = ex2(x[u][0] - (m[n][0] - TOP)), e1 = ex2(x[u][1] - (m[n][1] - TOP));
+                        const float e0 = ex2(x[u][0]), e1 = ex2(x[u][1]);
                         l[n][0] = fmaf(e0, back[u], l[n][0]);
                         l[n][1] = fmaf(e1, back[u], l[n][1]);
-                        const __half2 hi = __floats2half2_rn(e0, e1);
-                        const float2 hf = __half22float2(hi);
-                        ph[n][u] = transposed8x8(*reinterpret_cast<const uint32_t*>(&hi));
-                        pl[n][u] = transposed8x8(f2_to_f16x2(e0 - hf.x, e1 - hf.y));
+                        pw[n][u] = transposed8x8(f2_to_f16x2(e0, e1));
                     }
                 }
                 // a lane's dims of keys 2 c4, 2 c4 + 1 and 8 on, of each 16 (values of keys that are not seen may be anything: they count as 0)
@@ -366,13 +366,11 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
                                 *reinterpret_cast<uint4*>(v[u]) =
                                     *reinterpret_cast<const uint4*>(vt + x * KT * 128 + (k0 + r) * 128 + ((g ^ (2 * c4 + (u & 1))) << 4));
                             }
-                        }
-                        if (!whole) {
-#pragma unroll
-                            for (int u = 0; u < 4; ++u)
+                            if (!WHOLE) {
 #pragma unroll
                                 for (int i = 0; i < M::CHUNK / 4; ++i)
-                                    if (y * 16 + 2 * c4 + (u & 1) + (u >> 1) * 8 >= nk) v[u][i] = 0u;
+                                    if (r >= nk) v[u][i] = 0u;
+                            }
                         }
 #pragma unroll
                         for (int i = 0; i < M::CHUNK / 4; ++i)
@@ -382,13 +380,13 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
                                 e4m3x4_to_f16(__byte_perm(v[0][i], v[1][i], u ? 0x7362 : 0x5140), a[0], a[1]);
                                 e4m3x4_to_f16(__byte_perm(v[2][i], v[3][i], u ? 0x7362 : 0x5140), a[2], a[3]);
 #pragma unroll
-                                for (int n = 0; n < NG; ++n) {
-                                    mma_f16_16816(acc[n][x * 8 + i * 2 + u], a, ph[n][y * 2], ph[n][y * 2 + 1]);
-                                    mma_f16_16816(acc[n][x * 8 + i * 2 + u], a, pl[n][y * 2], pl[n][y * 2 + 1]);
-                                }
+                                for (int n = 0; n < NG; ++n) mma_f16_16816(acc[n][x * 8 + i * 2 + u], a, pw[n][y * 2], pw[n][y * 2 + 1]);
                             }
                     }
-            }
+            };
+            if (nk >= 32) tile(std::true_type{});
+            else if (nk > 0) tile(std::false_type{});
+            fresh &= nk <= 0;
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(free_ + stage);
         }
@@ -400,7 +398,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) l[n][u] += __shfl_xor_sync(0xffffffffu, l[n][u], o);
                 const int r = n * 8 + c4 * 2 + u;
-                if (g == 0) { sm[warp * M::HG + r] = m[n][u]; sm[(WARPS + warp) * M::HG + r] = l[n][u]; }
+                if (g == 0) { sm[warp * M::HG + r] = fresh ? -INFINITY : m[n][u]; sm[(WARPS + warp) * M::HG + r] = l[n][u]; }
 #pragma unroll
                 for (int i = 0; i < MT; ++i) {                       // a chunk's pairs are turned by its number, for the banks
                     const int d = (i >> (M::CHUNK == 16 ? 3 : 2)) * 128 + g * M::CHUNK + ((i * 2 + g * 2) & (M::CHUNK - 1));
@@ -417,7 +415,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
             for (int y = 1; y < WARPS; ++y) top = fmaxf(top, sm[y * M::HG + r]);
 #pragma unroll
             for (int y = 0; y < WARPS; ++y) {
-                const float ref = sm[y * M::HG + r], f = ref == -INFINITY ? 0.f : ex2(ref - top);
+                const float f = ex2(sm[y * M::HG + r] - top);
                 const float2 o = *reinterpret_cast<const float2*>(so + (y * M::HG + r) * M::LO + x);
                 den += f * sm[(WARPS + y) * M::HG + r];
                 a += f * o.x;
