@@ -1,13 +1,13 @@
 // Attention of one new token per sequence over the 8-bit key/value cache (kv8.cuh): every cached byte is read once, so what counts is bytes in
 // flight and few instructions a byte.
 //
-// All histories are cut into tiles of 64 keys of one key head (and of up to 8 or 16 of its query heads); the tiles of the whole batch, one
+// All histories are cut into tiles of 64 or 32 keys of one key head (and of up to 8 or 16 of its query heads); the tiles of the whole batch, one
 // history behind the other, are dealt out to the blocks in equal shares, so that a batch of ragged histories, one long history and many short ones
 // fill the device alike.  A history that lies in several shares leaves a partial result in each, which kv8_merge_kernel joins.
 //
 // kv8_decode_kernel: a fetching warp brings tiles (TMA, swizzled) and their exponent bytes through a ring of stages, also across the ends of
-// histories; two pairs of warps take tiles in turn, a warp 32 keys of one, with softmax states of their own and no barrier before a history's
-// end.
+// histories; two pairs of warps (heads of more than 128 values: four warps) take tiles in turn, a warp 32
+// keys of one, with softmax states of their own and no barrier before a history's end.
 //
 //   S^T = K Q^T      keys are the 16-row operand: a lane's 16 bytes of two keys are four steps of the product as they lie, since any order
 //                    of the summed dims will do that the queries follow
@@ -33,11 +33,12 @@ struct Kv8DecodeParams {
     float scale;
     bf16* out;                           // [T, n_heads, hd]
     float *o_part, *lse_part;            // [blocks, 2, rows, width], [blocks, 2, rows]
+    int4* jobs;                          // [blocks] what kv8_merge_kernel joins: history (token x items + item), first block, parts, -
     int T;
     int* err;                            // error word of bounded waits
 };
 
-constexpr int KT = 64, WARPS = 4, THREADS = WARPS * 32 + 32, MAX_T = 1024;
+constexpr int WARPS = 4, THREADS = WARPS * 32 + 32, MAX_T = 256;      // MAX_T: tokens a launch
 // Weights are 2^(score + exponent of the value's scale - reference).  A row's reference is raised to 2^TOP below the largest when one would be above
 // 2^(TOP + RAISE), which fp16 holds; fp32 weights reach down to 2^-126, so that two rows whose scales are the format's limits apart (2^120) are told
 // apart by weights down to 2^-14 of the largest.
@@ -68,90 +69,122 @@ __device__ __forceinline__ uint32_t f2_to_f16x2(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
-// The batch's tiles, numbered token by token, key head (and group of query heads) by key head, tile by tile.
+// What a block knows of the batch (shared memory).
+struct Batch {
+    int before[MAX_T + 1];               // tiles of one key head in front of a token
+    int row[MAX_T];                      // page-table row
+    uint8_t last[MAX_T];                 // keys of the last tile - 1
+};
+
+// The batch's tiles of KT keys, numbered token by token, key head (and group of query heads) by key head, tile by tile.
+template <int KT>
 struct Tiles {
-    const int* before;                   // [T + 1] tiles of one key head in front of a token
+    const Batch& batch;
     int T, items;                        // key heads x groups of query heads
     int blocks;                          // that get a share
 
-    __device__ __forceinline__ long long total() const { return (long long)before[T] * items; }
+    // All threads of the block.  At least `per_block` tiles a block.
+    __device__ __forceinline__ Tiles(Batch& b, const Kv8DecodeParams& p, int items_, int most, int per_block) : batch(b), T(p.T), items(items_) {
+        for (int t = threadIdx.x; t < T; t += blockDim.x) {
+            const int pos = p.positions[t];
+            b.before[t + 1] = pos < 0 ? 0 : pos / KT + 1;
+            b.last[t] = (uint8_t)(pos & (KT - 1));
+            b.row[t] = p.batch_idx[t];
+        }
+        if (threadIdx.x == 0) b.before[0] = 0;
+        __syncthreads();
+        if (threadIdx.x < 32) {
+            int sum = 0;
+            for (int t0 = 1; t0 <= T; t0 += 32) {
+                const int t = t0 + threadIdx.x;
+                int x = t <= T ? b.before[t] : 0;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int y = __shfl_up_sync(0xffffffffu, x, o);
+                    if ((int)threadIdx.x >= o) x += y;
+                }
+                if (t <= T) b.before[t] = sum + x;
+                sum += __shfl_sync(0xffffffffu, x, 31);
+            }
+        }
+        __syncthreads();
+        blocks = (int)max(1ll, min((long long)most, (total() + per_block - 1) / per_block));
+    }
+    __device__ __forceinline__ long long total() const { return (long long)batch.before[T] * items; }
     __device__ __forceinline__ long long begin(int b) const { return total() * b / blocks; }
+    __device__ __forceinline__ int block_of(long long w) const { return (int)(((w + 1) * blocks - 1) / total()); }
+    __device__ __forceinline__ int count(int t) const { return batch.before[t + 1] - batch.before[t]; }
     struct Place { int t, item, tile, n; };          // n: tiles of the item
     __device__ __forceinline__ Place at(long long w) const {
-        const int x = (int)(w / items);
+        const int x = total() <= 0x7fffffff ? (int)w / items : (int)(w / items);
         int lo = 0, hi = T;                          // the last token with before <= x (tokens without tiles lie in front of it)
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if (before[mid] <= x) lo = mid;
+            if (batch.before[mid] <= x) lo = mid;
             else hi = mid;
         }
-        const int n = before[lo + 1] - before[lo], off = (int)(w - (long long)before[lo] * items);
+        const int n = count(lo), off = (int)(w - (long long)batch.before[lo] * items);
         return {lo, off / n, off % n, n};
     }
-};
-
-// Fills `before` (shared, T + 1) and returns the numbering; all threads of the block.
-__device__ __forceinline__ Tiles number_tiles(int* before, const int* positions, int T, int items, int blocks, int per_block) {
-    for (int t = threadIdx.x; t < T; t += blockDim.x) before[t + 1] = positions[t] < 0 ? 0 : positions[t] / KT + 1;
-    if (threadIdx.x == 0) before[0] = 0;
-    __syncthreads();
-    if (threadIdx.x < 32) {
-        int sum = 0;
-        for (int t0 = 1; t0 <= T; t0 += 32) {
-            const int t = t0 + threadIdx.x;
-            int x = t <= T ? before[t] : 0;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(0xffffffffu, x, o);
-                if ((int)threadIdx.x >= o) x += y;
-            }
-            if (t <= T) before[t] = sum + x;
-            sum += __shfl_sync(0xffffffffu, x, 31);
-        }
+    // The first tile of the next item (there is one).
+    __device__ __forceinline__ void next(Place& a) const {
+        a.tile = 0;
+        if (++a.item < items) return;
+        a.item = 0;
+        do { ++a.t; } while (count(a.t) == 0);
+        a.n = count(a.t);
     }
-    __syncthreads();
-    Tiles tl{before, T, items, 1};
-    tl.blocks = (int)max(1ll, min((long long)blocks, (tl.total() + per_block - 1) / per_block));
-    return tl;
-}
+};
 
 template <int D, int NG>
 struct Cfg {
+    static constexpr int KT = D > 128 ? 32 : 64, TEAM = KT / 32, TURNS = WARPS / TEAM;      // keys of a tile, warps that share one, tiles at a time
     static constexpr int ROW = D < 128 ? D : 128, HALVES = D / ROW;      // bytes of a row in one box, boxes
-    static constexpr int STAGES = D == 64 ? 6 : D == 128 ? 4 : 2, HG = 8 * NG, LO = D + 4;
+    static constexpr int STAGES = D == 64 ? 6 : D == 128 && NG == 1 ? 6 : 5, HG = 8 * NG;
+    static constexpr int PER_SM = D == 64 ? 3 : 2;
+    static constexpr int CHUNK = D < 128 ? 8 : 16, MT = D / 16;          // neighbouring dims of a lane, 16-dim rows of products
     static constexpr int CODES = KT * D, STAGE = 2 * CODES;              // keys, values
-    static constexpr int EXPS = STAGES * STAGE;                          // 64 bytes of the keys, 64 of the values
-    static constexpr int JOIN = EXPS + STAGES * 2 * KT;                  // fp32 [WARPS][HG][LO], then [2][WARPS][HG]
-    static constexpr int BEFORE = JOIN + (WARPS * HG * LO + 2 * WARPS * HG) * 4;
-    static constexpr int BARS = (BEFORE + (MAX_T + 1) * 4 + 7) / 8 * 8;
-    static constexpr int TOTAL = BARS + 2 * STAGES * 8;
-    static constexpr int PER_SM = D == 64 && NG == 1 ? 3 : 2;
-    static_assert(STAGES % 2 == 0, "a stage belongs to one pair of warps: a barrier is never two phases ahead of who waits for it");
-    static constexpr int CHUNK = D < 128 ? 8 : 16;                       // neighbouring dims of a lane
+    static constexpr int EXPS = STAGES * STAGE;                          // KT bytes of the keys, KT of the values
+    static constexpr int Q = EXPS + STAGES * 2 * KT, Q_BYTES = HG * D * 2;         // two histories' queries
+    static constexpr int JOIN = Q + 2 * Q_BYTES, SLOT = NG * MT * 4 * 32 * 4 + 2 * HG * 4;       // sums as they lie in registers, references, denominators
+    static constexpr int BATCH = JOIN + 2 * SLOT;
+    static constexpr int BARS = (BATCH + (int)sizeof(Batch) + 7) / 8 * 8;
+    static constexpr int TOTAL = BARS + (2 * STAGES + 4) * 8;
 };
+
+__device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 
 // grid: blocks of the device, block 160
 template <int D, int NG>
 __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                                                                               Kv8DecodeParams p, int box, int per_block) {
+                                                                               Kv8DecodeParams p, int box, int per_block, bool by_item) {
     using M = Cfg<D, NG>;
+    constexpr int KT = M::KT, MT = M::MT;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    uint64_t *full = reinterpret_cast<uint64_t*>(smem + M::BARS), *free_ = full + M::STAGES;
+    uint64_t *full = reinterpret_cast<uint64_t*>(smem + M::BARS), *free_ = full + M::STAGES, *q_full = free_ + M::STAGES, *q_free = q_full + 2;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
         for (int i = 0; i < M::STAGES; ++i) {
             tc::mbar_init(full + i, 1);
-            tc::mbar_init(free_ + i, 2);
+            tc::mbar_init(free_ + i, WARPS);
+        }
+        for (int i = 0; i < 2; ++i) {
+            tc::mbar_init(q_full + i, 1);
+            tc::mbar_init(q_free + i, WARPS);
         }
         tc::mbar_fence_init();
     }
     pdl_grid_sync();
     const int group = p.n_heads / p.n_kv, hg = (group + M::HG - 1) / M::HG;
-    const Tiles tiles = number_tiles(reinterpret_cast<int*>(smem + M::BEFORE), p.positions, p.T, p.n_kv * hg, gridDim.x, per_block);
+    const Tiles<KT> tiles(*reinterpret_cast<Batch*>(smem + M::BATCH), p, p.n_kv * hg, gridDim.x, per_block);
     for (int t = blockIdx.x; t < p.T; t += gridDim.x)
-        if (p.positions[t] < 0)
+        if (tiles.count(t) == 0) {
             for (int i = tid; i < p.n_heads * p.hd / 2; i += THREADS) reinterpret_cast<uint32_t*>(p.out + (size_t)t * p.n_heads * p.hd)[i] = 0u;
+            if (by_item)
+                for (int i = tid; i < tiles.items; i += THREADS) p.jobs[t * tiles.items + i] = make_int4(0, 0, 0, 0);
+        }
+    if (!by_item && tid == 0) p.jobs[blockIdx.x] = make_int4(0, 0, 0, 0);
     if (blockIdx.x >= tiles.blocks) return;
     const long long w0 = tiles.begin(blockIdx.x), w1 = tiles.begin(blockIdx.x + 1);
     if (w0 >= w1) return;
@@ -159,33 +192,39 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
     if (warp == WARPS) {
         // ---- fetching: a lane looks up the place of one box of a tile ahead ----
         const int subs = KT / box, batch = 32 / subs;
-        const bool one = p.pages.page_size == box;               // a box's exponent bytes of keys and values are neighbours
-        auto look = [&](long long w, int& row, int& head) {
-            row = -2;                                            // nothing to fetch
-            head = 0;
-            if (w >= w1) return;
-            const Tiles::Place at = tiles.at(w);
-            const int key = at.tile * KT + lane % subs * box;
-            head = at.item / hg;
-            if (key <= p.positions[at.t]) row = kv8_slot(p.pages, 32, p.batch_idx[at.t], key);
+        struct Ahead { int row, t, item; bool first; };          // slot of a box (-1: a page that is not there, -2: nothing to fetch); a history's first tile
+        auto look = [&](long long w) -> Ahead {
+            if (w >= w1) return {-2, 0, 0, false};
+            const typename Tiles<KT>::Place at = tiles.at(w);
+            const int key = at.tile * KT + lane % subs * box, n = at.n * KT - (KT - 1) + tiles.batch.last[at.t];
+            return {key < n ? kv8_slot(p.pages, 32, tiles.batch.row[at.t], key) : -2, at.t, at.item, w == w0 || at.tile == 0};
         };
-        int row, head, nrow, nhead, issued = 0;
+        int issued = 0, asked = 0;                               // tiles, histories
         bool ok = true;
-        look(w0 + lane / subs, nrow, nhead);
+        Ahead now, then = look(w0 + lane / subs);
         for (long long w = w0; w < w1 && ok; w += batch) {
-            row = nrow;
-            head = nhead;
+            now = then;
             const int n = (int)min((long long)batch, w1 - w);
             for (int i = 0; i < n; ++i, ++issued) {
-                if (i == min(n - 1, M::STAGES)) look(w + batch + lane / subs, nrow, nhead);      // (some microseconds; the ring is full)
-                const int st = issued % M::STAGES;
+                if (i == min(n - 1, M::STAGES)) then = look(w + batch + lane / subs);      // (a microsecond; the ring is full)
+                const int st = issued % M::STAGES, item = __shfl_sync(0xffffffffu, now.item, i * subs), h = item / hg;
+                if (__shfl_sync(0xffffffffu, (int)now.first, i * subs)) {
+                    const int qb = asked & 1, t = __shfl_sync(0xffffffffu, now.t, i * subs), r_lo = item % hg * M::HG;
+                    if (asked >= 2 && !tc::mbar_wait_warp(q_free + qb, (uint32_t)((asked >> 1) + 1) & 1)) { ok = false; break; }
+                    if (lane == 0) {
+                        const uint32_t bytes = min(M::HG, group - r_lo) * p.hd * 2;
+                        tc::mbar_expect_tx(q_full + qb, bytes);
+                        tc::bulk_load_1d(smem + M::Q + qb * M::Q_BYTES, p.q + ((size_t)t * p.n_heads + h * group + r_lo) * p.hd, bytes, q_full + qb);
+                    }
+                    ++asked;
+                }
                 if (issued >= M::STAGES && !tc::mbar_wait_warp(free_ + st, (uint32_t)(issued / M::STAGES + 1) & 1)) { ok = false; break; }
-                const uint32_t there = __ballot_sync(0xffffffffu, row > -2 && lane / subs == i);
+                const uint32_t there = __ballot_sync(0xffffffffu, now.row > -2 && lane / subs == i);
                 if (lane == 0) tc::mbar_expect_tx(full + st, __popc(there) * box * (2 * D + 2));
                 uint8_t* codes = smem + st * M::STAGE;
                 uint8_t* exps = smem + M::EXPS + st * 2 * KT;
                 for (int u = 0; u < subs; ++u) {
-                    const int r = __shfl_sync(0xffffffffu, row, i * subs + u), h = __shfl_sync(0xffffffffu, head, i * subs + u);
+                    const int r = __shfl_sync(0xffffffffu, now.row, i * subs + u);
                     if (r > -2 && lane == 0) {
 #pragma unroll
                         for (int x = 0; x < M::HALVES; ++x) {    // (a page that is not there: rows in front of the tensor read as zeros)
@@ -193,7 +232,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
                             tc::tma_load_3d(codes + M::CODES + x * KT * M::ROW + u * box * M::ROW, &map_v, full + st, x * 128, h, r < 0 ? -KT : r);
                         }
                         const uint8_t* e = p.exps + kv8_exp_at(p.pages, p.n_kv, max(r, 0), h);
-                        if (one && box == KT) {
+                        if (box == KT && p.pages.page_size == KT) {          // the bytes of keys and values are neighbours
                             tc::bulk_load_1d(exps, e, 2 * KT, full + st);
                         } else {
                             tc::bulk_load_1d(exps + u * box, e, box, full + st);
@@ -206,30 +245,30 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
         }
         // nothing is in flight when the block ends, also where a wait ran out
         for (int j = max(0, issued - M::STAGES); j < issued; ++j) ok &= tc::mbar_wait_warp(full + j % M::STAGES, (uint32_t)(j / M::STAGES) & 1);
+        for (int j = max(0, asked - 2); j < asked; ++j) ok &= tc::mbar_wait_warp(q_full + (j & 1), (uint32_t)(j >> 1) & 1);
         if (!ok && lane == 0) atomicExch(p.err, 50);
         return;
     }
 
-    // ---- products: a pair of warps takes every other tile, a warp 32 of its keys ----
-    const int g = lane >> 2, c4 = lane & 3, k0 = (warp & 1) * 32;
-    float* const so = reinterpret_cast<float*>(smem + M::JOIN);
-    float* const sm = so + WARPS * M::HG * M::LO;                    // references, then sums
-    constexpr int MT = D / 16, CH = D < 128 ? 1 : D / 64;            // 16-dim rows of products, 16-byte pieces of a key row a lane reads
+    // ---- products: the warps of a team take 32 keys each of every tile that is their turn ----
+    const int g = lane >> 2, c4 = lane & 3, k0 = warp % M::TEAM * 32;
+    constexpr int CH = D < 128 ? 1 : D / 64;                         // 16-byte pieces of a key row a lane reads
     // places of a lane's pieces in a tile
     const int ks = D < 128 ? (k0 + g) * 64 + ((c4 ^ (g >> 1 & 3)) << 4) : (k0 + g) * 128;
-    int st = 0, turn = warp >> 1;                                    // 0: this pair's tile
+    int st = 0, turn = warp / M::TEAM, done = 0;                     // 0: this team's tile; histories behind it
     uint32_t phase = 0;
     bool ok = true;
-    for (long long w = w0; w < w1;) {
-        const Tiles::Place at = tiles.at(w);
+    typename Tiles<KT>::Place at = tiles.at(w0);
+    for (long long w = w0;;) {
         const int count = (int)min((long long)(at.n - at.tile), w1 - w), t = at.t, hkv = at.item / hg, r_lo = at.item % hg * M::HG;
-        const int nr = min(M::HG, group - r_lo), h0 = hkv * group + r_lo, keys = p.positions[t] + 1;
+        const int nr = min(M::HG, group - r_lo), h0 = hkv * group + r_lo, keys = at.n * KT - (KT - 1) + tiles.batch.last[t];
         // queries as fp16 times 2^-eq: a lane holds head g's dims of its pieces, in the order of the pieces' bytes
         uint32_t q[NG][CH * 4][2];
         float qf[NG][2];                                             // factors on the scores of heads 2 c4 and 2 c4 + 1
+        if (ok) ok = tc::mbar_wait_warp(q_full + (done & 1), (uint32_t)(done >> 1) & 1);
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
-            const bf16* src = p.q + ((size_t)t * p.n_heads + h0 + n * 8 + g) * p.hd;
+            const uint8_t* src = smem + M::Q + (done & 1) * M::Q_BYTES + (n * 8 + g) * p.hd * 2;
             uint4 raw[CH][2];
             float top = 0.f;
 #pragma unroll
@@ -237,8 +276,8 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
                 const int d = D < 128 ? c4 * 16 : (j >> 1) * 128 + (2 * c4 + (j & 1)) * 16;
                 raw[j][0] = raw[j][1] = make_uint4(0u, 0u, 0u, 0u);
                 if (n * 8 + g < nr && d < p.hd) {
-                    raw[j][0] = *reinterpret_cast<const uint4*>(src + d);
-                    raw[j][1] = *reinterpret_cast<const uint4*>(src + d + 8);
+                    raw[j][0] = *reinterpret_cast<const uint4*>(src + d * 2);
+                    raw[j][1] = *reinterpret_cast<const uint4*>(src + d * 2 + 16);
                 }
                 const uint32_t* u = reinterpret_cast<const uint32_t*>(raw[j]);
 #pragma unroll
@@ -264,6 +303,9 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
                 }
             }
         }
+        __syncwarp();
+        if (lane == 0) tc::mbar_arrive(q_free + (done & 1));
+        ++done;
         float m[NG][2], l[NG][2], acc[NG][MT][4];                    // heads 2 c4 and 2 c4 + 1
 #pragma unroll
         for (int n = 0; n < NG; ++n) {
@@ -275,13 +317,13 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
         bool fresh = true;                                           // no reference yet
         for (int j = at.tile; j < at.tile + count; ++j) {
             const int stage = st;
-            const uint32_t par = phase;
+            // (also where it is another team's turn: a barrier must not be two phases ahead of who waits for it)
+            if (ok) ok = tc::mbar_wait_warp(full + stage, phase);
             if (++st == M::STAGES) { st = 0; phase ^= 1u; }
-            turn ^= 1;
-            if (turn == 0) continue;
-            if (ok) ok = tc::mbar_wait_warp(full + stage, par);
+            const bool mine = turn == 0;
+            if (++turn == M::TURNS) turn = 0;
             const uint8_t *kt = smem + stage * M::STAGE, *vt = kt + M::CODES, *exps = smem + M::EXPS + stage * 2 * KT + k0;
-            const int nk = keys - j * KT - k0;                       // of this warp's 32
+            const int nk = mine ? keys - j * KT - k0 : 0;            // of this warp's 32
             auto tile = [&](auto all_seen) {
                 constexpr bool WHOLE = decltype(all_seen)::value;
                 float s[NG][2][4];                                   // keys g and g + 8 of 16, heads 2 c4 and 2 c4 + 1
@@ -387,81 +429,121 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
             if (nk >= 32) tile(std::true_type{});
             else if (nk > 0) tile(std::false_type{});
             fresh &= nk <= 0;
+
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(free_ + stage);
         }
-        // ---- join the warps ----
+        // ---- join the warps, 1 into 0, 3 into 2, 2 into 0: lanes of the same number have the same places ----
 #pragma unroll
         for (int n = 0; n < NG; ++n)
 #pragma unroll
-            for (int u = 0; u < 2; ++u) {
+            for (int h = 0; h < 2; ++h) {
 #pragma unroll
-                for (int o = 4; o < 32; o <<= 1) l[n][u] += __shfl_xor_sync(0xffffffffu, l[n][u], o);
-                const int r = n * 8 + c4 * 2 + u;
-                if (g == 0) { sm[warp * M::HG + r] = fresh ? -INFINITY : m[n][u]; sm[(WARPS + warp) * M::HG + r] = l[n][u]; }
+                for (int o = 4; o < 32; o <<= 1) l[n][h] += __shfl_xor_sync(0xffffffffu, l[n][h], o);
+                if (fresh) m[n][h] = -INFINITY;
+            }
+        float* const slot = reinterpret_cast<float*>(smem + M::JOIN + (warp >> 1) * M::SLOT);
+        auto give = [&](float* to) {
+            float* const state = to + NG * MT * 4 * 32;
 #pragma unroll
-                for (int i = 0; i < MT; ++i) {                       // a chunk's pairs are turned by its number, for the banks
-                    const int d = (i >> (M::CHUNK == 16 ? 3 : 2)) * 128 + g * M::CHUNK + ((i * 2 + g * 2) & (M::CHUNK - 1));
-                    *reinterpret_cast<float2*>(so + (warp * M::HG + r) * M::LO + d) = make_float2(acc[n][i][u], acc[n][i][2 + u]);
+            for (int n = 0; n < NG; ++n) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) to[((n * MT + i) * 4 + x) * 32 + lane] = acc[n][i][x];
+                if (g == 0)
+#pragma unroll
+                    for (int h = 0; h < 2; ++h) {
+                        state[n * 8 + c4 * 2 + h] = m[n][h];
+                        state[M::HG + n * 8 + c4 * 2 + h] = l[n][h];
+                    }
+            }
+        };
+        auto take = [&](const float* from) {
+            const float* const state = from + NG * MT * 4 * 32;
+#pragma unroll
+            for (int n = 0; n < NG; ++n)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float mo = state[n * 8 + c4 * 2 + h], top = fmaxf(m[n][h], mo);
+                    const float f = m[n][h] == -INFINITY ? 0.f : ex2(m[n][h] - top), fo = mo == -INFINITY ? 0.f : ex2(mo - top);
+                    m[n][h] = top;
+                    l[n][h] = f * l[n][h] + fo * state[M::HG + n * 8 + c4 * 2 + h];
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+#pragma unroll
+                        for (int x = h; x < 4; x += 2) acc[n][i][x] = f * acc[n][i][x] + fo * from[((n * MT + i) * 4 + x) * 32 + lane];
                 }
+        };
+        pair_sync(1 + (warp >> 1));                                  // (the slot's last reader is done)
+        if (warp & 1) give(slot);
+        pair_sync(1 + (warp >> 1));
+        if (warp == 2) {
+            take(slot);
+            __syncwarp();
+            give(slot);
+            pair_sync(3);
+            pair_sync(3);                                            // (warp 0 has read the slot)
+        } else if (warp == 0) {
+            take(slot);
+            pair_sync(3);
+            take(reinterpret_cast<const float*>(smem + M::JOIN + M::SLOT));
+            pair_sync(3);
+            const bool whole = count == at.n;
+            const size_t part = (size_t)blockIdx.x * 2 + (at.tile == 0 ? 1 : 0);
+            if (at.tile == 0 && lane == 0) {
+                const int parts = whole ? 1 : tiles.block_of(w + at.n - 1) - (int)blockIdx.x + 1;
+                if (by_item) p.jobs[t * tiles.items + at.item] = make_int4(t * tiles.items + at.item, blockIdx.x, parts, 0);
+                else if (!whole) p.jobs[blockIdx.x] = make_int4(t * tiles.items + at.item, blockIdx.x, parts, 0);
             }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
-        const bool whole = count == at.n;
-        const size_t part = (size_t)blockIdx.x * 2 + (at.tile == 0 ? 1 : 0);
-        for (int i = tid; i < nr * (D / 2); i += WARPS * 32) {
-            const int r = i / (D / 2), d = i % (D / 2) * 2, ch = d / M::CHUNK, x = ch * M::CHUNK + ((d + (ch & 7) * 2) & (M::CHUNK - 1));
-            float top = sm[r], den = 0.f, a = 0.f, b = 0.f;
 #pragma unroll
-            for (int y = 1; y < WARPS; ++y) top = fmaxf(top, sm[y * M::HG + r]);
+            for (int n = 0; n < NG; ++n)
 #pragma unroll
-            for (int y = 0; y < WARPS; ++y) {
-                const float f = ex2(sm[y * M::HG + r] - top);
-                const float2 o = *reinterpret_cast<const float2*>(so + (y * M::HG + r) * M::LO + x);
-                den += f * sm[(WARPS + y) * M::HG + r];
-                a += f * o.x;
-                b += f * o.y;
-            }
-            a /= den;
-            b /= den;
-            if (whole) {
-                if (d < p.hd) *reinterpret_cast<uint32_t*>(p.out + ((size_t)t * p.n_heads + h0 + r) * p.hd + d) = f2_to_bf162(a, b);
-            } else {
-                *reinterpret_cast<float2*>(p.o_part + (part * M::HG + r) * D + d) = make_float2(a, b);
-                if (d == 0) p.lse_part[part * M::HG + r] = top + log2f(den);
-            }
+                for (int h = 0; h < 2; ++h) {
+                    const int r = n * 8 + c4 * 2 + h;
+                    if (r >= nr) continue;
+                    const float inv = 1.f / l[n][h];
+                    if (!whole && g == 0) p.lse_part[part * M::HG + r] = m[n][h] + log2f(l[n][h]);
+#pragma unroll
+                    for (int x = 0; x < M::HALVES; ++x) {
+                        const int d = x * 128 + g * M::CHUNK, i0 = x * 8;
+                        if (whole && d < p.hd) {
+                            uint4* dst = reinterpret_cast<uint4*>(p.out + ((size_t)t * p.n_heads + h0 + r) * p.hd + d);
+                            uint32_t o[M::CHUNK / 2];
+#pragma unroll
+                            for (int i = 0; i < M::CHUNK / 2; ++i) o[i] = f2_to_bf162(acc[n][i0 + i][h] * inv, acc[n][i0 + i][2 + h] * inv);
+#pragma unroll
+                            for (int i = 0; i < M::CHUNK / 8; ++i) dst[i] = make_uint4(o[i * 4], o[i * 4 + 1], o[i * 4 + 2], o[i * 4 + 3]);
+                        } else if (!whole) {
+                            float4* dst = reinterpret_cast<float4*>(p.o_part + (part * M::HG + r) * D + d);
+#pragma unroll
+                            for (int i = 0; i < M::CHUNK / 4; ++i)
+                                dst[i] = make_float4(acc[n][i0 + i * 2][h] * inv, acc[n][i0 + i * 2][2 + h] * inv, acc[n][i0 + i * 2 + 1][h] * inv,
+                                                     acc[n][i0 + i * 2 + 1][2 + h] * inv);
+                        }
+                    }
+                }
         }
-        asm volatile("bar.sync 1, 128;" ::: "memory");
         w += count;
+        if (w >= w1) break;
+        tiles.next(at);
     }
     if (!ok && lane == 0) atomicExch(p.err, 51);
 }
 
 // Joins the partial results of histories that lie in several shares: the first part is its block's second partial result, the others are their
-// blocks' first.  Block (i, y): the i-th history (ALL), or the one that share i + 1 begins inside of, if no share in front of it does; rows y * R ..
-// of its query heads.  A thread has 4 neighbouring values, D / 4 threads a row and 512 / (D / 4) / R of the parts in turn.
-template <int D, int HG, int R, bool ALL>
-__global__ void __launch_bounds__(512) kv8_merge_kernel(Kv8DecodeParams p, int blocks, int per_block) {
+// blocks' first.  Block (i, y): jobs[i], rows y * R .. of its query heads.  A thread has 4 neighbouring values, D / 4 threads a row and
+// 512 / (D / 4) / R of the parts in turn.
+template <int D, int HG, int R>
+__global__ void __launch_bounds__(512) kv8_merge_kernel(Kv8DecodeParams p) {
     constexpr int LANES = D / 4, TURNS = 512 / LANES / R, AHEAD = 4;
-    __shared__ int before[MAX_T + 1];
     __shared__ float4 sums[512];
     __shared__ float2 state[512 / LANES];            // reference and denominator
     pdl_grid_sync();
-    const int group = p.n_heads / p.n_kv, hg = (group + HG - 1) / HG, tid = threadIdx.x;
-    const Tiles tiles = number_tiles(before, p.positions, p.T, p.n_kv * hg, blocks, per_block);
-    long long w;
-    if (ALL) {
-        const int t = blockIdx.x / tiles.items;
-        w = (long long)before[t] * tiles.items + (long long)(blockIdx.x % tiles.items) * (before[t + 1] - before[t]);
-        if (before[t + 1] == before[t]) return;
-    } else {
-        if ((int)blockIdx.x + 1 >= tiles.blocks) return;
-        w = tiles.begin(blockIdx.x + 1);
-    }
-    const Tiles::Place at = tiles.at(w);
-    const long long first = w - at.tile, total = tiles.total();
-    const int b0 = (int)(((first + 1) * tiles.blocks - 1) / total), b1 = (int)(((first + at.n) * tiles.blocks - 1) / total), n = b1 - b0 + 1;
-    if (n == 1 || (!ALL && (at.tile == 0 || b0 != (int)blockIdx.x))) return;
-    const int hkv = at.item / hg, r_lo = at.item % hg * HG, part_row = tid / LANES, r = blockIdx.y * R + part_row % R, d = tid % LANES * 4;
+    const int4 job = p.jobs[blockIdx.x];
+    if (job.z < 2) return;
+    const int group = p.n_heads / p.n_kv, hg = (group + HG - 1) / HG, tid = threadIdx.x, t = job.x / (p.n_kv * hg), item = job.x % (p.n_kv * hg), b0 = job.y, n = job.z;
+    const int hkv = item / hg, r_lo = item % hg * HG, part_row = tid / LANES, r = blockIdx.y * R + part_row % R, d = tid % LANES * 4;
     const bool on = r < min(HG, group - r_lo);
     float top = -INFINITY, den = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -510,7 +592,7 @@ __global__ void __launch_bounds__(512) kv8_merge_kernel(Kv8DecodeParams p, int b
         }
     }
     if (on && d < p.hd)
-        *reinterpret_cast<uint2*>(p.out + ((size_t)at.t * p.n_heads + hkv * group + r_lo + r) * p.hd + d) =
+        *reinterpret_cast<uint2*>(p.out + ((size_t)t * p.n_heads + hkv * group + r_lo + r) * p.hd + d) =
             make_uint2(f2_to_bf162(o.x / den, o.y / den), f2_to_bf162(o.z / den, o.w / den));
 }
 
@@ -535,7 +617,7 @@ int launch(const Kv8DecodeParams* all, int T, int blocks, cudaStream_t s) {
     constexpr int smem = M::TOTAL + 1024;
     static_assert(M::PER_SM * (smem + 1024) <= 228 * 1024, "blocks per SM");
     static SmemOptIn opt_in;
-    const int box = all->pages.page_size % 64 == 0 ? 64 : all->pages.page_size % 32 == 0 ? 32 : 16, per_block = 1;
+    const int page = all->pages.page_size, box = page % M::KT == 0 ? M::KT : page % 32 == 0 ? 32 : 16, per_block = 1;
     CUtensorMap mk, mv;
     int rc = map_codes(&mk, all->k_codes, all, D, box);
     if (rc == 0) rc = map_codes(&mv, all->v_codes, all, D, box);
@@ -549,11 +631,12 @@ int launch(const Kv8DecodeParams* all, int T, int blocks, cudaStream_t s) {
         p.out += t * row;
         p.positions += t;
         p.batch_idx += t;
-        sl_launch(kv8_decode_kernel<D, NG>, blocks, THREADS, smem, s, mk, mv, p, box, per_block);
-        // few histories have many parts each: a block a query head; many have few: a block for all of a share's border
+        // few histories have many parts each: a block a query head; many have few: a block for the one that a share's end cuts
         const int group = p.n_heads / p.n_kv, items = p.T * p.n_kv * ((group + M::HG - 1) / M::HG);
-        if (blocks > 1 && items < blocks) sl_launch(kv8_merge_kernel<D, M::HG, 1, true>, dim3(items, M::HG < group ? M::HG : group), 512, 0, s, p, blocks, per_block);
-        else if (blocks > 1) sl_launch(kv8_merge_kernel<D, M::HG, M::HG, false>, blocks - 1, 512, 0, s, p, blocks, per_block);
+        const bool by_item = items <= blocks;
+        sl_launch(kv8_decode_kernel<D, NG>, blocks, THREADS, smem, s, mk, mv, p, box, per_block, by_item);
+        if (by_item) sl_launch(kv8_merge_kernel<D, M::HG, 1>, dim3(items, M::HG < group ? M::HG : group), 512, 0, s, p);
+        else sl_launch(kv8_merge_kernel<D, M::HG, M::HG>, blocks, 512, 0, s, p);
         rc = SL_LAUNCH_CHECK();
         if (rc != 0) return rc;
     }
@@ -562,7 +645,7 @@ int launch(const Kv8DecodeParams* all, int T, int blocks, cudaStream_t s) {
 
 }  // namespace
 
-// Blocks that attention of these sizes is dealt out to, and what a partial result takes: 2 `rows` x `width` sums (and as many / `width` references) a block.
+// Blocks that attention of these sizes is dealt out to, and what a partial result takes: 2 `rows` x `width` sums, 2 `rows` references and 16 bytes a block.
 SL_API int sl_kv8_decode_plan(int n_heads, int n_kv, int hd, int* blocks, int* rows, int* width) {
     if (hd < 16 || hd > 256 || hd % 16 != 0 || n_kv < 1 || n_heads < n_kv || n_heads % n_kv != 0) return -1;
     int device = 0, sms = 0;
@@ -570,7 +653,7 @@ SL_API int sl_kv8_decode_plan(int n_heads, int n_kv, int hd, int* blocks, int* r
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
     if (e != cudaSuccess) return (int)e;
     const Shape sh = shape_of(n_heads, n_kv, hd);
-    *blocks = sms * (sh.width == 64 && sh.tiles == 1 ? 3 : 2);
+    *blocks = sms * (sh.width == 64 ? 3 : 2);
     *rows = 8 * sh.tiles;
     *width = sh.width;
     return 0;
@@ -580,8 +663,8 @@ SL_API int sl_kv8_decode_plan(int n_heads, int n_kv, int hd, int* blocks, int* r
 SL_API int sl_kv8_decode(const Kv8DecodeParams* p, int T, int blocks, cudaStream_t s) {
     if (T == 0) return 0;
     if (p->hd < 16 || p->hd > 256 || p->hd % 16 != 0 || p->n_kv < 1 || p->n_heads % p->n_kv != 0 || blocks < 1) return -1;
-    if (p->pages.page_size < 16 || p->pages.page_size % 16 != 0 || p->o_part == nullptr || p->lse_part == nullptr) return -1;
-    if ((((uintptr_t)p->q | (uintptr_t)p->k_codes | (uintptr_t)p->v_codes | (uintptr_t)p->exps | (uintptr_t)p->out | (uintptr_t)p->o_part) & 15) != 0) return -1;
+    if (p->pages.page_size < 16 || p->pages.page_size % 16 != 0 || p->o_part == nullptr || p->lse_part == nullptr || p->jobs == nullptr) return -1;
+    if ((((uintptr_t)p->q | (uintptr_t)p->k_codes | (uintptr_t)p->v_codes | (uintptr_t)p->exps | (uintptr_t)p->out | (uintptr_t)p->o_part | (uintptr_t)p->jobs) & 15) != 0) return -1;
     const Shape sh = shape_of(p->n_heads, p->n_kv, p->hd);
     if (sh.width == 64) return sh.tiles == 2 ? launch<64, 2>(p, T, blocks, s) : launch<64, 1>(p, T, blocks, s);
     if (sh.width == 128) return sh.tiles == 2 ? launch<128, 2>(p, T, blocks, s) : launch<128, 1>(p, T, blocks, s);

@@ -60,7 +60,7 @@ class Kv8UnpackParams(C.Structure):
 class Kv8DecodeParams(C.Structure):
     _fields_ = [("q", C.c_void_p), ("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("exps", C.c_void_p), ("positions", C.c_void_p),
                 ("batch_idx", C.c_void_p), ("pages", _Pages), ("n_heads", C.c_int), ("n_kv", C.c_int), ("hd", C.c_int), ("scale", C.c_float),
-                ("out", C.c_void_p), ("o_part", C.c_void_p), ("lse_part", C.c_void_p), ("T", C.c_int), ("err", C.c_void_p)]
+                ("out", C.c_void_p), ("o_part", C.c_void_p), ("lse_part", C.c_void_p), ("jobs", C.c_void_p), ("T", C.c_int), ("err", C.c_void_p)]
 
 
 @dataclass
@@ -247,10 +247,11 @@ def kv8_attention(q, cache: Kv8Cache, positions, batch_idx, page_table, sm_scale
     if qo_indptr is None:
         from . import tcgen05
         blocks, rows, wide = _decode_plan(q.get_device(), n_heads, n_kv, hd)
-        part = torch.empty(blocks * 2 * rows * (wide + 1), dtype=torch.float32, device=q.device)
+        part = torch.empty(blocks * (2 * rows * (wide + 1) + 4), dtype=torch.float32, device=q.device)
+        sums = part.data_ptr() + blocks * 16
         p = Kv8DecodeParams(q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.exps.data_ptr(), positions.data_ptr(), batch_idx.data_ptr(),
-                            _pages(cache, page_table), n_heads, n_kv, hd, sm_scale, out.data_ptr(), part.data_ptr(),
-                            part.data_ptr() + blocks * 2 * rows * wide * 4, 0, tcgen05.error_flag(q.device).data_ptr())
+                            _pages(cache, page_table), n_heads, n_kv, hd, sm_scale, out.data_ptr(), sums,
+                            sums + blocks * 2 * rows * wide * 4, part.data_ptr(), 0, tcgen05.error_flag(q.device).data_ptr())
         _call(q, "sl_kv8_decode", C.byref(p), T, blocks)
         return out
     if hd not in (64, 128):
