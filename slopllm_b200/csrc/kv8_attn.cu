@@ -17,8 +17,6 @@
 // the largest value.  The keys' scales go onto the scores.  The values' scales go into the weights: the reference of a row is the maximum of
 // score + exponent (in powers of two), so weights times scales stay within fp16, and the denominator takes the scale out again.  Weights are
 // one fp16 term for the products (2^-12 of a weight at most, an eighth of the output's rounding to bf16) and fp32 for the denominator.
-#include <type_traits>
-
 #include "kv8.cuh"
 #include "tcgen05.cuh"
 
@@ -69,6 +67,9 @@ __device__ __forceinline__ uint32_t f2_to_f16x2(float a, float b) {
     return *reinterpret_cast<const uint32_t*>(&h);
 }
 
+// What kv8_merge_kernel finds in `jobs`: nothing (shares end where histories do), a history, or the history that a block's share ends inside of.
+enum class Parts { NONE, BY_ITEM, BY_BLOCK };
+
 // What a block knows of the batch (shared memory).
 struct Batch {
     int before[MAX_T + 1];               // tiles of one key head in front of a token
@@ -83,40 +84,54 @@ struct Tiles {
     int T, items;                        // key heads x groups of query heads
     int blocks;                          // that get a share
 
-    // All threads of the block.  At least `per_block` tiles a block.
-    __device__ __forceinline__ Tiles(Batch& b, const Kv8DecodeParams& p, int items_, int most, int per_block) : batch(b), T(p.T), items(items_) {
-        for (int t = threadIdx.x; t < T; t += blockDim.x) {
-            const int pos = p.positions[t];
-            b.before[t + 1] = pos < 0 ? 0 : pos / KT + 1;
-            b.last[t] = (uint8_t)(pos & (KT - 1));
-            b.row[t] = p.batch_idx[t];
+    // Tiles of token t.
+    __device__ __forceinline__ static int note(const Kv8DecodeParams& p, Batch& b, int t) {
+        const int pos = p.positions[t];
+        b.last[t] = (uint8_t)(pos & (KT - 1));
+        b.row[t] = p.batch_idx[t];
+        return pos < 0 ? 0 : pos / KT + 1;
+    }
+    // All threads of the block.
+    __device__ __forceinline__ Tiles(Batch& b, const Kv8DecodeParams& p, int items_, int most) : batch(b), T(p.T), items(items_) {
+        if (T > 32) {
+            for (int t = threadIdx.x; t < T; t += blockDim.x) b.before[t + 1] = note(p, b, t);
+            __syncthreads();
         }
-        if (threadIdx.x == 0) b.before[0] = 0;
-        __syncthreads();
         if (threadIdx.x < 32) {
             int sum = 0;
-            for (int t0 = 1; t0 <= T; t0 += 32) {
+            for (int t0 = 0; t0 < T; t0 += 32) {
                 const int t = t0 + threadIdx.x;
-                int x = t <= T ? b.before[t] : 0;
+                int x = t >= T ? 0 : T > 32 ? b.before[t + 1] : note(p, b, t);
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
                     const int y = __shfl_up_sync(0xffffffffu, x, o);
                     if ((int)threadIdx.x >= o) x += y;
                 }
-                if (t <= T) b.before[t] = sum + x;
+                if (t < T) b.before[t + 1] = sum + x;
                 sum += __shfl_sync(0xffffffffu, x, 31);
             }
+            if (threadIdx.x == 0) b.before[0] = 0;
         }
         __syncthreads();
-        blocks = (int)max(1ll, min((long long)most, (total() + per_block - 1) / per_block));
+        blocks = (int)max(1ll, min((long long)most, total()));
     }
     __device__ __forceinline__ long long total() const { return (long long)batch.before[T] * items; }
-    __device__ __forceinline__ long long begin(int b) const { return total() * b / blocks; }
-    __device__ __forceinline__ int block_of(long long w) const { return (int)(((w + 1) * blocks - 1) / total()); }
-    __device__ __forceinline__ int count(int t) const { return batch.before[t + 1] - batch.before[t]; }
     struct Place { int t, item, tile, n; };          // n: tiles of the item
+    // (a division of 64 bits takes some hundred instructions)
+    __device__ __forceinline__ bool small() const { return total() < 1 << 20; }
+    __device__ __forceinline__ long long begin(int b) const { return small() ? (uint32_t)total() * b / (uint32_t)blocks : total() * b / blocks; }
+    __device__ __forceinline__ int block_of(long long w) const {
+        return small() ? (int)(((uint32_t)(w + 1) * blocks - 1) / (uint32_t)total()) : (int)(((w + 1) * blocks - 1) / total());
+    }
+    // The start of the first item that does not begin in front of tile w.
+    __device__ __forceinline__ long long whole(long long w) const {
+        if (w >= total()) return total();
+        const Place a = at(w);
+        return a.tile == 0 ? w : w - a.tile + a.n;
+    }
+    __device__ __forceinline__ int count(int t) const { return batch.before[t + 1] - batch.before[t]; }
     __device__ __forceinline__ Place at(long long w) const {
-        const int x = total() <= 0x7fffffff ? (int)w / items : (int)(w / items);
+        const int x = small() ? (int)((uint32_t)w / (uint32_t)items) : (int)(w / items);
         int lo = 0, hi = T;                          // the last token with before <= x (tokens without tiles lie in front of it)
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
@@ -157,7 +172,7 @@ __device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 6
 // grid: blocks of the device, block 160
 template <int D, int NG>
 __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                                                                               Kv8DecodeParams p, int box, int per_block, bool by_item) {
+                                                                               Kv8DecodeParams p, int box, Parts parts) {
     using M = Cfg<D, NG>;
     constexpr int KT = M::KT, MT = M::MT;
     extern __shared__ uint8_t smem_raw[];
@@ -174,73 +189,96 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
             tc::mbar_init(q_free + i, WARPS);
         }
         tc::mbar_fence_init();
+        tc::tma_prefetch_desc(&map_k);
+        tc::tma_prefetch_desc(&map_v);
     }
     pdl_grid_sync();
     const int group = p.n_heads / p.n_kv, hg = (group + M::HG - 1) / M::HG;
-    const Tiles<KT> tiles(*reinterpret_cast<Batch*>(smem + M::BATCH), p, p.n_kv * hg, gridDim.x, per_block);
+    const Tiles<KT> tiles(*reinterpret_cast<Batch*>(smem + M::BATCH), p, p.n_kv * hg, gridDim.x);
+    const bool by_item = parts == Parts::BY_ITEM, by_block = parts == Parts::BY_BLOCK;
     for (int t = blockIdx.x; t < p.T; t += gridDim.x)
         if (tiles.count(t) == 0) {
             for (int i = tid; i < p.n_heads * p.hd / 2; i += THREADS) reinterpret_cast<uint32_t*>(p.out + (size_t)t * p.n_heads * p.hd)[i] = 0u;
             if (by_item)
                 for (int i = tid; i < tiles.items; i += THREADS) p.jobs[t * tiles.items + i] = make_int4(0, 0, 0, 0);
         }
-    if (!by_item && tid == 0) p.jobs[blockIdx.x] = make_int4(0, 0, 0, 0);
+    if (by_block && tid == 0) p.jobs[blockIdx.x] = make_int4(0, 0, 0, 0);
     if (blockIdx.x >= tiles.blocks) return;
-    const long long w0 = tiles.begin(blockIdx.x), w1 = tiles.begin(blockIdx.x + 1);
+    long long w0 = tiles.begin(blockIdx.x), w1 = tiles.begin(blockIdx.x + 1);
+    if (parts == Parts::NONE) {
+        w0 = tiles.whole(w0);
+        w1 = tiles.whole(w1);
+    }
     if (w0 >= w1) return;
 
     if (warp == WARPS) {
-        // ---- fetching: a lane looks up the place of one box of a tile ahead ----
+        // ---- fetching: a lane looks up one box of a tile ahead, and sends for it when the tile's turn comes ----
         const int subs = KT / box, batch = 32 / subs;
-        struct Ahead { int row, t, item; bool first; };          // slot of a box (-1: a page that is not there, -2: nothing to fetch); a history's first tile
-        auto look = [&](long long w) -> Ahead {
-            if (w >= w1) return {-2, 0, 0, false};
+        struct Ahead {
+            int page, key, head;                                 // entry of the page table, first key of the box (-1: nothing to fetch), key head
+            const bf16* q;                                       // of a history's first tile: its queries, or null
+            uint32_t q_bytes;
+        };
+        auto look = [&](long long w) -> Ahead {                  // (the entry is not looked at here: it is on its way)
+            Ahead a{-1, -1, 0, nullptr, 0u};
+            if (w >= w1) return a;
             const typename Tiles<KT>::Place at = tiles.at(w);
             const int key = at.tile * KT + lane % subs * box, n = at.n * KT - (KT - 1) + tiles.batch.last[at.t];
-            return {key < n ? kv8_slot(p.pages, 32, tiles.batch.row[at.t], key) : -2, at.t, at.item, w == w0 || at.tile == 0};
+            const int r_lo = hg == 1 ? 0 : at.item % hg * M::HG, b = tiles.batch.row[at.t], page = key / p.pages.page_size;
+            a.head = hg == 1 ? at.item : at.item / hg;
+            if (lane % subs == 0 && (w == w0 || at.tile == 0)) {
+                a.q = p.q + ((size_t)at.t * p.n_heads + a.head * group + r_lo) * p.hd;
+                a.q_bytes = (uint32_t)(min(M::HG, group - r_lo) * p.hd * 2);
+            }
+            if (key >= n) return a;
+            a.key = key;
+            if (guard_ok(p.pages.guard, 32, b, p.pages.pt_rows) && guard_ok(p.pages.guard, 32, page, p.pages.pt_width))
+                a.page = p.pages.page_table[(size_t)b * p.pages.pt_stride + page];
+            return a;
         };
-        int issued = 0, asked = 0;                               // tiles, histories
+        int issued = 0, asked = 0, st = 0;                       // tiles, histories, stage
         bool ok = true;
         Ahead now, then = look(w0 + lane / subs);
         for (long long w = w0; w < w1 && ok; w += batch) {
             now = then;
-            const int n = (int)min((long long)batch, w1 - w);
+            const int n = (int)min((long long)batch, w1 - w), off = now.key % p.pages.page_size;
+            const uint32_t firsts = __ballot_sync(0xffffffffu, now.q != nullptr), boxes = __ballot_sync(0xffffffffu, now.key >= 0);
+            // a page that is not there is recorded; rows in front of the tensor read as zeros
+            const bool there = now.key >= 0 && guard_ok(p.pages.guard, 32, (long long)now.page * p.pages.page_size, p.pages.num_slots);
+            const int row = there ? now.page * p.pages.page_size + off : -KT;
+            const uint8_t* from = p.exps + (((size_t)(there ? now.page : 0) * p.n_kv + now.head) * 2) * p.pages.page_size + off;
             for (int i = 0; i < n; ++i, ++issued) {
-                if (i == min(n - 1, M::STAGES)) then = look(w + batch + lane / subs);      // (a microsecond; the ring is full)
-                const int st = issued % M::STAGES, item = __shfl_sync(0xffffffffu, now.item, i * subs), h = item / hg;
-                if (__shfl_sync(0xffffffffu, (int)now.first, i * subs)) {
-                    const int qb = asked & 1, t = __shfl_sync(0xffffffffu, now.t, i * subs), r_lo = item % hg * M::HG;
+                if (i == min(n - 1, M::STAGES)) then = look(w + batch + lane / subs);
+                const int at = i * subs;
+                if (firsts >> at & 1) {
+                    const int qb = asked & 1;
                     if (asked >= 2 && !tc::mbar_wait_warp(q_free + qb, (uint32_t)((asked >> 1) + 1) & 1)) { ok = false; break; }
-                    if (lane == 0) {
-                        const uint32_t bytes = min(M::HG, group - r_lo) * p.hd * 2;
-                        tc::mbar_expect_tx(q_full + qb, bytes);
-                        tc::bulk_load_1d(smem + M::Q + qb * M::Q_BYTES, p.q + ((size_t)t * p.n_heads + h * group + r_lo) * p.hd, bytes, q_full + qb);
+                    if (lane == at) {
+                        tc::mbar_expect_tx(q_full + qb, now.q_bytes);
+                        tc::bulk_load_1d(smem + M::Q + qb * M::Q_BYTES, now.q, now.q_bytes, q_full + qb);
                     }
                     ++asked;
                 }
                 if (issued >= M::STAGES && !tc::mbar_wait_warp(free_ + st, (uint32_t)(issued / M::STAGES + 1) & 1)) { ok = false; break; }
-                const uint32_t there = __ballot_sync(0xffffffffu, now.row > -2 && lane / subs == i);
-                if (lane == 0) tc::mbar_expect_tx(full + st, __popc(there) * box * (2 * D + 2));
-                uint8_t* codes = smem + st * M::STAGE;
-                uint8_t* exps = smem + M::EXPS + st * 2 * KT;
-                for (int u = 0; u < subs; ++u) {
-                    const int r = __shfl_sync(0xffffffffu, now.row, i * subs + u);
-                    if (r > -2 && lane == 0) {
+                if (lane == at) tc::mbar_expect_tx(full + st, __popc(boxes >> at & ((1u << subs) - 1)) * box * (2 * D + 2));
+                __syncwarp();
+                if ((uint32_t)(lane - at) < (uint32_t)subs && now.key >= 0) {
+                    const int u = lane - at;
+                    uint8_t *codes = smem + st * M::STAGE + u * box * M::ROW, *exps = smem + M::EXPS + st * 2 * KT;
 #pragma unroll
-                        for (int x = 0; x < M::HALVES; ++x) {    // (a page that is not there: rows in front of the tensor read as zeros)
-                            tc::tma_load_3d(codes + x * KT * M::ROW + u * box * M::ROW, &map_k, full + st, x * 128, h, r < 0 ? -KT : r);
-                            tc::tma_load_3d(codes + M::CODES + x * KT * M::ROW + u * box * M::ROW, &map_v, full + st, x * 128, h, r < 0 ? -KT : r);
-                        }
-                        const uint8_t* e = p.exps + kv8_exp_at(p.pages, p.n_kv, max(r, 0), h);
-                        if (box == KT && p.pages.page_size == KT) {          // the bytes of keys and values are neighbours
-                            tc::bulk_load_1d(exps, e, 2 * KT, full + st);
-                        } else {
-                            tc::bulk_load_1d(exps + u * box, e, box, full + st);
-                            tc::bulk_load_1d(exps + KT + u * box, e + p.pages.page_size, box, full + st);
-                        }
+                    for (int x = 0; x < M::HALVES; ++x) {
+                        tc::tma_load_3d(codes + x * KT * M::ROW, &map_k, full + st, x * 128, now.head, row);
+                        tc::tma_load_3d(codes + M::CODES + x * KT * M::ROW, &map_v, full + st, x * 128, now.head, row);
+                    }
+                    if (box == KT && p.pages.page_size == KT) {              // the bytes of keys and values are neighbours
+                        tc::bulk_load_1d(exps, from, 2 * KT, full + st);
+                    } else {
+                        tc::bulk_load_1d(exps + u * box, from, box, full + st);
+                        tc::bulk_load_1d(exps + KT + u * box, from + p.pages.page_size, box, full + st);
                     }
                 }
                 __syncwarp();
+                if (++st == M::STAGES) st = 0;
             }
         }
         // nothing is in flight when the block ends, also where a wait ran out
@@ -324,8 +362,16 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
             if (++turn == M::TURNS) turn = 0;
             const uint8_t *kt = smem + stage * M::STAGE, *vt = kt + M::CODES, *exps = smem + M::EXPS + stage * 2 * KT + k0;
             const int nk = mine ? keys - j * KT - k0 : 0;            // of this warp's 32
-            auto tile = [&](auto all_seen) {
-                constexpr bool WHOLE = decltype(all_seen)::value;
+            if (nk > 0 && nk < 32) {                                 // rows behind the history may hold anything
+                for (int i = lane; i < (32 - nk) * (D / 16); i += 32) {
+                    const int r = k0 + nk + i / (D / 16), x = i % (D / 16);
+                    uint8_t* at16 = smem + stage * M::STAGE + (x * 16 / M::ROW) * KT * M::ROW + r * M::ROW + x * 16 % M::ROW;
+                    *reinterpret_cast<uint4*>(at16) = *reinterpret_cast<uint4*>(at16 + M::CODES) = make_uint4(0u, 0u, 0u, 0u);
+                }
+                tc::fence_proxy_async_smem();                        // (the next copy into these rows comes behind)
+                __syncwarp();
+            }
+            if (nk > 0) {
                 float s[NG][2][4];                                   // keys g and g + 8 of 16, heads 2 c4 and 2 c4 + 1
 #pragma unroll
                 for (int n = 0; n < NG; ++n)
@@ -351,10 +397,10 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
                 float kf[4], ev[4], back[4];
 #pragma unroll
                 for (int u = 0; u < 4; ++u) {
-                    uint32_t eb = exps[g + u * 8], vb = exps[KT + g + u * 8];
-                    if (!WHOLE && g + u * 8 >= nk) eb = vb = KV8_BIAS;
+                    const bool seen = g + u * 8 < nk;
+                    const uint32_t eb = seen ? exps[g + u * 8] : KV8_BIAS, vb = seen ? exps[KT + g + u * 8] : KV8_BIAS;
                     kf[u] = __uint_as_float(eb << 23);
-                    ev[u] = __uint_as_float(0x4b000000u | vb) - (8388608.f + KV8_BIAS);
+                    ev[u] = seen ? __uint_as_float(0x4b000000u | vb) - (8388608.f + KV8_BIAS) : -INFINITY;
                     back[u] = __uint_as_float((2 * KV8_BIAS - vb) << 23);
                 }
                 uint32_t pw[NG][4];                                  // weights times scales: head g, keys 2 c4 and 2 c4 + 1 of every 8
@@ -364,10 +410,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
 #pragma unroll
                     for (int u = 0; u < 4; ++u)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) {
-                            x[u][h] = fmaf(s[n][u >> 1][(u & 1) * 2 + h] * kf[u], qf[n][h], ev[u] - m[n][h]);
-                            if (!WHOLE && g + u * 8 >= nk) x[u][h] = -INFINITY;
-                        }
+                        for (int h = 0; h < 2; ++h) x[u][h] = fmaf(s[n][u >> 1][(u & 1) * 2 + h] * kf[u], qf[n][h], ev[u] - m[n][h]);
                     float top[2];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) top[h] = fmaxf(fmaxf(x[0][h], x[1][h]), fmaxf(x[2][h], x[3][h]));
@@ -393,7 +436,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
                         pw[n][u] = transposed8x8(f2_to_f16x2(e0, e1));
                     }
                 }
-                // a lane's dims of keys 2 c4, 2 c4 + 1 and 8 on, of each 16 (values of keys that are not seen may be anything: they count as 0)
+                // a lane's dims of keys 2 c4, 2 c4 + 1 and 8 on, of each 16
 #pragma unroll
                 for (int x = 0; x < M::HALVES; ++x)
 #pragma unroll
@@ -408,11 +451,6 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
                                 *reinterpret_cast<uint4*>(v[u]) =
                                     *reinterpret_cast<const uint4*>(vt + x * KT * 128 + (k0 + r) * 128 + ((g ^ (2 * c4 + (u & 1))) << 4));
                             }
-                            if (!WHOLE) {
-#pragma unroll
-                                for (int i = 0; i < M::CHUNK / 4; ++i)
-                                    if (r >= nk) v[u][i] = 0u;
-                            }
                         }
 #pragma unroll
                         for (int i = 0; i < M::CHUNK / 4; ++i)
@@ -425,9 +463,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
                                 for (int n = 0; n < NG; ++n) mma_f16_16816(acc[n][x * 8 + i * 2 + u], a, pw[n][y * 2], pw[n][y * 2 + 1]);
                             }
                     }
-            };
-            if (nk >= 32) tile(std::true_type{});
-            else if (nk > 0) tile(std::false_type{});
+            }
             fresh &= nk <= 0;
 
             __syncwarp();
@@ -492,9 +528,9 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
             const bool whole = count == at.n;
             const size_t part = (size_t)blockIdx.x * 2 + (at.tile == 0 ? 1 : 0);
             if (at.tile == 0 && lane == 0) {
-                const int parts = whole ? 1 : tiles.block_of(w + at.n - 1) - (int)blockIdx.x + 1;
-                if (by_item) p.jobs[t * tiles.items + at.item] = make_int4(t * tiles.items + at.item, blockIdx.x, parts, 0);
-                else if (!whole) p.jobs[blockIdx.x] = make_int4(t * tiles.items + at.item, blockIdx.x, parts, 0);
+                const int n = whole ? 1 : tiles.block_of(w + at.n - 1) - (int)blockIdx.x + 1;
+                if (by_item) p.jobs[t * tiles.items + at.item] = make_int4(t * tiles.items + at.item, blockIdx.x, n, 0);
+                else if (by_block && !whole) p.jobs[blockIdx.x] = make_int4(t * tiles.items + at.item, blockIdx.x, n, 0);
             }
 #pragma unroll
             for (int n = 0; n < NG; ++n)
@@ -611,13 +647,15 @@ int map_codes(CUtensorMap* map, const void* codes, const Kv8DecodeParams* p, int
 struct Shape { int width, tiles; };
 Shape shape_of(int n_heads, int n_kv, int hd) { return {hd <= 64 ? 64 : hd <= 128 ? 128 : 256, hd <= 128 && n_heads / n_kv > 8 ? 2 : 1}; }
 
+constexpr int WHOLE = 512;
+
 template <int D, int NG>
-int launch(const Kv8DecodeParams* all, int T, int blocks, cudaStream_t s) {
+int launch(const Kv8DecodeParams* all, int T, int blocks, int longest, cudaStream_t s) {
     using M = Cfg<D, NG>;
     constexpr int smem = M::TOTAL + 1024;
     static_assert(M::PER_SM * (smem + 1024) <= 228 * 1024, "blocks per SM");
     static SmemOptIn opt_in;
-    const int page = all->pages.page_size, box = page % M::KT == 0 ? M::KT : page % 32 == 0 ? 32 : 16, per_block = 1;
+    const int page = all->pages.page_size, box = page % M::KT == 0 ? M::KT : page % 32 == 0 ? 32 : 16;
     CUtensorMap mk, mv;
     int rc = map_codes(&mk, all->k_codes, all, D, box);
     if (rc == 0) rc = map_codes(&mv, all->v_codes, all, D, box);
@@ -631,12 +669,13 @@ int launch(const Kv8DecodeParams* all, int T, int blocks, cudaStream_t s) {
         p.out += t * row;
         p.positions += t;
         p.batch_idx += t;
-        // few histories have many parts each: a block a query head; many have few: a block for the one that a share's end cuts
+        // histories of up to WHOLE tokens are not cut; else, few histories have many parts each: a block a query head; many have few: a block for the one
+        // that a share's end cuts
         const int group = p.n_heads / p.n_kv, items = p.T * p.n_kv * ((group + M::HG - 1) / M::HG);
-        const bool by_item = items <= blocks;
-        sl_launch(kv8_decode_kernel<D, NG>, blocks, THREADS, smem, s, mk, mv, p, box, per_block, by_item);
-        if (by_item) sl_launch(kv8_merge_kernel<D, M::HG, 1>, dim3(items, M::HG < group ? M::HG : group), 512, 0, s, p);
-        else sl_launch(kv8_merge_kernel<D, M::HG, M::HG>, blocks, 512, 0, s, p);
+        const Parts parts = longest > 0 && longest <= WHOLE ? Parts::NONE : items <= blocks ? Parts::BY_ITEM : Parts::BY_BLOCK;
+        sl_launch(kv8_decode_kernel<D, NG>, blocks, THREADS, smem, s, mk, mv, p, box, parts);
+        if (parts == Parts::BY_ITEM) sl_launch(kv8_merge_kernel<D, M::HG, 1>, dim3(items, M::HG < group ? M::HG : group), 512, 0, s, p);
+        else if (parts == Parts::BY_BLOCK) sl_launch(kv8_merge_kernel<D, M::HG, M::HG>, blocks, 512, 0, s, p);
         rc = SL_LAUNCH_CHECK();
         if (rc != 0) return rc;
     }
@@ -659,14 +698,14 @@ SL_API int sl_kv8_decode_plan(int n_heads, int n_kv, int hd, int* blocks, int* r
     return 0;
 }
 
-// out = attention of T tokens; `blocks`: of sl_kv8_decode_plan.
-SL_API int sl_kv8_decode(const Kv8DecodeParams* p, int T, int blocks, cudaStream_t s) {
+// out = attention of T tokens; `blocks`: of sl_kv8_decode_plan; `longest`: keys of the longest history, if known (a wrong one costs time only).
+SL_API int sl_kv8_decode(const Kv8DecodeParams* p, int T, int blocks, int longest, cudaStream_t s) {
     if (T == 0) return 0;
     if (p->hd < 16 || p->hd > 256 || p->hd % 16 != 0 || p->n_kv < 1 || p->n_heads % p->n_kv != 0 || blocks < 1) return -1;
     if (p->pages.page_size < 16 || p->pages.page_size % 16 != 0 || p->o_part == nullptr || p->lse_part == nullptr || p->jobs == nullptr) return -1;
     if ((((uintptr_t)p->q | (uintptr_t)p->k_codes | (uintptr_t)p->v_codes | (uintptr_t)p->exps | (uintptr_t)p->out | (uintptr_t)p->o_part | (uintptr_t)p->jobs) & 15) != 0) return -1;
     const Shape sh = shape_of(p->n_heads, p->n_kv, p->hd);
-    if (sh.width == 64) return sh.tiles == 2 ? launch<64, 2>(p, T, blocks, s) : launch<64, 1>(p, T, blocks, s);
-    if (sh.width == 128) return sh.tiles == 2 ? launch<128, 2>(p, T, blocks, s) : launch<128, 1>(p, T, blocks, s);
-    return launch<256, 1>(p, T, blocks, s);
+    if (sh.width == 64) return sh.tiles == 2 ? launch<64, 2>(p, T, blocks, longest, s) : launch<64, 1>(p, T, blocks, longest, s);
+    if (sh.width == 128) return sh.tiles == 2 ? launch<128, 2>(p, T, blocks, longest, s) : launch<128, 1>(p, T, blocks, longest, s);
+    return launch<256, 1>(p, T, blocks, longest, s);
 }

@@ -252,7 +252,7 @@ def kv8_attention(q, cache: Kv8Cache, positions, batch_idx, page_table, sm_scale
         p = Kv8DecodeParams(q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.exps.data_ptr(), positions.data_ptr(), batch_idx.data_ptr(),
                             _pages(cache, page_table), n_heads, n_kv, hd, sm_scale, out.data_ptr(), sums,
                             sums + blocks * 2 * rows * wide * 4, part.data_ptr(), 0, tcgen05.error_flag(q.device).data_ptr())
-        _call(q, "sl_kv8_decode", C.byref(p), T, blocks)
+        _call(q, "sl_kv8_decode", C.byref(p), T, blocks, max_kv_len)
         return out
     if hd not in (64, 128):
         raise ValueError(f"heads of {hd} values: attention of prompts takes 64 or 128")

@@ -48,6 +48,14 @@ def test_decoding_of_other_pages(page):
     decode([1, 15, 16, 17, 48, 49, 500, 1030], 8, 2, 128, page=page)
 
 
+@pytest.mark.parametrize("longest", [0, 1, 512, 100000])
+def test_decoding_with_any_hint(longest):
+    """The longest history is told for speed only: one that is wrong changes nothing but roundings."""
+    cache, table, q, pos, idx, got = decode([700, 65, 1, 5000], 8, 2, 128)
+    again = K8.kv8_attention(q, cache, pos, idx, table, 128 ** -0.5, max_kv_len=longest)
+    assert torch.allclose(again.float(), got.float(), rtol=2 ** -7, atol=2 ** -12)
+
+
 def test_decoding_of_many_rows():
     """More rows than one launch takes."""
     decode([1 + i % 70 for i in range(1500)], 4, 2, 64)
