@@ -2,8 +2,9 @@
 // flight and few instructions a byte.
 //
 // All histories are cut into tiles of 64 or 32 keys of one key head (and of up to 8 or 16 of its query heads); the tiles of the whole batch, one
-// history behind the other, are dealt out to the blocks in equal shares, so that a batch of ragged histories, one long history and many short ones
-// fill the device alike.  A history that lies in several shares leaves a partial result in each, which kv8_merge_kernel joins.
+// history behind the other, are dealt out in equal shares to the blocks of a head, so that a batch of ragged histories, one long history and many
+// short ones fill the device alike.  Neighbouring blocks take the heads of one share: their rows are neighbours in memory, and are read at
+// about the same time.  A history that lies in several shares leaves a partial result in each, which kv8_merge_kernel joins.
 //
 // kv8_decode_kernel: a fetching warp brings tiles (TMA, swizzled) and their exponent bytes through a ring of stages, also across the ends of
 // histories; two pairs of warps (heads of more than 128 values: four warps) take tiles in turn, a warp 32
@@ -30,8 +31,8 @@ struct Kv8DecodeParams {
     int n_heads, n_kv, hd;
     float scale;
     bf16* out;                           // [T, n_heads, hd]
-    float *o_part, *lse_part;            // [blocks, 2, rows, width], [blocks, 2, rows]
-    int4* jobs;                          // [blocks] what kv8_merge_kernel joins: history (token x items + item), first block, parts, -
+    float *o_part, *lse_part;            // [blocks x passes, 2, rows, width], [blocks x passes, 2, rows]
+    int4* jobs;                          // [blocks x passes] what kv8_merge_kernel joins: token, item, parts, place of the first one
     int T;
     int* err;                            // error word of bounded waits
 };
@@ -77,22 +78,25 @@ struct Batch {
     uint8_t last[MAX_T];                 // keys of the last tile - 1
 };
 
-// The batch's tiles of KT keys, numbered token by token, key head (and group of query heads) by key head, tile by tile.
+// How the blocks of a launch are dealt out: items (key heads x groups of query heads) i, i + abreast, ... belong to every abreast-th block, and
+// the blocks of one item share the tiles of the batch.
+struct Deal { int items, abreast, passes; };         // passes: items of a block at most
+
+// The batch's tiles of KT keys of one item, numbered token by token.
 template <int KT>
 struct Tiles {
     const Batch& batch;
-    int T, items;                        // key heads x groups of query heads
-    int blocks;                          // that get a share
+    int T, shares;                       // tokens; shares that the tiles are cut into
 
     // Tiles of token t.
     __device__ __forceinline__ static int note(const Kv8DecodeParams& p, Batch& b, int t) {
         const int pos = p.positions[t];
         b.last[t] = (uint8_t)(pos & (KT - 1));
         b.row[t] = p.batch_idx[t];
-        return pos < 0 ? 0 : pos / KT + 1;
+        return pos < 0 || !guard_ok(p.pages.guard, 32, pos / p.pages.page_size, p.pages.pt_width) ? 0 : pos / KT + 1;
     }
     // All threads of the block.
-    __device__ __forceinline__ Tiles(Batch& b, const Kv8DecodeParams& p, int items_, int most) : batch(b), T(p.T), items(items_) {
+    __device__ __forceinline__ Tiles(Batch& b, const Kv8DecodeParams& p, int most) : batch(b), T(p.T) {
         if (T > 32) {
             for (int t = threadIdx.x; t < T; t += blockDim.x) b.before[t + 1] = note(p, b, t);
             __syncthreads();
@@ -113,39 +117,36 @@ struct Tiles {
             if (threadIdx.x == 0) b.before[0] = 0;
         }
         __syncthreads();
-        blocks = (int)max(1ll, min((long long)most, total()));
+        shares = max(1, min(most, total()));
     }
-    __device__ __forceinline__ long long total() const { return (long long)batch.before[T] * items; }
-    struct Place { int t, item, tile, n; };          // n: tiles of the item
+    __device__ __forceinline__ int total() const { return batch.before[T]; }
+    __device__ __forceinline__ int count(int t) const { return batch.before[t + 1] - batch.before[t]; }
     // (a division of 64 bits takes some hundred instructions)
-    __device__ __forceinline__ bool small() const { return total() < 1 << 20; }
-    __device__ __forceinline__ long long begin(int b) const { return small() ? (uint32_t)total() * b / (uint32_t)blocks : total() * b / blocks; }
-    __device__ __forceinline__ int block_of(long long w) const {
-        return small() ? (int)(((uint32_t)(w + 1) * blocks - 1) / (uint32_t)total()) : (int)(((w + 1) * blocks - 1) / total());
+    __device__ __forceinline__ int begin(int j) const {
+        return total() < 1 << 20 ? (int)((uint32_t)total() * j / (uint32_t)shares) : (int)((long long)total() * j / shares);
     }
-    // The start of the first item that does not begin in front of tile w.
-    __device__ __forceinline__ long long whole(long long w) const {
+    __device__ __forceinline__ int share_of(int w) const {
+        return total() < 1 << 20 ? (int)((uint32_t)((w + 1) * shares - 1) / (uint32_t)total()) : (int)(((w + 1ll) * shares - 1) / total());
+    }
+    struct Place { int t, tile, n; };                // n: tiles of the token
+    __device__ __forceinline__ Place at(int w) const {
+        int lo = 0, hi = T;                          // the last token with before <= w (tokens without tiles lie in front of it)
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if (batch.before[mid] <= w) lo = mid;
+            else hi = mid;
+        }
+        return {lo, w - batch.before[lo], count(lo)};
+    }
+    // The start of the first token that does not begin in front of tile w.
+    __device__ __forceinline__ int whole(int w) const {
         if (w >= total()) return total();
         const Place a = at(w);
         return a.tile == 0 ? w : w - a.tile + a.n;
     }
-    __device__ __forceinline__ int count(int t) const { return batch.before[t + 1] - batch.before[t]; }
-    __device__ __forceinline__ Place at(long long w) const {
-        const int x = small() ? (int)((uint32_t)w / (uint32_t)items) : (int)(w / items);
-        int lo = 0, hi = T;                          // the last token with before <= x (tokens without tiles lie in front of it)
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) >> 1;
-            if (batch.before[mid] <= x) lo = mid;
-            else hi = mid;
-        }
-        const int n = count(lo), off = (int)(w - (long long)batch.before[lo] * items);
-        return {lo, off / n, off % n, n};
-    }
-    // The first tile of the next item (there is one).
+    // The first tile of the next token (there is one).
     __device__ __forceinline__ void next(Place& a) const {
         a.tile = 0;
-        if (++a.item < items) return;
-        a.item = 0;
         do { ++a.t; } while (count(a.t) == 0);
         a.n = count(a.t);
     }
@@ -172,7 +173,7 @@ __device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 6
 // grid: blocks of the device, block 160
 template <int D, int NG>
 __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                                                                               Kv8DecodeParams p, int box, Parts parts) {
+                                                                               Kv8DecodeParams p, Deal deal, int box, Parts parts) {
     using M = Cfg<D, NG>;
     constexpr int KT = M::KT, MT = M::MT;
     extern __shared__ uint8_t smem_raw[];
@@ -194,22 +195,25 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
     }
     pdl_grid_sync();
     const int group = p.n_heads / p.n_kv, hg = (group + M::HG - 1) / M::HG;
-    const Tiles<KT> tiles(*reinterpret_cast<Batch*>(smem + M::BATCH), p, p.n_kv * hg, gridDim.x);
+    const Tiles<KT> tiles(*reinterpret_cast<Batch*>(smem + M::BATCH), p, gridDim.x / deal.abreast);
     const bool by_item = parts == Parts::BY_ITEM, by_block = parts == Parts::BY_BLOCK;
     for (int t = blockIdx.x; t < p.T; t += gridDim.x)
         if (tiles.count(t) == 0) {
             for (int i = tid; i < p.n_heads * p.hd / 2; i += THREADS) reinterpret_cast<uint32_t*>(p.out + (size_t)t * p.n_heads * p.hd)[i] = 0u;
             if (by_item)
-                for (int i = tid; i < tiles.items; i += THREADS) p.jobs[t * tiles.items + i] = make_int4(0, 0, 0, 0);
+                for (int i = tid; i < deal.items; i += THREADS) p.jobs[t * deal.items + i] = make_int4(0, 0, 0, 0);
         }
-    if (by_block && tid == 0) p.jobs[blockIdx.x] = make_int4(0, 0, 0, 0);
-    if (blockIdx.x >= tiles.blocks) return;
-    long long w0 = tiles.begin(blockIdx.x), w1 = tiles.begin(blockIdx.x + 1);
+    if (by_block && tid < deal.passes) p.jobs[blockIdx.x * deal.passes + tid] = make_int4(0, 0, 0, 0);
+    const int share = blockIdx.x / deal.abreast, first_item = blockIdx.x % deal.abreast, passes = (deal.items - first_item + deal.abreast - 1) / deal.abreast;
+    if (share >= tiles.shares) return;
+    int s0 = tiles.begin(share), s1 = tiles.begin(share + 1);
     if (parts == Parts::NONE) {
-        w0 = tiles.whole(w0);
-        w1 = tiles.whole(w1);
+        s0 = tiles.whole(s0);
+        s1 = tiles.whole(s1);
     }
-    if (w0 >= w1) return;
+    const int len = s1 - s0;
+    if (len <= 0) return;
+    const long long w1 = (long long)len * passes;                // this block's tiles, item by item
 
     if (warp == WARPS) {
         // ---- fetching: a lane looks up one box of a tile ahead, and sends for it when the tile's turn comes ----
@@ -222,11 +226,12 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
         auto look = [&](long long w) -> Ahead {                  // (the entry is not looked at here: it is on its way)
             Ahead a{-1, -1, 0, nullptr, 0u};
             if (w >= w1) return a;
-            const typename Tiles<KT>::Place at = tiles.at(w);
+            const int pass = passes == 1 ? 0 : (int)(w / len), s = s0 + (int)(w - (long long)pass * len), item = first_item + pass * deal.abreast;
+            const typename Tiles<KT>::Place at = tiles.at(s);
             const int key = at.tile * KT + lane % subs * box, n = at.n * KT - (KT - 1) + tiles.batch.last[at.t];
-            const int r_lo = hg == 1 ? 0 : at.item % hg * M::HG, b = tiles.batch.row[at.t], page = key / p.pages.page_size;
-            a.head = hg == 1 ? at.item : at.item / hg;
-            if (lane % subs == 0 && (w == w0 || at.tile == 0)) {
+            const int r_lo = hg == 1 ? 0 : item % hg * M::HG, b = tiles.batch.row[at.t], page = key / p.pages.page_size;
+            a.head = hg == 1 ? item : item / hg;
+            if (lane % subs == 0 && (s == s0 || at.tile == 0)) {
                 a.q = p.q + ((size_t)at.t * p.n_heads + a.head * group + r_lo) * p.hd;
                 a.q_bytes = (uint32_t)(min(M::HG, group - r_lo) * p.hd * 2);
             }
@@ -238,8 +243,8 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
         };
         int issued = 0, asked = 0, st = 0;                       // tiles, histories, stage
         bool ok = true;
-        Ahead now, then = look(w0 + lane / subs);
-        for (long long w = w0; w < w1 && ok; w += batch) {
+        Ahead now, then = look(lane / subs);
+        for (long long w = 0; w < w1 && ok; w += batch) {
             now = then;
             const int n = (int)min((long long)batch, w1 - w), off = now.key % p.pages.page_size;
             const uint32_t firsts = __ballot_sync(0xffffffffu, now.q != nullptr), boxes = __ballot_sync(0xffffffffu, now.key >= 0);
@@ -296,9 +301,10 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
     int st = 0, turn = warp / M::TEAM, done = 0;                     // 0: this team's tile; histories behind it
     uint32_t phase = 0;
     bool ok = true;
-    typename Tiles<KT>::Place at = tiles.at(w0);
-    for (long long w = w0;;) {
-        const int count = (int)min((long long)(at.n - at.tile), w1 - w), t = at.t, hkv = at.item / hg, r_lo = at.item % hg * M::HG;
+    const typename Tiles<KT>::Place begin = tiles.at(s0);
+    typename Tiles<KT>::Place at = begin;
+    for (int s = s0, pass = 0;;) {
+        const int item = first_item + pass * deal.abreast, count = min(at.n - at.tile, s1 - s), t = at.t, hkv = item / hg, r_lo = item % hg * M::HG;
         const int nr = min(M::HG, group - r_lo), h0 = hkv * group + r_lo, keys = at.n * KT - (KT - 1) + tiles.batch.last[t];
         // queries as fp16 times 2^-eq: a lane holds head g's dims of its pieces, in the order of the pieces' bytes
         uint32_t q[NG][CH * 4][2];
@@ -372,11 +378,11 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
                 __syncwarp();
             }
             if (nk > 0) {
-                float s[NG][2][4];                                   // keys g and g + 8 of 16, heads 2 c4 and 2 c4 + 1
+                float sc[NG][2][4];                                  // keys g and g + 8 of 16, heads 2 c4 and 2 c4 + 1
 #pragma unroll
                 for (int n = 0; n < NG; ++n)
 #pragma unroll
-                    for (int y = 0; y < 2; ++y) s[n][y][0] = s[n][y][1] = s[n][y][2] = s[n][y][3] = 0.f;
+                    for (int y = 0; y < 2; ++y) sc[n][y][0] = sc[n][y][1] = sc[n][y][2] = sc[n][y][3] = 0.f;
 #pragma unroll
                 for (int x = 0; x < CH; ++x)
 #pragma unroll
@@ -390,7 +396,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
                             e4m3x4_to_f16(r0[i], a[0], a[2]);
                             e4m3x4_to_f16(r1[i], a[1], a[3]);
 #pragma unroll
-                            for (int n = 0; n < NG; ++n) mma_f16_16816(s[n][y], a, q[n][x * 4 + i][0], q[n][x * 4 + i][1]);
+                            for (int n = 0; n < NG; ++n) mma_f16_16816(sc[n][y], a, q[n][x * 4 + i][0], q[n][x * 4 + i][1]);
                         }
                     }
                 // exponents of keys g, g + 8, g + 16, g + 24 (of a key that is not seen: any)
@@ -410,7 +416,7 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
 #pragma unroll
                     for (int u = 0; u < 4; ++u)
 #pragma unroll
-                        for (int h = 0; h < 2; ++h) x[u][h] = fmaf(s[n][u >> 1][(u & 1) * 2 + h] * kf[u], qf[n][h], ev[u] - m[n][h]);
+                        for (int h = 0; h < 2; ++h) x[u][h] = fmaf(sc[n][u >> 1][(u & 1) * 2 + h] * kf[u], qf[n][h], ev[u] - m[n][h]);
                     float top[2];
 #pragma unroll
                     for (int h = 0; h < 2; ++h) top[h] = fmaxf(fmaxf(x[0][h], x[1][h]), fmaxf(x[2][h], x[3][h]));
@@ -526,11 +532,11 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
             take(reinterpret_cast<const float*>(smem + M::JOIN + M::SLOT));
             pair_sync(3);
             const bool whole = count == at.n;
-            const size_t part = (size_t)blockIdx.x * 2 + (at.tile == 0 ? 1 : 0);
+            const size_t part = ((size_t)blockIdx.x * deal.passes + pass) * 2 + (at.tile == 0 ? 1 : 0);
             if (at.tile == 0 && lane == 0) {
-                const int n = whole ? 1 : tiles.block_of(w + at.n - 1) - (int)blockIdx.x + 1;
-                if (by_item) p.jobs[t * tiles.items + at.item] = make_int4(t * tiles.items + at.item, blockIdx.x, n, 0);
-                else if (by_block && !whole) p.jobs[blockIdx.x] = make_int4(t * tiles.items + at.item, blockIdx.x, n, 0);
+                const int4 job = make_int4(t, item, whole ? 1 : tiles.share_of(s + at.n - 1) - share + 1, (int)part >> 1);
+                if (by_item) p.jobs[t * deal.items + item] = job;
+                else if (by_block && !whole) p.jobs[part >> 1] = job;
             }
 #pragma unroll
             for (int n = 0; n < NG; ++n)
@@ -560,25 +566,30 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
                     }
                 }
         }
-        w += count;
-        if (w >= w1) break;
-        tiles.next(at);
+        s += count;
+        if (s < s1) {
+            tiles.next(at);
+        } else {
+            if (++pass == passes) break;
+            s = s0;
+            at = begin;
+        }
     }
     if (!ok && lane == 0) atomicExch(p.err, 51);
 }
 
-// Joins the partial results of histories that lie in several shares: the first part is its block's second partial result, the others are their
-// blocks' first.  Block (i, y): jobs[i], rows y * R .. of its query heads.  A thread has 4 neighbouring values, D / 4 threads a row and
+// Joins the partial results of histories that lie in several shares: the first part is its block's second partial result, the others are the first ones of
+// the blocks of the item behind it.  Block (i, y): jobs[i], rows y * R .. of its query heads.  A thread has 4 neighbouring values, D / 4 threads a row and
 // 512 / (D / 4) / R of the parts in turn.
 template <int D, int HG, int R>
-__global__ void __launch_bounds__(512) kv8_merge_kernel(Kv8DecodeParams p) {
+__global__ void __launch_bounds__(512) kv8_merge_kernel(Kv8DecodeParams p, Deal deal) {
     constexpr int LANES = D / 4, TURNS = 512 / LANES / R, AHEAD = 4;
     __shared__ float4 sums[512];
     __shared__ float2 state[512 / LANES];            // reference and denominator
     pdl_grid_sync();
     const int4 job = p.jobs[blockIdx.x];
     if (job.z < 2) return;
-    const int group = p.n_heads / p.n_kv, hg = (group + HG - 1) / HG, tid = threadIdx.x, t = job.x / (p.n_kv * hg), item = job.x % (p.n_kv * hg), b0 = job.y, n = job.z;
+    const int group = p.n_heads / p.n_kv, hg = (group + HG - 1) / HG, tid = threadIdx.x, t = job.x, item = job.y, n = job.z;
     const int hkv = item / hg, r_lo = item % hg * HG, part_row = tid / LANES, r = blockIdx.y * R + part_row % R, d = tid % LANES * 4;
     const bool on = r < min(HG, group - r_lo);
     float top = -INFINITY, den = 0.f;
@@ -590,7 +601,7 @@ __global__ void __launch_bounds__(512) kv8_merge_kernel(Kv8DecodeParams p) {
         for (int u = 0; u < AHEAD; ++u) {
             const int i = i0 + u * TURNS;
             const bool there = on && i < n;
-            const size_t part = ((size_t)(b0 + i) * 2 + (i == 0 ? 1 : 0)) * HG + r;
+            const size_t part = (((size_t)job.w + (size_t)i * deal.abreast * deal.passes) * 2 + (i == 0 ? 1 : 0)) * HG + r;
             lse[u] = there ? p.lse_part[part] : -INFINITY;
             v[u] = there ? *reinterpret_cast<const float4*>(p.o_part + part * D + d) : make_float4(0.f, 0.f, 0.f, 0.f);
         }
@@ -639,18 +650,27 @@ int map_codes(CUtensorMap* map, const void* codes, const Kv8DecodeParams* p, int
     cuuint64_t dims[3] = {(cuuint64_t)p->hd, (cuuint64_t)p->n_kv, (cuuint64_t)p->pages.num_slots}, strides[2] = {(cuuint64_t)p->hd, (cuuint64_t)p->n_kv * p->hd};
     cuuint32_t box[3] = {(cuuint32_t)(width < 128 ? width : 128), 1, (cuuint32_t)rows}, steps[3] = {1, 1, 1};
     return enc(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(codes), dims, strides, box, steps, CU_TENSOR_MAP_INTERLEAVE_NONE,
-               width < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, width < 128 ? CU_TENSOR_MAP_L2_PROMOTION_L2_64B : CU_TENSOR_MAP_L2_PROMOTION_L2_128B,
+               width < 128 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -102;
 }
 
-// width of the heads in the kernels, tiles of 8 query heads
-struct Shape { int width, tiles; };
-Shape shape_of(int n_heads, int n_kv, int hd) { return {hd <= 64 ? 64 : hd <= 128 ? 128 : 256, hd <= 128 && n_heads / n_kv > 8 ? 2 : 1}; }
+// width of the heads in the kernels, tiles of 8 query heads, blocks an SM
+struct Shape { int width, tiles, per_sm; };
+Shape shape_of(int n_heads, int n_kv, int hd) {
+    const int width = hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
+    return {width, hd <= 128 && n_heads / n_kv > 8 ? 2 : 1, width == 64 ? 3 : 2};
+}
+// The items that are walked abreast read neighbouring bytes at the same time, so as many as there are, up to 32 (where a few blocks would be left
+// over, at most a ninth of them): 48 histories of up to 8192, 8 key heads of 128: 75 us, one item behind the other 90.
+Deal deal_of(const Shape& sh, int n_heads, int n_kv, int blocks) {
+    const int items = n_kv * ((n_heads / n_kv + sh.tiles * 8 - 1) / (sh.tiles * 8)), passes = (items + 31) / 32, abreast = (items + passes - 1) / passes;
+    return {items, abreast < blocks ? abreast : blocks, abreast < blocks ? passes : (items + blocks - 1) / blocks};
+}
 
 constexpr int WHOLE = 512;
 
 template <int D, int NG>
-int launch(const Kv8DecodeParams* all, int T, int blocks, int longest, cudaStream_t s) {
+int launch(const Kv8DecodeParams* all, int T, int blocks, const Deal& deal, int longest, cudaStream_t s) {
     using M = Cfg<D, NG>;
     constexpr int smem = M::TOTAL + 1024;
     static_assert(M::PER_SM * (smem + 1024) <= 228 * 1024, "blocks per SM");
@@ -671,11 +691,11 @@ int launch(const Kv8DecodeParams* all, int T, int blocks, int longest, cudaStrea
         p.batch_idx += t;
         // histories of up to WHOLE tokens are not cut; else, few histories have many parts each: a block a query head; many have few: a block for the one
         // that a share's end cuts
-        const int group = p.n_heads / p.n_kv, items = p.T * p.n_kv * ((group + M::HG - 1) / M::HG);
-        const Parts parts = longest > 0 && longest <= WHOLE ? Parts::NONE : items <= blocks ? Parts::BY_ITEM : Parts::BY_BLOCK;
-        sl_launch(kv8_decode_kernel<D, NG>, blocks, THREADS, smem, s, mk, mv, p, box, parts);
-        if (parts == Parts::BY_ITEM) sl_launch(kv8_merge_kernel<D, M::HG, 1>, dim3(items, M::HG < group ? M::HG : group), 512, 0, s, p);
-        else if (parts == Parts::BY_BLOCK) sl_launch(kv8_merge_kernel<D, M::HG, M::HG>, blocks, 512, 0, s, p);
+        const int items = p.T * deal.items, rows = p.n_heads / p.n_kv < M::HG ? p.n_heads / p.n_kv : M::HG;
+        const Parts parts = longest > 0 && longest <= WHOLE ? Parts::NONE : items <= blocks * deal.passes ? Parts::BY_ITEM : Parts::BY_BLOCK;
+        sl_launch(kv8_decode_kernel<D, NG>, blocks, THREADS, smem, s, mk, mv, p, deal, box, parts);
+        if (parts == Parts::BY_ITEM) sl_launch(kv8_merge_kernel<D, M::HG, 1>, dim3(items, rows), 512, 0, s, p, deal);
+        else if (parts == Parts::BY_BLOCK) sl_launch(kv8_merge_kernel<D, M::HG, M::HG>, blocks * deal.passes, 512, 0, s, p, deal);
         rc = SL_LAUNCH_CHECK();
         if (rc != 0) return rc;
     }
@@ -684,15 +704,17 @@ int launch(const Kv8DecodeParams* all, int T, int blocks, int longest, cudaStrea
 
 }  // namespace
 
-// Blocks that attention of these sizes is dealt out to, and what a partial result takes: 2 `rows` x `width` sums, 2 `rows` references and 16 bytes a block.
-SL_API int sl_kv8_decode_plan(int n_heads, int n_kv, int hd, int* blocks, int* rows, int* width) {
-    if (hd < 16 || hd > 256 || hd % 16 != 0 || n_kv < 1 || n_heads < n_kv || n_heads % n_kv != 0) return -1;
+// Blocks that attention of these sizes is dealt out to, and what their partial results take: 2 `rows` x `width` sums, 2 `rows` references and 16 bytes for
+// each of `parts`.
+SL_API int sl_kv8_decode_plan(int n_heads, int n_kv, int hd, int* blocks, int* parts, int* rows, int* width) {
+    if (hd < 16 || hd > 256 || hd % 16 != 0 || n_kv < 1 || n_heads < n_kv || n_heads % n_kv != 0 || n_heads > 1024) return -1;
     int device = 0, sms = 0;
     cudaError_t e = cudaGetDevice(&device);
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
     if (e != cudaSuccess) return (int)e;
     const Shape sh = shape_of(n_heads, n_kv, hd);
-    *blocks = sms * (sh.width == 64 ? 3 : 2);
+    *blocks = sms * sh.per_sm;
+    *parts = *blocks * deal_of(sh, n_heads, n_kv, *blocks).passes;
     *rows = 8 * sh.tiles;
     *width = sh.width;
     return 0;
@@ -701,11 +723,13 @@ SL_API int sl_kv8_decode_plan(int n_heads, int n_kv, int hd, int* blocks, int* r
 // out = attention of T tokens; `blocks`: of sl_kv8_decode_plan; `longest`: keys of the longest history, if known (a wrong one costs time only).
 SL_API int sl_kv8_decode(const Kv8DecodeParams* p, int T, int blocks, int longest, cudaStream_t s) {
     if (T == 0) return 0;
-    if (p->hd < 16 || p->hd > 256 || p->hd % 16 != 0 || p->n_kv < 1 || p->n_heads % p->n_kv != 0 || blocks < 1) return -1;
+    if (p->hd < 16 || p->hd > 256 || p->hd % 16 != 0 || p->n_kv < 1 || p->n_heads % p->n_kv != 0 || p->n_heads > 1024 || blocks < 1) return -1;
     if (p->pages.page_size < 16 || p->pages.page_size % 16 != 0 || p->o_part == nullptr || p->lse_part == nullptr || p->jobs == nullptr) return -1;
     if ((((uintptr_t)p->q | (uintptr_t)p->k_codes | (uintptr_t)p->v_codes | (uintptr_t)p->exps | (uintptr_t)p->out | (uintptr_t)p->o_part | (uintptr_t)p->jobs) & 15) != 0) return -1;
     const Shape sh = shape_of(p->n_heads, p->n_kv, p->hd);
-    if (sh.width == 64) return sh.tiles == 2 ? launch<64, 2>(p, T, blocks, longest, s) : launch<64, 1>(p, T, blocks, longest, s);
-    if (sh.width == 128) return sh.tiles == 2 ? launch<128, 2>(p, T, blocks, longest, s) : launch<128, 1>(p, T, blocks, longest, s);
-    return launch<256, 1>(p, T, blocks, longest, s);
+    const Deal deal = deal_of(sh, p->n_heads, p->n_kv, blocks);
+    if ((long long)(p->pages.pt_width) * p->pages.page_size / 32 > 0x7fffffff / MAX_T - 1) return -1;        // tiles are counted in 32 bits
+    if (sh.width == 64) return sh.tiles == 2 ? launch<64, 2>(p, T, blocks, deal, longest, s) : launch<64, 1>(p, T, blocks, deal, longest, s);
+    if (sh.width == 128) return sh.tiles == 2 ? launch<128, 2>(p, T, blocks, deal, longest, s) : launch<128, 1>(p, T, blocks, deal, longest, s);
+    return launch<256, 1>(p, T, blocks, deal, longest, s);
 }

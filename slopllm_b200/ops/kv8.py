@@ -246,12 +246,12 @@ def kv8_attention(q, cache: Kv8Cache, positions, batch_idx, page_table, sm_scale
         return out
     if qo_indptr is None:
         from . import tcgen05
-        blocks, rows, wide = _decode_plan(q.get_device(), n_heads, n_kv, hd)
-        part = torch.empty(blocks * (2 * rows * (wide + 1) + 4), dtype=torch.float32, device=q.device)
-        sums = part.data_ptr() + blocks * 16
+        blocks, parts, rows, wide = _decode_plan(q.get_device(), n_heads, n_kv, hd)
+        part = torch.empty(parts * (2 * rows * (wide + 1) + 4), dtype=torch.float32, device=q.device)
+        sums = part.data_ptr() + parts * 16
         p = Kv8DecodeParams(q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.exps.data_ptr(), positions.data_ptr(), batch_idx.data_ptr(),
                             _pages(cache, page_table), n_heads, n_kv, hd, sm_scale, out.data_ptr(), sums,
-                            sums + blocks * 2 * rows * wide * 4, part.data_ptr(), 0, tcgen05.error_flag(q.device).data_ptr())
+                            sums + parts * 2 * rows * wide * 4, part.data_ptr(), 0, tcgen05.error_flag(q.device).data_ptr())
         _call(q, "sl_kv8_decode", C.byref(p), T, blocks, max_kv_len)
         return out
     if hd not in (64, 128):
@@ -261,13 +261,13 @@ def kv8_attention(q, cache: Kv8Cache, positions, batch_idx, page_table, sm_scale
 
 
 @lru_cache(maxsize=None)
-def _decode_plan(device: int, n_heads: int, n_kv: int, hd: int) -> Tuple[int, int, int]:
-    """(blocks, rows and width of a partial result) of the decode kernel on a device."""
+def _decode_plan(device: int, n_heads: int, n_kv: int, hd: int) -> Tuple[int, ...]:
+    """(blocks, partial results, their rows and width) of the decode kernel on a device."""
     N = _native()
-    out = (C.c_int * 3)()
+    out = (C.c_int * 4)()
     at = C.addressof(out)
     with torch.cuda.device(device):
-        N.check(N.fn("sl_kv8_decode_plan")(n_heads, n_kv, hd, at, at + 4, at + 8), "sl_kv8_decode_plan")
+        N.check(N.fn("sl_kv8_decode_plan")(n_heads, n_kv, hd, at, at + 4, at + 8, at + 12), "sl_kv8_decode_plan")
     return tuple(out)
 
 

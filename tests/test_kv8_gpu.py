@@ -29,7 +29,7 @@ def decode(histories, h, kv, hd, seed=3, page=64, scale=1.0, sizes=0.7):
 @pytest.mark.parametrize("histories,h,kv,hd,scale", [
     ([1], 16, 8, 128, 1.0), ([2, 15, 16, 17, 47, 48, 63, 64, 65], 8, 8, 128, 1.0), ([127, 128, 129, 700, 3], 32, 2, 128, 3.0), ([130] * 33, 8, 4, 64, 1.0),
     ([9000], 4, 1, 64, 1.0), ([77, 500, 1], 4, 2, 256, 2.0), ([40, 4100], 16, 1, 128, 1.0), ([1, 3000, 2], 64, 8, 128, 1.0), ([5000, 70], 16, 1, 256, 1.0),
-    ([640] * 300, 2, 2, 64, 1.0),
+    ([640] * 300, 2, 2, 64, 1.0), ([700, 30, 2000], 40, 40, 64, 1.0), ([3000, 5, 1200], 100, 50, 128, 1.0), ([900] * 30, 66, 33, 256, 1.0),
 ])
 def test_decoding(histories, h, kv, hd, scale):
     """Tile edges, one and several pieces of a history, ragged batches, 1 to 16 query heads a key head, caches of NaN outside the histories."""
