@@ -152,12 +152,15 @@ struct Tiles {
     }
 };
 
+// Spilled registers cost more than blocks bring (shared memory leaves no L1 to speak of): the sums of 16 heads of 128, or of 8 of 256, take the
+// registers of a block by itself.
+constexpr int blocks_per_sm(int width, int tiles) { return width == 64 ? (tiles == 1 ? 3 : 2) : width * tiles == 128 ? 2 : 1; }
+
 template <int D, int NG>
 struct Cfg {
     static constexpr int KT = D > 128 ? 32 : 64, TEAM = KT / 32, TURNS = WARPS / TEAM;      // keys of a tile, warps that share one, tiles at a time
     static constexpr int ROW = D < 128 ? D : 128, HALVES = D / ROW;      // bytes of a row in one box, boxes
-    static constexpr int STAGES = D == 64 ? 6 : D == 128 && NG == 1 ? 6 : 5, HG = 8 * NG;
-    static constexpr int PER_SM = D == 64 ? 3 : 2;
+    static constexpr int PER_SM = blocks_per_sm(D, NG), STAGES = PER_SM == 1 ? 10 : 6, HG = 8 * NG;
     static constexpr int CHUNK = D < 128 ? 8 : 16, MT = D / 16;          // neighbouring dims of a lane, 16-dim rows of products
     static constexpr int CODES = KT * D, STAGE = 2 * CODES;              // keys, values
     static constexpr int EXPS = STAGES * STAGE;                          // KT bytes of the keys, KT of the values
@@ -654,11 +657,11 @@ int map_codes(CUtensorMap* map, const void* codes, const Kv8DecodeParams* p, int
                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS ? 0 : -102;
 }
 
-// width of the heads in the kernels, tiles of 8 query heads, blocks an SM
-struct Shape { int width, tiles, per_sm; };
+// width of the heads in the kernels, tiles of 8 query heads
+struct Shape { int width, tiles; };
 Shape shape_of(int n_heads, int n_kv, int hd) {
     const int width = hd <= 64 ? 64 : hd <= 128 ? 128 : 256;
-    return {width, hd <= 128 && n_heads / n_kv > 8 ? 2 : 1, width == 64 ? 3 : 2};
+    return {width, hd <= 128 && n_heads / n_kv > 8 ? 2 : 1};
 }
 // The items that are walked abreast read neighbouring bytes at the same time, so as many as there are, up to 32 (where a few blocks would be left
 // over, at most a ninth of them): 48 histories of up to 8192, 8 key heads of 128: 75 us, one item behind the other 90.
@@ -713,7 +716,7 @@ SL_API int sl_kv8_decode_plan(int n_heads, int n_kv, int hd, int* blocks, int* p
     if (e == cudaSuccess) e = cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, device);
     if (e != cudaSuccess) return (int)e;
     const Shape sh = shape_of(n_heads, n_kv, hd);
-    *blocks = sms * sh.per_sm;
+    *blocks = sms * blocks_per_sm(sh.width, sh.tiles);
     *parts = *blocks * deal_of(sh, n_heads, n_kv, *blocks).passes;
     *rows = 8 * sh.tiles;
     *width = sh.width;
