@@ -7,8 +7,8 @@
 // about the same time.  A history that lies in several shares leaves a partial result in each, which kv8_merge_kernel joins.
 //
 // kv8_decode_kernel: a fetching warp brings tiles (TMA, swizzled) and their exponent bytes through a ring of stages, also across the ends of
-// histories; two pairs of warps (heads of more than 128 values: four warps) take tiles in turn, a warp 32
-// keys of one, with softmax states of their own and no barrier before a history's end.
+// histories; two or three pairs of warps (heads of more than 128 values: seven warps) take tiles in turn,
+// a warp 32 keys of one, with softmax states of their own and no barrier before a history's end.
 //
 //   S^T = K Q^T      keys are the 16-row operand: a lane's 16 bytes of two keys are four steps of the product as they lie, since any order
 //                    of the summed dims will do that the queries follow
@@ -37,7 +37,7 @@ struct Kv8DecodeParams {
     int* err;                            // error word of bounded waits
 };
 
-constexpr int WARPS = 4, THREADS = WARPS * 32 + 32, MAX_T = 256;      // MAX_T: tokens a launch
+constexpr int MAX_T = 256;                       // tokens a launch
 // Weights are 2^(score + exponent of the value's scale - reference).  A row's reference is raised to 2^TOP below the largest when one would be above
 // 2^(TOP + RAISE), which fp16 holds; fp32 weights reach down to 2^-126, so that two rows whose scales are the format's limits apart (2^120) are told
 // apart by weights down to 2^-14 of the largest.
@@ -76,6 +76,7 @@ struct Batch {
     int before[MAX_T + 1];               // tiles of one key head in front of a token
     int row[MAX_T];                      // page-table row
     uint8_t last[MAX_T];                 // keys of the last tile - 1
+    int sums[MAX_T / 32];                // of 32 tokens
 };
 
 // How the blocks of a launch are dealt out: items (key heads x groups of query heads) i, i + abreast, ... belong to every abreast-th block, and
@@ -97,25 +98,29 @@ struct Tiles {
     }
     // All threads of the block.
     __device__ __forceinline__ Tiles(Batch& b, const Kv8DecodeParams& p, int most) : batch(b), T(p.T) {
-        if (T > 32) {
-            for (int t = threadIdx.x; t < T; t += blockDim.x) b.before[t + 1] = note(p, b, t);
-            __syncthreads();
-        }
-        if (threadIdx.x < 32) {
-            int sum = 0;
-            for (int t0 = 0; t0 < T; t0 += 32) {
-                const int t = t0 + threadIdx.x;
-                int x = t >= T ? 0 : T > 32 ? b.before[t + 1] : note(p, b, t);
+        const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
+        int x[2], n = 0;                             // (at least four warps)
 #pragma unroll
-                for (int o = 1; o < 32; o <<= 1) {
-                    const int y = __shfl_up_sync(0xffffffffu, x, o);
-                    if ((int)threadIdx.x >= o) x += y;
-                }
-                if (t < T) b.before[t + 1] = sum + x;
-                sum += __shfl_sync(0xffffffffu, x, 31);
-            }
-            if (threadIdx.x == 0) b.before[0] = 0;
+        for (int u = 0; u < 2; ++u) {
+            const int t = (warp + u * warps) * 32 + lane;
+            x[u] = t < T ? note(p, b, t) : 0;
         }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int c = warp + u * warps;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, x[u], o);
+                if (lane >= o) x[u] += y;
+            }
+            if (lane == 31 && c * 32 < T) b.sums[c] = x[u];
+        }
+        if (T > 32) __syncthreads();
+        for (int i = 0, c = warp; c * 32 < T; c += warps, ++i) {
+            for (int u = i == 0 ? 0 : c - warps; u < c; ++u) n += b.sums[u];
+            if (c * 32 + lane < T) b.before[c * 32 + lane + 1] = n + (i == 0 ? x[0] : x[1]);
+        }
+        if (threadIdx.x == 0) b.before[0] = 0;
         __syncthreads();
         shares = max(1, min(most, total()));
     }
@@ -154,31 +159,31 @@ struct Tiles {
 
 // Spilled registers cost more than blocks bring (shared memory leaves no L1 to speak of): the sums of 16 heads of 128, or of 8 of 256, take the
 // registers of a block by itself.
+// Blocks an SM and warps of products; four sub-cores share the warps, and a block by itself has two on each.
 constexpr int blocks_per_sm(int width, int tiles) { return width == 64 ? (tiles == 1 ? 3 : 2) : width * tiles == 128 ? 2 : 1; }
 
 template <int D, int NG>
 struct Cfg {
+    static constexpr int PER_SM = blocks_per_sm(D, NG), WARPS = PER_SM > 1 ? 4 : D == 128 ? 6 : 7, THREADS = WARPS * 32 + 32;
     static constexpr int KT = D > 128 ? 32 : 64, TEAM = KT / 32, TURNS = WARPS / TEAM;      // keys of a tile, warps that share one, tiles at a time
     static constexpr int ROW = D < 128 ? D : 128, HALVES = D / ROW;      // bytes of a row in one box, boxes
-    static constexpr int PER_SM = blocks_per_sm(D, NG), STAGES = PER_SM == 1 ? 10 : 6, HG = 8 * NG;
+    static constexpr int STAGES = D == 64 ? 6 : D == 256 ? 9 : NG == 1 ? 5 : 10, HG = 8 * NG;
     static constexpr int CHUNK = D < 128 ? 8 : 16, MT = D / 16;          // neighbouring dims of a lane, 16-dim rows of products
     static constexpr int CODES = KT * D, STAGE = 2 * CODES;              // keys, values
     static constexpr int EXPS = STAGES * STAGE;                          // KT bytes of the keys, KT of the values
     static constexpr int Q = EXPS + STAGES * 2 * KT, Q_BYTES = HG * D * 2;         // two histories' queries
     static constexpr int JOIN = Q + 2 * Q_BYTES, SLOT = NG * MT * 4 * 32 * 4 + 2 * HG * 4;       // sums as they lie in registers, references, denominators
-    static constexpr int BATCH = JOIN + 2 * SLOT;
+    static constexpr int BATCH = JOIN + WARPS * SLOT;
     static constexpr int BARS = (BATCH + (int)sizeof(Batch) + 7) / 8 * 8;
     static constexpr int TOTAL = BARS + (2 * STAGES + 4) * 8;
 };
 
-__device__ __forceinline__ void pair_sync(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
-
-// grid: blocks of the device, block 160
+// grid: blocks of the device
 template <int D, int NG>
-__global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+__global__ void __launch_bounds__(Cfg<D, NG>::THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                                                                                Kv8DecodeParams p, Deal deal, int box, Parts parts) {
     using M = Cfg<D, NG>;
-    constexpr int KT = M::KT, MT = M::MT;
+    constexpr int KT = M::KT, MT = M::MT, WARPS = M::WARPS, THREADS = M::THREADS;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint64_t *full = reinterpret_cast<uint64_t*>(smem + M::BARS), *free_ = full + M::STAGES, *q_full = free_ + M::STAGES, *q_free = q_full + 2;
@@ -478,96 +483,70 @@ __global__ void __launch_bounds__(THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel
             __syncwarp();
             if (lane == 0) tc::mbar_arrive(free_ + stage);
         }
-        // ---- join the warps, 1 into 0, 3 into 2, 2 into 0: lanes of the same number have the same places ----
+        // ---- join the warps: sums as they lie in registers go through shared memory, a warp joins some of the columns ----
+        auto together = [] { asm volatile("bar.sync 1, %0;" ::"n"(WARPS * 32) : "memory"); };
+        float* const slots = reinterpret_cast<float*>(smem + M::JOIN);
+        constexpr int SLOT = M::SLOT / 4, STATE = NG * MT * 4 * 32;
+        together();                                                  // (what the previous history left has been read)
 #pragma unroll
-        for (int n = 0; n < NG; ++n)
+        for (int n = 0; n < NG; ++n) {
 #pragma unroll
             for (int h = 0; h < 2; ++h) {
 #pragma unroll
                 for (int o = 4; o < 32; o <<= 1) l[n][h] += __shfl_xor_sync(0xffffffffu, l[n][h], o);
-                if (fresh) m[n][h] = -INFINITY;
-            }
-        float* const slot = reinterpret_cast<float*>(smem + M::JOIN + (warp >> 1) * M::SLOT);
-        auto give = [&](float* to) {
-            float* const state = to + NG * MT * 4 * 32;
-#pragma unroll
-            for (int n = 0; n < NG; ++n) {
-#pragma unroll
-                for (int i = 0; i < MT; ++i)
-#pragma unroll
-                    for (int x = 0; x < 4; ++x) to[((n * MT + i) * 4 + x) * 32 + lane] = acc[n][i][x];
-                if (g == 0)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        state[n * 8 + c4 * 2 + h] = m[n][h];
-                        state[M::HG + n * 8 + c4 * 2 + h] = l[n][h];
-                    }
-            }
-        };
-        auto take = [&](const float* from) {
-            const float* const state = from + NG * MT * 4 * 32;
-#pragma unroll
-            for (int n = 0; n < NG; ++n)
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float mo = state[n * 8 + c4 * 2 + h], top = fmaxf(m[n][h], mo);
-                    const float f = m[n][h] == -INFINITY ? 0.f : ex2(m[n][h] - top), fo = mo == -INFINITY ? 0.f : ex2(mo - top);
-                    m[n][h] = top;
-                    l[n][h] = f * l[n][h] + fo * state[M::HG + n * 8 + c4 * 2 + h];
-#pragma unroll
-                    for (int i = 0; i < MT; ++i)
-#pragma unroll
-                        for (int x = h; x < 4; x += 2) acc[n][i][x] = f * acc[n][i][x] + fo * from[((n * MT + i) * 4 + x) * 32 + lane];
+                if (g == 0) {
+                    slots[warp * SLOT + STATE + n * 8 + c4 * 2 + h] = fresh ? -INFINITY : m[n][h];
+                    slots[warp * SLOT + STATE + M::HG + n * 8 + c4 * 2 + h] = l[n][h];
                 }
-        };
-        pair_sync(1 + (warp >> 1));                                  // (the slot's last reader is done)
-        if (warp & 1) give(slot);
-        pair_sync(1 + (warp >> 1));
-        if (warp == 2) {
-            take(slot);
-            __syncwarp();
-            give(slot);
-            pair_sync(3);
-            pair_sync(3);                                            // (warp 0 has read the slot)
-        } else if (warp == 0) {
-            take(slot);
-            pair_sync(3);
-            take(reinterpret_cast<const float*>(smem + M::JOIN + M::SLOT));
-            pair_sync(3);
-            const bool whole = count == at.n;
-            const size_t part = ((size_t)blockIdx.x * deal.passes + pass) * 2 + (at.tile == 0 ? 1 : 0);
-            if (at.tile == 0 && lane == 0) {
-                const int4 job = make_int4(t, item, whole ? 1 : tiles.share_of(s + at.n - 1) - share + 1, (int)part >> 1);
-                if (by_item) p.jobs[t * deal.items + item] = job;
-                else if (by_block && !whole) p.jobs[part >> 1] = job;
             }
 #pragma unroll
-            for (int n = 0; n < NG; ++n)
+            for (int i = 0; i < MT; ++i)
+#pragma unroll
+                for (int x = 0; x < 4; ++x) slots[warp * SLOT + ((n * MT + i) * 4 + x) * 32 + lane] = acc[n][i][x];
+        }
+        together();
+        const bool whole = count == at.n;
+        const size_t part = ((size_t)blockIdx.x * deal.passes + pass) * 2 + (at.tile == 0 ? 1 : 0);
+        if (at.tile == 0 && tid == 0) {
+            const int4 job = make_int4(t, item, whole ? 1 : tiles.share_of(s + at.n - 1) - share + 1, (int)part >> 1);
+            if (by_item) p.jobs[t * deal.items + item] = job;
+            else if (by_block && !whole) p.jobs[part >> 1] = job;
+        }
+#pragma unroll
+        for (int n = 0; n < NG; ++n) {
+            const float* const state = slots + STATE + n * 8 + c4 * 2;
+            float top[2], den[2] = {0.f, 0.f}, f[WARPS][2];
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                top[h] = state[h];
+#pragma unroll
+                for (int y = 1; y < WARPS; ++y) top[h] = fmaxf(top[h], state[y * SLOT + h]);
+#pragma unroll
+                for (int y = 0; y < WARPS; ++y) {
+                    const float mo = state[y * SLOT + h];
+                    f[y][h] = mo == -INFINITY ? 0.f : ex2(mo - top[h]);
+                    den[h] += f[y][h] * state[y * SLOT + M::HG + h];
+                }
+            }
+            const float inv[2] = {1.f / den[0], 1.f / den[1]};
+            if (!whole && warp == 0 && g == 0)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) p.lse_part[part * M::HG + n * 8 + c4 * 2 + h] = top[h] + log2f(den[h]);
+            for (int i = MT * warp / WARPS; i < MT * (warp + 1) / WARPS; ++i) {
+                float o[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int y = 0; y < WARPS; ++y)
+#pragma unroll
+                    for (int x = 0; x < 4; ++x) o[x] += f[y][x & 1] * slots[y * SLOT + ((n * MT + i) * 4 + x) * 32 + lane];
+                const int d = i / (M::CHUNK / 2) * 128 + g * M::CHUNK + i % (M::CHUNK / 2) * 2;
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int r = n * 8 + c4 * 2 + h;
                     if (r >= nr) continue;
-                    const float inv = 1.f / l[n][h];
-                    if (!whole && g == 0) p.lse_part[part * M::HG + r] = m[n][h] + log2f(l[n][h]);
-#pragma unroll
-                    for (int x = 0; x < M::HALVES; ++x) {
-                        const int d = x * 128 + g * M::CHUNK, i0 = x * 8;
-                        if (whole && d < p.hd) {
-                            uint4* dst = reinterpret_cast<uint4*>(p.out + ((size_t)t * p.n_heads + h0 + r) * p.hd + d);
-                            uint32_t o[M::CHUNK / 2];
-#pragma unroll
-                            for (int i = 0; i < M::CHUNK / 2; ++i) o[i] = f2_to_bf162(acc[n][i0 + i][h] * inv, acc[n][i0 + i][2 + h] * inv);
-#pragma unroll
-                            for (int i = 0; i < M::CHUNK / 8; ++i) dst[i] = make_uint4(o[i * 4], o[i * 4 + 1], o[i * 4 + 2], o[i * 4 + 3]);
-                        } else if (!whole) {
-                            float4* dst = reinterpret_cast<float4*>(p.o_part + (part * M::HG + r) * D + d);
-#pragma unroll
-                            for (int i = 0; i < M::CHUNK / 4; ++i)
-                                dst[i] = make_float4(acc[n][i0 + i * 2][h] * inv, acc[n][i0 + i * 2][2 + h] * inv, acc[n][i0 + i * 2 + 1][h] * inv,
-                                                     acc[n][i0 + i * 2 + 1][2 + h] * inv);
-                        }
-                    }
+                    if (!whole) *reinterpret_cast<float2*>(p.o_part + (part * M::HG + r) * D + d) = make_float2(o[h] * inv[h], o[2 + h] * inv[h]);
+                    else if (d < p.hd) *reinterpret_cast<uint32_t*>(p.out + ((size_t)t * p.n_heads + h0 + r) * p.hd + d) = f2_to_bf162(o[h] * inv[h], o[2 + h] * inv[h]);
                 }
+            }
         }
         s += count;
         if (s < s1) {
@@ -696,7 +675,7 @@ int launch(const Kv8DecodeParams* all, int T, int blocks, const Deal& deal, int 
         // that a share's end cuts
         const int items = p.T * deal.items, rows = p.n_heads / p.n_kv < M::HG ? p.n_heads / p.n_kv : M::HG;
         const Parts parts = longest > 0 && longest <= WHOLE ? Parts::NONE : items <= blocks * deal.passes ? Parts::BY_ITEM : Parts::BY_BLOCK;
-        sl_launch(kv8_decode_kernel<D, NG>, blocks, THREADS, smem, s, mk, mv, p, deal, box, parts);
+        sl_launch(kv8_decode_kernel<D, NG>, blocks, M::THREADS, smem, s, mk, mv, p, deal, box, parts);
         if (parts == Parts::BY_ITEM) sl_launch(kv8_merge_kernel<D, M::HG, 1>, dim3(items, rows), 512, 0, s, p, deal);
         else if (parts == Parts::BY_BLOCK) sl_launch(kv8_merge_kernel<D, M::HG, M::HG>, blocks * deal.passes, 512, 0, s, p, deal);
         rc = SL_LAUNCH_CHECK();
