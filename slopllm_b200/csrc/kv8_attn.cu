@@ -1,14 +1,13 @@
 // Attention of one new token per sequence over the 8-bit key/value cache (kv8.cuh): every cached byte is read once, so what counts is bytes in
 // flight and few instructions a byte.
 //
-// All histories are cut into tiles of 64 or 32 keys of one key head (and of up to 8 or 16 of its query heads); the tiles of the whole batch, one
+// All histories are cut into tiles of 64 keys of one key head (and of up to 8 or 16 of its query heads); the tiles of the whole batch, one
 // history behind the other, are dealt out in equal shares to the blocks of a head, so that a batch of ragged histories, one long history and many
 // short ones fill the device alike.  Neighbouring blocks take the heads of one share: their rows are neighbours in memory, and are read at
 // about the same time.  A history that lies in several shares leaves a partial result in each, which kv8_merge_kernel joins.
 //
 // kv8_decode_kernel: a fetching warp brings tiles (TMA, swizzled) and their exponent bytes through a ring of stages, also across the ends of
-// histories; two or three pairs of warps (heads of more than 128 values: seven warps) take tiles in turn,
-// a warp 32 keys of one, with softmax states of their own and no barrier before a history's end.
+// histories; two or three pairs of warps take tiles in turn, a warp 32 keys of one, with softmax states of their own and no barrier before a history's end.
 //
 //   S^T = K Q^T      keys are the 16-row operand: a lane's 16 bytes of two keys are four steps of the product as they lie, since any order
 //                    of the summed dims will do that the queries follow
@@ -37,7 +36,7 @@ struct Kv8DecodeParams {
     int* err;                            // error word of bounded waits
 };
 
-constexpr int MAX_T = 256;                       // tokens a launch
+constexpr int KT = 64, MAX_T = 256;              // keys a tile, tokens a launch
 // Weights are 2^(score + exponent of the value's scale - reference).  A row's reference is raised to 2^TOP below the largest when one would be above
 // 2^(TOP + RAISE), which fp16 holds; fp32 weights reach down to 2^-126, so that two rows whose scales are the format's limits apart (2^120) are told
 // apart by weights down to 2^-14 of the largest.
@@ -84,7 +83,6 @@ struct Batch {
 struct Deal { int items, abreast, passes; };         // passes: items of a block at most
 
 // The batch's tiles of KT keys of one item, numbered token by token.
-template <int KT>
 struct Tiles {
     const Batch& batch;
     int T, shares;                       // tokens; shares that the tiles are cut into
@@ -164,10 +162,10 @@ constexpr int blocks_per_sm(int width, int tiles) { return width == 64 ? (tiles 
 
 template <int D, int NG>
 struct Cfg {
-    static constexpr int PER_SM = blocks_per_sm(D, NG), WARPS = PER_SM > 1 ? 4 : D == 128 ? 6 : 7, THREADS = WARPS * 32 + 32;
-    static constexpr int KT = D > 128 ? 32 : 64, TEAM = KT / 32, TURNS = WARPS / TEAM;      // keys of a tile, warps that share one, tiles at a time
+    static constexpr int PER_SM = blocks_per_sm(D, NG), WARPS = PER_SM > 1 ? 4 : 6, THREADS = WARPS * 32 + 32;
+    static constexpr int TURNS = WARPS / 2;                              // tiles at a time, a pair of warps to each
     static constexpr int ROW = D < 128 ? D : 128, HALVES = D / ROW;      // bytes of a row in one box, boxes
-    static constexpr int STAGES = D == 64 ? 6 : D == 256 ? 9 : NG == 1 ? 5 : 10, HG = 8 * NG;
+    static constexpr int STAGES = D == 64 ? 6 : D == 256 ? 4 : NG == 1 ? 5 : 10, HG = 8 * NG;
     static constexpr int CHUNK = D < 128 ? 8 : 16, MT = D / 16;          // neighbouring dims of a lane, 16-dim rows of products
     static constexpr int CODES = KT * D, STAGE = 2 * CODES;              // keys, values
     static constexpr int EXPS = STAGES * STAGE;                          // KT bytes of the keys, KT of the values
@@ -183,7 +181,7 @@ template <int D, int NG>
 __global__ void __launch_bounds__(Cfg<D, NG>::THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                                                                                Kv8DecodeParams p, Deal deal, int box, Parts parts) {
     using M = Cfg<D, NG>;
-    constexpr int KT = M::KT, MT = M::MT, WARPS = M::WARPS, THREADS = M::THREADS;
+    constexpr int MT = M::MT, WARPS = M::WARPS, THREADS = M::THREADS;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint64_t *full = reinterpret_cast<uint64_t*>(smem + M::BARS), *free_ = full + M::STAGES, *q_full = free_ + M::STAGES, *q_free = q_full + 2;
@@ -203,7 +201,7 @@ __global__ void __launch_bounds__(Cfg<D, NG>::THREADS, Cfg<D, NG>::PER_SM) kv8_d
     }
     pdl_grid_sync();
     const int group = p.n_heads / p.n_kv, hg = (group + M::HG - 1) / M::HG;
-    const Tiles<KT> tiles(*reinterpret_cast<Batch*>(smem + M::BATCH), p, gridDim.x / deal.abreast);
+    const Tiles tiles(*reinterpret_cast<Batch*>(smem + M::BATCH), p, gridDim.x / deal.abreast);
     const bool by_item = parts == Parts::BY_ITEM, by_block = parts == Parts::BY_BLOCK;
     for (int t = blockIdx.x; t < p.T; t += gridDim.x)
         if (tiles.count(t) == 0) {
@@ -235,7 +233,7 @@ __global__ void __launch_bounds__(Cfg<D, NG>::THREADS, Cfg<D, NG>::PER_SM) kv8_d
             Ahead a{-1, -1, 0, nullptr, 0u};
             if (w >= w1) return a;
             const int pass = passes == 1 ? 0 : (int)(w / len), s = s0 + (int)(w - (long long)pass * len), item = first_item + pass * deal.abreast;
-            const typename Tiles<KT>::Place at = tiles.at(s);
+            const Tiles::Place at = tiles.at(s);
             const int key = at.tile * KT + lane % subs * box, n = at.n * KT - (KT - 1) + tiles.batch.last[at.t];
             const int r_lo = hg == 1 ? 0 : item % hg * M::HG, b = tiles.batch.row[at.t], page = key / p.pages.page_size;
             a.head = hg == 1 ? item : item / hg;
@@ -249,6 +247,7 @@ __global__ void __launch_bounds__(Cfg<D, NG>::THREADS, Cfg<D, NG>::PER_SM) kv8_d
                 a.page = p.pages.page_table[(size_t)b * p.pages.pt_stride + page];
             return a;
         };
+        auto of_lane = [](int x, int from) { return __shfl_sync(0xffffffffu, x, from); };
         int issued = 0, asked = 0, st = 0;                       // tiles, histories, stage
         bool ok = true;
         Ahead now, then = look(lane / subs);
@@ -259,7 +258,8 @@ __global__ void __launch_bounds__(Cfg<D, NG>::THREADS, Cfg<D, NG>::PER_SM) kv8_d
             // a page that is not there is recorded; rows in front of the tensor read as zeros
             const bool there = now.key >= 0 && guard_ok(p.pages.guard, 32, (long long)now.page * p.pages.page_size, p.pages.num_slots);
             const int row = there ? now.page * p.pages.page_size + off : -KT;
-            const uint8_t* from = p.exps + (((size_t)(there ? now.page : 0) * p.n_kv + now.head) * 2) * p.pages.page_size + off;
+            // (exponent bytes of a box start at multiples of 16)
+            const uint32_t from = (uint32_t)(((((size_t)(there ? now.page : 0) * p.n_kv + max(now.head, 0)) * 2) * p.pages.page_size + max(off, 0)) / 16);
             for (int i = 0; i < n; ++i, ++issued) {
                 if (i == min(n - 1, M::STAGES)) then = look(w + batch + lane / subs);
                 const int at = i * subs;
@@ -273,21 +273,24 @@ __global__ void __launch_bounds__(Cfg<D, NG>::THREADS, Cfg<D, NG>::PER_SM) kv8_d
                     ++asked;
                 }
                 if (issued >= M::STAGES && !tc::mbar_wait_warp(free_ + st, (uint32_t)(issued / M::STAGES + 1) & 1)) { ok = false; break; }
-                if (lane == at) tc::mbar_expect_tx(full + st, __popc(boxes >> at & ((1u << subs) - 1)) * box * (2 * D + 2));
-                __syncwarp();
-                if ((uint32_t)(lane - at) < (uint32_t)subs && now.key >= 0) {
-                    const int u = lane - at;
+                const uint32_t there = boxes >> at & ((1u << subs) - 1), bytes = __popc(there) * box * (2 * D + 2);
+                for (int u = 0; u < subs && (there >> u & 1) != 0; ++u) {    // (boxes behind the history are left out)
+                    const int row_u = of_lane(row, at + u), head_u = of_lane(now.head, at + u);
+                    const uint8_t* from_u = p.exps + (size_t)(uint32_t)of_lane((int)from, at + u) * 16;
                     uint8_t *codes = smem + st * M::STAGE + u * box * M::ROW, *exps = smem + M::EXPS + st * 2 * KT;
+                    if (tc::elect_one()) {
+                        if (u == 0) tc::mbar_expect_tx(full + st, bytes);
 #pragma unroll
-                    for (int x = 0; x < M::HALVES; ++x) {
-                        tc::tma_load_3d(codes + x * KT * M::ROW, &map_k, full + st, x * 128, now.head, row);
-                        tc::tma_load_3d(codes + M::CODES + x * KT * M::ROW, &map_v, full + st, x * 128, now.head, row);
-                    }
-                    if (box == KT && p.pages.page_size == KT) {              // the bytes of keys and values are neighbours
-                        tc::bulk_load_1d(exps, from, 2 * KT, full + st);
-                    } else {
-                        tc::bulk_load_1d(exps + u * box, from, box, full + st);
-                        tc::bulk_load_1d(exps + KT + u * box, from + p.pages.page_size, box, full + st);
+                        for (int x = 0; x < M::HALVES; ++x) {
+                            tc::tma_load_3d(codes + x * KT * M::ROW, &map_k, full + st, x * 128, head_u, row_u);
+                            tc::tma_load_3d(codes + M::CODES + x * KT * M::ROW, &map_v, full + st, x * 128, head_u, row_u);
+                        }
+                        if (box == KT && p.pages.page_size == KT) {          // the bytes of keys and values are neighbours
+                            tc::bulk_load_1d(exps, from_u, 2 * KT, full + st);
+                        } else {
+                            tc::bulk_load_1d(exps + u * box, from_u, box, full + st);
+                            tc::bulk_load_1d(exps + KT + u * box, from_u + p.pages.page_size, box, full + st);
+                        }
                     }
                 }
                 __syncwarp();
@@ -301,16 +304,16 @@ __global__ void __launch_bounds__(Cfg<D, NG>::THREADS, Cfg<D, NG>::PER_SM) kv8_d
         return;
     }
 
-    // ---- products: the warps of a team take 32 keys each of every tile that is their turn ----
-    const int g = lane >> 2, c4 = lane & 3, k0 = warp % M::TEAM * 32;
+    // ---- products: a pair of warps takes every tile that is its turn, a warp 32 of its keys ----
+    const int g = lane >> 2, c4 = lane & 3, k0 = (warp & 1) * 32;
     constexpr int CH = D < 128 ? 1 : D / 64;                         // 16-byte pieces of a key row a lane reads
     // places of a lane's pieces in a tile
     const int ks = D < 128 ? (k0 + g) * 64 + ((c4 ^ (g >> 1 & 3)) << 4) : (k0 + g) * 128;
-    int st = 0, turn = warp / M::TEAM, done = 0;                     // 0: this team's tile; histories behind it
+    int st = 0, turn = warp >> 1, done = 0;                     // 0: this pair's tile; histories behind it
     uint32_t phase = 0;
     bool ok = true;
-    const typename Tiles<KT>::Place begin = tiles.at(s0);
-    typename Tiles<KT>::Place at = begin;
+    const Tiles::Place begin = tiles.at(s0);
+    Tiles::Place at = begin;
     for (int s = s0, pass = 0;;) {
         const int item = first_item + pass * deal.abreast, count = min(at.n - at.tile, s1 - s), t = at.t, hkv = item / hg, r_lo = item % hg * M::HG;
         const int nr = min(M::HG, group - r_lo), h0 = hkv * group + r_lo, keys = at.n * KT - (KT - 1) + tiles.batch.last[t];
@@ -369,7 +372,7 @@ __global__ void __launch_bounds__(Cfg<D, NG>::THREADS, Cfg<D, NG>::PER_SM) kv8_d
         bool fresh = true;                                           // no reference yet
         for (int j = at.tile; j < at.tile + count; ++j) {
             const int stage = st;
-            // (also where it is another team's turn: a barrier must not be two phases ahead of who waits for it)
+            // (also where it is another pair's turn: a barrier must not be two phases ahead of who waits for it)
             if (ok) ok = tc::mbar_wait_warp(full + stage, phase);
             if (++st == M::STAGES) { st = 0; phase ^= 1u; }
             const bool mine = turn == 0;
@@ -657,7 +660,7 @@ int launch(const Kv8DecodeParams* all, int T, int blocks, const Deal& deal, int 
     constexpr int smem = M::TOTAL + 1024;
     static_assert(M::PER_SM * (smem + 1024) <= 228 * 1024, "blocks per SM");
     static SmemOptIn opt_in;
-    const int page = all->pages.page_size, box = page % M::KT == 0 ? M::KT : page % 32 == 0 ? 32 : 16;
+    const int page = all->pages.page_size, box = page % 64 == 0 ? 64 : page % 32 == 0 ? 32 : 16;
     CUtensorMap mk, mv;
     int rc = map_codes(&mk, all->k_codes, all, D, box);
     if (rc == 0) rc = map_codes(&mv, all->v_codes, all, D, box);
@@ -710,7 +713,7 @@ SL_API int sl_kv8_decode(const Kv8DecodeParams* p, int T, int blocks, int longes
     if ((((uintptr_t)p->q | (uintptr_t)p->k_codes | (uintptr_t)p->v_codes | (uintptr_t)p->exps | (uintptr_t)p->out | (uintptr_t)p->o_part | (uintptr_t)p->jobs) & 15) != 0) return -1;
     const Shape sh = shape_of(p->n_heads, p->n_kv, p->hd);
     const Deal deal = deal_of(sh, p->n_heads, p->n_kv, blocks);
-    if ((long long)(p->pages.pt_width) * p->pages.page_size / 32 > 0x7fffffff / MAX_T - 1) return -1;        // tiles are counted in 32 bits
+    if ((long long)(p->pages.pt_width) * p->pages.page_size / KT > 0x7fffffff / MAX_T - 1) return -1;        // tiles are counted in 32 bits
     if (sh.width == 64) return sh.tiles == 2 ? launch<64, 2>(p, T, blocks, deal, longest, s) : launch<64, 1>(p, T, blocks, deal, longest, s);
     if (sh.width == 128) return sh.tiles == 2 ? launch<128, 2>(p, T, blocks, deal, longest, s) : launch<128, 1>(p, T, blocks, deal, longest, s);
     return launch<256, 1>(p, T, blocks, deal, longest, s);
