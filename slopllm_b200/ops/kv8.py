@@ -18,7 +18,7 @@ from typing import Optional, Tuple
 
 import torch
 
-from . import reference as R
+from . import native as N, reference as R, tcgen05
 from .dense import AttnParams, _slots
 from .rotary import RotaryTable
 
@@ -26,40 +26,32 @@ LOW, HIGH, BIAS = -60, 60, 127         # limits of the exponent, and what is add
 UNPACK_BUDGET_BYTES = 1 << 30          # transient bf16 rows of a prompt step; more sequences go in groups
 
 
-def _native():
-    from . import native as N
-    return N
-
-
-class _Pages(C.Structure):
-    _fields_ = [("page_table", C.c_void_p), ("pt_stride", C.c_int), ("pt_rows", C.c_int), ("pt_width", C.c_int), ("page_size", C.c_int),
-                ("num_slots", C.c_int), ("guard", C.c_void_p)]
+# (Kv8Pages and Kv8Rows of the kernels, spliced into the structures that hold them: a call makes one object)
+_PAGES = [("page_table", C.c_void_p), ("pt_stride", C.c_int), ("pt_rows", C.c_int), ("pt_width", C.c_int), ("page_size", C.c_int),
+          ("num_slots", C.c_int), ("guard", C.c_void_p)]
+_ROWS = [("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("exps", C.c_void_p), *_PAGES, ("n_kv", C.c_int), ("hd", C.c_int)]
 
 
 class Kv8StoreParams(C.Structure):
     _fields_ = [("q", C.c_void_p), ("ldq", C.c_int), ("k", C.c_void_p), ("ldk", C.c_int), ("v", C.c_void_p), ("ldv", C.c_int),
                 ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("freq", C.c_void_p), ("gain", C.c_float), ("rot_dims", C.c_int),
-                ("positions", C.c_void_p), ("batch_idx", C.c_void_p), ("pages", _Pages), ("n_heads", C.c_int), ("n_kv", C.c_int),
+                ("positions", C.c_void_p), ("batch_idx", C.c_void_p), *_PAGES, ("n_heads", C.c_int), ("n_kv", C.c_int),
                 ("hd", C.c_int), ("q_stride", C.c_int), ("eps", C.c_float), ("q_out", C.c_void_p), ("k_codes", C.c_void_p),
                 ("v_codes", C.c_void_p), ("exps", C.c_void_p)]
 
 
-class _Rows(C.Structure):
-    _fields_ = [("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("exps", C.c_void_p), ("pages", _Pages), ("n_kv", C.c_int), ("hd", C.c_int)]
-
-
 class Kv8ReadParams(C.Structure):
-    _fields_ = [("c", _Rows), ("ranges", C.c_void_p), ("rows", C.c_int), ("k", C.c_void_p), ("v", C.c_void_p)]
+    _fields_ = [*_ROWS, ("ranges", C.c_void_p), ("rows", C.c_int), ("k", C.c_void_p), ("v", C.c_void_p)]
 
 
 class Kv8UnpackParams(C.Structure):
-    _fields_ = [("c", _Rows), ("qo_indptr", C.c_void_p), ("positions", C.c_void_p), ("batch_idx", C.c_void_p), ("per_seq", C.c_int),
+    _fields_ = [*_ROWS, ("qo_indptr", C.c_void_p), ("positions", C.c_void_p), ("batch_idx", C.c_void_p), ("per_seq", C.c_int),
                 ("k", C.c_void_p), ("v", C.c_void_p), ("table", C.c_void_p), ("rows_out", C.c_void_p), ("positions_out", C.c_void_p)]
 
 
 class Kv8DecodeParams(C.Structure):
     _fields_ = [("q", C.c_void_p), ("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("exps", C.c_void_p), ("positions", C.c_void_p),
-                ("batch_idx", C.c_void_p), ("pages", _Pages), ("n_heads", C.c_int), ("n_kv", C.c_int), ("hd", C.c_int), ("scale", C.c_float),
+                ("batch_idx", C.c_void_p), *_PAGES, ("n_heads", C.c_int), ("n_kv", C.c_int), ("hd", C.c_int), ("scale", C.c_float),
                 ("out", C.c_void_p), ("o_part", C.c_void_p), ("lse_part", C.c_void_p), ("jobs", C.c_void_p), ("T", C.c_int), ("err", C.c_void_p)]
 
 
@@ -94,33 +86,31 @@ class Kv8Cache:
         return Kv8Cache(codes(), codes(), torch.zeros(num_pages, n_kv, 2, page_size, dtype=torch.uint8, device=device))
 
 
-def _check_step(x: torch.Tensor, cache: Kv8Cache, *tables: torch.Tensor) -> None:
-    """Tables of a step are int32 on the device of `x` and the cache, with values side by side."""
+def _check_step(device: int, cache: Kv8Cache, *tables: torch.Tensor) -> None:
+    """Tables of a step are int32 on the device of the data and the cache, with values side by side."""
+    if cache.k.get_device() != device:
+        raise ValueError(f"data on device {device}, cache on {cache.k.device}")
     for t in tables:
-        if t.dtype != torch.int32 or t.device != x.device or (t.shape[-1] > 1 and t.stride(-1) != 1):
+        if t.dtype != torch.int32 or t.get_device() != device or (t.stride(-1) != 1 and t.shape[-1] > 1):
             raise ValueError("positions, rows, ranges and page tables are int32, on the device of the data, with values side by side")
-    if cache.k.device != x.device:
-        raise ValueError(f"data on {x.device}, cache on {cache.k.device}")
 
 
-def _pages(cache: Kv8Cache, page_table: torch.Tensor) -> _Pages:
-    from . import tcgen05
+def _pages(cache: Kv8Cache, page_table: torch.Tensor) -> tuple:
     rows, width = page_table.shape
-    return _Pages(page_table.data_ptr(), page_table.stride(0), rows, width, cache.exps.shape[3], cache.k.shape[0],
-                  tcgen05.error_flag(cache.k.device).data_ptr() + 16)
+    return (page_table.data_ptr(), page_table.stride(0), rows, width, cache.exps.shape[3], cache.k.shape[0],
+            tcgen05.error_flag(cache.k.device).data_ptr() + 16)
 
 
-def _rows(cache: Kv8Cache, page_table: torch.Tensor) -> _Rows:
-    return _Rows(cache.k.data_ptr(), cache.v.data_ptr(), cache.exps.data_ptr(), _pages(cache, page_table), cache.k.shape[1], cache.k.shape[2])
+def _rows(cache: Kv8Cache, page_table: torch.Tensor) -> tuple:
+    return (cache.k.data_ptr(), cache.v.data_ptr(), cache.exps.data_ptr(), *_pages(cache, page_table), cache.k.shape[1], cache.k.shape[2])
 
 
-def _call(x: torch.Tensor, name: str, *args) -> None:
-    """A kernel call on the stream and device of `x`."""
-    N = _native()
-    if x.get_device() == torch.cuda.current_device():
+def _call(device: int, name: str, *args) -> None:
+    """A kernel call on the current stream of a device."""
+    if device == torch.cuda.current_device():
         N.call(name, *args, N.stream())
     else:
-        with torch.cuda.device(x.device):
+        with torch.cuda.device(device):
             N.call(name, *args, N.stream())
 
 
@@ -155,7 +145,7 @@ def kv8_store(q, k, v, q_norm, k_norm, rot: RotaryTable, positions, batch_idx, p
     h * q_stride), k / v [T, n_kv * hd], bf16 on a GPU with rows of any stride.  Everything is fp32 between the rows and the one rounding of a
     result (angles: position * frequency in 64 bits).  A token whose position is negative leaves the cache as it is.  Returns
     the queries [T, n_heads, hd]."""
-    T, (_, n_kv, hd) = q.shape[0], cache.k.shape
+    T, (_, n_kv, hd), device = q.shape[0], cache.k.shape, q.get_device()
     q_stride = hd if q_stride is None else q_stride
     if q.shape[1] != n_heads * q_stride or q_stride < hd or k.shape != (T, n_kv * hd) or v.shape != k.shape:
         raise ValueError(f"projections {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)} for {n_heads} heads over {n_kv} of {hd} values")
@@ -163,19 +153,21 @@ def kv8_store(q, k, v, q_norm, k_norm, rot: RotaryTable, positions, batch_idx, p
         raise ValueError(f"{rot.dims} rotated values with {rot.freq.numel()} frequencies in heads of {hd}")
     if positions.shape != (T,) or batch_idx.shape != (T,):
         raise ValueError(f"{T} tokens with positions {tuple(positions.shape)} and rows {tuple(batch_idx.shape)}")
-    _check_step(q, cache, positions, batch_idx, page_table)
-    if q.is_cuda:
+    _check_step(device, cache, positions, batch_idx, page_table)
+    if device >= 0:
         for x in (q, k, v, q_norm, k_norm):
-            if x is not None and (x.dtype != torch.bfloat16 or x.device != q.device or x.stride(-1) != 1):
+            if x is not None and (x.dtype != torch.bfloat16 or x.get_device() != device or x.stride(-1) != 1):
                 raise ValueError("projection rows and norm weights are bf16, on one device, with values side by side")
-        if rot.freq.dtype != torch.float32 or rot.freq.device != q.device or not rot.freq.is_contiguous():
+        for w in (q_norm, k_norm):
+            if w is not None and w.shape != (hd,):
+                raise ValueError(f"norm weights of {tuple(w.shape)} for heads of {hd} values")
+        if rot.freq.dtype != torch.float32 or rot.freq.get_device() != device or not rot.freq.is_contiguous():
             raise ValueError("frequencies are fp32, contiguous and on the device of the data")
-        N = _native()
         out = torch.empty(T, n_heads, hd, dtype=torch.bfloat16, device=q.device)
         p = Kv8StoreParams(q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), N.ptr(q_norm), N.ptr(k_norm),
-                           rot.freq.data_ptr(), rot.gain, rot.dims, positions.data_ptr(), batch_idx.data_ptr(), _pages(cache, page_table),
+                           rot.freq.data_ptr(), rot.gain, rot.dims, positions.data_ptr(), batch_idx.data_ptr(), *_pages(cache, page_table),
                            n_heads, n_kv, hd, q_stride, eps, out.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.exps.data_ptr())
-        _call(q, "sl_kv8_store", C.byref(p), T)
+        _call(device, "sl_kv8_store", C.byref(p), T)
         return out
 
     def turned(x, w):
@@ -201,12 +193,14 @@ def kv8_read(cache: Kv8Cache, ranges: torch.Tensor, rows: int, longest: int, pag
     of tokens (at most `longest`), first row of the result; rows in no range are not written."""
     if ranges.dim() != 2 or ranges.shape[1] != 4 or not ranges.is_contiguous():
         raise ValueError(f"ranges are [R, 4] and contiguous, not {tuple(ranges.shape)}")
-    _check_step(ranges, cache, ranges, page_table)
+    device = ranges.get_device()
+    _check_step(device, cache, ranges, page_table)
     _, n_kv, hd = cache.k.shape
-    k, v = (torch.empty(rows, n_kv, hd, dtype=torch.bfloat16, device=cache.k.device) for _ in range(2))
-    if ranges.is_cuda:
-        p = Kv8ReadParams(_rows(cache, page_table), ranges.data_ptr(), rows, k.data_ptr(), v.data_ptr())
-        _call(k, "sl_kv8_read", C.byref(p), ranges.shape[0], longest)
+    k = torch.empty(rows, n_kv, hd, dtype=torch.bfloat16, device=cache.k.device)
+    v = torch.empty_like(k)
+    if device >= 0:
+        p = Kv8ReadParams(*_rows(cache, page_table), ranges.data_ptr(), rows, k.data_ptr(), v.data_ptr())
+        _call(device, "sl_kv8_read", C.byref(p), ranges.shape[0], longest)
         return k, v
     for b, first, n, row in ranges.tolist():
         pos = torch.arange(first, first + n)
@@ -221,14 +215,14 @@ def kv8_attention(q, cache: Kv8Cache, positions, batch_idx, page_table, sm_scale
     page-table row batch_idx[t]) over the keys 0..position of its sequence.  q [T, n_heads, hd], bf16 on a GPU -> [T, n_heads, hd].  With
     `qo_indptr` ([B + 1], contiguous token ranges of the sequences, at most `max_q` tokens and `max_kv_len` keys each; 0: not known) heads have 64
     or 128 values on a GPU; without it a row may have no keys (position -1), and is zero."""
-    T, n_heads, hd = q.shape
+    (T, n_heads, hd), device = q.shape, q.get_device()
     _, n_kv, width = cache.k.shape
     if hd != width or n_heads % n_kv:
         raise ValueError(f"{n_heads} query heads of {hd} values over {n_kv} key heads of {width}")
     if positions.shape != (T,) or batch_idx.shape != (T,):
         raise ValueError(f"{T} tokens with positions {tuple(positions.shape)} and rows {tuple(batch_idx.shape)}")
-    _check_step(q, cache, positions, batch_idx, page_table, *(() if qo_indptr is None else (qo_indptr,)))
-    if not q.is_cuda:
+    _check_step(device, cache, positions, batch_idx, page_table)
+    if device < 0:
         out = torch.zeros(T, n_heads, hd, dtype=torch.float32)
         for t in range(T):
             n = int(positions[t]) + 1
@@ -241,19 +235,19 @@ def kv8_attention(q, cache: Kv8Cache, positions, batch_idx, page_table, sm_scale
         raise ValueError(f"queries of type {q.dtype}: the kernels take bf16")
     if not q.is_contiguous() or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
-    out = torch.empty(T, n_heads, hd, dtype=torch.bfloat16, device=q.device)
+    out = torch.empty_like(q)
     if T == 0:
         return out
     if qo_indptr is None:
-        from . import tcgen05
-        blocks, parts, rows, wide = _decode_plan(q.get_device(), n_heads, n_kv, hd)
+        blocks, parts, rows, wide = _decode_plan(device, n_heads, n_kv, hd)
         part = torch.empty(parts * (2 * rows * (wide + 1) + 4), dtype=torch.float32, device=q.device)
         sums = part.data_ptr() + parts * 16
         p = Kv8DecodeParams(q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.exps.data_ptr(), positions.data_ptr(), batch_idx.data_ptr(),
-                            _pages(cache, page_table), n_heads, n_kv, hd, sm_scale, out.data_ptr(), sums,
+                            *_pages(cache, page_table), n_heads, n_kv, hd, sm_scale, out.data_ptr(), sums,
                             sums + parts * 2 * rows * wide * 4, part.data_ptr(), 0, tcgen05.error_flag(q.device).data_ptr())
-        _call(q, "sl_kv8_decode", C.byref(p), T, blocks, max_kv_len)
+        _call(device, "sl_kv8_decode", C.byref(p), T, blocks, max_kv_len)
         return out
+    _check_step(device, cache, qo_indptr)
     if hd not in (64, 128):
         raise ValueError(f"heads of {hd} values: attention of prompts takes 64 or 128")
     _prompts(q, cache, positions, batch_idx, page_table, sm_scale, qo_indptr, max_q or T, max_kv_len, out)
@@ -263,7 +257,6 @@ def kv8_attention(q, cache: Kv8Cache, positions, batch_idx, page_table, sm_scale
 @lru_cache(maxsize=None)
 def _decode_plan(device: int, n_heads: int, n_kv: int, hd: int) -> Tuple[int, ...]:
     """(blocks, partial results, their rows and width) of the decode kernel on a device."""
-    N = _native()
     out = (C.c_int * 4)()
     at = C.addressof(out)
     with torch.cuda.device(device):
@@ -274,9 +267,8 @@ def _decode_plan(device: int, n_heads: int, n_kv: int, hd: int) -> Tuple[int, ..
 def _prompts(q, cache, positions, batch_idx, page_table, sm_scale, qo_indptr, max_q, max_kv_len, out) -> None:
     """Histories are read back into bf16 pages of 64 tokens, over which the prompt kernel attends.  Done once per key head and token, that
     costs less than codes that every block of the kernel (query heads x 128 queries) turns into an operand anew."""
-    from . import tcgen05
-    T, n_heads, hd = q.shape
-    n_kv, B, dev = cache.k.shape[1], qo_indptr.numel() - 1, q.device
+    (T, n_heads, hd), device, dev = q.shape, q.get_device(), q.device
+    n_kv, B = cache.k.shape[1], qo_indptr.numel() - 1
     most = page_table.shape[1] * cache.page_size
     per_seq = max(1, -(-min(max_kv_len or most, most) // 64))
     group = max(1, min(B, UNPACK_BUDGET_BYTES // (per_seq * 64 * n_kv * hd * 4)))
@@ -286,9 +278,9 @@ def _prompts(q, cache, positions, batch_idx, page_table, sm_scale, qo_indptr, ma
     rows = _rows(cache, page_table)
     for s in range(0, B, group):
         n, ends = min(group, B - s), qo_indptr.data_ptr() + 4 * s
-        up = Kv8UnpackParams(rows, ends, positions.data_ptr(), batch_idx.data_ptr(), per_seq, k.data_ptr(), v.data_ptr(), table, rows_out, positions_out)
-        _call(q, "sl_kv8_unpack", C.byref(up), n)
+        up = Kv8UnpackParams(*rows, ends, positions.data_ptr(), batch_idx.data_ptr(), per_seq, k.data_ptr(), v.data_ptr(), table, rows_out, positions_out)
+        _call(device, "sl_kv8_unpack", C.byref(up), n)
         p = AttnParams(q=q.data_ptr(), k_cache=k.data_ptr(), v_cache=v.data_ptr(), positions=positions_out, batch_idx=rows_out, page_table=table,
                        pt_stride=per_seq, page_size=64, qo_indptr=ends, n_heads=n_heads, n_kv=n_kv, hd=hd, sm_scale=sm_scale, out=out.data_ptr(), T=T,
                        num_slots=k.shape[0], max_keys=max_kv_len, err=tcgen05.error_flag(dev).data_ptr())
-        _call(q, "sl_paged_attn_prefill", C.byref(p), n, int(max_q))
+        _call(device, "sl_paged_attn_prefill", C.byref(p), n, int(max_q))

@@ -5,6 +5,7 @@ import torch
 from kv8_util import attend, exponent, filled, held, near, round_e4m3, table_of
 from slopllm_b200.ops import kv8 as K8
 from slopllm_b200.ops import tcgen05
+from slopllm_b200.ops.native import NativeError
 from slopllm_b200.ops.rotary import RotaryTable, rotary_table
 
 pytestmark = pytest.mark.gpu
@@ -182,13 +183,13 @@ def test_tables_that_point_nowhere():
                  lambda: K8.kv8_read(cache, ints([[row, pos, 1, 0]]), 1, 1, t))
         for call in calls:
             call()
-            with pytest.raises(K8._native().NativeError):
+            with pytest.raises(NativeError):
                 tcgen05.check_errors(q.device)
     K8.kv8_read(cache, ints([[0, 0, 10, 5]]), 12, 10, table)
-    with pytest.raises(K8._native().NativeError):
+    with pytest.raises(NativeError):
         tcgen05.check_errors(q.device)
     K8.kv8_read(cache, ints([[0, -1, 1, 0]]), 1, 1, table)
-    with pytest.raises(K8._native().NativeError):
+    with pytest.raises(NativeError):
         tcgen05.check_errors(q.device)
     assert all(torch.equal(a, b) for a, b in zip(before, (cache.k, cache.v, cache.exps)))
 
