@@ -24,15 +24,48 @@ struct Kv8StoreParams {
 
 constexpr double TWO_PI = 6.283185307179586476925;
 
-// grid (T, y), block 256: a warp per row of a head (queries, then keys, then values), P neighbouring values a lane.  VEC: rows are aligned to
-// a lane's values.
-template <int P, bool VEC>
+// 8 bf16 values; VEC: 16 bytes at once
+template <bool VEC>
+__device__ __forceinline__ uint4 load8(const bf16* p) {
+    if (VEC) return *reinterpret_cast<const uint4*>(p);
+    const uint16_t* u = reinterpret_cast<const uint16_t*>(p);
+    uint32_t w[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) w[i] = (uint32_t)u[2 * i] | (uint32_t)u[2 * i + 1] << 16;
+    return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ void unpack8(const uint4& u, float (&x)[8]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const float2 f = bf162_to_f2(w[i]);
+        x[2 * i] = f.x;
+        x[2 * i + 1] = f.y;
+    }
+}
+
+// grid (T, y), block 256.  A row of a head (queries, then keys, then values) has L lanes of 8 neighbouring values, a warp 32 / L rows at a time; a lane
+// keeps the angles and weights of its values for all rows.  VEC: rows are aligned to 16 bytes.  EVEN: partners of a rotation are whole lanes
+// apart (shuffles), else they come through shared memory.
+template <int L, bool VEC, bool EVEN>
 __global__ void __launch_bounds__(256) kv8_store_kernel(Kv8StoreParams p) {
     pdl_grid_sync();
+    constexpr int ROWS = 32 / L, AT_ONCE = 8 * ROWS;
     __shared__ float2 turn[128];                     // (cos, sin) of each pair
-    __shared__ float row[8][32 * P];
-    const int t = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = p.rot_dims / 2;
-    const int pos = p.positions[t];
+    __shared__ float part[EVEN ? 1 : 8][EVEN ? 1 : 256];
+    const int t = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = p.rot_dims / 2, jobs = p.n_heads + 2 * p.n_kv;
+    const int own = lane % L, d0 = own * 8, step = gridDim.y * AT_ONCE;
+    const bool on = d0 < p.hd;
+    auto source = [&](int job) {
+        return (job < p.n_heads ? p.q + (size_t)t * p.ldq + (size_t)job * p.q_stride
+                : job < p.n_heads + p.n_kv ? p.k + (size_t)t * p.ldk + (size_t)(job - p.n_heads) * p.hd
+                                           : p.v + (size_t)t * p.ldv + (size_t)(job - p.n_heads - p.n_kv) * p.hd) + d0;
+    };
+    int job = (blockIdx.y * 8 + warp) * ROWS + lane / L;
+    const uint4 none = make_uint4(0u, 0u, 0u, 0u);
+    uint4 next = on && job < jobs ? load8<VEC>(source(job)) : none;
+    const uint4 wq = on && p.q_norm != nullptr ? load8<VEC>(p.q_norm + d0) : none, wk = on && p.k_norm != nullptr ? load8<VEC>(p.k_norm + d0) : none;
+    const int pos = p.positions[t], b = p.batch_idx[t];
     // fp32 keeps no digits of the angle of a far position: the product and its remainder are taken in 64 bits
     for (int i = threadIdx.x; i < half; i += 256) {
         const double a = (double)pos * (double)p.freq[i];
@@ -40,96 +73,84 @@ __global__ void __launch_bounds__(256) kv8_store_kernel(Kv8StoreParams p) {
         sincosf((float)fma(-rint(a * (1.0 / TWO_PI)), TWO_PI, a), &sn, &cs);
         turn[i] = make_float2(cs * p.gain, sn * p.gain);
     }
-    const int slot = pos < 0 ? -1 : kv8_slot(p.pages, 30, p.batch_idx[t], pos);
+    const int slot = pos < 0 ? -1 : kv8_slot(p.pages, 30, b, pos);
     __syncthreads();
-    const int d0 = lane * P;
-    const bool on = d0 < p.hd;
-    for (int job = blockIdx.y * 8 + warp; job < p.n_heads + 2 * p.n_kv; job += gridDim.y * 8) {
-        const int what = job < p.n_heads ? 0 : job < p.n_heads + p.n_kv ? 1 : 2;         // query, key, value
-        const int h = what == 0 ? job : what == 1 ? job - p.n_heads : job - p.n_heads - p.n_kv;
-        const bf16* src = what == 0 ? p.q + (size_t)t * p.ldq + (size_t)h * p.q_stride
-                                    : (what == 1 ? p.k + (size_t)t * p.ldk : p.v + (size_t)t * p.ldv) + (size_t)h * p.hd;
-        auto load = [&](const bf16* from, float (&x)[P]) {
-            if (VEC) {
-                uint32_t w[P / 2];
-                if (P == 8) *reinterpret_cast<uint4*>(w) = *reinterpret_cast<const uint4*>(from + d0);
-                else if (P == 4) *reinterpret_cast<uint2*>(w) = *reinterpret_cast<const uint2*>(from + d0);
-                else w[0] = *reinterpret_cast<const uint32_t*>(from + d0);
+    float cs[8], sn[8];                              // value' = value * cs + partner * sn
 #pragma unroll
-                for (int i = 0; i < P; i += 2) {
-                    const float2 f = bf162_to_f2(w[i / 2]);
-                    x[i] = f.x;
-                    x[i + 1] = f.y;
-                }
-            } else {
-#pragma unroll
-                for (int i = 0; i < P; ++i) x[i] = __bfloat162float(from[d0 + i]);
-            }
-        };
-        float x[P];
-#pragma unroll
-        for (int i = 0; i < P; ++i) x[i] = 0.f;
-        if (on) load(src, x);
-        const bf16* w = what == 0 ? p.q_norm : what == 1 ? p.k_norm : nullptr;
-        if (w != nullptr) {
+    for (int i = 0; i < 8; ++i) {
+        const int d = d0 + i;
+        const float2 a = d < p.rot_dims ? turn[d < half ? d : d - half] : make_float2(1.f, 0.f);
+        cs[i] = a.x;
+        sn[i] = d < half ? -a.y : a.y;
+    }
+    const int partner = EVEN ? lane + (d0 < half ? half / 8 : d0 < p.rot_dims ? -half / 8 : 0) : 0;
+    for (int base = blockIdx.y * AT_ONCE; base < jobs; base += step, job += step) {          // (warps stay together: shuffles)
+        float x[8];
+        unpack8(next, x);
+        const bool there = job < jobs, query = job < p.n_heads, key = !query && job < p.n_heads + p.n_kv;
+        next = on && job + step < jobs ? load8<VEC>(source(job + step)) : none;
+        if (p.q_norm != nullptr || p.k_norm != nullptr) {
             float ss = 0.f;
 #pragma unroll
-            for (int i = 0; i < P; ++i) ss += x[i] * x[i];
-            const float inv = 1.f / sqrtf(warp_sum(ss) / (float)p.hd + p.eps);
-            if (on) {
-                float g[P];
-                load(w, g);
+            for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
 #pragma unroll
-                for (int i = 0; i < P; ++i) x[i] = x[i] * inv * g[i];
+            for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            if ((query && p.q_norm != nullptr) || (key && p.k_norm != nullptr)) {
+                const float inv = 1.f / sqrtf(ss / (float)p.hd + p.eps);
+                float g[8];
+                unpack8(query ? wq : wk, g);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * g[i];
             }
         }
-        if (what < 2 && half > 0) {                  // (warp-uniform)
-            __syncwarp();
+        if (half > 0) {
+            float y[8];
+            if (EVEN) {
 #pragma unroll
-            for (int i = 0; i < P; ++i) row[warp][d0 + i] = x[i];
-            __syncwarp();
+                for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(0xffffffffu, x[i], partner);
+            } else {
+                __syncwarp();
 #pragma unroll
-            for (int i = 0; i < P; ++i) {
-                const int d = d0 + i;
-                if (d < half) x[i] = x[i] * turn[d].x - row[warp][d + half] * turn[d].y;
-                else if (d < p.rot_dims) x[i] = x[i] * turn[d - half].x + row[warp][d - half] * turn[d - half].y;
+                for (int i = 0; i < 8; ++i) part[EVEN ? 0 : warp][EVEN ? 0 : lane * 8 + i] = x[i];
+                __syncwarp();
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int d = d0 + i, other = d < half ? half : d < p.rot_dims ? -half : 0;
+                    y[i] = part[EVEN ? 0 : warp][EVEN ? 0 : lane * 8 + i + other];
+                }
             }
-        }
-        if (what == 0) {
-            bf16* dst = p.q_out + ((size_t)t * p.n_heads + h) * p.hd + d0;
-            if (on) {
-                uint32_t w2[P / 2];
+            if (query || key)
 #pragma unroll
-                for (int i = 0; i < P; i += 2) w2[i / 2] = f2_to_bf162(x[i], x[i + 1]);
-                if (P == 8) *reinterpret_cast<uint4*>(dst) = *reinterpret_cast<const uint4*>(w2);
-                else if (P == 4) *reinterpret_cast<uint2*>(dst) = *reinterpret_cast<const uint2*>(w2);
-                else *reinterpret_cast<uint32_t*>(dst) = w2[0];
-            }
-            continue;
+                for (int i = 0; i < 8; ++i)
+                    if (d0 + i < p.rot_dims) x[i] = x[i] * cs[i] + y[i] * sn[i];
         }
-        float top = 0.f;                             // of the finite values
+        if (there && query && on)
+            *reinterpret_cast<uint4*>(p.q_out + ((size_t)t * p.n_heads + job) * p.hd + d0) =
+                make_uint4(f2_to_bf162(x[0], x[1]), f2_to_bf162(x[2], x[3]), f2_to_bf162(x[4], x[5]), f2_to_bf162(x[6], x[7]));
+        if (base + AT_ONCE <= p.n_heads) continue;               // no keys or values among these rows
+        float top = 0.f;                                         // of the finite values
 #pragma unroll
-        for (int i = 0; i < P; ++i) {
+        for (int i = 0; i < 8; ++i) {
             if (!(fabsf(x[i]) <= FLT_MAX)) x[i] = __int_as_float(0x7fc00000);
             else top = fmaxf(top, fabsf(x[i]));
         }
-        top = warp_max(top);
-        if (slot < 0) continue;
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (!there || query || slot < 0) continue;
         // top = m 2^n with m in [1, 2), 448 = 1.75 * 2^8
         const uint32_t bits = __float_as_uint(top);
         const int e = min(KV8_HIGH, max(KV8_LOW, (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0)));
         const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
-        uint8_t* dst = (what == 1 ? p.k_codes : p.v_codes) + ((size_t)slot * p.n_kv + h) * p.hd + d0;
+        const int h = job - p.n_heads - (key ? 0 : p.n_kv);
         if (on) {
-            uint32_t c[(P + 3) / 4] = {};
+            uint32_t c[2];
 #pragma unroll
-            for (int i = 0; i < P; i += 2)
-                c[i / 4] |= (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[i] * inv, x[i + 1] * inv), __NV_SATFINITE, __NV_E4M3) << (i % 4 * 8);
-            if (P == 8) *reinterpret_cast<uint2*>(dst) = make_uint2(c[0], c[P / 8]);
-            else if (P == 4) *reinterpret_cast<uint32_t*>(dst) = c[0];
-            else *reinterpret_cast<uint16_t*>(dst) = (uint16_t)c[0];
+            for (int i = 0; i < 8; i += 4)
+                c[i / 4] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[i] * inv, x[i + 1] * inv), __NV_SATFINITE, __NV_E4M3) |
+                           (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[i + 2] * inv, x[i + 3] * inv), __NV_SATFINITE, __NV_E4M3) << 16;
+            *reinterpret_cast<uint2*>((key ? p.k_codes : p.v_codes) + ((size_t)slot * p.n_kv + h) * p.hd + d0) = make_uint2(c[0], c[1]);
         }
-        if (lane == 0) p.exps[kv8_exp_at(p.pages, p.n_kv, slot, h) + (what == 1 ? 0 : p.pages.page_size)] = (uint8_t)(e + KV8_BIAS);
+        if (own == 0) p.exps[kv8_exp_at(p.pages, p.n_kv, slot, h) + (key ? 0 : p.pages.page_size)] = (uint8_t)(e + KV8_BIAS);
     }
 }
 
@@ -156,59 +177,82 @@ struct Kv8UnpackParams {
     int *table, *rows_out, *positions_out;           // [sequences, per_seq], [T], [T]
 };
 
-// Rows `first` .. first + n - 1 (n <= 64) of page-table row b -> rows of k and v: 16 codes a thread at a time.
-__device__ __forceinline__ void read_rows(const Kv8Rows& c, int b, int first, int n, bf16* k, bf16* v) {
-    __shared__ int slots[64];
-    if (threadIdx.x < n) slots[threadIdx.x] = kv8_slot(c.pages, 31, b, first + threadIdx.x);
-    __syncthreads();
-    const int per = c.n_kv * c.hd / 16;              // pieces of a row
-    for (int x = threadIdx.x; x < 2 * n * per; x += blockDim.x) {
-        const int which = x >= n * per ? 1 : 0, y = x - which * n * per, i = y / per, d = (y - i * per) * 16, slot = slots[i];
-        uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;                  // (a token that is not there reads as zeros)
-        if (slot >= 0) {
-            const uint4 w = ldg_nc_16((which ? c.v_codes : c.k_codes) + (size_t)slot * c.n_kv * c.hd + d);
-            const float s = __uint_as_float((uint32_t)c.exps[kv8_exp_at(c.pages, c.n_kv, slot, d / c.hd) + which * c.pages.page_size] << 23);
-            auto two = [&](uint32_t u) {
-                const float2 f = e4m3x2_to_float2((uint16_t)u);
-                return f2_to_bf162(f.x * s, f.y * s);
-            };
-            lo = make_uint4(two(w.x & 0xffff), two(w.x >> 16), two(w.y & 0xffff), two(w.y >> 16));
-            hi = make_uint4(two(w.z & 0xffff), two(w.z >> 16), two(w.w & 0xffff), two(w.w >> 16));
+// 32 bytes at once
+__device__ __forceinline__ void store_32(void* p, const uint32_t (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};"
+                 ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
+
+constexpr int READ_ROWS = 4;         // a warp's at a time
+
+// Rows `first` .. first + n - 1 of page-table row b, keys (which 0) or values, -> dst: a warp takes READ_ROWS of them, a lane 16 codes of each at a time.
+__device__ __forceinline__ void read_rows(const Kv8Rows& c, int which, int b, int first, int n, bf16* dst) {
+    const int lane = threadIdx.x & 31, per = c.n_kv * c.hd / 16, per_head = c.hd / 16, page = c.pages.page_size;
+    const uint8_t* codes = which ? c.v_codes : c.k_codes;
+    for (int i0 = (threadIdx.x >> 5) * READ_ROWS; i0 < n; i0 += (blockDim.x >> 5) * READ_ROWS) {
+        int slot[READ_ROWS];
+        const uint8_t* exps[READ_ROWS];
+#pragma unroll
+        for (int i = 0; i < READ_ROWS; ++i) {
+            slot[i] = i0 + i < n ? kv8_slot(c.pages, 31, b, first + i0 + i) : -1;
+            exps[i] = c.exps + kv8_exp_at(c.pages, c.n_kv, max(slot[i], 0), 0) + which * page;
         }
-        uint4* dst = reinterpret_cast<uint4*>((which ? v : k) + (size_t)i * c.n_kv * c.hd + d);
-        dst[0] = lo;
-        dst[1] = hi;
+        for (int x = lane; x < per; x += 32) {
+            const int h = x / per_head;
+            uint4 u[READ_ROWS];
+            float s[READ_ROWS];
+#pragma unroll
+            for (int i = 0; i < READ_ROWS; ++i)
+                if (slot[i] >= 0) {
+                    u[i] = ldg_nc_16(codes + ((size_t)slot[i] * per + x) * 16);
+                    s[i] = __uint_as_float((uint32_t)exps[i][(size_t)h * 2 * page] << 23);
+                } else {
+                    u[i] = make_uint4(0u, 0u, 0u, 0u);           // (a token that is not there reads as zeros)
+                    s[i] = 0.f;
+                }
+#pragma unroll
+            for (int i = 0; i < READ_ROWS; ++i) {
+                if (i0 + i >= n) continue;
+                const uint32_t in[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+                uint32_t out[8];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float2 lo = e4m3x2_to_float2((uint16_t)in[k]), hi = e4m3x2_to_float2((uint16_t)(in[k] >> 16));
+                    out[2 * k] = f2_to_bf162(lo.x * s[i], lo.y * s[i]);
+                    out[2 * k + 1] = f2_to_bf162(hi.x * s[i], hi.y * s[i]);
+                }
+                store_32(dst + ((size_t)(i0 + i) * per + x) * 16, out);
+            }
+        }
     }
 }
 
-// grid (ceil(longest / 64), R), block 256
+// grid (ceil(longest / 32), R, 2), block 256: 32 rows of keys or of values
 __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8ReadParams p) {
     pdl_grid_sync();
     const int* r = p.ranges + blockIdx.y * 4;
-    const int i0 = blockIdx.x * 64, n = min(64, r[2] - i0), out = r[3] + i0;
+    const int i0 = blockIdx.x * 32, n = min(32, r[2] - i0), out = r[3] + i0;
     if (n <= 0 || !guard_ok(p.c.pages.guard, 31, out, (long long)p.rows - n + 1)) return;
-    const size_t at = (size_t)out * p.c.n_kv * p.c.hd;
-    read_rows(p.c, r[0], r[1] + i0, n, p.k + at, p.v + at);
+    read_rows(p.c, blockIdx.z, r[0], r[1] + i0, n, (blockIdx.z ? p.v : p.k) + (size_t)out * p.c.n_kv * p.c.hd);
 }
 
-// grid (per_seq, sequences), block 256: a page of a sequence's workspace
+// grid (per_seq * 2, sequences, 2), block 256: half a page of a sequence's workspace
 __global__ void __launch_bounds__(256) kv8_unpack_kernel(Kv8UnpackParams p) {
     pdl_grid_sync();
-    const int s = blockIdx.y, page = s * p.per_seq + blockIdx.x, q0 = p.qo_indptr[s], q1 = p.qo_indptr[s + 1], most = p.per_seq * 64;
+    const int s = blockIdx.y, page = s * p.per_seq + (blockIdx.x >> 1), q0 = p.qo_indptr[s], q1 = p.qo_indptr[s + 1], most = p.per_seq * 64;
     if (q0 >= q1) return;
     int n = p.positions[q1 - 1] + 1;                 // positions ascend within a sequence
     if (!guard_ok(p.c.pages.guard, 33, n, (long long)most + 1)) n = most;
-    if (threadIdx.x == 0) p.table[page] = page;
-    if (blockIdx.x == 0)
+    if (blockIdx.z == 0 && (blockIdx.x & 1) == 0 && threadIdx.x == 0) p.table[page] = page;
+    if (blockIdx.x == 0 && blockIdx.z == 0)
         for (int t = q0 + threadIdx.x; t < q1; t += 256) {
             p.rows_out[t] = s;
             p.positions_out[t] = min(p.positions[t], most - 1);
         }
-    const int i0 = blockIdx.x * 64;
-    n = min(64, n - i0);
+    const int i0 = blockIdx.x * 32;
+    n = min(32, n - i0);
     if (n <= 0) return;
-    const size_t at = (size_t)page * 64 * p.c.n_kv * p.c.hd;
-    read_rows(p.c, p.batch_idx[q0], i0, n, p.k + at, p.v + at);
+    read_rows(p.c, blockIdx.z, p.batch_idx[q0], i0, n, (blockIdx.z ? p.v : p.k) + ((size_t)s * most + i0) * p.c.n_kv * p.c.hd);
 }
 
 }  // namespace
@@ -217,35 +261,37 @@ SL_API int sl_kv8_store(const Kv8StoreParams* p, int T, cudaStream_t s) {
     if (T == 0) return 0;
     if (p->hd < 16 || p->hd > 256 || p->hd % 16 != 0 || p->rot_dims < 0 || p->rot_dims > p->hd || p->rot_dims % 2 != 0 || p->n_kv < 1 || p->n_heads < 1) return -1;
     if ((((uintptr_t)p->k_codes | (uintptr_t)p->v_codes | (uintptr_t)p->q_out) & 15) != 0 || p->pages.page_size < 1) return -1;
-    const int P = p->hd <= 64 ? 2 : p->hd <= 128 ? 4 : 8, jobs = p->n_heads + 2 * p->n_kv;
+    const int L = p->hd <= 64 ? 8 : p->hd <= 128 ? 16 : 32, at_once = 8 * 32 / L, jobs = p->n_heads + 2 * p->n_kv;
     const uintptr_t at = (uintptr_t)p->q | (uintptr_t)p->k | (uintptr_t)p->v | (uintptr_t)p->q_norm | (uintptr_t)p->k_norm;
-    const bool vec = at % (2 * P) == 0 && (p->ldq | p->ldk | p->ldv | p->q_stride) % P == 0;
-    const dim3 grid(T, T < 512 ? (jobs + 7) / 8 : 1);                // few tokens: a warp per row; many: the angles once a token
-#define SL_KS(PP)                                                                       \
-    {                                                                                   \
-        if (vec) sl_launch(kv8_store_kernel<PP, true>, grid, 256, 0, s, *p);            \
-        else sl_launch(kv8_store_kernel<PP, false>, grid, 256, 0, s, *p);               \
+    const bool vec = at % 16 == 0 && (p->ldq | p->ldk | p->ldv | p->q_stride) % 8 == 0, even = p->rot_dims % 16 == 0;
+    const dim3 grid(T, T < 512 ? (jobs + at_once - 1) / at_once : 1);            // few tokens: a warp's rows each; many: the angles once a token
+#define SL_KS(LL)                                                                                  \
+    {                                                                                              \
+        if (vec && even) sl_launch(kv8_store_kernel<LL, true, true>, grid, 256, 0, s, *p);         \
+        else if (vec) sl_launch(kv8_store_kernel<LL, true, false>, grid, 256, 0, s, *p);           \
+        else if (even) sl_launch(kv8_store_kernel<LL, false, true>, grid, 256, 0, s, *p);          \
+        else sl_launch(kv8_store_kernel<LL, false, false>, grid, 256, 0, s, *p);                   \
     }
-    if (P == 2) SL_KS(2) else if (P == 4) SL_KS(4) else SL_KS(8)
+    if (L == 8) SL_KS(8) else if (L == 16) SL_KS(16) else SL_KS(32)
 #undef SL_KS
     return SL_LAUNCH_CHECK();
 }
 
 static bool kv8_rows_ok(const Kv8Rows& c, const void* k, const void* v) {
     return c.hd >= 16 && c.hd % 16 == 0 && c.n_kv >= 1 && c.pages.page_size >= 1 &&
-           (((uintptr_t)c.k_codes | (uintptr_t)c.v_codes | (uintptr_t)k | (uintptr_t)v) & 15) == 0;
+           (((uintptr_t)c.k_codes | (uintptr_t)c.v_codes) & 15) == 0 && (((uintptr_t)k | (uintptr_t)v) & 31) == 0;
 }
 
 SL_API int sl_kv8_read(const Kv8ReadParams* p, int ranges, int longest, cudaStream_t s) {
     if (ranges == 0 || longest <= 0) return 0;
     if (!kv8_rows_ok(p->c, p->k, p->v) || ranges > 65535) return -1;
-    sl_launch(kv8_read_kernel, dim3((longest + 63) / 64, ranges), 256, 0, s, *p);
+    sl_launch(kv8_read_kernel, dim3((longest + 31) / 32, ranges, 2), 256, 0, s, *p);
     return SL_LAUNCH_CHECK();
 }
 
 SL_API int sl_kv8_unpack(const Kv8UnpackParams* p, int sequences, cudaStream_t s) {
     if (sequences == 0) return 0;
     if (!kv8_rows_ok(p->c, p->k, p->v) || sequences > 65535 || p->per_seq < 1) return -1;
-    sl_launch(kv8_unpack_kernel, dim3(p->per_seq, sequences), 256, 0, s, *p);
+    sl_launch(kv8_unpack_kernel, dim3(p->per_seq * 2, sequences, 2), 256, 0, s, *p);
     return SL_LAUNCH_CHECK();
 }
