@@ -20,22 +20,19 @@ struct Kv8StoreParams {
     float eps;
     bf16* q_out;                     // [T, n_heads, hd]
     uint8_t *k_codes, *v_codes, *exps;
+    int T;
 };
 
-constexpr double TWO_PI = 6.283185307179586476925;
-
-// 8 bf16 values; VEC: 16 bytes at once
+// 4 bf16 values; VEC: 8 bytes at once
 template <bool VEC>
-__device__ __forceinline__ uint4 load8(const bf16* p) {
-    if (VEC) return *reinterpret_cast<const uint4*>(p);
+__device__ __forceinline__ uint2 load4(const bf16* p) {
+    if (VEC) return *reinterpret_cast<const uint2*>(p);
     const uint16_t* u = reinterpret_cast<const uint16_t*>(p);
-    uint32_t w[4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i) w[i] = (uint32_t)u[2 * i] | (uint32_t)u[2 * i + 1] << 16;
-    return make_uint4(w[0], w[1], w[2], w[3]);
+    return make_uint2((uint32_t)u[0] | (uint32_t)u[1] << 16, (uint32_t)u[2] | (uint32_t)u[3] << 16);
 }
-__device__ __forceinline__ void unpack8(const uint4& u, float (&x)[8]) {
-    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+struct Raw { uint2 a, b; };
+__device__ __forceinline__ void unpack(const Raw& r, float (&x)[8]) {
+    const uint32_t w[4] = {r.a.x, r.a.y, r.b.x, r.b.y};
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const float2 f = bf162_to_f2(w[i]);
@@ -44,114 +41,165 @@ __device__ __forceinline__ void unpack8(const uint4& u, float (&x)[8]) {
     }
 }
 
-// grid (T, y), block 256.  A row of a head (queries, then keys, then values) has L lanes of 8 neighbouring values, a warp 32 / L rows at a time; a lane
-// keeps the angles and weights of its values for all rows.  VEC: rows are aligned to 16 bytes.  EVEN: partners of a rotation are whole lanes
-// apart (shuffles), else they come through shared memory.
+enum Kind { QUERY, KEY, VALUE };
+
+// A row of a head has L lanes of 8 values, a warp 32 / L rows of one kind at a time; a lane keeps the angles and weights of its values for all rows.
+// EVEN: four of a lane's values and the four that they turn with, so a rotation stays in the lane; else eight neighbours, whose partners come
+// through shared memory.  VEC: rows are aligned to 8 bytes.
 template <int L, bool VEC, bool EVEN>
-__global__ void __launch_bounds__(256) kv8_store_kernel(Kv8StoreParams p) {
-    pdl_grid_sync();
-    constexpr int ROWS = 32 / L, AT_ONCE = 8 * ROWS;
-    __shared__ float2 turn[128];                     // (cos, sin) of each pair
-    __shared__ float part[EVEN ? 1 : 8][EVEN ? 1 : 256];
-    const int t = blockIdx.x, lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = p.rot_dims / 2, jobs = p.n_heads + 2 * p.n_kv;
-    const int own = lane % L, d0 = own * 8, step = gridDim.y * AT_ONCE;
-    const bool on = d0 < p.hd;
-    auto source = [&](int job) {
-        return (job < p.n_heads ? p.q + (size_t)t * p.ldq + (size_t)job * p.q_stride
-                : job < p.n_heads + p.n_kv ? p.k + (size_t)t * p.ldk + (size_t)(job - p.n_heads) * p.hd
-                                           : p.v + (size_t)t * p.ldv + (size_t)(job - p.n_heads - p.n_kv) * p.hd) + d0;
-    };
-    int job = (blockIdx.y * 8 + warp) * ROWS + lane / L;
-    const uint4 none = make_uint4(0u, 0u, 0u, 0u);
-    uint4 next = on && job < jobs ? load8<VEC>(source(job)) : none;
-    const uint4 wq = on && p.q_norm != nullptr ? load8<VEC>(p.q_norm + d0) : none, wk = on && p.k_norm != nullptr ? load8<VEC>(p.k_norm + d0) : none;
-    const int pos = p.positions[t], b = p.batch_idx[t];
-    // fp32 keeps no digits of the angle of a far position: the product and its remainder are taken in 64 bits
-    for (int i = threadIdx.x; i < half; i += 256) {
-        const double a = (double)pos * (double)p.freq[i];
-        float sn, cs;
-        sincosf((float)fma(-rint(a * (1.0 / TWO_PI)), TWO_PI, a), &sn, &cs);
-        turn[i] = make_float2(cs * p.gain, sn * p.gain);
+struct Writer {
+    static constexpr int ROWS = 32 / L;
+    const Kv8StoreParams& p;
+    int t, slot;                                     // token, its slot or -1
+    int da, db, sub;                                 // the lane's first and fifth value, row of the warp's
+    bool on, turning;                                // the lane has values; they are pairs of the rotation (EVEN)
+    float* part;                                     // 256 values of the warp (not EVEN)
+    float cs[EVEN ? 4 : 8], sn[EVEN ? 4 : 8];
+
+    template <int KIND>
+    __device__ __forceinline__ Raw fetch(int h) const {
+        const int n = KIND == QUERY ? p.n_heads : p.n_kv;
+        if (!on || h >= n) return {make_uint2(0u, 0u), make_uint2(0u, 0u)};
+        const bf16* src = KIND == QUERY ? p.q + ((size_t)t * p.ldq + (size_t)h * p.q_stride)
+                                        : (KIND == KEY ? p.k + (size_t)t * p.ldk : p.v + (size_t)t * p.ldv) + (size_t)h * p.hd;
+        return {load4<VEC>(src + da), load4<VEC>(src + db)};
     }
-    const int slot = pos < 0 ? -1 : kv8_slot(p.pages, 30, b, pos);
-    __syncthreads();
-    float cs[8], sn[8];                              // value' = value * cs + partner * sn
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int d = d0 + i;
-        const float2 a = d < p.rot_dims ? turn[d < half ? d : d - half] : make_float2(1.f, 0.f);
-        cs[i] = a.x;
-        sn[i] = d < half ? -a.y : a.y;
-    }
-    const int partner = EVEN ? lane + (d0 < half ? half / 8 : d0 < p.rot_dims ? -half / 8 : 0) : 0;
-    for (int base = blockIdx.y * AT_ONCE; base < jobs; base += step, job += step) {          // (warps stay together: shuffles)
+    // Row `h` of the lane, which `raw` holds.
+    template <int KIND>
+    __device__ __forceinline__ void row(int h, const Raw& raw, const float (&g)[8], bool normed, float per) const {
         float x[8];
-        unpack8(next, x);
-        const bool there = job < jobs, query = job < p.n_heads, key = !query && job < p.n_heads + p.n_kv;
-        next = on && job + step < jobs ? load8<VEC>(source(job + step)) : none;
-        if (p.q_norm != nullptr || p.k_norm != nullptr) {
+        unpack(raw, x);
+        const bool there = on && h < (KIND == QUERY ? p.n_heads : p.n_kv);
+        if (KIND != VALUE && normed) {
             float ss = 0.f;
 #pragma unroll
             for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
 #pragma unroll
             for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            if ((query && p.q_norm != nullptr) || (key && p.k_norm != nullptr)) {
-                const float inv = 1.f / sqrtf(ss / (float)p.hd + p.eps);
-                float g[8];
-                unpack8(query ? wq : wk, g);
+            const float inv = rsqrtf(fmaf(ss, per, p.eps));
 #pragma unroll
-                for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * g[i];
-            }
+            for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * g[i];
         }
-        if (half > 0) {
-            float y[8];
-            if (EVEN) {
+        if (KIND != VALUE && EVEN) {
+            if (turning) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) y[i] = __shfl_sync(0xffffffffu, x[i], partner);
-            } else {
-                __syncwarp();
-#pragma unroll
-                for (int i = 0; i < 8; ++i) part[EVEN ? 0 : warp][EVEN ? 0 : lane * 8 + i] = x[i];
-                __syncwarp();
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    const int d = d0 + i, other = d < half ? half : d < p.rot_dims ? -half : 0;
-                    y[i] = part[EVEN ? 0 : warp][EVEN ? 0 : lane * 8 + i + other];
+                for (int i = 0; i < 4; ++i) {
+                    const float a = x[i], b = x[4 + i];
+                    x[i] = a * cs[i] - b * sn[i];
+                    x[4 + i] = b * cs[i] + a * sn[i];
                 }
             }
-            if (query || key)
+        } else if (KIND != VALUE && p.rot_dims > 0) {
+            const int half = p.rot_dims / 2, at = (threadIdx.x & 31) * 8;
+            __syncwarp();
 #pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (d0 + i < p.rot_dims) x[i] = x[i] * cs[i] + y[i] * sn[i];
+            for (int i = 0; i < 8; ++i) part[at + i] = x[i];
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int d = da + i;
+                const float y = part[at + i + (d < half ? half : d < p.rot_dims ? -half : 0)];
+                if (d < half) x[i] = x[i] * cs[EVEN ? 0 : i] - y * sn[EVEN ? 0 : i];
+                else if (d < p.rot_dims) x[i] = x[i] * cs[EVEN ? 0 : i] + y * sn[EVEN ? 0 : i];
+            }
         }
-        if (there && query && on)
-            *reinterpret_cast<uint4*>(p.q_out + ((size_t)t * p.n_heads + job) * p.hd + d0) =
-                make_uint4(f2_to_bf162(x[0], x[1]), f2_to_bf162(x[2], x[3]), f2_to_bf162(x[4], x[5]), f2_to_bf162(x[6], x[7]));
-        if (base + AT_ONCE <= p.n_heads) continue;               // no keys or values among these rows
-        float top = 0.f;                                         // of the finite values
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            if (!(fabsf(x[i]) <= FLT_MAX)) x[i] = __int_as_float(0x7fc00000);
-            else top = fmaxf(top, fabsf(x[i]));
+        if (KIND == QUERY) {
+            if (there) {
+                bf16* dst = p.q_out + ((size_t)t * p.n_heads + h) * p.hd;
+                *reinterpret_cast<uint2*>(dst + da) = make_uint2(f2_to_bf162(x[0], x[1]), f2_to_bf162(x[2], x[3]));
+                *reinterpret_cast<uint2*>(dst + db) = make_uint2(f2_to_bf162(x[4], x[5]), f2_to_bf162(x[6], x[7]));
+            }
+            return;
         }
+        uint32_t top = 0u;                           // magnitudes compare like integers; infinities and NaN are the largest
+        constexpr uint32_t INF = 0x7f800000u;
 #pragma unroll
-        for (int o = L / 2; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-        if (!there || query || slot < 0) continue;
+        for (int i = 0; i < 8; ++i) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+#pragma unroll
+        for (int o = L / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (__any_sync(0xffffffffu, top >= INF)) {   // values that are not finite are NaN, and the others make the scale
+            top = 0u;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t m = __float_as_uint(x[i]) & 0x7fffffffu;
+                if (m >= INF) x[i] = __int_as_float(0x7fc00000);
+                else top = max(top, m);
+            }
+#pragma unroll
+            for (int o = L / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+        }
+        if (!there || slot < 0) return;
         // top = m 2^n with m in [1, 2), 448 = 1.75 * 2^8
-        const uint32_t bits = __float_as_uint(top);
-        const int e = min(KV8_HIGH, max(KV8_LOW, (int)(bits >> 23) - 127 - 8 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0)));
+        const int e = min(KV8_HIGH, max(KV8_LOW, (int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0)));
         const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
-        const int h = job - p.n_heads - (key ? 0 : p.n_kv);
-        if (on) {
-            uint32_t c[2];
+        uint32_t c[2];
 #pragma unroll
-            for (int i = 0; i < 8; i += 4)
-                c[i / 4] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[i] * inv, x[i + 1] * inv), __NV_SATFINITE, __NV_E4M3) |
-                           (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[i + 2] * inv, x[i + 3] * inv), __NV_SATFINITE, __NV_E4M3) << 16;
-            *reinterpret_cast<uint2*>((key ? p.k_codes : p.v_codes) + ((size_t)slot * p.n_kv + h) * p.hd + d0) = make_uint2(c[0], c[1]);
-        }
-        if (own == 0) p.exps[kv8_exp_at(p.pages, p.n_kv, slot, h) + (key ? 0 : p.pages.page_size)] = (uint8_t)(e + KV8_BIAS);
+        for (int i = 0; i < 8; i += 4)
+            c[i / 4] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[i] * inv, x[i + 1] * inv), __NV_SATFINITE, __NV_E4M3) |
+                       (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[i + 2] * inv, x[i + 3] * inv), __NV_SATFINITE, __NV_E4M3) << 16;
+        uint8_t* dst = (KIND == KEY ? p.k_codes : p.v_codes) + ((size_t)slot * p.n_kv + h) * p.hd;
+        *reinterpret_cast<uint32_t*>(dst + da) = c[0];
+        *reinterpret_cast<uint32_t*>(dst + db) = c[1];
+        if (da == 0) p.exps[kv8_exp_at(p.pages, p.n_kv, slot, h) + (KIND == KEY ? 0 : p.pages.page_size)] = (uint8_t)(e + KV8_BIAS);
     }
+    // Heads (u, u + step, ..) * ROWS + sub of a kind; the rows of two steps are on their way.
+    template <int KIND>
+    __device__ __forceinline__ void rows(int u, int step, Raw next) const {
+        const int n = KIND == QUERY ? p.n_heads : p.n_kv;
+        if (u * ROWS >= n) return;
+        const bf16* w = KIND == QUERY ? p.q_norm : KIND == KEY ? p.k_norm : nullptr;
+        Raw then = fetch<KIND>((u + step) * ROWS + sub);
+        float g[8] = {};
+        if (on && w != nullptr) unpack(Raw{load4<VEC>(w + da), load4<VEC>(w + db)}, g);
+        const float per = 1.f / (float)p.hd;
+        for (; u * ROWS < n; u += step) {
+            const Raw now = next;
+            next = then;
+            then = fetch<KIND>((u + 2 * step) * ROWS + sub);
+            row<KIND>(u * ROWS + sub, now, g, w != nullptr, per);
+        }
+    }
+};
+
+// `share` warps to a token, which make its angles for themselves (a block that waits for them waits longer than they take) and take every share-th
+// step of its queries, keys and values.  Grid ceil(T * share / 8), block 256.
+template <int L, bool VEC, bool EVEN>
+__global__ void __launch_bounds__(256, 4) kv8_store_kernel(Kv8StoreParams p, int share) {
+    pdl_grid_sync();
+    using W = Writer<L, VEC, EVEN>;
+    __shared__ float2 turns[8][128];                 // (cos, sin) of each pair
+    __shared__ float part[EVEN ? 1 : 8][EVEN ? 1 : 256];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = p.rot_dims / 2, own = lane % L;
+    const long long id = (long long)blockIdx.x * 8 + warp;
+    const int t = (int)(id / share), mine = (int)(id - (long long)t * share);
+    if (t >= p.T) return;
+    const bool turning = EVEN && own * 8 < p.rot_dims;
+    W w{p, t, -1, turning ? own * 4 : own * 8, turning ? half + own * 4 : own * 8 + 4, lane / L, own * 8 < p.hd, turning, part[EVEN ? 0 : warp]};
+    // steps are numbered through queries, keys and values: this warp's first ones
+    const int uq = (p.n_heads + W::ROWS - 1) / W::ROWS, uk = (p.n_kv + W::ROWS - 1) / W::ROWS;
+    const int q0 = mine, k0 = (mine + share - uq % share) % share, v0 = (k0 + share - uk % share) % share;
+    const Raw q = w.template fetch<QUERY>(q0 * W::ROWS + w.sub), k = w.template fetch<KEY>(k0 * W::ROWS + w.sub), v = w.template fetch<VALUE>(v0 * W::ROWS + w.sub);
+    const int pos = p.positions[t], b = p.batch_idx[t];
+    // fp32 keeps no digits of the angle of a far position: turns and their remainder are taken in 64 bits
+    float2* const turn = turns[warp];
+    for (int i = lane; i < half; i += 32) {
+        const double a = (double)pos * (double)p.freq[i] * 0.15915494309189533577;           // 1 / (2 pi)
+        float sn, cs;
+        sincospif(2.f * (float)(a - rint(a)), &sn, &cs);
+        turn[i] = make_float2(cs * p.gain, sn * p.gain);
+    }
+    if (pos >= 0) w.slot = kv8_slot(p.pages, 30, b, pos);
+    __syncwarp();
+#pragma unroll
+    for (int i = 0; i < (EVEN ? 4 : 8); ++i) {
+        const int d = w.da + i;
+        const float2 a = d < half ? turn[d] : d < p.rot_dims ? turn[d - half] : make_float2(1.f, 0.f);
+        w.cs[i] = a.x;
+        w.sn[i] = a.y;
+    }
+    w.template rows<QUERY>(q0, share, q);
+    w.template rows<KEY>(k0, share, k);
+    w.template rows<VALUE>(v0, share, v);
 }
 
 struct Kv8Rows {
@@ -255,22 +303,29 @@ __global__ void __launch_bounds__(256) kv8_unpack_kernel(Kv8UnpackParams p) {
     read_rows(p.c, blockIdx.z, p.batch_idx[q0], i0, n, (blockIdx.z ? p.v : p.k) + ((size_t)s * most + i0) * p.c.n_kv * p.c.hd);
 }
 
+constexpr int WARPS_WANTED = 148 * 32;
+
 }  // namespace
 
 SL_API int sl_kv8_store(const Kv8StoreParams* p, int T, cudaStream_t s) {
     if (T == 0) return 0;
     if (p->hd < 16 || p->hd > 256 || p->hd % 16 != 0 || p->rot_dims < 0 || p->rot_dims > p->hd || p->rot_dims % 2 != 0 || p->n_kv < 1 || p->n_heads < 1) return -1;
     if ((((uintptr_t)p->k_codes | (uintptr_t)p->v_codes | (uintptr_t)p->q_out) & 15) != 0 || p->pages.page_size < 1) return -1;
-    const int L = p->hd <= 64 ? 8 : p->hd <= 128 ? 16 : 32, at_once = 8 * 32 / L, jobs = p->n_heads + 2 * p->n_kv;
+    const int L = p->hd <= 64 ? 8 : p->hd <= 128 ? 16 : 32, rows = 32 / L, steps = (p->n_heads + rows - 1) / rows + 2 * ((p->n_kv + rows - 1) / rows);
     const uintptr_t at = (uintptr_t)p->q | (uintptr_t)p->k | (uintptr_t)p->v | (uintptr_t)p->q_norm | (uintptr_t)p->k_norm;
-    const bool vec = at % 16 == 0 && (p->ldq | p->ldk | p->ldv | p->q_stride) % 8 == 0, even = p->rot_dims % 16 == 0;
-    const dim3 grid(T, T < 512 ? (jobs + at_once - 1) / at_once : 1);            // few tokens: a warp's rows each; many: the angles once a token
-#define SL_KS(LL)                                                                                  \
-    {                                                                                              \
-        if (vec && even) sl_launch(kv8_store_kernel<LL, true, true>, grid, 256, 0, s, *p);         \
-        else if (vec) sl_launch(kv8_store_kernel<LL, true, false>, grid, 256, 0, s, *p);           \
-        else if (even) sl_launch(kv8_store_kernel<LL, false, true>, grid, 256, 0, s, *p);          \
-        else sl_launch(kv8_store_kernel<LL, false, false>, grid, 256, 0, s, *p);                   \
+    const bool vec = at % 8 == 0 && (p->ldq | p->ldk | p->ldv | p->q_stride) % 4 == 0, even = p->rot_dims % 8 == 0;
+    Kv8StoreParams q = *p;
+    q.T = T;
+    // warps for all sub-cores, if there are steps for them
+    const int share = max(1, min(steps, WARPS_WANTED / T));
+    const long long blocks = ((long long)T * share + 7) / 8;
+    if (blocks > 0x7fffffff) return -1;
+#define SL_KS(LL)                                                                                          \
+    {                                                                                                      \
+        if (vec && even) sl_launch(kv8_store_kernel<LL, true, true>, (unsigned)blocks, 256, 0, s, q, share);         \
+        else if (vec) sl_launch(kv8_store_kernel<LL, true, false>, (unsigned)blocks, 256, 0, s, q, share);           \
+        else if (even) sl_launch(kv8_store_kernel<LL, false, true>, (unsigned)blocks, 256, 0, s, q, share);          \
+        else sl_launch(kv8_store_kernel<LL, false, false>, (unsigned)blocks, 256, 0, s, q, share);                   \
     }
     if (L == 8) SL_KS(8) else if (L == 16) SL_KS(16) else SL_KS(32)
 #undef SL_KS

@@ -37,7 +37,7 @@ class Kv8StoreParams(C.Structure):
                 ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("freq", C.c_void_p), ("gain", C.c_float), ("rot_dims", C.c_int),
                 ("positions", C.c_void_p), ("batch_idx", C.c_void_p), *_PAGES, ("n_heads", C.c_int), ("n_kv", C.c_int),
                 ("hd", C.c_int), ("q_stride", C.c_int), ("eps", C.c_float), ("q_out", C.c_void_p), ("k_codes", C.c_void_p),
-                ("v_codes", C.c_void_p), ("exps", C.c_void_p)]
+                ("v_codes", C.c_void_p), ("exps", C.c_void_p), ("T", C.c_int)]
 
 
 class Kv8ReadParams(C.Structure):
