@@ -86,7 +86,7 @@ def mixer_rows(emit, tokens, iters: int, flush, peaks, dev, h: int = 16, dk: int
     windowed grouped-query attention, GLA, mLSTM and latent attention beside Gated DeltaNet and paged grouped-query attention.  More than 64 tokens: one prompt; fewer: that many sequences of `context` tokens decode one each."""
     import types
     from ..models.glm_moe_dsa import StepState
-    from ..ops import delta as DL, delta_chunk as DC, dense as D, get_ops, grouped as G, latent as L, recurrent as RC, shift as SH, talking as TK
+    from ..ops import delta as DL, delta_chunk as DC, dense as D, get_ops, grouped as G, kv8 as K8, latent as L, recurrent as RC, shift as SH, talking as TK
     from ..ops.rotary import AngleTable, rotary_table
     ops = get_ops(types.SimpleNamespace(rms_norm_eps=1e-6), dev)
     g = torch.Generator(device=dev).manual_seed(3)
@@ -220,6 +220,17 @@ def mixer_rows(emit, tokens, iters: int, flush, peaks, dev, h: int = 16, dk: int
         us = time_op(lambda: D.qk_norm_rope_cache(qk[:, :h * 128], qk[:, h * 128:(h + n_kv) * 128], qk[:, (h + n_kv) * 128:], None, None, st.positions,
                                                   st.batch_idx, pt, 64, kc, vc, h, n_kv, 128, 64, 1e6, 1e-6), iters, flush)
         emit(roofline_row("qk_norm_rope_cache", T, us, 4 * T * (h + 2 * n_kv) * 128, 0.0, peaks))
+        # the same over the 8-bit cache
+        k8, q8rot = K8.Kv8Cache.allocate(B * width, 64, n_kv, 128, dev), rotary_table(64, 1e6).to(dev)
+        us = time_op(lambda: K8.kv8_store(qk[:, :h * 128], qk[:, h * 128:(h + n_kv) * 128], qk[:, (h + n_kv) * 128:], None, None, q8rot, st.positions,
+                                          st.batch_idx, pt, k8, h, 1e-6), iters, flush)
+        emit(roofline_row("kv8_store", T, us, T * 128 * (4 * h + 6 * n_kv), 0.0, peaks))
+        us = time_op(lambda: K8.kv8_attention(q, k8, st.positions, st.batch_idx, pt, 128 ** -0.5, qo_indptr=qo if prompt else None, max_q=T,
+                                              max_kv_len=kv), iters, flush)
+        emit(roofline_row("kv8_attention (full context)", T, us, (T if prompt else T * kv) * n_kv * 258 + 4.0 * T * h * 128, 4.0 * full * h * 128, peaks))
+        ranges = torch.tensor([[b, 0, kv, b * kv] for b in range(B)], dtype=torch.int32, device=dev)
+        us = time_op(lambda: K8.kv8_read(k8, ranges, B * kv, kv, pt), iters, flush)
+        emit(roofline_row("kv8_read", B * kv, us, B * kv * n_kv * (258 + 512), 0.0, peaks))
         # talking heads in chunks and over the whole context, the join with the token shift, the activation of an ungated feed-forward
         for what, chunk in (("chunk", window), ("full context", 0)):
             ts = TK.TalkingShape(h, n_kv, h, n_kv, 128, 128, 128 ** -0.5, chunk, 1e-6)

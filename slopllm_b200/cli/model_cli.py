@@ -28,6 +28,9 @@ def add_model_args(ap: argparse.ArgumentParser) -> None:
     ap.add_argument("--dtype", choices=("bfloat16", "float32"), default=None,
                     help="activation and weight type; default bfloat16 on a GPU.  float32 (no reduced-precision products) for the "
                          "families that have it")
+    ap.add_argument("--kv-dtype", choices=("auto", "e4m3"), default="auto",
+                    help="type of cached keys and values: auto is the model's own; e4m3 keeps them in 8 bits with a scale per token and key head, "
+                         "for about half of the cache's bytes (qwen3, qwen3_5)")
     ap.add_argument("--gpus", default="", help="comma-separated device list; its length must equal the number of ranks")
     ap.add_argument("--arena", type=float, default=0.0,
                     help="GiB of device memory this process may allocate per GPU (weights + KV cache + step buffers); a larger "
@@ -129,7 +132,7 @@ def check_memory_plan(args, ctx: ParallelContext, model_dir: str, model_type: st
         with open(os.path.join(model_dir, "config.json")) as f:
             dcfg = DenseConfig.from_hf_dict(json.load(f))
         p = plan_dense(dcfg, world=ctx.world, batch_size=args.batch_size, chunk_size=args.chunk_size, max_pages=args.max_pages,
-                       arena_gb=args.arena, device_gb=total / GIB)
+                       arena_gb=args.arena, device_gb=total / GIB, kv_dtype=_kv_dtype(args))
     if p.requested_fits:
         return None
     msg = (f"memory plan: {p.weights_bytes / GIB:.1f} GiB of weights per rank + about {p.workspace_bytes / GIB:.1f} GiB of "
@@ -140,11 +143,18 @@ def check_memory_plan(args, ctx: ParallelContext, model_dir: str, model_type: st
     return msg
 
 
-def _random_model(spec: str, ctx: ParallelContext, mtp: int, dtype_name: Optional[str] = None):
+def _kv_dtype(args) -> Optional[str]:
+    name = getattr(args, "kv_dtype", "auto")
+    return None if name == "auto" else name
+
+
+def _random_model(spec: str, ctx: ParallelContext, mtp: int, dtype_name: Optional[str] = None, kv_dtype: Optional[str] = None):
     from ..parallel.fused import make_comm
     dtype = torch.bfloat16 if ctx.device.type == "cuda" else torch.float32
     from ..models.registry import hybrid_family
     family = hybrid_family(spec)
+    if kv_dtype is not None and not spec.startswith("qwen"):
+        raise SystemExit(f"--random-init {spec} does not cache keys and values in {kv_dtype}")
     if family is not None:
         cfg = family.config.tiny()
         model = family.model.from_tensors(cfg, family.random_tensors(cfg), ctx, getattr(torch, dtype_name) if dtype_name else dtype)
@@ -157,7 +167,7 @@ def _random_model(spec: str, ctx: ParallelContext, mtp: int, dtype_name: Optiona
         from ..models.dense import DenseConfig, DenseModel, random_dense_model
         cfg = DenseConfig.tiny(hybrid=spec.startswith("qwen35"))
         w, _ = random_dense_model(cfg, 0, ctx.device, dtype, tp_rank, tp_world)
-        return cfg, DenseModel(cfg, w, ctx), cfg.model_type
+        return cfg, DenseModel(cfg, w, ctx, kv_dtype=kv_dtype), cfg.model_type
     from ..models.glm_moe_dsa import GlmMoeDsaModel
     from ..models.weights import random_model
     if spec.startswith("glm5"):
@@ -185,7 +195,7 @@ def build_runtime(args, with_scheduler: bool = True) -> Runtime:
         os.environ["SLOPLLM_B200_FUSED"] = "0"
     model_dir: Optional[str] = None
     if args.random_init:
-        cfg, model, model_type = _random_model(args.random_init, ctx, args.mtp, getattr(args, "dtype", None))
+        cfg, model, model_type = _random_model(args.random_init, ctx, args.mtp, getattr(args, "dtype", None), _kv_dtype(args))
     else:
         if not args.model:
             raise SystemExit("give --model DIR|HUB_ID or --random-init SPEC")
@@ -195,7 +205,7 @@ def build_runtime(args, with_scheduler: bool = True) -> Runtime:
             args.max_model_len = max_position_embeddings(model_dir)
         model_type, reg, _ = inspect_model(model_dir, cp=args.cp, mtp=args.mtp)
         check_memory_plan(args, ctx, model_dir, model_type)
-        cfg, model = load_registered(reg, model_dir, ctx, args.mtp, getattr(args, "dtype", None))
+        cfg, model = load_registered(reg, model_dir, ctx, args.mtp, getattr(args, "dtype", None), _kv_dtype(args))
     if getattr(args, "max_model_len", None) is None:
         args.max_model_len = 65536
     if getattr(cfg, "max_positions", 0):

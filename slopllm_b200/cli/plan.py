@@ -57,6 +57,7 @@ def main(argv=None) -> int:
     ap.add_argument("--max-pages", type=int, default=0)
     ap.add_argument("--arena", type=float, default=0.0, help="GiB the process may allocate (0: the whole device)")
     ap.add_argument("--device-gb", type=float, default=180.0, help="device memory in GiB when --arena is not given")
+    ap.add_argument("--kv-dtype", choices=("auto", "e4m3"), default="auto", help="type of cached keys and values (qwen3, qwen3_5)")
     ap.add_argument("--context", type=int, default=0, help="longest sequence assumed for the workspace estimate")
     args = ap.parse_args(argv)
     cfg = _config(args)
@@ -64,9 +65,15 @@ def main(argv=None) -> int:
         from ..models.registry import hybrid_family
         from ..utils.sizing import plan_dense
         family = hybrid_family(cfg.model_type)
-        planner = plan_dense if family is None else family.plan
+        planner, more = plan_dense if family is None else family.plan, {}
+        if args.kv_dtype != "auto":
+            if family is not None:
+                raise SystemExit(f"plan: {cfg.model_type} does not cache keys and values in {args.kv_dtype}")
+            more = {"kv_dtype": args.kv_dtype}
         p = planner(cfg, world=args.world, batch_size=args.batch_size, chunk_size=args.chunk_size, max_pages=args.max_pages,
-                       arena_gb=args.arena, device_gb=args.device_gb)
+                    arena_gb=args.arena, device_gb=args.device_gb, **more)
+    elif args.kv_dtype != "auto":
+        raise SystemExit(f"plan: glm_moe_dsa does not cache keys and values in {args.kv_dtype}")
     else:
         p = plan_memory(cfg, world=args.world, cp=args.cp, ep=args.ep, mtp=args.mtp, batch_size=args.batch_size,
                         chunk_size=args.chunk_size, max_pages=args.max_pages, arena_gb=args.arena, device_gb=args.device_gb,

@@ -17,11 +17,12 @@ from ..config import PAGE_SIZE
 
 @dataclass(frozen=True)
 class CacheSpec:
-    """What one layer keeps: shapes of its per-token rows (stored in the cache's row type) and of its per-sequence state
-    (always fp32, zero at the start of a sequence)."""
+    """What one layer keeps: shapes of its per-token rows (stored in the cache's row type, or in one of their own) and of its
+    per-sequence state (always fp32, zero at the start of a sequence)."""
 
     rows: Dict[str, Tuple[int, ...]] = field(default_factory=dict)
     state: Dict[str, Tuple[int, ...]] = field(default_factory=dict)
+    row_types: Dict[str, torch.dtype] = field(default_factory=dict)
 
     def row_values(self) -> int:
         return sum(_numel(s) for s in self.rows.values())
@@ -45,7 +46,8 @@ class HybridCache:
         self.rows: List[Dict[str, torch.Tensor]] = []
         self.state: List[Dict[str, torch.Tensor]] = []
         for s in self.specs:
-            self.rows.append({n: torch.zeros(num_pages * PAGE_SIZE, *shape, dtype=dtype, device=device) for n, shape in s.rows.items()})
+            self.rows.append({n: torch.zeros(num_pages * PAGE_SIZE, *shape, dtype=s.row_types.get(n, dtype), device=device)
+                              for n, shape in s.rows.items()})
             self.state.append({n: torch.zeros(max_states, *shape, dtype=torch.float32, device=device) for n, shape in s.state.items()})
 
     @property

@@ -19,9 +19,11 @@ from typing import Dict, List, Optional
 
 import torch
 
+from ..config import PAGE_SIZE
 from ..kv.hybrid import CacheSpec, HybridCache
 from ..ops import dense as D
-from ..ops import get_ops, recurrent as RC
+from ..ops import get_ops, kv8 as K8, recurrent as RC
+from ..ops.rotary import rotary_table
 from ..parallel.dist import Comm, ParallelContext
 from ..utils.tracing import traced
 from .stack import DecoderStack, Sublayer, token_ranges
@@ -147,36 +149,49 @@ class DenseWeights:
     vocab_offset: int = 0
 
 
-def dense_cache_specs(cfg: DenseConfig, tp: int = 1) -> List[CacheSpec]:
-    """Paged K/V rows per full-attention layer; conv + recurrent state per linear-attention layer."""
+KV_DTYPES = ("e4m3",)      # types of cached keys and values beside the model's own
+
+
+def dense_cache_specs(cfg: DenseConfig, tp: int = 1, kv_dtype: Optional[str] = None) -> List[CacheSpec]:
+    """Paged K/V rows per full-attention layer; conv + recurrent state per linear-attention layer.  `kv_dtype` "e4m3": the rows are
+    codes, with two exponent bytes per token and key head (`ops/kv8.py`; a page's bytes are laid out by head)."""
     n_kv = max(1, cfg.num_key_value_heads // tp)
+    if kv_dtype is not None and kv_dtype not in KV_DTYPES:
+        raise ValueError(f"no cache of type {kv_dtype}; there is {', '.join(KV_DTYPES)}")
+    if kv_dtype is not None and (cfg.head_dim % 16 or cfg.head_dim > 256):
+        raise ValueError(f"the 8-bit cache takes heads of a multiple of 16 values up to 256, not {cfg.head_dim}")
     lh = max(1, cfg.linear_num_key_heads // tp)
     cdim = lh * (2 * cfg.linear_key_head_dim + cfg.linear_value_head_dim)
     full = CacheSpec(rows={"k": (n_kv, cfg.head_dim), "v": (n_kv, cfg.head_dim)})
+    if kv_dtype is not None:
+        full = CacheSpec(rows={**full.rows, "exps": (n_kv, 2)}, row_types={n: torch.uint8 for n in ("k", "v", "exps")})
     lin = CacheSpec(state={"conv": (cdim, cfg.linear_conv_kernel_dim - 1),
                            "rec": (lh, cfg.linear_key_head_dim, cfg.linear_value_head_dim)})
     return [full if kind == "full_attention" else lin for kind in cfg.layer_types]
 
 
 class DenseCache(HybridCache):
-    """:class:`HybridCache` of a Qwen3 / Qwen3.5 decoder, with the tensors by layer number."""
+    """:class:`HybridCache` of a Qwen3 / Qwen3.5 decoder, with the tensors by layer number (`kv8`: the 8-bit ones)."""
 
-    def __init__(self, cfg: DenseConfig, num_pages: int, device, tp: int = 1, max_states: int = 64, dtype=torch.bfloat16):
-        super().__init__(dense_cache_specs(cfg, tp), num_pages, device, max_states, dtype)
+    def __init__(self, cfg: DenseConfig, num_pages: int, device, tp: int = 1, max_states: int = 64, dtype=torch.bfloat16,
+                 kv_dtype: Optional[str] = None):
+        super().__init__(dense_cache_specs(cfg, tp, kv_dtype), num_pages, device, max_states, dtype)
+        self.kv8 = {i: K8.Kv8Cache(r["k"], r["v"], r["exps"].view(num_pages, -1, 2, PAGE_SIZE)) for i, r in enumerate(self.rows) if "exps" in r}
         self.k, self.v = ({i: r[n] for i, r in enumerate(self.rows) if n in r} for n in ("k", "v"))
         self.conv, self.rec = ({i: r[n] for i, r in enumerate(self.state) if n in r} for n in ("conv", "rec"))
 
 
 class DenseModel(DecoderStack):
-    """Forward pass of the Qwen3 / Qwen3.5 decoders over the paged cache."""
+    """Forward pass of the Qwen3 / Qwen3.5 decoders over the paged cache.  `kv_dtype` "e4m3": keys and values are cached in 8 bits."""
 
     norm_ahead = True
 
     def __init__(self, cfg: DenseConfig, weights: DenseWeights, ctx: Optional[ParallelContext] = None, ops=None,
-                 comm: Optional[Comm] = None):
-        self.cfg, self.w = cfg, weights
+                 comm: Optional[Comm] = None, kv_dtype: Optional[str] = None):
+        self.cfg, self.w, self.kv_dtype = cfg, weights, kv_dtype
         ctx = ctx or ParallelContext()
-        self.specs = dense_cache_specs(cfg, ctx.world)
+        self.specs = dense_cache_specs(cfg, ctx.world, kv_dtype)
+        self.rot = None if kv_dtype is None else rotary_table(cfg.rope_dim, cfg.rope_theta).to(ctx.device)
         self.sublayers = []
         for i, lw in enumerate(weights.layers):
             mixer = self._full_attention if lw.kind == "full_attention" else self._linear_attention
@@ -186,7 +201,7 @@ class DenseModel(DecoderStack):
                          torch.bfloat16 if ctx.device.type == "cuda" else torch.float32)
 
     def _make_cache(self, num_pages: int, max_states: int) -> DenseCache:
-        return DenseCache(self.cfg, num_pages, self.ctx.device, self.ctx.world, max_states, dtype=self.cache_dtype)
+        return DenseCache(self.cfg, num_pages, self.ctx.device, self.ctx.world, max_states, dtype=self.cache_dtype, kv_dtype=self.kv_dtype)
 
     # ---- layers -------------------------------------------------------------------------------------------
     @traced(lambda self, i, *a, **k: f"layer{i}.attention")
@@ -198,12 +213,18 @@ class DenseModel(DecoderStack):
         qs = cfg.head_dim * (2 if cfg.attn_output_gate else 1)
         qkv = ops.linear(x, lw.w_qkv)
         q, k, v = qkv[:, :hl * qs], qkv[:, hl * qs:hl * qs + kvl * cfg.head_dim], qkv[:, hl * qs + kvl * cfg.head_dim:]
-        q_out = D.qk_norm_rope_cache(q, k, v, lw.q_norm, lw.k_norm, st.positions, st.batch_idx, st.page_table, st.page_size,
-                                     cache.k[i], cache.v[i], hl, kvl, cfg.head_dim, cfg.rope_dim, cfg.rope_theta,
-                                     cfg.rms_norm_eps, q_stride=qs)
         qo, max_q = token_ranges(st)
-        o = D.paged_attention(q_out, cache.k[i], cache.v[i], st.positions, st.batch_idx, st.page_table, st.page_size,
-                              cfg.scaling, qo_indptr=qo, max_q=max_q, max_kv_len=st.max_kv_len)
+        if i in cache.kv8:
+            q_out = K8.kv8_store(q, k, v, lw.q_norm, lw.k_norm, self.rot, st.positions, st.batch_idx, st.page_table, cache.kv8[i], hl,
+                                 cfg.rms_norm_eps, q_stride=qs)
+            o = K8.kv8_attention(q_out, cache.kv8[i], st.positions, st.batch_idx, st.page_table, cfg.scaling, qo_indptr=qo, max_q=max_q,
+                                 max_kv_len=st.max_kv_len)
+        else:
+            q_out = D.qk_norm_rope_cache(q, k, v, lw.q_norm, lw.k_norm, st.positions, st.batch_idx, st.page_table, st.page_size,
+                                         cache.k[i], cache.v[i], hl, kvl, cfg.head_dim, cfg.rope_dim, cfg.rope_theta,
+                                         cfg.rms_norm_eps, q_stride=qs)
+            o = D.paged_attention(q_out, cache.k[i], cache.v[i], st.positions, st.batch_idx, st.page_table, st.page_size,
+                                  cfg.scaling, qo_indptr=qo, max_q=max_q, max_kv_len=st.max_kv_len)
         if cfg.attn_output_gate:
             o = D.gate_heads(o, q, qs)
         return ops.linear(o.reshape(T, hl * cfg.head_dim), lw.o_proj, out_f32=True)
@@ -397,7 +418,7 @@ def assemble_dense_weights(cfg: DenseConfig, tensors: Dict[str, torch.Tensor], d
                         vocab_offset=rank * vloc)
 
 
-def load_dense_model(model_dir: str, ctx: Optional[ParallelContext] = None, dtype=torch.bfloat16):
+def load_dense_model(model_dir: str, ctx: Optional[ParallelContext] = None, dtype=torch.bfloat16, kv_dtype: Optional[str] = None):
     """(cfg, DenseModel) from a HF directory of safetensors shards (text decoder only: `model.visual.*` is skipped)."""
     from ..checkpoint.safetensors_io import SafetensorsFile
     ctx = ctx or ParallelContext()
@@ -411,4 +432,4 @@ def load_dense_model(model_dir: str, ctx: Optional[ParallelContext] = None, dtyp
                 if not name.startswith("model.visual."):
                     tensors[name] = sf.tensor(name)
     w = assemble_dense_weights(cfg, tensors, ctx.device, dtype, ctx.rank if ctx.world > 1 else 0, ctx.world)
-    return cfg, DenseModel(cfg, w, ctx)
+    return cfg, DenseModel(cfg, w, ctx, kv_dtype=kv_dtype)

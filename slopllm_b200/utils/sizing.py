@@ -174,23 +174,26 @@ def dense_weight_bytes(cfg, tp: int = 1, elem: int = 2, fp8: bool = False) -> in
     return b
 
 
-def dense_kv_page_bytes(cfg, tp: int = 1, elem: int = 2) -> int:
+def dense_kv_page_bytes(cfg, tp: int = 1, elem: int = 2, kv_dtype=None) -> int:
     """Bytes of one 64-token page on one rank: K and V rows of every full-attention layer (recurrent layers keep their
-    state per sequence, not per page)."""
+    state per sequence, not per page).  `kv_dtype` "e4m3": a byte a value and one exponent a row."""
     n_kv = max(1, cfg.num_key_value_heads // tp)
     full = sum(1 for k in cfg.layer_types if k == "full_attention")
-    return full * 2 * n_kv * cfg.head_dim * elem * PAGE_SIZE
+    return full * 2 * n_kv * (cfg.head_dim * elem if kv_dtype is None else cfg.head_dim + 1) * PAGE_SIZE
 
 
 def plan_dense(cfg, world: int = 1, batch_size: int = 8, chunk_size: int = 8192, max_pages: int = 0, arena_gb: float = 0.0,
-               device_gb: float = 180.0, fp8: bool = False, reserve_gb: float = 4.0) -> MemoryPlan:
+               device_gb: float = 180.0, fp8: bool = False, reserve_gb: float = 4.0, kv_dtype=None) -> MemoryPlan:
     """`plan_memory` for the dense families (tensor parallel only; the workspace estimate is the residual / activation rows
-    plus the MLP's gate-up rows of one chunk)."""
+    plus the MLP's gate-up rows of one chunk, and the rows that prompts read back from an 8-bit cache)."""
     weights = dense_weight_bytes(cfg, world, fp8=fp8)
-    page = max(1, dense_kv_page_bytes(cfg, world))
+    page = max(1, dense_kv_page_bytes(cfg, world, kv_dtype=kv_dtype))
     requested = max_pages if max_pages > 0 else batch_size * -(-chunk_size // PAGE_SIZE)
     work = chunk_size * (cfg.hidden_size * 12 + 2 * (cfg.intermediate_size // world) * 4
                          + (cfg.num_attention_heads // world) * cfg.head_dim * 8)
+    if kv_dtype is not None:
+        from ..ops.kv8 import UNPACK_BUDGET_BYTES
+        work += UNPACK_BUDGET_BYTES
     budget = int(((arena_gb if arena_gb > 0 else device_gb) - reserve_gb) * GIB)
     fit = max(0, (budget - weights - work) // page)
     return MemoryPlan(tp=world, cp=1, ep=False, weights_bytes=weights, page_bytes=page, tokens_per_page=PAGE_SIZE,
