@@ -334,6 +334,12 @@ static bool short_prefill(const PagedPrefillParams* p, int B, int max_q) {
     return p->hd == 64 ? p->max_keys <= (blocks >= 512 ? 64 : 32) : p->max_keys <= 32 && blocks >= 1024;
 }
 
+bool paged_prefill_in_tcgen05(const PagedPrefillParams* p, int B, int max_q) {
+    // a page is a key tile of the tcgen05 kernel (a row's reference there is the largest score before the scale)
+    return p->n_heads % p->n_kv == 0 && p->page_size == 64 && (p->hd == 128 || p->hd == 64) && p->err != nullptr && p->sm_scale > 0.f && B <= 65535 &&
+           max_q <= 65535 * 128 && (((uintptr_t)p->q | (uintptr_t)p->k_cache | (uintptr_t)p->v_cache | (uintptr_t)p->out) & 15) == 0 && !short_prefill(p, B, max_q);
+}
+
 template <int HD, int TERMS>
 static void launch_prefill(const PagedPrefillParams* p, dim3 grid, cudaStream_t s) {
     const size_t smem = (size_t)3 * 64 * (HD + 8) * sizeof(bf16);
@@ -347,7 +353,6 @@ SL_API int sl_paged_attn_prefill(const PagedPrefillParams* p, int B, int max_q, 
     if (B == 0 || max_q == 0) return 0;
     if (p->n_heads % p->n_kv != 0) return -1;
     dim3 grid((max_q + QT - 1) / QT, p->n_heads, B);
-    // a page is a key tile of the tcgen05 kernel (a row's reference there is the largest score before the scale)
     if (p->page_size == 64 && (p->hd == 128 || p->hd == 64) && p->err != nullptr && p->sm_scale > 0.f && B <= 65535 && max_q <= 65535 * 128 &&
         (((uintptr_t)p->q | (uintptr_t)p->k_cache | (uintptr_t)p->v_cache | (uintptr_t)p->out) & 15) == 0) {
         if (!short_prefill(p, B, max_q)) return paged_prefill_tcgen05(p, B, max_q, s);

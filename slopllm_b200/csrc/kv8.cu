@@ -4,6 +4,7 @@
 //    result; keys and values are scaled by the power of two that brings their largest magnitude to (224, 448] and rounded to e4m3.
 //  * kv8_read_kernel: rows of given tokens out of their pages as bf16, which holds them exactly.
 #include "kv8.cuh"
+#include "prefill_attn.cuh"
 
 namespace {
 
@@ -215,14 +216,15 @@ struct Kv8ReadParams {
     bf16 *k, *v;                     // [rows, n_kv, hd]
 };
 
-// Histories of sequences as bf16 pages of 64 tokens, `per_seq` to a sequence, with a page table, rows of it and positions for a kernel that
-// reads such pages.
+// Histories of sequences as pages of 64 tokens, `per_seq` to a sequence, with a page table, rows of it and positions for a kernel that reads such
+// pages.  Keys are bf16; values are, too, or (HALF) fp16 times a power of two per page and head, the largest scale of its tokens.
 struct Kv8UnpackParams {
     Kv8Rows c;
     const int *qo_indptr, *positions, *batch_idx;    // token ranges of the sequences, [T], [T]
     int per_seq;
     bf16 *k, *v;                     // [sequences * per_seq * 64, n_kv, hd]
     int *table, *rows_out, *positions_out;           // [sequences, per_seq], [T], [T]
+    int* exps;                       // [sequences, per_seq, n_kv] exponents of the values' scales (HALF)
 };
 
 // 32 bytes at once
@@ -234,7 +236,9 @@ __device__ __forceinline__ void store_32(void* p, const uint32_t (&w)[8]) {
 constexpr int READ_ROWS = 4;         // a warp's at a time
 
 // Rows `first` .. first + n - 1 of page-table row b, keys (which 0) or values, -> dst: a warp takes READ_ROWS of them, a lane 16 codes of each at a time.
-__device__ __forceinline__ void read_rows(const Kv8Rows& c, int which, int b, int first, int n, bf16* dst) {
+// HALF: as fp16, divided by 2^top[head].
+template <bool HALF>
+__device__ __forceinline__ void read_rows(const Kv8Rows& c, int which, int b, int first, int n, bf16* dst, const int* top = nullptr) {
     const int lane = threadIdx.x & 31, per = c.n_kv * c.hd / 16, per_head = c.hd / 16, page = c.pages.page_size;
     const uint8_t* codes = which ? c.v_codes : c.k_codes;
     for (int i0 = (threadIdx.x >> 5) * READ_ROWS; i0 < n; i0 += (blockDim.x >> 5) * READ_ROWS) {
@@ -253,7 +257,8 @@ __device__ __forceinline__ void read_rows(const Kv8Rows& c, int which, int b, in
             for (int i = 0; i < READ_ROWS; ++i)
                 if (slot[i] >= 0) {
                     u[i] = ldg_nc_16(codes + ((size_t)slot[i] * per + x) * 16);
-                    s[i] = __uint_as_float((uint32_t)exps[i][(size_t)h * 2 * page] << 23);
+                    const uint32_t e = exps[i][(size_t)h * 2 * page];
+                    s[i] = __uint_as_float((HALF ? max(0, (int)e - top[h]) : e) << 23);      // (smaller than 2^-126: nothing is left in fp16)
                 } else {
                     u[i] = make_uint4(0u, 0u, 0u, 0u);           // (a token that is not there reads as zeros)
                     s[i] = 0.f;
@@ -266,8 +271,14 @@ __device__ __forceinline__ void read_rows(const Kv8Rows& c, int which, int b, in
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
                     const float2 lo = e4m3x2_to_float2((uint16_t)in[k]), hi = e4m3x2_to_float2((uint16_t)(in[k] >> 16));
-                    out[2 * k] = f2_to_bf162(lo.x * s[i], lo.y * s[i]);
-                    out[2 * k + 1] = f2_to_bf162(hi.x * s[i], hi.y * s[i]);
+                    if (HALF) {
+                        const __half2 a = __floats2half2_rn(lo.x * s[i], lo.y * s[i]), d = __floats2half2_rn(hi.x * s[i], hi.y * s[i]);
+                        out[2 * k] = *reinterpret_cast<const uint32_t*>(&a);
+                        out[2 * k + 1] = *reinterpret_cast<const uint32_t*>(&d);
+                    } else {
+                        out[2 * k] = f2_to_bf162(lo.x * s[i], lo.y * s[i]);
+                        out[2 * k + 1] = f2_to_bf162(hi.x * s[i], hi.y * s[i]);
+                    }
                 }
                 store_32(dst + ((size_t)(i0 + i) * per + x) * 16, out);
             }
@@ -281,26 +292,44 @@ __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8ReadParams p) {
     const int* r = p.ranges + blockIdx.y * 4;
     const int i0 = blockIdx.x * 32, n = min(32, r[2] - i0), out = r[3] + i0;
     if (n <= 0 || !guard_ok(p.c.pages.guard, 31, out, (long long)p.rows - n + 1)) return;
-    read_rows(p.c, blockIdx.z, r[0], r[1] + i0, n, (blockIdx.z ? p.v : p.k) + (size_t)out * p.c.n_kv * p.c.hd);
+    read_rows<false>(p.c, blockIdx.z, r[0], r[1] + i0, n, (blockIdx.z ? p.v : p.k) + (size_t)out * p.c.n_kv * p.c.hd);
 }
 
-// grid (per_seq * 2, sequences, 2), block 256: half a page of a sequence's workspace
-__global__ void __launch_bounds__(256) kv8_unpack_kernel(Kv8UnpackParams p) {
+// grid (per_seq, sequences, 2), block 512: a page of a sequence's workspace, keys or values
+template <bool HALF>
+__global__ void __launch_bounds__(512) kv8_unpack_kernel(Kv8UnpackParams p) {
     pdl_grid_sync();
-    const int s = blockIdx.y, page = s * p.per_seq + (blockIdx.x >> 1), q0 = p.qo_indptr[s], q1 = p.qo_indptr[s + 1], most = p.per_seq * 64;
+    __shared__ int top[HALF ? KV8_HEADS : 1];        // exponents of the page's values
+    const int s = blockIdx.y, page = s * p.per_seq + blockIdx.x, q0 = p.qo_indptr[s], q1 = p.qo_indptr[s + 1], most = p.per_seq * 64;
     if (q0 >= q1) return;
     int n = p.positions[q1 - 1] + 1;                 // positions ascend within a sequence
     if (!guard_ok(p.c.pages.guard, 33, n, (long long)most + 1)) n = most;
-    if (blockIdx.z == 0 && (blockIdx.x & 1) == 0 && threadIdx.x == 0) p.table[page] = page;
+    if (blockIdx.z == 0 && threadIdx.x == 0) p.table[page] = page;
     if (blockIdx.x == 0 && blockIdx.z == 0)
-        for (int t = q0 + threadIdx.x; t < q1; t += 256) {
+        for (int t = q0 + threadIdx.x; t < q1; t += 512) {
             p.rows_out[t] = s;
             p.positions_out[t] = min(p.positions[t], most - 1);
         }
-    const int i0 = blockIdx.x * 32;
-    n = min(32, n - i0);
+    const int i0 = blockIdx.x * 64, b = p.batch_idx[q0];
+    n = min(64, n - i0);
     if (n <= 0) return;
-    read_rows(p.c, blockIdx.z, p.batch_idx[q0], i0, n, (blockIdx.z ? p.v : p.k) + ((size_t)s * most + i0) * p.c.n_kv * p.c.hd);
+    bf16* dst = (blockIdx.z ? p.v : p.k) + (size_t)page * 64 * p.c.n_kv * p.c.hd;
+    if (!HALF || blockIdx.z == 0) {
+        read_rows<false>(p.c, blockIdx.z, b, i0, n, dst);
+        return;
+    }
+    const int lane = threadIdx.x & 31, size = p.c.pages.page_size;
+    const int s0 = lane < n ? kv8_slot(p.c.pages, 33, b, i0 + lane) : -1, s1 = lane + 32 < n ? kv8_slot(p.c.pages, 33, b, i0 + lane + 32) : -1;
+    for (int h = threadIdx.x >> 5; h < p.c.n_kv; h += 16) {
+        const int e0 = s0 >= 0 ? p.c.exps[kv8_exp_at(p.c.pages, p.c.n_kv, s0, h) + size] : 0, e1 = s1 >= 0 ? p.c.exps[kv8_exp_at(p.c.pages, p.c.n_kv, s1, h) + size] : 0;
+        const int e = __reduce_max_sync(0xffffffffu, max(e0, e1));
+        if (lane == 0) {
+            top[h] = e - KV8_BIAS;
+            p.exps[(size_t)page * p.c.n_kv + h] = e - KV8_BIAS;
+        }
+    }
+    __syncthreads();
+    read_rows<HALF>(p.c, 1, b, i0, n, dst, top);
 }
 
 constexpr int WARPS_WANTED = 148 * 32;
@@ -344,9 +373,15 @@ SL_API int sl_kv8_read(const Kv8ReadParams* p, int ranges, int longest, cudaStre
     return SL_LAUNCH_CHECK();
 }
 
-SL_API int sl_kv8_unpack(const Kv8UnpackParams* p, int sequences, cudaStream_t s) {
-    if (sequences == 0) return 0;
-    if (!kv8_rows_ok(p->c, p->k, p->v) || sequences > 65535 || p->per_seq < 1) return -1;
-    sl_launch(kv8_unpack_kernel, dim3(p->per_seq * 2, sequences, 2), 256, 0, s, *p);
-    return SL_LAUNCH_CHECK();
+// Causal attention of `sequences` token ranges over their histories: the histories' pages into the workspace of `up`, whose memory `attn` reads.
+SL_API int sl_kv8_prompts(const Kv8UnpackParams* up, const PagedPrefillParams* attn, int sequences, int max_q, cudaStream_t s) {
+    if (sequences == 0 || max_q == 0) return 0;
+    if (!kv8_rows_ok(up->c, up->k, up->v) || sequences > 65535 || up->per_seq < 1 || up->c.n_kv > KV8_HEADS) return -1;
+    const bool half = paged_prefill_in_tcgen05(attn, sequences, max_q);
+    const dim3 grid(up->per_seq, sequences, 2);
+    if (half) sl_launch(kv8_unpack_kernel<true>, grid, 512, 0, s, *up);
+    else sl_launch(kv8_unpack_kernel<false>, grid, 512, 0, s, *up);
+    const int rc = SL_LAUNCH_CHECK();
+    if (rc != 0) return rc;
+    return half ? paged_prefill_tcgen05(attn, sequences, max_q, s, {up->exps, up->per_seq}) : sl_paged_attn_prefill(attn, sequences, max_q, s);
 }

@@ -8,6 +8,7 @@
 
 #include "common.cuh"
 
+constexpr int KV8_HEADS = 1024;                  // key heads at most
 constexpr int KV8_BIAS = 127, KV8_LOW = -60, KV8_HIGH = 60;      // exponents that are written
 
 // Where a step's tokens lie: checked places of the page table.

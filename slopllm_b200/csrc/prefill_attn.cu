@@ -13,6 +13,11 @@
 // 4096 tokens, 16 heads of 128 over 4, a layer: 667 us -> 103 us, 0.67 PFLOP/s; three prompts of 2500 tokens in all: 117 -> 33 us (B200).  With P in one term:
 // 85 us, and 1.3 times the error against 64 bits; the older kernel, also with one term, has that error too.
 //
+// HALF (workspaces of the 8-bit cache, kv8.cu): values are fp16 times a power of two per page and head, and P is one fp16 term: its 11 bits are enough
+// beside the output's 8, and the second product against the same values (a third of the tensor time) and the making of the second term fall away.
+// The page's exponent goes into the weights, as part of the row's reference, and out of the denominator.  Chunk of 4096 behind 8192, 32 heads of 128 over 8:
+// 749 -> 590 us (B200).
+//
 // Rows of the last page behind the last visible key may hold anything: their scores are masked, their values zeroed in shared memory.  A value
 // that is not finite in front of it reaches all queries of its block, whose weights for it may be 0 (the other kernel's blocks have 64 queries).
 // Waits are bounded; one that runs out sets the error word and ends the block.
@@ -42,9 +47,9 @@ __device__ __forceinline__ float ex2_approx(float x) {
 }
 
 // grid (heads, ceil(max_q / 128), B), block 192
-template <int HD>
+template <int HD, bool HALF>
 __global__ void __launch_bounds__(THREADS, 2) prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                                                                  const __grid_constant__ CUtensorMap map_v, PagedPrefillParams p) {
+                                                                  const __grid_constant__ CUtensorMap map_v, PagedPrefillParams p, HalfValues half) {
     extern __shared__ uint8_t smem_raw[];
     using M = Smem<HD>;
     uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -118,7 +123,7 @@ __global__ void __launch_bounds__(THREADS, 2) prefill_attn_kernel(const __grid_c
         }
     } else if (warp == 5) {
         constexpr uint32_t IDESC_S = tc::idesc_f16(QT, KT, 1);
-        constexpr uint32_t IDESC_PV = tc::idesc_f16(QT, HD, 1) | tc::IDESC_B_MN_MAJOR;
+        constexpr uint32_t IDESC_PV = tc::idesc_f16(QT, HD, HALF ? 0 : 1) | tc::IDESC_B_MN_MAJOR;
         const uint64_t dq = tc::smem_desc_sw128(tc::smem_u32(smem + M::Q)), dk = tc::smem_desc_sw128(tc::smem_u32(smem + M::K));
         const uint64_t dv = tc::smem_desc_mn_sw128(tc::smem_u32(smem + M::V), M::K_TILE);
         const uint32_t t_base = tc::warp_uniform(tmem);
@@ -147,8 +152,8 @@ __global__ void __launch_bounds__(THREADS, 2) prefill_attn_kernel(const __grid_c
             if (i == nt - 1 && n_keys % KT != 0) {               // value rows behind the last visible key
                 const int r0 = n_keys % KT;
                 for (int x = lane; x < M::HALVES * (KT - r0) * 8; x += 32) {
-                    const int half = x / ((KT - r0) * 8), y = x % ((KT - r0) * 8);
-                    *reinterpret_cast<uint4*>(smem + M::V + (st * M::HALVES + half) * M::K_TILE + (r0 + y / 8) * 128 + y % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
+                    const int side = x / ((KT - r0) * 8), y = x % ((KT - r0) * 8);
+                    *reinterpret_cast<uint4*>(smem + M::V + (st * M::HALVES + side) * M::K_TILE + (r0 + y / 8) * 128 + y % 8 * 16) = make_uint4(0u, 0u, 0u, 0u);
                 }
                 tc::fence_proxy_async_smem();
                 __syncwarp();
@@ -159,7 +164,7 @@ __global__ void __launch_bounds__(THREADS, 2) prefill_attn_kernel(const __grid_c
                 if (ok && tc::elect_one()) {
                     const uint64_t value = tc::desc_at(dv, st * M::HALVES * M::K_TILE);
 #pragma unroll
-                    for (int k = 0; k < KT / 8; ++k)                // the high terms of P, then the low ones, against the same values
+                    for (int k = 0; k < KT / (HALF ? 16 : 8); ++k)  // the high terms of P, then the low ones, against the same values
                         tc::mma_f16_ts(t_base + COL_O, t_base + COL_S + (i & 1) * KT + k * 8,
                                        tc::desc_at(value, (k & 3) * 16 * 128), IDESC_PV, (i > 0 || k > 0) ? 1u : 0u);
                     tc::mma_commit(i + 1 < nt ? pv_done : o_done);
@@ -176,7 +181,11 @@ __global__ void __launch_bounds__(THREADS, 2) prefill_attn_kernel(const __grid_c
         const float scale = p.sm_scale * 1.4426950408889634f;
         float m = -INFINITY, l = 0.f;                               // reference in log2 units, denominator
         bool ok = true;
+        const int* exps = HALF ? half.exps + (size_t)seq * half.per_seq * p.n_kv + hkv : nullptr;
+        int next_exp = HALF ? exps[0] : 0;
         for (int j = 0; j < tiles; ++j) {
+            const int exp_j = next_exp;                             // of the tile's values
+            if (HALF && j + 1 < tiles) next_exp = exps[(size_t)(j + 1) * p.n_kv];
             ok = tc::mbar_wait(s_ready + (j & 1), (uint32_t)(j >> 1) & 1);
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
@@ -199,7 +208,7 @@ __global__ void __launch_bounds__(THREADS, 2) prefill_attn_kernel(const __grid_c
                 t2 = fmaxf(t2, __uint_as_float(s[1][x]));
                 t3 = fmaxf(t3, __uint_as_float(s[1][x + 1]));
             }
-            const float top = fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * scale;
+            const float top = HALF ? fmaf(fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)), scale, (float)exp_j) : fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * scale;
             if (__any_sync(0xffffffffu, top > m + RAISE)) {
                 const float mn = fmaxf(m, top), f = m == -INFINITY ? 0.f : ex2_approx(m - mn);
                 if (j > 0) {                                        // the sum so far: not while the previous product adds to it
@@ -219,25 +228,30 @@ __global__ void __launch_bounds__(THREADS, 2) prefill_attn_kernel(const __grid_c
                 l *= f;
                 m = mn;
             }
-            const float base = m == -INFINITY ? 0.f : m;
+            const float base = m == -INFINITY ? 0.f : HALF ? m - (float)exp_j : m;
             float l0 = 0.f, l1 = 0.f;
 #pragma unroll
-            for (int half = 0; half < 2; ++half) {                  // 32 keys: 16 columns of high terms, 16 of low ones
+            for (int part = 0; part < 2; ++part) {                  // 32 keys: 16 columns of high terms, 16 of low ones
                 uint32_t hi[16], lo[16];
 #pragma unroll
                 for (int x = 0; x < 16; ++x) {
-                    const float e0 = ex2_approx(fmaf(__uint_as_float(s[half][x * 2]), scale, -base));
-                    const float e1 = ex2_approx(fmaf(__uint_as_float(s[half][x * 2 + 1]), scale, -base));
+                    const float e0 = ex2_approx(fmaf(__uint_as_float(s[part][x * 2]), scale, -base));
+                    const float e1 = ex2_approx(fmaf(__uint_as_float(s[part][x * 2 + 1]), scale, -base));
                     l0 += e0;
                     l1 += e1;
-                    hi[x] = f2_to_bf162(e0, e1);
-                    const float2 h = bf162_to_f2(hi[x]);
-                    lo[x] = f2_to_bf162(e0 - h.x, e1 - h.y);
+                    if (HALF) {
+                        const __half2 h = __floats2half2_rn(e0, e1);
+                        hi[x] = *reinterpret_cast<const uint32_t*>(&h);
+                    } else {
+                        hi[x] = f2_to_bf162(e0, e1);
+                        const float2 h = bf162_to_f2(hi[x]);
+                        lo[x] = f2_to_bf162(e0 - h.x, e1 - h.y);
+                    }
                 }
-                tc::tmem_st_32x16(lane_at + COL_S + (j & 1) * KT + half * 16, hi);
-                tc::tmem_st_32x16(lane_at + COL_S + (j & 1) * KT + 32 + half * 16, lo);
+                tc::tmem_st_32x16(lane_at + COL_S + (j & 1) * KT + part * 16, hi);
+                if (!HALF) tc::tmem_st_32x16(lane_at + COL_S + (j & 1) * KT + 32 + part * 16, lo);
             }
-            l += l0 + l1;
+            l = HALF ? fmaf(l0 + l1, __uint_as_float((uint32_t)(127 - exp_j) << 23), l) : l + (l0 + l1);
             tc::tmem_st_wait();
             tc::fence_before_sync();
             tc::mbar_arrive(p_ready + (j & 1));
@@ -276,23 +290,24 @@ __global__ void __launch_bounds__(THREADS, 2) prefill_attn_kernel(const __grid_c
     }
 }
 
-template <int HD>
-int launch(const PagedPrefillParams* p, int B, int max_q, cudaStream_t s) {
+template <int HD, bool HALF>
+int launch(const PagedPrefillParams* p, int B, int max_q, cudaStream_t s, const HalfValues& half) {
     CUtensorMap mq, mk, mv;
     int r = make_tmap_2d(&mq, p->q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p->T, (uint64_t)p->n_heads * HD, (uint64_t)p->n_heads * HD * 2, QT, 64);
     if (r == 0) r = make_tmap_2d(&mk, p->k_cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p->num_slots, (uint64_t)p->n_kv * HD, (uint64_t)p->n_kv * HD * 2, KT, 64);
     if (r == 0) r = make_tmap_2d(&mv, p->v_cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p->num_slots, (uint64_t)p->n_kv * HD, (uint64_t)p->n_kv * HD * 2, KT, 64);
     if (r != 0) return r;
-    auto kern = prefill_attn_kernel<HD>;
+    auto kern = prefill_attn_kernel<HD, HALF>;
     constexpr int smem = Smem<HD>::TOTAL + 1024;
     static_assert(2 * (smem + 1024) <= 228 * 1024, "two blocks per SM");
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    sl_launch(kern, dim3(p->n_heads, (max_q + QT - 1) / QT, B), THREADS, smem, s, mq, mk, mv, *p);
+    sl_launch(kern, dim3(p->n_heads, (max_q + QT - 1) / QT, B), THREADS, smem, s, mq, mk, mv, *p, half);
     return SL_LAUNCH_CHECK();
 }
 
 }  // namespace
 
-int paged_prefill_tcgen05(const PagedPrefillParams* p, int B, int max_q, cudaStream_t s) {
-    return p->hd == 128 ? launch<128>(p, B, max_q, s) : launch<64>(p, B, max_q, s);
+int paged_prefill_tcgen05(const PagedPrefillParams* p, int B, int max_q, cudaStream_t s, const HalfValues& half) {
+    if (half.exps != nullptr) return p->hd == 128 ? launch<128, true>(p, B, max_q, s, half) : launch<64, true>(p, B, max_q, s, half);
+    return p->hd == 128 ? launch<128, false>(p, B, max_q, s, half) : launch<64, false>(p, B, max_q, s, half);
 }

@@ -4,6 +4,9 @@
 
 #include "common.cuh"
 
+struct PagedPrefillParams;
+SL_API int sl_paged_attn_prefill(const PagedPrefillParams* p, int B, int max_q, cudaStream_t s);
+
 struct PagedPrefillParams {
     const bf16* q;                   // [T, n_heads, hd]
     const bf16* k_cache;             // [num_slots, n_kv, hd]
@@ -20,5 +23,14 @@ struct PagedPrefillParams {
     int* err;                        // error word of bounded waits
 };
 
+// Values as fp16 times a power of two per page and key head: exponents [B, pages of a sequence, n_kv]; sequence b's pages are numbered from 0.
+struct HalfValues {
+    const int* exps;                 // null: values are bf16
+    int per_seq;
+};
+
+// Whether the tcgen05 kernel takes these arguments (dense_attn.cu).
+bool paged_prefill_in_tcgen05(const PagedPrefillParams* p, int B, int max_q);
+
 // Pages of 64 tokens, heads of 64 or 128 values, 16-byte aligned rows (prefill_attn.cu).
-int paged_prefill_tcgen05(const PagedPrefillParams* p, int B, int max_q, cudaStream_t s);
+int paged_prefill_tcgen05(const PagedPrefillParams* p, int B, int max_q, cudaStream_t s, const HalfValues& half = {nullptr, 0});

@@ -46,7 +46,8 @@ class Kv8ReadParams(C.Structure):
 
 class Kv8UnpackParams(C.Structure):
     _fields_ = [*_ROWS, ("qo_indptr", C.c_void_p), ("positions", C.c_void_p), ("batch_idx", C.c_void_p), ("per_seq", C.c_int),
-                ("k", C.c_void_p), ("v", C.c_void_p), ("table", C.c_void_p), ("rows_out", C.c_void_p), ("positions_out", C.c_void_p)]
+                ("k", C.c_void_p), ("v", C.c_void_p), ("table", C.c_void_p), ("rows_out", C.c_void_p), ("positions_out", C.c_void_p),
+                ("exps_out", C.c_void_p)]
 
 
 class Kv8DecodeParams(C.Structure):
@@ -265,22 +266,25 @@ def _decode_plan(device: int, n_heads: int, n_kv: int, hd: int) -> Tuple[int, ..
 
 
 def _prompts(q, cache, positions, batch_idx, page_table, sm_scale, qo_indptr, max_q, max_kv_len, out) -> None:
-    """Histories are read back into bf16 pages of 64 tokens, over which the prompt kernel attends.  Done once per key head and token, that
-    costs less than codes that every block of the kernel (query heads x 128 queries) turns into an operand anew."""
+    """Histories are read back into pages of 64 tokens (keys bf16; values fp16 with a power of two per page and head, where the tcgen05 kernel
+    takes them), over which the prompt kernel attends.  Done once per key head and token, that costs less than codes that every block of the
+    kernel (query heads x 128 queries) turns into an operand anew."""
     (T, n_heads, hd), device, dev = q.shape, q.get_device(), q.device
     n_kv, B = cache.k.shape[1], qo_indptr.numel() - 1
     most = page_table.shape[1] * cache.page_size
     per_seq = max(1, -(-min(max_kv_len or most, most) // 64))
     group = max(1, min(B, UNPACK_BUDGET_BYTES // (per_seq * 64 * n_kv * hd * 4)))
     k, v = (torch.empty(group * per_seq * 64, n_kv, hd, dtype=torch.bfloat16, device=dev) for _ in range(2))
-    ints = torch.empty(group * per_seq + 2 * T, dtype=torch.int32, device=dev)
-    table, rows_out, positions_out = ints.data_ptr(), ints.data_ptr() + 4 * group * per_seq, ints.data_ptr() + 4 * (group * per_seq + T)
+    pages = group * per_seq
+    ints = torch.empty(pages * (1 + n_kv) + 2 * T, dtype=torch.int32, device=dev)
+    table, exps, rows_out = (ints.data_ptr() + 4 * i for i in (0, pages, pages * (1 + n_kv)))
+    positions_out = rows_out + 4 * T
     rows = _rows(cache, page_table)
     for s in range(0, B, group):
         n, ends = min(group, B - s), qo_indptr.data_ptr() + 4 * s
-        up = Kv8UnpackParams(*rows, ends, positions.data_ptr(), batch_idx.data_ptr(), per_seq, k.data_ptr(), v.data_ptr(), table, rows_out, positions_out)
-        _call(device, "sl_kv8_unpack", C.byref(up), n)
+        up = Kv8UnpackParams(*rows, ends, positions.data_ptr(), batch_idx.data_ptr(), per_seq, k.data_ptr(), v.data_ptr(), table, rows_out, positions_out,
+                             exps)
         p = AttnParams(q=q.data_ptr(), k_cache=k.data_ptr(), v_cache=v.data_ptr(), positions=positions_out, batch_idx=rows_out, page_table=table,
                        pt_stride=per_seq, page_size=64, qo_indptr=ends, n_heads=n_heads, n_kv=n_kv, hd=hd, sm_scale=sm_scale, out=out.data_ptr(), T=T,
                        num_slots=k.shape[0], max_keys=max_kv_len, err=tcgen05.error_flag(dev).data_ptr())
-        _call(device, "sl_paged_attn_prefill", C.byref(p), n, int(max_q))
+        _call(device, "sl_kv8_prompts", C.byref(up), C.byref(p), n, int(max_q))

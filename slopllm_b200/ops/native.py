@@ -270,7 +270,7 @@ _SIGS = {
     "sl_paged_attn_prefill": [vp, i32, i32, vp],
     "sl_kv8_store": [vp, i32, vp],
     "sl_kv8_read": [vp, i32, i32, vp],
-    "sl_kv8_unpack": [vp, i32, vp],
+    "sl_kv8_prompts": [vp, vp, i32, i32, vp],
     "sl_kv8_decode_plan": [i32, i32, i32, vp, vp, vp, vp],
     "sl_kv8_decode": [vp, i32, i32, i32, vp],
     "sl_delta_scan": [vp, i32, vp],
