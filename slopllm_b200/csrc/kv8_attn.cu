@@ -50,11 +50,11 @@ __device__ __forceinline__ float ex2(float x) {
 
 __device__ __forceinline__ uint32_t transposed8x8(uint32_t x) {
     uint32_t y;
-    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
     return y;
 }
 __device__ __forceinline__ void mma_f16_16816(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
                  : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
@@ -158,7 +158,7 @@ struct Tiles {
 // Spilled registers cost more than blocks bring (shared memory leaves no L1 to speak of): the sums of 16 heads of 128, or of 8 of 256, take the
 // registers of a block by itself.
 // Blocks an SM and warps of products; four sub-cores share the warps, and a block by itself has two on each.
-constexpr int blocks_per_sm(int width, int tiles) { return width == 64 ? (tiles == 1 ? 3 : 2) : width * tiles == 128 ? 2 : 1; }
+constexpr int blocks_per_sm(int width, int tiles) { return width == 64 ? 3 : width * tiles == 128 ? 2 : 1; }
 
 template <int D, int NG>
 struct Cfg {
@@ -395,21 +395,25 @@ __global__ void __launch_bounds__(Cfg<D, NG>::THREADS, Cfg<D, NG>::PER_SM) kv8_d
 #pragma unroll
                     for (int y = 0; y < 2; ++y) sc[n][y][0] = sc[n][y][1] = sc[n][y][2] = sc[n][y][3] = 0.f;
 #pragma unroll
-                for (int x = 0; x < CH; ++x)
+                for (int x = 0; x < CH; ++x) {
+                    uint4 u[2][2];
 #pragma unroll
                     for (int y = 0; y < 2; ++y) {
                         const uint8_t* a0 = kt + (D < 128 ? ks : (x >> 1) * KT * 128 + ks + (((2 * c4 + (x & 1)) ^ g) << 4)) + y * 16 * M::ROW;
-                        const uint4 u0 = *reinterpret_cast<const uint4*>(a0), u1 = *reinterpret_cast<const uint4*>(a0 + 8 * M::ROW);
-                        const uint32_t r0[4] = {u0.x, u0.y, u0.z, u0.w}, r1[4] = {u1.x, u1.y, u1.z, u1.w};
+                        u[y][0] = *reinterpret_cast<const uint4*>(a0);
+                        u[y][1] = *reinterpret_cast<const uint4*>(a0 + 8 * M::ROW);
+                    }
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
+                    for (int i = 0; i < 4; ++i)
+#pragma unroll
+                        for (int y = 0; y < 2; ++y) {                // (independent sums in turn)
                             uint32_t a[4];
-                            e4m3x4_to_f16(r0[i], a[0], a[2]);
-                            e4m3x4_to_f16(r1[i], a[1], a[3]);
+                            e4m3x4_to_f16(reinterpret_cast<const uint32_t*>(&u[y][0])[i], a[0], a[2]);
+                            e4m3x4_to_f16(reinterpret_cast<const uint32_t*>(&u[y][1])[i], a[1], a[3]);
 #pragma unroll
                             for (int n = 0; n < NG; ++n) mma_f16_16816(sc[n][y], a, q[n][x * 4 + i][0], q[n][x * 4 + i][1]);
                         }
-                    }
+                }
                 // exponents of keys g, g + 8, g + 16, g + 24 (of a key that is not seen: any)
                 float kf[4], ev[4], back[4];
 #pragma unroll
