@@ -389,6 +389,16 @@ __global__ void __launch_bounds__(Cfg<D, NG>::THREADS, Cfg<D, NG>::PER_SM) kv8_d
                 __syncwarp();
             }
             if (nk > 0) {
+                // exponents of keys g, g + 8, g + 16, g + 24 (of a key that is not seen: any)
+                float kf[4], ev[4], back[4];
+#pragma unroll
+                for (int u = 0; u < 4; ++u) {
+                    const bool seen = g + u * 8 < nk;
+                    const uint32_t eb = seen ? exps[g + u * 8] : KV8_BIAS, vb = seen ? exps[KT + g + u * 8] : KV8_BIAS;
+                    kf[u] = __uint_as_float(eb << 23);
+                    ev[u] = seen ? __uint_as_float(0x4b000000u | vb) - (8388608.f + KV8_BIAS) : -INFINITY;
+                    back[u] = __uint_as_float((2 * KV8_BIAS - vb) << 23);
+                }
                 float sc[NG][2][4];                                  // keys g and g + 8 of 16, heads 2 c4 and 2 c4 + 1
 #pragma unroll
                 for (int n = 0; n < NG; ++n)
@@ -414,15 +424,24 @@ __global__ void __launch_bounds__(Cfg<D, NG>::THREADS, Cfg<D, NG>::PER_SM) kv8_d
                             for (int n = 0; n < NG; ++n) mma_f16_16816(sc[n][y], a, q[n][x * 4 + i][0], q[n][x * 4 + i][1]);
                         }
                 }
-                // exponents of keys g, g + 8, g + 16, g + 24 (of a key that is not seen: any)
-                float kf[4], ev[4], back[4];
+                // a lane's dims of keys 2 c4, 2 c4 + 1 and 8 on, of each 16; the first ones are read ahead of the weights
+                auto values = [&](int x, int y, uint32_t (&v)[4][M::CHUNK / 4]) {
 #pragma unroll
-                for (int u = 0; u < 4; ++u) {
-                    const bool seen = g + u * 8 < nk;
-                    const uint32_t eb = seen ? exps[g + u * 8] : KV8_BIAS, vb = seen ? exps[KT + g + u * 8] : KV8_BIAS;
-                    kf[u] = __uint_as_float(eb << 23);
-                    ev[u] = seen ? __uint_as_float(0x4b000000u | vb) - (8388608.f + KV8_BIAS) : -INFINITY;
-                    back[u] = __uint_as_float((2 * KV8_BIAS - vb) << 23);
+                    for (int u = 0; u < 4; ++u) {
+                        const int r = y * 16 + 2 * c4 + (u & 1) + (u >> 1) * 8;
+                        if (D < 128) {
+                            *reinterpret_cast<uint2*>(v[u]) = *reinterpret_cast<const uint2*>(vt + (k0 + r) * 64 + (((g >> 1) ^ c4) << 4) + (g & 1) * 8);
+                        } else {
+                            *reinterpret_cast<uint4*>(v[u]) =
+                                *reinterpret_cast<const uint4*>(vt + x * KT * 128 + (k0 + r) * 128 + ((g ^ (2 * c4 + (u & 1))) << 4));
+                        }
+                    }
+                };
+                constexpr bool AHEAD = NG == 1;                      // (where registers are left)
+                uint32_t early[2][4][M::CHUNK / 4];
+                if (AHEAD) {
+                    values(0, 0, early[0]);
+                    values(0, 1, early[1]);
                 }
                 uint32_t pw[NG][4];                                  // weights times scales: head g, keys 2 c4 and 2 c4 + 1 of every 8
 #pragma unroll
@@ -457,21 +476,18 @@ __global__ void __launch_bounds__(Cfg<D, NG>::THREADS, Cfg<D, NG>::PER_SM) kv8_d
                         pw[n][u] = transposed8x8(f2_to_f16x2(e0, e1));
                     }
                 }
-                // a lane's dims of keys 2 c4, 2 c4 + 1 and 8 on, of each 16
 #pragma unroll
                 for (int x = 0; x < M::HALVES; ++x)
 #pragma unroll
                     for (int y = 0; y < 2; ++y) {
                         uint32_t v[4][M::CHUNK / 4];
+                        if (AHEAD && x == 0) {
 #pragma unroll
-                        for (int u = 0; u < 4; ++u) {
-                            const int r = y * 16 + 2 * c4 + (u & 1) + (u >> 1) * 8;
-                            if (D < 128) {
-                                *reinterpret_cast<uint2*>(v[u]) = *reinterpret_cast<const uint2*>(vt + (k0 + r) * 64 + (((g >> 1) ^ c4) << 4) + (g & 1) * 8);
-                            } else {
-                                *reinterpret_cast<uint4*>(v[u]) =
-                                    *reinterpret_cast<const uint4*>(vt + x * KT * 128 + (k0 + r) * 128 + ((g ^ (2 * c4 + (u & 1))) << 4));
-                            }
+                            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                                for (int i = 0; i < M::CHUNK / 4; ++i) v[u][i] = early[y][u][i];
+                        } else {
+                            values(x, y, v);
                         }
 #pragma unroll
                         for (int i = 0; i < M::CHUNK / 4; ++i)
