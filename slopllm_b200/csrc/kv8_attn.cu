@@ -697,7 +697,7 @@ int launch(const Kv8DecodeParams* all, int T, int blocks, const Deal& deal, int 
         // histories of up to WHOLE tokens are not cut; else, few histories have many parts each: a block a query head; many have few: a block for the one
         // that a share's end cuts
         const int items = p.T * deal.items, rows = p.n_heads / p.n_kv < M::HG ? p.n_heads / p.n_kv : M::HG;
-        const Parts parts = longest > 0 && longest <= WHOLE ? Parts::NONE : items <= blocks * deal.passes ? Parts::BY_ITEM : Parts::BY_BLOCK;
+        const Parts parts = longest > 0 && longest <= WHOLE ? Parts::NONE : p.T * 8 <= blocks / deal.abreast && items <= blocks * deal.passes ? Parts::BY_ITEM : Parts::BY_BLOCK;
         sl_launch(kv8_decode_kernel<D, NG>, blocks, M::THREADS, smem, s, mk, mv, p, deal, box, parts);
         if (parts == Parts::BY_ITEM) sl_launch(kv8_merge_kernel<D, M::HG, 1>, dim3(items, rows), 512, 0, s, p, deal);
         else if (parts == Parts::BY_BLOCK) sl_launch(kv8_merge_kernel<D, M::HG, M::HG>, blocks * deal.passes, 512, 0, s, p, deal);
