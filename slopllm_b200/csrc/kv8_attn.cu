@@ -37,6 +37,7 @@ struct Kv8DecodeParams {
 };
 
 constexpr int KT = 64, MAX_T = 256;              // keys a tile, tokens a launch
+constexpr int CLUSTER_SIZE = 8;
 // Weights are 2^(score + exponent of the value's scale - reference).  A row's reference is raised to 2^TOP below the largest when one would be above
 // 2^(TOP + RAISE), which fp16 holds; fp32 weights reach down to 2^-126, so that two rows whose scales are the format's limits apart (2^120) are told
 // apart by weights down to 2^-14 of the largest.
@@ -176,14 +177,13 @@ struct Cfg {
     static constexpr int TOTAL = BARS + (2 * STAGES + 4) * 8;
 };
 
-// grid: blocks of the device
-template <int D, int NG>
-__global__ void __launch_bounds__(Cfg<D, NG>::THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
-                                                                               Kv8DecodeParams p, Deal deal, int box, Parts parts) {
+// A block's part of the work; `smem`: Cfg::TOTAL bytes, aligned to 1024.  CLUSTER: of one history and `item`, shared by `CLUSTER_SIZE` blocks, of which
+// this is number `rank`; its partial result is the first of o_part.  Returns the shares that the tiles are cut into.
+template <int D, int NG, bool CLUSTER>
+__device__ __forceinline__ int decode_block(const CUtensorMap& map_k, const CUtensorMap& map_v, const Kv8DecodeParams& p, const Deal& deal, int box, Parts parts,
+                                            uint8_t* smem, int rank, int only) {
     using M = Cfg<D, NG>;
     constexpr int MT = M::MT, WARPS = M::WARPS, THREADS = M::THREADS;
-    extern __shared__ uint8_t smem_raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
     uint64_t *full = reinterpret_cast<uint64_t*>(smem + M::BARS), *free_ = full + M::STAGES, *q_full = free_ + M::STAGES, *q_free = q_full + 2;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     if (tid == 0) {
@@ -201,24 +201,25 @@ __global__ void __launch_bounds__(Cfg<D, NG>::THREADS, Cfg<D, NG>::PER_SM) kv8_d
     }
     pdl_grid_sync();
     const int group = p.n_heads / p.n_kv, hg = (group + M::HG - 1) / M::HG;
-    const Tiles tiles(*reinterpret_cast<Batch*>(smem + M::BATCH), p, gridDim.x / deal.abreast);
+    const Tiles tiles(*reinterpret_cast<Batch*>(smem + M::BATCH), p, CLUSTER ? CLUSTER_SIZE : gridDim.x / deal.abreast);
     const bool by_item = parts == Parts::BY_ITEM, by_block = parts == Parts::BY_BLOCK;
-    for (int t = blockIdx.x; t < p.T; t += gridDim.x)
+    for (int t = CLUSTER ? rank : blockIdx.x; t < p.T; t += CLUSTER ? CLUSTER_SIZE : gridDim.x)
         if (tiles.count(t) == 0) {
             for (int i = tid; i < p.n_heads * p.hd / 2; i += THREADS) reinterpret_cast<uint32_t*>(p.out + (size_t)t * p.n_heads * p.hd)[i] = 0u;
             if (by_item)
                 for (int i = tid; i < deal.items; i += THREADS) p.jobs[t * deal.items + i] = make_int4(0, 0, 0, 0);
         }
     if (by_block && tid < deal.passes) p.jobs[blockIdx.x * deal.passes + tid] = make_int4(0, 0, 0, 0);
-    const int share = blockIdx.x / deal.abreast, first_item = blockIdx.x % deal.abreast, passes = (deal.items - first_item + deal.abreast - 1) / deal.abreast;
-    if (share >= tiles.shares) return;
+    const int share = CLUSTER ? rank : blockIdx.x / deal.abreast, first_item = CLUSTER ? only : blockIdx.x % deal.abreast;
+    const int passes = CLUSTER ? 1 : (deal.items - first_item + deal.abreast - 1) / deal.abreast;
+    if (share >= tiles.shares) return tiles.shares;
     int s0 = tiles.begin(share), s1 = tiles.begin(share + 1);
-    if (parts == Parts::NONE) {
+    if (!CLUSTER && parts == Parts::NONE) {
         s0 = tiles.whole(s0);
         s1 = tiles.whole(s1);
     }
     const int len = s1 - s0;
-    if (len <= 0) return;
+    if (len <= 0) return tiles.shares;
     const long long w1 = (long long)len * passes;                // this block's tiles, item by item
 
     if (warp == WARPS) {
@@ -301,7 +302,7 @@ __global__ void __launch_bounds__(Cfg<D, NG>::THREADS, Cfg<D, NG>::PER_SM) kv8_d
         for (int j = max(0, issued - M::STAGES); j < issued; ++j) ok &= tc::mbar_wait_warp(full + j % M::STAGES, (uint32_t)(j / M::STAGES) & 1);
         for (int j = max(0, asked - 2); j < asked; ++j) ok &= tc::mbar_wait_warp(q_full + (j & 1), (uint32_t)(j >> 1) & 1);
         if (!ok && lane == 0) atomicExch(p.err, 50);
-        return;
+        return tiles.shares;
     }
 
     // ---- products: a pair of warps takes every tile that is its turn, a warp 32 of its keys ----
@@ -529,8 +530,8 @@ __global__ void __launch_bounds__(Cfg<D, NG>::THREADS, Cfg<D, NG>::PER_SM) kv8_d
         }
         together();
         const bool whole = count == at.n;
-        const size_t part = ((size_t)blockIdx.x * deal.passes + pass) * 2 + (at.tile == 0 ? 1 : 0);
-        if (at.tile == 0 && tid == 0) {
+        const size_t part = CLUSTER ? 0 : ((size_t)blockIdx.x * deal.passes + pass) * 2 + (at.tile == 0 ? 1 : 0);
+        if (!CLUSTER && at.tile == 0 && tid == 0) {
             const int4 job = make_int4(t, item, whole ? 1 : tiles.share_of(s + at.n - 1) - share + 1, (int)part >> 1);
             if (by_item) p.jobs[t * deal.items + item] = job;
             else if (by_block && !whole) p.jobs[part >> 1] = job;
@@ -581,6 +582,67 @@ __global__ void __launch_bounds__(Cfg<D, NG>::THREADS, Cfg<D, NG>::PER_SM) kv8_d
         }
     }
     if (!ok && lane == 0) atomicExch(p.err, 51);
+    return tiles.shares;
+}
+
+__device__ __forceinline__ uint8_t* aligned_1024(uint8_t* p) { return reinterpret_cast<uint8_t*>(((uintptr_t)p + 1023) & ~(uintptr_t)1023); }
+
+// grid: blocks of the device
+template <int D, int NG>
+__global__ void __launch_bounds__(Cfg<D, NG>::THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
+                                                                               const __grid_constant__ Kv8DecodeParams p, Deal deal, int box, Parts parts) {
+    extern __shared__ uint8_t smem_raw[];
+    decode_block<D, NG, false>(map_k, map_v, p, deal, box, parts, aligned_1024(smem_raw), 0, 0);
+}
+
+// Little work: a cluster of CLUSTER_SIZE blocks to a token and item, which join their parts out of one another's shared memory.  One token over
+// 700 keys, 16 heads of 128 over 8: 9.3 -> 7.3 us (B200).  grid: tokens x items x CLUSTER_SIZE
+template <int D, int NG>
+__global__ void __cluster_dims__(CLUSTER_SIZE) __launch_bounds__(Cfg<D, NG>::THREADS, Cfg<D, NG>::PER_SM)
+kv8_cluster_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, Kv8DecodeParams p, int items, int box) {
+    using M = Cfg<D, NG>;
+    extern __shared__ uint8_t smem_raw[];
+    uint8_t* const smem = aligned_1024(smem_raw);
+    const int rank = blockIdx.x % CLUSTER_SIZE, t = blockIdx.x / CLUSTER_SIZE / items, item = blockIdx.x / CLUSTER_SIZE % items;
+    const size_t row = (size_t)p.n_heads * p.hd;
+    p.q += t * row;
+    p.out += t * row;
+    p.positions += t;
+    p.batch_idx += t;
+    p.T = 1;
+    // (the stages are done with by the time that a block has its part)
+    p.o_part = reinterpret_cast<float*>(smem);
+    p.lse_part = p.o_part + M::HG * D;
+    const int shares = decode_block<D, NG, true>(map_k, map_v, p, Deal{items, 1, 1}, box, Parts::NONE, smem, rank, item);
+    if (shares == 1) return;                                         // (all blocks of the cluster)
+    auto meet = [] {
+        asm volatile("barrier.cluster.arrive.release;" ::: "memory");
+        asm volatile("barrier.cluster.wait.acquire;" ::: "memory");
+    };
+    meet();
+    const int group = p.n_heads / p.n_kv, hg = (group + M::HG - 1) / M::HG, h0 = item / hg * group + item % hg * M::HG, nr = min(M::HG, group - item % hg * M::HG);
+    for (int r = rank; r < nr; r += CLUSTER_SIZE)
+        for (int d = threadIdx.x * 2; d < p.hd; d += M::THREADS * 2) {
+            float lse[CLUSTER_SIZE], top = -INFINITY, den = 0.f;
+            float2 v[CLUSTER_SIZE], o = make_float2(0.f, 0.f);
+#pragma unroll
+            for (int i = 0; i < CLUSTER_SIZE; ++i) {
+                const float* other;
+                asm("mapa.u64 %0, %1, %2;" : "=l"(other) : "l"(p.o_part), "r"(i));
+                lse[i] = i < shares ? other[M::HG * D + r] : -INFINITY;
+                v[i] = i < shares ? *reinterpret_cast<const float2*>(other + r * D + d) : make_float2(0.f, 0.f);
+                top = fmaxf(top, lse[i]);
+            }
+#pragma unroll
+            for (int i = 0; i < CLUSTER_SIZE; ++i) {
+                const float f = lse[i] == -INFINITY ? 0.f : exp2f(lse[i] - top);
+                den += f;
+                o.x += f * v[i].x;
+                o.y += f * v[i].y;
+            }
+            *reinterpret_cast<uint32_t*>(p.out + (size_t)(h0 + r) * p.hd + d) = f2_to_bf162(o.x / den, o.y / den);
+        }
+    meet();                                                          // (what the others read is still there)
 }
 
 // Joins the partial results of histories that lie in several shares: the first part is its block's second partial result, the others are the first ones of
@@ -674,18 +736,51 @@ Deal deal_of(const Shape& sh, int n_heads, int n_kv, int blocks) {
 
 constexpr int WHOLE = 512;
 
+// Whether clusters are the faster form, for `jobs` tokens x items.  All of them have to run at once, and a block there must not have many more keys
+// than here, where the blocks of the device share the batch (histories of half the longest on average) and a second kernel joins.  One item of heads
+// of 128 over 700 keys: 7.3 us and 9.3 here; 16 heads over 8 key heads of 128, 1 token of 2000 keys 8.6 and 10.1, of 4000 10.4 and 10.6, of 8000 14.0
+// and 11.9, 4 tokens of 2000 9.8 and 12.9, 8 tokens (more clusters than run at once) 20.7 and 18.7; one token of 100 keys 7.0, and 6.4 whole.
+template <int D, int NG>
+bool clusters_pay(int longest, long long jobs, int blocks, int smem) {
+    if (longest <= 2 * KT || jobs * CLUSTER_SIZE > blocks || longest * (blocks - jobs * CLUSTER_SIZE / 2) > 256ll * CLUSTER_SIZE * blocks) return false;
+    static const int at_once = [=] {                                 // (the devices are alike)
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = CLUSTER_SIZE;
+        cfg.blockDim = Cfg<D, NG>::THREADS;
+        cfg.dynamicSmemBytes = smem;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = CLUSTER_SIZE;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int got = 0;
+        if (cudaOccupancyMaxActiveClusters(&got, kv8_cluster_kernel<D, NG>, &cfg) != cudaSuccess) {
+            cudaGetLastError();
+            got = 0;
+        }
+        return got;
+    }();
+    return jobs <= at_once;
+}
+
 template <int D, int NG>
 int launch(const Kv8DecodeParams* all, int T, int blocks, const Deal& deal, int longest, cudaStream_t s) {
     using M = Cfg<D, NG>;
     constexpr int smem = M::TOTAL + 1024;
     static_assert(M::PER_SM * (smem + 1024) <= 228 * 1024, "blocks per SM");
-    static SmemOptIn opt_in;
+    static SmemOptIn opt_in, cluster_opt_in;
     const int page = all->pages.page_size, box = page % 64 == 0 ? 64 : page % 32 == 0 ? 32 : 16;
     CUtensorMap mk, mv;
     int rc = map_codes(&mk, all->k_codes, all, D, box);
     if (rc == 0) rc = map_codes(&mv, all->v_codes, all, D, box);
     if (rc == 0) rc = opt_in((const void*)kv8_decode_kernel<D, NG>, smem);
+    if (rc == 0) rc = cluster_opt_in((const void*)kv8_cluster_kernel<D, NG>, smem);
     if (rc != 0) return rc;
+    if (clusters_pay<D, NG>(longest, (long long)T * deal.items, blocks, smem)) {
+        sl_launch(kv8_cluster_kernel<D, NG>, T * deal.items * CLUSTER_SIZE, M::THREADS, smem, s, mk, mv, *all, deal.items, box);
+        return SL_LAUNCH_CHECK();
+    }
     for (int t = 0; t < T; t += MAX_T) {
         Kv8DecodeParams p = *all;
         const size_t row = (size_t)p.n_heads * p.hd;

@@ -49,7 +49,25 @@ def test_decoding_of_other_pages(page):
     decode([1, 15, 16, 17, 48, 49, 500, 1030], 8, 2, 128, page=page)
 
 
-@pytest.mark.parametrize("longest", [0, 1, 512, 100000])
+@pytest.mark.parametrize("histories,h,kv,hd", [([700], 16, 8, 128), ([64, 65, 1, 0, 2048], 8, 2, 128), ([513, 1500], 16, 1, 64), ([300, 2000], 8, 1, 256),
+                                               ([128 * i + 1 for i in range(1, 9)], 6, 3, 96), ([1025], 32, 1, 80), ([449], 1, 1, 16)])
+@pytest.mark.parametrize("page", [64, 48])
+def test_decoding_in_clusters(histories, h, kv, hd, page):
+    """Little work: blocks that join their parts in shared memory; fewer tiles than blocks, rows without keys, 16 query heads a key head and more."""
+    cache, table, keys, values, g = filled([max(n, 1) for n in histories], kv, hd, 11, page)
+    q = torch.randn(len(histories), h, hd, generator=g, device="cuda").to(torch.bfloat16)
+    pos, idx = ints([n - 1 for n in histories]), torch.arange(len(histories), dtype=torch.int32, device="cuda")
+    for longest in (max(histories), 0):
+        got = K8.kv8_attention(q, cache, pos, idx, table, hd ** -0.5, max_kv_len=longest)
+        tcgen05.check_errors(q.device)
+        for b, n in enumerate(histories):
+            if n == 0:
+                assert (got[b] == 0).all()
+            else:
+                assert near(got[b:b + 1], attend(q[b:b + 1], keys[b], values[b], pos[b:b + 1], hd ** -0.5), values[b]), (longest, n)
+
+
+@pytest.mark.parametrize("longest", [0, 1, 512, 2048, 100000])
 def test_decoding_with_any_hint(longest):
     """The longest history is told for speed only: one that is wrong changes nothing but roundings."""
     cache, table, q, pos, idx, got = decode([700, 65, 1, 5000], 8, 2, 128)
@@ -125,20 +143,20 @@ def test_rows_of_any_order_views_and_streams():
     the same bits."""
     cache, table, q, pos, idx, got = decode([700, 65, 129, 2000], 8, 2, 128)
     perm = torch.tensor([2, 0, 3, 1], device="cuda")
-    again = K8.kv8_attention(q[perm], cache, pos[perm], idx[perm], table, 128 ** -0.5)
+    again = K8.kv8_attention(q[perm], cache, pos[perm], idx[perm], table, 128 ** -0.5, max_kv_len=2000)
     close = lambda a, b: torch.allclose(a.float(), b.float(), rtol=2 ** -7, atol=2 ** -12)
     assert close(again, got[perm])
     odd = torch.cat([q.new_zeros(1), q.flatten()])[1:].view_as(q)
     apart = torch.stack([q, q], 2)[:, :, 0]
     for x in (odd, apart):
-        assert torch.equal(K8.kv8_attention(x, cache, pos, idx, table, 128 ** -0.5), got)
+        assert torch.equal(K8.kv8_attention(x, cache, pos, idx, table, 128 ** -0.5, max_kv_len=2000), got)
     both = K8.kv8_attention(q[[0, 0]], cache, ints([699, 350]), ints([0, 0]), table, 128 ** -0.5)
     assert close(both[:1], got[:1])
     wide = torch.cat([table, table], 1)[:, :table.shape[1]]
     s = torch.cuda.Stream()
     s.wait_stream(torch.cuda.current_stream())
     with torch.cuda.stream(s):
-        on_s = K8.kv8_attention(q, cache, pos, idx, wide, 128 ** -0.5)
+        on_s = K8.kv8_attention(q, cache, pos, idx, wide, 128 ** -0.5, max_kv_len=2000)
     torch.cuda.current_stream().wait_stream(s)
     assert torch.equal(on_s, got)
     tcgen05.check_errors(q.device)
