@@ -98,14 +98,15 @@ struct Tiles {
     // All threads of the block.
     __device__ __forceinline__ Tiles(Batch& b, const Kv8DecodeParams& p, int most) : batch(b), T(p.T) {
         const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, warps = blockDim.x >> 5;
-        int x[2], n = 0;                             // (at least four warps)
+        constexpr int ROUNDS = (MAX_T / 32 + 2) / 3;                 // (at least three warps)
+        int x[ROUNDS], n = 0;
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < ROUNDS; ++u) {
             const int t = (warp + u * warps) * 32 + lane;
             x[u] = t < T ? note(p, b, t) : 0;
         }
 #pragma unroll
-        for (int u = 0; u < 2; ++u) {
+        for (int u = 0; u < ROUNDS; ++u) {
             const int c = warp + u * warps;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -115,9 +116,11 @@ struct Tiles {
             if (lane == 31 && c * 32 < T) b.sums[c] = x[u];
         }
         if (T > 32) __syncthreads();
-        for (int i = 0, c = warp; c * 32 < T; c += warps, ++i) {
-            for (int u = i == 0 ? 0 : c - warps; u < c; ++u) n += b.sums[u];
-            if (c * 32 + lane < T) b.before[c * 32 + lane + 1] = n + (i == 0 ? x[0] : x[1]);
+#pragma unroll
+        for (int u = 0; u < ROUNDS; ++u) {
+            const int c = warp + u * warps, t = c * 32 + lane;
+            for (int i = u == 0 ? 0 : c - warps; i < c && t < T; ++i) n += b.sums[i];
+            if (t < T) b.before[t + 1] = n + x[u];
         }
         if (threadIdx.x == 0) b.before[0] = 0;
         __syncthreads();
@@ -156,17 +159,18 @@ struct Tiles {
     }
 };
 
-// Spilled registers cost more than blocks bring (shared memory leaves no L1 to speak of): the sums of 16 heads of 128, or of 8 of 256, take the
-// registers of a block by itself.
-// Blocks an SM and warps of products; four sub-cores share the warps, and a block by itself has two on each.
-constexpr int blocks_per_sm(int width, int tiles) { return width == 64 ? 3 : width * tiles == 128 ? 2 : 1; }
+// Blocks an SM, and warps of products.  Spilled registers cost more than blocks bring (shared memory leaves no L1 to speak of): the sums of 16 heads of
+// 128, or of 8 of 256, take the registers of a block by itself, with two warps on each sub-core.  Heads of 64: four blocks with one pair of warps each
+// (200 histories of up to 2500, 16 heads a key head: 55 us; three blocks of two pairs, which spill, 57; five blocks 61; two blocks of three pairs 70).
+// Heads of 128: two blocks of two pairs (48 histories of up to 8192: 75 us; three blocks of one pair 78).
+constexpr int blocks_per_sm(int width, int tiles) { return width == 64 ? 4 : width * tiles == 128 ? 2 : 1; }
 
 template <int D, int NG>
 struct Cfg {
-    static constexpr int PER_SM = blocks_per_sm(D, NG), WARPS = PER_SM > 1 ? 4 : 6, THREADS = WARPS * 32 + 32;
+    static constexpr int PER_SM = blocks_per_sm(D, NG), WARPS = PER_SM == 4 ? 2 : PER_SM == 2 ? 4 : 6, THREADS = WARPS * 32 + 32;
     static constexpr int TURNS = WARPS / 2;                              // tiles at a time, a pair of warps to each
     static constexpr int ROW = D < 128 ? D : 128, HALVES = D / ROW;      // bytes of a row in one box, boxes
-    static constexpr int STAGES = D == 64 ? 6 : D == 256 ? 4 : NG == 1 ? 5 : 10, HG = 8 * NG;
+    static constexpr int STAGES = D == 64 ? 4 : D == 256 ? 4 : NG == 1 ? 5 : 10, HG = 8 * NG;
     static constexpr int CHUNK = D < 128 ? 8 : 16, MT = D / 16;          // neighbouring dims of a lane, 16-dim rows of products
     static constexpr int CODES = KT * D, STAGE = 2 * CODES;              // keys, values
     static constexpr int EXPS = STAGES * STAGE;                          // KT bytes of the keys, KT of the values
@@ -438,7 +442,7 @@ __device__ __forceinline__ int decode_block(const CUtensorMap& map_k, const CUte
                         }
                     }
                 };
-                constexpr bool AHEAD = NG == 1;                      // (where registers are left)
+                constexpr bool AHEAD = D == 64 || NG == 1;           // (where registers are left)
                 uint32_t early[2][4][M::CHUNK / 4];
                 if (AHEAD) {
                     values(0, 0, early[0]);
