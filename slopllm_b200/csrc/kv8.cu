@@ -3,6 +3,7 @@
 //  * kv8_store_kernel: per-head RMS norm and rotate-half of queries and keys, in fp32 from the projection rows to the one rounding of the
 //    result; keys and values are scaled by the power of two that brings their largest magnitude to (224, 448] and rounded to e4m3.
 //  * kv8_read_kernel: rows of given tokens out of their pages as bf16, which holds them exactly.
+#include "f32x2.cuh"
 #include "kv8.cuh"
 #include "prefill_attn.cuh"
 
@@ -32,17 +33,30 @@ __device__ __forceinline__ uint2 load4(const bf16* p) {
     return make_uint2((uint32_t)u[0] | (uint32_t)u[1] << 16, (uint32_t)u[2] | (uint32_t)u[3] << 16);
 }
 struct Raw { uint2 a, b; };
-__device__ __forceinline__ void unpack(const Raw& r, float (&x)[8]) {
-    const uint32_t w[4] = {r.a.x, r.a.y, r.b.x, r.b.y};
+// Eight values, two to a register pair.
+struct Values {
+    f32x2 x[4];
+    __device__ __forceinline__ explicit Values(const Raw& r) {
+        const uint32_t w[4] = {r.a.x, r.a.y, r.b.x, r.b.y};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const float2 f = bf162_to_f2(w[i]);
-        x[2 * i] = f.x;
-        x[2 * i + 1] = f.y;
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = bf162_to_f2(w[i]);
+            x[i] = pair(f.x, f.y);
+        }
     }
-}
+    __device__ __forceinline__ void to(float (&y)[8]) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float2 f = unpair(x[i]);
+            y[2 * i] = f.x;
+            y[2 * i + 1] = f.y;
+        }
+    }
+};
 
 enum Kind { QUERY, KEY, VALUE };
+
+constexpr int WARPS = 4;             // of a block of kv8_store_kernel
 
 // A row of a head has L lanes of 8 values, a warp 32 / L rows of one kind at a time; a lane keeps the angles and weights of its values for all rows.
 // EVEN: four of a lane's values and the four that they turn with, so a rotation stays in the lane; else eight neighbours, whose partners come
@@ -51,46 +65,76 @@ template <int L, bool VEC, bool EVEN>
 struct Writer {
     static constexpr int ROWS = 32 / L;
     const Kv8StoreParams& p;
-    int t, slot;                                     // token, its slot or -1
+    int t;                                           // token
+    bool placed;                                     // it has a slot: its codes at `codes`, its first head's exponents at `exps` of the cache
+    size_t codes, exps;
     int da, db, sub;                                 // the lane's first and fifth value, row of the warp's
     bool on, turning;                                // the lane has values; they are pairs of the rotation (EVEN)
     float* part;                                     // 256 values of the warp (not EVEN)
     float cs[EVEN ? 4 : 8], sn[EVEN ? 4 : 8];
 
-    template <int KIND>
-    __device__ __forceinline__ Raw fetch(int h) const {
-        const int n = KIND == QUERY ? p.n_heads : p.n_kv;
-        if (!on || h >= n) return {make_uint2(0u, 0u), make_uint2(0u, 0u)};
-        const bf16* src = KIND == QUERY ? p.q + ((size_t)t * p.ldq + (size_t)h * p.q_stride)
-                                        : (KIND == KEY ? p.k + (size_t)t * p.ldk : p.v + (size_t)t * p.ldv) + (size_t)h * p.hd;
-        return {load4<VEC>(src + da), load4<VEC>(src + db)};
+    // What a kind's values are multiplied with.  EVEN: (a, b) becomes (a aa - b ab, b bb + a ba), weights, cos and sin in one factor; else aa and bb are
+    // the weights.
+    struct Factors { f32x2 aa[2], ab[2], bb[2], ba[2]; };
+    __device__ __forceinline__ Factors factors(const bf16* weights) const {
+        Factors f;
+        Values g(Raw{make_uint2(0x3f803f80u, 0x3f803f80u), make_uint2(0x3f803f80u, 0x3f803f80u)});           // ones
+        if (on && weights != nullptr) g = Values(Raw{load4<VEC>(weights + da), load4<VEC>(weights + db)});
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            const f32x2 c = EVEN && turning ? pair(cs[2 * i], cs[2 * i + 1]) : pair(1.f, 1.f), s = EVEN ? pair(sn[2 * i], sn[2 * i + 1]) : pair(0.f, 0.f);
+            f.aa[i] = mul2(g.x[i], c);
+            f.bb[i] = mul2(g.x[2 + i], c);
+            f.ab[i] = mul2(mul2(g.x[2 + i], s), pair(-1.f, -1.f));
+            f.ba[i] = mul2(g.x[i], s);
+        }
+        return f;
     }
+    __device__ __forceinline__ static Raw load(const bf16* row, int da, int db, bool there) {
+        if (!there) return {make_uint2(0u, 0u), make_uint2(0u, 0u)};
+        return {load4<VEC>(row + da), load4<VEC>(row + db)};
+    }
+    template <int KIND>
+    __device__ __forceinline__ int heads() const { return KIND == QUERY ? p.n_heads : p.n_kv; }
+    // Row of a head (it may lie behind the last one).
+    template <int KIND>
+    __device__ __forceinline__ const bf16* source(int h) const {
+        return KIND == QUERY ? p.q + ((size_t)t * p.ldq + (size_t)h * p.q_stride) : (KIND == KEY ? p.k + (size_t)t * p.ldk : p.v + (size_t)t * p.ldv) + (size_t)h * p.hd;
+    }
+    template <int KIND>
+    __device__ __forceinline__ Raw fetch(int h) const { return load(source<KIND>(h), da, db, on && h < heads<KIND>()); }
     // Row `h` of the lane, which `raw` holds.
     template <int KIND>
-    __device__ __forceinline__ void row(int h, const Raw& raw, const float (&g)[8], bool normed, float per) const {
-        float x[8];
-        unpack(raw, x);
-        const bool there = on && h < (KIND == QUERY ? p.n_heads : p.n_kv);
-        if (KIND != VALUE && normed) {
-            float ss = 0.f;
+    __device__ __forceinline__ void row(int h, const Raw& raw, const Factors& f, bool normed, float per) const {
+        Values v(raw);
+        const bool there = on && h < heads<KIND>();
+        if (KIND != VALUE) {
+            if (normed) {
+                f32x2 sq = mul2(v.x[0], v.x[0]);
 #pragma unroll
-            for (int i = 0; i < 8; ++i) ss += x[i] * x[i];
+                for (int i = 1; i < 4; ++i) sq = fma2(v.x[i], v.x[i], sq);
+                const float2 both = unpair(sq);
+                float ss = both.x + both.y;
 #pragma unroll
-            for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            const float inv = rsqrtf(fmaf(ss, per, p.eps));
+                for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+                const float inv = rsqrtf(fmaf(ss, per, p.eps));
 #pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = x[i] * inv * g[i];
-        }
-        if (KIND != VALUE && EVEN) {
-            if (turning) {
+                for (int i = 0; i < 4; ++i) v.x[i] = mul2(v.x[i], pair(inv, inv));
+            }
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float a = x[i], b = x[4 + i];
-                    x[i] = a * cs[i] - b * sn[i];
-                    x[4 + i] = b * cs[i] + a * sn[i];
+            for (int i = 0; i < 2; ++i) {
+                const f32x2 a = v.x[i], b = v.x[2 + i];
+                v.x[i] = mul2(a, f.aa[i]);
+                v.x[2 + i] = mul2(b, f.bb[i]);
+                if (EVEN && turning) {               // (0 times a value that is not finite would not be 0)
+                    v.x[i] = fma2(b, f.ab[i], v.x[i]);
+                    v.x[2 + i] = fma2(a, f.ba[i], v.x[2 + i]);
                 }
             }
-        } else if (KIND != VALUE && p.rot_dims > 0) {
+        }
+        float x[8];
+        v.to(x);
+        if (!EVEN && KIND != VALUE && p.rot_dims > 0) {
             const int half = p.rot_dims / 2, at = (threadIdx.x & 31) * 8;
             __syncwarp();
 #pragma unroll
@@ -106,7 +150,7 @@ struct Writer {
         }
         if (KIND == QUERY) {
             if (there) {
-                bf16* dst = p.q_out + ((size_t)t * p.n_heads + h) * p.hd;
+                bf16* dst = p.q_out + (size_t)t * (uint32_t)(p.n_heads * p.hd) + (uint32_t)(h * p.hd);
                 *reinterpret_cast<uint2*>(dst + da) = make_uint2(f2_to_bf162(x[0], x[1]), f2_to_bf162(x[2], x[3]));
                 *reinterpret_cast<uint2*>(dst + db) = make_uint2(f2_to_bf162(x[4], x[5]), f2_to_bf162(x[6], x[7]));
             }
@@ -129,7 +173,7 @@ struct Writer {
 #pragma unroll
             for (int o = L / 2; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
         }
-        if (!there || slot < 0) return;
+        if (!there || !placed) return;
         // top = m 2^n with m in [1, 2), 448 = 1.75 * 2^8
         const int e = min(KV8_HIGH, max(KV8_LOW, (int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0)));
         const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
@@ -138,44 +182,51 @@ struct Writer {
         for (int i = 0; i < 8; i += 4)
             c[i / 4] = (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[i] * inv, x[i + 1] * inv), __NV_SATFINITE, __NV_E4M3) |
                        (uint32_t)__nv_cvt_float2_to_fp8x2(make_float2(x[i + 2] * inv, x[i + 3] * inv), __NV_SATFINITE, __NV_E4M3) << 16;
-        uint8_t* dst = (KIND == KEY ? p.k_codes : p.v_codes) + ((size_t)slot * p.n_kv + h) * p.hd;
+        uint8_t* dst = (KIND == KEY ? p.k_codes : p.v_codes) + codes + (uint32_t)(h * p.hd);
         *reinterpret_cast<uint32_t*>(dst + da) = c[0];
         *reinterpret_cast<uint32_t*>(dst + db) = c[1];
-        if (da == 0) p.exps[kv8_exp_at(p.pages, p.n_kv, slot, h) + (KIND == KEY ? 0 : p.pages.page_size)] = (uint8_t)(e + KV8_BIAS);
+        if (da == 0) p.exps[exps + (size_t)(2 * h + (KIND == KEY ? 0 : 1)) * p.pages.page_size] = (uint8_t)(e + KV8_BIAS);
     }
     // Heads (u, u + step, ..) * ROWS + sub of a kind; the rows of two steps are on their way.
     template <int KIND>
     __device__ __forceinline__ void rows(int u, int step, Raw next) const {
-        const int n = KIND == QUERY ? p.n_heads : p.n_kv;
+        const int n = heads<KIND>();
         if (u * ROWS >= n) return;
         const bf16* w = KIND == QUERY ? p.q_norm : KIND == KEY ? p.k_norm : nullptr;
-        Raw then = fetch<KIND>((u + step) * ROWS + sub);
-        float g[8] = {};
-        if (on && w != nullptr) unpack(Raw{load4<VEC>(w + da), load4<VEC>(w + db)}, g);
+        const size_t between = (size_t)step * ROWS * (KIND == QUERY ? p.q_stride : p.hd);
+        int h = u * ROWS + sub;
+        const bf16* src = source<KIND>(h) + between;
+        Raw then = load(src, da, db, on && h + step * ROWS < n);
+        const Factors f = factors(w);
         const float per = 1.f / (float)p.hd;
-        for (; u * ROWS < n; u += step) {
+        for (; u * ROWS < n; u += step, h += step * ROWS) {
             const Raw now = next;
             next = then;
-            then = fetch<KIND>((u + 2 * step) * ROWS + sub);
-            row<KIND>(u * ROWS + sub, now, g, w != nullptr, per);
+            src += between;
+            then = load(src, da, db, on && h + 2 * step * ROWS < n);
+            row<KIND>(h, now, f, w != nullptr, per);
         }
     }
 };
 
 // `share` warps to a token, which make its angles for themselves (a block that waits for them waits longer than they take) and take every share-th
-// step of its queries, keys and values.  Grid ceil(T * share / 8), block 256.
+// step of its queries, keys and values.  Grid ceil(T * share / WARPS).
+// What bounds it is the issue of instructions (two thirds of the cycles): fp32 math goes two values to an instruction, addresses are made once a token.
+// Blocks of four warps lie evenly on the SMs where those of eight leave a ninth idle (4096 tokens).  4096 tokens, 32 heads over 8 of 128, weights and
+// rotation: 24.7 us, 3.8 TB/s (one value to an instruction, 64-bit addresses a row, blocks of eight warps: 28.4; rows asked for ahead into L2 30.2); one
+// token 3.0 us.
 template <int L, bool VEC, bool EVEN>
-__global__ void __launch_bounds__(256, 4) kv8_store_kernel(Kv8StoreParams p, int share) {
+__global__ void __launch_bounds__(WARPS * 32, 28 / WARPS) kv8_store_kernel(const __grid_constant__ Kv8StoreParams p, int share) {
     pdl_grid_sync();
     using W = Writer<L, VEC, EVEN>;
-    __shared__ float2 turns[8][128];                 // (cos, sin) of each pair
-    __shared__ float part[EVEN ? 1 : 8][EVEN ? 1 : 256];
+    __shared__ float2 turns[WARPS][128];                 // (cos, sin) of each pair
+    __shared__ float part[EVEN ? 1 : WARPS][EVEN ? 1 : 256];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = p.rot_dims / 2, own = lane % L;
-    const long long id = (long long)blockIdx.x * 8 + warp;
+    const long long id = (long long)blockIdx.x * WARPS + warp;
     const int t = (int)(id / share), mine = (int)(id - (long long)t * share);
     if (t >= p.T) return;
     const bool turning = EVEN && own * 8 < p.rot_dims;
-    W w{p, t, -1, turning ? own * 4 : own * 8, turning ? half + own * 4 : own * 8 + 4, lane / L, own * 8 < p.hd, turning, part[EVEN ? 0 : warp]};
+    W w{p, t, false, 0, 0, turning ? own * 4 : own * 8, turning ? half + own * 4 : own * 8 + 4, lane / L, own * 8 < p.hd, turning, part[EVEN ? 0 : warp]};
     // steps are numbered through queries, keys and values: this warp's first ones
     const int uq = (p.n_heads + W::ROWS - 1) / W::ROWS, uk = (p.n_kv + W::ROWS - 1) / W::ROWS;
     const int q0 = mine, k0 = (mine + share - uq % share) % share, v0 = (k0 + share - uk % share) % share;
@@ -189,7 +240,14 @@ __global__ void __launch_bounds__(256, 4) kv8_store_kernel(Kv8StoreParams p, int
         sincospif(2.f * (float)(a - rint(a)), &sn, &cs);
         turn[i] = make_float2(cs * p.gain, sn * p.gain);
     }
-    if (pos >= 0) w.slot = kv8_slot(p.pages, 30, b, pos);
+    if (pos >= 0) {
+        const int slot = kv8_slot(p.pages, 30, b, pos);
+        if (slot >= 0) {
+            w.placed = true;
+            w.codes = (size_t)slot * (uint32_t)(p.n_kv * p.hd);
+            w.exps = kv8_exp_at(p.pages, p.n_kv, slot, 0);
+        }
+    }
     __syncwarp();
 #pragma unroll
     for (int i = 0; i < (EVEN ? 4 : 8); ++i) {
@@ -286,7 +344,8 @@ __device__ __forceinline__ void read_rows(const Kv8Rows& c, int which, int b, in
     }
 }
 
-// grid (ceil(longest / 32), R, 2), block 256: 32 rows of keys or of values
+// grid (ceil(longest / 32), R, 2), block 256: 32 rows of keys or of values.  9000 tokens of five sequences, 8 heads of 128: 27.5 us, 4.8 TB/s, of which
+// two thirds are written
 __global__ void __launch_bounds__(256) kv8_read_kernel(Kv8ReadParams p) {
     pdl_grid_sync();
     const int* r = p.ranges + blockIdx.y * 4;
@@ -332,7 +391,7 @@ __global__ void __launch_bounds__(512) kv8_unpack_kernel(Kv8UnpackParams p) {
     read_rows<HALF>(p.c, 1, b, i0, n, dst, top);
 }
 
-constexpr int WARPS_WANTED = 148 * 32;
+constexpr int WARPS_WANTED = 148 * 28;       // that are resident at once; twice as many with half of the steps each: 2048 tokens 13.8 -> 16.8 us
 
 }  // namespace
 
@@ -345,16 +404,16 @@ SL_API int sl_kv8_store(const Kv8StoreParams* p, int T, cudaStream_t s) {
     const bool vec = at % 8 == 0 && (p->ldq | p->ldk | p->ldv | p->q_stride) % 4 == 0, even = p->rot_dims % 8 == 0;
     Kv8StoreParams q = *p;
     q.T = T;
-    // warps for all sub-cores, if there are steps for them
-    const int share = max(1, min(steps, WARPS_WANTED / T));
-    const long long blocks = ((long long)T * share + 7) / 8;
+    // warps for all sub-cores, if there are steps for them; no more than need as many steps each
+    const int each = (steps - 1) / max(1, min(steps, WARPS_WANTED / T)) + 1, share = (steps - 1) / each + 1;
+    const long long blocks = ((long long)T * share + WARPS - 1) / WARPS;
     if (blocks > 0x7fffffff) return -1;
 #define SL_KS(LL)                                                                                          \
     {                                                                                                      \
-        if (vec && even) sl_launch(kv8_store_kernel<LL, true, true>, (unsigned)blocks, 256, 0, s, q, share);         \
-        else if (vec) sl_launch(kv8_store_kernel<LL, true, false>, (unsigned)blocks, 256, 0, s, q, share);           \
-        else if (even) sl_launch(kv8_store_kernel<LL, false, true>, (unsigned)blocks, 256, 0, s, q, share);          \
-        else sl_launch(kv8_store_kernel<LL, false, false>, (unsigned)blocks, 256, 0, s, q, share);                   \
+        if (vec && even) sl_launch(kv8_store_kernel<LL, true, true>, (unsigned)blocks, WARPS * 32, 0, s, q, share);         \
+        else if (vec) sl_launch(kv8_store_kernel<LL, true, false>, (unsigned)blocks, WARPS * 32, 0, s, q, share);           \
+        else if (even) sl_launch(kv8_store_kernel<LL, false, true>, (unsigned)blocks, WARPS * 32, 0, s, q, share);          \
+        else sl_launch(kv8_store_kernel<LL, false, false>, (unsigned)blocks, WARPS * 32, 0, s, q, share);                   \
     }
     if (L == 8) SL_KS(8) else if (L == 16) SL_KS(16) else SL_KS(32)
 #undef SL_KS
