@@ -71,8 +71,9 @@ class Kv8Cache:
             raise ValueError(f"codes {tuple(self.k.shape)} and {tuple(self.v.shape)} do not go with exponents {tuple(self.exps.shape)}")
         if hd % 16 or not 16 <= hd <= 256 or page_size % 16 or not page_size:
             raise ValueError(f"heads of {hd} values in pages of {page_size} tokens: the 8-bit cache takes multiples of 16, heads of up to 256")
+        device = self.k.device
         for x in (self.k, self.v, self.exps):
-            if x.dtype != torch.uint8 or not x.is_contiguous() or x.device != self.k.device:
+            if x.dtype is not torch.uint8 or not x.is_contiguous() or x.device != device:
                 raise ValueError("the tensors of an 8-bit cache are contiguous, of type uint8 and on one device")
         if (self.k.data_ptr() | self.v.data_ptr() | self.exps.data_ptr()) % 16:
             raise ValueError("the tensors of an 8-bit cache start at multiples of 16 bytes")
@@ -92,14 +93,20 @@ def _check_step(device: int, cache: Kv8Cache, *tables: torch.Tensor) -> None:
     if cache.k.get_device() != device:
         raise ValueError(f"data on device {device}, cache on {cache.k.device}")
     for t in tables:
-        if t.dtype != torch.int32 or t.get_device() != device or (t.stride(-1) != 1 and t.shape[-1] > 1):
+        if t.dtype is not torch.int32 or t.get_device() != device or not (t.is_contiguous() or t.stride(-1) == 1 or t.shape[-1] <= 1):
             raise ValueError("positions, rows, ranges and page tables are int32, on the device of the data, with values side by side")
+
+
+@lru_cache(maxsize=None)
+def _status(device: int) -> int:
+    """Address of a device's status words, which stay where they are."""
+    return tcgen05.error_flag(torch.device("cuda", device)).data_ptr()
 
 
 def _pages(cache: Kv8Cache, page_table: torch.Tensor) -> tuple:
     rows, width = page_table.shape
     return (page_table.data_ptr(), page_table.stride(0), rows, width, cache.exps.shape[3], cache.k.shape[0],
-            tcgen05.error_flag(cache.k.device).data_ptr() + 16)
+            _status(cache.k.get_device()) + 16)
 
 
 def _rows(cache: Kv8Cache, page_table: torch.Tensor) -> tuple:
@@ -108,8 +115,8 @@ def _rows(cache: Kv8Cache, page_table: torch.Tensor) -> tuple:
 
 def _call(device: int, name: str, *args) -> None:
     """A kernel call on the current stream of a device."""
-    if device == torch.cuda.current_device():
-        N.call(name, *args, N.stream())
+    if device == torch._C._cuda_getDevice():
+        N.call(name, *args, torch._C._cuda_getCurrentRawStream(device))
     else:
         with torch.cuda.device(device):
             N.call(name, *args, N.stream())
@@ -146,9 +153,9 @@ def kv8_store(q, k, v, q_norm, k_norm, rot: RotaryTable, positions, batch_idx, p
     h * q_stride), k / v [T, n_kv * hd], bf16 on a GPU with rows of any stride.  Everything is fp32 between the rows and the one rounding of a
     result (angles: position * frequency in 64 bits).  A token whose position is negative leaves the cache as it is.  Returns
     the queries [T, n_heads, hd]."""
-    T, (_, n_kv, hd), device = q.shape[0], cache.k.shape, q.get_device()
+    (T, width), (_, n_kv, hd), device = q.shape, cache.k.shape, q.get_device()
     q_stride = hd if q_stride is None else q_stride
-    if q.shape[1] != n_heads * q_stride or q_stride < hd or k.shape != (T, n_kv * hd) or v.shape != k.shape:
+    if width != n_heads * q_stride or q_stride < hd or k.shape != (T, n_kv * hd) or v.shape != k.shape:
         raise ValueError(f"projections {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)} for {n_heads} heads over {n_kv} of {hd} values")
     if rot.dims > hd or rot.freq.numel() != rot.dims // 2 or rot.dims % 2:
         raise ValueError(f"{rot.dims} rotated values with {rot.freq.numel()} frequencies in heads of {hd}")
@@ -156,18 +163,23 @@ def kv8_store(q, k, v, q_norm, k_norm, rot: RotaryTable, positions, batch_idx, p
         raise ValueError(f"{T} tokens with positions {tuple(positions.shape)} and rows {tuple(batch_idx.shape)}")
     _check_step(device, cache, positions, batch_idx, page_table)
     if device >= 0:
-        for x in (q, k, v, q_norm, k_norm):
-            if x is not None and (x.dtype != torch.bfloat16 or x.get_device() != device or x.stride(-1) != 1):
-                raise ValueError("projection rows and norm weights are bf16, on one device, with values side by side")
-        for w in (q_norm, k_norm):
-            if w is not None and w.shape != (hd,):
+        (ldq, q_by), (ldk, k_by), (ldv, v_by) = q.stride(), k.stride(), v.stride()
+        weights = [w for w in (q_norm, k_norm) if w is not None]
+        for x in (q, k, v, *weights):
+            if x.dtype is not torch.bfloat16 or x.get_device() != device:
+                raise ValueError("projection rows and norm weights are bf16 and on one device")
+        if q_by != 1 or k_by != 1 or v_by != 1 or any(w.stride(-1) != 1 for w in weights):
+            raise ValueError("the values of projection rows and norm weights lie side by side")
+        for w in weights:
+            if w.shape != (hd,):
                 raise ValueError(f"norm weights of {tuple(w.shape)} for heads of {hd} values")
-        if rot.freq.dtype != torch.float32 or rot.freq.get_device() != device or not rot.freq.is_contiguous():
+        freq = rot.freq
+        if freq.dtype is not torch.float32 or freq.get_device() != device or not freq.is_contiguous():
             raise ValueError("frequencies are fp32, contiguous and on the device of the data")
-        out = torch.empty(T, n_heads, hd, dtype=torch.bfloat16, device=q.device)
-        p = Kv8StoreParams(q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(), v.stride(0), N.ptr(q_norm), N.ptr(k_norm),
-                           rot.freq.data_ptr(), rot.gain, rot.dims, positions.data_ptr(), batch_idx.data_ptr(), *_pages(cache, page_table),
-                           n_heads, n_kv, hd, q_stride, eps, out.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.exps.data_ptr())
+        out = q.new_empty((T, n_heads, hd))
+        p = Kv8StoreParams(q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, N.ptr(q_norm), N.ptr(k_norm), freq.data_ptr(), rot.gain,
+                           rot.dims, positions.data_ptr(), batch_idx.data_ptr(), *_pages(cache, page_table), n_heads, n_kv, hd,
+                           q_stride, eps, out.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.exps.data_ptr())
         _call(device, "sl_kv8_store", C.byref(p), T)
         return out
 
@@ -232,7 +244,7 @@ def kv8_attention(q, cache: Kv8Cache, positions, batch_idx, page_table, sm_scale
                 k, v = _cached(cache, _slots(kp, torch.full_like(kp, int(batch_idx[t])), page_table, cache.page_size))
                 out[t] = R.dense_attention(q[t:t + 1], k, v, sm_scale, causal_offset=n - 1)[0]
         return out.to(q.dtype)
-    if q.dtype != torch.bfloat16:
+    if q.dtype is not torch.bfloat16:
         raise ValueError(f"queries of type {q.dtype}: the kernels take bf16")
     if not q.is_contiguous() or q.data_ptr() % 16:
         q = q.clone(memory_format=torch.contiguous_format)
@@ -245,7 +257,7 @@ def kv8_attention(q, cache: Kv8Cache, positions, batch_idx, page_table, sm_scale
         sums = part.data_ptr() + parts * 16
         p = Kv8DecodeParams(q.data_ptr(), cache.k.data_ptr(), cache.v.data_ptr(), cache.exps.data_ptr(), positions.data_ptr(), batch_idx.data_ptr(),
                             *_pages(cache, page_table), n_heads, n_kv, hd, sm_scale, out.data_ptr(), sums,
-                            sums + parts * 2 * rows * wide * 4, part.data_ptr(), 0, tcgen05.error_flag(q.device).data_ptr())
+                            sums + parts * 2 * rows * wide * 4, part.data_ptr(), 0, _status(device))
         _call(device, "sl_kv8_decode", C.byref(p), T, blocks, max_kv_len)
         return out
     _check_step(device, cache, qo_indptr)
@@ -286,5 +298,5 @@ def _prompts(q, cache, positions, batch_idx, page_table, sm_scale, qo_indptr, ma
                              exps)
         p = AttnParams(q=q.data_ptr(), k_cache=k.data_ptr(), v_cache=v.data_ptr(), positions=positions_out, batch_idx=rows_out, page_table=table,
                        pt_stride=per_seq, page_size=64, qo_indptr=ends, n_heads=n_heads, n_kv=n_kv, hd=hd, sm_scale=sm_scale, out=out.data_ptr(), T=T,
-                       num_slots=k.shape[0], max_keys=max_kv_len, err=tcgen05.error_flag(dev).data_ptr())
+                       num_slots=k.shape[0], max_keys=max_kv_len, err=_status(device))
         _call(device, "sl_kv8_prompts", C.byref(up), C.byref(p), n, int(max_q))
