@@ -275,14 +275,16 @@ struct Kv8ReadParams {
 };
 
 // Histories of sequences as pages of 64 tokens, `per_seq` to a sequence, with a page table, rows of it and positions for a kernel that reads such
-// pages.  Keys are bf16; values are, too, or (HALF) fp16 times a power of two per page and head, the largest scale of its tokens.
+// pages.  Keys are bf16; values are, too, or (HALF) fp16: of a page and head whose scales' exponents e are at most NARROW apart, codes times 2^(e - the
+// largest), which fp16 holds exactly (2^-9 2^-15 is its smallest number); else the codes alone, with e and 2^-e of each token beside them.
 struct Kv8UnpackParams {
     Kv8Rows c;
     const int *qo_indptr, *positions, *batch_idx;    // token ranges of the sequences, [T], [T]
     int per_seq;
     bf16 *k, *v;                     // [sequences * per_seq * 64, n_kv, hd]
     int *table, *rows_out, *positions_out;           // [sequences, per_seq], [T], [T]
-    int* exps;                       // [sequences, per_seq, n_kv] exponents of the values' scales (HALF)
+    int* exps;                       // [sequences, per_seq, n_kv] largest exponent of the values' scales, or KV8_WIDE (HALF)
+    float* scales;                   // [sequences, per_seq, n_kv, 2, 64] e and 2^-e, where that is KV8_WIDE
 };
 
 // 32 bytes at once
@@ -292,9 +294,10 @@ __device__ __forceinline__ void store_32(void* p, const uint32_t (&w)[8]) {
 }
 
 constexpr int READ_ROWS = 4;         // a warp's at a time
+constexpr int NARROW = 15;
 
 // Rows `first` .. first + n - 1 of page-table row b, keys (which 0) or values, -> dst: a warp takes READ_ROWS of them, a lane 16 codes of each at a time.
-// HALF: as fp16, divided by 2^top[head].
+// HALF: as fp16, divided by 2^top[head]; where that is KV8_WIDE, the codes alone.
 template <bool HALF>
 __device__ __forceinline__ void read_rows(const Kv8Rows& c, int which, int b, int first, int n, bf16* dst, const int* top = nullptr) {
     const int lane = threadIdx.x & 31, per = c.n_kv * c.hd / 16, page = c.pages.page_size;
@@ -319,8 +322,8 @@ __device__ __forceinline__ void read_rows(const Kv8Rows& c, int which, int b, in
             for (int i = 0; i < READ_ROWS; ++i)
                 if (slot[i] >= 0) {
                     u[i] = ldg_nc_16(codes + ((size_t)slot[i] * (uint32_t)per + (uint32_t)x) * 16);
-                    const uint32_t e = exps[i][(size_t)h * (uint32_t)(2 * page)];
-                    s[i] = __uint_as_float((HALF ? max(0, (int)e - top[h]) : e) << 23);      // (smaller than 2^-126: nothing is left in fp16)
+                    const int e = exps[i][(size_t)h * (uint32_t)(2 * page)];
+                    s[i] = HALF && top[h] == KV8_WIDE ? 1.f : __uint_as_float((uint32_t)(HALF ? e - top[h] : e) << 23);
                 } else {
                     u[i] = make_uint4(0u, 0u, 0u, 0u);           // (a token that is not there reads as zeros)
                     s[i] = 0.f;
@@ -383,11 +386,31 @@ __global__ void __launch_bounds__(512) kv8_unpack_kernel(Kv8UnpackParams p) {
     const int lane = threadIdx.x & 31, size = p.c.pages.page_size;
     const int s0 = lane < n ? kv8_slot(p.c.pages, 33, b, i0 + lane) : -1, s1 = lane + 32 < n ? kv8_slot(p.c.pages, 33, b, i0 + lane + 32) : -1;
     for (int h = threadIdx.x >> 5; h < p.c.n_kv; h += 16) {
-        const int e0 = s0 >= 0 ? p.c.exps[kv8_exp_at(p.c.pages, p.c.n_kv, s0, h) + size] : 0, e1 = s1 >= 0 ? p.c.exps[kv8_exp_at(p.c.pages, p.c.n_kv, s1, h) + size] : 0;
-        const int e = __reduce_max_sync(0xffffffffu, max(e0, e1));
+        int e[2], hi = -1, lo = 256;                 // bytes
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int slot = u ? s1 : s0;
+            e[u] = slot >= 0 ? p.c.exps[kv8_exp_at(p.c.pages, p.c.n_kv, slot, h) + size] : -1;
+            if (e[u] >= 0) {
+                hi = max(hi, e[u]);
+                lo = min(lo, e[u]);
+            }
+        }
+        hi = __reduce_max_sync(0xffffffffu, hi);
+        lo = __reduce_min_sync(0xffffffffu, lo);
+        const bool wide = hi - lo > NARROW;          // (not where there are none)
         if (lane == 0) {
-            top[h] = e - KV8_BIAS;
-            p.exps[(size_t)page * p.c.n_kv + h] = e - KV8_BIAS;
+            top[h] = wide ? KV8_WIDE : hi - KV8_BIAS;
+            p.exps[(size_t)page * p.c.n_kv + h] = top[h];
+        }
+        if (wide) {
+            float* const out = p.scales + ((size_t)page * p.c.n_kv + h) * 128;
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {            // (0 and 1 for tokens that are not there)
+                const int x = e[u] >= 0 ? max(-126, min(126, e[u] - KV8_BIAS)) : 0;
+                out[u * 32 + lane] = (float)x;
+                out[64 + u * 32 + lane] = __uint_as_float((uint32_t)(127 - x) << 23);
+            }
         }
     }
     __syncthreads();
@@ -445,5 +468,5 @@ SL_API int sl_kv8_prompts(const Kv8UnpackParams* up, const PagedPrefillParams* a
     else sl_launch(kv8_unpack_kernel<false>, grid, 512, 0, s, *up);
     const int rc = SL_LAUNCH_CHECK();
     if (rc != 0) return rc;
-    return half ? paged_prefill_tcgen05(attn, sequences, max_q, s, {up->exps, up->per_seq}) : sl_paged_attn_prefill(attn, sequences, max_q, s);
+    return half ? paged_prefill_tcgen05(attn, sequences, max_q, s, {up->exps, up->scales, up->per_seq}) : sl_paged_attn_prefill(attn, sequences, max_q, s);
 }

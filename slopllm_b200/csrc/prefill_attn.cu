@@ -13,9 +13,9 @@
 // 4096 tokens, 16 heads of 128 over 4, a layer: 667 us -> 103 us, 0.67 PFLOP/s; three prompts of 2500 tokens in all: 117 -> 33 us (B200).  With P in one term:
 // 85 us, and 1.3 times the error against 64 bits; the older kernel, also with one term, has that error too.
 //
-// HALF (workspaces of the 8-bit cache, kv8.cu): values are fp16 times a power of two per page and head, and P is one fp16 term: its 11 bits are enough
-// beside the output's 8, and the second product against the same values (a third of the tensor time) and the making of the second term fall away.
-// The page's exponent goes into the weights, as part of the row's reference, and out of the denominator.  Chunk of 4096 behind 8192, 32 heads of 128 over
+// HALF (workspaces of the 8-bit cache, kv8.cu): values are fp16 times a power of two per page and head, or, where a page's scales are too far apart for
+// that to be exact, per token; P is one fp16 term: its 11 bits are enough beside the output's 8, and the second product against the same values (a third of the tensor time) and the making of the second term fall away.
+// The exponents go into the weights, as part of the row's reference, and out of the denominator.  Chunk of 4096 behind 8192, 32 heads of 128 over
 // 8, with the reading of the cache (24 us): 808 to 842 us with bf16 values, 615 to 660 so (1.1 PFLOP/s; the clock follows the power limit).  The
 // products are what bounds it: of the 850 cycles a tile of 64 keys takes, S needs 8 x 76, as its operands come from shared memory (32 of arithmetic).  Blocks
 // of 256 queries with tiles of 128 keys read less for it, but a tile's next scores have no room beside its weights: 623 us.
@@ -29,7 +29,7 @@
 namespace {
 
 constexpr int QT = 128, KT = 64, STAGES = 2, THREADS = 192;
-constexpr float RAISE = 8.f;
+constexpr float RAISE = 8.f, LIFT = 6.f;         // HALF: weights are up to 2^14, so that fewer fall below fp16's normal numbers
 constexpr uint32_t COL_S = 0, COL_O = 128, TMEM_COLS = 256;
 
 template <int HD>
@@ -192,6 +192,23 @@ __global__ void __launch_bounds__(THREADS, 2) prefill_attn_kernel(const __grid_c
             ok = __all_sync(0xffffffffu, ok);
             if (!ok) break;
             tc::fence_after_sync();
+            // HALF: score * by + plus is log2 of a weight times its value's scale.  A scale per token is put in first, in TMEM (rolled loops: it is rare, and
+            // should not cost the others their registers)
+            const bool wide = HALF && exp_j == KV8_WIDE;
+            const float by = wide ? 1.f : scale, plus = wide ? 0.f : (float)exp_j;
+            const float* const scales = HALF ? half.scales + (((size_t)seq * half.per_seq + j) * p.n_kv + hkv) * 128 : nullptr;
+            if (wide) {
+#pragma unroll 1
+                for (int c = 0; c < KT; c += 16) {
+                    uint32_t o[16];
+                    tc::tmem_ld_32x16(lane_at + COL_S + (j & 1) * KT + c, o);
+                    tc::tmem_ld_wait();
+#pragma unroll
+                    for (int x = 0; x < 16; ++x) o[x] = __float_as_uint(fmaf(__uint_as_float(o[x]), scale, scales[c + x]));
+                    tc::tmem_st_32x16(lane_at + COL_S + (j & 1) * KT + c, o);
+                }
+                tc::tmem_st_wait();
+            }
             uint32_t s[2][32];
             tc::tmem_ld_32x32(lane_at + COL_S + (j & 1) * KT, s[0]);
             tc::tmem_ld_32x32(lane_at + COL_S + (j & 1) * KT + 32, s[1]);
@@ -210,7 +227,7 @@ __global__ void __launch_bounds__(THREADS, 2) prefill_attn_kernel(const __grid_c
                 t2 = fmaxf(t2, __uint_as_float(s[1][x]));
                 t3 = fmaxf(t3, __uint_as_float(s[1][x + 1]));
             }
-            const float top = HALF ? fmaf(fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)), scale, (float)exp_j) : fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * scale;
+            const float top = HALF ? fmaf(fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)), by, plus) : fmaxf(fmaxf(t0, t1), fmaxf(t2, t3)) * scale;
             if (__any_sync(0xffffffffu, top > m + RAISE)) {
                 const float mn = fmaxf(m, top), f = m == -INFINITY ? 0.f : ex2_approx(m - mn);
                 if (j > 0) {                                        // the sum so far: not while the previous product adds to it
@@ -230,15 +247,25 @@ __global__ void __launch_bounds__(THREADS, 2) prefill_attn_kernel(const __grid_c
                 l *= f;
                 m = mn;
             }
-            const float base = m == -INFINITY ? 0.f : HALF ? m - (float)exp_j : m;
-            float l0 = 0.f, l1 = 0.f;
+            const float base = m == -INFINITY ? 0.f : HALF ? m - plus - LIFT : m;
+            float l0 = 0.f, l1 = 0.f, l_wide = 0.f;
+            if (wide)
+#pragma unroll 1
+                for (int c = 0; c < KT; c += 16) {
+                    uint32_t o[16];
+                    tc::tmem_ld_32x16(lane_at + COL_S + (j & 1) * KT + c, o);
+                    tc::tmem_ld_wait();
+#pragma unroll
+                    for (int x = 0; x < 16; ++x)
+                        if (c + x <= pos - j * KT) l_wide = fmaf(ex2_approx(__uint_as_float(o[x]) - base), scales[64 + c + x], l_wide);
+                }
 #pragma unroll
             for (int part = 0; part < 2; ++part) {                  // 32 keys: 16 columns of high terms, 16 of low ones
                 uint32_t hi[16], lo[16];
 #pragma unroll
                 for (int x = 0; x < 16; ++x) {
-                    const float e0 = ex2_approx(fmaf(__uint_as_float(s[part][x * 2]), scale, -base));
-                    const float e1 = ex2_approx(fmaf(__uint_as_float(s[part][x * 2 + 1]), scale, -base));
+                    const float e0 = ex2_approx(fmaf(__uint_as_float(s[part][x * 2]), HALF ? by : scale, -base));
+                    const float e1 = ex2_approx(fmaf(__uint_as_float(s[part][x * 2 + 1]), HALF ? by : scale, -base));
                     l0 += e0;
                     l1 += e1;
                     if (HALF) {
@@ -253,7 +280,7 @@ __global__ void __launch_bounds__(THREADS, 2) prefill_attn_kernel(const __grid_c
                 tc::tmem_st_32x16(lane_at + COL_S + (j & 1) * KT + part * 16, hi);
                 if (!HALF) tc::tmem_st_32x16(lane_at + COL_S + (j & 1) * KT + 32 + part * 16, lo);
             }
-            l = HALF ? fmaf(l0 + l1, __uint_as_float((uint32_t)(127 - exp_j) << 23), l) : l + (l0 + l1);
+            l = wide ? l + l_wide : HALF ? fmaf(l0 + l1, __uint_as_float((uint32_t)(127 - exp_j) << 23), l) : l + (l0 + l1);
             tc::tmem_st_wait();
             tc::fence_before_sync();
             tc::mbar_arrive(p_ready + (j & 1));

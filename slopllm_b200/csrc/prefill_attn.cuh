@@ -23,9 +23,12 @@ struct PagedPrefillParams {
     int* err;                        // error word of bounded waits
 };
 
-// Values as fp16 times a power of two per page and key head: exponents [B, pages of a sequence, n_kv]; sequence b's pages are numbered from 0.
+// Values as fp16 times a power of two per page and key head, whose exponents are [B, pages of a sequence, n_kv]; where that is KV8_WIDE, one per token, of
+// which [B, pages, n_kv, 2, 64] exponents e and factors 2^-e.
+constexpr int KV8_WIDE = 1 << 20;
 struct HalfValues {
     const int* exps;                 // null: values are bf16
+    const float* scales;
     int per_seq;
 };
 
@@ -33,4 +36,4 @@ struct HalfValues {
 bool paged_prefill_in_tcgen05(const PagedPrefillParams* p, int B, int max_q);
 
 // Pages of 64 tokens, heads of 64 or 128 values, 16-byte aligned rows (prefill_attn.cu).
-int paged_prefill_tcgen05(const PagedPrefillParams* p, int B, int max_q, cudaStream_t s, const HalfValues& half = {nullptr, 0});
+int paged_prefill_tcgen05(const PagedPrefillParams* p, int B, int max_q, cudaStream_t s, const HalfValues& half = {nullptr, nullptr, 0});

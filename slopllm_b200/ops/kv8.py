@@ -47,7 +47,7 @@ class Kv8ReadParams(C.Structure):
 class Kv8UnpackParams(C.Structure):
     _fields_ = [*_ROWS, ("qo_indptr", C.c_void_p), ("positions", C.c_void_p), ("batch_idx", C.c_void_p), ("per_seq", C.c_int),
                 ("k", C.c_void_p), ("v", C.c_void_p), ("table", C.c_void_p), ("rows_out", C.c_void_p), ("positions_out", C.c_void_p),
-                ("exps_out", C.c_void_p)]
+                ("exps_out", C.c_void_p), ("scales", C.c_void_p)]
 
 
 class Kv8DecodeParams(C.Structure):
@@ -69,6 +69,8 @@ class Kv8Cache:
         pages, heads, two, page_size = self.exps.shape
         if self.v.shape != self.k.shape or (pages * page_size, heads, two) != (slots, n_kv, 2):
             raise ValueError(f"codes {tuple(self.k.shape)} and {tuple(self.v.shape)} do not go with exponents {tuple(self.exps.shape)}")
+        if slots >> 31:
+            raise ValueError(f"{slots} slots: they are numbered in 31 bits")
         if hd % 16 or not 16 <= hd <= 256 or page_size % 16 or not page_size:
             raise ValueError(f"heads of {hd} values in pages of {page_size} tokens: the 8-bit cache takes multiples of 16, heads of up to 256")
         device = self.k.device
@@ -285,17 +287,17 @@ def _prompts(q, cache, positions, batch_idx, page_table, sm_scale, qo_indptr, ma
     n_kv, B = cache.k.shape[1], qo_indptr.numel() - 1
     most = page_table.shape[1] * cache.page_size
     per_seq = max(1, -(-min(max_kv_len or most, most) // 64))
-    group = max(1, min(B, UNPACK_BUDGET_BYTES // (per_seq * 64 * n_kv * hd * 4)))
+    group = max(1, min(B, 65535, UNPACK_BUDGET_BYTES // (per_seq * 64 * n_kv * hd * 4)))
     k, v = (torch.empty(group * per_seq * 64, n_kv, hd, dtype=torch.bfloat16, device=dev) for _ in range(2))
     pages = group * per_seq
-    ints = torch.empty(pages * (1 + n_kv) + 2 * T, dtype=torch.int32, device=dev)
-    table, exps, rows_out = (ints.data_ptr() + 4 * i for i in (0, pages, pages * (1 + n_kv)))
+    words = torch.empty(pages * (n_kv * 129 + 1) + 2 * T, dtype=torch.int32, device=dev)
+    scales, exps, table, rows_out = (words.data_ptr() + 4 * pages * i for i in (0, n_kv * 128, n_kv * 129, n_kv * 129 + 1))
     positions_out = rows_out + 4 * T
     rows = _rows(cache, page_table)
     for s in range(0, B, group):
         n, ends = min(group, B - s), qo_indptr.data_ptr() + 4 * s
         up = Kv8UnpackParams(*rows, ends, positions.data_ptr(), batch_idx.data_ptr(), per_seq, k.data_ptr(), v.data_ptr(), table, rows_out, positions_out,
-                             exps)
+                             exps, scales)
         p = AttnParams(q=q.data_ptr(), k_cache=k.data_ptr(), v_cache=v.data_ptr(), positions=positions_out, batch_idx=rows_out, page_table=table,
                        pt_stride=per_seq, page_size=64, qo_indptr=ends, n_heads=n_heads, n_kv=n_kv, hd=hd, sm_scale=sm_scale, out=out.data_ptr(), T=T,
                        num_slots=k.shape[0], max_keys=max_kv_len, err=_status(device))

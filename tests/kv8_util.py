@@ -66,6 +66,6 @@ def attend(q, k, v, positions, scale):
 
 
 def near(got, want, values):
-    """bf16 results of fp32 attention: half a step of bf16 (2^-8 of the value), and 2^-14 of the largest cached value for weights whose
-    scores (below 64) are good to 2^-21 and whose terms are good to 2^-21."""
+    """bf16 results of fp32 attention: half a step of bf16 (2^-8 of the value), and 2^-14 of the largest cached value for scores (below 64) that are
+    good to 2^-21 and weights of one fp16 term: 2^-11 of each, of either sign, over the tens of keys that make a row's sum."""
     return bool(((got.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -14 * values.abs().max()).all())

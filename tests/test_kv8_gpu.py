@@ -307,7 +307,7 @@ def test_read(kv, hd, page):
 ])
 def test_prompts(spans, h, kv, hd, scale, page, monkeypatch):
     """(cached, new) tokens of each sequence: tile and page edges, ragged batches; all at once and in groups of sequences, with the longest history
-    known or not, and with the first sequence's tokens as two ranges.  Bound as for decoding: the same kernel as the bf16 cache's, whose weights have two terms."""
+    known or not, and with the first sequence's tokens as two ranges.  Bound as for decoding."""
     cache, table, keys, values, g = filled([c + n for c, n in spans], kv, hd, 1, page)
     T = sum(n for _, n in spans)
     q = (torch.randn(T, h, hd, generator=g, device="cuda") * scale).to(torch.bfloat16)
@@ -325,6 +325,68 @@ def test_prompts(spans, h, kv, hd, scale, page, monkeypatch):
         assert torch.equal(K8.kv8_attention(q, cache, pos, idx, table, hd ** -0.5, qo_indptr=ints(ends), max_q=max(n for _, n in spans), max_kv_len=known), got)
         monkeypatch.undo()
     tcgen05.check_errors(q.device)
+
+
+@pytest.mark.parametrize("hd", [64, 128])
+@pytest.mark.parametrize("apart", [14, 15, 16, 40, 100])
+def test_prompts_of_values_far_apart(hd, apart):
+    """Pages whose values' scales are 2^apart apart, small ones first: what a query does not see yet leaves its result alone.  Tokens 100 on are the large ones,
+    then every fifth from 300 on.  Bound as elsewhere, of the largest value that the query sees."""
+    n, kv, h = 460, 2, 4
+    cache, table, keys, _, g = filled([n], kv, hd, 5)
+    x = torch.randn(n, kv, hd, generator=g, device="cuda")
+    large = torch.zeros(n, dtype=torch.bool, device="cuda")
+    large[100:140], large[300::5] = True, True
+    x = torch.where(large[:, None, None], x * 2.0 ** (apart - apart // 2), x * 2.0 ** -(apart // 2))
+    c, e = K8.kv8_quantize(x)
+    slots = (table[0, torch.arange(n, device="cuda") // 64].long() * 64 + torch.arange(n, device="cuda") % 64)
+    cache.v[slots] = c
+    cache.exps[slots // 64, :, 1, slots % 64] = e
+    values = held(c, e)
+    first = 30
+    q = torch.randn(n - first, h, hd, generator=g, device="cuda").to(torch.bfloat16)
+    pos, idx = torch.arange(first, n, dtype=torch.int32, device="cuda"), torch.zeros(n - first, dtype=torch.int32, device="cuda")
+    got = K8.kv8_attention(q, cache, pos, idx, table, hd ** -0.5, qo_indptr=ints([0, n - first]), max_q=n - first, max_kv_len=n)
+    tcgen05.check_errors(q.device)
+    want = attend(q, keys[0], values, pos, hd ** -0.5)
+    for a, b in ((0, 100 - first), (100 - first, n - first)):
+        assert near(got[a:b], want[a:b], values[:b + first])
+
+
+def test_calls_in_a_captured_graph():
+    """A step of prompts and one of single tokens, written, attended over and read back in one graph that is replayed with other rows, on another stream."""
+    h, kv, hd, n = 8, 2, 128, 200
+    rot = rotary_table(hd, 1e4).to("cuda")
+    g = torch.Generator(device="cuda").manual_seed(4)
+    rows = lambda t: torch.randn(t, (h + 2 * kv) * hd, generator=g, device="cuda").to(torch.bfloat16)
+    table = ints([[3, 1, 0, 5]])
+    cache, plain = (K8.Kv8Cache.allocate(6, 64, kv, hd, "cuda") for _ in range(2))
+    prompt, token = rows(n), rows(1)
+    pos, last, zeros = torch.arange(n, dtype=torch.int32, device="cuda"), ints([n]), torch.zeros(n, dtype=torch.int32, device="cuda")
+    ends, ranges = ints([0, n]), ints([[0, 0, n + 1, 0]])
+
+    def step(cache):
+        out = []
+        for x, p, more in ((prompt, pos, dict(qo_indptr=ends, max_q=n, max_kv_len=n)), (token, last, dict(max_kv_len=n + 1))):
+            q, k, v = x.split([h * hd, kv * hd, kv * hd], 1)
+            q = K8.kv8_store(q, k, v, None, None, rot, p, zeros[:x.shape[0]], table, cache, h, 1e-6)
+            out.append(K8.kv8_attention(q, cache, p, zeros[:x.shape[0]], table, hd ** -0.5, **more))
+        return [*out, *K8.kv8_read(cache, ranges, n + 1, n + 1, table)]
+
+    step(cache)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(cache)
+    other = torch.cuda.Stream()
+    for _ in range(3):
+        prompt.copy_(rows(n)), token.copy_(rows(1))
+        want = step(plain)
+        other.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(other):
+            graph.replay()
+        torch.cuda.current_stream().wait_stream(other)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    tcgen05.check_errors(torch.device("cuda"))
 
 
 def test_refusals_on_a_gpu():
