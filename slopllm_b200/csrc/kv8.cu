@@ -117,7 +117,7 @@ struct Writer {
                 float ss = both.x + both.y;
 #pragma unroll
                 for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                const float inv = rsqrtf(fmaf(ss, per, p.eps));
+                const float mean = fmaf(ss, per, p.eps), r = rsqrtf(mean), inv = fmaf(0.5f * r, fmaf(-mean * r, r, 1.f), r);      // (Newton: half a step instead of two)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) v.x[i] = mul2(v.x[i], pair(inv, inv));
             }
@@ -232,13 +232,16 @@ __global__ void __launch_bounds__(WARPS * 32, 28 / WARPS) kv8_store_kernel(const
     const int q0 = mine, k0 = (mine + share - uq % share) % share, v0 = (k0 + share - uk % share) % share;
     const Raw q = w.template fetch<QUERY>(q0 * W::ROWS + w.sub), k = w.template fetch<KEY>(k0 * W::ROWS + w.sub), v = w.template fetch<VALUE>(v0 * W::ROWS + w.sub);
     const int pos = p.positions[t], b = p.batch_idx[t];
-    // fp32 keeps no digits of the angle of a far position: turns and their remainder are taken in 64 bits
+    // fp32 keeps no digits of the angle of a far position: quarter turns and their remainder are taken in 64 bits (a remainder of an eighth of a turn at
+    // most: rounded to fp32 it costs sine and cosine less than their own roundings)
     float2* const turn = turns[warp];
     for (int i = lane; i < half; i += 32) {
-        const double a = (double)pos * (double)p.freq[i] * 0.15915494309189533577;           // 1 / (2 pi)
+        const double a = (double)pos * (double)p.freq[i] * 0.63661977236758134308, whole = rint(a);      // 2 / pi
+        const int quarter = (int)(long long)whole;
         float sn, cs;
-        sincospif(2.f * (float)(a - rint(a)), &sn, &cs);
-        turn[i] = make_float2(cs * p.gain, sn * p.gain);
+        sincospif(0.5f * (float)(a - whole), &sn, &cs);
+        const float c = quarter & 1 ? -sn : cs, s = quarter & 1 ? cs : sn;
+        turn[i] = quarter & 2 ? make_float2(-c * p.gain, -s * p.gain) : make_float2(c * p.gain, s * p.gain);
     }
     if (pos >= 0) {
         const int slot = kv8_slot(p.pages, 30, b, pos);
