@@ -117,7 +117,8 @@ struct Writer {
                 float ss = both.x + both.y;
 #pragma unroll
                 for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-                const float mean = fmaf(ss, per, p.eps), r = rsqrtf(mean), inv = fmaf(0.5f * r, fmaf(-mean * r, r, 1.f), r);      // (Newton: half a step instead of two)
+                // one step of Newton: off by half a step instead of two (a root of an infinite mean is 0 as it is)
+                const float mean = fmaf(ss, per, p.eps), r = rsqrtf(mean), inv = r > 0.f ? fmaf(0.5f * r, fmaf(-mean * r, r, 1.f), r) : r;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) v.x[i] = mul2(v.x[i], pair(inv, inv));
             }

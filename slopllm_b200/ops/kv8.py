@@ -153,8 +153,8 @@ def kv8_store(q, k, v, q_norm, k_norm, rot: RotaryTable, positions, batch_idx, p
     """:func:`~slopllm_b200.ops.dense.qk_norm_rope_cache` for the 8-bit cache: per-head RMS norm (weights [hd], or None) and rotation of the first
     `rot.dims` values of queries and keys; key and value rows go into their places quantised.  q [T, n_heads * q_stride] (head h starts at
     h * q_stride), k / v [T, n_kv * hd], bf16 on a GPU with rows of any stride.  Everything is fp32 between the rows and the one rounding of a
-    result (angles: position * frequency in 64 bits).  A token whose position is negative leaves the cache as it is.  Returns
-    the queries [T, n_heads, hd]."""
+    result (angles: position * frequency in 64 bits).  A token whose position is negative leaves the cache as it is;
+    no two tokens of a call have the same place.  Returns the queries [T, n_heads, hd]."""
     (T, width), (_, n_kv, hd), device = q.shape, cache.k.shape, q.get_device()
     q_stride = hd if q_stride is None else q_stride
     if width != n_heads * q_stride or q_stride < hd or k.shape != (T, n_kv * hd) or v.shape != k.shape:
@@ -228,8 +228,9 @@ def kv8_attention(q, cache: Kv8Cache, positions, batch_idx, page_table, sm_scale
                   max_kv_len: int = 0) -> torch.Tensor:
     """:func:`~slopllm_b200.ops.dense.paged_attention` over the 8-bit cache: causal attention of each query token (position positions[t],
     page-table row batch_idx[t]) over the keys 0..position of its sequence.  q [T, n_heads, hd], bf16 on a GPU -> [T, n_heads, hd].  With
-    `qo_indptr` ([B + 1], contiguous token ranges of the sequences, at most `max_q` tokens and `max_kv_len` keys each; 0: not known) heads have 64
-    or 128 values on a GPU; without it a row may have no keys (position -1), and is zero."""
+    `qo_indptr` ([B + 1], contiguous token ranges of the sequences, at most `max_q` tokens and `max_kv_len` keys each; 0: not known; positions ascend
+    within a range) heads have 64 or 128 values on a GPU, and rows in no range are not written; without it `max_kv_len` is a hint, and a row may have
+    no keys (position -1) and is zero.  At most 1024 query heads."""
     (T, n_heads, hd), device = q.shape, q.get_device()
     _, n_kv, width = cache.k.shape
     if hd != width or n_heads % n_kv:

@@ -287,6 +287,25 @@ def test_store_of_rows_that_are_not_finite_and_of_padding():
     tcgen05.check_errors(v.device)
 
 
+def test_store_of_normed_rows_without_a_finite_mean():
+    """Means of squares of zero, beyond fp32 and infinite, as the definition on a CPU has them: zeros beside a value that is not finite."""
+    hd, w = 64, torch.ones(64, dtype=torch.bfloat16)
+    x = torch.randn(5, 2 * hd, generator=torch.Generator().manual_seed(2)).to(torch.bfloat16)
+    x[0] = 0
+    x[1, 3], x[2, 70], x[3, 5] = float("inf"), 3e38, float("nan")
+    results = []
+    for device in ("cpu", "cuda"):
+        y, weights = x.to(device), w.to(device)
+        i32 = lambda v: torch.tensor(v, dtype=torch.int32, device=device)
+        cache, table = K8.Kv8Cache.allocate(1, 64, 2, hd, device), i32([[0]])
+        q = K8.kv8_store(y, y, y, weights, weights, RotaryTable(0, torch.empty(0, device=device), 1.0), i32(list(range(5))), i32([0] * 5), table, cache, 2, 1e-6)
+        results.append([t.float().cpu() for t in (q, *K8.kv8_read(cache, i32([[0, 0, 5, 0]]), 5, 5, table))])
+    for a, b in zip(*results):
+        assert torch.equal(a.isnan(), b.isnan()) and torch.allclose(a.nan_to_num(7.0), b.nan_to_num(7.0), rtol=2.0 ** -7, atol=0)
+    assert results[0][0].isnan().any() and (results[0][0][1, 0].nan_to_num(0.0) == 0).all()
+    tcgen05.check_errors(torch.device("cuda"))
+
+
 @pytest.mark.parametrize("kv,hd,page", [(1, 16, 16), (3, 80, 64), (8, 128, 64), (2, 256, 48)])
 def test_read(kv, hd, page):
     """Ranges of all lengths and starts, in any order, and rows between them that stay as they are."""
