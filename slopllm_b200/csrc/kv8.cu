@@ -1,6 +1,6 @@
 // Writing and reading back the 8-bit key/value cache (kv8.cuh).
 //
-//  * kv8_store_kernel: per-head RMS norm and rotate-half of queries and keys, in fp32 from the projection rows to the one rounding of the
+//  * kv8_store_kernel: per-head RMS norm and rotate-half of queries (fp32) and keys (64 bits) from the projection rows to the one rounding of the
 //    result; keys and values are scaled by the power of two that brings their largest magnitude to (224, 448] and rounded to e4m3.
 //  * kv8_read_kernel: rows of given tokens out of their pages as bf16, which holds them exactly.
 #include "f32x2.cuh"
@@ -70,16 +70,16 @@ struct Writer {
     size_t codes, exps;
     int da, db, sub;                                 // the lane's first and fifth value, row of the warp's
     bool on, turning;                                // the lane has values; they are pairs of the rotation (EVEN)
-    float* part;                                     // 256 values of the warp (not EVEN)
+    double* part;                                    // 256 values of the warp (not EVEN)
+    const double2* turn;                             // (cos, sin) of each pair
     float cs[EVEN ? 4 : 8], sn[EVEN ? 4 : 8];
 
-    // What a kind's values are multiplied with.  EVEN: (a, b) becomes (a aa - b ab, b bb + a ba), weights, cos and sin in one factor; else aa and bb are
+    // What queries are multiplied with.  EVEN: (a, b) becomes (a aa - b ab, b bb + a ba), weights, cos and sin in one factor; else aa and bb are
     // the weights.
     struct Factors { f32x2 aa[2], ab[2], bb[2], ba[2]; };
-    __device__ __forceinline__ Factors factors(const bf16* weights) const {
+    __device__ __forceinline__ Factors factors(const Raw& weights) const {
         Factors f;
-        Values g(Raw{make_uint2(0x3f803f80u, 0x3f803f80u), make_uint2(0x3f803f80u, 0x3f803f80u)});           // ones
-        if (on && weights != nullptr) g = Values(Raw{load4<VEC>(weights + da), load4<VEC>(weights + db)});
+        const Values g(weights);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             const f32x2 c = EVEN && turning ? pair(cs[2 * i], cs[2 * i + 1]) : pair(1.f, 1.f), s = EVEN ? pair(sn[2 * i], sn[2 * i + 1]) : pair(0.f, 0.f);
@@ -103,12 +103,62 @@ struct Writer {
     }
     template <int KIND>
     __device__ __forceinline__ Raw fetch(int h) const { return load(source<KIND>(h), da, db, on && h < heads<KIND>()); }
+    // Keys in 64 bits: a code lies on one side or the other of the middle between two, and fp32's roundings would decide that for one in some 100
+    // thousand (none of 4.2 million now, 6 before).  `x` is rounded to odd (cut off, with the last bit set where something was), so that the one rounding of it to a code is the value's.
+    __device__ __forceinline__ void key(const Raw& raw, const Raw& weights, bool normed, float (&x)[8]) const {
+        float g[8];
+        Values(raw).to(x);
+        Values(weights).to(g);
+        double inv = 1.;
+        if (normed) {
+            double ss = 0.;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) ss = fma((double)x[i], (double)x[i], ss);
+#pragma unroll
+            for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+            const double mean = ss / (double)p.hd + (double)p.eps;
+            inv = mean > 3.4028234663852886e38 ? 0. : rsqrt(mean);   // (fp32's largest)
+        }
+        double z[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) z[i] = normed ? (double)x[i] * inv * (double)g[i] : (double)x[i];
+        if (EVEN) {
+            if (turning) {
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const double2 t = turn[da + i];
+                    const double a = z[i], b = z[4 + i];
+                    z[i] = a * t.x - b * t.y;
+                    z[4 + i] = b * t.x + a * t.y;
+                }
+            }
+        } else if (p.rot_dims > 0) {
+            const int half = p.rot_dims / 2, at = (threadIdx.x & 31) * 8;
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) part[at + i] = z[i];
+            __syncwarp();
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int d = da + i;
+                if (d >= p.rot_dims) continue;
+                const double2 t = turn[d < half ? d : d - half];
+                const double y = part[at + i + (d < half ? half : -half)];
+                z[i] = d < half ? z[i] * t.x - y * t.y : z[i] * t.x + y * t.y;
+            }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float f = __double2float_rz(z[i]);
+            x[i] = __uint_as_float(__float_as_uint(f) | ((__double2loint(z[i]) & 0x1fffffff) != 0 ? 1u : 0u));
+        }
+    }
     // Row `h` of the lane, which `raw` holds.
     template <int KIND>
-    __device__ __forceinline__ void row(int h, const Raw& raw, const Factors& f, bool normed, float per) const {
+    __device__ __forceinline__ void row(int h, const Raw& raw, const Factors& f, const Raw& weights, bool normed, float per) const {
         Values v(raw);
         const bool there = on && h < heads<KIND>();
-        if (KIND != VALUE) {
+        if (KIND == QUERY) {
             if (normed) {
                 f32x2 sq = mul2(v.x[0], v.x[0]);
 #pragma unroll
@@ -134,9 +184,11 @@ struct Writer {
             }
         }
         float x[8];
-        v.to(x);
-        if (!EVEN && KIND != VALUE && p.rot_dims > 0) {
+        if (KIND == KEY) key(raw, weights, normed, x);
+        else v.to(x);
+        if (!EVEN && KIND == QUERY && p.rot_dims > 0) {
             const int half = p.rot_dims / 2, at = (threadIdx.x & 31) * 8;
+            float* const part = reinterpret_cast<float*>(this->part);
             __syncwarp();
 #pragma unroll
             for (int i = 0; i < 8; ++i) part[at + i] = x[i];
@@ -198,36 +250,39 @@ struct Writer {
         int h = u * ROWS + sub;
         const bf16* src = source<KIND>(h) + between;
         Raw then = load(src, da, db, on && h + step * ROWS < n);
-        const Factors f = factors(w);
+        Raw g{make_uint2(0x3f803f80u, 0x3f803f80u), make_uint2(0x3f803f80u, 0x3f803f80u)};                   // ones
+        if (w != nullptr && on) g = load(w, da, db, true);
+        Factors f;
+        if (KIND == QUERY) f = factors(g);
         const float per = 1.f / (float)p.hd;
         for (; u * ROWS < n; u += step, h += step * ROWS) {
             const Raw now = next;
             next = then;
             src += between;
             then = load(src, da, db, on && h + 2 * step * ROWS < n);
-            row<KIND>(h, now, f, w != nullptr, per);
+            row<KIND>(h, now, f, g, w != nullptr, per);
         }
     }
 };
 
 // `share` warps to a token, which make its angles for themselves (a block that waits for them waits longer than they take) and take every share-th
 // step of its queries, keys and values.  Grid ceil(T * share / WARPS).
-// What bounds it is the issue of instructions (two thirds of the cycles): fp32 math goes two values to an instruction, addresses are made once a token.
-// Blocks of four warps lie evenly on the SMs where those of eight leave a ninth idle (4096 tokens).  4096 tokens, 32 heads over 8 of 128, weights and
-// rotation: 24.7 us, 3.8 TB/s (one value to an instruction, 64-bit addresses a row, blocks of eight warps: 28.4; rows asked for ahead into L2 30.2); one
-// token 3.0 us.
+// What bounds it is the issue of instructions: queries go two values to an instruction, addresses are made once a token.  Blocks of four warps lie evenly on
+// the SMs where those of eight leave a ninth idle (4096 tokens).  4096 tokens, 32 heads over 8 of 128, weights and rotation: 28.8 us, 3.3 TB/s; one token
+// 3.8 us.  With keys in fp32 24.8 and 3.0 us; then also with one value to an instruction, 64-bit addresses a row and blocks of eight warps 28.4; rows
+// asked for ahead into L2 30.2.
 template <int L, bool VEC, bool EVEN>
 __global__ void __launch_bounds__(WARPS * 32, 28 / WARPS) kv8_store_kernel(const __grid_constant__ Kv8StoreParams p, int share) {
     pdl_grid_sync();
     using W = Writer<L, VEC, EVEN>;
-    __shared__ float2 turns[WARPS][128];                 // (cos, sin) of each pair
-    __shared__ float part[EVEN ? 1 : WARPS][EVEN ? 1 : 256];
+    __shared__ double2 turns[WARPS][128];                // (cos, sin) of each pair
+    __shared__ double part[EVEN ? 1 : WARPS][EVEN ? 1 : 256];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = p.rot_dims / 2, own = lane % L;
     const long long id = (long long)blockIdx.x * WARPS + warp;
     const int t = (int)(id / share), mine = (int)(id - (long long)t * share);
     if (t >= p.T) return;
     const bool turning = EVEN && own * 8 < p.rot_dims;
-    W w{p, t, false, 0, 0, turning ? own * 4 : own * 8, turning ? half + own * 4 : own * 8 + 4, lane / L, own * 8 < p.hd, turning, part[EVEN ? 0 : warp]};
+    W w{p, t, false, 0, 0, turning ? own * 4 : own * 8, turning ? half + own * 4 : own * 8 + 4, lane / L, own * 8 < p.hd, turning, part[EVEN ? 0 : warp], turns[warp]};
     // steps are numbered through queries, keys and values: this warp's first ones
     const int uq = (p.n_heads + W::ROWS - 1) / W::ROWS, uk = (p.n_kv + W::ROWS - 1) / W::ROWS;
     const int q0 = mine, k0 = (mine + share - uq % share) % share, v0 = (k0 + share - uk % share) % share;
@@ -235,14 +290,22 @@ __global__ void __launch_bounds__(WARPS * 32, 28 / WARPS) kv8_store_kernel(const
     const int pos = p.positions[t], b = p.batch_idx[t];
     // fp32 keeps no digits of the angle of a far position: quarter turns and their remainder are taken in 64 bits (a remainder of an eighth of a turn at
     // most: rounded to fp32 it costs sine and cosine less than their own roundings)
-    float2* const turn = turns[warp];
+    double2* const turn = turns[warp];
+    const bool keys = k0 * W::ROWS < p.n_kv;         // (a warp without needs fp32)
     for (int i = lane; i < half; i += 32) {
         const double a = (double)pos * (double)p.freq[i] * 0.63661977236758134308, whole = rint(a);      // 2 / pi
         const int quarter = (int)(long long)whole;
-        float sn, cs;
-        sincospif(0.5f * (float)(a - whole), &sn, &cs);
-        const float c = quarter & 1 ? -sn : cs, s = quarter & 1 ? cs : sn;
-        turn[i] = quarter & 2 ? make_float2(-c * p.gain, -s * p.gain) : make_float2(c * p.gain, s * p.gain);
+        double sn, cs;
+        if (keys) {
+            sincospi(0.5 * (a - whole), &sn, &cs);
+        } else {
+            float s, c;
+            sincospif(0.5f * (float)(a - whole), &s, &c);
+            sn = s;
+            cs = c;
+        }
+        const double c = quarter & 1 ? -sn : cs, s = quarter & 1 ? cs : sn, gain = quarter & 2 ? -(double)p.gain : (double)p.gain;
+        turn[i] = make_double2(c * gain, s * gain);
     }
     if (pos >= 0) {
         const int slot = kv8_slot(p.pages, 30, b, pos);
@@ -256,9 +319,9 @@ __global__ void __launch_bounds__(WARPS * 32, 28 / WARPS) kv8_store_kernel(const
 #pragma unroll
     for (int i = 0; i < (EVEN ? 4 : 8); ++i) {
         const int d = w.da + i;
-        const float2 a = d < half ? turn[d] : d < p.rot_dims ? turn[d - half] : make_float2(1.f, 0.f);
-        w.cs[i] = a.x;
-        w.sn[i] = a.y;
+        const double2 a = d < half ? turn[d] : d < p.rot_dims ? turn[d - half] : make_double2(1., 0.);
+        w.cs[i] = (float)a.x;
+        w.sn[i] = (float)a.y;
     }
     w.template rows<QUERY>(q0, share, q);
     w.template rows<KEY>(k0, share, k);
@@ -421,7 +484,7 @@ __global__ void __launch_bounds__(512) kv8_unpack_kernel(Kv8UnpackParams p) {
     read_rows<HALF>(p.c, 1, b, i0, n, dst, top);
 }
 
-constexpr int WARPS_WANTED = 148 * 28;       // that are resident at once; twice as many with half of the steps each: 2048 tokens 13.8 -> 16.8 us
+constexpr int WARPS_WANTED = 148 * 28;       // that are resident at once; twice as many with half of the steps each take a fifth longer (2048 tokens)
 
 }  // namespace
 

@@ -152,8 +152,8 @@ def kv8_store(q, k, v, q_norm, k_norm, rot: RotaryTable, positions, batch_idx, p
               q_stride: Optional[int] = None) -> torch.Tensor:
     """:func:`~slopllm_b200.ops.dense.qk_norm_rope_cache` for the 8-bit cache: per-head RMS norm (weights [hd], or None) and rotation of the first
     `rot.dims` values of queries and keys; key and value rows go into their places quantised.  q [T, n_heads * q_stride] (head h starts at
-    h * q_stride), k / v [T, n_kv * hd], bf16 on a GPU with rows of any stride.  Everything is fp32 between the rows and the one rounding of a
-    result (angles: position * frequency in 64 bits).  A token whose position is negative leaves the cache as it is;
+    h * q_stride), k / v [T, n_kv * hd], bf16 on a GPU with rows of any stride.  Between the rows and the one rounding of a result everything
+    is fp32, angles (position * frequency) are 64 bits, and on a GPU keys are, too.  A token whose position is negative leaves the cache as it is;
     no two tokens of a call have the same place.  Returns the queries [T, n_heads, hd]."""
     (T, width), (_, n_kv, hd), device = q.shape, cache.k.shape, q.get_device()
     q_stride = hd if q_stride is None else q_stride
