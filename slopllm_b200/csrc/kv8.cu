@@ -103,8 +103,9 @@ struct Writer {
     }
     template <int KIND>
     __device__ __forceinline__ Raw fetch(int h) const { return load(source<KIND>(h), da, db, on && h < heads<KIND>()); }
-    // Keys in 64 bits: a code lies on one side or the other of the middle between two, and fp32's roundings would decide that for one in some 100
-    // thousand (none of 4.2 million now, 6 before).  `x` is rounded to odd (cut off, with the last bit set where something was), so that the one rounding of it to a code is the value's.
+    // Keys in 64 bits: a code lies on one side or the other of the middle between two, and fp32's roundings would decide that for one in some 700 thousand
+    // (6 of the 4.2 million of 4096 tokens, now none).  `x` is rounded to odd (cut off, with the last bit set where something was), so that the one
+    // rounding of it to a code is the value's.
     __device__ __forceinline__ void key(const Raw& raw, const Raw& weights, bool normed, float (&x)[8]) const {
         float g[8];
         Values(raw).to(x);
