@@ -14,6 +14,7 @@ from __future__ import annotations
 import ctypes as C
 from dataclasses import dataclass
 from functools import lru_cache
+from itertools import accumulate
 from typing import Optional, Tuple
 
 import torch
@@ -289,17 +290,15 @@ def _prompts(q, cache, positions, batch_idx, page_table, sm_scale, qo_indptr, ma
     most = page_table.shape[1] * cache.page_size
     per_seq = max(1, -(-min(max_kv_len or most, most) // 64))
     group = max(1, min(B, 65535, UNPACK_BUDGET_BYTES // (per_seq * 64 * n_kv * hd * 4)))
-    k, v = (torch.empty(group * per_seq * 64, n_kv, hd, dtype=torch.bfloat16, device=dev) for _ in range(2))
-    pages = group * per_seq
-    words = torch.empty(pages * (n_kv * 129 + 1) + 2 * T, dtype=torch.int32, device=dev)
-    scales, exps, table, rows_out = (words.data_ptr() + 4 * pages * i for i in (0, n_kv * 128, n_kv * 129, n_kv * 129 + 1))
+    # one piece of memory: keys, values, then what the kernels know of pages and tokens (in words of 4 bytes a page)
+    pages, page = group * per_seq, 32 * n_kv * hd
+    room = torch.empty(pages * (2 * page + 129 * n_kv + 1) + 2 * T, dtype=torch.int32, device=dev)
+    k, v, scales, exps, table, rows_out = (room.data_ptr() + 4 * pages * x for x in accumulate((0, page, page, n_kv * 128, n_kv, 1)))
     positions_out = rows_out + 4 * T
     rows = _rows(cache, page_table)
     for s in range(0, B, group):
         n, ends = min(group, B - s), qo_indptr.data_ptr() + 4 * s
-        up = Kv8UnpackParams(*rows, ends, positions.data_ptr(), batch_idx.data_ptr(), per_seq, k.data_ptr(), v.data_ptr(), table, rows_out, positions_out,
-                             exps, scales)
-        p = AttnParams(q=q.data_ptr(), k_cache=k.data_ptr(), v_cache=v.data_ptr(), positions=positions_out, batch_idx=rows_out, page_table=table,
-                       pt_stride=per_seq, page_size=64, qo_indptr=ends, n_heads=n_heads, n_kv=n_kv, hd=hd, sm_scale=sm_scale, out=out.data_ptr(), T=T,
-                       num_slots=k.shape[0], max_keys=max_kv_len, err=_status(device))
+        up = Kv8UnpackParams(*rows, ends, positions.data_ptr(), batch_idx.data_ptr(), per_seq, k, v, table, rows_out, positions_out, exps, scales)
+        p = AttnParams(q.data_ptr(), k, v, positions_out, rows_out, table, per_seq, 64, ends, n_heads, n_kv, hd, sm_scale, out.data_ptr(), T, pages * 64,
+                       max_kv_len, _status(device))
         _call(device, "sl_kv8_prompts", C.byref(up), C.byref(p), n, int(max_q))
