@@ -37,7 +37,6 @@ struct Kv8DecodeParams {
 };
 
 constexpr int KT = 64, MAX_T = 256;              // keys a tile, tokens a launch
-constexpr int CLUSTER_SIZE = 8;
 // Weights are 2^(score + exponent of the value's scale - reference).  A row's reference is raised to 2^TOP below the largest when one would be above
 // 2^(TOP + RAISE), which fp16 holds; fp32 weights reach down to 2^-126, so that two rows whose scales are the format's limits apart (2^120) are told
 // apart by weights down to 2^-14 of the largest.
@@ -181,9 +180,9 @@ struct Cfg {
     static constexpr int TOTAL = BARS + (2 * STAGES + 4) * 8;
 };
 
-// A block's part of the work; `smem`: Cfg::TOTAL bytes, aligned to 1024.  CLUSTER: of one history and `item`, shared by `CLUSTER_SIZE` blocks, of which
+// A block's part of the work; `smem`: Cfg::TOTAL bytes, aligned to 1024.  CLUSTER: of one history and `item`, shared by so many blocks, of which
 // this is number `rank`; its partial result is the first of o_part.  Returns the shares that the tiles are cut into.
-template <int D, int NG, bool CLUSTER>
+template <int D, int NG, int CLUSTER>
 __device__ __forceinline__ int decode_block(const CUtensorMap& map_k, const CUtensorMap& map_v, const Kv8DecodeParams& p, const Deal& deal, int box, Parts parts,
                                             uint8_t* smem, int rank, int only) {
     using M = Cfg<D, NG>;
@@ -205,9 +204,9 @@ __device__ __forceinline__ int decode_block(const CUtensorMap& map_k, const CUte
     }
     pdl_grid_sync();
     const int group = p.n_heads / p.n_kv, hg = (group + M::HG - 1) / M::HG;
-    const Tiles tiles(*reinterpret_cast<Batch*>(smem + M::BATCH), p, CLUSTER ? CLUSTER_SIZE : gridDim.x / deal.abreast);
+    const Tiles tiles(*reinterpret_cast<Batch*>(smem + M::BATCH), p, CLUSTER ? CLUSTER : gridDim.x / deal.abreast);
     const bool by_item = parts == Parts::BY_ITEM, by_block = parts == Parts::BY_BLOCK;
-    for (int t = CLUSTER ? rank : blockIdx.x; t < p.T; t += CLUSTER ? CLUSTER_SIZE : gridDim.x)
+    for (int t = CLUSTER ? rank : blockIdx.x; t < p.T; t += CLUSTER ? CLUSTER : gridDim.x)
         if (tiles.count(t) == 0) {
             for (int i = tid; i < p.n_heads * p.hd / 2; i += THREADS) reinterpret_cast<uint32_t*>(p.out + (size_t)t * p.n_heads * p.hd)[i] = 0u;
             if (by_item)
@@ -596,18 +595,18 @@ template <int D, int NG>
 __global__ void __launch_bounds__(Cfg<D, NG>::THREADS, Cfg<D, NG>::PER_SM) kv8_decode_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                                                                                const __grid_constant__ Kv8DecodeParams p, Deal deal, int box, Parts parts) {
     extern __shared__ uint8_t smem_raw[];
-    decode_block<D, NG, false>(map_k, map_v, p, deal, box, parts, aligned_1024(smem_raw), 0, 0);
+    decode_block<D, NG, 0>(map_k, map_v, p, deal, box, parts, aligned_1024(smem_raw), 0, 0);
 }
 
-// Little work: a cluster of CLUSTER_SIZE blocks to a token and item, which join their parts out of one another's shared memory.  One token over
-// 700 keys, 16 heads of 128 over 8: 9.3 -> 7.3 us (B200).  grid: tokens x items x CLUSTER_SIZE
-template <int D, int NG>
-__global__ void __cluster_dims__(CLUSTER_SIZE) __launch_bounds__(Cfg<D, NG>::THREADS, Cfg<D, NG>::PER_SM)
+// Little work: a cluster of SIZE blocks to a token and item, which join their parts out of one another's shared memory, in place of a second kernel
+// behind parts in global memory (figures: clusters_pay).  grid: tokens x items x SIZE
+template <int D, int NG, int SIZE>
+__global__ void __cluster_dims__(SIZE) __launch_bounds__(Cfg<D, NG>::THREADS, Cfg<D, NG>::PER_SM)
 kv8_cluster_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v, Kv8DecodeParams p, int items, int box) {
     using M = Cfg<D, NG>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* const smem = aligned_1024(smem_raw);
-    const int rank = blockIdx.x % CLUSTER_SIZE, t = blockIdx.x / CLUSTER_SIZE / items, item = blockIdx.x / CLUSTER_SIZE % items;
+    const int rank = blockIdx.x % SIZE, t = blockIdx.x / SIZE / items, item = blockIdx.x / SIZE % items;
     const size_t row = (size_t)p.n_heads * p.hd;
     p.q += t * row;
     p.out += t * row;
@@ -617,7 +616,7 @@ kv8_cluster_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     // (the stages are done with by the time that a block has its part)
     p.o_part = reinterpret_cast<float*>(smem);
     p.lse_part = p.o_part + M::HG * D;
-    const int shares = decode_block<D, NG, true>(map_k, map_v, p, Deal{items, 1, 1}, box, Parts::NONE, smem, rank, item);
+    const int shares = decode_block<D, NG, SIZE>(map_k, map_v, p, Deal{items, 1, 1}, box, Parts::NONE, smem, rank, item);
     if (shares == 1) return;                                         // (all blocks of the cluster)
     auto meet = [] {
         asm volatile("barrier.cluster.arrive.release;" ::: "memory");
@@ -625,12 +624,12 @@ kv8_cluster_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
     };
     meet();
     const int group = p.n_heads / p.n_kv, hg = (group + M::HG - 1) / M::HG, h0 = item / hg * group + item % hg * M::HG, nr = min(M::HG, group - item % hg * M::HG);
-    for (int r = rank; r < nr; r += CLUSTER_SIZE)
+    for (int r = rank; r < nr; r += SIZE)
         for (int d = threadIdx.x * 2; d < p.hd; d += M::THREADS * 2) {
-            float lse[CLUSTER_SIZE], top = -INFINITY, den = 0.f;
-            float2 v[CLUSTER_SIZE], o = make_float2(0.f, 0.f);
+            float lse[SIZE], top = -INFINITY, den = 0.f;
+            float2 v[SIZE], o = make_float2(0.f, 0.f);
 #pragma unroll
-            for (int i = 0; i < CLUSTER_SIZE; ++i) {
+            for (int i = 0; i < SIZE; ++i) {
                 const float* other;
                 asm("mapa.u64 %0, %1, %2;" : "=l"(other) : "l"(p.o_part), "r"(i));
                 lse[i] = i < shares ? other[M::HG * D + r] : -INFINITY;
@@ -638,7 +637,7 @@ kv8_cluster_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_const
                 top = fmaxf(top, lse[i]);
             }
 #pragma unroll
-            for (int i = 0; i < CLUSTER_SIZE; ++i) {
+            for (int i = 0; i < SIZE; ++i) {
                 const float f = lse[i] == -INFINITY ? 0.f : exp2f(lse[i] - top);
                 den += f;
                 o.x += f * v[i].x;
@@ -740,26 +739,28 @@ Deal deal_of(const Shape& sh, int n_heads, int n_kv, int blocks) {
 
 constexpr int WHOLE = 512;
 
-// Whether clusters are the faster form, for `jobs` tokens x items.  All of them have to run at once, and a block there must not have many more keys
-// than here, where the blocks of the device share the batch (histories of half the longest on average) and a second kernel joins.  One item of heads
-// of 128 over 700 keys: 7.3 us and 9.3 here; 16 heads over 8 key heads of 128, 1 token of 2000 keys 8.6 and 10.1, of 4000 10.4 and 10.6, of 8000 14.0
-// and 11.9, 4 tokens of 2000 9.8 and 12.9, 8 tokens (more clusters than run at once) 20.7 and 18.7; one token of 100 keys 7.0, and 6.4 whole.
-template <int D, int NG>
+// Whether clusters of SIZE are the faster form, for `jobs` tokens x items.  All of them have to run at once, and a block there must not have many more
+// keys than here, where the blocks of the device share the batch (histories of half the longest on average) and a second kernel joins: 400 more, 256 in
+// the instances for 16 heads.  16 heads over 8 key heads of 128, us in clusters and without: 1 token of 100 keys 7.0 and 6.4, of 700 7.2 and 9.3, of 2000
+// 8.2 and 10.2, of 4000 10.4 and 10.6, of 8000 14.0 and 11.9; 8 tokens of 1000 keys (clusters of 4) 9.7 and 15.0, of 2000 13.8 and 18.9, where clusters
+// of 8, more than run at once, take 20.7; 16 tokens of 500 keys (of 2) 9.4 and 15.2.  7 tokens of up to 5000 keys, 16 heads over 2 of 256: 14.4 and 17.4.
+template <int D, int NG, int SIZE>
 bool clusters_pay(int longest, long long jobs, int blocks, int smem) {
-    if (longest <= 2 * KT || jobs * CLUSTER_SIZE > blocks || longest * (blocks - jobs * CLUSTER_SIZE / 2) > 256ll * CLUSTER_SIZE * blocks) return false;
+    constexpr int MORE = NG == 2 ? 256 : 400;                        // keys
+    if (longest <= 2 * KT || jobs * SIZE > blocks || longest * (2 * blocks - jobs * SIZE) > 2ll * MORE * SIZE * blocks) return false;
     static const int at_once = [=] {                                 // (the devices are alike)
         cudaLaunchConfig_t cfg = {};
-        cfg.gridDim = CLUSTER_SIZE;
+        cfg.gridDim = SIZE;
         cfg.blockDim = Cfg<D, NG>::THREADS;
         cfg.dynamicSmemBytes = smem;
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;
-        attr[0].val.clusterDim.x = CLUSTER_SIZE;
+        attr[0].val.clusterDim.x = SIZE;
         attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
         cfg.attrs = attr;
         cfg.numAttrs = 1;
         int got = 0;
-        if (cudaOccupancyMaxActiveClusters(&got, kv8_cluster_kernel<D, NG>, &cfg) != cudaSuccess) {
+        if (cudaOccupancyMaxActiveClusters(&got, kv8_cluster_kernel<D, NG, SIZE>, &cfg) != cudaSuccess) {
             cudaGetLastError();
             got = 0;
         }
@@ -768,23 +769,36 @@ bool clusters_pay(int longest, long long jobs, int blocks, int smem) {
     return jobs <= at_once;
 }
 
+constexpr int NOT_HERE = -2;             // another form is the faster one
+
+// 0 after the launch of clusters of SIZE, or NOT_HERE, or an error.
+template <int D, int NG, int SIZE>
+int in_clusters(const CUtensorMap& mk, const CUtensorMap& mv, const Kv8DecodeParams* p, int T, int blocks, const Deal& deal, int box, int longest, int smem,
+                cudaStream_t s) {
+    static SmemOptIn opt_in;
+    const int rc = opt_in((const void*)kv8_cluster_kernel<D, NG, SIZE>, smem);       // (before it is asked how many run at once)
+    if (rc != 0) return rc;
+    if (!clusters_pay<D, NG, SIZE>(longest, (long long)T * deal.items, blocks, smem)) return NOT_HERE;
+    sl_launch(kv8_cluster_kernel<D, NG, SIZE>, T * deal.items * SIZE, Cfg<D, NG>::THREADS, smem, s, mk, mv, *p, deal.items, box);
+    return SL_LAUNCH_CHECK();
+}
+
 template <int D, int NG>
 int launch(const Kv8DecodeParams* all, int T, int blocks, const Deal& deal, int longest, cudaStream_t s) {
     using M = Cfg<D, NG>;
     constexpr int smem = M::TOTAL + 1024;
     static_assert(M::PER_SM * (smem + 1024) <= 228 * 1024, "blocks per SM");
-    static SmemOptIn opt_in, cluster_opt_in;
+    static SmemOptIn opt_in;
     const int page = all->pages.page_size, box = page % 64 == 0 ? 64 : page % 32 == 0 ? 32 : 16;
     CUtensorMap mk, mv;
     int rc = map_codes(&mk, all->k_codes, all, D, box);
     if (rc == 0) rc = map_codes(&mv, all->v_codes, all, D, box);
     if (rc == 0) rc = opt_in((const void*)kv8_decode_kernel<D, NG>, smem);
-    if (rc == 0) rc = cluster_opt_in((const void*)kv8_cluster_kernel<D, NG>, smem);
     if (rc != 0) return rc;
-    if (clusters_pay<D, NG>(longest, (long long)T * deal.items, blocks, smem)) {
-        sl_launch(kv8_cluster_kernel<D, NG>, T * deal.items * CLUSTER_SIZE, M::THREADS, smem, s, mk, mv, *all, deal.items, box);
-        return SL_LAUNCH_CHECK();
-    }
+    rc = in_clusters<D, NG, 8>(mk, mv, all, T, blocks, deal, box, longest, smem, s);
+    if (rc == NOT_HERE) rc = in_clusters<D, NG, 4>(mk, mv, all, T, blocks, deal, box, longest, smem, s);
+    if (rc == NOT_HERE) rc = in_clusters<D, NG, 2>(mk, mv, all, T, blocks, deal, box, longest, smem, s);
+    if (rc != NOT_HERE) return rc;
     for (int t = 0; t < T; t += MAX_T) {
         Kv8DecodeParams p = *all;
         const size_t row = (size_t)p.n_heads * p.hd;

@@ -50,10 +50,12 @@ def test_decoding_of_other_pages(page):
 
 
 @pytest.mark.parametrize("histories,h,kv,hd", [([700], 16, 8, 128), ([64, 65, 1, 0, 2048], 8, 2, 128), ([513, 1500], 16, 1, 64), ([300, 2000], 8, 1, 256),
-                                               ([128 * i + 1 for i in range(1, 9)], 6, 3, 96), ([1025], 32, 1, 80), ([449], 1, 1, 16)])
+                                               ([128 * i + 1 for i in range(1, 9)], 6, 3, 96), ([1025], 32, 1, 80), ([449], 1, 1, 16),
+                                               ([90 * i + 57 for i in range(8)], 16, 8, 128), ([0, 700, *range(1, 17)], 16, 8, 128),
+                                               ([15 * i + 1 for i in range(64)], 16, 1, 64), ([33 * i + 2 for i in range(30)], 8, 2, 256)])
 @pytest.mark.parametrize("page", [64, 48])
 def test_decoding_in_clusters(histories, h, kv, hd, page):
-    """Little work: blocks that join their parts in shared memory; fewer tiles than blocks, rows without keys, 16 query heads a key head and more."""
+    """Little work: eight, four or two blocks that join their parts in shared memory; fewer tiles than blocks, rows without keys, 16 query heads a key head and more."""
     cache, table, keys, values, g = filled([max(n, 1) for n in histories], kv, hd, 11, page)
     q = torch.randn(len(histories), h, hd, generator=g, device="cuda").to(torch.bfloat16)
     pos, idx = ints([n - 1 for n in histories]), torch.arange(len(histories), dtype=torch.int32, device="cuda")
