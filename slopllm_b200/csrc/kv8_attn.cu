@@ -4,10 +4,11 @@
 // All histories are cut into tiles of 64 keys of one key head (and of up to 8 or 16 of its query heads); the tiles of the whole batch, one
 // history behind the other, are dealt out in equal shares to the blocks of a head, so that a batch of ragged histories, one long history and many
 // short ones fill the device alike.  Neighbouring blocks take the heads of one share: their rows are neighbours in memory, and are read at
-// about the same time.  A history that lies in several shares leaves a partial result in each, which kv8_merge_kernel joins.
+// about the same time.  A history that lies in several shares leaves a partial result in each, which kv8_merge_kernel joins.  Where there is little work,
+// kv8_cluster_kernel joins the parts itself.
 //
 // kv8_decode_kernel: a fetching warp brings tiles (TMA, swizzled) and their exponent bytes through a ring of stages, also across the ends of
-// histories; two or three pairs of warps take tiles in turn, a warp 32 keys of one, with softmax states of their own and no barrier before a history's end.
+// histories; one to three pairs of warps take tiles in turn, a warp 32 keys of one, with softmax states of their own and no barrier before a history's end.
 //
 //   S^T = K Q^T      keys are the 16-row operand: a lane's 16 bytes of two keys are four steps of the product as they lie, since any order
 //                    of the summed dims will do that the queries follow
@@ -16,7 +17,7 @@
 // e4m3 codes become fp16 exactly (mma.sync f16, fp32 sums); the queries are fp16 times a power of two per head, which loses less than 2^-24 of
 // the largest value.  The keys' scales go onto the scores.  The values' scales go into the weights: the reference of a row is the maximum of
 // score + exponent (in powers of two), so weights times scales stay within fp16, and the denominator takes the scale out again.  Weights are
-// one fp16 term for the products (2^-12 of a weight at most, an eighth of the output's rounding to bf16) and fp32 for the denominator.
+// one fp16 term for the products (2^-11 of a weight at most, an eighth of the output's rounding to bf16) and fp32 for the denominator.
 #include "kv8.cuh"
 #include "tcgen05.cuh"
 
@@ -737,6 +738,8 @@ Deal deal_of(const Shape& sh, int n_heads, int n_kv, int blocks) {
     return {items, abreast < blocks ? abreast : blocks, abreast < blocks ? passes : (items + blocks - 1) / blocks};
 }
 
+// Longer ones cost a ragged batch more than the join (16 heads over 8 of 128, us whole and cut: 32 tokens of 500 keys 13.7 and 18.4, of 1000 19.5 and 24.4, of
+// up to 1500, ragged, 25.8 and 24.0; 48 tokens of up to 1500 34.3 and 31.5).
 constexpr int WHOLE = 512;
 
 // Whether clusters of SIZE are the faster form, for `jobs` tokens x items.  All of them have to run at once, and a block there must not have many more
