@@ -173,9 +173,10 @@ __global__ void __launch_bounds__(256) qk_norm_rope_vec_kernel(NormRopeParams p)
 constexpr int QT = 64;      // queries per CTA (4 warps x 16)
 constexpr int KT = 64;      // keys per tile
 
-// grid (ceil(max_q / 64), n_heads, B); block 128.  HD in {64, 128}; TERMS: bf16 terms of a weight.
-template <int HD, int TERMS>
-__global__ void __launch_bounds__(128) paged_attn_prefill_kernel(PagedPrefillParams p) {
+// grid (ceil(max_q / 64), n_heads, B); block 128.  HD in {64, 128}; TERMS: bf16 terms of a weight; CLEAN: of a workspace
+// whose values that are not finite are zeros (an instance of its own: ten registers are a block an SM).
+template <int HD, int TERMS, bool CLEAN>
+__global__ void __launch_bounds__(128) paged_attn_prefill_kernel(PagedPrefillParams p, SpoiledValues spoiled) {
     pdl_grid_sync();
     constexpr int DP = HD + 8;                       // padded row (16-byte aligned, bank-skewed)
     extern __shared__ __align__(16) unsigned char smraw[];
@@ -297,9 +298,15 @@ __global__ void __launch_bounds__(128) paged_attn_prefill_kernel(PagedPrefillPar
         }
     }
     const float i0 = l0 > 0.f ? 1.f / l0 : 0.f, i1 = l1 > 0.f ? 1.f / l1 : 0.f;
+    const bool bad = CLEAN && spoiled.any(seq, p.n_kv, hkv, max_pos + 1);
 #pragma unroll
     for (int i = 0; i < HD / 8; ++i) {
         const int d = i * 8 + 2 * c;
+        if (bad) {
+#pragma unroll
+            for (int x = 0; x < 4; ++x)
+                if (spoiled.seen(seq, p.n_kv, hkv, HD, x < 2 ? pos0 : pos1, d + (x & 1))) oacc[i][x] = __int_as_float(0x7fc00000);
+        }
         if (r0 < nq) *reinterpret_cast<uint32_t*>(p.out + ((size_t)(q0 + r0) * p.n_heads + hq) * HD + d) = f2_to_bf162(oacc[i][0] * i0, oacc[i][1] * i0);
         if (r1 < nq) *reinterpret_cast<uint32_t*>(p.out + ((size_t)(q0 + r1) * p.n_heads + hq) * HD + d) = f2_to_bf162(oacc[i][2] * i1, oacc[i][3] * i1);
     }
@@ -340,28 +347,35 @@ bool paged_prefill_in_tcgen05(const PagedPrefillParams* p, int B, int max_q) {
            max_q <= 65535 * 128 && (((uintptr_t)p->q | (uintptr_t)p->k_cache | (uintptr_t)p->v_cache | (uintptr_t)p->out) & 15) == 0 && !short_prefill(p, B, max_q);
 }
 
-template <int HD, int TERMS>
-static void launch_prefill(const PagedPrefillParams* p, dim3 grid, cudaStream_t s) {
+template <int HD, int TERMS, bool CLEAN>
+static void launch_prefill(const PagedPrefillParams* p, dim3 grid, cudaStream_t s, const SpoiledValues& spoiled) {
     const size_t smem = (size_t)3 * 64 * (HD + 8) * sizeof(bf16);
-    auto kern = paged_attn_prefill_kernel<HD, TERMS>;
+    auto kern = paged_attn_prefill_kernel<HD, TERMS, CLEAN>;
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem);
-    sl_launch(kern, grid, 128, smem, s, *p);
+    sl_launch(kern, grid, 128, smem, s, *p, spoiled);
 }
 
-// Causal attention of B sequences' query ranges over their cached keys 0..position.  hd in {64, 128}.
-SL_API int sl_paged_attn_prefill(const PagedPrefillParams* p, int B, int max_q, cudaStream_t s) {
+template <bool CLEAN>
+static int prefill(const PagedPrefillParams* p, int B, int max_q, cudaStream_t s, const SpoiledValues& spoiled) {
     if (B == 0 || max_q == 0) return 0;
     if (p->n_heads % p->n_kv != 0) return -1;
     dim3 grid((max_q + QT - 1) / QT, p->n_heads, B);
     if (p->page_size == 64 && (p->hd == 128 || p->hd == 64) && p->err != nullptr && p->sm_scale > 0.f && B <= 65535 && max_q <= 65535 * 128 &&
         (((uintptr_t)p->q | (uintptr_t)p->k_cache | (uintptr_t)p->v_cache | (uintptr_t)p->out) & 15) == 0) {
         if (!short_prefill(p, B, max_q)) return paged_prefill_tcgen05(p, B, max_q, s);
-        if (p->hd == 128) launch_prefill<128, 2>(p, grid, s);
-        else launch_prefill<64, 2>(p, grid, s);
+        if (p->hd == 128) launch_prefill<128, 2, CLEAN>(p, grid, s, spoiled);
+        else launch_prefill<64, 2, CLEAN>(p, grid, s, spoiled);
         return SL_LAUNCH_CHECK();
     }
-    if (p->hd == 128) launch_prefill<128, 1>(p, grid, s);
-    else if (p->hd == 64) launch_prefill<64, 1>(p, grid, s);
+    if (p->hd == 128) launch_prefill<128, 1, CLEAN>(p, grid, s, spoiled);
+    else if (p->hd == 64) launch_prefill<64, 1, CLEAN>(p, grid, s, spoiled);
     else return -1;
     return SL_LAUNCH_CHECK();
 }
+
+// Causal attention of B sequences' query ranges over their cached keys 0..position.  hd in {64, 128}.
+SL_API int sl_paged_attn_prefill(const PagedPrefillParams* p, int B, int max_q, cudaStream_t s) {
+    return prefill<false>(p, B, max_q, s, {nullptr, nullptr, 0});
+}
+
+int paged_prefill(const PagedPrefillParams* p, int B, int max_q, cudaStream_t s, const SpoiledValues& spoiled) { return prefill<true>(p, B, max_q, s, spoiled); }

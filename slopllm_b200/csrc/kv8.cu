@@ -353,6 +353,7 @@ struct Kv8UnpackParams {
     int *table, *rows_out, *positions_out;           // [sequences, per_seq], [T], [T]
     int* exps;                       // [sequences, per_seq, n_kv] largest exponent of the values' scales, or KV8_WIDE (HALF)
     float* scales;                   // [sequences, per_seq, n_kv, 2, 64] e and 2^-e, where that is KV8_WIDE
+    int* spoiled_pages; uint8_t* spoiled_dims;       // SpoiledValues
 };
 
 // 32 bytes at once
@@ -364,13 +365,18 @@ __device__ __forceinline__ void store_32(void* p, const uint32_t (&w)[8]) {
 constexpr int READ_ROWS = 4;         // a warp's at a time
 constexpr int NARROW = 15;
 
+// NaN codes among four: 0x80 in their bytes.
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
+
 // Rows `first` .. first + n - 1 of page-table row b, keys (which 0) or values, -> dst: a warp takes READ_ROWS of them, a lane 16 codes of each at a time.
-// HALF: as fp16, divided by 2^top[head]; where that is KV8_WIDE, the codes alone.
-template <bool HALF>
-__device__ __forceinline__ void read_rows(const Kv8Rows& c, int which, int b, int first, int n, bf16* dst, const int* top = nullptr) {
+// HALF: as fp16, divided by 2^top[head]; where that is KV8_WIDE, the codes alone.  CLEAN: NaN codes as zeros, and the first row with one to
+// spoiled[head]; returns whether this thread found one.
+template <bool HALF, bool CLEAN>
+__device__ __forceinline__ bool read_rows(const Kv8Rows& c, int which, int b, int first, int n, bf16* dst, const int* top, int* spoiled) {
     const int lane = threadIdx.x & 31, per = c.n_kv * c.hd / 16, page = c.pages.page_size;
     const uint32_t of_head = (1u << 27) / (uint32_t)(c.hd / 16) + 1;             // x / (hd / 16) is (x * of_head) >> 27: x < 2^14, so it is off by less than 1 / 16
     const uint8_t* codes = which ? c.v_codes : c.k_codes;
+    bool found = false;
     for (int i0 = (threadIdx.x >> 5) * READ_ROWS; i0 < n; i0 += (blockDim.x >> 5) * READ_ROWS) {
         // a lane looks up one of the rows
         const int mine = i0 + lane < n && lane < READ_ROWS ? kv8_slot(c.pages, 31, b, first + i0 + lane) : -1;
@@ -399,7 +405,13 @@ __device__ __forceinline__ void read_rows(const Kv8Rows& c, int which, int b, in
 #pragma unroll
             for (int i = 0; i < READ_ROWS; ++i) {
                 if (i0 + i >= n) continue;
-                const uint32_t in[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+                uint32_t in[4] = {u[i].x, u[i].y, u[i].z, u[i].w};
+                if (CLEAN && (nan_codes(in[0]) | nan_codes(in[1]) | nan_codes(in[2]) | nan_codes(in[3])) != 0u) {
+                    found = true;
+                    atomicMin(spoiled + h, i0 + i);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) in[k] &= ~((nan_codes(in[k]) >> 7) * 255u);
+                }
                 uint32_t out[8];
 #pragma unroll
                 for (int k = 0; k < 8; ++k) {
@@ -416,6 +428,7 @@ __device__ __forceinline__ void read_rows(const Kv8Rows& c, int which, int b, in
             }
         }
     }
+    return found;
 }
 
 // grid (ceil(longest / 32), R, 2), block 256: 32 rows of keys or of values.  9000 tokens of five sequences, 8 heads of 128: 23.5 us, 5.6 TB/s, of which
@@ -425,14 +438,15 @@ __global__ void __launch_bounds__(256, 4) kv8_read_kernel(Kv8ReadParams p) {
     const int* r = p.ranges + blockIdx.y * 4;
     const int i0 = blockIdx.x * 32, n = min(32, r[2] - i0), out = r[3] + i0;
     if (n <= 0 || !guard_ok(p.c.pages.guard, 31, out, (long long)p.rows - n + 1)) return;
-    read_rows<false>(p.c, blockIdx.z, r[0], r[1] + i0, n, (blockIdx.z ? p.v : p.k) + (size_t)out * p.c.n_kv * p.c.hd);
+    read_rows<false, false>(p.c, blockIdx.z, r[0], r[1] + i0, n, (blockIdx.z ? p.v : p.k) + (size_t)out * p.c.n_kv * p.c.hd, nullptr, nullptr);
 }
 
 // grid (per_seq, sequences, 2), block 512: a page of a sequence's workspace, keys or values
 template <bool HALF>
-__global__ void __launch_bounds__(512) kv8_unpack_kernel(Kv8UnpackParams p) {
+__global__ void __launch_bounds__(512, 2) kv8_unpack_kernel(Kv8UnpackParams p) {
     pdl_grid_sync();
     __shared__ int top[HALF ? KV8_HEADS : 1];        // exponents of the page's values
+    __shared__ int spoiled[KV8_HEADS];               // first row with a value that is not finite
     const int s = blockIdx.y, page = s * p.per_seq + blockIdx.x, q0 = p.qo_indptr[s], q1 = p.qo_indptr[s + 1], most = p.per_seq * 64;
     if (q0 >= q1) return;
     int n = p.positions[q1 - 1] + 1;                 // positions ascend within a sequence
@@ -447,13 +461,14 @@ __global__ void __launch_bounds__(512) kv8_unpack_kernel(Kv8UnpackParams p) {
     n = min(64, n - i0);
     if (n <= 0) return;
     bf16* dst = (blockIdx.z ? p.v : p.k) + (size_t)page * 64 * p.c.n_kv * p.c.hd;
-    if (!HALF || blockIdx.z == 0) {
-        read_rows<false>(p.c, blockIdx.z, b, i0, n, dst);
+    if (blockIdx.z == 0) {
+        read_rows<false, false>(p.c, 0, b, i0, n, dst, nullptr, nullptr);
         return;
     }
     const int lane = threadIdx.x & 31, size = p.c.pages.page_size;
+    for (int h = threadIdx.x; h < p.c.n_kv; h += 512) p.spoiled_pages[(size_t)page * p.c.n_kv + h] = spoiled[h] = 64;
     const int s0 = lane < n ? kv8_slot(p.c.pages, 33, b, i0 + lane) : -1, s1 = lane + 32 < n ? kv8_slot(p.c.pages, 33, b, i0 + lane + 32) : -1;
-    for (int h = threadIdx.x >> 5; h < p.c.n_kv; h += 16) {
+    for (int h = threadIdx.x >> 5; HALF && h < p.c.n_kv; h += 16) {
         int e[2], hi = -1, lo = 256;                 // bytes
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -482,7 +497,20 @@ __global__ void __launch_bounds__(512) kv8_unpack_kernel(Kv8UnpackParams p) {
         }
     }
     __syncthreads();
-    read_rows<HALF>(p.c, 1, b, i0, n, dst, top);
+    if (__syncthreads_or(read_rows<HALF, true>(p.c, 1, b, i0, n, dst, top, spoiled)) == 0) return;
+    for (int h = threadIdx.x >> 5; h < p.c.n_kv; h += 16) {          // (rare: the codes are read once more)
+        const size_t at = (size_t)page * p.c.n_kv + h;
+        if (spoiled[h] == 64) continue;
+        if (lane == 0) p.spoiled_pages[at] = spoiled[h];
+        for (int d = lane; d < p.c.hd; d += 32) {
+            int first = 64;
+            for (int t = spoiled[h]; t < n && first == 64; ++t) {
+                const int slot = kv8_slot(p.c.pages, 33, b, i0 + t);
+                if (slot >= 0 && (p.c.v_codes[((size_t)slot * p.c.n_kv + h) * p.c.hd + d] & 0x7f) == 0x7f) first = t;
+            }
+            p.spoiled_dims[at * p.c.hd + d] = (uint8_t)first;
+        }
+    }
 }
 
 constexpr int WARPS_WANTED = 148 * 28;       // that are resident at once; twice as many with half of the steps each take a fifth longer (2048 tokens)
@@ -536,5 +564,6 @@ SL_API int sl_kv8_prompts(const Kv8UnpackParams* up, const PagedPrefillParams* a
     else sl_launch(kv8_unpack_kernel<false>, grid, 512, 0, s, *up);
     const int rc = SL_LAUNCH_CHECK();
     if (rc != 0) return rc;
-    return half ? paged_prefill_tcgen05(attn, sequences, max_q, s, {up->exps, up->scales, up->per_seq}) : sl_paged_attn_prefill(attn, sequences, max_q, s);
+    const SpoiledValues spoiled = {up->spoiled_pages, up->spoiled_dims, up->per_seq};
+    return half ? paged_prefill_tcgen05(attn, sequences, max_q, s, {up->exps, up->scales, up->per_seq}, spoiled) : paged_prefill(attn, sequences, max_q, s, spoiled);
 }

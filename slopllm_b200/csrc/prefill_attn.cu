@@ -21,8 +21,9 @@
 // operands come from shared memory (32 of arithmetic), and 256 for P V.  Blocks of 256 queries with tiles of 128 keys read less for S, but a tile's next
 // scores have no room beside its weights: 623 us.
 //
-// Rows of the last page behind the last visible key may hold anything: their scores are masked, their values zeroed in shared memory.  A value
-// that is not finite in front of it reaches all queries of its block, whose weights for it may be 0 (the other kernel's blocks have 64 queries).
+// Rows of the last page behind the last visible key may hold anything: their scores are masked, their values zeroed in shared memory.  A bf16 value
+// that is not finite in front of it reaches all queries of its block, whose weights for it may be 0 (the other kernel's blocks have 64 queries).  HALF: only
+// the queries that see it, to whose results it is added at the end (SpoiledValues).
 // Waits are bounded; one that runs out sets the error word and ends the block.
 #include "prefill_attn.cuh"
 #include "tcgen05.cuh"
@@ -52,7 +53,8 @@ __device__ __forceinline__ float ex2_approx(float x) {
 // grid (heads, ceil(max_q / 128), B), block 192
 template <int HD, bool HALF>
 __global__ void __launch_bounds__(THREADS, 2) prefill_attn_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_k,
-                                                                  const __grid_constant__ CUtensorMap map_v, PagedPrefillParams p, HalfValues half) {
+                                                                  const __grid_constant__ CUtensorMap map_v, PagedPrefillParams p, HalfValues half,
+                                                                  SpoiledValues spoiled) {
     extern __shared__ uint8_t smem_raw[];
     using M = Smem<HD>;
     uint8_t* smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
@@ -186,6 +188,7 @@ __global__ void __launch_bounds__(THREADS, 2) prefill_attn_kernel(const __grid_c
         bool ok = true;
         const int* exps = HALF ? half.exps + (size_t)seq * half.per_seq * p.n_kv + hkv : nullptr;
         int next_exp = HALF ? exps[0] : 0;
+        const bool bad = HALF && spoiled.any(seq, p.n_kv, hkv, n_keys);         // (while the first rows are on their way)
         for (int j = 0; j < tiles; ++j) {
             const int exp_j = next_exp;                             // of the tile's values
             if (HALF && j + 1 < tiles) next_exp = exps[(size_t)(j + 1) * p.n_kv];
@@ -297,6 +300,14 @@ __global__ void __launch_bounds__(THREADS, 2) prefill_attn_kernel(const __grid_c
                 uint32_t o[32];
                 tc::tmem_ld_32x32(lane_at + COL_O + c, o);
                 tc::tmem_ld_wait();
+                if (bad) {
+                    uint32_t nan = 0;
+#pragma unroll 1
+                    for (int x = 0; x < 32; ++x) nan |= (uint32_t)spoiled.seen(seq, p.n_kv, hkv, HD, pos, c + x) << x;
+#pragma unroll
+                    for (int x = 0; x < 32; ++x)
+                        if (nan >> x & 1) o[x] = 0x7fc00000u;
+                }
                 if (r < nq)
 #pragma unroll
                     for (int x = 0; x < 32; x += 8) {
@@ -321,7 +332,7 @@ __global__ void __launch_bounds__(THREADS, 2) prefill_attn_kernel(const __grid_c
 }
 
 template <int HD, bool HALF>
-int launch(const PagedPrefillParams* p, int B, int max_q, cudaStream_t s, const HalfValues& half) {
+int launch(const PagedPrefillParams* p, int B, int max_q, cudaStream_t s, const HalfValues& half, const SpoiledValues& spoiled) {
     CUtensorMap mq, mk, mv;
     int r = make_tmap_2d(&mq, p->q, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p->T, (uint64_t)p->n_heads * HD, (uint64_t)p->n_heads * HD * 2, QT, 64);
     if (r == 0) r = make_tmap_2d(&mk, p->k_cache, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, p->num_slots, (uint64_t)p->n_kv * HD, (uint64_t)p->n_kv * HD * 2, KT, 64);
@@ -331,13 +342,13 @@ int launch(const PagedPrefillParams* p, int B, int max_q, cudaStream_t s, const 
     constexpr int smem = Smem<HD>::TOTAL + 1024;
     static_assert(2 * (smem + 1024) <= 228 * 1024, "two blocks per SM");
     cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, smem);
-    sl_launch(kern, dim3(p->n_heads, (max_q + QT - 1) / QT, B), THREADS, smem, s, mq, mk, mv, *p, half);
+    sl_launch(kern, dim3(p->n_heads, (max_q + QT - 1) / QT, B), THREADS, smem, s, mq, mk, mv, *p, half, spoiled);
     return SL_LAUNCH_CHECK();
 }
 
 }  // namespace
 
-int paged_prefill_tcgen05(const PagedPrefillParams* p, int B, int max_q, cudaStream_t s, const HalfValues& half) {
-    if (half.exps != nullptr) return p->hd == 128 ? launch<128, true>(p, B, max_q, s, half) : launch<64, true>(p, B, max_q, s, half);
-    return p->hd == 128 ? launch<128, false>(p, B, max_q, s, half) : launch<64, false>(p, B, max_q, s, half);
+int paged_prefill_tcgen05(const PagedPrefillParams* p, int B, int max_q, cudaStream_t s, const HalfValues& half, const SpoiledValues& spoiled) {
+    if (half.exps != nullptr) return p->hd == 128 ? launch<128, true>(p, B, max_q, s, half, spoiled) : launch<64, true>(p, B, max_q, s, half, spoiled);
+    return p->hd == 128 ? launch<128, false>(p, B, max_q, s, half, spoiled) : launch<64, false>(p, B, max_q, s, half, spoiled);
 }

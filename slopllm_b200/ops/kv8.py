@@ -48,7 +48,7 @@ class Kv8ReadParams(C.Structure):
 class Kv8UnpackParams(C.Structure):
     _fields_ = [*_ROWS, ("qo_indptr", C.c_void_p), ("positions", C.c_void_p), ("batch_idx", C.c_void_p), ("per_seq", C.c_int),
                 ("k", C.c_void_p), ("v", C.c_void_p), ("table", C.c_void_p), ("rows_out", C.c_void_p), ("positions_out", C.c_void_p),
-                ("exps_out", C.c_void_p), ("scales", C.c_void_p)]
+                ("exps_out", C.c_void_p), ("scales", C.c_void_p), ("spoiled_pages", C.c_void_p), ("spoiled_dims", C.c_void_p)]
 
 
 class Kv8DecodeParams(C.Structure):
@@ -283,8 +283,8 @@ def _decode_plan(device: int, n_heads: int, n_kv: int, hd: int) -> Tuple[int, ..
 
 def _prompts(q, cache, positions, batch_idx, page_table, sm_scale, qo_indptr, max_q, max_kv_len, out) -> None:
     """Histories are read back into pages of 64 tokens (keys bf16; values fp16 with a power of two per page and head, where the tcgen05 kernel
-    takes them), over which the prompt kernel attends.  Done once per key head and token, that costs less than codes that every block of the
-    kernel (query heads x 128 queries) turns into an operand anew."""
+    takes them; values that are not finite as zeros, with a note of where they were), over which the prompt kernel attends.  Done once per key
+    head and token, that costs less than codes that every block of the kernel (query heads x 128 queries) turns into an operand anew."""
     (T, n_heads, hd), device, dev = q.shape, q.get_device(), q.device
     n_kv, B = cache.k.shape[1], qo_indptr.numel() - 1
     most = page_table.shape[1] * cache.page_size
@@ -292,13 +292,15 @@ def _prompts(q, cache, positions, batch_idx, page_table, sm_scale, qo_indptr, ma
     group = max(1, min(B, 65535, UNPACK_BUDGET_BYTES // (per_seq * 64 * n_kv * hd * 4)))
     # one piece of memory: keys, values, then what the kernels know of pages and tokens (in words of 4 bytes a page)
     pages, page = group * per_seq, 32 * n_kv * hd
-    room = torch.empty(pages * (2 * page + 129 * n_kv + 1) + 2 * T, dtype=torch.int32, device=dev)
-    k, v, scales, exps, table, rows_out = (room.data_ptr() + 4 * pages * x for x in accumulate((0, page, page, n_kv * 128, n_kv, 1)))
+    parts = (page, page, n_kv * 128, n_kv, n_kv, n_kv * hd // 4, 1)
+    room = torch.empty(pages * sum(parts) + 2 * T, dtype=torch.int32, device=dev)
+    k, v, scales, exps, spoiled, dims, table, rows_out = (room.data_ptr() + 4 * pages * x for x in accumulate((0, *parts)))
     positions_out = rows_out + 4 * T
     rows = _rows(cache, page_table)
     for s in range(0, B, group):
         n, ends = min(group, B - s), qo_indptr.data_ptr() + 4 * s
-        up = Kv8UnpackParams(*rows, ends, positions.data_ptr(), batch_idx.data_ptr(), per_seq, k, v, table, rows_out, positions_out, exps, scales)
+        up = Kv8UnpackParams(*rows, ends, positions.data_ptr(), batch_idx.data_ptr(), per_seq, k, v, table, rows_out, positions_out, exps, scales,
+                             spoiled, dims)
         p = AttnParams(q.data_ptr(), k, v, positions_out, rows_out, table, per_seq, 64, ends, n_heads, n_kv, hd, sm_scale, out.data_ptr(), T, pages * 64,
                        max_kv_len, _status(device))
         _call(device, "sl_kv8_prompts", C.byref(up), C.byref(p), n, int(max_q))

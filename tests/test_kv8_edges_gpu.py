@@ -1,0 +1,66 @@
+"""The 8-bit key/value cache on a GPU where it is easily wrong: codes at the middle between two, bits that must not depend on the batch, weights of values whose
+scales are the format's limits apart, values that are not finite behind a query, workspaces, ranges without keys."""
+import pytest
+import torch
+
+from kv8_util import attend, filled, held, near
+from slopllm_b200.ops import kv8 as K8
+from slopllm_b200.ops import tcgen05
+
+pytestmark = pytest.mark.gpu
+
+
+def ints(x):
+    return torch.tensor(x, dtype=torch.int32, device="cuda")
+
+
+def put(cache, table, b, positions, which, rows):
+    """fp32 rows [n, kv, hd] into places of sequence b, as keys (0) or values (1); what the cache then holds of them."""
+    codes, exps = K8.kv8_quantize(rows)
+    page = cache.page_size
+    slots = table[b, (positions // page).long()].long() * page + positions.long() % page
+    (cache.v if which else cache.k)[slots] = codes
+    cache.exps[slots // page, :, which, slots % page] = exps
+    return held(codes, exps)
+
+
+@pytest.mark.parametrize("apart", [0, 40])
+@pytest.mark.parametrize("n,first,h,kv,hd,scale", [(300, 0, 4, 2, 128, 0.1), (300, 100, 8, 2, 64, 0.1), (300, 0, 4, 2, 64, -0.1), (30, 0, 4, 2, 64, 0.1), (300, 230, 2, 2, 128, -0.1),
+                                                   (2500, 2300, 16, 4, 128, 0.05)])
+def test_values_that_are_not_finite_in_prompts(n, first, h, kv, hd, scale, apart):
+    """A value's NaN code spoils its column for the queries that see it, a key's the heads of those queries, and nothing in front of them: both prompt kernels, pages of one
+    scale and pages with a scale per token.  Bound as for decoding."""
+    cache, table, keys, values, g = filled([n], kv, hd, n + hd)
+    if apart:                                        # every seventh row is small
+        x = torch.randn(n, kv, hd, generator=g, device="cuda")
+        x[::7] *= 2.0 ** -apart
+        values[0] = put(cache, table, 0, torch.arange(n, device="cuda"), 1, x)
+    slot = lambda p: int(table[0, p // 64]) * 64 + p % 64
+    bad = [(first + (n - first) * 2 // 5, 0, 5), (first + (n - first) // 2, kv - 1, 9), (first + (n - first) // 2 + 1, kv - 1, 9), (n - 1, 0, hd - 1)]
+    spoiled_key = n - 3
+    for p, head, d in bad:
+        cache.v[slot(p), head, d] = 0xff if d == 9 else 0x7f
+        values[0][p, head, d] = 0
+    cache.k[slot(spoiled_key), kv - 1, 3] = 0x7f
+    keys[0][spoiled_key, kv - 1, 3] = 0
+    T = n - first
+    q = torch.randn(T, h, hd, generator=g, device="cuda").to(torch.bfloat16)
+    pos, idx = torch.arange(first, n, dtype=torch.int32, device="cuda"), torch.zeros(T, dtype=torch.int32, device="cuda")
+    want = attend(q, keys[0], values[0], pos, scale)
+    spoiled = torch.zeros_like(want, dtype=torch.bool)
+    group = h // kv
+    for p, head, d in bad:
+        spoiled[:, head * group:(head + 1) * group, d] |= (pos >= p)[:, None]
+    spoiled[:, (kv - 1) * group:] |= (pos >= spoiled_key)[:, None, None]
+    assert spoiled.any() and not spoiled.all()
+    got = K8.kv8_attention(q, cache, pos, idx, table, scale, qo_indptr=ints([0, T]), max_q=T, max_kv_len=n)
+    tcgen05.check_errors(q.device)
+    assert torch.equal(got.isnan(), spoiled)
+    if scale > 0:
+        assert near(got.masked_fill(spoiled, 0), want.masked_fill(spoiled, 0), values[0])
+    else:                                            # (weights are one bf16 term in that kernel: 2^-8 of each)
+        assert ((got.double() - want).masked_fill(spoiled, 0).abs() <= 2.0 ** -8 * (want.abs() + values[0].abs().max())).all()
+    # single tokens have the same definition
+    one = K8.kv8_attention(q, cache, pos, idx, table, scale, max_kv_len=n)
+    assert torch.equal(one.isnan(), spoiled) and near(one.masked_fill(spoiled, 0), want.masked_fill(spoiled, 0), values[0])
+    tcgen05.check_errors(q.device)
