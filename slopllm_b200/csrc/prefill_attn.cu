@@ -134,6 +134,8 @@ __global__ void __launch_bounds__(THREADS, 2) prefill_attn_kernel(const __grid_c
         const uint32_t t_base = tc::warp_uniform(tmem);
         const int nt = tc::warp_uniform(tiles);
         bool ok = tc::mbar_wait_warp(q_full, 0);
+        if (nt <= 0 && tc::elect_one()) tc::mma_commit(o_done);     // (no query of the block has a key)
+        __syncwarp();
         for (int j = 0; j <= nt; ++j) {
             if (j < nt && ok) {
                 const int st = j % STAGES;
@@ -300,6 +302,10 @@ __global__ void __launch_bounds__(THREADS, 2) prefill_attn_kernel(const __grid_c
                 uint32_t o[32];
                 tc::tmem_ld_32x32(lane_at + COL_O + c, o);
                 tc::tmem_ld_wait();
+                if (tiles <= 0) {                                   // (no product has written the sums)
+#pragma unroll
+                    for (int x = 0; x < 32; ++x) o[x] = 0u;
+                }
                 if (bad) {
                     uint32_t nan = 0;
 #pragma unroll 1

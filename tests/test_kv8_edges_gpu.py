@@ -4,6 +4,7 @@ import pytest
 import torch
 
 from kv8_util import attend, filled, held, near
+from slopllm_b200.ops import dense as D
 from slopllm_b200.ops import kv8 as K8
 from slopllm_b200.ops import tcgen05
 
@@ -64,3 +65,27 @@ def test_values_that_are_not_finite_in_prompts(n, first, h, kv, hd, scale, apart
     one = K8.kv8_attention(q, cache, pos, idx, table, scale, max_kv_len=n)
     assert torch.equal(one.isnan(), spoiled) and near(one.masked_fill(spoiled, 0), want.masked_fill(spoiled, 0), values[0])
     tcgen05.check_errors(q.device)
+
+
+@pytest.mark.parametrize("scale", [0.1, -0.1])
+def test_ranges_without_keys(scale):
+    """Positions of -1 in a range of queries: rows without keys are zero, whole blocks of them too, also over the bf16 cache."""
+    cache, table, keys, values, g = filled([100, 70], 2, 64, 5)
+    q = torch.randn(400, 4, 64, generator=g, device="cuda").to(torch.bfloat16)
+    pos = ints([-1] * 150 + list(range(100)) + [-1] * 10 + list(range(70)) + [-1] * 70)
+    idx = ints([0] * 250 + [1] * 150)
+    got = K8.kv8_attention(q, cache, pos, idx, table, scale, qo_indptr=ints([0, 250, 330, 400]), max_q=250, max_kv_len=100)
+    tcgen05.check_errors(q.device)
+    assert (got[pos < 0] == 0).all()
+    for b, (a, e) in enumerate(((150, 250), (260, 330))):
+        want = attend(q[a:e], keys[b], values[b], pos[a:e], scale)
+        # (weights are one bf16 term in the kernel for a negative scale: 2^-8 of each)
+        assert near(got[a:e], want, values[b]) if scale > 0 else ((got[a:e].double() - want).abs() <= 2.0 ** -8 * (want.abs() + values[b].abs().max())).all()
+    rows = [torch.zeros(cache.k.shape, dtype=torch.bfloat16, device="cuda") for _ in range(2)]
+    for x, kept in zip(rows, (keys, values)):
+        for b, y in enumerate(kept):
+            at = torch.arange(y.shape[0], device="cuda")
+            x[table[b, at // 64].long() * 64 + at % 64] = y.to(torch.bfloat16)
+    plain = D.paged_attention(q, *rows, pos, idx, table, 64, scale, qo_indptr=ints([0, 250, 330, 400]), max_q=250, max_kv_len=100)
+    tcgen05.check_errors(q.device)
+    assert (plain[pos < 0] == 0).all() and not plain.isnan().any()
