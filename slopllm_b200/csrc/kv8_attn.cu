@@ -40,7 +40,8 @@ struct Kv8DecodeParams {
 constexpr int KT = 64, MAX_T = 256;              // keys a tile, tokens a launch
 // Weights are 2^(score + exponent of the value's scale - reference).  A row's reference is raised to 2^TOP below the largest when one would be above
 // 2^(TOP + RAISE), which fp16 holds; fp32 weights reach down to 2^-126, so that two rows whose scales are the format's limits apart (2^120) are told
-// apart by weights down to 2^-14 of the largest.
+// apart by weights down to 2^-14 of the largest.  Denominators, from which the scales are taken out, reach further, and are multiplied by the two halves of a
+// power of two in turn.
 constexpr float TOP = 8.f, RAISE = 7.f;
 
 __device__ __forceinline__ float ex2(float x) {
@@ -464,9 +465,9 @@ __device__ __forceinline__ int decode_block(const CUtensorMap& map_k, const CUte
                         for (int h = 0; h < 2; ++h) {
 #pragma unroll
                             for (int o = 4; o < 32; o <<= 1) top[h] = fmaxf(top[h], __shfl_xor_sync(0xffffffffu, top[h], o));
-                            const float up = fresh ? top[h] - TOP : fmaxf(top[h] - TOP, 0.f), f = fresh ? 1.f : ex2(-up);
+                            const float up = fresh ? top[h] - TOP : fmaxf(top[h] - TOP, 0.f), root = fresh ? 1.f : ex2(-0.5f * up), f = root * root;
                             m[n][h] += up;
-                            l[n][h] *= f;
+                            l[n][h] = l[n][h] * root * root;
 #pragma unroll
                             for (int u = 0; u < 4; ++u) x[u][h] -= up;
 #pragma unroll
@@ -552,8 +553,9 @@ __device__ __forceinline__ int decode_block(const CUtensorMap& map_k, const CUte
 #pragma unroll
                 for (int y = 0; y < WARPS; ++y) {
                     const float mo = state[y * SLOT + h];
-                    f[y][h] = mo == -INFINITY ? 0.f : ex2(mo - top[h]);
-                    den[h] += f[y][h] * state[y * SLOT + M::HG + h];
+                    const float root = mo == -INFINITY ? 0.f : ex2(0.5f * (mo - top[h]));
+                    f[y][h] = root * root;
+                    den[h] += state[y * SLOT + M::HG + h] * root * root;
                 }
             }
             const float inv[2] = {1.f / den[0], 1.f / den[1]};

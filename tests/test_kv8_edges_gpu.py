@@ -3,7 +3,7 @@ scales are the format's limits apart, values that are not finite behind a query,
 import pytest
 import torch
 
-from kv8_util import attend, filled, held, near
+from kv8_util import attend, exponent, filled, held, near
 from slopllm_b200.ops import dense as D
 from slopllm_b200.ops import kv8 as K8
 from slopllm_b200.ops import tcgen05
@@ -23,6 +23,37 @@ def put(cache, table, b, positions, which, rows):
     (cache.v if which else cache.k)[slots] = codes
     cache.exps[slots // page, :, which, slots % page] = exps
     return held(codes, exps)
+
+
+# ---- attention ---------------------------------------------------------------------------------------------------------------
+
+def limits_apart(n, at, above, hd, page=64):
+    """A history of keys and values of zero (exponent -60) with, at `at`, a row of the largest scale whose score lies 2^above above the others'."""
+    cache, table, _, _, g = filled([n], 1, hd, n + at, page)
+    every = torch.arange(n, device="cuda")
+    keys, values = torch.zeros(n, 1, hd, device="cuda"), torch.zeros(n, 1, hd, device="cuda")
+    values[at] = torch.randn(1, hd, generator=g, device="cuda").clamp(-3, 3) * 2.0 ** 66
+    keys[at, 0, 0] = above * 0.6931471805599453
+    k = put(cache, table, 0, every, 0, keys)
+    v = put(cache, table, 0, every, 1, values)
+    assert cache.exps[table[0, at // page].long(), 0, 1, at % page] > 127 + 56
+    return cache, table, k, v
+
+
+@pytest.mark.parametrize("above", [5, 9, 12])
+@pytest.mark.parametrize("n,at", [(8000, 0), (8000, 4321), (8000, 7999), (300, 40), (300, 299)])
+@pytest.mark.parametrize("h,hd", [(4, 64), (8, 128), (4, 256), (16, 64)])
+def test_scales_at_the_limits_in_decoding(n, at, above, h, hd):
+    """Rows of zeros count in the denominator beside a value of the largest scale, in the same warp, another one, another block.  A result is one weight
+    (fp16, 2^-11) over a sum in fp32, rounded to bf16 (2^-8)."""
+    cache, table, k, v = limits_apart(n, at, above, hd)
+    q = torch.ones(1, h, hd, device="cuda").to(torch.bfloat16)
+    pos, idx = ints([n - 1]), ints([0])
+    want = attend(q, k, v, pos, 1.0)
+    for longest in (n, 0):
+        got = K8.kv8_attention(q, cache, pos, idx, table, 1.0, max_kv_len=longest)
+        assert ((got.double() - want).abs() <= (2.0 ** -8 + 2.0 ** -10) * want.abs()).all(), (got.double() / want).flatten()[:4]
+    tcgen05.check_errors(q.device)
 
 
 @pytest.mark.parametrize("apart", [0, 40])
