@@ -250,7 +250,12 @@ __global__ void __launch_bounds__(THREADS, 2) prefill_attn_kernel(const __grid_c
                         tc::tmem_st_32x16(lane_at + COL_O + c, o);
                     }
                 }
-                l *= f;
+                if (HALF) {                                         // (scales far apart: f may be 0 where l, without them, is large)
+                    const float root = m == -INFINITY ? 0.f : ex2_approx(0.5f * (m - mn));
+                    l = l * root * root;
+                } else {
+                    l *= f;
+                }
                 m = mn;
             }
             const float base = m == -INFINITY ? 0.f : HALF ? m - plus - LIFT : m;

@@ -56,6 +56,21 @@ def test_scales_at_the_limits_in_decoding(n, at, above, h, hd):
     tcgen05.check_errors(q.device)
 
 
+@pytest.mark.parametrize("above", [5, 9, 11])
+@pytest.mark.parametrize("n,at", [(2000, 0), (2000, 1000), (2000, 1700), (150, 20)])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_scales_at_the_limits_in_prompts(n, at, above, hd):
+    """The same for prompts, in pages of one scale and in those with a scale per token; queries in front of the large value give zeros."""
+    cache, table, k, v = limits_apart(n, at, above, hd)
+    first = n - 140
+    q = torch.ones(140, 4, hd, device="cuda").to(torch.bfloat16)
+    pos, idx = torch.arange(first, n, dtype=torch.int32, device="cuda"), torch.zeros(140, dtype=torch.int32, device="cuda")
+    got = K8.kv8_attention(q, cache, pos, idx, table, 1.0, qo_indptr=ints([0, 140]), max_q=140, max_kv_len=n)
+    want = attend(q, k, v, pos, 1.0)
+    assert ((got.double() - want).abs() <= (2.0 ** -8 + 2.0 ** -10) * want.abs()).all()
+    tcgen05.check_errors(q.device)
+
+
 @pytest.mark.parametrize("apart", [0, 40])
 @pytest.mark.parametrize("n,first,h,kv,hd,scale", [(300, 0, 4, 2, 128, 0.1), (300, 100, 8, 2, 64, 0.1), (300, 0, 4, 2, 64, -0.1), (30, 0, 4, 2, 64, 0.1), (300, 230, 2, 2, 128, -0.1),
                                                    (2500, 2300, 16, 4, 128, 0.05)])
@@ -95,6 +110,23 @@ def test_values_that_are_not_finite_in_prompts(n, first, h, kv, hd, scale, apart
     # single tokens have the same definition
     one = K8.kv8_attention(q, cache, pos, idx, table, scale, max_kv_len=n)
     assert torch.equal(one.isnan(), spoiled) and near(one.masked_fill(spoiled, 0), want.masked_fill(spoiled, 0), values[0])
+    tcgen05.check_errors(q.device)
+
+
+@pytest.mark.parametrize("scale", [-0.09, 0.0])
+@pytest.mark.parametrize("hd", [64, 128])
+def test_scales_of_scores_that_are_not_positive(scale, hd):
+    """Negative and zero `sm_scale`, for which prompts take the other kernel."""
+    n, first = 200, 60
+    cache, table, keys, values, g = filled([n], 2, hd, 3)
+    q = torch.randn(n - first, 4, hd, generator=g, device="cuda").to(torch.bfloat16)
+    pos, idx = torch.arange(first, n, dtype=torch.int32, device="cuda"), torch.zeros(n - first, dtype=torch.int32, device="cuda")
+    want = attend(q, keys[0], values[0], pos, scale)
+    one = K8.kv8_attention(q, cache, pos, idx, table, scale, max_kv_len=n)
+    assert near(one, want, values[0])
+    got = K8.kv8_attention(q, cache, pos, idx, table, scale, qo_indptr=ints([0, n - first]), max_q=n - first, max_kv_len=n)
+    # (weights are one bf16 term there: 2^-8 of each)
+    assert ((got.double() - want).abs() <= 2.0 ** -8 * (want.abs() + values[0].abs().max())).all()
     tcgen05.check_errors(q.device)
 
 
