@@ -346,7 +346,8 @@ struct Kv8ReadParams {
 // pages.  Keys are bf16; values are, too, or (HALF) fp16: of a page and head whose scales' exponents e are at most NARROW apart, codes times 2^(e - the
 // largest), which fp16 holds exactly (2^-9 2^-15 is its smallest number); else the codes alone, with e and 2^-e of each token beside them.
 struct Kv8UnpackParams {
-    Kv8Rows c;
+    Kv8Rows c;                       // its codes and exponents start at the first key head of a call's
+    int heads;                       // key heads of the call: n_kv below
     const int *qo_indptr, *positions, *batch_idx;    // token ranges of the sequences, [T], [T]
     int per_seq;
     bf16 *k, *v;                     // [sequences * per_seq * 64, n_kv, hd]
@@ -368,12 +369,12 @@ constexpr int NARROW = 15;
 // NaN codes among four: 0x80 in their bytes.
 __device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u; }
 
-// Rows `first` .. first + n - 1 of page-table row b, keys (which 0) or values, -> dst: a warp takes READ_ROWS of them, a lane 16 codes of each at a time.
+// Rows `first` .. first + n - 1 of page-table row b, `heads` key heads of keys (which 0) or values, -> dst: a warp takes READ_ROWS of them, a lane 16 codes of each at a time.
 // HALF: as fp16, divided by 2^top[head]; where that is KV8_WIDE, the codes alone.  CLEAN: NaN codes as zeros, and the first row with one to
 // spoiled[head]; returns whether this thread found one.
 template <bool HALF, bool CLEAN>
-__device__ __forceinline__ bool read_rows(const Kv8Rows& c, int which, int b, int first, int n, bf16* dst, const int* top, int* spoiled) {
-    const int lane = threadIdx.x & 31, per = c.n_kv * c.hd / 16, page = c.pages.page_size;
+__device__ __forceinline__ bool read_rows(const Kv8Rows& c, int heads, int which, int b, int first, int n, bf16* dst, const int* top, int* spoiled) {
+    const int lane = threadIdx.x & 31, per = heads * c.hd / 16, cached = c.n_kv * c.hd / 16, page = c.pages.page_size;
     const uint32_t of_head = (1u << 27) / (uint32_t)(c.hd / 16) + 1;             // x / (hd / 16) is (x * of_head) >> 27: x < 2^14, so it is off by less than 1 / 16
     const uint8_t* codes = which ? c.v_codes : c.k_codes;
     bool found = false;
@@ -395,7 +396,7 @@ __device__ __forceinline__ bool read_rows(const Kv8Rows& c, int which, int b, in
 #pragma unroll
             for (int i = 0; i < READ_ROWS; ++i)
                 if (slot[i] >= 0) {
-                    u[i] = ldg_nc_16(codes + ((size_t)slot[i] * (uint32_t)per + (uint32_t)x) * 16);
+                    u[i] = ldg_nc_16(codes + ((size_t)slot[i] * (uint32_t)cached + (uint32_t)x) * 16);
                     const int e = exps[i][(size_t)h * (uint32_t)(2 * page)];
                     s[i] = HALF && top[h] == KV8_WIDE ? 1.f : __uint_as_float((uint32_t)(HALF ? e - top[h] : e) << 23);
                 } else {
@@ -438,7 +439,7 @@ __global__ void __launch_bounds__(256, 4) kv8_read_kernel(Kv8ReadParams p) {
     const int* r = p.ranges + blockIdx.y * 4;
     const int i0 = blockIdx.x * 32, n = min(32, r[2] - i0), out = r[3] + i0;
     if (n <= 0 || !guard_ok(p.c.pages.guard, 31, out, (long long)p.rows - n + 1)) return;
-    read_rows<false, false>(p.c, blockIdx.z, r[0], r[1] + i0, n, (blockIdx.z ? p.v : p.k) + (size_t)out * p.c.n_kv * p.c.hd, nullptr, nullptr);
+    read_rows<false, false>(p.c, p.c.n_kv, blockIdx.z, r[0], r[1] + i0, n, (blockIdx.z ? p.v : p.k) + (size_t)out * p.c.n_kv * p.c.hd, nullptr, nullptr);
 }
 
 // grid (per_seq, sequences, 2), block 512: a page of a sequence's workspace, keys or values
@@ -460,15 +461,15 @@ __global__ void __launch_bounds__(512, 2) kv8_unpack_kernel(Kv8UnpackParams p) {
     const int i0 = blockIdx.x * 64, b = p.batch_idx[q0];
     n = min(64, n - i0);
     if (n <= 0) return;
-    bf16* dst = (blockIdx.z ? p.v : p.k) + (size_t)page * 64 * p.c.n_kv * p.c.hd;
+    bf16* dst = (blockIdx.z ? p.v : p.k) + (size_t)page * 64 * p.heads * p.c.hd;
     if (blockIdx.z == 0) {
-        read_rows<false, false>(p.c, 0, b, i0, n, dst, nullptr, nullptr);
+        read_rows<false, false>(p.c, p.heads, 0, b, i0, n, dst, nullptr, nullptr);
         return;
     }
     const int lane = threadIdx.x & 31, size = p.c.pages.page_size;
-    for (int h = threadIdx.x; h < p.c.n_kv; h += 512) p.spoiled_pages[(size_t)page * p.c.n_kv + h] = spoiled[h] = 64;
+    for (int h = threadIdx.x; h < p.heads; h += 512) p.spoiled_pages[(size_t)page * p.heads + h] = spoiled[h] = 64;
     const int s0 = lane < n ? kv8_slot(p.c.pages, 33, b, i0 + lane) : -1, s1 = lane + 32 < n ? kv8_slot(p.c.pages, 33, b, i0 + lane + 32) : -1;
-    for (int h = threadIdx.x >> 5; HALF && h < p.c.n_kv; h += 16) {
+    for (int h = threadIdx.x >> 5; HALF && h < p.heads; h += 16) {
         int e[2], hi = -1, lo = 256;                 // bytes
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -484,10 +485,10 @@ __global__ void __launch_bounds__(512, 2) kv8_unpack_kernel(Kv8UnpackParams p) {
         const bool wide = hi - lo > NARROW;          // (not where there are none)
         if (lane == 0) {
             top[h] = wide ? KV8_WIDE : hi - KV8_BIAS;
-            p.exps[(size_t)page * p.c.n_kv + h] = top[h];
+            p.exps[(size_t)page * p.heads + h] = top[h];
         }
         if (wide) {
-            float* const out = p.scales + ((size_t)page * p.c.n_kv + h) * 128;
+            float* const out = p.scales + ((size_t)page * p.heads + h) * 128;
 #pragma unroll
             for (int u = 0; u < 2; ++u) {            // (0 and 1 for tokens that are not there)
                 const int x = e[u] >= 0 ? max(-126, min(126, e[u] - KV8_BIAS)) : 0;
@@ -497,9 +498,9 @@ __global__ void __launch_bounds__(512, 2) kv8_unpack_kernel(Kv8UnpackParams p) {
         }
     }
     __syncthreads();
-    if (__syncthreads_or(read_rows<HALF, true>(p.c, 1, b, i0, n, dst, top, spoiled)) == 0) return;
-    for (int h = threadIdx.x >> 5; h < p.c.n_kv; h += 16) {          // (rare: the codes are read once more)
-        const size_t at = (size_t)page * p.c.n_kv + h;
+    if (__syncthreads_or(read_rows<HALF, true>(p.c, p.heads, 1, b, i0, n, dst, top, spoiled)) == 0) return;
+    for (int h = threadIdx.x >> 5; h < p.heads; h += 16) {           // (rare: the codes are read once more)
+        const size_t at = (size_t)page * p.heads + h;
         if (spoiled[h] == 64) continue;
         if (lane == 0) p.spoiled_pages[at] = spoiled[h];
         for (int d = lane; d < p.c.hd; d += 32) {
@@ -557,7 +558,7 @@ SL_API int sl_kv8_read(const Kv8ReadParams* p, int ranges, int longest, cudaStre
 // Causal attention of `sequences` token ranges over their histories: the histories' pages into the workspace of `up`, whose memory `attn` reads.
 SL_API int sl_kv8_prompts(const Kv8UnpackParams* up, const PagedPrefillParams* attn, int sequences, int max_q, cudaStream_t s) {
     if (sequences == 0 || max_q == 0) return 0;
-    if (!kv8_rows_ok(up->c, up->k, up->v) || sequences > 65535 || up->per_seq < 1 || up->c.n_kv > KV8_HEADS) return -1;
+    if (!kv8_rows_ok(up->c, up->k, up->v) || sequences > 65535 || up->per_seq < 1 || up->heads < 1 || up->heads > up->c.n_kv || up->heads > KV8_HEADS || attn->n_kv != up->heads) return -1;
     const bool half = paged_prefill_in_tcgen05(attn, sequences, max_q);
     const dim3 grid(up->per_seq, sequences, 2);
     if (half) sl_launch(kv8_unpack_kernel<true>, grid, 512, 0, s, *up);

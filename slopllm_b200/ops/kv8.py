@@ -24,7 +24,8 @@ from .dense import AttnParams, _slots
 from .rotary import RotaryTable
 
 LOW, HIGH, BIAS = -60, 60, 127         # limits of the exponent, and what is added to it in its byte
-UNPACK_BUDGET_BYTES = 1 << 30          # transient bf16 rows of a prompt step; more sequences go in groups
+# Transient rows of a prompt step: more sequences go in groups, a longer history in groups of key heads (one head of 128 values takes it at 2.0 million tokens).
+UNPACK_BUDGET_BYTES = 1 << 30
 
 
 # (Kv8Pages and Kv8Rows of the kernels, spliced into the structures that hold them: a call makes one object)
@@ -46,7 +47,7 @@ class Kv8ReadParams(C.Structure):
 
 
 class Kv8UnpackParams(C.Structure):
-    _fields_ = [*_ROWS, ("qo_indptr", C.c_void_p), ("positions", C.c_void_p), ("batch_idx", C.c_void_p), ("per_seq", C.c_int),
+    _fields_ = [*_ROWS, ("heads", C.c_int), ("qo_indptr", C.c_void_p), ("positions", C.c_void_p), ("batch_idx", C.c_void_p), ("per_seq", C.c_int),
                 ("k", C.c_void_p), ("v", C.c_void_p), ("table", C.c_void_p), ("rows_out", C.c_void_p), ("positions_out", C.c_void_p),
                 ("exps_out", C.c_void_p), ("scales", C.c_void_p), ("spoiled_pages", C.c_void_p), ("spoiled_dims", C.c_void_p)]
 
@@ -289,18 +290,28 @@ def _prompts(q, cache, positions, batch_idx, page_table, sm_scale, qo_indptr, ma
     n_kv, B = cache.k.shape[1], qo_indptr.numel() - 1
     most = page_table.shape[1] * cache.page_size
     per_seq = max(1, -(-min(max_kv_len or most, most) // 64))
-    group = max(1, min(B, 65535, UNPACK_BUDGET_BYTES // (per_seq * 64 * n_kv * hd * 4)))
     # one piece of memory: keys, values, then what the kernels know of pages and tokens (in words of 4 bytes a page)
-    pages, page = group * per_seq, 32 * n_kv * hd
-    parts = (page, page, n_kv * 128, n_kv, n_kv, n_kv * hd // 4, 1)
-    room = torch.empty(pages * sum(parts) + 2 * T, dtype=torch.int32, device=dev)
-    k, v, scales, exps, spoiled, dims, table, rows_out = (room.data_ptr() + 4 * pages * x for x in accumulate((0, *parts)))
+    layout = lambda n: (32 * n * hd, 32 * n * hd, n * 128, n, n, n * hd // 4, 1)
+    room = max(1, UNPACK_BUDGET_BYTES // (4 * per_seq))          # words a page, if one sequence has them all
+    heads, group = n_kv, max(1, min(B, 65535, room // sum(layout(n_kv))))
+    if sum(layout(n_kv)) > room:                                 # one history is too long: some key heads at a time
+        heads = max(1, (room - 1) // (sum(layout(1)) - 1))
+        heads = -(-n_kv // -(-n_kv // heads))
+    pages, parts = group * per_seq, layout(heads)
+    space = torch.empty(pages * sum(parts) + 2 * T, dtype=torch.int32, device=dev)
+    k, v, scales, exps, spoiled, dims, table, rows_out = (space.data_ptr() + 4 * pages * x for x in accumulate((0, *parts)))
     positions_out = rows_out + 4 * T
-    rows = _rows(cache, page_table)
-    for s in range(0, B, group):
-        n, ends = min(group, B - s), qo_indptr.data_ptr() + 4 * s
-        up = Kv8UnpackParams(*rows, ends, positions.data_ptr(), batch_idx.data_ptr(), per_seq, k, v, table, rows_out, positions_out, exps, scales,
-                             spoiled, dims)
-        p = AttnParams(q.data_ptr(), k, v, positions_out, rows_out, table, per_seq, 64, ends, n_heads, n_kv, hd, sm_scale, out.data_ptr(), T, pages * 64,
-                       max_kv_len, _status(device))
-        _call(device, "sl_kv8_prompts", C.byref(up), C.byref(p), n, int(max_q))
+    k_codes, v_codes, exps_in, *rows = _rows(cache, page_table)
+    for h in range(0, n_kv, heads):
+        n_h, per = min(heads, n_kv - h), n_heads // n_kv
+        mine = slice(h * per, (h + n_h) * per)
+        q_h, out_h = (q, out) if n_h == n_kv else (q[:, mine].contiguous(), out.new_empty(T, n_h * per, hd))
+        for s in range(0, B, group):
+            n, ends = min(group, B - s), qo_indptr.data_ptr() + 4 * s
+            up = Kv8UnpackParams(k_codes + h * hd, v_codes + h * hd, exps_in + h * 2 * cache.page_size, *rows, n_h, ends, positions.data_ptr(),
+                                 batch_idx.data_ptr(), per_seq, k, v, table, rows_out, positions_out, exps, scales, spoiled, dims)
+            p = AttnParams(q_h.data_ptr(), k, v, positions_out, rows_out, table, per_seq, 64, ends, n_h * per, n_h, hd, sm_scale, out_h.data_ptr(), T,
+                           pages * 64, max_kv_len, _status(device))
+            _call(device, "sl_kv8_prompts", C.byref(up), C.byref(p), n, int(max_q))
+        if out_h is not out:
+            out[:, mine] = out_h

@@ -130,6 +130,32 @@ def test_scales_of_scores_that_are_not_positive(scale, hd):
     tcgen05.check_errors(q.device)
 
 
+@pytest.mark.parametrize("hd,kv,budget_pages_of_a_head", [(128, 4, 20), (64, 6, 45), (128, 4, 9)])
+def test_the_workspace_keeps_its_budget(hd, kv, budget_pages_of_a_head, monkeypatch):
+    """One history beyond the budget goes in groups of key heads: the same bits, and no more memory than the budget (of one key head, where that is more)."""
+    n, T, h = 64 * 9 - 5, 6, 3 * kv
+    cache, table, keys, values, g = filled([n, 100], kv, hd, 8)
+    q = torch.randn(T + 3, h, hd, generator=g, device="cuda").to(torch.bfloat16)
+    pos = torch.cat([torch.arange(n - T, n), torch.arange(97, 100)]).to(torch.int32).cuda()
+    idx, ends = ints([0] * T + [1] * 3), ints([0, T, T + 3])
+    call = lambda: K8.kv8_attention(q, cache, pos, idx, table, hd ** -0.5, qo_indptr=ends, max_q=T, max_kv_len=n)
+    plain = call()
+    budget = budget_pages_of_a_head * (64 * hd * 4 + 4 * 129 + 4)
+    monkeypatch.setattr(K8, "UNPACK_BUDGET_BYTES", budget)
+    torch.cuda.synchronize()
+    base = torch.cuda.memory_allocated()
+    torch.cuda.reset_peak_memory_stats()
+    got = call()
+    torch.cuda.synchronize()
+    # beside the workspace: the result, queries and results of the heads of a group, what the allocator rounds up
+    more = 3 * q.numel() * 2 + 8 * 512 + 8 * T
+    assert torch.cuda.max_memory_allocated() - base <= budget + more
+    assert torch.equal(got, plain)
+    tcgen05.check_errors(q.device)
+    for b, (a, e) in enumerate(((0, T), (T, T + 3))):
+        assert near(got[a:e], attend(q[a:e], keys[b], values[b], pos[a:e], hd ** -0.5), values[b])
+
+
 @pytest.mark.parametrize("scale", [0.1, -0.1])
 def test_ranges_without_keys(scale):
     """Positions of -1 in a range of queries: rows without keys are zero, whole blocks of them too, also over the bf16 cache."""
