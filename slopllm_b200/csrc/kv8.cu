@@ -72,7 +72,7 @@ struct Writer {
     bool on, turning;                                // the lane has values; they are pairs of the rotation (EVEN)
     double* part;                                    // 256 values of the warp (not EVEN)
     const double2* turn;                             // (cos, sin) of each pair
-    float cs[EVEN ? 4 : 8], sn[EVEN ? 4 : 8];
+    float cs[EVEN ? 4 : 8], sn[EVEN ? 4 : 8];        // of queries: fp32, whether the warp has keys or not, so that their bits are the token's alone
 
     // What queries are multiplied with.  EVEN: (a, b) becomes (a aa - b ab, b bb + a ba), weights, cos and sin in one factor; else aa and bb are
     // the weights.
@@ -276,7 +276,8 @@ template <int L, bool VEC, bool EVEN>
 __global__ void __launch_bounds__(WARPS * 32, 28 / WARPS) kv8_store_kernel(const __grid_constant__ Kv8StoreParams p, int share) {
     pdl_grid_sync();
     using W = Writer<L, VEC, EVEN>;
-    __shared__ double2 turns[WARPS][128];                // (cos, sin) of each pair
+    __shared__ double2 turns[WARPS][128];                // (cos, sin) of each pair, for keys
+    __shared__ float2 turns_q[WARPS][128];               // for queries
     __shared__ double part[EVEN ? 1 : WARPS][EVEN ? 1 : 256];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, half = p.rot_dims / 2, own = lane % L;
     const long long id = (long long)blockIdx.x * WARPS + warp;
@@ -292,21 +293,20 @@ __global__ void __launch_bounds__(WARPS * 32, 28 / WARPS) kv8_store_kernel(const
     // fp32 keeps no digits of the angle of a far position: quarter turns and their remainder are taken in 64 bits (a remainder of an eighth of a turn at
     // most: rounded to fp32 it costs sine and cosine less than their own roundings)
     double2* const turn = turns[warp];
-    const bool keys = k0 * W::ROWS < p.n_kv;         // (a warp without needs fp32)
+    float2* const turn_q = turns_q[warp];
+    const bool keys = k0 * W::ROWS < p.n_kv;         // of this warp
     for (int i = lane; i < half; i += 32) {
         const double a = (double)pos * (double)p.freq[i] * 0.63661977236758134308, whole = rint(a);      // 2 / pi
         const int quarter = (int)(long long)whole;
-        double sn, cs;
+        float s, c;
+        sincospif(0.5f * (float)(a - whole), &s, &c);
+        const float gain = quarter & 2 ? -p.gain : p.gain;
+        turn_q[i] = make_float2((quarter & 1 ? -s : c) * gain, (quarter & 1 ? c : s) * gain);
         if (keys) {
+            double sn, cs;
             sincospi(0.5 * (a - whole), &sn, &cs);
-        } else {
-            float s, c;
-            sincospif(0.5f * (float)(a - whole), &s, &c);
-            sn = s;
-            cs = c;
+            turn[i] = make_double2((quarter & 1 ? -sn : cs) * (double)gain, (quarter & 1 ? cs : sn) * (double)gain);
         }
-        const double c = quarter & 1 ? -sn : cs, s = quarter & 1 ? cs : sn, gain = quarter & 2 ? -(double)p.gain : (double)p.gain;
-        turn[i] = make_double2(c * gain, s * gain);
     }
     if (pos >= 0) {
         const int slot = kv8_slot(p.pages, 30, b, pos);
@@ -320,9 +320,9 @@ __global__ void __launch_bounds__(WARPS * 32, 28 / WARPS) kv8_store_kernel(const
 #pragma unroll
     for (int i = 0; i < (EVEN ? 4 : 8); ++i) {
         const int d = w.da + i;
-        const double2 a = d < half ? turn[d] : d < p.rot_dims ? turn[d - half] : make_double2(1., 0.);
-        w.cs[i] = (float)a.x;
-        w.sn[i] = (float)a.y;
+        const float2 a = d < half ? turn_q[d] : d < p.rot_dims ? turn_q[d - half] : make_float2(1.f, 0.f);
+        w.cs[i] = a.x;
+        w.sn[i] = a.y;
     }
     w.template rows<QUERY>(q0, share, q);
     w.template rows<KEY>(k0, share, k);

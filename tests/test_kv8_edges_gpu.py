@@ -7,6 +7,7 @@ from kv8_util import attend, exponent, filled, held, near
 from slopllm_b200.ops import dense as D
 from slopllm_b200.ops import kv8 as K8
 from slopllm_b200.ops import tcgen05
+from slopllm_b200.ops.rotary import rotary_table
 
 pytestmark = pytest.mark.gpu
 
@@ -23,6 +24,30 @@ def put(cache, table, b, positions, which, rows):
     (cache.v if which else cache.k)[slots] = codes
     cache.exps[slots // page, :, which, slots % page] = exps
     return held(codes, exps)
+
+
+# ---- writer ------------------------------------------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("T,h,kv,hd,dims,norm", [(3, 32, 8, 128, 128, True), (300, 9, 2, 64, 64, True), (5000, 32, 8, 128, 64, False), (700, 3, 1, 80, 20, True)])
+def test_queries_do_not_depend_on_the_batch(T, h, kv, hd, dims, norm):
+    """A token's query has the same bits alone, in a batch and in a chunk, whichever warp makes it."""
+    g = torch.Generator(device="cuda").manual_seed(T)
+    x = torch.randn(T, (h + 2 * kv) * hd, generator=g, device="cuda").to(torch.bfloat16)
+    w = (1 + 0.1 * torch.randn(hd, generator=g, device="cuda")).to(torch.bfloat16) if norm else None
+    rot = rotary_table(dims, 1e6).to("cuda")
+    pos = torch.randint(0, 100000, (T,), generator=g, device="cuda").to(torch.int32)
+    idx, table = torch.zeros(T, dtype=torch.int32, device="cuda"), torch.zeros(1, 1, dtype=torch.int32, device="cuda")
+    cache = K8.Kv8Cache.allocate(1, 64, kv, hd, "cuda")
+
+    def queries(n):                                  # (places beyond the table are reported; only the queries count here)
+        q, k, v = x[:n].split([h * hd, kv * hd, kv * hd], 1)
+        out = K8.kv8_store(q, k, v, w, w, rot, pos[:n], idx[:n], table, cache, h, 1e-6)
+        tcgen05.error_flag(out.device).zero_()
+        return out
+
+    whole = queries(T)
+    for n in {1, 2, 17, 64, 299, 1100} & set(range(T)):
+        assert torch.equal(queries(n), whole[:n]), n
 
 
 # ---- attention ---------------------------------------------------------------------------------------------------------------
