@@ -14,12 +14,12 @@ struct Kv8StoreParams {
     const bf16* k; int ldk;          // [T, n_kv * hd]
     const bf16* v; int ldv;
     const bf16 *q_norm, *k_norm;     // [hd] or null
-    const float* freq; float gain;   // [rot_dims / 2] angle per position; factor on cos and sin
+    const float* freq; double gain;  // [rot_dims / 2] angle per position; factor on cos and sin
     int rot_dims;
     const int* positions; const int* batch_idx;      // [T]; a negative position: nothing is written to the cache
     Kv8Pages pages;
     int n_heads, n_kv, hd, q_stride;
-    float eps;
+    double eps;
     bf16* q_out;                     // [T, n_heads, hd]
     uint8_t *k_codes, *v_codes, *exps;
     int T;
@@ -117,7 +117,7 @@ struct Writer {
             for (int i = 0; i < 8; ++i) ss = fma((double)x[i], (double)x[i], ss);
 #pragma unroll
             for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
-            const double mean = ss / (double)p.hd + (double)p.eps;
+            const double mean = ss / (double)p.hd + p.eps;
             inv = mean > 3.4028234663852886e38 ? 0. : rsqrt(mean);   // (fp32's largest)
         }
         double z[8];
@@ -169,7 +169,7 @@ struct Writer {
 #pragma unroll
                 for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
                 // one step of Newton: off by half a step instead of two (a root of an infinite mean is 0 as it is)
-                const float mean = fmaf(ss, per, p.eps), r = rsqrtf(mean), inv = r > 0.f ? fmaf(0.5f * r, fmaf(-mean * r, r, 1.f), r) : r;
+                const float mean = fmaf(ss, per, (float)p.eps), r = rsqrtf(mean), inv = r > 0.f ? fmaf(0.5f * r, fmaf(-mean * r, r, 1.f), r) : r;
 #pragma unroll
                 for (int i = 0; i < 4; ++i) v.x[i] = mul2(v.x[i], pair(inv, inv));
             }
@@ -300,12 +300,12 @@ __global__ void __launch_bounds__(WARPS * 32, 28 / WARPS) kv8_store_kernel(const
         const int quarter = (int)(long long)whole;
         float s, c;
         sincospif(0.5f * (float)(a - whole), &s, &c);
-        const float gain = quarter & 2 ? -p.gain : p.gain;
-        turn_q[i] = make_float2((quarter & 1 ? -s : c) * gain, (quarter & 1 ? c : s) * gain);
+        const double gain = quarter & 2 ? -p.gain : p.gain;
+        turn_q[i] = make_float2((quarter & 1 ? -s : c) * (float)gain, (quarter & 1 ? c : s) * (float)gain);
         if (keys) {
             double sn, cs;
             sincospi(0.5 * (a - whole), &sn, &cs);
-            turn[i] = make_double2((quarter & 1 ? -sn : cs) * (double)gain, (quarter & 1 ? cs : sn) * (double)gain);
+            turn[i] = make_double2((quarter & 1 ? -sn : cs) * gain, (quarter & 1 ? cs : sn) * gain);
         }
     }
     if (pos >= 0) {

@@ -36,9 +36,9 @@ _ROWS = [("k_codes", C.c_void_p), ("v_codes", C.c_void_p), ("exps", C.c_void_p),
 
 class Kv8StoreParams(C.Structure):
     _fields_ = [("q", C.c_void_p), ("ldq", C.c_int), ("k", C.c_void_p), ("ldk", C.c_int), ("v", C.c_void_p), ("ldv", C.c_int),
-                ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("freq", C.c_void_p), ("gain", C.c_float), ("rot_dims", C.c_int),
+                ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("freq", C.c_void_p), ("gain", C.c_double), ("rot_dims", C.c_int),
                 ("positions", C.c_void_p), ("batch_idx", C.c_void_p), *_PAGES, ("n_heads", C.c_int), ("n_kv", C.c_int),
-                ("hd", C.c_int), ("q_stride", C.c_int), ("eps", C.c_float), ("q_out", C.c_void_p), ("k_codes", C.c_void_p),
+                ("hd", C.c_int), ("q_stride", C.c_int), ("eps", C.c_double), ("q_out", C.c_void_p), ("k_codes", C.c_void_p),
                 ("v_codes", C.c_void_p), ("exps", C.c_void_p), ("T", C.c_int)]
 
 

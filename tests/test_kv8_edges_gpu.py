@@ -1,13 +1,14 @@
 """The 8-bit key/value cache on a GPU where it is easily wrong: codes at the middle between two, bits that must not depend on the batch, weights of values whose
 scales are the format's limits apart, values that are not finite behind a query, workspaces, ranges without keys."""
+import numpy as np
 import pytest
 import torch
 
-from kv8_util import attend, exponent, filled, held, near
+from kv8_util import attend, filled, held, near, round_e4m3
 from slopllm_b200.ops import dense as D
 from slopllm_b200.ops import kv8 as K8
 from slopllm_b200.ops import tcgen05
-from slopllm_b200.ops.rotary import rotary_table
+from slopllm_b200.ops.rotary import RotaryTable, rotary_table
 
 pytestmark = pytest.mark.gpu
 
@@ -48,6 +49,68 @@ def test_queries_do_not_depend_on_the_batch(T, h, kv, hd, dims, norm):
     whole = queries(T)
     for n in {1, 2, 17, 64, 299, 1100} & set(range(T)):
         assert torch.equal(queries(n), whole[:n]), n
+
+
+@pytest.mark.parametrize("seed", [0, 1, 2, 3])
+@pytest.mark.parametrize("hd,dims,norm,size", [(128, 128, True, 1.5), (128, 128, False, 1.5), (80, 20, True, 1.5), (256, 64, True, 1e-3), (64, 34, False, 1.5), (64, 64, True, 100.0)])
+def test_stored_keys_are_the_nearest_codes(hd, dims, norm, size, seed):
+    """Exponent and code of every key are those of the value in 64 bits.  Left out: values nearer than 2^-36 of the row's largest to the middle between two codes
+    (the angle of position 6000 in quarter turns is good to 2^-41, products to 2^-52; fp32 gets some five of four million wrong, one if only the end is rounded to it)."""
+    T, kv = 4096, 1024 // hd
+    g = torch.Generator(device="cuda").manual_seed(hd + dims + 1000 * seed)
+    k = (torch.randn(T, kv * hd, generator=g, device="cuda") * size).to(torch.bfloat16)
+    w = (1 + 0.1 * torch.randn(hd, generator=g, device="cuda")).to(torch.bfloat16) if norm else None
+    first = 2000
+    pos, idx = torch.arange(first, first + T, dtype=torch.int32, device="cuda"), torch.zeros(T, dtype=torch.int32, device="cuda")
+    table = ints([[max(0, i - first // 64) for i in range((first + T) // 64 + 1)]])
+    cache = K8.Kv8Cache.allocate(int(table.max()) + 1, 64, kv, hd, "cuda")
+    rot = RotaryTable(dims, rotary_table(dims, 1e6).freq.cuda(), 1.25)
+    K8.kv8_store(k[:, :hd], k, k, None, w, rot, pos, idx, table, cache, 1, 1e-6)
+    tcgen05.check_errors(k.device)
+    x = k.view(T, kv, hd).double()
+    if norm:
+        x = x / torch.sqrt(x.square().mean(-1, keepdim=True) + 1e-6) * w.double()
+    ang = (pos.double()[:, None] * rot.freq.double())[:, None]
+    a, b = x[..., :dims // 2], x[..., dims // 2:dims]
+    want = torch.cat([(a * ang.cos() - b * ang.sin()) * 1.25, (b * ang.cos() + a * ang.sin()) * 1.25, x[..., dims:]], -1)
+    slots = table[0, (pos // 64).long()].long() * 64 + pos.long() % 64
+    exps = cache.exps[slots // 64, :, 0, slots % 64]
+    top = want.abs().amax(-1)
+    m, e = torch.frexp(top)                          # (logarithms on a GPU are off by a bit at powers of two)
+    assert torch.equal(exps.int() - 127, e - 9 + (m > 0.875))
+    scale = torch.exp2(exps.double() - 127)[..., None]
+    z = want / scale
+    step = torch.exp2(torch.floor(torch.log2(z.abs().clamp(min=2.0 ** -6))) - 3)
+    middle = (torch.floor(z.abs() / step) + 0.5) * step
+    off = (z.abs() - middle).abs()
+    sure = (off == 0) | (off > 2.0 ** -36 * (top[..., None] / scale))
+    assert sure.double().mean() > 1 - 1e-5
+    assert torch.equal(held(cache.k[slots], exps)[sure], (round_e4m3(z) * scale)[sure])
+
+
+def test_keys_take_epsilon_and_gain_as_they_are():
+    """`eps` and the rotation's gain are not rounded to fp32 on their way to a key: either would move these across the middle between two codes."""
+    hd = 64
+    ones = torch.ones(1, hd, device="cuda").to(torch.bfloat16)
+    cache, table, zero = K8.Kv8Cache.allocate(1, 64, 1, hd, "cuda"), ints([[0]]), ints([0])
+    free = RotaryTable(0, torch.empty(0, device="cuda"), 1.0)
+    checked = [0, 0]
+    for code in range(8, 15):                        # the middle between significands code / 8 and (code + 1) / 8
+        m = (code + 0.5) / 16
+        for up in (1, -1):
+            eps = 1 / m ** 2 - 1 - up * 1e-12        # smaller: the key lies above the middle
+            if (float(np.float32(eps)) - (1 / m ** 2 - 1)) * up > 0:
+                K8.kv8_store(ones, ones, ones, None, torch.ones(hd, device="cuda").to(torch.bfloat16), free, zero, zero, table, cache, 1, eps)
+                key = K8.kv8_read(cache, ints([[0, 0, 1, 0]]), 1, 1, table)[0].double()
+                assert ((key - m) * up > 0).all(), (code, up)
+                checked[0] += 1
+        gain = m + 1e-12                             # (fp32 holds the middle itself, which would go to the even code)
+        rot = RotaryTable(hd, torch.zeros(hd // 2, device="cuda"), gain)
+        K8.kv8_store(ones, ones, ones, None, None, rot, zero, zero, table, cache, 1, 1e-6)
+        assert (K8.kv8_read(cache, ints([[0, 0, 1, 0]]), 1, 1, table)[0].double() > m).all(), code
+        checked[1] += 1
+    assert min(checked) >= 3
+    tcgen05.check_errors(ones.device)
 
 
 # ---- attention ---------------------------------------------------------------------------------------------------------------
