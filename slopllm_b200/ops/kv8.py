@@ -207,7 +207,7 @@ def kv8_store(q, k, v, q_norm, k_norm, rot: RotaryTable, positions, batch_idx, p
 
 def kv8_read(cache: Kv8Cache, ranges: torch.Tensor, rows: int, longest: int, page_table: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor]:
     """Cached keys and values [rows, n_kv, hd] in bf16, which holds them exactly.  `ranges` int32 [R, 4]: page-table row, first position, number
-    of tokens (at most `longest`), first row of the result; rows in no range are not written."""
+    of tokens (at most `longest`; more are reported after the step), first row of the result; rows in no range are not written."""
     if ranges.dim() != 2 or ranges.shape[1] != 4 or not ranges.is_contiguous():
         raise ValueError(f"ranges are [R, 4] and contiguous, not {tuple(ranges.shape)}")
     device = ranges.get_device()

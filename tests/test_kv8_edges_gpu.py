@@ -8,6 +8,7 @@ from kv8_util import attend, filled, held, near, round_e4m3
 from slopllm_b200.ops import dense as D
 from slopllm_b200.ops import kv8 as K8
 from slopllm_b200.ops import tcgen05
+from slopllm_b200.ops.native import NativeError
 from slopllm_b200.ops.rotary import RotaryTable, rotary_table
 
 pytestmark = pytest.mark.gpu
@@ -111,6 +112,19 @@ def test_keys_take_epsilon_and_gain_as_they_are():
         checked[1] += 1
     assert min(checked) >= 3
     tcgen05.check_errors(ones.device)
+
+
+def test_ranges_longer_than_promised_are_reported():
+    """A range of more tokens than `longest` covers would leave rows unwritten."""
+    cache, table, keys, values, _ = filled([500], 2, 64, 4)
+    for longest in (400, 0):
+        K8.kv8_read(cache, ints([[0, 0, 500, 0]]), 500, longest, table)
+        with pytest.raises(NativeError):
+            tcgen05.check_errors(cache.k.device)
+    K8.kv8_read(cache, ints([[0, 0, 0, 0]]), 0, 0, table)
+    got = K8.kv8_read(cache, ints([[0, 0, 500, 0]]), 500, 500, table)
+    assert torch.equal(got[0].double(), keys[0]) and torch.equal(got[1].double(), values[0])
+    tcgen05.check_errors(cache.k.device)
 
 
 # ---- attention ---------------------------------------------------------------------------------------------------------------
