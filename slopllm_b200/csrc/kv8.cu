@@ -309,7 +309,7 @@ __global__ void __launch_bounds__(WARPS * 32, 28 / WARPS) kv8_store_kernel(const
         }
     }
     if (pos >= 0) {
-        const int slot = kv8_slot(p.pages, 30, b, pos);
+        const int slot = kv8_slot(p.pages, KV8_SITE_STORE, b, pos);
         if (slot >= 0) {
             w.placed = true;
             w.codes = (size_t)slot * (uint32_t)(p.n_kv * p.hd);
@@ -373,14 +373,14 @@ __device__ __forceinline__ uint32_t nan_codes(uint32_t w) { return ((w & 0x7f7f7
 // HALF: as fp16, divided by 2^top[head]; where that is KV8_WIDE, the codes alone.  CLEAN: NaN codes as zeros, and the first row with one to
 // spoiled[head]; returns whether this thread found one.
 template <bool HALF, bool CLEAN>
-__device__ __forceinline__ bool read_rows(const Kv8Rows& c, int heads, int which, int b, int first, int n, bf16* dst, const int* top, int* spoiled) {
+__device__ __forceinline__ bool read_rows(const Kv8Rows& c, int site, int heads, int which, int b, int first, int n, bf16* dst, const int* top, int* spoiled) {
     const int lane = threadIdx.x & 31, per = heads * c.hd / 16, cached = c.n_kv * c.hd / 16, page = c.pages.page_size;
     const uint32_t of_head = (1u << 27) / (uint32_t)(c.hd / 16) + 1;             // x / (hd / 16) is (x * of_head) >> 27: x < 2^14, so it is off by less than 1 / 16
     const uint8_t* codes = which ? c.v_codes : c.k_codes;
     bool found = false;
     for (int i0 = (threadIdx.x >> 5) * READ_ROWS; i0 < n; i0 += (blockDim.x >> 5) * READ_ROWS) {
         // a lane looks up one of the rows
-        const int mine = i0 + lane < n && lane < READ_ROWS ? kv8_slot(c.pages, 31, b, first + i0 + lane) : -1;
+        const int mine = i0 + lane < n && lane < READ_ROWS ? kv8_slot(c.pages, site, b, first + i0 + lane) : -1;
         const unsigned long long my_exps = kv8_exp_at(c.pages, c.n_kv, max(mine, 0), 0) + which * page;
         int slot[READ_ROWS];
         const uint8_t* exps[READ_ROWS];
@@ -437,10 +437,10 @@ __device__ __forceinline__ bool read_rows(const Kv8Rows& c, int heads, int which
 __global__ void __launch_bounds__(256, 4) kv8_read_kernel(Kv8ReadParams p) {
     pdl_grid_sync();
     const int* r = p.ranges + blockIdx.y * 4;
-    if (blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0) guard_ok(p.c.pages.guard, 31, r[2], (long long)gridDim.x * 32 + 1);
+    if (blockIdx.x == 0 && blockIdx.z == 0 && threadIdx.x == 0) guard_ok(p.c.pages.guard, KV8_SITE_READ, r[2], (long long)gridDim.x * 32 + 1);
     const int i0 = blockIdx.x * 32, n = min(32, r[2] - i0), out = r[3] + i0;
-    if (n <= 0 || !guard_ok(p.c.pages.guard, 31, out, (long long)p.rows - n + 1)) return;
-    read_rows<false, false>(p.c, p.c.n_kv, blockIdx.z, r[0], r[1] + i0, n, (blockIdx.z ? p.v : p.k) + (size_t)out * p.c.n_kv * p.c.hd, nullptr, nullptr);
+    if (n <= 0 || !guard_ok(p.c.pages.guard, KV8_SITE_READ, out, (long long)p.rows - n + 1)) return;
+    read_rows<false, false>(p.c, KV8_SITE_READ, p.c.n_kv, blockIdx.z, r[0], r[1] + i0, n, (blockIdx.z ? p.v : p.k) + (size_t)out * p.c.n_kv * p.c.hd, nullptr, nullptr);
 }
 
 // grid (per_seq, sequences, 2), block 512: a page of a sequence's workspace, keys or values
@@ -452,7 +452,7 @@ __global__ void __launch_bounds__(512, 2) kv8_unpack_kernel(Kv8UnpackParams p) {
     const int s = blockIdx.y, page = s * p.per_seq + blockIdx.x, q0 = p.qo_indptr[s], q1 = p.qo_indptr[s + 1], most = p.per_seq * 64;
     if (q0 >= q1) return;
     int n = p.positions[q1 - 1] + 1;                 // positions ascend within a sequence
-    if (!guard_ok(p.c.pages.guard, 33, n, (long long)most + 1)) n = most;
+    if (!guard_ok(p.c.pages.guard, KV8_SITE_PROMPTS, n, (long long)most + 1)) n = most;
     if (blockIdx.z == 0 && threadIdx.x == 0) p.table[page] = page;
     if (blockIdx.x == 0 && blockIdx.z == 0)
         for (int t = q0 + threadIdx.x; t < q1; t += 512) {
@@ -464,12 +464,12 @@ __global__ void __launch_bounds__(512, 2) kv8_unpack_kernel(Kv8UnpackParams p) {
     if (n <= 0) return;
     bf16* dst = (blockIdx.z ? p.v : p.k) + (size_t)page * 64 * p.heads * p.c.hd;
     if (blockIdx.z == 0) {
-        read_rows<false, false>(p.c, p.heads, 0, b, i0, n, dst, nullptr, nullptr);
+        read_rows<false, false>(p.c, KV8_SITE_PROMPTS, p.heads, 0, b, i0, n, dst, nullptr, nullptr);
         return;
     }
     const int lane = threadIdx.x & 31, size = p.c.pages.page_size;
     for (int h = threadIdx.x; h < p.heads; h += 512) p.spoiled_pages[(size_t)page * p.heads + h] = spoiled[h] = 64;
-    const int s0 = lane < n ? kv8_slot(p.c.pages, 33, b, i0 + lane) : -1, s1 = lane + 32 < n ? kv8_slot(p.c.pages, 33, b, i0 + lane + 32) : -1;
+    const int s0 = lane < n ? kv8_slot(p.c.pages, KV8_SITE_PROMPTS, b, i0 + lane) : -1, s1 = lane + 32 < n ? kv8_slot(p.c.pages, KV8_SITE_PROMPTS, b, i0 + lane + 32) : -1;
     for (int h = threadIdx.x >> 5; HALF && h < p.heads; h += 16) {
         int e[2], hi = -1, lo = 256;                 // bytes
 #pragma unroll
@@ -499,7 +499,7 @@ __global__ void __launch_bounds__(512, 2) kv8_unpack_kernel(Kv8UnpackParams p) {
         }
     }
     __syncthreads();
-    if (__syncthreads_or(read_rows<HALF, true>(p.c, p.heads, 1, b, i0, n, dst, top, spoiled)) == 0) return;
+    if (__syncthreads_or(read_rows<HALF, true>(p.c, KV8_SITE_PROMPTS, p.heads, 1, b, i0, n, dst, top, spoiled)) == 0) return;
     for (int h = threadIdx.x >> 5; h < p.heads; h += 16) {           // (rare: the codes are read once more)
         const size_t at = (size_t)page * p.heads + h;
         if (spoiled[h] == 64) continue;
@@ -507,7 +507,7 @@ __global__ void __launch_bounds__(512, 2) kv8_unpack_kernel(Kv8UnpackParams p) {
         for (int d = lane; d < p.c.hd; d += 32) {
             int first = 64;
             for (int t = spoiled[h]; t < n && first == 64; ++t) {
-                const int slot = kv8_slot(p.c.pages, 33, b, i0 + t);
+                const int slot = kv8_slot(p.c.pages, KV8_SITE_PROMPTS, b, i0 + t);
                 if (slot >= 0 && (p.c.v_codes[((size_t)slot * p.c.n_kv + h) * p.c.hd + d] & 0x7f) == 0x7f) first = t;
             }
             p.spoiled_dims[at * p.c.hd + d] = (uint8_t)first;

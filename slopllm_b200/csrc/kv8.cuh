@@ -11,6 +11,10 @@
 constexpr int KV8_HEADS = 1024;                  // key heads at most
 constexpr int KV8_BIAS = 127, KV8_LOW = -60, KV8_HIGH = 60;      // exponents that are written
 
+// Numbers under which the kernels report a place that is not there (guard_ok) and a wait that ran out (error word); no other kernel's.
+constexpr int KV8_SITE_STORE = 60, KV8_SITE_READ = 61, KV8_SITE_DECODE = 62, KV8_SITE_PROMPTS = 63;
+constexpr int KV8_WAIT_FETCH = 60, KV8_WAIT_PRODUCTS = 61;
+
 // Where a step's tokens lie: checked places of the page table.
 struct Kv8Pages {
     const int* page_table; int pt_stride, pt_rows, pt_width, page_size;

@@ -94,7 +94,7 @@ struct Tiles {
         const int pos = p.positions[t];
         b.last[t] = (uint8_t)(pos & (KT - 1));
         b.row[t] = p.batch_idx[t];
-        return pos < 0 || !guard_ok(p.pages.guard, 32, pos / p.pages.page_size, p.pages.pt_width) ? 0 : pos / KT + 1;
+        return pos < 0 || !guard_ok(p.pages.guard, KV8_SITE_DECODE, pos / p.pages.page_size, p.pages.pt_width) ? 0 : pos / KT + 1;
     }
     // All threads of the block.
     __device__ __forceinline__ Tiles(Batch& b, const Kv8DecodeParams& p, int most) : batch(b), T(p.T) {
@@ -249,7 +249,7 @@ __device__ __forceinline__ int decode_block(const CUtensorMap& map_k, const CUte
             }
             if (key >= n) return a;
             a.key = key;
-            if (guard_ok(p.pages.guard, 32, b, p.pages.pt_rows) && guard_ok(p.pages.guard, 32, page, p.pages.pt_width))
+            if (guard_ok(p.pages.guard, KV8_SITE_DECODE, b, p.pages.pt_rows) && guard_ok(p.pages.guard, KV8_SITE_DECODE, page, p.pages.pt_width))
                 a.page = p.pages.page_table[(size_t)b * p.pages.pt_stride + page];
             return a;
         };
@@ -262,7 +262,7 @@ __device__ __forceinline__ int decode_block(const CUtensorMap& map_k, const CUte
             const int n = (int)min((long long)batch, w1 - w), off = now.key % p.pages.page_size;
             const uint32_t firsts = __ballot_sync(0xffffffffu, now.q != nullptr), boxes = __ballot_sync(0xffffffffu, now.key >= 0);
             // a page that is not there is recorded; rows in front of the tensor read as zeros
-            const bool there = now.key >= 0 && guard_ok(p.pages.guard, 32, (long long)now.page * p.pages.page_size, p.pages.num_slots);
+            const bool there = now.key >= 0 && guard_ok(p.pages.guard, KV8_SITE_DECODE, (long long)now.page * p.pages.page_size, p.pages.num_slots);
             const int row = there ? now.page * p.pages.page_size + off : -KT;
             // (exponent bytes of a box start at multiples of 16)
             const uint32_t from = (uint32_t)(((((size_t)(there ? now.page : 0) * p.n_kv + max(now.head, 0)) * 2) * p.pages.page_size + max(off, 0)) / 16);
@@ -306,7 +306,7 @@ __device__ __forceinline__ int decode_block(const CUtensorMap& map_k, const CUte
         // nothing is in flight when the block ends, also where a wait ran out
         for (int j = max(0, issued - M::STAGES); j < issued; ++j) ok &= tc::mbar_wait_warp(full + j % M::STAGES, (uint32_t)(j / M::STAGES) & 1);
         for (int j = max(0, asked - 2); j < asked; ++j) ok &= tc::mbar_wait_warp(q_full + (j & 1), (uint32_t)(j >> 1) & 1);
-        if (!ok && lane == 0) atomicExch(p.err, 50);
+        if (!ok && lane == 0) atomicExch(p.err, KV8_WAIT_FETCH);
         return tiles.shares;
     }
 
@@ -587,7 +587,7 @@ __device__ __forceinline__ int decode_block(const CUtensorMap& map_k, const CUte
             at = begin;
         }
     }
-    if (!ok && lane == 0) atomicExch(p.err, 51);
+    if (!ok && lane == 0) atomicExch(p.err, KV8_WAIT_PRODUCTS);
     return tiles.shares;
 }
 

@@ -127,6 +127,20 @@ def test_ranges_longer_than_promised_are_reported():
     tcgen05.check_errors(cache.k.device)
 
 
+def test_reports_name_the_operator():
+    """What a self-check finds is reported under the operator's own number."""
+    cache, table, _, _, g = filled([100], 2, 64, 9)
+    q = torch.randn(1, 4, 64, generator=g, device="cuda").to(torch.bfloat16)
+    k, pos, row = q[:, :2].reshape(1, 128), ints([99]), ints([5])
+    for site, call in ((60, lambda: K8.kv8_store(q.view(1, 256), k, k, None, None, rotary_table(64, 1e4).to("cuda"), pos, row, table, cache, 4, 1e-6)),
+                       (61, lambda: K8.kv8_read(cache, ints([[5, 0, 1, 0]]), 1, 1, table)),
+                       (62, lambda: K8.kv8_attention(q, cache, pos, row, table, 0.125)),
+                       (63, lambda: K8.kv8_attention(q, cache, pos, row, table, 0.125, qo_indptr=ints([0, 1]), max_q=1, max_kv_len=100))):
+        call()
+        with pytest.raises(NativeError, match=f"site {site}:"):
+            tcgen05.check_errors(q.device)
+
+
 # ---- attention ---------------------------------------------------------------------------------------------------------------
 
 def limits_apart(n, at, above, hd, page=64):
