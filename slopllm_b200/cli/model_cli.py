@@ -30,7 +30,7 @@ def add_model_args(ap: argparse.ArgumentParser) -> None:
                          "families that have it")
     ap.add_argument("--kv-dtype", choices=("auto", "e4m3"), default="auto",
                     help="type of cached keys and values: auto is the model's own; e4m3 keeps them in 8 bits with a scale per token and key head, "
-                         "for about half of the cache's bytes (qwen3, qwen3_5)")
+                         "for about half of the cache's bytes (qwen3, qwen3_5; on a GPU heads of 64 or 128 values)")
     ap.add_argument("--gpus", default="", help="comma-separated device list; its length must equal the number of ranks")
     ap.add_argument("--arena", type=float, default=0.0,
                     help="GiB of device memory this process may allocate per GPU (weights + KV cache + step buffers); a larger "
@@ -148,6 +148,20 @@ def _kv_dtype(args) -> Optional[str]:
     return None if name == "auto" else name
 
 
+def _refuse_kv_dtype(args, ctx: ParallelContext, reg, model_type: str, raw: dict) -> None:
+    """Ends with a line of text where a checkpoint's keys and values are not cached in the type asked for."""
+    kv_dtype = _kv_dtype(args)
+    if kv_dtype is None:
+        return
+    if not reg.kv8:
+        raise SystemExit(f"{args.model}: {model_type} does not cache keys and values in {kv_dtype}")
+    from ..models.dense import DenseConfig, check_kv_dtype
+    try:
+        check_kv_dtype(DenseConfig.from_hf_dict(raw), kv_dtype, ctx.device.type == "cuda")
+    except ValueError as e:
+        raise SystemExit(f"{args.model}: {e}")
+
+
 def _random_model(spec: str, ctx: ParallelContext, mtp: int, dtype_name: Optional[str] = None, kv_dtype: Optional[str] = None):
     from ..parallel.fused import make_comm
     dtype = torch.bfloat16 if ctx.device.type == "cuda" else torch.float32
@@ -203,7 +217,8 @@ def build_runtime(args, with_scheduler: bool = True) -> Runtime:
         if getattr(args, "max_model_len", None) is None:
             from ..utils.generation_config import max_position_embeddings
             args.max_model_len = max_position_embeddings(model_dir)
-        model_type, reg, _ = inspect_model(model_dir, cp=args.cp, mtp=args.mtp)
+        model_type, reg, raw = inspect_model(model_dir, cp=args.cp, mtp=args.mtp)
+        _refuse_kv_dtype(args, ctx, reg, model_type, raw)
         check_memory_plan(args, ctx, model_dir, model_type)
         cfg, model = load_registered(reg, model_dir, ctx, args.mtp, getattr(args, "dtype", None), _kv_dtype(args))
     if getattr(args, "max_model_len", None) is None:

@@ -57,7 +57,7 @@ def main(argv=None) -> int:
     ap.add_argument("--max-pages", type=int, default=0)
     ap.add_argument("--arena", type=float, default=0.0, help="GiB the process may allocate (0: the whole device)")
     ap.add_argument("--device-gb", type=float, default=180.0, help="device memory in GiB when --arena is not given")
-    ap.add_argument("--kv-dtype", choices=("auto", "e4m3"), default="auto", help="type of cached keys and values (qwen3, qwen3_5)")
+    ap.add_argument("--kv-dtype", choices=("auto", "e4m3"), default="auto", help="type of cached keys and values (qwen3, qwen3_5; heads of 64 or 128 values)")
     ap.add_argument("--context", type=int, default=0, help="longest sequence assumed for the workspace estimate")
     args = ap.parse_args(argv)
     cfg = _config(args)
@@ -70,6 +70,11 @@ def main(argv=None) -> int:
             if family is not None:
                 raise SystemExit(f"plan: {cfg.model_type} does not cache keys and values in {args.kv_dtype}")
             more = {"kv_dtype": args.kv_dtype}
+            from ..models.dense import check_kv_dtype
+            try:
+                check_kv_dtype(cfg, args.kv_dtype)
+            except ValueError as e:
+                raise SystemExit(f"plan: {e}")
         p = planner(cfg, world=args.world, batch_size=args.batch_size, chunk_size=args.chunk_size, max_pages=args.max_pages,
                     arena_gb=args.arena, device_gb=args.device_gb, **more)
     elif args.kv_dtype != "auto":

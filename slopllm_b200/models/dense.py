@@ -152,14 +152,23 @@ class DenseWeights:
 KV_DTYPES = ("e4m3",)      # types of cached keys and values beside the model's own
 
 
+def check_kv_dtype(cfg: DenseConfig, kv_dtype: Optional[str], on_gpu: bool = True) -> None:
+    """ValueError where a model's keys and values are not cached in `kv_dtype` (None: its own type), before anything is loaded."""
+    if kv_dtype is None:
+        return
+    if kv_dtype not in KV_DTYPES:
+        raise ValueError(f"no cache of type {kv_dtype}; there is {', '.join(KV_DTYPES)}")
+    if cfg.head_dim % 16 or cfg.head_dim > 256:
+        raise ValueError(f"the 8-bit cache takes heads of a multiple of 16 values up to 256, not {cfg.head_dim}")
+    if on_gpu and cfg.head_dim not in K8.PROMPT_HEADS:
+        raise ValueError(f"over the 8-bit cache a GPU serves models with heads of {' or '.join(map(str, K8.PROMPT_HEADS))} values, not {cfg.head_dim}")
+
+
 def dense_cache_specs(cfg: DenseConfig, tp: int = 1, kv_dtype: Optional[str] = None) -> List[CacheSpec]:
     """Paged K/V rows per full-attention layer; conv + recurrent state per linear-attention layer.  `kv_dtype` "e4m3": the rows are
     codes, with two exponent bytes per token and key head (`ops/kv8.py`; a page's bytes are laid out by head)."""
     n_kv = max(1, cfg.num_key_value_heads // tp)
-    if kv_dtype is not None and kv_dtype not in KV_DTYPES:
-        raise ValueError(f"no cache of type {kv_dtype}; there is {', '.join(KV_DTYPES)}")
-    if kv_dtype is not None and (cfg.head_dim % 16 or cfg.head_dim > 256):
-        raise ValueError(f"the 8-bit cache takes heads of a multiple of 16 values up to 256, not {cfg.head_dim}")
+    check_kv_dtype(cfg, kv_dtype, on_gpu=False)
     lh = max(1, cfg.linear_num_key_heads // tp)
     cdim = lh * (2 * cfg.linear_key_head_dim + cfg.linear_value_head_dim)
     full = CacheSpec(rows={"k": (n_kv, cfg.head_dim), "v": (n_kv, cfg.head_dim)})
@@ -190,6 +199,7 @@ class DenseModel(DecoderStack):
                  comm: Optional[Comm] = None, kv_dtype: Optional[str] = None):
         self.cfg, self.w, self.kv_dtype = cfg, weights, kv_dtype
         ctx = ctx or ParallelContext()
+        check_kv_dtype(cfg, kv_dtype, ctx.device.type == "cuda")
         self.specs = dense_cache_specs(cfg, ctx.world, kv_dtype)
         self.rot = None if kv_dtype is None else rotary_table(cfg.rope_dim, cfg.rope_theta).to(ctx.device)
         self.sublayers = []
@@ -424,6 +434,7 @@ def load_dense_model(model_dir: str, ctx: Optional[ParallelContext] = None, dtyp
     ctx = ctx or ParallelContext()
     with open(os.path.join(model_dir, "config.json")) as f:
         cfg = DenseConfig.from_hf_dict(json.load(f))
+    check_kv_dtype(cfg, kv_dtype, ctx.device.type == "cuda")
     tensors: Dict[str, torch.Tensor] = {}
     for fn in sorted(os.listdir(model_dir)):
         if fn.endswith(".safetensors"):

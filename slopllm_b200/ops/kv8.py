@@ -23,6 +23,7 @@ from . import native as N, reference as R, tcgen05
 from .dense import AttnParams, _slots
 from .rotary import RotaryTable
 
+PROMPT_HEADS = (64, 128)               # widths of heads whose prompts the kernels attend over
 LOW, HIGH, BIAS = -60, 60, 127         # limits of the exponent, and what is added to it in its byte
 # Transient rows of a prompt step: more sequences go in groups, a longer history in groups of key heads (one head of 128 values takes it at 2.0 million tokens).
 UNPACK_BUDGET_BYTES = 1 << 30
@@ -266,7 +267,7 @@ def kv8_attention(q, cache: Kv8Cache, positions, batch_idx, page_table, sm_scale
         _call(device, "sl_kv8_decode", C.byref(p), T, blocks, max_kv_len)
         return out
     _check_step(device, cache, qo_indptr)
-    if hd not in (64, 128):
+    if hd not in PROMPT_HEADS:
         raise ValueError(f"heads of {hd} values: attention of prompts takes 64 or 128")
     _prompts(q, cache, positions, batch_idx, page_table, sm_scale, qo_indptr, max_q or T, max_kv_len, out)
     return out

@@ -186,6 +186,9 @@ def plan_dense(cfg, world: int = 1, batch_size: int = 8, chunk_size: int = 8192,
                device_gb: float = 180.0, fp8: bool = False, reserve_gb: float = 4.0, kv_dtype=None) -> MemoryPlan:
     """`plan_memory` for the dense families (tensor parallel only; the workspace estimate is the residual / activation rows
     plus the MLP's gate-up rows of one chunk, and the rows that prompts read back from an 8-bit cache)."""
+    if kv_dtype is not None:
+        from ..models.dense import check_kv_dtype
+        check_kv_dtype(cfg, kv_dtype)
     weights = dense_weight_bytes(cfg, world, fp8=fp8)
     page = max(1, dense_kv_page_bytes(cfg, world, kv_dtype=kv_dtype))
     requested = max_pages if max_pages > 0 else batch_size * -(-chunk_size // PAGE_SIZE)

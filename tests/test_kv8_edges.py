@@ -1,7 +1,15 @@
-"""The 8-bit key/value cache on the CPU: what the kernels' reports name."""
+"""The 8-bit key/value cache on the CPU: what the kernels' reports name, and which models take the cache."""
+import argparse
 import glob
+import json
 import os
 import re
+
+import pytest
+import torch
+
+from slopllm_b200.models.dense import DenseConfig, DenseModel, load_dense_model, random_dense_model
+from slopllm_b200.parallel.dist import ParallelContext
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "slopllm_b200", "csrc")
 
@@ -20,3 +28,45 @@ def test_reports_name_one_kernel():
     assert used["site"] and used["wait"]
     assert not set(sites) & set(used["site"]) and not set(waits) & set(used["wait"])
     assert not any(name.startswith("kv8") for names in (*used["site"].values(), *used["wait"].values()) for name in names)
+
+
+def wide(**kw):
+    """Qwen3.5's widths: 16 heads of 256 over 2, a quarter of them rotated, a gate behind each query."""
+    return DenseConfig(hidden_size=64, intermediate_size=128, num_hidden_layers=1, num_attention_heads=16, num_key_value_heads=2, head_dim=256, vocab_size=100,
+                       partial_rotary_factor=0.25, attn_output_gate=True, **kw)
+
+
+def raw_config(head_dim):
+    return {"model_type": "qwen3", "hidden_size": 64, "intermediate_size": 128, "num_hidden_layers": 1, "num_attention_heads": 16, "num_key_value_heads": 2,
+            "head_dim": head_dim, "vocab_size": 100, "eos_token_id": 1}
+
+
+def test_widths_without_prompts_are_refused_before_loading(tmp_path, capsys):
+    """A GPU has no attention of prompts for heads of 256 over this cache: the model, its loading and the plan say so, in front of weights and pages.  The CPU has it."""
+    from slopllm_b200.cli import plan as plan_cli
+    from slopllm_b200.utils.sizing import plan_dense
+    gpu = ParallelContext(device=torch.device("cuda", 0))
+    for head_dim in (256, 96):
+        (tmp_path / "config.json").write_text(json.dumps(raw_config(head_dim)))
+        for call in (lambda: DenseModel(wide() if head_dim == 256 else DenseConfig(head_dim=96), None, gpu, kv_dtype="e4m3"),
+                     lambda: load_dense_model(str(tmp_path), gpu, kv_dtype="e4m3"), lambda: plan_dense(DenseConfig(head_dim=head_dim), kv_dtype="e4m3")):
+            with pytest.raises(ValueError, match=f"64 or 128 values, not {head_dim}"):
+                call()
+        with pytest.raises(SystemExit, match="64 or 128"):
+            plan_cli.main(["--model", str(tmp_path), "--kv-dtype", "e4m3"])
+        assert plan_cli.main(["--model", str(tmp_path)]) == 0
+    capsys.readouterr()
+    cfg = wide()
+    w, _ = random_dense_model(cfg, seed=1, device="cpu", dtype=torch.float32)
+    assert DenseModel(cfg, w, ParallelContext(device=torch.device("cpu")), kv_dtype="e4m3").allocate_cache(2).kv8
+
+
+def test_checkpoints_that_do_not_take_the_cache_end_the_command(tmp_path):
+    """One line of text, as with random weights, not a traceback."""
+    from slopllm_b200.cli.model_cli import add_model_args, build_runtime
+    ap = argparse.ArgumentParser()
+    add_model_args(ap)
+    for raw, what in (({"model_type": "zemezen"}, "zemezen does not cache keys and values in e4m3"), (raw_config(72), "multiple of 16")):
+        (tmp_path / "config.json").write_text(json.dumps(raw))
+        with pytest.raises(SystemExit, match=what):
+            build_runtime(ap.parse_args(["--cpu", "--model", str(tmp_path), "--kv-dtype", "e4m3"]))
