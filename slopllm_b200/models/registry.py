@@ -146,11 +146,12 @@ def load_registered(reg: ModelRegistration, model_dir: str, ctx: ParallelContext
     """`dtype`: "bfloat16" / "float32" (None: bfloat16 on a GPU, float32 on the CPU).  `kv_dtype`: "e4m3", or None for the model's own."""
     if kv_dtype is not None and not reg.kv8:
         raise ValueError(f"{model_dir}: this model family does not cache keys and values in {kv_dtype}")
+    more = {} if kv_dtype is None else {"kv_dtype": kv_dtype}
     if dtype is None or (dtype == "bfloat16") == (ctx.device.type == "cuda"):
-        return reg.load(model_dir, ctx, mtp, **({} if kv_dtype is None else {"kv_dtype": kv_dtype}))
+        return reg.load(model_dir, ctx, mtp, **more)
     if not reg.float32:
         raise ValueError(f"{model_dir}: this model family does not run in {dtype} on {ctx.device.type}")
-    return reg.load(model_dir, ctx, mtp, dtype=getattr(torch, dtype))
+    return reg.load(model_dir, ctx, mtp, dtype=getattr(torch, dtype), **more)
 
 
 def load_any(model_dir: str, ctx: Optional[ParallelContext] = None, mtp: int = 0, dtype: Optional[str] = None, kv_dtype: Optional[str] = None):

@@ -70,3 +70,15 @@ def test_checkpoints_that_do_not_take_the_cache_end_the_command(tmp_path):
         (tmp_path / "config.json").write_text(json.dumps(raw))
         with pytest.raises(SystemExit, match=what):
             build_runtime(ap.parse_args(["--cpu", "--model", str(tmp_path), "--kv-dtype", "e4m3"]))
+
+
+def test_both_types_reach_the_loader(tmp_path):
+    """`dtype` and `kv_dtype` together: a family that has both gets both."""
+    from slopllm_b200.models.registry import ModelRegistration, load_registered
+    got = []
+    reg = ModelRegistration(False, False, False, False, lambda *a, **k: got.append(k), float32=True, kv8=True)
+    gpu, cpu = ParallelContext(device=torch.device("cuda", 0)), ParallelContext(device=torch.device("cpu"))
+    load_registered(reg, str(tmp_path), gpu, 0, "float32", "e4m3")
+    load_registered(reg, str(tmp_path), cpu, 0, "float32", "e4m3")
+    load_registered(reg, str(tmp_path), cpu, 0, None, None)
+    assert got == [{"dtype": torch.float32, "kv_dtype": "e4m3"}, {"kv_dtype": "e4m3"}, {}]
