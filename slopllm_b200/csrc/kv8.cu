@@ -451,7 +451,7 @@ __global__ void __launch_bounds__(512, 2) kv8_unpack_kernel(Kv8UnpackParams p) {
     __shared__ int spoiled[KV8_HEADS];               // first row with a value that is not finite
     const int s = blockIdx.y, page = s * p.per_seq + blockIdx.x, q0 = p.qo_indptr[s], q1 = p.qo_indptr[s + 1], most = p.per_seq * 64;
     if (q0 >= q1) return;
-    int n = p.positions[q1 - 1] + 1;                 // positions ascend within a sequence
+    int n = max(p.positions[q1 - 1] + 1, 0);         // positions ascend within a sequence; a negative one has no keys
     if (!guard_ok(p.c.pages.guard, KV8_SITE_PROMPTS, n, (long long)most + 1)) n = most;
     if (blockIdx.z == 0 && threadIdx.x == 0) p.table[page] = page;
     if (blockIdx.x == 0 && blockIdx.z == 0)

@@ -233,7 +233,7 @@ def kv8_attention(q, cache: Kv8Cache, positions, batch_idx, page_table, sm_scale
     page-table row batch_idx[t]) over the keys 0..position of its sequence.  q [T, n_heads, hd], bf16 on a GPU -> [T, n_heads, hd].  With
     `qo_indptr` ([B + 1], contiguous token ranges of the sequences, at most `max_q` tokens and `max_kv_len` keys each; 0: not known; positions ascend
     within a range) heads have 64 or 128 values on a GPU, and rows in no range are not written; without it `max_kv_len` is a hint.  A row
-    may have no keys (position -1) and is zero.  At most 1024 query heads."""
+    may have no keys (a negative position) and is zero.  At most 1024 query heads."""
     (T, n_heads, hd), device = q.shape, q.get_device()
     _, n_kv, width = cache.k.shape
     if hd != width or n_heads % n_kv:
@@ -244,7 +244,7 @@ def kv8_attention(q, cache: Kv8Cache, positions, batch_idx, page_table, sm_scale
     if device < 0:
         out = torch.zeros(T, n_heads, hd, dtype=torch.float32)
         for t in range(T):
-            n = int(positions[t]) + 1
+            n = max(int(positions[t]) + 1, 0)
             kp = torch.arange(n)
             if n:
                 k, v = _cached(cache, _slots(kp, torch.full_like(kp, int(batch_idx[t])), page_table, cache.page_size))

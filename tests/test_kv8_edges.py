@@ -8,7 +8,9 @@ import re
 import pytest
 import torch
 
+from mp_util import run_ranks
 from slopllm_b200.models.dense import DenseConfig, DenseModel, load_dense_model, random_dense_model
+from slopllm_b200.ops import kv8 as K8
 from slopllm_b200.parallel.dist import ParallelContext
 
 CSRC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "slopllm_b200", "csrc")
@@ -82,3 +84,42 @@ def test_both_types_reach_the_loader(tmp_path):
     load_registered(reg, str(tmp_path), cpu, 0, "float32", "e4m3")
     load_registered(reg, str(tmp_path), cpu, 0, None, None)
     assert got == [{"dtype": torch.float32, "kv_dtype": "e4m3"}, {"kv_dtype": "e4m3"}, {}]
+
+
+def _two_ranks(rank, world, hybrid):
+    from slopllm_b200.parallel.dist import init_from_env
+    from slopllm_b200.runtime.engine import Engine
+    cfg = DenseConfig.tiny(hybrid=hybrid)
+    prompt = torch.randint(2, cfg.vocab_size, (90,), generator=torch.Generator().manual_seed(5)).tolist()
+
+    def serve(ctx, r, n):
+        w, _ = random_dense_model(cfg, 3, "cpu", torch.float32, r, n)
+        eng = Engine(cfg, DenseModel(cfg, w, ctx, kv_dtype="e4m3"), num_pages=8, max_batch=2, max_seq_len=256)
+        s, _ = eng.kv.start_request(prompt)
+        _, hid = eng.prefill([s], [prompt], chunk_size=64, want_hidden=True)
+        return [eng.model.compute_logits(hid[0])[-1:].float(), *(eng.step([s], [[7 + i]], [[0]])[0][None].float() for i in range(3))], eng.cache
+
+    got, cache = serve(init_from_env("gloo"), rank, world)
+    want, whole = serve(ParallelContext(device=torch.device("cpu")), 0, 1)
+    i = min(cache.kv8)
+    n_kv = cache.kv8[i].k.shape[1]
+    heads = slice(rank * n_kv, (rank + 1) * n_kv)
+    # (the first full-attention layer's rows see no sum over ranks in front of them where it is the model's first layer)
+    same = hybrid or all(torch.equal(getattr(cache.kv8[i], x), getattr(whole.kv8[i], x)[:, heads]) for x in ("k", "v", "exps"))
+    return same, n_kv * world == whole.kv8[i].k.shape[1], max(((a - b).abs().max() / b.abs().max()).item() for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("hybrid", [False, True])
+def test_two_ranks(hybrid):
+    """Key heads over two ranks: each rank's part of the cache is the whole one's, and so are the logits, up to the order of sums over ranks, which can move a
+    value of a later layer to the next code (2^-3 of it, of some 64 in a head)."""
+    for same, shared, err in run_ranks(_two_ranks, 2, hybrid):
+        assert same and shared and err < 2e-2, err
+
+
+def test_negative_positions_have_no_keys():
+    """Any negative position, as on a GPU."""
+    cache = K8.Kv8Cache.allocate(1, 16, 1, 16, "cpu")
+    i32 = lambda *x: torch.tensor(x, dtype=torch.int32)
+    got = K8.kv8_attention(torch.ones(3, 2, 16), cache, i32(-1, -2, -70), i32(0, 0, 0), i32(0)[None], 1.0)
+    assert (got == 0).all()

@@ -294,3 +294,14 @@ def test_ranges_without_keys(scale):
     plain = D.paged_attention(q, *rows, pos, idx, table, 64, scale, qo_indptr=ints([0, 250, 330, 400]), max_q=250, max_kv_len=100)
     tcgen05.check_errors(q.device)
     assert (plain[pos < 0] == 0).all() and not plain.isnan().any()
+
+
+def test_any_negative_position_has_no_keys():
+    """Not only -1: decoding and both prompt kernels."""
+    cache, table, keys, values, g = filled([100], 2, 64, 6)
+    q = torch.randn(6, 4, 64, generator=g, device="cuda").to(torch.bfloat16)
+    pos, idx = ints([-1000, -64, -2, -90, -7, 99]), ints([0] * 6)
+    for scale, more in ((0.1, {}), (0.1, dict(qo_indptr=ints([0, 3, 6]), max_q=3, max_kv_len=100)), (-0.1, dict(qo_indptr=ints([0, 3, 6]), max_q=3, max_kv_len=100))):
+        got = K8.kv8_attention(q, cache, pos, idx, table, scale, **more)
+        tcgen05.check_errors(q.device)
+        assert (got[:5] == 0).all() and got[5].abs().max() > 0
