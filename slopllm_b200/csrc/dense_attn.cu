@@ -341,10 +341,14 @@ static bool short_prefill(const PagedPrefillParams* p, int B, int max_q) {
     return p->hd == 64 ? p->max_keys <= (blocks >= 512 ? 64 : 32) : p->max_keys <= 32 && blocks >= 1024;
 }
 
+// Whether the tcgen05 kernel can take these arguments: a page is a key tile there, and a row's reference the largest score before the scale.
+static bool tcgen05_takes(const PagedPrefillParams* p, int B, int max_q) {
+    return p->page_size == 64 && (p->hd == 128 || p->hd == 64) && p->err != nullptr && p->sm_scale > 0.f && B <= 65535 && max_q <= 65535 * 128 &&
+           (((uintptr_t)p->q | (uintptr_t)p->k_cache | (uintptr_t)p->v_cache | (uintptr_t)p->out) & 15) == 0;
+}
+
 bool paged_prefill_in_tcgen05(const PagedPrefillParams* p, int B, int max_q) {
-    // a page is a key tile of the tcgen05 kernel (a row's reference there is the largest score before the scale)
-    return p->n_heads % p->n_kv == 0 && p->page_size == 64 && (p->hd == 128 || p->hd == 64) && p->err != nullptr && p->sm_scale > 0.f && B <= 65535 &&
-           max_q <= 65535 * 128 && (((uintptr_t)p->q | (uintptr_t)p->k_cache | (uintptr_t)p->v_cache | (uintptr_t)p->out) & 15) == 0 && !short_prefill(p, B, max_q);
+    return p->n_heads % p->n_kv == 0 && tcgen05_takes(p, B, max_q) && !short_prefill(p, B, max_q);
 }
 
 template <int HD, int TERMS, bool CLEAN>
@@ -360,9 +364,8 @@ static int prefill(const PagedPrefillParams* p, int B, int max_q, cudaStream_t s
     if (B == 0 || max_q == 0) return 0;
     if (p->n_heads % p->n_kv != 0) return -1;
     dim3 grid((max_q + QT - 1) / QT, p->n_heads, B);
-    if (p->page_size == 64 && (p->hd == 128 || p->hd == 64) && p->err != nullptr && p->sm_scale > 0.f && B <= 65535 && max_q <= 65535 * 128 &&
-        (((uintptr_t)p->q | (uintptr_t)p->k_cache | (uintptr_t)p->v_cache | (uintptr_t)p->out) & 15) == 0) {
-        if (!short_prefill(p, B, max_q)) return paged_prefill_tcgen05(p, B, max_q, s);
+    if (tcgen05_takes(p, B, max_q)) {
+        if (!short_prefill(p, B, max_q)) return CLEAN ? -1 : paged_prefill_tcgen05(p, B, max_q, s);      // (a workspace for it is another one)
         if (p->hd == 128) launch_prefill<128, 2, CLEAN>(p, grid, s, spoiled);
         else launch_prefill<64, 2, CLEAN>(p, grid, s, spoiled);
         return SL_LAUNCH_CHECK();
