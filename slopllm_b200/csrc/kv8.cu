@@ -515,7 +515,14 @@ __global__ void __launch_bounds__(512, 2) kv8_unpack_kernel(Kv8UnpackParams p) {
     }
 }
 
-constexpr int WARPS_WANTED = 148 * 28;       // that are resident at once; twice as many with half of the steps each take a fifth longer (2048 tokens)
+// Warps that are resident at once; twice as many with half of the steps each take a fifth longer (2048 tokens).
+int warps_wanted() {
+    static const int sms = [] {                  // (the devices are alike)
+        int device = 0, n = 0;
+        return cudaGetDevice(&device) == cudaSuccess && cudaDeviceGetAttribute(&n, cudaDevAttrMultiProcessorCount, device) == cudaSuccess && n > 0 ? n : 148;
+    }();
+    return sms * 28;
+}
 
 }  // namespace
 
@@ -529,7 +536,7 @@ SL_API int sl_kv8_store(const Kv8StoreParams* p, int T, cudaStream_t s) {
     Kv8StoreParams q = *p;
     q.T = T;
     // warps for all sub-cores, if there are steps for them; no more than need as many steps each
-    const int each = (steps - 1) / max(1, min(steps, WARPS_WANTED / T)) + 1, share = (steps - 1) / each + 1;
+    const int each = (steps - 1) / max(1, min(steps, warps_wanted() / T)) + 1, share = (steps - 1) / each + 1;
     const long long blocks = ((long long)T * share + WARPS - 1) / WARPS;
     if (blocks > 0x7fffffff) return -1;
 #define SL_KS(LL)                                                                                          \
