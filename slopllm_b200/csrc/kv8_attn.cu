@@ -740,19 +740,27 @@ Deal deal_of(const Shape& sh, int n_heads, int n_kv, int blocks) {
     return {items, abreast < blocks ? abreast : blocks, abreast < blocks ? passes : (items + blocks - 1) / blocks};
 }
 
-// Longer ones cost a ragged batch more than the join (16 heads over 8 of 128, us whole and cut: 32 tokens of 500 keys 13.7 and 18.4, of 1000 19.5 and 24.4, of
-// up to 1500, ragged, 25.8 and 24.0; 48 tokens of up to 1500 34.3 and 31.5).
+// Up to here a history is not cut: faster at every batch measured, while longer ones depend on how evenly the tokens fill the blocks.  16 heads over 8 of 128, us
+// whole and cut: 32 tokens of 500 keys 12.0 and 16.6, of up to 500, ragged, 13.2 and 15.2; of 1000 17.1 and 21.4, ragged 17.3 and 20.8, but ragged 1500 21.2
+// and 20.9, and 48 ragged 1000 24.6 and 23.6.  (A captured step of the engine tells a power of two of 1024 or more: it is cut.)
 constexpr int WHOLE = 512;
 
 // Whether clusters of SIZE are the faster form, for `jobs` tokens x items.  All of them have to run at once, and a block there must not have many more
-// keys than here, where the blocks of the device share the batch (histories of half the longest on average) and a second kernel joins: 400 more, 256 in
-// the instances for 16 heads.  16 heads over 8 key heads of 128, us in clusters and without: 1 token of 100 keys 7.0 and 6.4, of 700 7.2 and 9.3, of 2000
-// 8.2 and 10.2, of 4000 10.4 and 10.6, of 8000 14.0 and 11.9; 8 tokens of 1000 keys (clusters of 4) 9.7 and 15.0, of 2000 13.8 and 18.9, where clusters
-// of 8, more than run at once, take 20.7; 16 tokens of 500 keys (of 2) 9.4 and 15.2.  7 tokens of up to 5000 keys, 16 heads over 2 of 256: 14.4 and 17.4.
+// keys than here, where the blocks of the device share the batch (histories of half the longest on average) and a second kernel joins.  How many more depends on how
+// much of the device the clusters take, since the second kernel costs more with more parts.  Measured on both sides (us, clusters and cut; keys more in brackets):
+// * up to a quarter of the blocks: one token, heads of 128 over 8, 4000 keys 10.1 and 10.4 (446), 6000 11.9 and 11.6 (669); of 64 over 8, 3000 9.5 and 9.8 (355), 4000 10.5
+//   and 9.9 (473); of 256 over 2, 3500 13.0 and 12.8 (414), two tokens of 4000 13.7 and 12.8 (446); 16 heads a key head: of 128 over 2, one of 2000 11.7 and 11.8
+//   (236), of 3000 12.3 and 11.9 (355); of 64 over 4, one of 1500 10.1 and 10.3 (182), of 2000 10.9 and 10.5 (243).
+// * two fifths and more: heads of 256 over 2, 4 tokens of 6000 15.8 and 16.9 (588), of 7000 17.5 and 16.9 (686), 7 of up to 8000, ragged, 18.9 and 20.3 (622); of 128 over 8,
+//   3 of up to 6000 13.3 and 15.0 (507), of up to 8000 14.8 and 14.6 (676); of 64 over 8, 8 of up to 9000 18.6 and 18.3 (639); 16 heads a key head: of 64 over 4, 8 of up to
+//   6000 19.9 and 22.4 (588), of 128 over 2, 4 of up to 6000 15.8 and 16.2 (588); clusters of 4 and 2: heads of 128 over 8, 8 of up to 5000 17.3 and 18.5 (709), 16 of up
+//   to 2500 17.7 and 18.1 (709).
+// 8 tokens of 1000 keys, 8 key heads of 128 (clusters of 4), 9.7 and 15.1; 16 of 500 (of 2) 9.3, and 11.9 uncut; clusters of 8 for 8 tokens of 2000, more than run
+// at once, 20.7, of 4 12.1.
 template <int D, int NG, int SIZE>
 bool clusters_pay(int longest, long long jobs, int blocks, int smem) {
-    constexpr int MORE = NG == 2 ? 256 : 400;                        // keys
-    if (longest <= 2 * KT || jobs * SIZE > blocks || longest * (2 * blocks - jobs * SIZE) > 2ll * MORE * SIZE * blocks) return false;
+    const int more = jobs * SIZE * 3 > blocks ? 640 : NG == 2 ? 256 : 400;           // keys
+    if (longest <= 2 * KT || jobs * SIZE > blocks || longest * (2 * blocks - jobs * SIZE) > 2ll * more * SIZE * blocks) return false;
     static const int at_once = [=] {                                 // (the devices are alike)
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = SIZE;
