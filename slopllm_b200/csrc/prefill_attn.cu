@@ -16,8 +16,8 @@
 // HALF (workspaces of the 8-bit cache, kv8.cu): values are fp16 times a power of two per page and head, or, where a page's scales are too far apart for
 // that to be exact, per token; P is one fp16 term: its 11 bits are enough beside the output's 8, and the second product against the same values (a
 // third of the tensor time) and the making of the second term fall away.  The exponents go into the weights, as part of the row's reference, and out of
-// the denominator.  Chunk of 4096 behind 8192, 32 heads of 128 over 8, with the reading of the cache (24 us): 808 to 842 us with bf16 values, 610 to
-// 660 so (1.1 PFLOP/s; the clock follows the power limit).  Of the 850 cycles that a tile of 64 keys takes, its products take 8 x 76 for S, whose
+// the denominator.  Chunk of 4096 behind 8192, 32 heads of 128 over 8, with the reading of the cache (24 us): 808 to 842 us with bf16 values, 590 to
+// 640 so (1.1 PFLOP/s; the clock follows the power limit).  Of the 850 cycles that a tile of 64 keys takes, its products take 8 x 76 for S, whose
 // operands come from shared memory (32 of arithmetic), and 256 for P V.  Blocks of 256 queries with tiles of 128 keys read less for S, but a tile's next
 // scores have no room beside its weights: 623 us.
 //
