@@ -305,3 +305,26 @@ def test_any_negative_position_has_no_keys():
         got = K8.kv8_attention(q, cache, pos, idx, table, scale, **more)
         tcgen05.check_errors(q.device)
         assert (got[:5] == 0).all() and got[5].abs().max() > 0
+
+
+@pytest.mark.parametrize("scale", [0.1, -0.1])
+def test_groups_of_key_heads_change_nothing(scale, monkeypatch):
+    """A history that goes in groups of key heads, with values that are not finite, pages with a scale per token and other page sizes: the same bits."""
+    n, first, h, kv, hd = 300, 90, 9, 3, 64
+    for page in (64, 48):
+        cache, table, _, _, g = filled([n], kv, hd, page, page)
+        x = torch.randn(n, kv, hd, generator=g, device="cuda")
+        x[::7, 1] *= 2.0 ** -40
+        put(cache, table, 0, torch.arange(n, device="cuda"), 1, x)
+        for p, head, d in ((120, 0, 3), (200, 2, 63), (201, 1, 0)):
+            cache.v[int(table[0, p // page]) * page + p % page, head, d] = 0x7f
+        q = torch.randn(n - first, h, hd, generator=g, device="cuda").to(torch.bfloat16)
+        pos, idx = torch.arange(first, n, dtype=torch.int32, device="cuda"), torch.zeros(n - first, dtype=torch.int32, device="cuda")
+        call = lambda: K8.kv8_attention(q, cache, pos, idx, table, scale, qo_indptr=ints([0, n - first]), max_q=n - first, max_kv_len=n)
+        whole = call()
+        assert whole.isnan().any() and not whole.isnan().all()
+        for heads in (1, 2):
+            monkeypatch.setattr(K8, "UNPACK_BUDGET_BYTES", heads * 5 * 17600)
+            assert torch.equal(call().view(torch.int16), whole.view(torch.int16))
+            monkeypatch.undo()
+    tcgen05.check_errors(q.device)
