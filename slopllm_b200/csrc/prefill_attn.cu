@@ -296,6 +296,12 @@ __global__ void __launch_bounds__(THREADS, 2) prefill_attn_kernel(const __grid_c
             tc::fence_before_sync();
             tc::mbar_arrive(p_ready + (j & 1));
         }
+        if (tiles <= 0) {                                           // no product has written the sums
+            const uint32_t zero[16] = {};
+#pragma unroll 1
+            for (int c = 0; c < HD; c += 16) tc::tmem_st_32x16(lane_at + COL_O + c, zero);
+            tc::tmem_st_wait();
+        }
         // (the last product has a barrier of its own: a phase can be waited for only while the barrier is at most one phase ahead of it)
         if (ok) ok = __all_sync(0xffffffffu, tc::mbar_wait(o_done, 0));
         tc::fence_after_sync();
@@ -307,10 +313,6 @@ __global__ void __launch_bounds__(THREADS, 2) prefill_attn_kernel(const __grid_c
                 uint32_t o[32];
                 tc::tmem_ld_32x32(lane_at + COL_O + c, o);
                 tc::tmem_ld_wait();
-                if (tiles <= 0) {                                   // (no product has written the sums)
-#pragma unroll
-                    for (int x = 0; x < 32; ++x) o[x] = 0u;
-                }
                 if (bad) {
                     uint32_t nan = 0;
 #pragma unroll 1
