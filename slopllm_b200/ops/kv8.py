@@ -3,8 +3,8 @@ single tokens.  It takes the place of the bf16 cache of `ops/dense.py` at half o
 
 A token's row of one key head is `hd` e4m3 codes and one exponent byte b, for keys and for values; value = code * 2^(b - 127).  The exponent
 is the smallest between -60 and 60 with which the largest finite magnitude of the row is at most 448; larger values saturate, and a value that
-is not finite is the NaN code.  Codes lie at [slot, head, :] with slot = page * page_size + offset, exponent bytes at [page, head, 0 (keys) or
-1 (values), offset].
+is not finite is the NaN code: in attention a value's spoils its column, a key's the whole head, for the queries that see it and no other.
+Codes lie at [slot, head, :] with slot = page * page_size + offset, exponent bytes at [page, head, 0 (keys) or 1 (values), offset].
 
 CUDA tensors run `csrc/kv8.cu` and `csrc/kv8_attn.cu` (prompts: the tcgen05 kernel of `csrc/prefill_attn.cu` over rows read back, which bf16 holds
 exactly); CPU tensors run the fp32 definition below.
