@@ -322,6 +322,10 @@ _SIGS = {
     "sl_build_group_tiles": [vp, vp, vp, i32, i32, i32, i32, vp],
     "sl_nvfp4_dequant_bf16": [vp, vp, vp, vp, i32, i32, i32, i32, i32, vp],
     "sl_linear_fp8_block": [vp, vp, vp, vp, i32, i32, i32, i32, i32, i32, i32, vp],
+    "sl_fp8_add_rmsnorm": [vp, i32, i32, i32, vp],
+    "sl_fp8_rows": [vp, i32, i32, vp],
+    "sl_fp8_values": [vp, vp],
+    "sl_fp8_linear": [vp, i32, vp, i32, vp, vp],
     "sl_fp8_block_dequant_bf16": [vp, vp, vp, i32, i32, i32, vp],
     "sl_moe_unsort_reduce": [vp, vp, vp, vp, i32, i32, i32, i32, i32, vp],
     "sl_gemm_pair_ok": [i32, i32],
