@@ -9,9 +9,8 @@
 // All mbarrier waits are bounded; where one runs out, the error word is set and the blocks still meet at the end.
 #include <algorithm>
 
-#include "f32x2.cuh"
 #include "fp8_rows.cuh"
-#include "tcgen05.cuh"
+#include "tcgen05_pair.cuh"
 
 namespace {
 
@@ -20,9 +19,6 @@ enum { WAIT_FREE = 70, WAIT_LANDED, WAIT_READ, WAIT_FETCHED, WAIT_SUMS };       
 
 __device__ __forceinline__ float two_to(int byte) {          // 2^(byte - 127), for the exponents that writers leave
     return __uint_as_float((uint32_t)(max(FP8_LOW, min(FP8_HIGH, byte - FP8_BIAS)) + 127) << 23);
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ float4 ld_cluster(uint32_t at, uint32_t rank) {
     float4 v;
@@ -87,7 +83,7 @@ __global__ void __launch_bounds__(192) fp8_few_kernel(const __grid_constant__ CU
             int it = 0;
             for (int kb = kb0; kb < kb1; ++kb, ++it) {
                 const int s = it % C::STAGES;
-                if (!tc::mbar_wait(&empty[s], ((it / C::STAGES) & 1) ^ 1)) { atomicExch(p.err, WAIT_FREE); break; }
+                if (!tc::mbar_wait_soon(&empty[s], ((it / C::STAGES) & 1) ^ 1)) { atomicExch(p.err, WAIT_FREE); break; }
                 tc::mbar_expect_tx(&full[s], C::STAGE);
                 tc::tma_load_2d(smem + s * C::STAGE, &tmW, &full[s], kb * BK, n0);
                 tc::tma_load_2d(smem + s * C::STAGE + C::A_BYTES, &tmX, &full[s], kb * BK, t0);
@@ -102,8 +98,8 @@ __global__ void __launch_bounds__(192) fp8_few_kernel(const __grid_constant__ CU
         const uint32_t t_base = tc::warp_uniform(tmem);
         for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {
             const int s = it % C::STAGES, buf = it % C::BUFS;
-            if (!tc::mbar_wait_warp(&acc_empty[buf], ((it / C::BUFS) & 1) ^ 1)) { if (lane == 0) atomicExch(p.err, WAIT_READ); break; }
-            if (!tc::mbar_wait_warp(&full[s], (it / C::STAGES) & 1)) { if (lane == 0) atomicExch(p.err, WAIT_FETCHED); break; }
+            if (!tc::mbar_wait_soon_warp(&acc_empty[buf], ((it / C::BUFS) & 1) ^ 1)) { if (lane == 0) atomicExch(p.err, WAIT_READ); break; }
+            if (!tc::mbar_wait_soon_warp(&full[s], (it / C::STAGES) & 1)) { if (lane == 0) atomicExch(p.err, WAIT_FETCHED); break; }
             tc::fence_after_sync();
             const uint64_t a = tc::desc_at(base, s * C::STAGE), b = tc::desc_at(a, C::A_BYTES);
             if (tc::elect_one()) {
@@ -138,7 +134,7 @@ __global__ void __launch_bounds__(192) fp8_few_kernel(const __grid_constant__ CU
             }
             const int buf = it % C::BUFS;
             if (ok) {
-                ok = tc::mbar_wait_warp(&acc_full[buf], (it / C::BUFS) & 1);
+                ok = tc::mbar_wait_soon_warp(&acc_full[buf], (it / C::BUFS) & 1);
                 if (!ok && lane == 0) atomicExch(p.err, WAIT_SUMS);
             }
             tc::fence_after_sync();
@@ -171,7 +167,7 @@ __global__ void __launch_bounds__(192) fp8_few_kernel(const __grid_constant__ CU
     }
     tc::fence_before_sync();
     __syncthreads();
-    cluster_sync();
+    tc::cluster_sync();
     {
         const int rows = min(BN, p.T - t0), units = rows * 32;
         const uint32_t part = tc::smem_u32(smem);
@@ -198,7 +194,7 @@ __global__ void __launch_bounds__(192) fp8_few_kernel(const __grid_constant__ CU
             }
         }
     }
-    cluster_sync();                                          // nobody's sums go away while they are read
+    tc::cluster_sync();                                          // nobody's sums go away while they are read
     if (warp == 1) {
         tc::fence_after_sync();
         tc::tmem_dealloc(tmem, C::COLS);
@@ -231,6 +227,12 @@ int launch_few(const void* x, int ldx, const void* W, int ldw, const Fp8LinearPa
     return rc != cudaSuccess ? (int)rc : SL_LAUNCH_CHECK();
 }
 
+bool aligned(const void* x, int ldx, const void* W, int ldw, const Fp8LinearParams& p) {
+    const int blocks = (p.K + BK - 1) / BK;
+    return p.K > 0 && p.K % 16 == 0 && ldx % 16 == 0 && ldw % 16 == 0 && p.lde % 16 == 0 && p.lds >= blocks && p.lde >= blocks &&
+           (((uintptr_t)x | (uintptr_t)W | (uintptr_t)p.exps | (uintptr_t)p.y) & 15) == 0;
+}
+
 }  // namespace
 
 // x: codes [T, K], rows `ldx` bytes apart; W: codes [N, K], rows `ldw` apart.  K, ldx, ldw and the rows of exponents are multiples of 16 and start there;
@@ -238,11 +240,10 @@ int launch_few(const void* x, int ldx, const void* W, int ldw, const Fp8LinearPa
 SL_API int sl_fp8_linear(const void* x, int ldx, const void* W, int ldw, const Fp8LinearParams* params, cudaStream_t s) {
     const Fp8LinearParams& p = *params;
     if (p.T <= 0 || p.N <= 0) return 0;
-    if (p.K <= 0 || p.K % 16 != 0 || ldx % 16 != 0 || ldw % 16 != 0 || p.lde % 16 != 0 || p.ldy % (p.out_f32 ? 4 : 8) != 0) return -1;
-    if ((((uintptr_t)x | (uintptr_t)W | (uintptr_t)p.exps | (uintptr_t)p.y) & 15) != 0 || p.lds < (p.K + BK - 1) / BK || p.lde < (p.K + BK - 1) / BK) return -1;
+    if (!aligned(x, ldx, W, ldw, p) || p.ldy % (p.out_f32 ? 4 : 8) != 0 || (p.N + 127) / 128 > 65535) return -1;
+    if (p.T > 128) return fp8_pair(x, ldx, W, ldw, p, false, s);
     const int bn = p.T <= 16 ? 16 : p.T <= 32 ? 32 : p.T <= 64 ? 64 : 128;
     const long long tiles = (long long)((p.N + 127) / 128) * ((p.T + bn - 1) / bn);
-    if ((p.N + 127) / 128 > 65535 || (p.T + bn - 1) / bn > 65535) return -1;
     const int blocks = (p.K + BK - 1) / BK;
     int shares = 1;
     while (shares < 8 && tiles * shares * 2 <= 296 && blocks >= shares * 4) shares *= 2;
@@ -250,4 +251,12 @@ SL_API int sl_fp8_linear(const void* x, int ldx, const void* W, int ldw, const F
     if (bn == 32) return launch_few<32>(x, ldx, W, ldw, p, shares, s);
     if (bn == 64) return launch_few<64>(x, ldx, W, ldw, p, shares, s);
     return launch_few<128>(x, ldx, W, ldw, p, shares, s);
+}
+
+// y: codes [T, N / 2] of silu(gate) * up, with exponents exps_out; W: N / 2 gate rows | N / 2 up rows, a multiple of 128 each.
+SL_API int sl_fp8_gate_up(const void* x, int ldx, const void* W, int ldw, const Fp8LinearParams* params, cudaStream_t s) {
+    const Fp8LinearParams& p = *params;
+    if (p.T <= 0 || p.N <= 0) return 0;
+    if (!aligned(x, ldx, W, ldw, p) || p.N % 256 != 0 || p.ldy % 16 != 0) return -1;
+    return fp8_pair(x, ldx, W, ldw, p, true, s);
 }

@@ -15,13 +15,7 @@ namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
 
-__device__ __forceinline__ bool finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
-
-// Smallest exponent with which a magnitude (bits of an fp32 number) is at most 448 * 2^exponent, within the limits.
-__device__ __forceinline__ int exponent_of(uint32_t top) {
-    const int e = (int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
-    return max(FP8_LOW, min(FP8_HIGH, e));
-}
+// Smallest exponent with which a magnitude is at most 448 * 2^exponent, within the limits.
 __device__ __forceinline__ int exponent_of(double top) {
     const uint64_t bits = (uint64_t)__double_as_longlong(top);
     const int e = (int)(bits >> 52) - 1023 - 8 + ((bits & 0xfffffffffffffull) > 0xc000000000000ull ? 1 : 0);
@@ -39,13 +33,7 @@ __device__ __forceinline__ bool near_middle(float f, uint32_t within) {
 // An fp32 number that any rounding to fewer bits takes where it would take `d`: cut off, with the last bit set where something was.
 __device__ __forceinline__ float to_odd(double d) {
     const float f = __double2float_rz(d);
-    return (double)f == d || !finite(f) ? f : __uint_as_float(__float_as_uint(f) | 1u);
-}
-
-__device__ __forceinline__ uint32_t codes_of(const float (&f)[4]) {
-    const uint32_t lo = __nv_cvt_float2_to_fp8x2(make_float2(f[0], f[1]), __NV_SATFINITE, __NV_E4M3);
-    const uint32_t hi = __nv_cvt_float2_to_fp8x2(make_float2(f[2], f[3]), __NV_SATFINITE, __NV_E4M3);
-    return lo | hi << 16;
+    return (double)f == d || !fp8_finite(f) ? f : __uint_as_float(__float_as_uint(f) | 1u);
 }
 
 // A group in a warp, four values a lane, in fp32 off by up to `within` of their last places (0: exact).  `again(i)`: value i in 64 bits.  The lane's codes;
@@ -54,9 +42,9 @@ template <class Again>
 __device__ __forceinline__ uint32_t quantize_group(float (&v)[4], uint32_t within, bool all, int& e, Again again) {
     uint32_t top = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) top = max(top, finite(v[i]) ? __float_as_uint(v[i]) & 0x7fffffffu : 0u);
+    for (int i = 0; i < 4; ++i) top = max(top, fp8_finite(v[i]) ? __float_as_uint(v[i]) & 0x7fffffffu : 0u);
     top = __reduce_max_sync(0xffffffffu, top);
-    e = exponent_of(top);
+    e = fp8_exponent(top);
     if (within != 0 && (all || (top & 0x7fffffu) - (0x600000u - within) <= 2 * within)) {
         double most = 0.0;
 #pragma unroll
@@ -72,7 +60,7 @@ __device__ __forceinline__ uint32_t quantize_group(float (&v)[4], uint32_t withi
     bool near = all;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        v[i] = finite(v[i]) ? v[i] * down : __uint_as_float(0x7fffffffu);
+        v[i] = fp8_finite(v[i]) ? v[i] * down : __uint_as_float(0x7fffffffu);
         if (within != 0) near |= near_middle(v[i], within);
     }
     if (within != 0 && near) {
@@ -82,7 +70,7 @@ __device__ __forceinline__ uint32_t quantize_group(float (&v)[4], uint32_t withi
             if (all || near_middle(v[i], within)) v[i] = fabs(d) <= (double)FLT_MAX ? to_odd(d * (double)down) : __uint_as_float(0x7fffffffu);
         }
     }
-    return codes_of(v);
+    return fp8_codes(v);
 }
 
 template <bool F32>

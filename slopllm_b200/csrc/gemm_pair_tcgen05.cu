@@ -17,7 +17,7 @@
 #include <algorithm>
 
 #include "gemm_pair.cuh"
-#include "tcgen05.cuh"
+#include "tcgen05_pair.cuh"
 
 namespace {
 
@@ -25,43 +25,6 @@ constexpr int BM = 128, BN = 256, BK = 64, STAGES = 6, EPI_WARPS = 8, THREADS = 
 constexpr int HALF_BYTES = 128 * BK * 2;                     // one operand of one SM: 16 KB
 constexpr int STAGE_BYTES = 2 * HALF_BYTES;
 constexpr int SMEM = STAGES * STAGE_BYTES + 1024 + 256;
-
-__device__ __forceinline__ uint32_t cluster_rank() {
-    uint32_t r;
-    asm volatile("mov.u32 %0, %cluster_ctarank;" : "=r"(r));
-    return r;
-}
-__device__ __forceinline__ void cluster_sync() {
-    asm volatile("barrier.cluster.arrive.release.aligned;\n barrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
-// address of `p` (shared memory of this block) in the leading block of the pair
-__device__ __forceinline__ uint32_t in_leader(const void* p) {
-    uint32_t r;
-    asm volatile("mapa.shared::cluster.u32 %0, %1, 0;" : "=r"(r) : "r"(tc::smem_u32(p)));
-    return r;
-}
-__device__ __forceinline__ void arrive_cluster(uint32_t bar) {
-    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-// into this block's shared memory, completion counted by a barrier that may be the other block's
-__device__ __forceinline__ void tma_load_2d_pair(void* dst, const CUtensorMap* map, uint32_t bar, int c0, int c1) {
-    asm volatile("cp.async.bulk.tensor.2d.cta_group::2.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4}], [%2];"
-                 ::"r"(tc::smem_u32(dst)), "l"(map), "r"(bar), "r"(c0), "r"(c1) : "memory");
-}
-__device__ __forceinline__ void mma_pair(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n"
-        ".reg .pred p;\n"
-        "setp.ne.b32 p, %4, 0;\n"
-        "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n"
-        "}\n"
-        ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate) : "memory");
-}
-// arrives on the barrier at this place in both blocks once the products issued so far are done
-__device__ __forceinline__ void commit_pair(uint64_t* bar) {
-    asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], %1;"
-                 ::"r"(tc::smem_u32(bar)), "h"((uint16_t)3) : "memory");
-}
 
 __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS) gemm_pair_kernel(const __grid_constant__ CUtensorMap tmA,
                                                                                      const __grid_constant__ CUtensorMap tmB, GemmPairParams p) {
@@ -73,7 +36,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS) gemm_pair_k
     uint64_t* acc_empty = acc_full + 2;                      // [2] accumulator read by both blocks (the leader's counts)
     uint32_t* holder = reinterpret_cast<uint32_t*>(acc_empty + 2);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const uint32_t rank = tc::warp_uniform(cluster_rank());
+    const uint32_t rank = tc::warp_uniform(tc::cluster_rank());
     if (warp == 0 && lane == 0) {
         tc::tma_prefetch_desc(&tmA);
         tc::tma_prefetch_desc(&tmB);
@@ -82,12 +45,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS) gemm_pair_k
         tc::mbar_fence_init();
     }
     if (warp == 1) {
-        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(tc::smem_u32(holder)), "r"(2u * BN) : "memory");
-        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;" ::: "memory");
+        tc::tmem_alloc_pair(holder, 2 * BN);
     }
     tc::fence_before_sync();
     __syncthreads();
-    cluster_sync();                                          // the other block's barriers exist
+    tc::cluster_sync();                                          // the other block's barriers exist
     tc::fence_after_sync();
     const uint32_t tmem = *holder;
     pdl_grid_sync();
@@ -114,10 +76,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS) gemm_pair_k
                     const int s = it % STAGES;
                     if (!tc::mbar_wait(&empty[s], ((it / STAGES) & 1) ^ 1)) { atomicExch(p.err, 50); ok = false; break; }
                     if (rank == 0) tc::mbar_expect_tx(&full[s], 2 * STAGE_BYTES);
-                    const uint32_t bar = in_leader(&full[s]);
+                    const uint32_t bar = tc::in_leader(&full[s]);
                     uint8_t* a = smem + s * STAGE_BYTES;
-                    tma_load_2d_pair(a, &tmA, bar, a_c0 + kb * BK, m0 + (int)rank * BM);
-                    tma_load_2d_pair(a + HALF_BYTES, &tmB, bar, kb * BK, b_row0);
+                    tc::tma_load_2d_pair(a, &tmA, bar, a_c0 + kb * BK, m0 + (int)rank * BM);
+                    tc::tma_load_2d_pair(a + HALF_BYTES, &tmB, bar, kb * BK, b_row0);
                 }
             }
             // Nothing is in flight when the pair ends, also where a wait ran out.  Both SMs' copies of a K block signal the leader's `full`, so the
@@ -147,12 +109,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS) gemm_pair_k
                     if (tc::elect_one()) {
 #pragma unroll
                         for (int k = 0; k < BK / 16; ++k)
-                            mma_pair(t_base + buf * BN, tc::desc_at(a, k * 32), tc::desc_at(b, k * 32), idesc, (kb > 0 || k > 0) ? 1u : 0u);
-                        commit_pair(&empty[s]);
+                            tc::mma_f16_pair(t_base + buf * BN, tc::desc_at(a, k * 32), tc::desc_at(b, k * 32), idesc, (kb > 0 || k > 0) ? 1u : 0u);
+                        tc::commit_pair(&empty[s]);
                     }
                     __syncwarp();
                 }
-                if (ok && tc::elect_one()) commit_pair(&acc_full[buf]);
+                if (ok && tc::elect_one()) tc::commit_pair(&acc_full[buf]);
                 __syncwarp();
             }
         }
@@ -233,15 +195,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS) gemm_pair_k
             }
             tc::fence_before_sync();
             __syncwarp();
-            if (lane == 0) arrive_cluster(in_leader(&acc_empty[buf]));
+            if (lane == 0) tc::arrive_cluster(tc::in_leader(&acc_empty[buf]));
         }
     }
     tc::fence_before_sync();
     __syncthreads();
-    cluster_sync();                                          // neither block leaves while the other may still signal it
+    tc::cluster_sync();                                          // neither block leaves while the other may still signal it
     if (warp == 1) {
         tc::fence_after_sync();
-        asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2u * BN) : "memory");
+        tc::tmem_dealloc_pair(tmem, 2 * BN);
     }
 }
 

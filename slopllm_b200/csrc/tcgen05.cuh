@@ -60,6 +60,12 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, uint64
         if ((i & 255u) == 255u && globaltimer_ns() - t0 > limit_ns) return false;
     }
 }
+// The same for places that are passed every few hundred cycles: the clock is not read before the wait has become a long one.
+__device__ __forceinline__ bool mbar_wait_soon(uint64_t* bar, uint32_t parity, uint64_t limit_ns = 2000000000ull) {
+    for (uint32_t i = 0; i < 64; ++i)
+        if (mbar_try_wait(bar, parity)) return true;
+    return mbar_wait(bar, parity, limit_ns);
+}
 
 // ---- TMA (tiled, 2D / 3D, no multicast) --------------------------------------------------------------
 __device__ __forceinline__ void tma_load_2d(void* smem_dst, const CUtensorMap* map, uint64_t* bar, int c0, int c1) {
@@ -161,6 +167,7 @@ constexpr uint32_t IDESC_B_MN_MAJOR = 1u << 16;     // ... the B operand
 
 // A wait that the whole (converged) warp makes: every lane learns the outcome.
 __device__ __forceinline__ bool mbar_wait_warp(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait(bar, parity)); }
+__device__ __forceinline__ bool mbar_wait_soon_warp(uint64_t* bar, uint32_t parity) { return __all_sync(0xffffffffu, mbar_wait_soon(bar, parity)); }
 // A value that is the same in all lanes, in a form that the compiler knows to be so.
 __device__ __forceinline__ uint32_t warp_uniform(uint32_t v) { return __shfl_sync(0xffffffffu, v, 0); }
 __device__ __forceinline__ int warp_uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }

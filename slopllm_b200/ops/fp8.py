@@ -42,7 +42,7 @@ class Fp8ValuesParams(C.Structure):
 
 class Fp8LinearParams(C.Structure):
     _fields_ = [("exps", C.c_void_p), ("lde", C.c_int), ("scale", C.c_void_p), ("lds", C.c_int), ("y", C.c_void_p), ("ldy", C.c_int),
-                ("out_f32", C.c_int), ("T", C.c_int), ("N", C.c_int), ("K", C.c_int), ("err", C.c_void_p)]
+                ("out_f32", C.c_int), ("T", C.c_int), ("N", C.c_int), ("K", C.c_int), ("exps_out", C.c_void_p), ("lde_out", C.c_int), ("err", C.c_void_p)]
 
 
 def _padded(k: int) -> int:
@@ -214,42 +214,55 @@ def fp8_add_rmsnorm(x: torch.Tensor, residual: Optional[torch.Tensor], w: torch.
 
 # ---- products ----------------------------------------------------------------------------------------------------------------------------
 
-def _check_weight(rows: Fp8Rows, w) -> Tuple[torch.Tensor, torch.Tensor]:
+def _operands(rows: Fp8Rows, w) -> Tuple[torch.Tensor, torch.Tensor]:
+    """Codes and scales of FP8 weights, checked and (on a GPU) as the kernels take them."""
     codes, scale = w.weight, w.fp8_scale
     if scale is None or codes.dtype not in (torch.float8_e4m3fn, torch.uint8):
         raise ValueError("rows in 8 bits are multiplied with FP8 weights (e4m3 and a scale for each block of 128 x 128)")
-    n, k = codes.shape
+    (n, k), device = codes.shape, rows.codes.get_device()
     if k != rows.codes.shape[1] or scale.shape[0] < -(-n // GROUP) or scale.shape[1] < -(-k // GROUP):
         raise ValueError(f"rows {tuple(rows.codes.shape)}, weights {tuple(codes.shape)} with scales {tuple(scale.shape)}")
-    if codes.get_device() != rows.codes.get_device() or scale.get_device() != rows.codes.get_device():
+    if codes.get_device() != device or scale.get_device() != device:
         raise ValueError("rows, weights and scales are on one device")
+    if device >= 0:
+        if codes.stride(1) != 1 or codes.stride(0) % 16 or codes.data_ptr() % 16:
+            codes = codes.clone(memory_format=torch.contiguous_format)
+        if scale.dtype is not torch.float32 or scale.stride(1) != 1:
+            scale = scale.to(torch.float32).contiguous()
     return codes, scale
+
+
+def _multiply(name: str, rows: Fp8Rows, codes: torch.Tensor, scale: torch.Tensor, y, ldy: int, f32: int, exps_out=None, lde_out: int = 0) -> None:
+    (T, K), x, e, device = rows.codes.shape, rows.codes, rows.exps, rows.codes.get_device()
+    ldx, lde = (x.stride(0), e.stride(0)) if T > 1 else (K, _padded(K))
+    p = Fp8LinearParams(e.data_ptr(), lde, scale.data_ptr(), scale.stride(0), y.data_ptr(), ldy, f32, T, codes.shape[0], K, N.ptr(exps_out), lde_out,
+                        _status(device))
+    _call(device, name, x.data_ptr(), ldx, codes.data_ptr(), codes.stride(0), C.byref(p))
 
 
 def fp8_linear(rows: Fp8Rows, w, out_f32: bool = False) -> torch.Tensor:
     """y = rows @ W^T [T, N], fp32 sums, in bf16 or fp32.  `w`: a :class:`~slopllm_b200.models.weights.LinearWeight` in FP8.  A NaN code spoils its row's (a
     weight's: its column's) results and no other."""
-    codes, scale = _check_weight(rows, w)
-    (T, K), n, device = rows.codes.shape, codes.shape[0], rows.codes.get_device()
-    kind = torch.float32 if out_f32 else torch.bfloat16
-    if device < 0:
+    codes, scale = _operands(rows, w)
+    n, kind = codes.shape[0], torch.float32 if out_f32 else torch.bfloat16
+    if rows.codes.get_device() < 0:
         return (_values(rows) @ quant.fp8_block_dequantize(codes, scale).t()).to(kind)
-    if codes.stride(1) != 1 or codes.stride(0) % 16 or codes.data_ptr() % 16:
-        codes = codes.clone(memory_format=torch.contiguous_format)
-    if scale.dtype is not torch.float32 or scale.stride(1) != 1:
-        scale = scale.to(torch.float32).contiguous()
     pad = 4 if out_f32 else 8                        # whole pieces of 16 bytes a row
     ld = -(-n // pad) * pad
-    y = torch.empty(T, ld, dtype=kind, device=rows.codes.device)
-    ldx, lde = (rows.codes.stride(0), rows.exps.stride(0)) if T > 1 else (K, _padded(K))
-    p = Fp8LinearParams(rows.exps.data_ptr(), lde, scale.data_ptr(), scale.stride(0), y.data_ptr(), ld, int(out_f32), T, n, K,
-                        _status(device))
-    _call(device, "sl_fp8_linear", rows.codes.data_ptr(), ldx, codes.data_ptr(), codes.stride(0), C.byref(p))
+    y = torch.empty(rows.codes.shape[0], ld, dtype=kind, device=rows.codes.device)
+    _multiply("sl_fp8_linear", rows, codes, scale, y, ld, int(out_f32))
     return y if ld == n else y[:, :n]
 
 
 def fp8_gate_up(rows: Fp8Rows, w) -> Fp8Rows:
-    """silu(rows @ Wg^T) * (rows @ Wu^T) in 8 bits, W = gate rows | up rows [2 I, K]: :func:`fp8_silu_mul` of the product's fp32 sums."""
+    """silu(rows @ Wg^T) * (rows @ Wu^T) in 8 bits, W = gate rows | up rows [2 I, K]: :func:`fp8_silu_mul` of the product's fp32 sums.  Many rows make the
+    activation in the product's epilogue, in fp32: a value next to the middle between two codes may get the other one."""
+    inner = w.weight.shape[0] // 2
     if w.weight.shape[0] % 32:
         raise ValueError(f"{w.weight.shape[0]} gate and up rows: rows in 8 bits have a multiple of 16 values")
-    return fp8_silu_mul(fp8_linear(rows, w, out_f32=True))
+    if not rows.codes.is_cuda or rows.codes.shape[0] <= 128 or inner % GROUP:
+        return fp8_silu_mul(fp8_linear(rows, w, out_f32=True))
+    codes, scale = _operands(rows, w)
+    out = Fp8Rows.allocate(rows.codes.shape[0], inner, rows.codes.device)
+    _multiply("sl_fp8_gate_up", rows, codes, scale, out.codes, inner, 0, out.exps, out.exps.stride(0))
+    return out
