@@ -9,60 +9,94 @@
 // All mbarrier waits are bounded; where one runs out, the error word is set and the blocks still meet at the end.
 #include <algorithm>
 
+#include "f32x2.cuh"
 #include "fp8_rows.cuh"
 #include "tcgen05_pair.cuh"
 
 namespace {
 
 constexpr int BK = 128;                                      // values (bytes) of a block of K
-enum { WAIT_FREE = 70, WAIT_LANDED, WAIT_READ, WAIT_FETCHED, WAIT_SUMS };       // numbers of waits that run out
+enum { WAIT_FREE = 80, WAIT_LANDED, WAIT_READ, WAIT_FETCHED, WAIT_SUMS, WAIT_SENT };       // numbers of waits that run out
 
 __device__ __forceinline__ float two_to(int byte) {          // 2^(byte - 127), for the exponents that writers leave
     return __uint_as_float((uint32_t)(max(FP8_LOW, min(FP8_HIGH, byte - FP8_BIAS)) + 127) << 23);
 }
-__device__ __forceinline__ float4 ld_cluster(uint32_t at, uint32_t rank) {
-    float4 v;
+// Address of `at` (shared memory of this block) in block `rank` of the cluster.
+__device__ __forceinline__ uint32_t in_block(uint32_t at, uint32_t rank) {
     uint32_t far;
     asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(far) : "r"(at), "r"(rank));
-    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(far) : "memory");
-    return v;
+    return far;
 }
+// A piece of this block's shared memory into another block's, counted by a barrier of that block.
+__device__ __forceinline__ void send(uint32_t to, const void* from, uint32_t bytes, uint32_t bar) {
+    asm volatile("cp.async.bulk.shared::cluster.shared::cta.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];"
+                 ::"r"(to), "r"(tc::smem_u32(from)), "r"(bytes), "r"(bar) : "memory");
+}
+// The wait for what other blocks have sent (bounded).
+__device__ __forceinline__ bool wait_sent(uint64_t* bar) {
+    const uint32_t at = tc::smem_u32(bar);
+    uint64_t t0 = 0;
+    for (uint32_t i = 0;; ++i) {
+        uint32_t ok;
+        asm volatile(
+            "{\n"
+            ".reg .pred p;\n"
+            "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], 0;\n"
+            "selp.u32 %0, 1, 0, p;\n"
+            "}\n"
+            : "=r"(ok) : "r"(at) : "memory");
+        if (ok) return true;
+        if (i == 64) t0 = tc::globaltimer_ns();
+        if (i > 64 && (i & 255u) == 255u && tc::globaltimer_ns() - t0 > 2000000000ull) return false;
+    }
+}
+// A meeting of the cluster that passes no memory on: nobody waits for loads and stores in flight (a release does: 6000 cycles beside a full memory).
+__device__ __forceinline__ void cluster_arrive_relaxed() { asm volatile("barrier.cluster.arrive.relaxed.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // ---- few rows: weights are the 128-row operand, rows the columns ---------------------------------------------------------------------------
 //
-// A block has 128 features, up to BN rows and a share of K; the blocks of a cluster have the shares of the same features and join their sums in shared
-// memory, in the order of the shares.  Warp 0 fetches (TMA ring), warp 1 multiplies, warps 2 to 5 have a feature a thread and add up.
+// A block has 128 features, up to BN rows and a share of K; the blocks of a cluster have the shares of the same features.  Each block completes BN / shares
+// of the rows: the others send their sums into its shared memory, and it adds them in the order of the shares.  Warp 0 fetches (TMA ring), warp 1 multiplies, the others have a feature and up to 64 rows a thread and add up.
 template <int BN>
 struct Few {
     static constexpr int A_BYTES = 128 * BK, B_BYTES = BN * BK, STAGE = A_BYTES + B_BYTES;
-    static constexpr int BUFS = BN >= 64 ? 2 : 4;            // accumulators
+    static constexpr int BUFS = 4;                           // accumulators
     static constexpr int COLS = BN * BUFS;
-    static constexpr int STAGES = BN >= 128 ? 3 : BN == 64 ? 4 : BN == 32 ? 5 : 5;        // (two blocks an SM)
+    static constexpr int PARTS = BN >= 64 ? 2 : 1, OWN = BN / PARTS;        // threads of a feature, rows of one
+    static constexpr int ADDERS = 4 * PARTS, THREADS = 64 + 32 * ADDERS;
+    static constexpr int STAGES = BN >= 64 ? 3 : BN == 32 ? 4 : 5;           // (two blocks an SM)
     static constexpr int RING = STAGES * STAGE;
-    static constexpr int PART = BN * 128 * 4;                // a block's sums, in place of the ring
-    static constexpr int AREA = RING > PART ? RING : PART;
+    static constexpr int SENT = BN * 128 * 4;                // [share][own row][feature]
     static constexpr int FACTORS = 16 * BN * 4;
-    static constexpr int SMEM = AREA + FACTORS + 1024 + 256;
+    static constexpr int SMEM = RING + SENT + FACTORS + 1024 + 256;
 };
 
 template <int BN>
-__global__ void __launch_bounds__(192) fp8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+__global__ void __launch_bounds__(Few<BN>::THREADS, 2) fp8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                                                       const __grid_constant__ Fp8LinearParams p) {
     using C = Few<BN>;
     extern __shared__ uint8_t smem_raw[];
     uint8_t* const smem = reinterpret_cast<uint8_t*>(((uintptr_t)smem_raw + 1023) & ~(uintptr_t)1023);
-    float* const factors = reinterpret_cast<float*>(smem + C::AREA);        // [16 blocks of K][BN]
-    uint64_t* const full = reinterpret_cast<uint64_t*>(smem + C::AREA + C::FACTORS);
+    float* const sent = reinterpret_cast<float*>(smem + C::RING);
+    float* const factors = reinterpret_cast<float*>(smem + C::RING + C::SENT);             // [16 blocks of K][BN]
+    uint64_t* const full = reinterpret_cast<uint64_t*>(smem + C::RING + C::SENT + C::FACTORS);
     uint64_t* const empty = full + C::STAGES;
     uint64_t* const acc_full = empty + C::STAGES;
     uint64_t* const acc_empty = acc_full + C::BUFS;
-    uint32_t* const holder = reinterpret_cast<uint32_t*>(acc_empty + C::BUFS);
+    uint64_t* const all_sent = acc_empty + C::BUFS;          // the other blocks' sums of this block's rows are there
+    uint32_t* const holder = reinterpret_cast<uint32_t*>(all_sent + 1);
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int share = blockIdx.x, shares = gridDim.x, n0 = blockIdx.y * 128, t0 = blockIdx.z * BN;
+    // `per` rows are completed by a block, `mine` of them are there in this one (shares and BN are powers of two)
+    const int rows = min(BN, p.T - t0), per = BN / shares, mine = max(0, min(per, rows - share * per));
     if (warp == 0 && lane == 0) {
         tc::tma_prefetch_desc(&tmW);
         tc::tma_prefetch_desc(&tmX);
         for (int s = 0; s < C::STAGES; ++s) { tc::mbar_init(&full[s], 1); tc::mbar_init(&empty[s], 1); }
-        for (int b = 0; b < C::BUFS; ++b) { tc::mbar_init(&acc_full[b], 1); tc::mbar_init(&acc_empty[b], 4); }
+        for (int b = 0; b < C::BUFS; ++b) { tc::mbar_init(&acc_full[b], 1); tc::mbar_init(&acc_empty[b], C::ADDERS); }
+        tc::mbar_init(all_sent, 1);
+        tc::mbar_expect_tx(all_sent, shares > 1 ? shares * mine * 128 * 4 : 0);
         tc::mbar_fence_init();
     }
     if (warp == 1) {
@@ -73,9 +107,9 @@ __global__ void __launch_bounds__(192) fp8_few_kernel(const __grid_constant__ CU
     __syncthreads();
     tc::fence_after_sync();
     const uint32_t tmem = *holder;
+    cluster_arrive_relaxed();                                // the barriers exist (waited for before the first is used from afar)
     pdl_grid_sync();
 
-    const int share = blockIdx.x, shares = gridDim.x, n0 = blockIdx.y * 128, t0 = blockIdx.z * BN;
     const int blocks = (p.K + BK - 1) / BK;
     const int kb0 = (int)((long long)blocks * share / shares), kb1 = (int)((long long)blocks * (share + 1) / shares);
     if (warp == 0) {
@@ -111,26 +145,27 @@ __global__ void __launch_bounds__(192) fp8_few_kernel(const __grid_constant__ CU
             __syncwarp();
         }
     } else {
-        const int q = warp & 3, tid = threadIdx.x - 64, feature = q * 32 + lane;
+        const int q = warp & 3, tid = threadIdx.x - 64, feature = q * 32 + lane, own = (warp - 2) / 4 * C::OWN;
         const float* const scales = p.scale + (size_t)blockIdx.y * p.lds;
-        float acc[BN];
+        f32x2 acc[C::OWN / 2];
 #pragma unroll
-        for (int j = 0; j < BN; ++j) acc[j] = 0.f;
+        for (int j = 0; j < C::OWN / 2; ++j) acc[j] = pair(0.f, 0.f);
         bool ok = true;
         for (int kb = kb0, it = 0; kb < kb1; ++kb, ++it) {     // (warps whose wait ran out keep meeting the others)
             if (it == 0 || (kb & 15) == 0) {                 // factors of up to sixteen blocks: a thread has a row's
-                asm volatile("bar.sync 1, 128;" ::: "memory");
-                const int first = kb & ~15;
+                asm volatile("bar.sync 1, %0;" ::"n"(32 * C::ADDERS) : "memory");
+                const int from = kb & ~15;
                 if (tid < BN) {
                     uint4 e = make_uint4(0, 0, 0, 0);
-                    if (t0 + tid < p.T) e = __ldg(reinterpret_cast<const uint4*>(p.exps + (size_t)(t0 + tid) * p.lde + first));
+                    if (t0 + tid < p.T) e = __ldg(reinterpret_cast<const uint4*>(p.exps + (size_t)(t0 + tid) * p.lde + from));
                     const uint32_t w[4] = {e.x, e.y, e.z, e.w};
+                    float f[16];
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        if (first + i >= kb && first + i < kb1)
-                            factors[i * BN + tid] = __ldg(scales + first + i) * two_to((w[i / 4] >> (i % 4 * 8)) & 255u);
+                    for (int i = 0; i < 16; ++i) f[i] = from + i >= kb && from + i < kb1 ? __ldg(scales + from + i) : 0.f;
+#pragma unroll
+                    for (int i = 0; i < 16; ++i) factors[i * BN + tid] = f[i] * two_to((w[i / 4] >> (i % 4 * 8)) & 255u);
                 }
-                asm volatile("bar.sync 1, 128;" ::: "memory");
+                asm volatile("bar.sync 1, %0;" ::"n"(32 * C::ADDERS) : "memory");
             }
             const int buf = it % C::BUFS;
             if (ok) {
@@ -138,48 +173,74 @@ __global__ void __launch_bounds__(192) fp8_few_kernel(const __grid_constant__ CU
                 if (!ok && lane == 0) atomicExch(p.err, WAIT_SUMS);
             }
             tc::fence_after_sync();
-            const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + buf * BN;
-            const float4* const f = reinterpret_cast<const float4*>(factors + (kb & 15) * BN);
+            const uint32_t at = tmem + ((uint32_t)(q * 32) << 16) + buf * BN + own;
+            const ulonglong2* const f = reinterpret_cast<const ulonglong2*>(factors + (kb & 15) * BN + own);
 #pragma unroll
-            for (int c = 0; c < BN; c += 16) {
+            for (int c = 0; c < C::OWN; c += 16) {
                 uint32_t r[16];
                 tc::tmem_ld_32x16(at + c, r);
                 tc::tmem_ld_wait();
+                if (c + 16 == C::OWN) {
+                    tc::fence_before_sync();
+                    if (tc::elect_one()) tc::mbar_arrive(&acc_empty[buf]);
+                }
 #pragma unroll
                 for (int j = 0; j < 16; j += 4) {
-                    const float4 g = f[(c + j) / 4];
-                    acc[c + j] = fmaf(__uint_as_float(r[j]), g.x, acc[c + j]);
-                    acc[c + j + 1] = fmaf(__uint_as_float(r[j + 1]), g.y, acc[c + j + 1]);
-                    acc[c + j + 2] = fmaf(__uint_as_float(r[j + 2]), g.z, acc[c + j + 2]);
-                    acc[c + j + 3] = fmaf(__uint_as_float(r[j + 3]), g.w, acc[c + j + 3]);
+                    const ulonglong2 g = f[(c + j) / 4];
+                    acc[(c + j) / 2] = fma2(pair(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), g.x, acc[(c + j) / 2]);
+                    acc[(c + j) / 2 + 1] = fma2(pair(__uint_as_float(r[j + 2]), __uint_as_float(r[j + 3])), g.y, acc[(c + j) / 2 + 1]);
                 }
             }
-            tc::fence_before_sync();
-            __syncwarp();
-            if (lane == 0) tc::mbar_arrive(&acc_empty[buf]);
         }
-        // the ring is free: all products of this block have been waited for.  [row][feature]: lanes side by side
-        float* const part = reinterpret_cast<float*>(smem);
-        if (ok) {
+        if (shares == 1) {
+            const int n = n0 + feature;
+            if (n < p.N) {
 #pragma unroll
-            for (int j = 0; j < BN; ++j) part[j * 128 + feature] = acc[j];
+                for (int j = 0; j < C::OWN; ++j) {
+                    const float2 a = unpair(acc[j / 2]);
+                    const float v = j % 2 ? a.y : a.x;
+                    const size_t at = (size_t)(t0 + own + j) * p.ldy + n;
+                    if (own + j < rows) {
+                        if (p.out_f32) ((float*)p.y)[at] = v;
+                        else ((bf16*)p.y)[at] = __float2bfloat16(v);
+                    }
+                }
+            }
+        } else {
+            // [row][feature] in the ring, which is free (all products of this block have been waited for), then a piece to each block.  (Stores into the
+            // other blocks' memory, 128 bytes a warp, took 2000 cycles for 64 rows where they went to all blocks in turn, 6500 where not.)
+            float* const part = reinterpret_cast<float*>(smem) + own * 128 + feature;
+#pragma unroll
+            for (int j = 0; j < C::OWN / 2; ++j) {
+                const float2 a = unpair(acc[j]);
+                part[2 * j * 128] = a.x;
+                part[(2 * j + 1) * 128] = a.y;
+            }
+            tc::fence_proxy_async_smem();
+            cluster_wait();
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * C::ADDERS) : "memory");
+            if (tid < shares) {
+                const int r = (share + tid) & (shares - 1), n = min(per, rows - r * per);
+                if (n > 0) send(in_block(tc::smem_u32(sent + share * per * 128), r), smem + r * per * 512, n * 512, in_block(tc::smem_u32(all_sent), r));
+            }
         }
     }
     tc::fence_before_sync();
-    __syncthreads();
-    tc::cluster_sync();
-    {
-        const int rows = min(BN, p.T - t0), units = rows * 32;
-        const uint32_t part = tc::smem_u32(smem);
-        for (int u = share * 192 + threadIdx.x; u < units; u += shares * 192) {
-            const int t = u / 32, f = u % 32 * 4;
-            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int r = 0; r < shares; ++r) {
-                const float4 a = ld_cluster(part + (t * 128 + f) * 4, r);
+    __syncwarp();
+    if (shares > 1) {
+        if (warp < 2) cluster_wait();
+        if (mine > 0 && !__all_sync(0xffffffffu, wait_sent(all_sent)) && lane == 0) atomicExch(p.err, WAIT_SENT);
+        __syncwarp();
+        cluster_arrive_relaxed();                            // this block has what was sent to it
+        for (int u = threadIdx.x; u < mine * 32; u += C::THREADS) {
+            const int f = u % 32 * 4, n = n0 + f;
+            const float* const at_sent = sent + u / 32 * 128 + f;
+            float4 v = *reinterpret_cast<const float4*>(at_sent);
+            for (int r = 1; r < shares; ++r) {
+                const float4 a = *reinterpret_cast<const float4*>(at_sent + r * per * 128);
                 v.x += a.x; v.y += a.y; v.z += a.z; v.w += a.w;
             }
-            const int n = n0 + f;
-            const size_t at = (size_t)(t0 + t) * p.ldy + n;
+            const size_t at = (size_t)(t0 + share * per + u / 32) * p.ldy + n;
             if (n + 4 <= p.N) {
                 if (p.out_f32) *reinterpret_cast<float4*>((float*)p.y + at) = v;
                 else *reinterpret_cast<uint2*>((bf16*)p.y + at) = make_uint2(f2_to_bf162(v.x, v.y), f2_to_bf162(v.z, v.w));
@@ -194,7 +255,9 @@ __global__ void __launch_bounds__(192) fp8_few_kernel(const __grid_constant__ CU
             }
         }
     }
-    tc::cluster_sync();                                          // nobody's sums go away while they are read
+    __syncwarp();
+    cluster_wait();                                          // nobody leaves before its sums have arrived
+    __syncthreads();
     if (warp == 1) {
         tc::fence_after_sync();
         tc::tmem_dealloc(tmem, C::COLS);
@@ -211,7 +274,7 @@ int launch_few(const void* x, int ldx, const void* W, int ldw, const Fp8LinearPa
     if (const int rc = optin((const void*)kern, Few<BN>::SMEM)) return rc;
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(shares, (p.N + 127) / 128, (p.T + BN - 1) / BN);
-    cfg.blockDim = 192;
+    cfg.blockDim = Few<BN>::THREADS;
     cfg.dynamicSmemBytes = Few<BN>::SMEM;
     cfg.stream = s;
     cudaLaunchAttribute attr[2];
@@ -225,6 +288,26 @@ int launch_few(const void* x, int ldx, const void* W, int ldw, const Fp8LinearPa
     ++g_sl_kernel_launches;
     const cudaError_t rc = cudaLaunchKernelEx(&cfg, kern, tmW, tmX, p);
     return rc != cudaSuccess ? (int)rc : SL_LAUNCH_CHECK();
+}
+
+// Whether pairs of SMs are the faster form.  Up to 64 rows they never are (64 by 16384 x 2048: 13.5 us without, 14.8 with them).  More: a pair takes 0.47 us for a
+// block of K of its 256 x 256 tile and 3 for what is around it, 74 run at once; 64-row tiles of one SM take 0.42 for a block and SM.  Microseconds without and with
+// pairs: 128 by 6144 x 4096 15.9, 20.8; 256 by 6144 x 4096 22.2, 21.0; 128 by 24576 x 4096 41.1, 37.5; 333 by 2321 x 5136 20.3, 24.4; 512 by 2048 x 2048 11.3,
+// 13.7; 1000 by 2048 x 2048 14.2, 13.8; 1000 by 1024 x 8192 23.2, 33.1.
+bool on_pairs(int T, int N, int K) {
+    if (T <= 64) return false;
+    const long long blocks = (K + BK - 1) / BK, cols = (N + 127) / 128;
+    const long long rounds = ((long long)(T + 255) / 256 * ((N + 255) / 256) + 73) / 74;
+    return 3.f + (float)rounds * (0.47f * (float)blocks + 3.f) <= 5.5f + 0.42f / 148.f * (float)((T + 63) / 64 * cols * blocks);
+}
+
+// Blocks that share a tile's K: twice as many while every block still has an SM to itself, and once more, two blocks an SM, where each has twelve blocks of K left to halve.
+// Microseconds with 4 and 8 shares: 16 by 4096 x 4096 8.0, 8.4 and 256 by 1024 x 2048 7.2, 8.4 (32 tiles), but 29 by 4096 x 12288 15.2, 14.2; 1 by 1024 x 2048
+// (8 tiles) 5.1, 4.6.  With 2 and 4: 32 by 6144 x 4096 11.8, 10.2 (48 tiles).
+int shares_of(long long tiles, int blocks) {
+    int shares = 1;
+    while (shares < 8 && blocks >= 2 * shares && (tiles * shares * 2 <= 148 || (tiles * shares * 2 <= 296 && blocks >= 12 * shares))) shares *= 2;
+    return shares;
 }
 
 bool aligned(const void* x, int ldx, const void* W, int ldw, const Fp8LinearParams& p) {
@@ -241,17 +324,17 @@ SL_API int sl_fp8_linear(const void* x, int ldx, const void* W, int ldw, const F
     const Fp8LinearParams& p = *params;
     if (p.T <= 0 || p.N <= 0) return 0;
     if (!aligned(x, ldx, W, ldw, p) || p.ldy % (p.out_f32 ? 4 : 8) != 0 || (p.N + 127) / 128 > 65535) return -1;
-    if (p.T > 128) return fp8_pair(x, ldx, W, ldw, p, false, s);
-    const int bn = p.T <= 16 ? 16 : p.T <= 32 ? 32 : p.T <= 64 ? 64 : 128;
-    const long long tiles = (long long)((p.N + 127) / 128) * ((p.T + bn - 1) / bn);
-    const int blocks = (p.K + BK - 1) / BK;
-    int shares = 1;
-    while (shares < 8 && tiles * shares * 2 <= 296 && blocks >= shares * 4) shares *= 2;
+    if (on_pairs(p.T, p.N, p.K)) return fp8_pair(x, ldx, W, ldw, p, false, s);
+    const int bn = p.T <= 16 ? 16 : p.T <= 32 ? 32 : 64;
+    if ((p.T + bn - 1) / bn > 65535) return -1;
+    const int shares = shares_of((long long)((p.N + 127) / 128) * ((p.T + bn - 1) / bn), (p.K + BK - 1) / BK);
     if (bn == 16) return launch_few<16>(x, ldx, W, ldw, p, shares, s);
     if (bn == 32) return launch_few<32>(x, ldx, W, ldw, p, shares, s);
-    if (bn == 64) return launch_few<64>(x, ldx, W, ldw, p, shares, s);
-    return launch_few<128>(x, ldx, W, ldw, p, shares, s);
+    return launch_few<64>(x, ldx, W, ldw, p, shares, s);
 }
+
+// 1 where products of this size run on pairs of SMs.
+SL_API int sl_fp8_on_pairs(int T, int N, int K) { return on_pairs(T, N, K); }
 
 // y: codes [T, N / 2] of silu(gate) * up, with exponents exps_out; W: N / 2 gate rows | N / 2 up rows, a multiple of 128 each.
 SL_API int sl_fp8_gate_up(const void* x, int ldx, const void* W, int ldw, const Fp8LinearParams* params, cudaStream_t s) {

@@ -9,6 +9,8 @@
 //
 // Codes are the nearest ones of the definition in 64 bits.  fp32 decides all but the values that lie within its error of the middle between two
 // codes; those are made again in 64 bits.
+#include <algorithm>
+
 #include "fp8_rows.cuh"
 
 namespace {
@@ -40,35 +42,43 @@ __device__ __forceinline__ float to_odd(double d) {
 // `e`: the group's exponent.  `all`: fp32 says nothing.
 template <class Again>
 __device__ __forceinline__ uint32_t quantize_group(float (&v)[4], uint32_t within, bool all, int& e, Again again) {
-    uint32_t top = 0;
+    const float most = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
+    uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(most, 0.f)));          // (fmaxf passes over NaN)
+    if (top == 0x7f800000u) {                                // an infinity: a NaN from here on, and not the largest magnitude
+        top = 0;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) top = max(top, fp8_finite(v[i]) ? __float_as_uint(v[i]) & 0x7fffffffu : 0u);
-    top = __reduce_max_sync(0xffffffffu, top);
+        for (int i = 0; i < 4; ++i) {
+            if (!fp8_finite(v[i])) v[i] = __uint_as_float(0x7fffffffu);
+            else top = max(top, __float_as_uint(v[i]) & 0x7fffffffu);
+        }
+        top = __reduce_max_sync(0xffffffffu, top);
+    }
     e = fp8_exponent(top);
     if (within != 0 && (all || (top & 0x7fffffu) - (0x600000u - within) <= 2 * within)) {
-        double most = 0.0;
+        double largest = 0.0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const double d = fabs(again(i));
-            if (d <= (double)FLT_MAX) most = fmax(most, d);
+            if (d <= (double)FLT_MAX) largest = fmax(largest, d);
         }
 #pragma unroll
-        for (int o = 16; o > 0; o >>= 1) most = fmax(most, __shfl_xor_sync(0xffffffffu, most, o));
-        e = exponent_of(most);
+        for (int o = 16; o > 0; o >>= 1) largest = fmax(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+        e = exponent_of(largest);
     }
     const float down = __uint_as_float((uint32_t)(127 - e) << 23);
     bool near = all;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        v[i] = fp8_finite(v[i]) ? v[i] * down : __uint_as_float(0x7fffffffu);
+        v[i] *= down;
         if (within != 0) near |= near_middle(v[i], within);
     }
     if (within != 0 && near) {
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const double d = again(i);
-            if (all || near_middle(v[i], within)) v[i] = fabs(d) <= (double)FLT_MAX ? to_odd(d * (double)down) : __uint_as_float(0x7fffffffu);
-        }
+        for (int i = 0; i < 4; ++i)
+            if (all || near_middle(v[i], within)) {
+                const double d = again(i);
+                v[i] = fabs(d) <= (double)FLT_MAX ? to_odd(d * (double)down) : __uint_as_float(0x7fffffffu);
+            }
     }
     return fp8_codes(v);
 }
@@ -153,54 +163,78 @@ __global__ void __launch_bounds__(1024) fp8_norm_kernel(const __grid_constant__ 
 
 // ---- rows, gated rows --------------------------------------------------------------------------------------------------------------------
 
-// A warp a group.  What fp32 is off by, in units of 2^-24: down to gates of -16 the exponential's argument is at most 23.1, its rounding 2^-20 and that of
-// log2(e) 3.1e-7, which makes 15; the exponential itself 4, sum, reciprocal and two products 1 each.  Gates below -16 are made in 64 bits.
+// The hardware's exponential of base 2 and reciprocal, each within 2^-22 of the result.
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float rcp(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// A warp has a group of 128 columns and walks over tokens, two at a time.  What fp32 is off by, in units of 2^-24: down to gates of -16 the exponential's
+// argument is at most 23.1, its rounding 2^-20 and that of log2(e) 3.1e-7, which makes 15; the exponential and the reciprocal 4 each, the sum and two products 1
+// each.  Gates below -16 are made in 64 bits.
 template <bool GATED, bool F32>
-__global__ void __launch_bounds__(256) fp8_rows_kernel(const __grid_constant__ Fp8RowsParams p) {
+__global__ void __launch_bounds__(256) fp8_rows_kernel(const __grid_constant__ Fp8RowsParams p, int groups, int abreast) {
     pdl_grid_sync();
-    const int groups = (p.K + 127) / 128, lane = threadIdx.x & 31, n4 = p.K / 4;
-    const long long total = (long long)p.T * groups, step = (long long)gridDim.x * 8;
-    for (long long at = (long long)blockIdx.x * 8 + (threadIdx.x >> 5); at < total; at += step) {
-        const int t = (int)(at / groups), g = (int)(at % groups), i = g * 32 + lane;
-        const char* const x = reinterpret_cast<const char*>(p.x) + (size_t)t * p.ldx * (F32 ? 4 : 2);
-        float v[4] = {0.f, 0.f, 0.f, 0.f}, a[4] = {0.f, 0.f, 0.f, 0.f}, u[4] = {0.f, 0.f, 0.f, 0.f};
+    const int lane = threadIdx.x & 31, n4 = p.K / 4, at = blockIdx.x * 8 + (threadIdx.x >> 5);
+    const int g = at % groups, i = g * 32 + lane;
+    const size_t size = F32 ? 4 : 2;
+    const char* const x = reinterpret_cast<const char*>(p.x);
+    auto load = [&](int t, float (&a)[4], float (&u)[4]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) a[j] = u[j] = 0.f;
+        if (i < n4) {
+            load4<F32>(x + (size_t)t * p.ldx * size, i, a);
+            if (GATED) load4<F32>(x + ((size_t)t * p.ldx + p.K) * size, i, u);
+        }
+    };
+    auto store = [&](int t, float (&a)[4], float (&u)[4]) {
         int e;
         uint32_t c;
         if (GATED) {
-            if (i < n4) {
-                load4<F32>(x, i, a);
-                load4<F32>(x + (size_t)p.K * (F32 ? 4 : 2), i, u);
-            }
             auto again = [&](int j) { return (double)a[j] / (1.0 + exp(-(double)a[j])) * (double)u[j]; };
+            float v[4];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = a[j] * __frcp_rn(1.f + exp2f(-a[j] * LOG2E)) * u[j];
+            for (int j = 0; j < 4; ++j) v[j] = a[j] * rcp(1.f + ex2(a[j] * -LOG2E)) * u[j];
             if (fminf(fminf(a[0], a[1]), fminf(a[2], a[3])) < -16.f) {
 #pragma unroll
                 for (int j = 0; j < 4; ++j)
                     if (a[j] < -16.f) v[j] = (float)again(j);
             }
-            c = quantize_group(v, 24, false, e, again);
+            c = quantize_group(v, 27, false, e, again);
         } else {
-            if (i < n4) load4<F32>(x, i, v);
-            c = quantize_group(v, 0, false, e, [](int) { return 0.0; });
+            c = quantize_group(a, 0, false, e, [](int) { return 0.0; });
         }
         if (i < n4) reinterpret_cast<uint32_t*>(p.codes + (size_t)t * p.ldc)[i] = c;
         if (lane == 0) p.exps[(size_t)t * p.lde + g] = (uint8_t)(e + FP8_BIAS);
+    };
+    for (int t = at / groups; t < p.T && at < groups * abreast; t += 2 * abreast) {
+        float a0[4], u0[4], a1[4], u1[4];
+        load(t, a0, u0);
+        const bool two = t + abreast < p.T;                  // (the same for the whole warp)
+        if (two) load(t + abreast, a1, u1);
+        store(t, a0, u0);
+        if (two) store(t + abreast, a1, u1);
     }
 }
 
 // ---- reading back ------------------------------------------------------------------------------------------------------------------------
 
-// Sixteen codes a thread.  Every value is exact in bf16: four significant bits, exponents from -69 to 68.
-__global__ void __launch_bounds__(256) fp8_values_kernel(const __grid_constant__ Fp8ValuesParams p) {
+// A thread has sixteen columns and walks over tokens.  Every value is exact in bf16: four significant bits, exponents from -69 to 68.
+__global__ void __launch_bounds__(256) fp8_values_kernel(const __grid_constant__ Fp8ValuesParams p, int units, int abreast) {
     pdl_grid_sync();
-    const int units = p.K / 16;
-    const long long total = (long long)p.T * units;
-    for (long long at = (long long)blockIdx.x * 256 + threadIdx.x; at < total; at += (long long)gridDim.x * 256) {
-        const int t = (int)(at / units), i = (int)(at % units);
+    const int at = blockIdx.x * 256 + threadIdx.x, i = at % units;
+    if (at >= units * abreast) return;
+#pragma unroll 2
+    for (int t = at / units; t < p.T; t += abreast) {
         const uint4 c = ldg_nc_16(p.codes + (size_t)t * p.ldc + i * 16);
         // (an exponent that no writer leaves is taken to the nearest one)
-        const int e = max(FP8_LOW, min(FP8_HIGH, (int)p.exps[(size_t)t * p.lde + i / 8] - FP8_BIAS));
+        const int e = max(FP8_LOW, min(FP8_HIGH, (int)__ldg(p.exps + (size_t)t * p.lde + i / 8) - FP8_BIAS));
         const float up = __uint_as_float((uint32_t)(127 + e) << 23);
         const uint32_t w[4] = {c.x, c.y, c.z, c.w};
         uint32_t o[8];
@@ -216,10 +250,8 @@ __global__ void __launch_bounds__(256) fp8_values_kernel(const __grid_constant__
     }
 }
 
-int blocks_for(long long units, int per_block) {
-    const long long want = (units + per_block - 1) / per_block;
-    return (int)(want < 148 * 16 ? want : 148 * 16);
-}
+// How many tokens are worked on at the same time where each is `each` workers: all, as far as the device has room for them.
+int tokens_abreast(int T, int each, int room) { return std::max(1, std::min(T, room / each)); }
 
 template <bool XF32, bool WF32>
 void launch_norm(const Fp8NormParams& p, int T, cudaStream_t s) {
@@ -252,13 +284,14 @@ SL_API int sl_fp8_add_rmsnorm(const Fp8NormParams* p, int T, int x_f32, int w_f3
 SL_API int sl_fp8_rows(const Fp8RowsParams* p, int gated, int f32, cudaStream_t s) {
     if (p->T == 0 || p->K == 0) return 0;
     if (p->T < 0 || p->K < 0 || p->K % 16 != 0) return -1;
-    const dim3 grid(blocks_for((long long)p->T * ((p->K + 127) / 128), 8));
+    const int groups = (p->K + 127) / 128, abreast = tokens_abreast(p->T, groups, 148 * 48);      // (48 warps an SM)
+    const dim3 grid((groups * abreast + 7) / 8);
     if (gated) {
-        if (f32) sl_launch(fp8_rows_kernel<true, true>, grid, 256, 0, s, *p);
-        else sl_launch(fp8_rows_kernel<true, false>, grid, 256, 0, s, *p);
+        if (f32) sl_launch(fp8_rows_kernel<true, true>, grid, 256, 0, s, *p, groups, abreast);
+        else sl_launch(fp8_rows_kernel<true, false>, grid, 256, 0, s, *p, groups, abreast);
     } else {
-        if (f32) sl_launch(fp8_rows_kernel<false, true>, grid, 256, 0, s, *p);
-        else sl_launch(fp8_rows_kernel<false, false>, grid, 256, 0, s, *p);
+        if (f32) sl_launch(fp8_rows_kernel<false, true>, grid, 256, 0, s, *p, groups, abreast);
+        else sl_launch(fp8_rows_kernel<false, false>, grid, 256, 0, s, *p, groups, abreast);
     }
     return SL_LAUNCH_CHECK();
 }
@@ -266,6 +299,7 @@ SL_API int sl_fp8_rows(const Fp8RowsParams* p, int gated, int f32, cudaStream_t 
 SL_API int sl_fp8_values(const Fp8ValuesParams* p, cudaStream_t s) {
     if (p->T == 0 || p->K == 0) return 0;
     if (p->T < 0 || p->K < 0 || p->K % 16 != 0) return -1;
-    sl_launch(fp8_values_kernel, dim3(blocks_for((long long)p->T * (p->K / 16), 256)), 256, 0, s, *p);
+    const int units = p->K / 16, abreast = tokens_abreast(p->T, units, 148 * 2048);
+    sl_launch(fp8_values_kernel, dim3((units * abreast + 255) / 256), 256, 0, s, *p, units, abreast);
     return SL_LAUNCH_CHECK();
 }

@@ -240,6 +240,11 @@ def _multiply(name: str, rows: Fp8Rows, codes: torch.Tensor, scale: torch.Tensor
     _call(device, name, x.data_ptr(), ldx, codes.data_ptr(), codes.stride(0), C.byref(p))
 
 
+@lru_cache(maxsize=4096)
+def _on_pairs(tokens: int, n: int, k: int) -> bool:
+    return bool(N.fn("sl_fp8_on_pairs")(tokens, n, k))
+
+
 def fp8_linear(rows: Fp8Rows, w, out_f32: bool = False) -> torch.Tensor:
     """y = rows @ W^T [T, N], fp32 sums, in bf16 or fp32.  `w`: a :class:`~slopllm_b200.models.weights.LinearWeight` in FP8.  A NaN code spoils its row's (a
     weight's: its column's) results and no other."""
@@ -256,11 +261,11 @@ def fp8_linear(rows: Fp8Rows, w, out_f32: bool = False) -> torch.Tensor:
 
 def fp8_gate_up(rows: Fp8Rows, w) -> Fp8Rows:
     """silu(rows @ Wg^T) * (rows @ Wu^T) in 8 bits, W = gate rows | up rows [2 I, K]: :func:`fp8_silu_mul` of the product's fp32 sums.  Many rows make the
-    activation in the product's epilogue, in fp32: a value next to the middle between two codes may get the other one."""
+    activation in the product's epilogue, in fp32 (`inner` a multiple of 128): a value next to the middle between two codes may get the other one."""
     inner = w.weight.shape[0] // 2
     if w.weight.shape[0] % 32:
         raise ValueError(f"{w.weight.shape[0]} gate and up rows: rows in 8 bits have a multiple of 16 values")
-    if not rows.codes.is_cuda or rows.codes.shape[0] <= 128 or inner % GROUP:
+    if not rows.codes.is_cuda or inner % GROUP or not _on_pairs(rows.codes.shape[0], 2 * inner, rows.codes.shape[1]):
         return fp8_silu_mul(fp8_linear(rows, w, out_f32=True))
     codes, scale = _operands(rows, w)
     out = Fp8Rows.allocate(rows.codes.shape[0], inner, rows.codes.device)

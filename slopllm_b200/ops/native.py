@@ -326,6 +326,7 @@ _SIGS = {
     "sl_fp8_rows": [vp, i32, i32, vp],
     "sl_fp8_values": [vp, vp],
     "sl_fp8_linear": [vp, i32, vp, i32, vp, vp],
+    "sl_fp8_on_pairs": [i32, i32, i32],
     "sl_fp8_gate_up": [vp, i32, vp, i32, vp, vp],
     "sl_fp8_block_dequant_bf16": [vp, vp, vp, i32, i32, i32, vp],
     "sl_moe_unsort_reduce": [vp, vp, vp, vp, i32, i32, i32, i32, i32, vp],
