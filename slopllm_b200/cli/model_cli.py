@@ -31,6 +31,9 @@ def add_model_args(ap: argparse.ArgumentParser) -> None:
     ap.add_argument("--kv-dtype", choices=("auto", "e4m3"), default="auto",
                     help="type of cached keys and values: auto is the model's own; e4m3 keeps them in 8 bits with a scale per token and key head, "
                          "for about half of the cache's bytes (qwen3, qwen3_5; on a GPU heads of 64 or 128 values)")
+    ap.add_argument("--act-dtype", choices=("auto", "e4m3"), default="auto",
+                    help="type of the rows in front of FP8 projections: auto is the model's own; e4m3 keeps an FP8 checkpoint's projections in FP8 and "
+                         "multiplies them with rows in 8 bits, a scale per 128 values (qwen3, qwen3_5)")
     ap.add_argument("--gpus", default="", help="comma-separated device list; its length must equal the number of ranks")
     ap.add_argument("--arena", type=float, default=0.0,
                     help="GiB of device memory this process may allocate per GPU (weights + KV cache + step buffers); a larger "
@@ -132,7 +135,7 @@ def check_memory_plan(args, ctx: ParallelContext, model_dir: str, model_type: st
         with open(os.path.join(model_dir, "config.json")) as f:
             dcfg = DenseConfig.from_hf_dict(json.load(f))
         p = plan_dense(dcfg, world=ctx.world, batch_size=args.batch_size, chunk_size=args.chunk_size, max_pages=args.max_pages,
-                       arena_gb=args.arena, device_gb=total / GIB, kv_dtype=_kv_dtype(args))
+                       arena_gb=args.arena, device_gb=total / GIB, fp8=_act_dtype(args) is not None, kv_dtype=_kv_dtype(args))
     if p.requested_fits:
         return None
     msg = (f"memory plan: {p.weights_bytes / GIB:.1f} GiB of weights per rank + about {p.workspace_bytes / GIB:.1f} GiB of "
@@ -146,6 +149,29 @@ def check_memory_plan(args, ctx: ParallelContext, model_dir: str, model_type: st
 def _kv_dtype(args) -> Optional[str]:
     name = getattr(args, "kv_dtype", "auto")
     return None if name == "auto" else name
+
+
+def _act_dtype(args) -> Optional[str]:
+    name = getattr(args, "act_dtype", "auto")
+    return None if name == "auto" else name
+
+
+def _refuse_act_dtype(args, ctx: ParallelContext, reg, model_type: str, raw: dict, model_dir: str) -> None:
+    """Ends with a line of text where a checkpoint's rows do not go to its projections in the type asked for."""
+    act_dtype = _act_dtype(args)
+    if act_dtype is None:
+        return
+    if not reg.act8:
+        raise SystemExit(f"{args.model}: {model_type} does not take activations in {act_dtype}")
+    from ..checkpoint.safetensors_io import SafetensorsFile
+    from ..models.dense import DenseConfig, check_act_dtype, has_fp8_projections
+    try:
+        check_act_dtype(DenseConfig.from_hf_dict(raw), act_dtype, ctx.world, ctx.device.type == "cuda")
+    except ValueError as e:
+        raise SystemExit(f"{args.model}: {e}")
+    shards = (os.path.join(model_dir, f) for f in sorted(os.listdir(model_dir)) if f.endswith(".safetensors"))
+    if not any(has_fp8_projections(SafetensorsFile(f).names()) for f in shards):
+        raise SystemExit(f"{args.model}: activations in 8 bits go with FP8 projections, and this checkpoint has none")
 
 
 def _refuse_kv_dtype(args, ctx: ParallelContext, reg, model_type: str, raw: dict) -> None:
@@ -162,13 +188,16 @@ def _refuse_kv_dtype(args, ctx: ParallelContext, reg, model_type: str, raw: dict
         raise SystemExit(f"{args.model}: {e}")
 
 
-def _random_model(spec: str, ctx: ParallelContext, mtp: int, dtype_name: Optional[str] = None, kv_dtype: Optional[str] = None):
+def _random_model(spec: str, ctx: ParallelContext, mtp: int, dtype_name: Optional[str] = None, kv_dtype: Optional[str] = None,
+                  act_dtype: Optional[str] = None):
     from ..parallel.fused import make_comm
     dtype = torch.bfloat16 if ctx.device.type == "cuda" else torch.float32
     from ..models.registry import hybrid_family
     family = hybrid_family(spec)
     if kv_dtype is not None and not spec.startswith("qwen"):
         raise SystemExit(f"--random-init {spec} does not cache keys and values in {kv_dtype}")
+    if act_dtype is not None and not spec.startswith("qwen"):
+        raise SystemExit(f"--random-init {spec} does not take activations in {act_dtype}")
     if family is not None:
         cfg = family.config.tiny()
         model = family.model.from_tensors(cfg, family.random_tensors(cfg), ctx, getattr(torch, dtype_name) if dtype_name else dtype)
@@ -180,8 +209,8 @@ def _random_model(spec: str, ctx: ParallelContext, mtp: int, dtype_name: Optiona
     if spec.startswith("qwen"):
         from ..models.dense import DenseConfig, DenseModel, random_dense_model
         cfg = DenseConfig.tiny(hybrid=spec.startswith("qwen35"))
-        w, _ = random_dense_model(cfg, 0, ctx.device, dtype, tp_rank, tp_world)
-        return cfg, DenseModel(cfg, w, ctx, kv_dtype=kv_dtype), cfg.model_type
+        w, _ = random_dense_model(cfg, 0, ctx.device, dtype, tp_rank, tp_world, fp8=act_dtype is not None)
+        return cfg, DenseModel(cfg, w, ctx, kv_dtype=kv_dtype, act_dtype=act_dtype), cfg.model_type
     from ..models.glm_moe_dsa import GlmMoeDsaModel
     from ..models.weights import random_model
     if spec.startswith("glm5"):
@@ -209,7 +238,8 @@ def build_runtime(args, with_scheduler: bool = True) -> Runtime:
         os.environ["SLOPLLM_B200_FUSED"] = "0"
     model_dir: Optional[str] = None
     if args.random_init:
-        cfg, model, model_type = _random_model(args.random_init, ctx, args.mtp, getattr(args, "dtype", None), _kv_dtype(args))
+        cfg, model, model_type = _random_model(args.random_init, ctx, args.mtp, getattr(args, "dtype", None), _kv_dtype(args),
+                                               _act_dtype(args))
     else:
         if not args.model:
             raise SystemExit("give --model DIR|HUB_ID or --random-init SPEC")
@@ -219,8 +249,9 @@ def build_runtime(args, with_scheduler: bool = True) -> Runtime:
             args.max_model_len = max_position_embeddings(model_dir)
         model_type, reg, raw = inspect_model(model_dir, cp=args.cp, mtp=args.mtp)
         _refuse_kv_dtype(args, ctx, reg, model_type, raw)
+        _refuse_act_dtype(args, ctx, reg, model_type, raw, model_dir)
         check_memory_plan(args, ctx, model_dir, model_type)
-        cfg, model = load_registered(reg, model_dir, ctx, args.mtp, getattr(args, "dtype", None), _kv_dtype(args))
+        cfg, model = load_registered(reg, model_dir, ctx, args.mtp, getattr(args, "dtype", None), _kv_dtype(args), _act_dtype(args))
     if getattr(args, "max_model_len", None) is None:
         args.max_model_len = 65536
     if getattr(cfg, "max_positions", 0):

@@ -58,6 +58,7 @@ def main(argv=None) -> int:
     ap.add_argument("--arena", type=float, default=0.0, help="GiB the process may allocate (0: the whole device)")
     ap.add_argument("--device-gb", type=float, default=180.0, help="device memory in GiB when --arena is not given")
     ap.add_argument("--kv-dtype", choices=("auto", "e4m3"), default="auto", help="type of cached keys and values (qwen3, qwen3_5; heads of 64 or 128 values)")
+    ap.add_argument("--act-dtype", choices=("auto", "e4m3"), default="auto", help="e4m3: an FP8 checkpoint's projections stay FP8 (qwen3, qwen3_5)")
     ap.add_argument("--context", type=int, default=0, help="longest sequence assumed for the workspace estimate")
     args = ap.parse_args(argv)
     cfg = _config(args)
@@ -75,8 +76,19 @@ def main(argv=None) -> int:
                 check_kv_dtype(cfg, args.kv_dtype)
             except ValueError as e:
                 raise SystemExit(f"plan: {e}")
+        if args.act_dtype != "auto":
+            if family is not None:
+                raise SystemExit(f"plan: {cfg.model_type} does not take activations in {args.act_dtype}")
+            from ..models.dense import check_act_dtype
+            try:
+                check_act_dtype(cfg, args.act_dtype, args.world)
+            except ValueError as e:
+                raise SystemExit(f"plan: {e}")
+            more["fp8"] = True
         p = planner(cfg, world=args.world, batch_size=args.batch_size, chunk_size=args.chunk_size, max_pages=args.max_pages,
                     arena_gb=args.arena, device_gb=args.device_gb, **more)
+    elif args.act_dtype != "auto":
+        raise SystemExit(f"plan: glm_moe_dsa does not take activations in {args.act_dtype}")
     elif args.kv_dtype != "auto":
         raise SystemExit(f"plan: glm_moe_dsa does not cache keys and values in {args.kv_dtype}")
     else:

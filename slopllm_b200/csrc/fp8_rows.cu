@@ -10,6 +10,7 @@
 // Codes are the nearest ones of the definition in 64 bits.  fp32 decides all but the values that lie within its error of the middle between two
 // codes; those are made again in 64 bits.
 #include <algorithm>
+#include <type_traits>
 
 #include "fp8_rows.cuh"
 
@@ -38,6 +39,13 @@ __device__ __forceinline__ float to_odd(double d) {
     return (double)f == d || !fp8_finite(f) ? f : __uint_as_float(__float_as_uint(f) | 1u);
 }
 
+// Element i of four registers.
+__device__ __forceinline__ float pick(const float (&v)[4], int i) { return i & 2 ? (i & 1 ? v[3] : v[2]) : (i & 1 ? v[1] : v[0]); }
+__device__ __forceinline__ void put(float (&v)[4], int i, float x) {
+#pragma unroll
+    for (int j = 0; j < 4; ++j) v[j] = i == j ? x : v[j];
+}
+
 // A group in a warp, four values a lane, in fp32 off by up to `within` of their last places (0: exact).  `again(i)`: value i in 64 bits.  The lane's codes;
 // `e`: the group's exponent.  `all`: fp32 says nothing.
 template <class Again>
@@ -56,7 +64,7 @@ __device__ __forceinline__ uint32_t quantize_group(float (&v)[4], uint32_t withi
     e = fp8_exponent(top);
     if (within != 0 && (all || (top & 0x7fffffu) - (0x600000u - within) <= 2 * within)) {
         double largest = 0.0;
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < 4; ++i) {
             const double d = fabs(again(i));
             if (d <= (double)FLT_MAX) largest = fmax(largest, d);
@@ -73,11 +81,11 @@ __device__ __forceinline__ uint32_t quantize_group(float (&v)[4], uint32_t withi
         if (within != 0) near |= near_middle(v[i], within);
     }
     if (within != 0 && near) {
-#pragma unroll
+#pragma unroll 1
         for (int i = 0; i < 4; ++i)
-            if (all || near_middle(v[i], within)) {
+            if (all || near_middle(pick(v, i), within)) {
                 const double d = again(i);
-                v[i] = fabs(d) <= (double)FLT_MAX ? to_odd(d * (double)down) : __uint_as_float(0x7fffffffu);
+                put(v, i, fabs(d) <= (double)FLT_MAX ? to_odd(d * (double)down) : __uint_as_float(0x7fffffffu));
             }
     }
     return fp8_codes(v);
@@ -155,7 +163,7 @@ __global__ void __launch_bounds__(1024) fp8_norm_kernel(const __grid_constant__ 
         for (int j = 0; j < 4; ++j) f[j] = v[q][j] * inv32 * w[j];
         int e;
         // three roundings to fp32 (the factor's, two products'): at most 3 last places
-        const uint32_t c = quantize_group(f, 4, all, e, [&](int j) { return (double)v[q][j] * inv * (double)w[j]; });
+        const uint32_t c = quantize_group(f, 4, all, e, [&](int j) { return (double)pick(v[q], j) * inv * (double)pick(w, j); });
         if (i < n4) reinterpret_cast<uint32_t*>(p.codes + (size_t)t * p.ldc)[i] = c;
         if (lane == 0) p.exps[(size_t)t * p.lde + i / 32] = (uint8_t)(e + FP8_BIAS);
     }
@@ -175,78 +183,105 @@ __device__ __forceinline__ float rcp(float x) {
     return y;
 }
 
-// A warp has a group of 128 columns and walks over tokens, two at a time.  What fp32 is off by, in units of 2^-24: down to gates of -16 the exponential's
-// argument is at most 23.1, its rounding 2^-20 and that of log2(e) 3.1e-7, which makes 15; the exponential and the reciprocal 4 each, the sum and two products 1
-// each.  Gates below -16 are made in 64 bits.
+// A warp has a group of 128 columns and walks over tokens, some at a time, so that enough loads are on their way.  What fp32 is off by, in units of 2^-24: down
+// to gates of -16 the exponential's argument is at most 23.1, its rounding 2^-20 and that of log2(e) 3.1e-7, which makes 15; the exponential and the
+// reciprocal 4 each, the sum and two products 1 each.  Gates below -16 are made in 64 bits.
 template <bool GATED, bool F32>
-__global__ void __launch_bounds__(256) fp8_rows_kernel(const __grid_constant__ Fp8RowsParams p, int groups, int abreast) {
+struct RowsCfg {
+    static constexpr int BLOCKS = GATED ? 4 : 6;                             // resident on an SM
+    static constexpr int TOKENS = F32 ? 2 : 4;                               // of a warp at a time
+};
+
+template <bool GATED, bool F32>
+__global__ void __launch_bounds__(256, RowsCfg<GATED, F32>::BLOCKS) fp8_rows_kernel(const __grid_constant__ Fp8RowsParams p, int groups, int abreast) {
     pdl_grid_sync();
+    constexpr int TOKENS = RowsCfg<GATED, F32>::TOKENS;
+    using Raw = std::conditional_t<F32, uint4, uint2>;
     const int lane = threadIdx.x & 31, n4 = p.K / 4, at = blockIdx.x * 8 + (threadIdx.x >> 5);
     const int g = at % groups, i = g * 32 + lane;
-    const size_t size = F32 ? 4 : 2;
-    const char* const x = reinterpret_cast<const char*>(p.x);
-    auto load = [&](int t, float (&a)[4], float (&u)[4]) {
-#pragma unroll
-        for (int j = 0; j < 4; ++j) a[j] = u[j] = 0.f;
-        if (i < n4) {
-            load4<F32>(x + (size_t)t * p.ldx * size, i, a);
-            if (GATED) load4<F32>(x + ((size_t)t * p.ldx + p.K) * size, i, u);
-        }
-    };
-    auto store = [&](int t, float (&a)[4], float (&u)[4]) {
-        int e;
-        uint32_t c;
-        if (GATED) {
-            auto again = [&](int j) { return (double)a[j] / (1.0 + exp(-(double)a[j])) * (double)u[j]; };
-            float v[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) v[j] = a[j] * rcp(1.f + ex2(a[j] * -LOG2E)) * u[j];
-            if (fminf(fminf(a[0], a[1]), fminf(a[2], a[3])) < -16.f) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-                    if (a[j] < -16.f) v[j] = (float)again(j);
-            }
-            c = quantize_group(v, 27, false, e, again);
+    if (at >= groups * abreast) return;
+    const Raw* const x = reinterpret_cast<const Raw*>(p.x) + i;              // (rows start at multiples of four values)
+    auto values = [](const Raw& r, float (&v)[4]) {
+        if constexpr (F32) {
+            v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w);
         } else {
-            c = quantize_group(a, 0, false, e, [](int) { return 0.0; });
+            const float2 lo = bf162_to_f2(r.x), hi = bf162_to_f2(r.y);
+            v[0] = lo.x; v[1] = lo.y; v[2] = hi.x; v[3] = hi.y;
         }
-        if (i < n4) reinterpret_cast<uint32_t*>(p.codes + (size_t)t * p.ldc)[i] = c;
-        if (lane == 0) p.exps[(size_t)t * p.lde + g] = (uint8_t)(e + FP8_BIAS);
     };
-    for (int t = at / groups; t < p.T && at < groups * abreast; t += 2 * abreast) {
-        float a0[4], u0[4], a1[4], u1[4];
-        load(t, a0, u0);
-        const bool two = t + abreast < p.T;                  // (the same for the whole warp)
-        if (two) load(t + abreast, a1, u1);
-        store(t, a0, u0);
-        if (two) store(t + abreast, a1, u1);
+    for (int t0 = at / groups; t0 < p.T; t0 += TOKENS * abreast) {
+        Raw gate[TOKENS], up[TOKENS];
+#pragma unroll
+        for (int b = 0; b < TOKENS; ++b) {
+            gate[b] = up[b] = Raw{};
+            const int t = t0 + b * abreast;
+            if (t < p.T && i < n4) {
+                gate[b] = __ldg(x + (size_t)t * p.ldx / 4);
+                if (GATED) up[b] = __ldg(x + ((size_t)t * p.ldx + p.K) / 4);
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < TOKENS; ++b) {
+            const int t = t0 + b * abreast;
+            if (t >= p.T) break;                             // (the same for the whole warp)
+            float a[4];
+            values(gate[b], a);
+            int e;
+            uint32_t c;
+            if constexpr (GATED) {
+                float u[4], v[4];
+                values(up[b], u);
+                auto again = [&](int j) {
+                    const double z = pick(a, j);
+                    return z / (1.0 + exp(-z)) * (double)pick(u, j);
+                };
+#pragma unroll
+                for (int j = 0; j < 4; ++j) v[j] = a[j] * rcp(1.f + ex2(a[j] * -LOG2E)) * u[j];
+                if (fminf(fminf(a[0], a[1]), fminf(a[2], a[3])) < -16.f) {
+#pragma unroll 1
+                    for (int j = 0; j < 4; ++j)
+                        if (pick(a, j) < -16.f) put(v, j, (float)again(j));
+                }
+                c = quantize_group(v, 27, false, e, again);
+            } else {
+                c = quantize_group(a, 0, false, e, [](int) { return 0.0; });
+            }
+            if (i < n4) reinterpret_cast<uint32_t*>(p.codes + (size_t)t * p.ldc)[i] = c;
+            if (lane == 0) p.exps[(size_t)t * p.lde + g] = (uint8_t)(e + FP8_BIAS);
+        }
     }
 }
 
 // ---- reading back ------------------------------------------------------------------------------------------------------------------------
 
-// A thread has sixteen columns and walks over tokens.  Every value is exact in bf16: four significant bits, exponents from -69 to 68.
+// A thread has eight columns (a warp's stores are whole lines; 4096 x 14336 with sixteen, two stores that fill lines in turn: 40 us) and walks over tokens, four
+// at a time.  Every value is exact in bf16: four significant bits, exponents from -69 to 68.
 __global__ void __launch_bounds__(256) fp8_values_kernel(const __grid_constant__ Fp8ValuesParams p, int units, int abreast) {
     pdl_grid_sync();
     const int at = blockIdx.x * 256 + threadIdx.x, i = at % units;
     if (at >= units * abreast) return;
-#pragma unroll 2
-    for (int t = at / units; t < p.T; t += abreast) {
-        const uint4 c = ldg_nc_16(p.codes + (size_t)t * p.ldc + i * 16);
-        // (an exponent that no writer leaves is taken to the nearest one)
-        const int e = max(FP8_LOW, min(FP8_HIGH, (int)__ldg(p.exps + (size_t)t * p.lde + i / 8) - FP8_BIAS));
-        const float up = __uint_as_float((uint32_t)(127 + e) << 23);
-        const uint32_t w[4] = {c.x, c.y, c.z, c.w};
-        uint32_t o[8];
+    for (int t0 = at / units; t0 < p.T; t0 += 4 * abreast) {
+        uint2 codes[4];
+        int exps[4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const float2 lo = e4m3x2_to_float2((uint16_t)(w[j] & 0xffffu)), hi = e4m3x2_to_float2((uint16_t)(w[j] >> 16));
-            o[2 * j] = f2_to_bf162(lo.x * up, lo.y * up);
-            o[2 * j + 1] = f2_to_bf162(hi.x * up, hi.y * up);
+        for (int b = 0; b < 4; ++b) {
+            const int t = t0 + b * abreast;
+            if (t < p.T) {
+                codes[b] = __ldg(reinterpret_cast<const uint2*>(p.codes + (size_t)t * p.ldc) + i);
+                exps[b] = __ldg(p.exps + (size_t)t * p.lde + i / 16);
+            }
         }
-        uint4* const dst = reinterpret_cast<uint4*>(p.out + (size_t)t * p.K + i * 16);
-        dst[0] = make_uint4(o[0], o[1], o[2], o[3]);
-        dst[1] = make_uint4(o[4], o[5], o[6], o[7]);
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const int t = t0 + b * abreast;
+            if (t >= p.T) break;
+            // (an exponent that no writer leaves is taken to the nearest one)
+            const float up = __uint_as_float((uint32_t)(127 + max(FP8_LOW, min(FP8_HIGH, exps[b] - FP8_BIAS))) << 23);
+            const float2 x0 = e4m3x2_to_float2((uint16_t)(codes[b].x & 0xffffu)), x1 = e4m3x2_to_float2((uint16_t)(codes[b].x >> 16));
+            const float2 x2 = e4m3x2_to_float2((uint16_t)(codes[b].y & 0xffffu)), x3 = e4m3x2_to_float2((uint16_t)(codes[b].y >> 16));
+            reinterpret_cast<uint4*>(p.out + (size_t)t * p.K)[i] = make_uint4(f2_to_bf162(x0.x * up, x0.y * up), f2_to_bf162(x1.x * up, x1.y * up),
+                                                                             f2_to_bf162(x2.x * up, x2.y * up), f2_to_bf162(x3.x * up, x3.y * up));
+        }
     }
 }
 
@@ -284,7 +319,7 @@ SL_API int sl_fp8_add_rmsnorm(const Fp8NormParams* p, int T, int x_f32, int w_f3
 SL_API int sl_fp8_rows(const Fp8RowsParams* p, int gated, int f32, cudaStream_t s) {
     if (p->T == 0 || p->K == 0) return 0;
     if (p->T < 0 || p->K < 0 || p->K % 16 != 0) return -1;
-    const int groups = (p->K + 127) / 128, abreast = tokens_abreast(p->T, groups, 148 * 48);      // (48 warps an SM)
+    const int groups = (p->K + 127) / 128, abreast = tokens_abreast(p->T, groups, 148 * 8 * (gated ? 4 : 6));     // (blocks that are resident)
     const dim3 grid((groups * abreast + 7) / 8);
     if (gated) {
         if (f32) sl_launch(fp8_rows_kernel<true, true>, grid, 256, 0, s, *p, groups, abreast);
@@ -299,7 +334,7 @@ SL_API int sl_fp8_rows(const Fp8RowsParams* p, int gated, int f32, cudaStream_t 
 SL_API int sl_fp8_values(const Fp8ValuesParams* p, cudaStream_t s) {
     if (p->T == 0 || p->K == 0) return 0;
     if (p->T < 0 || p->K < 0 || p->K % 16 != 0) return -1;
-    const int units = p->K / 16, abreast = tokens_abreast(p->T, units, 148 * 2048);
+    const int units = p->K / 8, abreast = tokens_abreast(p->T, units, 148 * 2048);
     sl_launch(fp8_values_kernel, dim3((units * abreast + 255) / 256), 256, 0, s, *p, units, abreast);
     return SL_LAUNCH_CHECK();
 }

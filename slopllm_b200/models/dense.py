@@ -22,7 +22,7 @@ import torch
 from ..config import PAGE_SIZE
 from ..kv.hybrid import CacheSpec, HybridCache
 from ..ops import dense as D
-from ..ops import get_ops, kv8 as K8, recurrent as RC
+from ..ops import fp8 as F8, get_ops, kv8 as K8, recurrent as RC
 from ..ops.rotary import rotary_table
 from ..parallel.dist import Comm, ParallelContext
 from ..utils.tracing import traced
@@ -164,6 +164,28 @@ def check_kv_dtype(cfg: DenseConfig, kv_dtype: Optional[str], on_gpu: bool = Tru
         raise ValueError(f"over the 8-bit cache a GPU serves models with heads of {' or '.join(map(str, K8.PROMPT_HEADS))} values, not {cfg.head_dim}")
 
 
+ACT_DTYPES = ("e4m3",)     # types of the rows in front of FP8 products beside the model's own
+
+
+def check_act_dtype(cfg: DenseConfig, act_dtype: Optional[str], tp: int = 1, on_gpu: bool = True) -> None:
+    """ValueError where a model's rows do not go to its FP8 products in `act_dtype` (None: its own type), before anything is loaded."""
+    if act_dtype is None:
+        return
+    if act_dtype not in ACT_DTYPES:
+        raise ValueError(f"no activations of type {act_dtype}; there are {', '.join(ACT_DTYPES)}")
+    for what, n in (("hidden_size", cfg.hidden_size), ("intermediate_size of a rank", cfg.intermediate_size // tp),
+                    ("attention values of a rank", cfg.num_attention_heads * cfg.head_dim // tp)):
+        if n % 16:
+            raise ValueError(f"activations in 8 bits come in multiples of 16 values: {what} is {n}")
+    if on_gpu and cfg.hidden_size > F8.MAX_NORM:
+        raise ValueError(f"activations in 8 bits come in rows of up to {F8.MAX_NORM} values on a GPU, not {cfg.hidden_size}")
+
+
+def has_fp8_projections(names) -> bool:
+    """Whether a checkpoint's tensor names say that projections are FP8 with a scale per block."""
+    return any(n.endswith("_proj.weight_scale_inv") for n in names)
+
+
 def dense_cache_specs(cfg: DenseConfig, tp: int = 1, kv_dtype: Optional[str] = None) -> List[CacheSpec]:
     """Paged K/V rows per full-attention layer; conv + recurrent state per linear-attention layer.  `kv_dtype` "e4m3": the rows are
     codes, with two exponent bytes per token and key head (`ops/kv8.py`; a page's bytes are laid out by head)."""
@@ -191,27 +213,36 @@ class DenseCache(HybridCache):
 
 
 class DenseModel(DecoderStack):
-    """Forward pass of the Qwen3 / Qwen3.5 decoders over the paged cache.  `kv_dtype` "e4m3": keys and values are cached in 8 bits."""
+    """Forward pass of the Qwen3 / Qwen3.5 decoders over the paged cache.  `kv_dtype` "e4m3": keys and values are cached in 8 bits.  `act_dtype`
+    "e4m3": rows go to the projections that are FP8 in 8 bits (`ops/fp8.py`)."""
 
     norm_ahead = True
 
     def __init__(self, cfg: DenseConfig, weights: DenseWeights, ctx: Optional[ParallelContext] = None, ops=None,
-                 comm: Optional[Comm] = None, kv_dtype: Optional[str] = None):
-        self.cfg, self.w, self.kv_dtype = cfg, weights, kv_dtype
+                 comm: Optional[Comm] = None, kv_dtype: Optional[str] = None, act_dtype: Optional[str] = None):
+        self.cfg, self.w, self.kv_dtype, self.act_dtype = cfg, weights, kv_dtype, act_dtype
         ctx = ctx or ParallelContext()
         check_kv_dtype(cfg, kv_dtype, ctx.device.type == "cuda")
+        check_act_dtype(cfg, act_dtype, ctx.world, ctx.device.type == "cuda")
         self.specs = dense_cache_specs(cfg, ctx.world, kv_dtype)
         self.rot = None if kv_dtype is None else rotary_table(cfg.rope_dim, cfg.rope_theta).to(ctx.device)
         self.sublayers = []
         for i, lw in enumerate(weights.layers):
-            mixer = self._full_attention if lw.kind == "full_attention" else self._linear_attention
-            self.sublayers.append(Sublayer(functools.partial(mixer, i, lw), lw.input_norm))
-            self.sublayers.append(Sublayer(functools.partial(self._mlp, lw), lw.post_attn_norm))
+            full = lw.kind == "full_attention"
+            mixer = self._full_attention if full else self._linear_attention
+            self.sublayers.append(Sublayer(functools.partial(mixer, i, lw), lw.input_norm, fp8_input=full and self._in_fp8(lw.w_qkv)))
+            self.sublayers.append(Sublayer(functools.partial(self._mlp, lw), lw.post_attn_norm, fp8_input=self._in_fp8(lw.mlp_w13)))
+        if act_dtype is not None and not any(s.fp8_input for s in self.sublayers):
+            raise ValueError("activations in 8 bits go with FP8 projections, and these weights have none")
         self._init_stack(ctx, ops or get_ops(cfg, ctx.device, ctx), comm,
                          torch.bfloat16 if ctx.device.type == "cuda" else torch.float32)
 
     def _make_cache(self, num_pages: int, max_states: int) -> DenseCache:
         return DenseCache(self.cfg, num_pages, self.ctx.device, self.ctx.world, max_states, dtype=self.cache_dtype, kv_dtype=self.kv_dtype)
+
+    def _in_fp8(self, w: Optional[LinearWeight]) -> bool:
+        """Whether a projection's rows come in 8 bits."""
+        return self.act_dtype is not None and w.is_fp8
 
     # ---- layers -------------------------------------------------------------------------------------------
     @traced(lambda self, i, *a, **k: f"layer{i}.attention")
@@ -237,7 +268,8 @@ class DenseModel(DecoderStack):
                                   cfg.scaling, qo_indptr=qo, max_q=max_q, max_kv_len=st.max_kv_len)
         if cfg.attn_output_gate:
             o = D.gate_heads(o, q, qs)
-        return ops.linear(o.reshape(T, hl * cfg.head_dim), lw.o_proj, out_f32=True)
+        o = o.reshape(T, hl * cfg.head_dim)
+        return ops.linear(F8.fp8_rows(o) if self._in_fp8(lw.o_proj) else o, lw.o_proj, out_f32=True)
 
     @traced(lambda self, i, *a, **k: f"layer{i}.linear_attention")
     def _linear_attention(self, i: int, lw: DenseLayer, x, st, cache: DenseCache):
@@ -269,9 +301,10 @@ def _lin(t: torch.Tensor) -> LinearWeight:
 
 
 def random_dense_model(cfg: DenseConfig, seed: int = 0, device="cpu", dtype=torch.bfloat16, rank: int = 0, world: int = 1,
-                       draw_device="cpu") -> DenseWeights:
+                       draw_device="cpu", fp8: bool = False) -> DenseWeights:
     """Random weights with the checkpoint's shapes, sharded for `rank` of `world`: the full
-    matrices are drawn from the seed on every rank and sliced, so shards agree.  `draw_device`: where they are drawn."""
+    matrices are drawn from the seed on every rank and sliced, so shards agree.  `draw_device`: where they are drawn.  `fp8`: the projections of
+    attention and MLP are those of an FP8 checkpoint, and stay FP8."""
     g = torch.Generator(device=draw_device).manual_seed(seed)
     H, I, hd = cfg.hidden_size, cfg.intermediate_size, cfg.head_dim
     tensors: Dict[str, torch.Tensor] = {}
@@ -315,7 +348,10 @@ def random_dense_model(cfg: DenseConfig, seed: int = 0, device="cpu", dtype=torc
     tensors[pfx + "norm.weight"] = norm_w(H)
     if not cfg.tie_word_embeddings:
         tensors["lm_head.weight"] = rnd(cfg.vocab_size, H)
-    return assemble_dense_weights(cfg, tensors, device, dtype, rank, world), tensors
+    if fp8:
+        for name in [n for n in tensors if n.endswith("_proj.weight") and "linear_attn" not in n]:
+            tensors[name], tensors[name + "_scale_inv"] = D.fp8_block_quantize(tensors[name])
+    return assemble_dense_weights(cfg, tensors, device, dtype, rank, world, keep_fp8=True if fp8 else None), tensors
 
 
 def _fp8_rows(w: LinearWeight, lo: int, hi: int) -> LinearWeight:
@@ -428,13 +464,16 @@ def assemble_dense_weights(cfg: DenseConfig, tensors: Dict[str, torch.Tensor], d
                         vocab_offset=rank * vloc)
 
 
-def load_dense_model(model_dir: str, ctx: Optional[ParallelContext] = None, dtype=torch.bfloat16, kv_dtype: Optional[str] = None):
-    """(cfg, DenseModel) from a HF directory of safetensors shards (text decoder only: `model.visual.*` is skipped)."""
+def load_dense_model(model_dir: str, ctx: Optional[ParallelContext] = None, dtype=torch.bfloat16, kv_dtype: Optional[str] = None,
+                     act_dtype: Optional[str] = None):
+    """(cfg, DenseModel) from a HF directory of safetensors shards (text decoder only: `model.visual.*` is skipped).  `act_dtype` keeps FP8
+    projections in FP8."""
     from ..checkpoint.safetensors_io import SafetensorsFile
     ctx = ctx or ParallelContext()
     with open(os.path.join(model_dir, "config.json")) as f:
         cfg = DenseConfig.from_hf_dict(json.load(f))
     check_kv_dtype(cfg, kv_dtype, ctx.device.type == "cuda")
+    check_act_dtype(cfg, act_dtype, ctx.world, ctx.device.type == "cuda")
     tensors: Dict[str, torch.Tensor] = {}
     for fn in sorted(os.listdir(model_dir)):
         if fn.endswith(".safetensors"):
@@ -442,5 +481,7 @@ def load_dense_model(model_dir: str, ctx: Optional[ParallelContext] = None, dtyp
             for name in sf.names():
                 if not name.startswith("model.visual."):
                     tensors[name] = sf.tensor(name)
-    w = assemble_dense_weights(cfg, tensors, ctx.device, dtype, ctx.rank if ctx.world > 1 else 0, ctx.world)
-    return cfg, DenseModel(cfg, w, ctx, kv_dtype=kv_dtype)
+    if act_dtype is not None and not has_fp8_projections(tensors):
+        raise ValueError(f"{model_dir}: activations in 8 bits go with FP8 projections, and this checkpoint has none")
+    w = assemble_dense_weights(cfg, tensors, ctx.device, dtype, ctx.rank if ctx.world > 1 else 0, ctx.world, keep_fp8=None if act_dtype is None else True)
+    return cfg, DenseModel(cfg, w, ctx, kv_dtype=kv_dtype, act_dtype=act_dtype)

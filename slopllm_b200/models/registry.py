@@ -17,9 +17,10 @@ class ModelRegistration:
     context_parallel: bool
     mtp: bool
     persistent_loader: bool
-    load: Callable            # (model_dir, ctx, mtp[, dtype][, kv_dtype]) -> (cfg, model)
+    load: Callable            # (model_dir, ctx, mtp[, dtype][, kv_dtype][, act_dtype]) -> (cfg, model)
     float32: bool = False     # also runs entirely in fp32 on a GPU (`load` then takes `dtype`)
     kv8: bool = False         # can keep keys and values in 8 bits (`load` then takes `kv_dtype`)
+    act8: bool = False        # can take rows to FP8 projections in 8 bits (`load` then takes `act_dtype`)
     kernel_sources: Optional[Tuple[str, ...]] = None     # csrc/*.cu that serve the family (None: the complete library)
 
 
@@ -33,9 +34,9 @@ def _load_glm_moe_dsa(model_dir: str, ctx: ParallelContext, mtp: int = 0):
     return cfg, GlmMoeDsaModel(cfg, w, ctx, comm=make_comm(ctx, cfg))
 
 
-def _load_dense(model_dir: str, ctx: ParallelContext, mtp: int = 0, kv_dtype: Optional[str] = None):
+def _load_dense(model_dir: str, ctx: ParallelContext, mtp: int = 0, kv_dtype: Optional[str] = None, act_dtype: Optional[str] = None):
     from .dense import load_dense_model
-    return load_dense_model(model_dir, ctx, kv_dtype=kv_dtype)
+    return load_dense_model(model_dir, ctx, kv_dtype=kv_dtype, act_dtype=act_dtype)
 
 
 def _load_glm5_next(model_dir: str, ctx: ParallelContext, mtp: int = 0):
@@ -75,8 +76,8 @@ def _load_pulunex(model_dir: str, ctx: ParallelContext, mtp: int = 0, dtype=None
 MODEL_REGISTRY: Dict[str, ModelRegistration] = {
     "glm_moe_dsa": ModelRegistration(True, True, True, True, _load_glm_moe_dsa),
     "glm5_next": ModelRegistration(False, False, False, True, _load_glm5_next),
-    "qwen3": ModelRegistration(False, False, False, True, _load_dense, kv8=True),
-    "qwen3_5": ModelRegistration(False, False, False, False, _load_dense, kv8=True),
+    "qwen3": ModelRegistration(False, False, False, True, _load_dense, kv8=True, act8=True),
+    "qwen3_5": ModelRegistration(False, False, False, False, _load_dense, kv8=True, act8=True),
     "gidisun": ModelRegistration(False, False, False, False, _load_gidisun, float32=True,
                                  kernel_sources=("elementwise", "gated_chunk", "gated_scan", "gemm_pair_tcgen05", "gemm_tcgen05", "gemv", "latent_attn", "latent_mma", "linear_simt",
                                                  "sampling", "sandwich_norm", "sparse_mla")),
@@ -142,11 +143,15 @@ def inspect_model(model_dir: str, cp: bool = False, mtp: int = 0):
 
 
 def load_registered(reg: ModelRegistration, model_dir: str, ctx: ParallelContext, mtp: int = 0, dtype: Optional[str] = None,
-                    kv_dtype: Optional[str] = None):
-    """`dtype`: "bfloat16" / "float32" (None: bfloat16 on a GPU, float32 on the CPU).  `kv_dtype`: "e4m3", or None for the model's own."""
+                    kv_dtype: Optional[str] = None, act_dtype: Optional[str] = None):
+    """`dtype`: "bfloat16" / "float32" (None: bfloat16 on a GPU, float32 on the CPU).  `kv_dtype`, `act_dtype`: "e4m3", or None for the model's own."""
     if kv_dtype is not None and not reg.kv8:
         raise ValueError(f"{model_dir}: this model family does not cache keys and values in {kv_dtype}")
+    if act_dtype is not None and not reg.act8:
+        raise ValueError(f"{model_dir}: this model family does not take activations in {act_dtype}")
     more = {} if kv_dtype is None else {"kv_dtype": kv_dtype}
+    if act_dtype is not None:
+        more["act_dtype"] = act_dtype
     if dtype is None or (dtype == "bfloat16") == (ctx.device.type == "cuda"):
         return reg.load(model_dir, ctx, mtp, **more)
     if not reg.float32:
@@ -154,7 +159,8 @@ def load_registered(reg: ModelRegistration, model_dir: str, ctx: ParallelContext
     return reg.load(model_dir, ctx, mtp, dtype=getattr(torch, dtype), **more)
 
 
-def load_any(model_dir: str, ctx: Optional[ParallelContext] = None, mtp: int = 0, dtype: Optional[str] = None, kv_dtype: Optional[str] = None):
+def load_any(model_dir: str, ctx: Optional[ParallelContext] = None, mtp: int = 0, dtype: Optional[str] = None, kv_dtype: Optional[str] = None,
+             act_dtype: Optional[str] = None):
     ctx = ctx or ParallelContext()
     _, reg, _ = inspect_model(model_dir, cp=ctx.cp, mtp=mtp)
-    return load_registered(reg, model_dir, ctx, mtp, dtype, kv_dtype)
+    return load_registered(reg, model_dir, ctx, mtp, dtype, kv_dtype, act_dtype)

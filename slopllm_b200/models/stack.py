@@ -14,7 +14,7 @@ from typing import Callable, List, Optional
 import torch
 
 from ..kv.hybrid import CacheSpec, HybridCache, StateSlots
-from ..ops import shift as SH
+from ..ops import fp8 as F8, shift as SH
 from ..parallel.dist import Comm, ParallelContext
 from ..utils.upload import upload
 
@@ -36,6 +36,7 @@ class Sublayer:
     alpha: Optional[float] = None              # factor on the residual of a sublayer whose sum is normalised
     bias: Optional[torch.Tensor] = None        # fp32 [H], added to the complete output (sums that are normalised)
     shift: Optional[TokenShift] = None         # mixes the normed input with the previous token's
+    fp8_input: bool = False                    # `run` takes its normed input as rows in 8 bits (`ops/fp8.py`)
 
 
 def token_ranges(st):
@@ -108,6 +109,8 @@ class DecoderStack:
             return ops.embed_rows(st.input_ids, self.w.embed)
         if self.fp32_norms or self.sublayers[0].post_norm is not None:
             return ops.embed_norm(st.input_ids, self.w.embed, norm, eps)
+        if sub.fp8_input:
+            return F8.fp8_add_rmsnorm(ops.embed(st.input_ids, self.w.embed), None, norm, eps)
         return ops.add_rmsnorm(ops.embed(st.input_ids, self.w.embed), None, norm, eps)
 
     def _join(self, y, residual, sub: Sublayer, nxt: Optional[Sublayer], st, cache):
@@ -120,6 +123,8 @@ class DecoderStack:
             return ops.sum_norm(self.comm.all_reduce(y), residual, sub.alpha, sub.bias, sub.post_norm, norm, eps)
         if self.fp32_norms or sub.post_norm is not None:
             return ops.post_norm(self.comm.all_reduce(y), residual, sub.post_norm, norm, eps)
+        if nxt is not None and nxt.fp8_input:
+            return F8.fp8_add_rmsnorm(y if self.ctx.world == 1 else self.comm._reduce_partial(y), residual, norm, eps)
         if nxt is not None and self.norm_ahead and self.ctx.world == 1 and hasattr(ops, "add_rmsnorm_ahead"):
             return ops.add_rmsnorm_ahead(y, residual, norm, eps)
         return self.comm.allreduce_add_rmsnorm(ops, y, residual, norm, eps)

@@ -16,7 +16,7 @@ from typing import Optional
 
 import torch
 
-from . import quant, reference as R
+from . import fp8 as F8, quant, reference as R
 
 
 class RefOps:
@@ -60,6 +60,8 @@ class RefOps:
         return (r if w_next is None else R.rmsnorm(r, w_next, eps)), r
 
     def linear(self, x, w, out_f32: bool = False, sink=None, defer_reduce: bool = False):
+        if isinstance(x, F8.Fp8Rows):
+            return F8.fp8_linear(x, w, out_f32=True)
         return R.linear(x, w)
 
     def merge_attention_partials(self, o, lse):
@@ -129,6 +131,10 @@ class RefOps:
 
     # -- MLP ------------------------------------------------------------------------------------
     def dense_mlp(self, x, lw, sink=None):
+        if isinstance(x, F8.Fp8Rows):
+            if lw.mlp_w2.is_fp8:
+                return self.linear(F8.fp8_gate_up(x, lw.mlp_w13), lw.mlp_w2)
+            return R.linear(R.silu_mul(self.linear(x, lw.mlp_w13)), lw.mlp_w2)
         return R.linear(R.silu_mul(R.linear(x, lw.mlp_w13)), lw.mlp_w2)
 
     def gated_act(self, gate_up, out, act: str = "silu", bias=None, row_gate=None):

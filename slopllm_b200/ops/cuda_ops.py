@@ -12,6 +12,7 @@ from typing import Optional
 
 import torch
 
+from . import fp8 as F8
 from . import native as N
 from . import reference as R
 
@@ -222,7 +223,11 @@ class CudaOps:
         """y = x @ W^T.  With `sink` (a receive buffer on every rank) the fp32 result rows are
         stored straight into the peers' memory by the producing kernel and the sink is returned.
         With `defer_reduce` a split-K product may come back as `SplitKSlabs` (fp32 partial sums the
-        consumer adds up while it loads them); only `attn_pre` and `q_post` accept that form."""
+        consumer adds up while it loads them); only `attn_pre` and `q_post` accept that form.  Rows in 8 bits
+        (`ops/fp8.py`) are multiplied with FP8 weights as they are."""
+        if isinstance(x, F8.Fp8Rows):
+            y = F8.fp8_linear(x, w, out_f32 or sink is not None)
+            return y if sink is None else sink.push_tensor(y)
         if isinstance(x, PendingNorm):
             y = x.product(w, out_f32, False) if sink is None and x.keeps_order(w) else None
             if y is not None:
@@ -633,12 +638,14 @@ class CudaOps:
         return act
 
     def dense_mlp(self, x, lw, sink=None):
+        if isinstance(x, F8.Fp8Rows) and lw.mlp_w2.is_fp8:
+            return self.linear(F8.fp8_gate_up(x, lw.mlp_w13), lw.mlp_w2, out_f32=True, sink=sink)
         if isinstance(x, PendingNorm):
             act = x.product(lw.mlp_w13, False, True) if x.keeps_order(lw.mlp_w13) else None
             if act is not None:
                 return self.linear(act, lw.mlp_w2, out_f32=True, sink=sink)
             x = x.rows()
-        act = self._gate_up_act(x, lw.mlp_w13)
+        act = None if isinstance(x, F8.Fp8Rows) else self._gate_up_act(x, lw.mlp_w13)
         if act is not None:
             return self.linear(act, lw.mlp_w2, out_f32=True, sink=sink)
         gu = self.linear(x, lw.mlp_w13)

@@ -13,7 +13,6 @@ CUDA tensors run `csrc/fp8_rows.cu` and `csrc/fp8_gemm_tcgen05.cu`; CPU tensors 
 from __future__ import annotations
 
 import ctypes as C
-from dataclasses import dataclass
 from functools import lru_cache
 from typing import Optional, Tuple
 
@@ -50,44 +49,66 @@ def _padded(k: int) -> int:
     return (k + 16 * GROUP - 1) // (16 * GROUP) * 16
 
 
-@dataclass
 class Fp8Rows:
     """`codes`: uint8 [T, K], e4m3; `exps`: uint8 [T, ceil(K / 128)], rows a multiple of 16 bytes apart (the bytes up to it may be read)."""
 
-    codes: torch.Tensor
-    exps: torch.Tensor
+    __slots__ = ("shape", "_space", "_codes", "_exps")         # (rows that were allocated here are one piece of memory, with views where asked for)
 
-    def __post_init__(self):
-        codes, exps = self.codes, self.exps
+    def __init__(self, codes: torch.Tensor, exps: torch.Tensor):
         if codes.dim() != 2 or exps.shape != (codes.shape[0], -(-codes.shape[1] // GROUP)):
             raise ValueError(f"codes {tuple(codes.shape)} do not go with exponents {tuple(exps.shape)}")
         (T, K), (ldc, by), (lde, by_e) = codes.shape, codes.stride(), exps.stride()
-        if codes.dtype is not torch.uint8 or exps.dtype is not torch.uint8 or codes.device != exps.device:
+        device = codes.get_device()
+        if codes.dtype is not torch.uint8 or exps.dtype is not torch.uint8 or device != exps.get_device():
             raise ValueError("rows in 8 bits are two tensors of type uint8 on one device")
         if K % 16 or K == 0:
             raise ValueError(f"rows of {K} values: rows in 8 bits have a multiple of 16")
         if T > 1 and (ldc % 16 or lde % 16 or ldc < K or lde < _padded(K)) or by != 1 or (by_e != 1 and exps.shape[1] > 1):
             raise ValueError("rows of codes and of exponents start at multiples of 16 bytes, with bytes side by side")
-        if T and codes.is_cuda and ((codes.data_ptr() | exps.data_ptr()) % 16
-                                    or exps.storage_offset() + (T - 1) * lde + _padded(K) > exps.untyped_storage().nbytes()):
+        if T and device >= 0 and ((codes.data_ptr() | exps.data_ptr()) % 16
+                                  or exps.storage_offset() + (T - 1) * lde + _padded(K) > exps.untyped_storage().nbytes()):
             raise ValueError("rows of codes and of exponents start at multiples of 16 bytes and are readable in pieces of 16")
-
-    @property
-    def shape(self) -> torch.Size:
-        return self.codes.shape
-
-    @property
-    def device(self) -> torch.device:
-        return self.codes.device
+        self.shape, self._space, self._codes, self._exps = (T, K), None, codes, exps
 
     @staticmethod
     def allocate(tokens: int, values: int, device) -> "Fp8Rows":
         if values % 16 or values <= 0:
             raise ValueError(f"rows of {values} values: rows in 8 bits have a multiple of 16")
         rows = object.__new__(Fp8Rows)
-        rows.codes = torch.empty(tokens, values, dtype=torch.uint8, device=device)
-        rows.exps = torch.empty(tokens, _padded(values), dtype=torch.uint8, device=device)[:, :-(-values // GROUP)]
+        rows.shape, rows._codes, rows._exps = (tokens, values), None, None
+        rows._space = torch.empty(tokens * (values + _padded(values)), dtype=torch.uint8, device=device)
         return rows
+
+    @property
+    def codes(self) -> torch.Tensor:
+        if self._codes is None:
+            T, K = self.shape
+            self._codes = self._space[:T * K].view(T, K)
+        return self._codes
+
+    @property
+    def exps(self) -> torch.Tensor:
+        if self._exps is None:
+            T, K = self.shape
+            self._exps = self._space[T * K:].view(T, _padded(K))[:, :-(-K // GROUP)]
+        return self._exps
+
+    @property
+    def _memory(self) -> torch.Tensor:
+        return self._codes if self._space is None else self._space
+
+    @property
+    def device(self) -> torch.device:
+        return self._memory.device
+
+    def _where(self) -> tuple:
+        """Addresses and row strides of codes and exponents (one row: those of an allocated one)."""
+        T, K = self.shape
+        if self._space is not None:
+            at = self._space.data_ptr()
+            return at, K, at + T * K, _padded(K)
+        codes, exps = self._codes, self._exps
+        return (codes.data_ptr(), codes.stride(0), exps.data_ptr(), exps.stride(0)) if T > 1 else (codes.data_ptr(), K, exps.data_ptr(), _padded(K))
 
 
 def _call(device: int, name: str, *args) -> None:
@@ -107,17 +128,21 @@ def _status(device: int) -> int:
 
 def _aligned(x: torch.Tensor) -> torch.Tensor:
     """Rows that loads of four values take: a copy where they do not start at multiples of that."""
-    size = 4 * x.element_size()
-    if x.stride(1) == 1 and x.data_ptr() % size == 0 and (x.stride(0) % 4 == 0 or x.shape[0] <= 1):
+    ld, by = x.stride()
+    if by == 1 and (ld % 4 == 0 or x.shape[0] <= 1) and x.data_ptr() % (16 if x.dtype is torch.float32 else 8) == 0:
         return x
     return x.clone(memory_format=torch.contiguous_format)
 
 
-def _check_rows(x: torch.Tensor, what: str) -> None:
+def _check_rows(x: torch.Tensor, what: str) -> tuple:
+    """(tokens, values, device number) of rows that the operators take."""
     if x.dim() != 2:
         raise ValueError(f"{what} of shape {tuple(x.shape)}: rows are [tokens, values]")
-    if x.is_cuda and x.dtype not in (torch.bfloat16, torch.float32):
-        raise ValueError(f"{what} of type {x.dtype}: the kernels take bf16 and fp32")
+    device, kind = x.get_device(), x.dtype
+    if device >= 0 and kind is not torch.bfloat16 and kind is not torch.float32:
+        raise ValueError(f"{what} of type {kind}: the kernels take bf16 and fp32")
+    T, K = x.shape
+    return T, K, device
 
 
 # ---- the format ----------------------------------------------------------------------------------------------------------------------
@@ -140,44 +165,45 @@ def _quantize(v: torch.Tensor) -> Fp8Rows:
 
 def _values(rows: Fp8Rows) -> torch.Tensor:
     """The fp32 values of rows (the definition)."""
-    e = (rows.exps.to(torch.int32) - BIAS).clamp(LOW, HIGH).repeat_interleave(GROUP, 1)[:, :rows.codes.shape[1]]
+    e = (rows.exps.to(torch.int32) - BIAS).clamp(LOW, HIGH).repeat_interleave(GROUP, 1)[:, :rows.shape[1]]
     return torch.ldexp(rows.codes.view(torch.float8_e4m3fn).to(torch.float32), e)
 
 
 def fp8_values(rows: Fp8Rows) -> torch.Tensor:
     """The values [T, K] of rows in 8 bits, in bf16, which holds them exactly."""
-    (T, K), device = rows.codes.shape, rows.codes.get_device()
+    (T, K), memory = rows.shape, rows._memory
+    device = memory.get_device()
     if device < 0:
         return _values(rows).to(torch.bfloat16)
-    out = torch.empty(T, K, dtype=torch.bfloat16, device=rows.codes.device)
-    p = Fp8ValuesParams(rows.codes.data_ptr(), rows.codes.stride(0), rows.exps.data_ptr(), rows.exps.stride(0), T, K, out.data_ptr())
+    out = memory.new_empty((T, K), dtype=torch.bfloat16)
+    p = Fp8ValuesParams(*rows._where(), T, K, out.data_ptr())
     _call(device, "sl_fp8_values", C.byref(p))
     return out
 
 
 # ---- making rows -----------------------------------------------------------------------------------------------------------------------
 
-def _make(x: torch.Tensor, values: int, gated: bool) -> Fp8Rows:
+def _make(x: torch.Tensor, tokens: int, values: int, device: int, gated: bool) -> Fp8Rows:
     x = _aligned(x)
-    out = Fp8Rows.allocate(x.shape[0], values, x.device)
-    p = Fp8RowsParams(x.data_ptr(), x.stride(0), x.shape[0], values, out.codes.data_ptr(), out.codes.stride(0), out.exps.data_ptr(), out.exps.stride(0))
-    _call(x.get_device(), "sl_fp8_rows", C.byref(p), int(gated), int(x.dtype is torch.float32))
+    out = Fp8Rows.allocate(tokens, values, x.device)
+    p = Fp8RowsParams(x.data_ptr(), x.stride(0), tokens, values, *out._where())
+    _call(device, "sl_fp8_rows", C.byref(p), gated, x.dtype is torch.float32)
     return out
 
 
 def fp8_rows(x: torch.Tensor) -> Fp8Rows:
     """Rows [T, K], bf16 or fp32, of any stride, in 8 bits."""
-    _check_rows(x, "rows")
-    return _make(x, x.shape[1], False) if x.is_cuda else _quantize(x.to(torch.float64))
+    T, K, device = _check_rows(x, "rows")
+    return _make(x, T, K, device, False) if device >= 0 else _quantize(x.to(torch.float64))
 
 
 def fp8_silu_mul(gate_up: torch.Tensor) -> Fp8Rows:
     """silu(gate) * up of rows gate | up [T, 2 K], bf16 or fp32, of any stride, in 8 bits: nothing is rounded in between."""
-    _check_rows(gate_up, "gate and up rows")
-    if gate_up.shape[1] % 2:
-        raise ValueError(f"gate and up rows of {gate_up.shape[1]} values together")
-    if gate_up.is_cuda:
-        return _make(gate_up, gate_up.shape[1] // 2, True)
+    T, K, device = _check_rows(gate_up, "gate and up rows")
+    if K % 2:
+        raise ValueError(f"gate and up rows of {K} values together")
+    if device >= 0:
+        return _make(gate_up, T, K // 2, device, True)
     g, u = gate_up.to(torch.float64).chunk(2, -1)
     return _quantize(g / (1.0 + torch.exp(-g)) * u)
 
@@ -185,9 +211,8 @@ def fp8_silu_mul(gate_up: torch.Tensor) -> Fp8Rows:
 def fp8_add_rmsnorm(x: torch.Tensor, residual: Optional[torch.Tensor], w: torch.Tensor, eps: float) -> Tuple[Fp8Rows, torch.Tensor]:
     """residual' = residual + x (fp32; x alone where there is no residual yet) and the rows residual' / rms(residual') * w in 8 bits.  x [T, H] bf16 or fp32, residual
     fp32, w [H] bf16 or fp32; H at most 16384 on a GPU.  The norm is that of the fp32 residual', in 64 bits.  Returns (rows, residual')."""
-    _check_rows(x, "rows")
-    (T, H), device = x.shape, x.get_device()
-    if w.shape != (H,) or (residual is not None and residual.shape != x.shape):
+    T, H, device = _check_rows(x, "rows")
+    if w.dim() != 1 or w.shape[0] != H or (residual is not None and residual.shape != x.shape):
         raise ValueError(f"rows {tuple(x.shape)} with a norm of {tuple(w.shape)} and a residual of {None if residual is None else tuple(residual.shape)}")
     if w.get_device() != device or (residual is not None and residual.get_device() != device):
         raise ValueError("rows, residual and norm weight are on one device")
@@ -197,47 +222,50 @@ def fp8_add_rmsnorm(x: torch.Tensor, residual: Optional[torch.Tensor], w: torch.
         return _quantize(v * torch.rsqrt(v.square().mean(-1, keepdim=True) + eps) * w.to(torch.float64)), r
     if H > MAX_NORM:
         raise ValueError(f"rows of {H} values: the norm takes up to {MAX_NORM}")
-    if (residual is not None and residual.dtype is not torch.float32) or w.dtype not in (torch.bfloat16, torch.float32):
+    kind, f32 = w.dtype, torch.float32
+    if (residual is not None and residual.dtype is not f32) or (kind is not torch.bfloat16 and kind is not f32):
         raise ValueError("the residual is fp32, the norm weight bf16 or fp32")
     x = _aligned(x)
+    at, ld = 0, 0
     if residual is not None:
         residual = _aligned(residual)
+        at, ld = residual.data_ptr(), residual.stride(0)
     if w.stride(0) != 1 or w.data_ptr() % 16:
         w = w.clone(memory_format=torch.contiguous_format)
     out = Fp8Rows.allocate(T, H, x.device)
-    res = torch.empty(T, H, dtype=torch.float32, device=x.device)
-    p = Fp8NormParams(x.data_ptr(), x.stride(0), N.ptr(residual), 0 if residual is None else residual.stride(0), w.data_ptr(), H, eps, res.data_ptr(),
-                      out.codes.data_ptr(), out.codes.stride(0), out.exps.data_ptr(), out.exps.stride(0))
-    _call(device, "sl_fp8_add_rmsnorm", C.byref(p), T, int(x.dtype is torch.float32), int(w.dtype is torch.float32))
+    res = x.new_empty((T, H), dtype=f32)
+    p = Fp8NormParams(x.data_ptr(), x.stride(0), at, ld, w.data_ptr(), H, eps, res.data_ptr(), *out._where())
+    _call(device, "sl_fp8_add_rmsnorm", C.byref(p), T, x.dtype is f32, kind is f32)
     return out, res
 
 
 # ---- products ----------------------------------------------------------------------------------------------------------------------------
 
-def _operands(rows: Fp8Rows, w) -> Tuple[torch.Tensor, torch.Tensor]:
-    """Codes and scales of FP8 weights, checked and (on a GPU) as the kernels take them."""
+def _operands(rows: Fp8Rows, w) -> Tuple[torch.Tensor, torch.Tensor, int]:
+    """Codes and scales of FP8 weights, checked and (on a GPU) as the kernels take them, and the device's number."""
     codes, scale = w.weight, w.fp8_scale
-    if scale is None or codes.dtype not in (torch.float8_e4m3fn, torch.uint8):
+    if scale is None or (codes.dtype is not torch.float8_e4m3fn and codes.dtype is not torch.uint8):
         raise ValueError("rows in 8 bits are multiplied with FP8 weights (e4m3 and a scale for each block of 128 x 128)")
-    (n, k), device = codes.shape, rows.codes.get_device()
-    if k != rows.codes.shape[1] or scale.shape[0] < -(-n // GROUP) or scale.shape[1] < -(-k // GROUP):
-        raise ValueError(f"rows {tuple(rows.codes.shape)}, weights {tuple(codes.shape)} with scales {tuple(scale.shape)}")
+    (n, k), (nb, kb), device = codes.shape, scale.shape, rows._memory.get_device()
+    if k != rows.shape[1] or nb * GROUP < n or kb * GROUP < k:
+        raise ValueError(f"rows {rows.shape}, weights {(n, k)} with scales {(nb, kb)}")
     if codes.get_device() != device or scale.get_device() != device:
         raise ValueError("rows, weights and scales are on one device")
     if device >= 0:
-        if codes.stride(1) != 1 or codes.stride(0) % 16 or codes.data_ptr() % 16:
+        ld, by = codes.stride()
+        if by != 1 or ld % 16 or codes.data_ptr() % 16:
             codes = codes.clone(memory_format=torch.contiguous_format)
         if scale.dtype is not torch.float32 or scale.stride(1) != 1:
             scale = scale.to(torch.float32).contiguous()
-    return codes, scale
+    return codes, scale, device
 
 
-def _multiply(name: str, rows: Fp8Rows, codes: torch.Tensor, scale: torch.Tensor, y, ldy: int, f32: int, exps_out=None, lde_out: int = 0) -> None:
-    (T, K), x, e, device = rows.codes.shape, rows.codes, rows.exps, rows.codes.get_device()
-    ldx, lde = (x.stride(0), e.stride(0)) if T > 1 else (K, _padded(K))
-    p = Fp8LinearParams(e.data_ptr(), lde, scale.data_ptr(), scale.stride(0), y.data_ptr(), ldy, f32, T, codes.shape[0], K, N.ptr(exps_out), lde_out,
-                        _status(device))
-    _call(device, name, x.data_ptr(), ldx, codes.data_ptr(), codes.stride(0), C.byref(p))
+def _multiply(name: str, device: int, rows: Fp8Rows, codes: torch.Tensor, n: int, scale: torch.Tensor, y: int, ldy: int, f32: bool, exps_out: int = 0,
+              lde_out: int = 0) -> None:
+    T, K = rows.shape
+    x, ldx, e, lde = rows._where()
+    p = Fp8LinearParams(e, lde, scale.data_ptr(), scale.stride(0), y, ldy, f32, T, n, K, exps_out, lde_out, _status(device))
+    _call(device, name, x, ldx, codes.data_ptr(), codes.stride(0), C.byref(p))
 
 
 @lru_cache(maxsize=4096)
@@ -248,26 +276,28 @@ def _on_pairs(tokens: int, n: int, k: int) -> bool:
 def fp8_linear(rows: Fp8Rows, w, out_f32: bool = False) -> torch.Tensor:
     """y = rows @ W^T [T, N], fp32 sums, in bf16 or fp32.  `w`: a :class:`~slopllm_b200.models.weights.LinearWeight` in FP8.  A NaN code spoils its row's (a
     weight's: its column's) results and no other."""
-    codes, scale = _operands(rows, w)
+    codes, scale, device = _operands(rows, w)
     n, kind = codes.shape[0], torch.float32 if out_f32 else torch.bfloat16
-    if rows.codes.get_device() < 0:
+    if device < 0:
         return (_values(rows) @ quant.fp8_block_dequantize(codes, scale).t()).to(kind)
     pad = 4 if out_f32 else 8                        # whole pieces of 16 bytes a row
     ld = -(-n // pad) * pad
-    y = torch.empty(rows.codes.shape[0], ld, dtype=kind, device=rows.codes.device)
-    _multiply("sl_fp8_linear", rows, codes, scale, y, ld, int(out_f32))
+    y = codes.new_empty((rows.shape[0], ld), dtype=kind)
+    _multiply("sl_fp8_linear", device, rows, codes, n, scale, y.data_ptr(), ld, out_f32)
     return y if ld == n else y[:, :n]
 
 
 def fp8_gate_up(rows: Fp8Rows, w) -> Fp8Rows:
     """silu(rows @ Wg^T) * (rows @ Wu^T) in 8 bits, W = gate rows | up rows [2 I, K]: :func:`fp8_silu_mul` of the product's fp32 sums.  Many rows make the
-    activation in the product's epilogue, in fp32 (`inner` a multiple of 128): a value next to the middle between two codes may get the other one."""
-    inner = w.weight.shape[0] // 2
-    if w.weight.shape[0] % 32:
-        raise ValueError(f"{w.weight.shape[0]} gate and up rows: rows in 8 bits have a multiple of 16 values")
-    if not rows.codes.is_cuda or inner % GROUP or not _on_pairs(rows.codes.shape[0], 2 * inner, rows.codes.shape[1]):
+    activation in the product's epilogue, in fp32 (I a multiple of 128): a value next to the middle between two codes may get the other one."""
+    n = w.weight.shape[0]
+    if n % 32:
+        raise ValueError(f"{n} gate and up rows: rows in 8 bits have a multiple of 16 values")
+    T, K = rows.shape
+    if n % (2 * GROUP) or rows._memory.get_device() < 0 or not _on_pairs(T, n, K):
         return fp8_silu_mul(fp8_linear(rows, w, out_f32=True))
-    codes, scale = _operands(rows, w)
-    out = Fp8Rows.allocate(rows.codes.shape[0], inner, rows.codes.device)
-    _multiply("sl_fp8_gate_up", rows, codes, scale, out.codes, inner, 0, out.exps, out.exps.stride(0))
+    codes, scale, device = _operands(rows, w)
+    out = Fp8Rows.allocate(T, n // 2, codes.device)
+    to, ld, exps, lde = out._where()
+    _multiply("sl_fp8_gate_up", device, rows, codes, n, scale, to, ld, False, exps, lde)
     return out
