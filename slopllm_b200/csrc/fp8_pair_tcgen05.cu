@@ -165,16 +165,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) fp8_pair
 #pragma unroll
             for (int i = 0; i < 64; ++i) acc[i] = pair(0.f, 0.f);
             const uint32_t lanes = tmem + ((uint32_t)(q * 32) << 16) + half * 128;
-            uint32_t r0[32], r1[32];
-            auto wait_sums = [&](int i) {
-                if (ok) {
-                    ok = tc::mbar_wait_soon_warp(&acc_full[i & 1], (i >> 1) & 1);
-                    if (!ok && lane == 0) atomicExch(p.err, WAIT_SUMS);
-                }
-                tc::fence_after_sync();
-            };
-            wait_sums(it);
-            tc::tmem_ld_32x32(lanes + (it & 1) * BN, r0);
+            uint32_t r[5][16];
 #pragma unroll 1
             for (int kb = 0; kb < blocks; ++kb, ++it) {
                 if ((kb & 15) == 0) {                        // the exponents of sixteen blocks of K are a load, one such load ahead
@@ -187,29 +178,31 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) fp8_pair
                 const f32x2 ff = pair(f, f);
                 scale = __ldg(scales + min(kb + 1, blocks - 1));
                 const uint32_t at = lanes + (it & 1) * BN;
-                auto add = [&](const uint32_t (&r)[32], int c) {
+                auto add = [&](const uint32_t (&v)[16], int c) {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        acc[c * 16 + i] = fma2(pair(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1])), ff, acc[c * 16 + i]);
+                    for (int i = 0; i < 8; ++i)
+                        acc[c * 8 + i] = fma2(pair(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), ff, acc[c * 8 + i]);
                 };
-                // while a quarter is added up the next is on its way, behind the last one the next block's first
+                if (ok) {
+                    ok = tc::mbar_wait_soon_warp(&acc_full[it & 1], (it >> 1) & 1);
+                    if (!ok && lane == 0) atomicExch(p.err, WAIT_SUMS);
+                }
+                tc::fence_after_sync();
+                // The accumulator goes back as soon as it is read.  Registers hold 80 of the 128 columns, so 48 are added up in between.
+#pragma unroll
+                for (int c = 0; c < 5; ++c) tc::tmem_ld_32x16(at + c * 16, r[c]);
                 tc::tmem_ld_wait();
-                tc::tmem_ld_32x32(at + 32, r1);
-                add(r0, 0);
-                tc::tmem_ld_wait();
-                tc::tmem_ld_32x32(at + 64, r0);
-                add(r1, 1);
-                tc::tmem_ld_wait();
-                tc::tmem_ld_32x32(at + 96, r1);
-                add(r0, 2);
+#pragma unroll
+                for (int c = 0; c < 3; ++c) add(r[c], c);
+#pragma unroll
+                for (int c = 0; c < 3; ++c) tc::tmem_ld_32x16(at + 80 + c * 16, r[c]);
                 tc::tmem_ld_wait();
                 tc::fence_before_sync();
                 if (tc::elect_one()) tc::arrive_cluster_soon(empty_at + (it & 1) * 8);
-                if (kb + 1 < blocks) {
-                    wait_sums(it + 1);
-                    tc::tmem_ld_32x32(lanes + ((it + 1) & 1) * BN, r0);
-                }
-                add(r1, 3);
+                add(r[3], 3);
+                add(r[4], 4);
+#pragma unroll
+                for (int c = 0; c < 3; ++c) add(r[c], 5 + c);
             }
             int m0, n0;
             coords(tile, m0, n0);

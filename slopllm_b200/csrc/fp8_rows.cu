@@ -7,8 +7,8 @@
 // the largest magnitude's own bits and on nothing that a division could round.  A value that fp32 does not hold as a finite number is the NaN
 // code; magnitudes above 448 * 2^60 saturate.  Exponent rows start at multiples of 16 bytes: the product reads sixteen groups at a time.
 //
-// Codes are the nearest ones of the definition in 64 bits.  fp32 decides all but the values that lie within its error of the middle between two
-// codes; those are made again in 64 bits.
+// Codes are the nearest ones of the definition in 64 bits (where products stay in the normal range of fp32).  fp32 decides all but the values that lie
+// within its error of the middle between two codes; those are made again in 64 bits.
 #include <algorithm>
 #include <type_traits>
 
@@ -108,18 +108,23 @@ __device__ __forceinline__ void load4(const void* row, int i, float (&v)[4]) {
 // One block a token; a warp has whole groups, a thread four values of each.  The sum of squares is taken in 64 bits: fp32 rows may be as large
 // as fp32 goes, and its rounding would move every code of the row.
 template <bool XF32, bool WF32, int Q>
-__global__ void __launch_bounds__(1024) fp8_norm_kernel(const __grid_constant__ Fp8NormParams p) {
+__global__ void __launch_bounds__(1024, 1) fp8_norm_kernel(const __grid_constant__ Fp8NormParams p) {
     pdl_grid_sync();
     __shared__ double sums[33];
     const int t = blockIdx.x, nt = blockDim.x, n4 = p.H / 4, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     const char* const x = reinterpret_cast<const char*>(p.x) + (size_t)t * p.ldx * (XF32 ? 4 : 2);
+    using WRaw = std::conditional_t<WF32, float4, uint2>;
+    WRaw gain[Q];                                            // (asked for with the row, used behind the sum)
     float v[Q][4];
     double ss = 0.0;
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
         const int i = threadIdx.x + q * nt;
-        if (i < n4) load4<XF32>(x, i, v[q]);
-        else v[q][0] = v[q][1] = v[q][2] = v[q][3] = 0.f;
+        gain[q] = WRaw{};
+        if (i < n4) {
+            load4<XF32>(x, i, v[q]);
+            gain[q] = __ldg(reinterpret_cast<const WRaw*>(p.w) + i);
+        } else v[q][0] = v[q][1] = v[q][2] = v[q][3] = 0.f;
     }
     if (p.residual != nullptr) {
         const float4* const r = reinterpret_cast<const float4*>(p.residual + (size_t)t * p.ldr);
@@ -157,8 +162,12 @@ __global__ void __launch_bounds__(1024) fp8_norm_kernel(const __grid_constant__ 
     for (int q = 0; q < Q; ++q) {
         const int i = threadIdx.x + q * nt;
         if (i - lane >= n4) break;                       // (the same for the whole warp)
-        float w[4] = {0.f, 0.f, 0.f, 0.f}, f[4];
-        if (i < n4) load4<WF32>(p.w, i, w);
+        float w[4], f[4];
+        if constexpr (WF32) { w[0] = gain[q].x; w[1] = gain[q].y; w[2] = gain[q].z; w[3] = gain[q].w; }
+        else {
+            const float2 lo = bf162_to_f2(gain[q].x), hi = bf162_to_f2(gain[q].y);
+            w[0] = lo.x; w[1] = lo.y; w[2] = hi.x; w[3] = hi.y;
+        }
 #pragma unroll
         for (int j = 0; j < 4; ++j) f[j] = v[q][j] * inv32 * w[j];
         int e;

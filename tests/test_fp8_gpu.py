@@ -26,7 +26,7 @@ def rms(r, w, eps):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("t,k", [(0, 128), (1, 16), (1, 128), (2, 144), (3, 272), (5, 1024), (7, 4112), (300, 2048), (1, 16384), (64, 31264)])
+@pytest.mark.parametrize("t,k", [(0, 128), (1, 16), (1, 128), (2, 144), (3, 272), (5, 1024), (7, 4112), (300, 2048), (1, 16384), (64, 31264), (2500, 4096), (700, 14352)])
 def test_rows(t, k, dtype):
     """Whole and cut groups, sizes that differ from token to token, one token and many."""
     x = (torch.randn(t, 2 * k, generator=gen(t + k), device="cuda") * torch.exp(torch.randn(t, 1, generator=gen(1), device="cuda") * 2)).to(dtype)
@@ -198,6 +198,35 @@ def test_gate_up(t, inner):
     step = torch.exp2(got.exps.double() - 127).repeat_interleave(128, 1)[:, :inner]
     assert ((held(got) - want).abs() <= off + torch.maximum(2.0 ** -4 * (want.abs() + off), 2.0 ** -10 * step)).all()
     tcgen05.check_errors(rows.device)
+
+
+def test_gate_up_of_many_tiles():
+    """More tiles than pairs of SMs, some of them cut by the last row: the codes of the product and the activation by themselves, all but those next to a middle."""
+    w, _ = weight(4096, 1040, 21)
+    rows = some_rows(2100, 1040, 22)
+    got, want = F8.fp8_gate_up(rows, w), F8.fp8_silu_mul(F8.fp8_linear(rows, w, out_f32=True))
+    assert (got.exps == want.exps).all() and (got.codes != want.codes).float().mean() < 1e-4
+    assert ((held(got) - held(want)).abs() <= 2.0 ** -3 * held(want).abs() + 2.0 ** -9 * torch.exp2(want.exps.double() - 127).repeat_interleave(128, 1)).all()
+    tcgen05.check_errors(rows.device)
+
+
+def test_calls_side_by_side():
+    """The forms of the product on several streams at once, over the same rows and weights: each gives what it gives by itself."""
+    (w, _), (big, _) = weight(1024, 2048, 23), weight(6144, 2048, 24)
+    some, many = some_rows(20, 2048, 25), some_rows(900, 2048, 26)
+    calls = [lambda: F8.fp8_linear(some, w), lambda: F8.fp8_linear(some, big, out_f32=True), lambda: F8.fp8_linear(many, big),
+             lambda: F8.fp8_gate_up(many, big).codes, lambda: F8.fp8_gate_up(some, big).codes]
+    want = [c() for c in calls]
+    streams = [torch.cuda.Stream() for _ in calls]
+    for _ in range(5):
+        got = []
+        for c, s in zip(calls, streams):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                got.append(c())
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    tcgen05.check_errors(w.weight.device)
 
 
 def layer(x, res, norm, gate_up, down):

@@ -232,3 +232,23 @@ def test_weights_that_are_partly_fp8():
                 t[n] = quant.fp8_block_dequantize(t[n], t.pop(n + "_scale_inv"))
         errs = errors(cfg, w, t, "cpu", prompt, 2, 32)
         assert max(errs) < 2e-2, (some, errs)
+
+
+@pytest.mark.gpu
+def test_weights_that_are_partly_fp8_on_a_gpu():
+    """A feed-forward of rows in 8 bits whose down projection is bf16: as its parts."""
+    from slopllm_b200.models.weights import LinearWeight
+    from slopllm_b200.ops import fp8 as F8
+    from slopllm_b200.ops.cuda_ops import CudaOps
+    cfg = DenseConfig.tiny()
+    w, _ = random_dense_model(cfg, seed=3, device="cuda", dtype=torch.bfloat16, fp8=True)
+    layer, ops = w.layers[0], CudaOps(cfg)
+    rows = F8.fp8_rows(torch.randn(5, cfg.hidden_size, generator=torch.Generator(device="cuda").manual_seed(1), device="cuda"))
+    layer.mlp_w2 = LinearWeight(layer.mlp_w2.dequant(torch.bfloat16))
+    y = ops.dense_mlp(rows, layer)
+    gu = F8.fp8_linear(rows, layer.mlp_w13).double()
+    g, u = gu.chunk(2, -1)
+    want = (g * torch.sigmoid(g) * u) @ layer.mlp_w2.weight.double().t()
+    # the activation is rounded to bf16 (2^-8 of each value), sums are fp32
+    most = (g * torch.sigmoid(g) * u).abs() @ layer.mlp_w2.weight.double().abs().t()
+    assert y.dtype == torch.float32 and ((y.double() - want).abs() <= 2.0 ** -7 * most).all()
