@@ -330,20 +330,20 @@ def main(argv=None) -> int:
                 x = torch.randn(T, k, device=dev, generator=g).to(torch.bfloat16)
                 us = time_op(lambda: ops.linear(x, w), args.iters, flush)
                 emit(roofline_row(name, T, us, n * k + 4 * sc.numel() + 2 * T * (n + k), 2.0 * T * n * k, peaks))
-                rows = F8.fp8_rows(x)
-                us = time_op(lambda: F8.fp8_linear(rows, w), args.iters, flush)
+                r8 = F8.fp8_rows(x)
+                us = time_op(lambda: F8.fp8_linear(r8, w), args.iters, flush)
                 emit(roofline_row(name + " (rows in 8 bits)", T, us, n * k + 4 * sc.numel() + T * (k + 2 * n), 2.0 * T * n * k, peaks))
                 if name == "fp8_gate_up":
-                    us = time_op(lambda: F8.fp8_gate_up(rows, w), args.iters, flush)
+                    us = time_op(lambda: F8.fp8_gate_up(r8, w), args.iters, flush)
                     emit(roofline_row("fp8_gate_up and activation (rows in 8 bits)", T, us, n * k + 4 * sc.numel() + T * (k + n // 2), 2.0 * T * n * k, peaks))
             del w, q
         for T in tokens:                                     # rows in 8 bits: norm of the residual stream, activation, and what they hold
             x, res = torch.randn(T, 4096, device=dev, generator=g), torch.randn(T, 4096, device=dev, generator=g)
             gain, gu = torch.ones(4096, device=dev, dtype=torch.bfloat16), torch.randn(T, 2 * 12288, device=dev, generator=g).to(torch.bfloat16)
-            rows = F8.fp8_rows(x)
+            r8 = F8.fp8_rows(x)
             for name, fn, per in (("fp8_add_rmsnorm", lambda: F8.fp8_add_rmsnorm(x, res, gain, 1e-6), 13 * 4096),
                                   ("fp8_silu_mul", lambda: F8.fp8_silu_mul(gu), 5 * 12288), ("fp8_rows", lambda: F8.fp8_rows(x), 5 * 4096),
-                                  ("fp8_values", lambda: F8.fp8_values(rows), 3 * 4096)):
+                                  ("fp8_values", lambda: F8.fp8_values(r8), 3 * 4096)):
                 emit(roofline_row(name, T, time_op(fn, args.iters, flush), T * per, 0.0, peaks))
     if "mixers" in cases:
         mixer_rows(emit, tokens, args.iters, flush, peaks, dev)
