@@ -4,7 +4,7 @@
 // A pair works on 256 rows by 256 columns, each SM with its 128 rows of the operand and of the result and half of the weights' rows.  A block of
 // 128 values of K is a product by itself in tensor memory (two accumulators of 256 columns), because its factor S[n / 128, b] * 2^E[t, b] differs from the
 // next one's:
-//   warp 0     fetches its SM's operand halves (TMA, six blocks of K ahead)
+//   warp 0     fetches its SM's operand halves (TMA, five blocks of K ahead)
 //   warp 1     of the leading SM multiplies
 //   warps 4-11 take a block's sums out of tensor memory and add them, times their factor, to fp32 registers: a thread has a row and 128 columns,
 //              64 instructions of two multiply-adds a block, while the tensor cores are at the next one (warps 2 and 3 only give their registers)
@@ -21,15 +21,15 @@
 
 namespace {
 
-constexpr int BM = 128, BN = 256, BK = 128, STAGES = 6, ADDERS = 8, THREADS = 128 + ADDERS * 32;
+constexpr int BM = 128, BN = 256, BK = 128, STAGES = 5, ADDERS = 8, THREADS = 128 + ADDERS * 32;
 constexpr int HALF_BYTES = 128 * BK;                         // one operand of one SM
 constexpr int STAGE_BYTES = 2 * HALF_BYTES;
 constexpr int FEW_REGS = 40, MANY_REGS = 232;
 static_assert(128 * FEW_REGS + ADDERS * 32 * MANY_REGS <= THREADS * 168, "registers are moved, not made");
 constexpr int PIECE = 32 * 128;                              // a warp's part of the result on its way out: 128 bytes of 32 rows
-constexpr int OUT = ADDERS * PIECE;                          // gated: half of it for codes, half for sums that threads of a row exchange
+constexpr int OUT = 2 * ADDERS * PIECE;                      // two a warp; gated: half of it for codes, half for sums that threads of a row exchange
 constexpr int SMEM = STAGES * STAGE_BYTES + OUT + 1024 + 256;
-static_assert(OUT / 2 >= 2 * 128 * 16 * 4, "sixteen columns of gate and up sums");
+static_assert(OUT / 2 >= 2 * 128 * 32 * 4, "32 columns of gate and up sums");
 enum { WAIT_FREE = 75, WAIT_LANDED, WAIT_READ, WAIT_FETCHED, WAIT_SUMS };       // numbers of waits that run out
 
 struct Tiles { int m, n, total; };
@@ -40,9 +40,10 @@ __device__ __forceinline__ float silu_mul(float g, float u) { return __fdividef(
 // A warp's piece of the result, shared memory to memory, and the wait until the last one has left shared memory; by the same thread.
 __device__ __forceinline__ void bulk_store(const CUtensorMap* map, const void* src, int c0, int c1) {
     asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.bulk_group [%0, {%2, %3}], [%1];" ::"l"(map), "r"(tc::smem_u32(src)), "r"(c0), "r"(c1) : "memory");
-    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
 }
-__device__ __forceinline__ void bulk_read() { asm volatile("cp.async.bulk.wait_group.read 0;" ::: "memory"); }
+__device__ __forceinline__ void bulk_commit() { asm volatile("cp.async.bulk.commit_group;" ::: "memory"); }
+template <int OTHERS>
+__device__ __forceinline__ void bulk_read() { asm volatile("cp.async.bulk.wait_group.read %0;" ::"n"(OTHERS) : "memory"); }
 __device__ __forceinline__ void meet() { asm volatile("bar.sync 1, 256;" ::: "memory"); }      // the adders
 
 template <bool GATED>
@@ -212,23 +213,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) fp8_pair
             auto piece = [&](uint8_t* at, int j) { return reinterpret_cast<uint4*>(at + lane * 128 + ((j ^ (lane & 7)) << 4)); };
             if (GATED) {
                 // Of a row's 128 columns the thread with the gate's sums makes the first 64, the one with the up rows' the others.  They exchange
-                // sixteen columns at a time, [side][column][row].
+                // 32 columns at a time, [side][column][row].
                 float* const swap = reinterpret_cast<float*>(out + OUT / 2);
-                if (half == 0 && lane == 0) bulk_read();     // (codes of the last tile are out before new ones are written behind the first meeting)
+                if (half == 0 && lane == 0) bulk_read<0>();     // (codes of the last tile are out before new ones are written behind the first meeting)
                 float act[64];
 #pragma unroll
-                for (int c = 0; c < 64; c += 16) {
-                    float* const mine = swap + half * 16 * 128 + in_tile;
-                    const float* const theirs = swap + (half ^ 1) * 16 * 128 + in_tile;
+                for (int c = 0; c < 64; c += 32) {
+                    float* const mine = swap + half * 32 * 128 + in_tile;
+                    const float* const theirs = swap + (half ^ 1) * 32 * 128 + in_tile;
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
+                    for (int i = 0; i < 16; ++i) {
                         const float2 lo = unpair(acc[c / 2 + i]), hi = unpair(acc[32 + c / 2 + i]);
                         mine[(2 * i) * 128] = half ? lo.x : hi.x;
                         mine[(2 * i + 1) * 128] = half ? lo.y : hi.y;
                     }
                     meet();
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
+                    for (int i = 0; i < 16; ++i) {
                         const float2 lo = unpair(acc[c / 2 + i]), hi = unpair(acc[32 + c / 2 + i]);
                         const float x = theirs[(2 * i) * 128], y = theirs[(2 * i + 1) * 128];
                         act[c + 2 * i] = half ? silu_mul(x, hi.x) : silu_mul(lo.x, x);
@@ -264,23 +265,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) fp8_pair
                 tc::fence_proxy_async_smem();
                 meet();                                      // (also: `tops` is read before it is written again)
                 if (half == 0) {
-                    if (lane == 0 && row0 < p.T) bulk_store(&tmY, codes, n0, row0);
+                    if (lane == 0 && row0 < p.T) {
+                        bulk_store(&tmY, codes, n0, row0);
+                        bulk_commit();
+                    }
                     if (row0 + lane < p.T) p.exps_out[(size_t)(row0 + lane) * p.lde_out + n0 / 128] = (uint8_t)(e + FP8_BIAS);
                 }
             } else {
                 // 128 bytes of each of the warp's rows at a time; rows and columns that are not there are left out by the copy
-                uint8_t* const mine = out + (warp - 4) * PIECE;
+                uint8_t* const mine = out + (warp - 4) * 2 * PIECE;
                 const int col = n0 + half * 128;
                 auto store = [&](auto bits, auto per) {      // `per` values to 16 bytes
 #pragma unroll
                     for (int c = 0; c < 128; c += 8 * per) {
-                        if (lane == 0) bulk_read();
+                        uint8_t* const here = mine + c / (8 * per) % 2 * PIECE;
+                        if (lane == 0) bulk_read<1>();       // (what was in it is out: at most the other one is still on its way)
                         __syncwarp();
 #pragma unroll
-                        for (int j = 0; j < 8; ++j) *piece(mine, j) = bits(c + j * per);
+                        for (int j = 0; j < 8; ++j) *piece(here, j) = bits(c + j * per);
                         tc::fence_proxy_async_smem();
                         __syncwarp();
-                        if (lane == 0 && row0 < p.T && col + c < p.N) bulk_store(&tmY, mine, col + c, row0);
+                        if (lane == 0) {
+                            if (row0 < p.T && col + c < p.N) bulk_store(&tmY, here, col + c, row0);
+                            bulk_commit();                   // (an empty group keeps the count)
+                        }
                     }
                 };
                 if (p.out_f32)
