@@ -4,7 +4,7 @@
 //   y[t, n] = sum over blocks b of  S[n / 128, b] * 2^(E[t, b] - 127) * (sum over the block's k of X[t, k] * W[n, k])
 //
 // The scales differ from block to block of K, so a block's sums leave the tensor memory 128 values of K later and are added, times their factor, in fp32
-// registers: one multiply-add a value and block, beside 128 multiply-adds of the tensor core.
+// registers: one multiply-add a value and block, beside 128 multiply-adds of the tensor core.  Few rows here, many on pairs of SMs (fp8_pair_tcgen05.cu).
 //
 // All mbarrier waits are bounded; where one runs out, the error word is set and the blocks still meet at the end.
 #include <algorithm>
@@ -57,7 +57,12 @@ __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.w
 // ---- few rows: weights are the 128-row operand, rows the columns ---------------------------------------------------------------------------
 //
 // A block has 128 features, up to BN rows and a share of K; the blocks of a cluster have the shares of the same features.  Each block completes BN / shares
-// of the rows: the others send their sums into its shared memory, and it adds them in the order of the shares.  Warp 0 fetches (TMA ring), warp 1 multiplies, the others have a feature and up to 64 rows a thread and add up.
+// of the rows: the others send their sums into its shared memory, and it adds them in the order of the shares.  Warp 0 fetches (TMA ring), warp 1
+// multiplies, the others have a feature and up to 32 rows a thread and add up.
+//
+// Bound by the weights' bytes and by what is around them: a launch (1.2 us), the first bytes (1.5), the joining of the shares (1).  8 rows by 28672 x 4096:
+// 22.6 us, 5.2 TB/s; 1 by 6144 x 4096: 7.8 us; 29 by 4096 x 12288: 13.7.  Weights are the operand of 128 rows because those are full whatever the batch.
+// 128 rows of X a block were slower than 64 twice (their sums do not fit the registers).
 template <int BN>
 struct Few {
     static constexpr int A_BYTES = 128 * BK, B_BYTES = BN * BK, STAGE = A_BYTES + B_BYTES;
@@ -290,10 +295,10 @@ int launch_few(const void* x, int ldx, const void* W, int ldw, const Fp8LinearPa
     return rc != cudaSuccess ? (int)rc : SL_LAUNCH_CHECK();
 }
 
-// Whether pairs of SMs are the faster form.  Up to 64 rows they never are (64 by 16384 x 2048: 13.5 us without, 14.8 with them).  More: a pair takes 0.47 us for a
-// block of K of its 256 x 256 tile and 3 for what is around it, 74 run at once; 64-row tiles of one SM take 0.42 for a block and SM.  Microseconds without and with
-// pairs: 128 by 6144 x 4096 15.9, 20.8; 256 by 6144 x 4096 22.2, 21.0; 128 by 24576 x 4096 41.1, 37.5; 333 by 2321 x 5136 20.3, 24.4; 512 by 2048 x 2048 11.3,
-// 13.7; 1000 by 2048 x 2048 14.2, 13.8; 1000 by 1024 x 8192 23.2, 33.1.
+// Whether pairs of SMs are the faster form.  Up to 64 rows they never are (64 by 16384 x 2048: 13.5 us without, 14.8 with them).  More: a pair takes 0.47 us
+// for a block of K of its 256 x 256 tile and 3 for what is around it, 74 run at once; 64-row tiles of one SM take 0.42 for a block and SM.
+// Microseconds without and with pairs: 128 by 6144 x 4096 15.9, 20.8; 256 by 6144 x 4096 22.2, 21.0; 128 by 24576 x 4096 41.1, 37.5; 333 by 2321 x 5136
+// 20.3, 24.4; 512 by 2048 x 2048 11.3, 13.7; 1000 by 2048 x 2048 14.2, 13.8; 1000 by 1024 x 8192 23.2, 33.1.
 bool on_pairs(int T, int N, int K) {
     if (T <= 64) return false;
     const long long blocks = (K + BK - 1) / BK, cols = (N + 127) / 128;
@@ -301,9 +306,9 @@ bool on_pairs(int T, int N, int K) {
     return 3.f + (float)rounds * (0.47f * (float)blocks + 3.f) <= 5.5f + 0.42f / 148.f * (float)((T + 63) / 64 * cols * blocks);
 }
 
-// Blocks that share a tile's K: twice as many while every block still has an SM to itself, and once more, two blocks an SM, where each has twelve blocks of K left to halve.
-// Microseconds with 4 and 8 shares: 16 by 4096 x 4096 8.0, 8.4 and 256 by 1024 x 2048 7.2, 8.4 (32 tiles), but 29 by 4096 x 12288 15.2, 14.2; 1 by 1024 x 2048
-// (8 tiles) 5.1, 4.6.  With 2 and 4: 32 by 6144 x 4096 11.8, 10.2 (48 tiles).
+// Blocks that share a tile's K: twice as many while every block still has an SM to itself, and once more, two blocks an SM, where each has twelve blocks
+// of K left to halve.  Microseconds with 4 and 8 shares: 16 by 4096 x 4096 8.0, 8.4 and 256 by 1024 x 2048 7.2, 8.4 (32 tiles), but 29 by 4096 x 12288
+// 15.2, 14.2; 1 by 1024 x 2048 (8 tiles) 5.1, 4.6.  With 2 and 4: 32 by 6144 x 4096 11.8, 10.2 (48 tiles).
 int shares_of(long long tiles, int blocks) {
     int shares = 1;
     while (shares < 8 && blocks >= 2 * shares && (tiles * shares * 2 <= 148 || (tiles * shares * 2 <= 296 && blocks >= 12 * shares))) shares *= 2;

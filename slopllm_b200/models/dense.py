@@ -232,7 +232,7 @@ class DenseModel(DecoderStack):
             mixer = self._full_attention if full else self._linear_attention
             self.sublayers.append(Sublayer(functools.partial(mixer, i, lw), lw.input_norm, fp8_input=full and self._in_fp8(lw.w_qkv)))
             self.sublayers.append(Sublayer(functools.partial(self._mlp, lw), lw.post_attn_norm, fp8_input=self._in_fp8(lw.mlp_w13)))
-        if act_dtype is not None and not any(s.fp8_input for s in self.sublayers):
+        if act_dtype is not None and not any(self._in_fp8(w) for lw in weights.layers for w in (lw.w_qkv, lw.o_proj, lw.mlp_w13) if w is not None):
             raise ValueError("activations in 8 bits go with FP8 projections, and these weights have none")
         self._init_stack(ctx, ops or get_ops(cfg, ctx.device, ctx), comm,
                          torch.bfloat16 if ctx.device.type == "cuda" else torch.float32)

@@ -209,8 +209,8 @@ def fp8_silu_mul(gate_up: torch.Tensor) -> Fp8Rows:
 
 
 def fp8_add_rmsnorm(x: torch.Tensor, residual: Optional[torch.Tensor], w: torch.Tensor, eps: float) -> Tuple[Fp8Rows, torch.Tensor]:
-    """residual' = residual + x (fp32; x alone where there is no residual yet) and the rows residual' / rms(residual') * w in 8 bits.  x [T, H] bf16 or fp32, residual
-    fp32, w [H] bf16 or fp32; H at most 16384 on a GPU.  The norm is that of the fp32 residual', in 64 bits.  Returns (rows, residual')."""
+    """residual' = residual + x (fp32; x alone where there is no residual yet) and the rows residual' / rms(residual') * w in 8 bits.  x [T, H] bf16 or
+    fp32, residual fp32, w [H] bf16 or fp32; H at most 16384 on a GPU.  The norm is that of the fp32 residual', in 64 bits.  Returns (rows, residual')."""
     T, H, device = _check_rows(x, "rows")
     if w.dim() != 1 or w.shape[0] != H or (residual is not None and residual.shape != x.shape):
         raise ValueError(f"rows {tuple(x.shape)} with a norm of {tuple(w.shape)} and a residual of {None if residual is None else tuple(residual.shape)}")

@@ -26,7 +26,8 @@ def rms(r, w, eps):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("t,k", [(0, 128), (1, 16), (1, 128), (2, 144), (3, 272), (5, 1024), (7, 4112), (300, 2048), (1, 16384), (64, 31264), (2500, 4096), (700, 14352)])
+@pytest.mark.parametrize("t,k", [(0, 128), (1, 16), (1, 128), (2, 144), (3, 272), (5, 1024), (7, 4112), (300, 2048), (1, 16384), (64, 31264), (2500, 4096),
+                                 (700, 14352)])
 def test_rows(t, k, dtype):
     """Whole and cut groups, sizes that differ from token to token, one token and many."""
     x = (torch.randn(t, 2 * k, generator=gen(t + k), device="cuda") * torch.exp(torch.randn(t, 1, generator=gen(1), device="cuda") * 2)).to(dtype)
