@@ -70,7 +70,8 @@ struct Few {
     static constexpr int COLS = BN * BUFS;
     static constexpr int PARTS = BN >= 64 ? 2 : 1, OWN = BN / PARTS;        // threads of a feature, rows of one
     static constexpr int ADDERS = 4 * PARTS, THREADS = 64 + 32 * ADDERS;
-    static constexpr int STAGES = BN >= 64 ? 3 : BN == 32 ? 4 : 5;           // (two blocks an SM)
+    static constexpr int RESIDENT = BN == 16 ? 3 : 2;        // blocks an SM
+    static constexpr int STAGES = BN == 32 ? 4 : 3;
     static constexpr int RING = STAGES * STAGE;
     static constexpr int SENT = BN * 128 * 4;                // [share][own row][feature]
     static constexpr int FACTORS = 16 * BN * 4;
@@ -78,7 +79,7 @@ struct Few {
 };
 
 template <int BN>
-__global__ void __launch_bounds__(Few<BN>::THREADS, 2) fp8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
+__global__ void __launch_bounds__(Few<BN>::THREADS, Few<BN>::RESIDENT) fp8_few_kernel(const __grid_constant__ CUtensorMap tmW, const __grid_constant__ CUtensorMap tmX,
                                                       const __grid_constant__ Fp8LinearParams p) {
     using C = Few<BN>;
     extern __shared__ uint8_t smem_raw[];
@@ -306,12 +307,16 @@ bool on_pairs(int T, int N, int K) {
     return 3.f + (float)rounds * (0.47f * (float)blocks + 3.f) <= 5.5f + 0.42f / 148.f * (float)((T + 63) / 64 * cols * blocks);
 }
 
-// Blocks that share a tile's K: twice as many while every block still has an SM to itself, and once more, two blocks an SM, where each has twelve blocks
-// of K left to halve.  Microseconds with 4 and 8 shares: 16 by 4096 x 4096 8.0, 8.4 and 256 by 1024 x 2048 7.2, 8.4 (32 tiles), but 29 by 4096 x 12288
-// 15.2, 14.2; 1 by 1024 x 2048 (8 tiles) 5.1, 4.6.  With 2 and 4: 32 by 6144 x 4096 11.8, 10.2 (48 tiles).
-int shares_of(long long tiles, int blocks) {
+// Blocks that share a tile's K: twice as many while every block still has an SM to itself, and on to what is resident at once (some less: clusters leave
+// SMs free) where each block keeps so many blocks of K.  Up to 16 rows, with 3 blocks an SM, microseconds with 2, 4 and 8 shares: 4096 x 4096 (32 tiles) 10.9,
+// 8.7, 8.4; 9472 x 4096 (74) 12.8, 11.6, 13.7; 12288 x 4096 (96) 14.7, 13.3, 15.5; 4096 x 14336 (32) 23.6, 16.7, 14.9; 18944 x 4096 (148) 17.7, 18.9, 20.7.  With
+// 2 blocks an SM instead 4096 x 4096 takes 8.0 (4 shares), but 9472 x 4096 12.1 (2), 12288 x 4096 14.5 (2) and 4096 x 14336 15.5 (4).  More rows, 2 blocks
+// an SM: 64 by 4096 x 4096 12.8, 10.4, 10.9; 64 by 9472 x 4096 15.0, 18.4, 21.3; 64 by 4096 x 12288 24.6, 17.4, 16.0; with
+// 4 and 8 shares 256 by 1024 x 2048 (32 tiles) 7.2, 8.4.
+int shares_of(long long tiles, int blocks, int bn) {
+    const int room = bn == 16 ? 384 : 256, least = bn == 16 ? 4 : 6;
     int shares = 1;
-    while (shares < 8 && blocks >= 2 * shares && (tiles * shares * 2 <= 148 || (tiles * shares * 2 <= 296 && blocks >= 12 * shares))) shares *= 2;
+    while (shares < 8 && blocks >= 2 * shares && (tiles * shares * 2 <= 148 || (tiles * shares * 2 <= room && blocks >= 2 * shares * least))) shares *= 2;
     return shares;
 }
 
@@ -332,7 +337,7 @@ SL_API int sl_fp8_linear(const void* x, int ldx, const void* W, int ldw, const F
     if (on_pairs(p.T, p.N, p.K)) return fp8_pair(x, ldx, W, ldw, p, false, s);
     const int bn = p.T <= 16 ? 16 : p.T <= 32 ? 32 : 64;
     if ((p.T + bn - 1) / bn > 65535) return -1;
-    const int shares = shares_of((long long)((p.N + 127) / 128) * ((p.T + bn - 1) / bn), (p.K + BK - 1) / BK);
+    const int shares = shares_of((long long)((p.N + 127) / 128) * ((p.T + bn - 1) / bn), (p.K + BK - 1) / BK, bn);
     if (bn == 16) return launch_few<16>(x, ldx, W, ldw, p, shares, s);
     if (bn == 32) return launch_few<32>(x, ldx, W, ldw, p, shares, s);
     return launch_few<64>(x, ldx, W, ldw, p, shares, s);
