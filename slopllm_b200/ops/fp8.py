@@ -23,6 +23,7 @@ from . import native as N, quant, tcgen05
 GROUP = 128
 LOW, HIGH, BIAS = -60, 60, 127         # limits of the exponent, and what is added to it in its byte
 MAX_NORM = 16384                       # values of a row that the norm takes on a GPU
+MOST = 2 ** 31 - 2 ** 20               # rows, values of a row, values from row to row: the kernels count them, and some steps beyond, in 32 bits
 
 
 class Fp8NormParams(C.Structure):
@@ -63,6 +64,8 @@ class Fp8Rows:
             raise ValueError("rows in 8 bits are two tensors of type uint8 on one device")
         if K % 16 or K == 0:
             raise ValueError(f"rows of {K} values: rows in 8 bits have a multiple of 16")
+        if max(T, K) > MOST or (T > 1 and max(ldc, lde) > MOST):
+            raise ValueError(f"{T} rows of {K} values, {ldc} and {lde} bytes apart: up to {MOST} of each")
         if T > 1 and (ldc % 16 or lde % 16 or ldc < K or lde < _padded(K)) or by != 1 or (by_e != 1 and exps.shape[1] > 1):
             raise ValueError("rows of codes and of exponents start at multiples of 16 bytes, with bytes side by side")
         if T and device >= 0 and ((codes.data_ptr() | exps.data_ptr()) % 16
@@ -127,9 +130,9 @@ def _status(device: int) -> int:
 
 
 def _aligned(x: torch.Tensor) -> torch.Tensor:
-    """Rows that loads of four values take: a copy where they do not start at multiples of that."""
+    """Rows that loads of four values take: a copy where they do not start at multiples of that, or are too far apart."""
     ld, by = x.stride()
-    if by == 1 and (ld % 4 == 0 or x.shape[0] <= 1) and x.data_ptr() % (16 if x.dtype is torch.float32 else 8) == 0:
+    if by == 1 and (ld % 4 == 0 and ld <= MOST or x.shape[0] <= 1) and x.data_ptr() % (16 if x.dtype is torch.float32 else 8) == 0:
         return x
     return x.clone(memory_format=torch.contiguous_format)
 
@@ -142,6 +145,8 @@ def _check_rows(x: torch.Tensor, what: str) -> tuple:
     if device >= 0 and kind is not torch.bfloat16 and kind is not torch.float32:
         raise ValueError(f"{what} of type {kind}: the kernels take bf16 and fp32")
     T, K = x.shape
+    if T > MOST or K > MOST:
+        raise ValueError(f"{what} of shape {(T, K)}: up to {MOST} rows and values of a row")
     return T, K, device
 
 
@@ -251,12 +256,14 @@ def _operands(rows: Fp8Rows, w) -> Tuple[torch.Tensor, torch.Tensor, int]:
         raise ValueError(f"rows {rows.shape}, weights {(n, k)} with scales {(nb, kb)}")
     if codes.get_device() != device or scale.get_device() != device:
         raise ValueError("rows, weights and scales are on one device")
+    if n > MOST:
+        raise ValueError(f"weights of shape {(n, k)}: up to {MOST} rows")
     if device >= 0:
         ld, by = codes.stride()
-        if by != 1 or ld % 16 or codes.data_ptr() % 16:
+        if by != 1 or ld % 16 or ld > MOST or codes.data_ptr() % 16:
             codes = codes.clone(memory_format=torch.contiguous_format)
-        if scale.dtype is not torch.float32 or scale.stride(1) != 1:
-            scale = scale.to(torch.float32).contiguous()
+        if scale.dtype is not torch.float32 or scale.stride(1) != 1 or scale.stride(0) > MOST:
+            scale = scale.to(torch.float32).clone(memory_format=torch.contiguous_format)
     return codes, scale, device
 
 

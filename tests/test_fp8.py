@@ -74,3 +74,24 @@ def test_refusals():
                  lambda: F8.fp8_add_rmsnorm(x, x, torch.ones(128), 1e-6)):
         with pytest.raises(ValueError):
             call()
+
+
+def test_more_rows_and_wider_strides_than_the_kernels_count():
+    """Rows, values and strides of 2^31 and more: refused, or (rows that are only read) a copy."""
+    far = lambda n, k, dtype: torch.empty(n, 2 ** 31, dtype=dtype, device="meta")[:, :k]
+    u8, one = torch.uint8, torch.zeros(1, 16)
+    near_by, spread = torch.empty(2, 16, dtype=u8, device="meta"), torch.empty(1, 16, dtype=u8, device="meta").expand(2 ** 31, 16)
+    tall = LinearWeight(torch.zeros(1, 16, dtype=u8).expand(2 ** 31, 16), fp8_scale=torch.ones(1, 1).expand(2 ** 24, 1))
+    for codes, exps in ((far(2, 16, u8), near_by[:, :1]), (near_by, far(2, 1, u8)), (spread, spread[:, :1])):
+        with pytest.raises(ValueError, match="up to"):
+            F8.Fp8Rows(codes, exps)
+    for call in (lambda: F8.fp8_rows(one.expand(2 ** 31, 16)), lambda: F8.fp8_silu_mul(one.expand(2 ** 32 + 1, 16)),
+                 lambda: F8.fp8_rows(one[:, :1].expand(1, 2 ** 31)),
+                 lambda: F8.fp8_add_rmsnorm(one.expand(2 ** 31, 16), None, torch.ones(16), 1e-6),
+                 lambda: F8.fp8_linear(some_rows(1, 16, device="cpu"), tall)):
+        with pytest.raises(ValueError, match="up to"):
+            call()
+    for dtype in (torch.bfloat16, torch.float32):
+        x = far(2, 32, dtype)
+        assert x.stride(0) == 2 ** 31 and F8._aligned(x).stride() == (32, 1)
+        assert F8._aligned(x[:1]).stride(0) == 2 ** 31                           # (one row: its stride is not used)

@@ -3,6 +3,7 @@ import pytest
 import torch
 
 from fp8_util import held, near, nearest, same, some_rows, weight
+from slopllm_b200.models.weights import LinearWeight
 from slopllm_b200.ops import fp8 as F8
 from slopllm_b200.ops import tcgen05
 
@@ -274,6 +275,23 @@ def test_a_row_is_the_same_in_any_batch():
     for i in (0, 7, 399):
         one, _ = F8.fp8_add_rmsnorm(x[i:i + 1], None, w, 1e-6)
         assert (one.codes == all_rows.codes[i:i + 1]).all() and (one.exps == all_rows.exps[i:i + 1]).all()
+
+
+def test_rows_far_apart():
+    """Strides that pass 32 bits: rows, residual, weights and their scales."""
+    step = 2 ** 31 + 64
+    space = torch.empty(2 * step, dtype=torch.uint8, device="cuda")
+    rows = torch.as_strided(torch.empty(step + 512, dtype=torch.bfloat16, device="cuda"), (2, 512), (step, 1))
+    rows.copy_(torch.randn(2, 512, generator=gen(0), device="cuda"))
+    near_by = rows.clone(memory_format=torch.contiguous_format)
+    for call in (F8.fp8_rows, F8.fp8_silu_mul, lambda x: F8.fp8_add_rmsnorm(x, None, torch.ones(512, device="cuda"), 1e-6)[0]):
+        far, close = call(rows), call(near_by)
+        assert torch.equal(far.codes, close.codes) and torch.equal(far.exps, close.exps)
+    w, _ = weight(2, 256)
+    x = some_rows(3, 256)
+    codes = torch.as_strided(space, (2, 256), (step, 1))
+    codes.copy_(w.weight.view(torch.uint8))
+    assert torch.equal(F8.fp8_linear(x, LinearWeight(codes, fp8_scale=w.fp8_scale)), F8.fp8_linear(x, w))
 
 
 def test_refusals():
