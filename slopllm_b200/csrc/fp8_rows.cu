@@ -26,14 +26,6 @@ __device__ __forceinline__ int exponent_of(double top) {
     return max(FP8_LOW, min(FP8_HIGH, e));
 }
 
-// Whether `f`, off by up to `within` of its last places, may lie on the other side of the middle between two codes.  Three bits of the significand
-// are kept; below 2^-6 codes have the steps that they have there.
-__device__ __forceinline__ bool near_middle(float f, uint32_t within) {
-    float a = fabsf(f);
-    if (a < 0.015625f) a += 0.015625f;
-    return (__float_as_uint(a) << 12) - ((0x80000u - within) << 12) <= 2 * within << 12;
-}
-
 // An fp32 number that any rounding to fewer bits takes where it would take `d`: cut off, with the last bit set where something was.
 __device__ __forceinline__ float to_odd(double d) {
     const float f = __double2float_rz(d);
@@ -47,12 +39,27 @@ __device__ __forceinline__ void put(float (&v)[4], int i, float x) {
     for (int j = 0; j < 4; ++j) v[j] = i == j ? x : v[j];
 }
 
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// Codes of four values times a factor (its bits).
+__device__ __forceinline__ uint32_t codes_of(const float (&v)[4], uint32_t factor) {
+    const float f = __uint_as_float(factor);
+    const f32x2 both = pair(f, f);
+    const float2 lo = unpair(mul2(pair(v[0], v[1]), both)), hi = unpair(mul2(pair(v[2], v[3]), both));
+    const float x[4] = {lo.x, lo.y, hi.x, hi.y};
+    return fp8_codes(x);
+}
+
 // A group in a warp, four values a lane, in fp32 off by up to `within` of their last places (0: exact).  `again(i)`: value i in 64 bits.  The lane's codes;
 // `e`: the group's exponent.  `all`: fp32 says nothing.
 template <class Again>
 __device__ __forceinline__ uint32_t quantize_group(float (&v)[4], uint32_t within, bool all, int& e, Again again) {
-    const float most = fmaxf(fmaxf(fabsf(v[0]), fabsf(v[1])), fmaxf(fabsf(v[2]), fabsf(v[3])));
-    uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(fmaxf(most, 0.f)));          // (fmaxf passes over NaN)
+    const float most = max3(max3(0.f, fabsf(v[0]), fabsf(v[1])), fabsf(v[2]), fabsf(v[3]));
+    uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));          // (max passes over NaN)
     if (top == 0x7f800000u) {                                // an infinity: a NaN from here on, and not the largest magnitude
         top = 0;
 #pragma unroll
@@ -74,21 +81,32 @@ __device__ __forceinline__ uint32_t quantize_group(float (&v)[4], uint32_t withi
         for (int o = 16; o > 0; o >>= 1) largest = fmax(largest, __shfl_xor_sync(0xffffffffu, largest, o));
         e = exponent_of(largest);
     }
-    const float down = __uint_as_float((uint32_t)(127 - e) << 23);
-    const f32x2 both = pair(down, down);
-    const float2 lo = unpair(mul2(pair(v[0], v[1]), both)), hi = unpair(mul2(pair(v[2], v[3]), both));
-    v[0] = lo.x; v[1] = lo.y; v[2] = hi.x; v[3] = hi.y;
-    bool near = all;
-    if (within != 0) near |= near_middle(v[0], within) | near_middle(v[1], within) | near_middle(v[2], within) | near_middle(v[3], within);
-    if (within != 0 && near) {
+    const uint32_t down = (uint32_t)(127 - e) << 23;
+    if (within == 0) return codes_of(v, down);
+    // The factor off by `within` / 2 + 1 places of 2^-23 either way, which is more than `within` of 2^-24 and the product's rounding: the value in 64 bits
+    // lies between the two, and where both have one code it is that one.  (A test of the product's bits for a middle took twice the instructions.)
+    const uint32_t low = codes_of(v, down - 2 * (within / 2 + 1)), high = codes_of(v, down + within / 2 + 1);
+    uint32_t codes = low;
+    if (all || low != high) {
 #pragma unroll 1
         for (int i = 0; i < 4; ++i)
-            if (all || near_middle(pick(v, i), within)) {
+            if (all || ((low ^ high) >> (8 * i) & 255u)) {
                 const double d = again(i);
-                put(v, i, fabs(d) <= (double)FLT_MAX ? to_odd(d * (double)down) : __uint_as_float(0x7fffffffu));
+                const float f = fabs(d) <= (double)FLT_MAX ? to_odd(d * (double)__uint_as_float(down)) : __uint_as_float(0x7fffffffu);
+                codes = (codes & ~(255u << (8 * i))) | (uint32_t)__nv_cvt_float_to_fp8(f, __NV_SATFINITE, __NV_E4M3) << (8 * i);
             }
     }
-    return fp8_codes(v);
+    return codes;
+}
+
+// The same without a branch, for groups that need none; true where `quantize_group` has to do it.
+__device__ __forceinline__ bool quantize_quick(const float (&v)[4], uint32_t within, int& e, uint32_t& codes) {
+    const float most = max3(max3(0.f, fabsf(v[0]), fabsf(v[1])), fabsf(v[2]), fabsf(v[3]));
+    const uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));
+    e = fp8_exponent(top);
+    const uint32_t down = (uint32_t)(127 - e) << 23;
+    codes = codes_of(v, down - 2 * (within / 2 + 1));
+    return (top == 0x7f800000u) | ((top & 0x7fffffu) - (0x600000u - within) <= 2 * within) | (codes != codes_of(v, down + within / 2 + 1));
 }
 
 template <bool F32>
@@ -198,12 +216,56 @@ __device__ __forceinline__ float rcp(float x) {
 // to gates of -16 the exponential's argument is at most 23.1, its rounding 2^-20 and that of log2(e) 3.1e-7, which makes 15; the exponential and the
 // reciprocal 4 each, the sum and two products 1 each.  Gates below -16 are made in 64 bits.
 //
-// Gated rows are bound by instructions (120 for four values of a lane: 4096 x 14336 bf16 pairs in 81 us, 3.6 TB/s), plain ones by memory (38 us, 4.6 TB/s).
+// Gated rows are bound by instructions (98 for four values of a lane, issued in two cycles of three) and by their loads in turn: 4096 x 14336 bf16 pairs
+// in 64 us, 4.6 TB/s; fp32 pairs in 83, 6.3 TB/s; plain rows in 35, 5.0 TB/s.  Where a group needs 64 bits, a vote and a call leave the way free for the
+// others (branches where each is needed: 73).  No faster, before the last instructions went (67): two tokens side by side (73), a warp with adjacent groups of a row
+// (75), the next tokens' loads between this one's results (69), five blocks an SM (73: 48 registers a thread do not hold it).
 template <bool GATED, bool F32>
 struct RowsCfg {
     static constexpr int BLOCKS = GATED ? 4 : 6;                             // resident on an SM
     static constexpr int TOKENS = F32 ? 2 : 4;                               // of a warp at a time
 };
+
+__device__ __forceinline__ void values_of(const uint4& r, float (&v)[4]) {
+    v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w);
+}
+__device__ __forceinline__ void values_of(const uint2& r, float (&v)[4]) {
+    const float2 lo = bf162_to_f2(r.x), hi = bf162_to_f2(r.y);
+    v[0] = lo.x; v[1] = lo.y; v[2] = hi.x; v[3] = hi.y;
+}
+
+constexpr uint32_t GATED_OFF = 27;                           // units of 2^-24, for gates down to
+constexpr float GATED_LOW = -16.f;
+
+__device__ __forceinline__ void activation(const float (&a)[4], const float (&u)[4], float (&v)[4]) {
+#pragma unroll
+    for (int j = 0; j < 4; j += 2) {                         // two values to an instruction
+        const f32x2 g = pair(a[j], a[j + 1]);
+        const float2 z = unpair(mul2(g, pair(-LOG2E, -LOG2E)));
+        const float2 d = unpair(add2(pair(ex2(z.x), ex2(z.y)), pair(1.f, 1.f)));
+        const float2 r = unpair(mul2(mul2(g, pair(rcp(d.x), rcp(d.y))), pair(u[j], u[j + 1])));
+        v[j] = r.x; v[j + 1] = r.y;
+    }
+}
+
+// A group of the activation where fp32 does not decide all of it (one in 200): codes and exponent.  A call, so that its registers are not the kernel's.
+template <class Raw>
+__device__ __noinline__ uint2 gated_group(Raw gate, Raw up) {
+    float a[4], u[4], v[4];
+    values_of(gate, a);
+    values_of(up, u);
+    auto again = [&](int j) {
+        const double z = pick(a, j);
+        return z / (1.0 + exp(-z)) * (double)pick(u, j);
+    };
+    activation(a, u, v);
+#pragma unroll 1
+    for (int j = 0; j < 4; ++j)
+        if (pick(a, j) < GATED_LOW) put(v, j, (float)again(j));
+    int e;
+    const uint32_t c = quantize_group(v, GATED_OFF, false, e, again);
+    return make_uint2(c, (uint32_t)e);
+}
 
 template <bool GATED, bool F32>
 __global__ void __launch_bounds__(256, RowsCfg<GATED, F32>::BLOCKS) fp8_rows_kernel(const __grid_constant__ Fp8RowsParams p, int groups, int abreast) {
@@ -214,14 +276,6 @@ __global__ void __launch_bounds__(256, RowsCfg<GATED, F32>::BLOCKS) fp8_rows_ker
     const int g = at % groups, i = g * 32 + lane;
     if (at >= groups * abreast) return;
     const Raw* const x = reinterpret_cast<const Raw*>(p.x) + i;              // (rows start at multiples of four values)
-    auto values = [](const Raw& r, float (&v)[4]) {
-        if constexpr (F32) {
-            v[0] = __uint_as_float(r.x); v[1] = __uint_as_float(r.y); v[2] = __uint_as_float(r.z); v[3] = __uint_as_float(r.w);
-        } else {
-            const float2 lo = bf162_to_f2(r.x), hi = bf162_to_f2(r.y);
-            v[0] = lo.x; v[1] = lo.y; v[2] = hi.x; v[3] = hi.y;
-        }
-    };
     for (int t0 = at / groups; t0 < p.T; t0 += TOKENS * abreast) {
         Raw gate[TOKENS], up[TOKENS];
 #pragma unroll
@@ -238,30 +292,19 @@ __global__ void __launch_bounds__(256, RowsCfg<GATED, F32>::BLOCKS) fp8_rows_ker
             const int t = t0 + b * abreast;
             if (t >= p.T) break;                             // (the same for the whole warp)
             float a[4];
-            values(gate[b], a);
+            values_of(gate[b], a);
             int e;
             uint32_t c;
             if constexpr (GATED) {
                 float u[4], v[4];
-                values(up[b], u);
-                auto again = [&](int j) {
-                    const double z = pick(a, j);
-                    return z / (1.0 + exp(-z)) * (double)pick(u, j);
-                };
-#pragma unroll
-                for (int j = 0; j < 4; j += 2) {             // two values to an instruction
-                    const f32x2 g = pair(a[j], a[j + 1]);
-                    const float2 z = unpair(mul2(g, pair(-LOG2E, -LOG2E)));
-                    const float2 d = unpair(add2(pair(ex2(z.x), ex2(z.y)), pair(1.f, 1.f)));
-                    const float2 r = unpair(mul2(mul2(g, pair(rcp(d.x), rcp(d.y))), pair(u[j], u[j + 1])));
-                    v[j] = r.x; v[j + 1] = r.y;
+                values_of(up[b], u);
+                activation(a, u, v);
+                const bool low = fminf(fminf(a[0], a[1]), fminf(a[2], a[3])) < GATED_LOW;
+                if (__any_sync(0xffffffffu, quantize_quick(v, GATED_OFF, e, c) | low)) {
+                    const uint2 r = gated_group(gate[b], up[b]);
+                    c = r.x;
+                    e = (int)r.y;
                 }
-                if (fminf(fminf(a[0], a[1]), fminf(a[2], a[3])) < -16.f) {
-#pragma unroll 1
-                    for (int j = 0; j < 4; ++j)
-                        if (pick(a, j) < -16.f) put(v, j, (float)again(j));
-                }
-                c = quantize_group(v, 27, false, e, again);
             } else {
                 c = quantize_group(a, 0, false, e, [](int) { return 0.0; });
             }

@@ -46,7 +46,7 @@ __device__ __forceinline__ bool fp8_finite(float v) { return (__float_as_uint(v)
 
 // Smallest exponent with which a magnitude (bits of an fp32 number) is at most 448 * 2^exponent, within the limits.
 __device__ __forceinline__ int fp8_exponent(uint32_t top) {
-    const int e = (int)(top >> 23) - 127 - 8 + ((top & 0x7fffffu) > 0x600000u ? 1 : 0);
+    const int e = (int)((top + 0x1fffffu) >> 23) - 127 - 8;   // (a significand above 448's carries into the exponent)
     return max(FP8_LOW, min(FP8_HIGH, e));
 }
 
