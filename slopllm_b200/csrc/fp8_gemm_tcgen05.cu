@@ -296,17 +296,6 @@ int launch_few(const void* x, int ldx, const void* W, int ldw, const Fp8LinearPa
     return rc != cudaSuccess ? (int)rc : SL_LAUNCH_CHECK();
 }
 
-// Whether pairs of SMs are the faster form.  Up to 64 rows they never are (64 by 16384 x 2048: 13.5 us without, 14.8 with them).  More: a pair takes 0.47 us
-// for a block of K of its 256 x 256 tile and 3 for what is around it, 74 run at once; 64-row tiles of one SM take 0.42 for a block and SM.
-// Microseconds without and with pairs: 128 by 6144 x 4096 15.9, 20.8; 256 by 6144 x 4096 22.2, 21.0; 128 by 24576 x 4096 41.1, 37.5; 333 by 2321 x 5136
-// 20.3, 24.4; 512 by 2048 x 2048 11.3, 13.7; 1000 by 2048 x 2048 14.2, 13.8; 1000 by 1024 x 8192 23.2, 33.1.
-bool on_pairs(int T, int N, int K) {
-    if (T <= 64) return false;
-    const long long blocks = (K + BK - 1) / BK, cols = (N + 127) / 128;
-    const long long rounds = ((long long)(T + 255) / 256 * ((N + 255) / 256) + 73) / 74;
-    return 3.f + (float)rounds * (0.47f * (float)blocks + 3.f) <= 5.5f + 0.42f / 148.f * (float)((T + 63) / 64 * cols * blocks);
-}
-
 // Blocks that share a tile's K: twice as many while every block still has an SM to itself, and on to what is resident at once (some less: clusters leave
 // SMs free) where each block keeps so many blocks of K.  Up to 16 rows, with 3 blocks an SM, microseconds with 2, 4 and 8 shares: 4096 x 4096 (32 tiles) 10.9,
 // 8.7, 8.4; 9472 x 4096 (74) 12.8, 11.6, 13.7; 12288 x 4096 (96) 14.7, 13.3, 15.5; 4096 x 14336 (32) 23.6, 16.7, 14.9; 18944 x 4096 (148) 17.7, 18.9, 20.7.  With
@@ -318,6 +307,41 @@ int shares_of(long long tiles, int blocks, int bn) {
     int shares = 1;
     while (shares < 8 && blocks >= 2 * shares && (tiles * shares * 2 <= 148 || (tiles * shares * 2 <= room && blocks >= 2 * shares * least))) shares *= 2;
     return shares;
+}
+
+long long cut(long long n, long long by) { return (n + by - 1) / by; }
+
+// Microseconds of the three forms, fitted to what they take (launch and a block of K of one tile, rounds of tiles that run at once).  One SM: tiles of 64 rows
+// by 128 columns, 296 at once, whose blocks of K take longer where two share an SM.  Pairs: 256 rows by 128 or 256 columns, 74 at once.
+float time_of_few(long long T, long long N, long long K) {
+    const long long tiles = cut(T, 64) * cut(N, 128), blocks = cut(K, BK);
+    const int shares = shares_of(tiles, (int)blocks, 64);
+    const float per = (float)blocks / (float)shares;
+    return 5.5f + (float)cut(tiles * shares, 296) * (tiles * shares <= 148 ? 0.34f * per + 1.7f : 0.5f * per + 2.7f);
+}
+float time_of_pairs(long long T, long long N, long long K, int columns) {
+    const long long blocks = cut(K, BK), rounds = cut(cut(T, 256) * cut(N, columns), 74);
+    return columns == 128 ? 5.3f + (float)rounds * (0.30f * (float)blocks + 1.4f) : 4.4f + (float)rounds * (0.43f * (float)blocks + 2.f);
+}
+
+// Columns of a pair's tile, or 0 for tiles of one SM, which are always the faster form up to 64 rows (64 by 16384 x 2048: 13.5 us, pairs 14.8).
+// Microseconds of one SM's tiles and pairs' of 128 and 256 columns: 128 by 6144 x 4096 16.6, 16.6, 20.1; 256 by 6144 x 4096 23.0, 16.6, 20.1; 128 by 24576 x
+// 4096 41.8, 38.7, 36.4; 512 by 2321 x 5136 28.8, 19.3, 23.9; 512 by 4096 x 12288 55.6, 37.6, 46.6; 512 by 2048 x 8192 24.4, 25.8, 32.8; 1000 by 2048 x 2048 14.8, 11.4,
+// 13.3; 1500 by 2048 x 8192 72, 47, 35; 4096 by 1024 x 8192 85, 51, 38.
+int pair_columns(int T, int N, int K) {
+    if (T <= 64) return 0;
+    const float few = time_of_few(T, N, K), narrow = time_of_pairs(T, N, K, 128), wide = time_of_pairs(T, N, K, 256);
+    return few <= std::min(narrow, wide) ? 0 : narrow < wide ? 128 : 256;
+}
+
+// Whether the activation of N gate and up columns is made in the pairs' epilogue (1.7 us a round), not by a pass over the fp32 rows of the product (3 us and the
+// rows' way through memory).  Microseconds with and without: 192 by 16384 x 2048 17.4, 21.3; 256 by 8192 x 4096 22.8, 20.7; 333 by 8192 x 4096 23.6, 26.6; 1000 by
+// 2048 x 8192 35.3, 31.5; 1500 by 2048 x 8192 36.1, 40.5; 65 by 2048 x 2048 14.3, 9.7.
+bool gated_on_pairs(int T, int N, int K) {
+    if (T <= 64) return false;
+    const float wide = time_of_pairs(T, N, K, 256), rounds = (float)cut(cut(T, 256) * cut(N, 256), 74);
+    const float apart = std::min(std::min(time_of_few(T, N, K), time_of_pairs(T, N, K, 128)), wide);
+    return wide + 1.7f * rounds <= apart + 3.f + 0.95e-6f * (float)T * (float)N;
 }
 
 bool aligned(const void* x, int ldx, const void* W, int ldw, const Fp8LinearParams& p) {
@@ -334,7 +358,7 @@ SL_API int sl_fp8_linear(const void* x, int ldx, const void* W, int ldw, const F
     const Fp8LinearParams& p = *params;
     if (p.T <= 0 || p.N <= 0) return 0;
     if (!aligned(x, ldx, W, ldw, p) || p.ldy % (p.out_f32 ? 4 : 8) != 0 || (p.N + 127) / 128 > 65535) return -1;
-    if (on_pairs(p.T, p.N, p.K)) return fp8_pair(x, ldx, W, ldw, p, false, s);
+    if (const int columns = pair_columns(p.T, p.N, p.K)) return fp8_pair(x, ldx, W, ldw, p, columns, s);
     const int bn = p.T <= 16 ? 16 : p.T <= 32 ? 32 : 64;
     if ((p.T + bn - 1) / bn > 65535) return -1;
     const int shares = shares_of((long long)((p.N + 127) / 128) * ((p.T + bn - 1) / bn), (p.K + BK - 1) / BK, bn);
@@ -343,13 +367,13 @@ SL_API int sl_fp8_linear(const void* x, int ldx, const void* W, int ldw, const F
     return launch_few<64>(x, ldx, W, ldw, p, shares, s);
 }
 
-// 1 where products of this size run on pairs of SMs.
-SL_API int sl_fp8_on_pairs(int T, int N, int K) { return on_pairs(T, N, K); }
+// 1 where gate and up products of this size are made with their activation (sl_fp8_gate_up).
+SL_API int sl_fp8_on_pairs(int T, int N, int K) { return gated_on_pairs(T, N, K); }
 
 // y: codes [T, N / 2] of silu(gate) * up, with exponents exps_out; W: N / 2 gate rows | N / 2 up rows, a multiple of 128 each.
 SL_API int sl_fp8_gate_up(const void* x, int ldx, const void* W, int ldw, const Fp8LinearParams* params, cudaStream_t s) {
     const Fp8LinearParams& p = *params;
     if (p.T <= 0 || p.N <= 0) return 0;
     if (!aligned(x, ldx, W, ldw, p) || p.N % 256 != 0 || p.ldy % 16 != 0) return -1;
-    return fp8_pair(x, ldx, W, ldw, p, true, s);
+    return fp8_pair_gated(x, ldx, W, ldw, p, s);
 }

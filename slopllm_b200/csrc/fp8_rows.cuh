@@ -39,8 +39,9 @@ struct Fp8LinearParams {
     int* err;
 };
 
-// Many rows, on pairs of SMs.  Gated: the activation of N / 2 gate and N / 2 up columns (a multiple of 128 each), in 8 bits.
-int fp8_pair(const void* x, int ldx, const void* W, int ldw, const Fp8LinearParams& p, bool gated, cudaStream_t s);
+// Many rows, on pairs of SMs, tiles of 256 rows by 128 or 256 columns.  Gated: the activation of N / 2 gate and N / 2 up columns (a multiple of 128 each), in 8 bits.
+int fp8_pair(const void* x, int ldx, const void* W, int ldw, const Fp8LinearParams& p, int columns, cudaStream_t s);
+int fp8_pair_gated(const void* x, int ldx, const void* W, int ldw, const Fp8LinearParams& p, cudaStream_t s);
 
 __device__ __forceinline__ bool fp8_finite(float v) { return (__float_as_uint(v) & 0x7f800000u) != 0x7f800000u; }
 

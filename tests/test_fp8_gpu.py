@@ -146,6 +146,17 @@ def test_products_of_all_sizes(t, n, k):
     tcgen05.check_errors(rows.device)
 
 
+@pytest.mark.parametrize("t,n,k", [(65, 16, 272), (192, 6144, 4096), (512, 4096, 2064), (777, 2064, 5136), (1000, 2048, 1168), (20000, 100, 400)])
+def test_products_of_narrow_tiles(t, n, k):
+    """Tiles of 128 columns on pairs of SMs: more and fewer than there are pairs, even and odd numbers of blocks of K, cut rows, columns and blocks."""
+    w, values = weight(n, k, 31, spread=3)
+    rows = some_rows(t, k, 32, spread=8)
+    y = F8.fp8_linear(rows, w, out_f32=True)
+    assert near(y, rows, values)
+    assert torch.equal(F8.fp8_linear(rows, w), y.bfloat16())
+    tcgen05.check_errors(rows.device)
+
+
 @pytest.mark.parametrize("t", [3, 50, 300])
 def test_scales_far_apart(t):
     """Exponents and scales that differ by many powers of two from block to block: a scale that meets another block would show."""
