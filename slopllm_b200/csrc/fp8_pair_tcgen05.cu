@@ -301,10 +301,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1) fp8_pair
                 uint8_t* const mine = out + (warp - 4) * 2 * PIECE;
                 const int col = n0 + half * OWN;
                 auto store = [&](auto bits, auto per) {      // `per` values to 16 bytes
+                    constexpr int PIECES = OWN / (8 * decltype(per)::value);       // (one of them: the next tile's goes where this one's is)
 #pragma unroll
                     for (int c = 0; c < OWN; c += 8 * per) {
                         uint8_t* const here = mine + c / (8 * per) % 2 * PIECE;
-                        if (lane == 0) bulk_read<1>();       // (what was in it is out: at most the other one is still on its way)
+                        if (lane == 0) bulk_read<PIECES == 1 ? 0 : 1>();       // (what was in it is out: at most the other one is still on its way)
                         __syncwarp();
 #pragma unroll
                         for (int j = 0; j < 8; ++j) *piece(here, j) = bits(c + j * per);

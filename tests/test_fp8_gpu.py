@@ -157,6 +157,18 @@ def test_products_of_narrow_tiles(t, n, k):
     tcgen05.check_errors(rows.device)
 
 
+@pytest.mark.parametrize("t,n,k", [(150000, 112, 16), (90000, 64, 144)])
+def test_tiles_that_follow_each_other(t, n, k):
+    """Tiles of one or two blocks of K, several of a pair: a result is on its way out when the next one is written."""
+    w, values = weight(n, k, 33)
+    rows = some_rows(t, k, 34)
+    want = F8.fp8_linear(rows, w, out_f32=True)
+    assert near(want, rows, values)
+    want = want.bfloat16()
+    assert all(torch.equal(F8.fp8_linear(rows, w), want) for _ in range(20))
+    tcgen05.check_errors(rows.device)
+
+
 @pytest.mark.parametrize("t", [3, 50, 300])
 def test_scales_far_apart(t):
     """Exponents and scales that differ by many powers of two from block to block: a scale that meets another block would show."""
