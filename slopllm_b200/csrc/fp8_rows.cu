@@ -177,7 +177,7 @@ __global__ void __launch_bounds__(1024, 1) fp8_norm_kernel(const __grid_constant
     __syncthreads();
     const double inv = sums[32];
     const float inv32 = (float)inv;
-    const bool all = !(inv < 1e30);                      // (beyond fp32, or no number)
+    const bool all = !(inv < 1e30 && inv > 1.2e-38);     // (beyond fp32 or below 2^-126, where its last place is 4 units of 2^-24 and more, or no number)
 #pragma unroll
     for (int q = 0; q < Q; ++q) {
         const int i = threadIdx.x + q * nt;

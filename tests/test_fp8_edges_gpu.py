@@ -1,0 +1,51 @@
+"""Rows in 8 bits and their products on a GPU where they are easily wrong: numbers by the limits of fp32, status words that a captured call makes, strides, what lies
+around results, and the activation that is made in a product's epilogue."""
+import numpy as np
+import pytest
+import torch
+
+from fp8_util import held, near, nearest, same, some_rows, weight
+from slopllm_b200.models.weights import LinearWeight
+from slopllm_b200.ops import fp8 as F8
+from slopllm_b200.ops import native as N
+from slopllm_b200.ops import tcgen05
+
+pytestmark = pytest.mark.gpu
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def silu_mul(gu):
+    g, u = gu.double().chunk(2, -1)
+    return g / (1 + torch.exp(-g)) * u
+
+
+def rms(r, w, eps):
+    v = r.double()
+    return v * torch.rsqrt(v.square().mean(-1, keepdim=True) + eps) * w.double()
+
+
+# ---- numbers by the limits of fp32 -------------------------------------------------------------------------------------------------
+
+def test_norms_whose_factor_is_subnormal():
+    """Rows of 3e38: 1 / rms lies below 2^-126, where fp32 has fewer bits.  Gains put every value next to the middle between two codes."""
+    g, largest, h = np.random.default_rng(2), np.finfo(np.float32).max, 4096
+    shape, rows = g.uniform(0.99, 1.0, h), 0
+    for size in np.linspace(0.9, 1.0, 4000):
+        v = (shape * size * largest).astype(np.float32)
+        inv = 1 / np.sqrt(np.mean(v.astype(np.float64) ** 2))
+        if abs(np.float64(np.float32(inv)) / inv - 1) < 3.75 * 2.0 ** -24:
+            continue
+        middles = (1 + (g.integers(0, 2, h) + 0.5) / 8) * 2.0 ** g.integers(3, 8, h)
+        w = torch.from_numpy((middles / (v.astype(np.float64) * inv)).astype(np.float32)).cuda()
+        x = torch.from_numpy(v).cuda()[None]
+        got, _ = F8.fp8_add_rmsnorm(x, None, w, 0.0)
+        assert same(got, rms(x, w, 0.0)), size
+        rows += 1
+    assert rows > 50
+    x = torch.randn(300, 1040, generator=gen(0), device="cuda").clamp(-3, 3) * 1e38
+    w = torch.randn(1040, generator=gen(1), device="cuda")
+    for weight_type in (torch.float32, torch.bfloat16):
+        assert same(F8.fp8_add_rmsnorm(x, None, w.to(weight_type), 1e-6)[0], rms(x, w.to(weight_type), 1e-6))
