@@ -243,7 +243,9 @@ __device__ __forceinline__ void activation(const float (&a)[4], const float (&u)
         const f32x2 g = pair(a[j], a[j + 1]);
         const float2 z = unpair(mul2(g, pair(-LOG2E, -LOG2E)));
         const float2 d = unpair(add2(pair(ex2(z.x), ex2(z.y)), pair(1.f, 1.f)));
-        const float2 r = unpair(mul2(mul2(g, pair(rcp(d.x), rcp(d.y))), pair(u[j], u[j + 1])));
+        // `up` before the gate: where a product with `up` leaves the normal range, the gate is above 17 and the reciprocal 1, or the result is below every code
+        // (a gate next to 0 left it before a large `up` brought it back)
+        const float2 r = unpair(mul2(mul2(pair(rcp(d.x), rcp(d.y)), pair(u[j], u[j + 1])), g));
         v[j] = r.x; v[j + 1] = r.y;
     }
 }

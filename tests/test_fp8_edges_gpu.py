@@ -49,3 +49,12 @@ def test_norms_whose_factor_is_subnormal():
     w = torch.randn(1040, generator=gen(1), device="cuda")
     for weight_type in (torch.float32, torch.bfloat16):
         assert same(F8.fp8_add_rmsnorm(x, None, w.to(weight_type), 1e-6)[0], rms(x, w.to(weight_type), 1e-6))
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gates_that_are_subnormal(dtype):
+    """silu(gate) below 2^-126 times a large value, and the other way round."""
+    size = torch.exp2(torch.rand(64, 512, generator=gen(2), device="cuda") * 14 - 138)
+    gate = size * torch.where(torch.rand(64, 512, generator=gen(3), device="cuda") < 0.5, -1.0, 1.0)
+    up = torch.randn(64, 512, generator=gen(4), device="cuda").clamp(-3, 3) * 1e38
+    for gu in (torch.cat([gate, up], 1), torch.cat([up.abs(), gate], 1)):
+        assert same(F8.fp8_silu_mul(gu.to(dtype)), silu_mul(gu.to(dtype)))
