@@ -7,8 +7,8 @@
 // the largest magnitude's own bits and on nothing that a division could round.  A value that fp32 does not hold as a finite number is the NaN
 // code; magnitudes above 448 * 2^60 saturate.  Exponent rows start at multiples of 16 bytes: the product reads sixteen groups at a time.
 //
-// Codes are the nearest ones of the definition in 64 bits (where products stay in the normal range of fp32).  fp32 decides all but the values that lie
-// within its error of the middle between two codes; those are made again in 64 bits.
+// Codes are the nearest ones of the definition in 64 bits.  fp32 decides all but the values that lie within its error of the middle between two codes or that
+// it does not hold; those are made again in 64 bits.
 #include <algorithm>
 #include <type_traits>
 
@@ -191,8 +191,9 @@ __global__ void __launch_bounds__(1024, 1) fp8_norm_kernel(const __grid_constant
 #pragma unroll
         for (int j = 0; j < 4; ++j) f[j] = v[q][j] * inv32 * w[j];
         int e;
-        // three roundings to fp32 (the factor's, two products'): at most 3 last places
-        const uint32_t c = quantize_group(f, 4, all, e, [&](int j) { return (double)pick(v[q], j) * inv * (double)pick(w, j); });
+        // three roundings to fp32 (the factor's, two products'): at most 3 last places, unless a gain of 2^54 or more brings back what was below 2^-126
+        const bool far = __any_sync(0xffffffffu, fmaxf(max3(fabsf(w[0]), fabsf(w[1]), fabsf(w[2])), fabsf(w[3])) >= 0x1p54f);
+        const uint32_t c = quantize_group(f, 4, all || far, e, [&](int j) { return (double)pick(v[q], j) * inv * (double)pick(w, j); });
         if (i < n4) reinterpret_cast<uint32_t*>(p.codes + (size_t)t * p.ldc)[i] = c;
         if (lane == 0) p.exps[(size_t)t * p.lde + i / 32] = (uint8_t)(e + FP8_BIAS);
     }

@@ -58,3 +58,14 @@ def test_gates_that_are_subnormal(dtype):
     up = torch.randn(64, 512, generator=gen(4), device="cuda").clamp(-3, 3) * 1e38
     for gu in (torch.cat([gate, up], 1), torch.cat([up.abs(), gate], 1)):
         assert same(F8.fp8_silu_mul(gu.to(dtype)), silu_mul(gu.to(dtype)))
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_gains_that_bring_tiny_values_back(dtype):
+    """Values 2^-140 of the row's size, times gains of 2^126."""
+    x = torch.randn(20, 1024, generator=gen(5), device="cuda")
+    x[:, 128:] *= 2.0 ** -140
+    w = torch.randn(1024, generator=gen(6), device="cuda").clamp(-3, 3)
+    w[128:] *= 2.0 ** 126
+    x, w = x.to(dtype), w.to(dtype)
+    for size in (1.0, 2.0 ** 40):
+        assert same(F8.fp8_add_rmsnorm(x.float() * size, None, w, 0.0)[0], rms(x.float() * size, w, 0.0))
