@@ -18,6 +18,7 @@
 namespace {
 
 constexpr float LOG2E = 1.4426950408889634f;
+constexpr uint32_t INFINITE = 0x7f800000u;                   // bits
 
 // Smallest exponent with which a magnitude is at most 448 * 2^exponent, within the limits.
 __device__ __forceinline__ int exponent_of(double top) {
@@ -60,7 +61,8 @@ template <class Again>
 __device__ __forceinline__ uint32_t quantize_group(float (&v)[4], uint32_t within, bool all, int& e, Again again) {
     const float most = max3(max3(0.f, fabsf(v[0]), fabsf(v[1])), fabsf(v[2]), fabsf(v[3]));
     uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));          // (max passes over NaN)
-    if (top == 0x7f800000u) {                                // an infinity: a NaN from here on, and not the largest magnitude
+    if (within != 0) all |= top >= INFINITE - within - 1;    // (64 bits say which of them fp32 holds)
+    if (top == INFINITE) {                                // an infinity: a NaN from here on, and not the largest magnitude
         top = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
@@ -75,7 +77,7 @@ __device__ __forceinline__ uint32_t quantize_group(float (&v)[4], uint32_t withi
 #pragma unroll 1
         for (int i = 0; i < 4; ++i) {
             const double d = fabs(again(i));
-            if (d <= (double)FLT_MAX) largest = fmax(largest, d);
+            if (fp8_finite((float)d)) largest = fmax(largest, d);
         }
 #pragma unroll
         for (int o = 16; o > 0; o >>= 1) largest = fmax(largest, __shfl_xor_sync(0xffffffffu, largest, o));
@@ -92,7 +94,7 @@ __device__ __forceinline__ uint32_t quantize_group(float (&v)[4], uint32_t withi
         for (int i = 0; i < 4; ++i)
             if (all || ((low ^ high) >> (8 * i) & 255u)) {
                 const double d = again(i);
-                const float f = fabs(d) <= (double)FLT_MAX ? to_odd(d * (double)__uint_as_float(down)) : __uint_as_float(0x7fffffffu);
+                const float f = fp8_finite((float)d) ? to_odd(d * (double)__uint_as_float(down)) : __uint_as_float(0x7fffffffu);
                 codes = (codes & ~(255u << (8 * i))) | (uint32_t)__nv_cvt_float_to_fp8(f, __NV_SATFINITE, __NV_E4M3) << (8 * i);
             }
     }
@@ -106,7 +108,7 @@ __device__ __forceinline__ bool quantize_quick(const float (&v)[4], uint32_t wit
     e = fp8_exponent(top);
     const uint32_t down = (uint32_t)(127 - e) << 23;
     codes = codes_of(v, down - 2 * (within / 2 + 1));
-    return (top == 0x7f800000u) | ((top & 0x7fffffu) - (0x600000u - within) <= 2 * within) | (codes != codes_of(v, down + within / 2 + 1));
+    return (top >= INFINITE - within - 1) | ((top & 0x7fffffu) - (0x600000u - within) <= 2 * within) | (codes != codes_of(v, down + within / 2 + 1));
 }
 
 template <bool F32>

@@ -69,3 +69,25 @@ def test_gains_that_bring_tiny_values_back(dtype):
     x, w = x.to(dtype), w.to(dtype)
     for size in (1.0, 2.0 ** 40):
         assert same(F8.fp8_add_rmsnorm(x.float() * size, None, w, 0.0)[0], rms(x.float() * size, w, 0.0))
+
+def test_products_by_the_largest_number():
+    """Gate times up where fp32 rounds to infinity and 64 bits to the largest finite number: a code, not NaN; beyond it, NaN."""
+    limit = (2 - 2.0 ** -24) * 2.0 ** 127                 # from here on fp32 has infinity
+    g = np.random.default_rng(0)
+    gate = g.uniform(16.7, 24, 4096).astype(np.float32)
+    up = (limit / gate.astype(np.float64)).astype(np.float32)
+    up = np.stack([np.nextafter(up, np.float32(0)), up, np.nextafter(up, np.float32(np.inf))])
+    d = gate.astype(np.float64) / (1 + np.exp(-gate.astype(np.float64))) * up
+    with np.errstate(over="ignore"):
+        assert (np.isinf(gate * up) & (d < limit)).any()
+    rows = torch.from_numpy(np.concatenate([np.stack([gate] * 3), up], 1)).cuda()
+    assert same(F8.fp8_silu_mul(rows), silu_mul(rows))
+    # the norm: rows of one large value, gains that take it there
+    x = torch.zeros(1, 256, device="cuda")
+    x[0, 5] = 3.0
+    for step in range(-3, 4):
+        w = torch.ones(256, device="cuda")
+        w[5] = float(np.float32(limit / 16)) * (1 + step * 2.0 ** -23)
+        for value in (3.0, 1.7, 1.1):
+            x[0, 5] = value
+            assert same(F8.fp8_add_rmsnorm(x, None, w, 0.0)[0], rms(x, w, 0.0))
