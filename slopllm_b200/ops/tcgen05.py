@@ -6,6 +6,7 @@ import torch
 from . import native as N
 
 _err = {}
+_filled = {}            # per device: event behind the zeros of words that were made while a graph was being captured
 _reset_hooks = {}
 
 ERROR_WORDS = 16        # [0] tcgen05 expired wait, [4..7] index self-check, [8..11] persistent-kernel wait, [12..15] collective wait
@@ -16,7 +17,17 @@ def error_flag(device) -> torch.Tensor:
     fails: one place, so that the engine reads everything back with the step's result in a single copy."""
     key = torch.device(device).index or 0
     if key not in _err:
-        _err[key] = torch.zeros(ERROR_WORDS, dtype=torch.int32, device=device)
+        words = _err[key] = torch.empty(ERROR_WORDS, dtype=torch.int32, device=device)
+        if words.is_cuda and torch.cuda.is_current_stream_capturing():
+            # not by the stream that is captured: each replay would clear what its kernels have reported
+            with torch.cuda.stream(torch.cuda.Stream(device)):
+                words.zero_()
+                _filled[key] = torch.cuda.Event()
+                _filled[key].record()
+        else:
+            words.zero_()
+    elif key in _filled and not torch.cuda.is_current_stream_capturing():
+        torch.cuda.current_stream(device).wait_event(_filled.pop(key))
     return _err[key]
 
 

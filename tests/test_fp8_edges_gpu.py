@@ -91,3 +91,26 @@ def test_products_by_the_largest_number():
         for value in (3.0, 1.7, 1.1):
             x[0, 5] = value
             assert same(F8.fp8_add_rmsnorm(x, None, w, 0.0)[0], rms(x, w, 0.0))
+
+
+# ---- status words, strides, what lies around results -----------------------------------------------------------------------------------
+
+def test_status_words_that_a_captured_call_makes(monkeypatch):
+    """A device's first call may be a captured one.  A replay leaves what a kernel has written into the status words."""
+    rows, (w, _) = some_rows(4, 256), weight(64, 256)
+    F8.fp8_linear(rows, w)
+    monkeypatch.setattr(tcgen05, "_err", {})
+    monkeypatch.setattr(F8, "_status", lambda device: tcgen05.error_flag(torch.device("cuda", device)).data_ptr())
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        F8.fp8_linear(rows, w)
+    words = tcgen05.error_flag(rows.device)
+    assert words.tolist() == [0] * tcgen05.ERROR_WORDS
+    words[0] = 7
+    graph.replay()
+    assert words[0] == 7
+    with pytest.raises(N.NativeError, match="site 7"):
+        tcgen05.check_errors(rows.device)
+    assert words.tolist() == [0] * tcgen05.ERROR_WORDS
