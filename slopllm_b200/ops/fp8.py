@@ -246,6 +246,14 @@ def fp8_add_rmsnorm(x: torch.Tensor, residual: Optional[torch.Tensor], w: torch.
 
 # ---- products ----------------------------------------------------------------------------------------------------------------------------
 
+def _scales(scale: torch.Tensor) -> torch.Tensor:
+    """Scales that the kernels take: a copy where they are no fp32, not side by side, or rows lie in one another or too far apart."""
+    ld, by = scale.stride()
+    if scale.dtype is torch.float32 and by == 1 and scale.shape[1] <= ld <= MOST:
+        return scale
+    return scale.to(torch.float32).clone(memory_format=torch.contiguous_format)
+
+
 def _operands(rows: Fp8Rows, w) -> Tuple[torch.Tensor, torch.Tensor, int]:
     """Codes and scales of FP8 weights, checked and (on a GPU) as the kernels take them, and the device's number."""
     codes, scale = w.weight, w.fp8_scale
@@ -262,8 +270,7 @@ def _operands(rows: Fp8Rows, w) -> Tuple[torch.Tensor, torch.Tensor, int]:
         ld, by = codes.stride()
         if by != 1 or ld % 16 or ld > MOST or codes.data_ptr() % 16:
             codes = codes.clone(memory_format=torch.contiguous_format)
-        if scale.dtype is not torch.float32 or scale.stride(1) != 1 or scale.stride(0) > MOST:
-            scale = scale.to(torch.float32).clone(memory_format=torch.contiguous_format)
+        scale = _scales(scale)
     return codes, scale, device
 
 

@@ -114,3 +114,18 @@ def test_status_words_that_a_captured_call_makes(monkeypatch):
     with pytest.raises(N.NativeError, match="site 7"):
         tcgen05.check_errors(rows.device)
     assert words.tolist() == [0] * tcgen05.ERROR_WORDS
+
+@pytest.mark.parametrize("t", [3, 200])
+def test_scales_whose_rows_lie_in_one_another(t):
+    """Scales that are one row for all blocks, a single row with a stride of its own, windows that overlap: as their contiguous copies."""
+    (w, _), rows = weight(300, 400, 20), some_rows(t, 400, 21)
+    s = w.fp8_scale
+    for scale in (s[:1].expand(3, 4), s.flatten()[:8].as_strided((3, 4), (2, 1)), s.flatten()[:8].as_strided((3, 4), (1, 2))):
+        got = F8.fp8_linear(rows, LinearWeight(w.weight, fp8_scale=scale), out_f32=True)
+        assert torch.equal(got, F8.fp8_linear(rows, LinearWeight(w.weight, fp8_scale=scale.contiguous()), out_f32=True))
+    few = LinearWeight(w.weight[:100], fp8_scale=s[:1].as_strided((1, 4), (1, 1)))
+    assert torch.equal(F8.fp8_linear(rows, few), F8.fp8_linear(rows, LinearWeight(w.weight[:100], fp8_scale=s[:1].clone())))
+    gated, _ = weight(512, 400, 22)
+    scale = gated.fp8_scale[:1].expand(4, 4)
+    got, want = (F8.fp8_gate_up(rows, LinearWeight(gated.weight, fp8_scale=x)) for x in (scale, scale.contiguous()))
+    assert torch.equal(got.codes, want.codes) and torch.equal(got.exps, want.exps)
