@@ -246,6 +246,14 @@ def fp8_add_rmsnorm(x: torch.Tensor, residual: Optional[torch.Tensor], w: torch.
 
 # ---- products ----------------------------------------------------------------------------------------------------------------------------
 
+def _codes(codes: torch.Tensor) -> torch.Tensor:
+    """Weights that the kernels take: a copy where rows do not start at multiples of 16 bytes, or lie in one another or too far apart."""
+    ld, by = codes.stride()
+    if by == 1 and ld % 16 == 0 and codes.shape[1] <= ld <= MOST and codes.data_ptr() % 16 == 0:
+        return codes
+    return codes.clone(memory_format=torch.contiguous_format)
+
+
 def _scales(scale: torch.Tensor) -> torch.Tensor:
     """Scales that the kernels take: a copy where they are no fp32, not side by side, or rows lie in one another or too far apart."""
     ld, by = scale.stride()
@@ -267,10 +275,7 @@ def _operands(rows: Fp8Rows, w) -> Tuple[torch.Tensor, torch.Tensor, int]:
     if n > MOST:
         raise ValueError(f"weights of shape {(n, k)}: up to {MOST} rows")
     if device >= 0:
-        ld, by = codes.stride()
-        if by != 1 or ld % 16 or ld > MOST or codes.data_ptr() % 16:
-            codes = codes.clone(memory_format=torch.contiguous_format)
-        scale = _scales(scale)
+        codes, scale = _codes(codes), _scales(scale)
     return codes, scale, device
 
 

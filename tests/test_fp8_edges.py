@@ -20,3 +20,14 @@ def test_scales_that_the_kernels_take():
     rows, scale = some_rows(5, 400, device="cpu"), w.fp8_scale[:1].expand(3, 4)
     values = values / w.fp8_scale.double().repeat_interleave(128, 0)[:300].repeat_interleave(128, 1)[:, :400]
     assert near(F8.fp8_linear(rows, LinearWeight(w.weight, fp8_scale=scale), out_f32=True), rows, values * scale[:1].double().repeat_interleave(128, 1)[:, :400])
+
+
+def test_weights_that_the_kernels_take():
+    w = torch.zeros(64, 256, dtype=torch.uint8)
+    assert F8._codes(w) is w and F8._codes(part := w[3:40:2, 16:160]) is part
+    w.copy_(torch.arange(64 * 256).view(64, 256) % 251)
+    for codes in (w[:1].expand(64, 256), w.flatten().as_strided((64, 256), (16, 1)), w[:1].as_strided((1, 256), (16, 1)), w[:, :144].t().contiguous().t(),
+                  torch.zeros(64, 264, dtype=torch.uint8)[:, :256]):
+        got = F8._codes(codes)
+        assert got.stride() == (codes.shape[1], 1) and torch.equal(got, codes)
+    assert F8._codes(torch.empty(2, 2 ** 31, dtype=torch.uint8, device="meta")[:, :256]).stride() == (256, 1)

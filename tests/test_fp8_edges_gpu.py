@@ -129,3 +129,14 @@ def test_scales_whose_rows_lie_in_one_another(t):
     scale = gated.fp8_scale[:1].expand(4, 4)
     got, want = (F8.fp8_gate_up(rows, LinearWeight(gated.weight, fp8_scale=x)) for x in (scale, scale.contiguous()))
     assert torch.equal(got.codes, want.codes) and torch.equal(got.exps, want.exps)
+
+@pytest.mark.parametrize("t", [3, 200])
+def test_weights_whose_rows_lie_in_one_another(t):
+    """One row for all columns, windows of a longer row, a single row with a stride of its own."""
+    (w, _), rows = weight(256, 400, 23), some_rows(t, 400, 24)
+    codes = w.weight.view(torch.uint8)
+    for part in (codes[:1].expand(256, 400), codes.flatten().as_strided((256, 400), (16, 1)), codes[:1].as_strided((1, 400), (16, 1))):
+        scale = w.fp8_scale[:-(-part.shape[0] // 128)]
+        got = F8.fp8_linear(rows, LinearWeight(part, fp8_scale=scale), out_f32=True)
+        assert torch.equal(got, F8.fp8_linear(rows, LinearWeight(part.clone(memory_format=torch.contiguous_format), fp8_scale=scale), out_f32=True))
+    tcgen05.check_errors(rows.device)
