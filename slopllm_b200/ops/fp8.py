@@ -23,6 +23,7 @@ from . import native as N, quant, tcgen05
 GROUP = 128
 LOW, HIGH, BIAS = -60, 60, 127         # limits of the exponent, and what is added to it in its byte
 MAX_NORM = 16384                       # values of a row that the norm takes on a GPU
+MAX_COLUMNS = 65535 * 128              # columns of a product on a GPU (a grid's second extent)
 MOST = 2 ** 31 - 2 ** 20               # rows, values of a row, values from row to row: the kernels count them, and some steps beyond, in 32 bits
 
 
@@ -272,8 +273,9 @@ def _operands(rows: Fp8Rows, w) -> Tuple[torch.Tensor, torch.Tensor, int]:
         raise ValueError(f"rows {rows.shape}, weights {(n, k)} with scales {(nb, kb)}")
     if codes.get_device() != device or scale.get_device() != device:
         raise ValueError("rows, weights and scales are on one device")
-    if n > MOST:
-        raise ValueError(f"weights of shape {(n, k)}: up to {MOST} rows")
+    most = MOST if device < 0 else MAX_COLUMNS
+    if n > most:
+        raise ValueError(f"weights of shape {(n, k)}: up to {most} rows")
     if device >= 0:
         codes, scale = _codes(codes), _scales(scale)
     return codes, scale, device

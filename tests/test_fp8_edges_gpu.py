@@ -140,3 +140,14 @@ def test_weights_whose_rows_lie_in_one_another(t):
         got = F8.fp8_linear(rows, LinearWeight(part, fp8_scale=scale), out_f32=True)
         assert torch.equal(got, F8.fp8_linear(rows, LinearWeight(part.clone(memory_format=torch.contiguous_format), fp8_scale=scale), out_f32=True))
     tcgen05.check_errors(rows.device)
+
+def test_more_columns_than_a_grid_has():
+    """Refused in words, and not copied before."""
+    n = 65535 * 128 + 1
+    codes = torch.zeros(1, 16, dtype=torch.uint8, device="cuda").expand(n, 16)
+    w = LinearWeight(codes, fp8_scale=torch.ones(1, 1, device="cuda").expand(65536, 1))
+    for t in (1, 100):
+        with pytest.raises(ValueError, match="up to 8388480"):
+            F8.fp8_linear(some_rows(t, 16), w)
+    y = F8.fp8_linear(some_rows(1, 16), LinearWeight(codes[1:].contiguous(), fp8_scale=w.fp8_scale[1:]))
+    assert y.shape == (1, n - 1) and (y == 0).all()
