@@ -152,20 +152,24 @@ def plan_memory(cfg: GlmMoeDsaConfig, world: int = 1, cp: bool = False, ep: bool
 def dense_weight_bytes(cfg, tp: int = 1, elem: int = 2, fp8: bool = False) -> int:
     """Per-rank weight bytes of a Qwen3 / Qwen3.5 decoder: attention and Gated-DeltaNet projections head-sharded, MLP
     column / row sharded, embedding whole, lm_head vocabulary-sharded.  `fp8`: the attention and MLP projections stay FP8
-    (one byte per weight + one fp32 scale per 128 x 128 block)."""
+    (one byte per weight + one fp32 scale per 128 x 128 block) where the loader keeps them: shards end on a block's edge, and so does each
+    part of a fused matrix but the last.  (Where they do not, the last rank's may; rank 0's, which is counted, does not.)"""
     H, I, hd = cfg.hidden_size, cfg.intermediate_size, cfg.head_dim
 
     def lin(n, k, quant=False):
         return n * k + (-(-n // 128)) * (-(-k // 128)) * 4 if quant else n * k * elem
+
+    def whole(*parts):                                              # a rank's rows (or columns) of one matrix
+        return fp8 and all(n % 128 == 0 for n in (parts if tp > 1 else parts[:-1]))
     b = cfg.vocab_size * H * elem + H * elem
     b += (cfg.vocab_size // tp) * H * elem                         # the head's shard is materialised even when it is tied
     for kind in cfg.layer_types:
         b += 2 * H * elem                                           # the two layer norms
-        b += lin(2 * I // tp, H, fp8) + lin(H, I // tp, fp8)
+        b += lin(2 * (I // tp), H, whole(I // tp, I // tp)) + lin(H, I // tp, whole(I // tp))
         if kind == "full_attention":
             qs = hd * (2 if cfg.attn_output_gate else 1)
             hq, hk = cfg.num_attention_heads // tp, max(1, cfg.num_key_value_heads // tp)
-            b += lin(hq * qs + 2 * hk * hd, H, fp8) + lin(H, hq * hd, fp8) + 2 * hd * elem      # qkv, o_proj, q/k norms
+            b += lin(hq * qs + 2 * hk * hd, H, whole(hq * qs, hk * hd, hk * hd)) + lin(H, hq * hd, whole(hq * hd)) + 2 * hd * elem      # qkv, o_proj, q/k norms
         else:
             lh, dk, dv = cfg.linear_num_key_heads // tp, cfg.linear_key_head_dim, cfg.linear_value_head_dim
             conv_dim = lh * (2 * dk + dv)

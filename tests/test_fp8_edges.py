@@ -31,3 +31,29 @@ def test_weights_that_the_kernels_take():
         got = F8._codes(codes)
         assert got.stride() == (codes.shape[1], 1) and torch.equal(got, codes)
     assert F8._codes(torch.empty(2, 2 ** 31, dtype=torch.uint8, device="meta")[:, :256]).stride() == (256, 1)
+
+
+def test_plans_count_what_loaders_expand():
+    """Weights of a rank against the plan: projections that end on the edges of blocks, shards and parts of fused matrices that do not."""
+    from slopllm_b200.models.dense import DenseConfig, random_dense_model
+    from slopllm_b200.runtime.workspace import walk_tensors
+    from slopllm_b200.utils.sizing import dense_weight_bytes
+    configs = [dict(hidden_size=256, intermediate_size=512, num_attention_heads=4, num_key_value_heads=4, head_dim=64),
+               dict(hidden_size=272, intermediate_size=1216, num_attention_heads=8, num_key_value_heads=2, head_dim=64),
+               dict(hidden_size=128, intermediate_size=192, num_attention_heads=2, num_key_value_heads=2, head_dim=32),
+               dict(hidden_size=400, intermediate_size=1024, num_attention_heads=6, num_key_value_heads=2, head_dim=128)]
+    some = set()
+    for cfg in [DenseConfig(num_hidden_layers=2, vocab_size=512, **c) for c in configs] + [DenseConfig.tiny(), DenseConfig.tiny(hybrid=True)]:
+        for tp in (1, 2):
+            w, _ = random_dense_model(cfg, 0, "cpu", torch.bfloat16, 0, tp, fp8=True)
+            seen, total = set(), [0]
+
+            def add(t):
+                if t.data_ptr() not in seen:
+                    seen.add(t.data_ptr())
+                    total[0] += t.numel() * t.element_size()
+            walk_tensors(w, add)
+            assert dense_weight_bytes(cfg, tp, fp8=True) == total[0], (cfg, tp)
+            layer = w.layers[-1]
+            some.add((layer.w_qkv.is_fp8, layer.o_proj.is_fp8, layer.mlp_w13.is_fp8, layer.mlp_w2.is_fp8))
+    assert len(some) > 3
