@@ -165,12 +165,13 @@ def _refuse_act_dtype(args, ctx: ParallelContext, reg, model_type: str, raw: dic
         raise SystemExit(f"{args.model}: {model_type} does not take activations in {act_dtype}")
     from ..checkpoint.safetensors_io import SafetensorsFile
     from ..models.dense import DenseConfig, check_act_dtype, has_fp8_projections
+    cfg = DenseConfig.from_hf_dict(raw)
     try:
-        check_act_dtype(DenseConfig.from_hf_dict(raw), act_dtype, ctx.world, ctx.device.type == "cuda")
+        check_act_dtype(cfg, act_dtype, ctx.world, ctx.device.type == "cuda")
     except ValueError as e:
         raise SystemExit(f"{args.model}: {e}")
     shards = (os.path.join(model_dir, f) for f in sorted(os.listdir(model_dir)) if f.endswith(".safetensors"))
-    if not any(has_fp8_projections(SafetensorsFile(f).names()) for f in shards):
+    if not any(has_fp8_projections(cfg, SafetensorsFile(f).names()) for f in shards):
         raise SystemExit(f"{args.model}: activations in 8 bits go with FP8 projections, and this checkpoint has none")
 
 

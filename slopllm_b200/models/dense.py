@@ -181,9 +181,13 @@ def check_act_dtype(cfg: DenseConfig, act_dtype: Optional[str], tp: int = 1, on_
         raise ValueError(f"activations in 8 bits come in rows of up to {F8.MAX_NORM} values on a GPU, not {cfg.hidden_size}")
 
 
-def has_fp8_projections(names) -> bool:
-    """Whether a checkpoint's tensor names say that projections are FP8 with a scale per block."""
-    return any(n.endswith("_proj.weight_scale_inv") for n in names)
+ROWS_IN_FP8 = tuple(f"{x}_proj.weight_scale_inv" for x in ("self_attn.q", "self_attn.k", "self_attn.v", "self_attn.o", "mlp.gate", "mlp.up"))
+
+
+def has_fp8_projections(cfg: DenseConfig, names) -> bool:
+    """Whether a checkpoint's tensor names say that projections whose rows come in 8 bits are FP8 with a scale per block (those of recurrent layers are
+    expanded, those of other towers not loaded, and a down projection by itself takes the rows of gate and up as they are)."""
+    return any(n.startswith(cfg.weight_prefix + "layers.") and n.endswith(ROWS_IN_FP8) for n in names)
 
 
 def dense_cache_specs(cfg: DenseConfig, tp: int = 1, kv_dtype: Optional[str] = None) -> List[CacheSpec]:
@@ -481,7 +485,7 @@ def load_dense_model(model_dir: str, ctx: Optional[ParallelContext] = None, dtyp
             for name in sf.names():
                 if not name.startswith("model.visual."):
                     tensors[name] = sf.tensor(name)
-    if act_dtype is not None and not has_fp8_projections(tensors):
+    if act_dtype is not None and not has_fp8_projections(cfg, tensors):
         raise ValueError(f"{model_dir}: activations in 8 bits go with FP8 projections, and this checkpoint has none")
     w = assemble_dense_weights(cfg, tensors, ctx.device, dtype, ctx.rank if ctx.world > 1 else 0, ctx.world, keep_fp8=None if act_dtype is None else True)
     return cfg, DenseModel(cfg, w, ctx, kv_dtype=kv_dtype, act_dtype=act_dtype)

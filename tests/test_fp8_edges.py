@@ -57,3 +57,60 @@ def test_plans_count_what_loaders_expand():
             layer = w.layers[-1]
             some.add((layer.w_qkv.is_fp8, layer.o_proj.is_fp8, layer.mlp_w13.is_fp8, layer.mlp_w2.is_fp8))
     assert len(some) > 3
+
+
+def fp8_checkpoint(path, cfg, keep):
+    """A checkpoint of `cfg` whose projections named by `keep` are FP8, others bf16."""
+    import json
+    import struct
+    from slopllm_b200.models.dense import random_dense_model
+    from slopllm_b200.ops import dense as D
+    _, tensors = random_dense_model(cfg, seed=3, device="cpu", dtype=torch.bfloat16)
+    for name in [n for n in tensors if any(n.endswith(k + ".weight") for k in keep)]:
+        tensors[name], tensors[name + "_scale_inv"] = D.fp8_block_quantize(tensors[name])
+    names = {torch.bfloat16: "BF16", torch.float32: "F32", torch.float8_e4m3fn: "F8_E4M3"}
+    head, blobs, at = {}, [], 0
+    for n, t in tensors.items():
+        blobs.append(bytes(t.contiguous().view(torch.uint8).numpy()))
+        head[n] = {"dtype": names[t.dtype], "shape": list(t.shape), "data_offsets": [at, at + len(blobs[-1])]}
+        at += len(blobs[-1])
+    text = json.dumps(head).encode()
+    text += b" " * (-len(text) % 8)
+    path.mkdir()
+    (path / "model.safetensors").write_bytes(struct.pack("<Q", len(text)) + text + b"".join(blobs))
+    raw = dict(model_type=cfg.model_type, hidden_size=cfg.hidden_size, intermediate_size=cfg.intermediate_size, num_hidden_layers=cfg.num_hidden_layers,
+               num_attention_heads=cfg.num_attention_heads, num_key_value_heads=cfg.num_key_value_heads, head_dim=cfg.head_dim, vocab_size=cfg.vocab_size)
+    if cfg.model_type == "qwen3_5":
+        raw.update(layer_types=cfg.layer_types, linear_num_key_heads=cfg.linear_num_key_heads, linear_key_head_dim=cfg.linear_key_head_dim,
+                   linear_num_value_heads=cfg.linear_num_value_heads, linear_value_head_dim=cfg.linear_value_head_dim, attn_output_gate=True,
+                   rope_parameters=dict(partial_rotary_factor=cfg.partial_rotary_factor))
+    (path / "config.json").write_text(json.dumps(raw))
+    return str(path)
+
+
+def model_args(*more):
+    import argparse
+    from slopllm_b200.cli import model_cli
+    ap = argparse.ArgumentParser()
+    model_cli.add_model_args(ap)
+    return ap.parse_args(["--cpu", "--act-dtype", "e4m3", "--max-pages", "8", *more])
+
+
+def test_checkpoints_whose_fp8_projections_take_no_rows(tmp_path, monkeypatch):
+    """FP8 in recurrent layers or in the down projection alone: refused by name, before anything is loaded."""
+    from slopllm_b200.cli import model_cli
+    from slopllm_b200.models import dense
+    from slopllm_b200.parallel.dist import ParallelContext
+    cfg, plain, cpu = dense.DenseConfig.tiny(hybrid=True), dense.DenseConfig.tiny(), ParallelContext(device=torch.device("cpu"))
+    linear = ("linear_attn.in_proj_qkv", "linear_attn.in_proj_z", "linear_attn.out_proj")
+    some = {"linear": (cfg, linear), "down": (plain, ("down_proj",)), "both": (cfg, (*linear, "self_attn.o_proj"))}
+    paths = {n: fp8_checkpoint(tmp_path / n, *x) for n, x in some.items()}
+    assert not dense.has_fp8_projections(plain, ["model.visual.layers.0.mlp.up_proj.weight_scale_inv", "mtp.layers.0.self_attn.q_proj.weight_scale_inv"])
+    _, model = dense.load_dense_model(paths["both"], cpu, act_dtype="e4m3")
+    assert [lw.o_proj.is_fp8 for lw in model.w.layers if lw.kind == "full_attention"] == [True]
+    monkeypatch.setattr(dense, "assemble_dense_weights", None)
+    for name in ("linear", "down"):
+        with pytest.raises(ValueError, match="has none"):
+            dense.load_dense_model(paths[name], cpu, act_dtype="e4m3")
+        with pytest.raises(SystemExit, match="has none"):
+            model_cli.build_runtime(model_args("--model", paths[name]), with_scheduler=False)
