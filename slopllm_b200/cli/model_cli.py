@@ -32,8 +32,8 @@ def add_model_args(ap: argparse.ArgumentParser) -> None:
                     help="type of cached keys and values: auto is the model's own; e4m3 keeps them in 8 bits with a scale per token and key head, "
                          "for about half of the cache's bytes (qwen3, qwen3_5; on a GPU heads of 64 or 128 values)")
     ap.add_argument("--act-dtype", choices=("auto", "e4m3"), default="auto",
-                    help="type of the rows in front of FP8 projections: auto is the model's own; e4m3 keeps an FP8 checkpoint's projections in FP8 and "
-                         "multiplies them with rows in 8 bits, a scale per 128 values (qwen3, qwen3_5)")
+                    help="type of the rows in front of FP8 projections: auto is the model's own; e4m3 keeps an FP8 checkpoint's projections of attention and MLP in FP8 and "
+                         "multiplies them with rows in 8 bits, a scale per 128 values (qwen3; qwen3_5, whose recurrent layers keep bf16 weights and rows)")
     ap.add_argument("--gpus", default="", help="comma-separated device list; its length must equal the number of ranks")
     ap.add_argument("--arena", type=float, default=0.0,
                     help="GiB of device memory this process may allocate per GPU (weights + KV cache + step buffers); a larger "
@@ -253,6 +253,12 @@ def build_runtime(args, with_scheduler: bool = True) -> Runtime:
         _refuse_act_dtype(args, ctx, reg, model_type, raw, model_dir)
         check_memory_plan(args, ctx, model_dir, model_type)
         cfg, model = load_registered(reg, model_dir, ctx, args.mtp, getattr(args, "dtype", None), _kv_dtype(args), _act_dtype(args))
+    if _act_dtype(args) is not None and ctx.rank == 0 and ctx.dp_rank == 0:
+        took, of = model.fp8_layers()
+        if took < of:
+            import sys
+            print(f"--act-dtype {_act_dtype(args)}: {took} of {of} matrices of the layers take rows in 8 bits; the others (of recurrent layers, of shards or fused "
+                  f"parts that end inside a block of 128, or not FP8 in the checkpoint) take them in the model's type", file=sys.stderr)
     if getattr(args, "max_model_len", None) is None:
         args.max_model_len = 65536
     if getattr(cfg, "max_positions", 0):

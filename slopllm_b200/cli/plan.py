@@ -58,7 +58,7 @@ def main(argv=None) -> int:
     ap.add_argument("--arena", type=float, default=0.0, help="GiB the process may allocate (0: the whole device)")
     ap.add_argument("--device-gb", type=float, default=180.0, help="device memory in GiB when --arena is not given")
     ap.add_argument("--kv-dtype", choices=("auto", "e4m3"), default="auto", help="type of cached keys and values (qwen3, qwen3_5; heads of 64 or 128 values)")
-    ap.add_argument("--act-dtype", choices=("auto", "e4m3"), default="auto", help="e4m3: an FP8 checkpoint's projections stay FP8 (qwen3, qwen3_5)")
+    ap.add_argument("--act-dtype", choices=("auto", "e4m3"), default="auto", help="e4m3: an FP8 checkpoint's projections of attention and MLP stay FP8 (qwen3, qwen3_5)")
     ap.add_argument("--context", type=int, default=0, help="longest sequence assumed for the workspace estimate")
     args = ap.parse_args(argv)
     cfg = _config(args)

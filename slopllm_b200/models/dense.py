@@ -248,6 +248,15 @@ class DenseModel(DecoderStack):
         """Whether a projection's rows come in 8 bits."""
         return self.act_dtype is not None and w.is_fp8
 
+    def fp8_layers(self):
+        """(matrices that take rows in 8 bits, matrices of the decoder's layers).  Recurrent layers, shards and parts of fused matrices that end inside a block
+        of scales, and what the checkpoint does not hold in FP8 take theirs as before."""
+        took = []
+        for lw in self.w.layers:
+            full, up = lw.kind == "full_attention", self._in_fp8(lw.mlp_w13)
+            took += [full and self._in_fp8(lw.w_qkv), full and self._in_fp8(lw.o_proj), up, up and self._in_fp8(lw.mlp_w2)]
+        return sum(took), len(took)
+
     # ---- layers -------------------------------------------------------------------------------------------
     @traced(lambda self, i, *a, **k: f"layer{i}.attention")
     def _full_attention(self, i: int, lw: DenseLayer, x, st, cache: DenseCache):

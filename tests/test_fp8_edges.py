@@ -114,3 +114,18 @@ def test_checkpoints_whose_fp8_projections_take_no_rows(tmp_path, monkeypatch):
             dense.load_dense_model(paths[name], cpu, act_dtype="e4m3")
         with pytest.raises(SystemExit, match="has none"):
             model_cli.build_runtime(model_args("--model", paths[name]), with_scheduler=False)
+
+
+def test_matrices_that_take_no_rows_in_8_bits_are_told(capsys, monkeypatch):
+    from slopllm_b200.cli import model_cli
+    from slopllm_b200.models.dense import DenseConfig, DenseModel, random_dense_model
+    from slopllm_b200.parallel.dist import ParallelContext
+    cpu = ParallelContext(device=torch.device("cpu"))
+    of = lambda cfg, tp=1: DenseModel(cfg, random_dense_model(cfg, 0, "cpu", torch.float32, 0, tp, fp8=True)[0], cpu, act_dtype="e4m3").fp8_layers()
+    assert of(DenseConfig.tiny()) == (8, 8) and of(DenseConfig.tiny(hybrid=True)) == (10, 16)
+    cut = DenseConfig(num_hidden_layers=1, vocab_size=512, hidden_size=256, intermediate_size=1216, num_attention_heads=4, num_key_value_heads=4, head_dim=64)
+    assert of(cut) == (2, 4) and of(cut, 2) == (2, 4)
+    for spec, told in (("qwen3-tiny", ""), ("qwen35-tiny", "10 of 16 matrices")):
+        model_cli.build_runtime(model_args("--random-init", spec), with_scheduler=False)
+        err = capsys.readouterr().err
+        assert told in err and bool(told) == ("--act-dtype" in err)
