@@ -124,7 +124,7 @@ class DecoderStack:
         if self.fp32_norms or sub.post_norm is not None:
             return ops.post_norm(self.comm.all_reduce(y), residual, sub.post_norm, norm, eps)
         if nxt is not None and nxt.fp8_input:
-            return F8.fp8_add_rmsnorm(y if self.ctx.world == 1 else self.comm._reduce_partial(y), residual, norm, eps)
+            return self.comm.allreduce_add_rmsnorm_fp8(y, residual, norm, eps)
         if nxt is not None and self.norm_ahead and self.ctx.world == 1 and hasattr(ops, "add_rmsnorm_ahead"):
             return ops.add_rmsnorm_ahead(y, residual, norm, eps)
         return self.comm.allreduce_add_rmsnorm(ops, y, residual, norm, eps)

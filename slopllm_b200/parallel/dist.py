@@ -14,6 +14,8 @@ from typing import List, Optional
 import torch
 import torch.distributed as dist
 
+from ..ops import fp8 as F8
+
 _PREFILL_AR_FP32 = os.environ.get("SLOPLLM_B200_PREFILL_AR_FP32", "0") == "1"
 
 
@@ -202,6 +204,10 @@ class Comm:
         if want_perm and getattr(ops, "name", "") == "cuda":
             return ops.add_rmsnorm(self._reduce_partial(partial), residual, weight, eps, want_perm=True)
         return ops.add_rmsnorm(self._reduce_partial(partial), residual, weight, eps)
+
+    def allreduce_add_rmsnorm_fp8(self, partial, residual, weight, eps):
+        """The same with the normed rows in 8 bits (`ops/fp8.py`)."""
+        return F8.fp8_add_rmsnorm(self._reduce_partial(partial), residual, weight, eps)
 
     PREFILL_AR_BF16_MIN_ROWS = 33
 

@@ -129,3 +129,34 @@ def test_matrices_that_take_no_rows_in_8_bits_are_told(capsys, monkeypatch):
         model_cli.build_runtime(model_args("--random-init", spec), with_scheduler=False)
         err = capsys.readouterr().err
         assert told in err and bool(told) == ("--act-dtype" in err)
+
+
+def test_communicators_join_rows_in_8_bits():
+    """Sums over the ranks and their norm in 8 bits are one call of the communicator, as those in 16 bits: what it overrides is used."""
+    from slopllm_b200.models.dense import DenseConfig, DenseModel, random_dense_model
+    from slopllm_b200.parallel.dist import Comm, ParallelContext
+    from slopllm_b200.runtime.engine import Engine
+    told = []
+
+    class Told(Comm):
+        def allreduce_add_rmsnorm_fp8(self, *args):
+            told.append(8)
+            return super().allreduce_add_rmsnorm_fp8(*args)
+
+        def allreduce_add_rmsnorm(self, *args, **kw):
+            told.append(16)
+            return super().allreduce_add_rmsnorm(*args, **kw)
+
+        def _reduce_partial(self, partial):
+            return super()._reduce_partial(partial) * 2
+
+    cfg, ctx = DenseConfig.tiny(), ParallelContext(device=torch.device("cpu"))
+    w, _ = random_dense_model(cfg, 0, "cpu", torch.float32, fp8=True)
+    logits = []
+    for comm in (Told(ctx), Comm(ctx)):
+        model = DenseModel(cfg, w, ctx, comm=comm, act_dtype="e4m3")
+        eng = Engine(cfg, model, num_pages=8, max_batch=2, max_seq_len=256)
+        s, _ = eng.kv.start_request([5, 6, 7])
+        _, hid = eng.prefill([s], [[5, 6, 7]], chunk_size=32, want_hidden=True)
+        logits.append(model.compute_logits(hid[0]))
+    assert told == [8, 8, 8, 16] and not torch.equal(*logits)
