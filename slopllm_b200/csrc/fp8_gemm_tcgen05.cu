@@ -353,7 +353,7 @@ bool aligned(const void* x, int ldx, const void* W, int ldw, const Fp8LinearPara
 }  // namespace
 
 // x: codes [T, K], rows `ldx` bytes apart; W: codes [N, K], rows `ldw` apart.  K, ldx, ldw and the rows of exponents are multiples of 16 and start there;
-// rows of y hold whole pieces of 16 bytes.
+// rows of y hold whole pieces of 16 bytes (the copy out of a pair's shared memory fills the last one up with zeros).
 SL_API int sl_fp8_linear(const void* x, int ldx, const void* W, int ldw, const Fp8LinearParams* params, cudaStream_t s) {
     const Fp8LinearParams& p = *params;
     if (p.T <= 0 || p.N <= 0) return 0;

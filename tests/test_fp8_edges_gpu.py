@@ -151,3 +151,98 @@ def test_more_columns_than_a_grid_has():
             F8.fp8_linear(some_rows(t, 16), w)
     y = F8.fp8_linear(some_rows(1, 16), LinearWeight(codes[1:].contiguous(), fp8_scale=w.fp8_scale[1:]))
     assert y.shape == (1, n - 1) and (y == 0).all()
+
+class Around:
+    """Rows of `width` bytes, `ld` apart, in a piece of memory whose every other byte is 0xa5 and has to stay so, but for those up to the next multiple of `piece`
+    behind a row."""
+
+    def __init__(self, rows, width, ld, piece=1, margin=8192):
+        self.rows, self.width, self.ld, self.margin, self.written = rows, width, ld, margin, -(-width // piece) * piece
+        self.space = torch.full((2 * margin + rows * ld,), 0xa5, dtype=torch.uint8, device="cuda")
+        self.at = self.space.data_ptr() + margin
+
+    def get(self, dtype=torch.uint8):
+        """The rows, once nothing else is found to be written."""
+        inside = self.space[self.margin:self.margin + self.rows * self.ld].view(self.rows, self.ld)
+        for other in (self.space[:self.margin], self.space[self.margin + self.rows * self.ld:], inside[:, self.written:]):
+            assert (other == 0xa5).all()
+        return inside[:, :self.width].contiguous().view(dtype)
+
+
+# forms of the product: one SM with 16, 32 and 64 rows, pairs with 128 and 256 columns, shares of K
+@pytest.mark.parametrize("t,n,k", [(1, 1, 16), (3, 130, 4112), (17, 130, 400), (40, 1001, 400), (65, 1001, 400), (129, 1001, 2064), (257, 130, 400), (1500, 1001, 400),
+                                   (4500, 130, 272), (333, 2321, 2064), (300, 1001, 144), (2500, 2321, 144), (1000, 1001, 16)])
+@pytest.mark.parametrize("f32", [True, False])
+def test_what_lies_around_a_product(t, n, k, f32):
+    """Columns behind the last piece of 16 bytes, rows behind the last and what is in front of the first are left as they were."""
+    (w, _), rows = weight(n, k, 25), some_rows(t, k, 26)
+    size = 4 if f32 else 2
+    for more in (0, 32):
+        ld = -(-n * size // 16) * 16 + more
+        y = Around(t, n * size, ld, 16)
+        F8._multiply("sl_fp8_linear", 0, rows, w.weight, n, w.fp8_scale, y.at, ld // size, f32)
+        assert torch.equal(y.get(torch.float32 if f32 else torch.bfloat16), F8.fp8_linear(rows, w, out_f32=f32))
+    tcgen05.check_errors(rows.device)
+
+
+@pytest.mark.parametrize("t,inner,k", [(65, 128, 144), (129, 384, 400), (257, 256, 144), (300, 512, 400), (2100, 1152, 272)])
+def test_what_lies_around_gated_rows_of_a_product(t, inner, k):
+    (w, _), rows = weight(2 * inner, k, 27), some_rows(t, k, 28)
+    codes, exps = Around(t, inner, inner + 32), Around(t, inner // 128, -(-inner // 2048) * 16 + 16)
+    F8._multiply("sl_fp8_gate_up", 0, rows, w.weight, 2 * inner, w.fp8_scale, codes.at, codes.ld, False, exps.at, exps.ld)
+    want = F8.fp8_silu_mul(F8.fp8_linear(rows, w, out_f32=True))
+    assert (exps.get() == want.exps).all() and (codes.get() != want.codes).float().mean() < 1e-4
+    if F8._on_pairs(t, 2 * inner, k):
+        got = F8.fp8_gate_up(rows, w)
+        assert torch.equal(codes.get(), got.codes) and torch.equal(exps.get(), got.exps)
+    tcgen05.check_errors(rows.device)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("t,k", [(1, 16), (3, 144), (17, 272), (300, 4112), (2500, 1040)])
+def test_what_lies_around_rows(t, k, dtype):
+    """Codes, exponents, residuals and values that are read back."""
+    import ctypes as C
+    x = torch.randn(t, 2 * k, generator=gen(29), device="cuda").to(dtype)
+    w, groups = torch.rand(k, generator=gen(30), device="cuda"), -(-k // 128)
+    f32 = dtype is torch.float32
+    res = torch.randn(t, k, generator=gen(31), device="cuda")
+
+    def rows():
+        return Around(t, k, k + 16), Around(t, groups, F8._padded(k) + 16)
+
+    def put(codes, exps):
+        return codes.at, codes.ld, exps.at, exps.ld
+
+    for gated, want in ((False, F8.fp8_rows(x[:, :k])), (True, F8.fp8_silu_mul(x))):
+        codes, exps = rows()
+        p = F8.Fp8RowsParams(x.data_ptr(), x.stride(0), t, k, *put(codes, exps))
+        F8._call(0, "sl_fp8_rows", C.byref(p), gated, f32)
+        assert torch.equal(codes.get(), want.codes) and torch.equal(exps.get(), want.exps)
+    values = Around(t, 2 * k, 2 * k)
+    p = F8.Fp8ValuesParams(*want._where(), t, k, values.at)
+    F8._call(0, "sl_fp8_values", C.byref(p))
+    assert torch.equal(values.get(torch.bfloat16), F8.fp8_values(want))
+    part = x[:, :k]
+    (codes, exps), r = rows(), Around(t, 4 * k, 4 * k)
+    p = F8.Fp8NormParams(part.data_ptr(), part.stride(0), res.data_ptr(), res.stride(0), w.data_ptr(), k, 1e-6, r.at, *put(codes, exps))
+    F8._call(0, "sl_fp8_add_rmsnorm", C.byref(p), t, f32, True)
+    want, r_want = F8.fp8_add_rmsnorm(part, res, w, 1e-6)
+    assert torch.equal(codes.get(), want.codes) and torch.equal(exps.get(), want.exps) and torch.equal(r.get(torch.float32), r_want)
+
+def test_residuals_and_scales_far_apart():
+    """Rows of the residual and of scales more than 2^31 values apart."""
+    step = 2 ** 31 + 64
+    space = torch.empty(step + 512, dtype=torch.float32, device="cuda")
+    far = torch.as_strided(space, (2, 512), (step, 1))
+    far.copy_(torch.randn(2, 512, generator=gen(32), device="cuda"))
+    x, w = torch.randn(2, 512, generator=gen(33), device="cuda"), torch.rand(512, generator=gen(34), device="cuda")
+    (got, r), (want, r_want) = (F8.fp8_add_rmsnorm(x, a, w, 1e-6) for a in (far, far.contiguous()))
+    assert torch.equal(r, r_want) and torch.equal(got.codes, want.codes) and torch.equal(got.exps, want.exps)
+    for n in (200, 512):
+        (w, _), rows = weight(n, 500 // 16 * 16, 35), some_rows(100, 496, 36)
+        scale = torch.as_strided(space, (w.fp8_scale.shape[0], 4), (step // (w.fp8_scale.shape[0] - 1) // 4 * 4, 1))
+        assert n > 256 or scale.stride(0) > 2 ** 31
+        scale.copy_(w.fp8_scale)
+        assert torch.equal(F8.fp8_linear(rows, LinearWeight(w.weight, fp8_scale=scale)), F8.fp8_linear(rows, w))
+    tcgen05.check_errors(rows.device)
