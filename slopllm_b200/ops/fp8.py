@@ -296,7 +296,8 @@ def _on_pairs(tokens: int, n: int, k: int) -> bool:
 
 def fp8_linear(rows: Fp8Rows, w, out_f32: bool = False) -> torch.Tensor:
     """y = rows @ W^T [T, N], fp32 sums, in bf16 or fp32.  `w`: a :class:`~slopllm_b200.models.weights.LinearWeight` in FP8.  A NaN code spoils its row's (a
-    weight's: its column's) results and no other."""
+    weight's: its column's) results and no other.  A block's factor, its scale times 2^exponent, is an fp32 number: results are those of the values as
+    long as it is a normal one (scales of 2^67 and more, or below 2^-66, leave that range together with exponents at their limits)."""
     codes, scale, device = _operands(rows, w)
     n, kind = codes.shape[0], torch.float32 if out_f32 else torch.bfloat16
     if device < 0:
@@ -310,7 +311,8 @@ def fp8_linear(rows: Fp8Rows, w, out_f32: bool = False) -> torch.Tensor:
 
 def fp8_gate_up(rows: Fp8Rows, w) -> Fp8Rows:
     """silu(rows @ Wg^T) * (rows @ Wu^T) in 8 bits, W = gate rows | up rows [2 I, K]: :func:`fp8_silu_mul` of the product's fp32 sums.  Many rows make the
-    activation in the product's epilogue, in fp32 (I a multiple of 128): a value next to the middle between two codes may get the other one."""
+    activation in the product's epilogue, in fp32 (I a multiple of 128): a value next to the middle between two codes may get the other one, and a gate
+    below -87 gives zeros (its SiLU is below 1e-36)."""
     n = w.weight.shape[0]
     if n % 32:
         raise ValueError(f"{n} gate and up rows: rows in 8 bits have a multiple of 16 values")

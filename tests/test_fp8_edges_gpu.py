@@ -246,3 +246,93 @@ def test_residuals_and_scales_far_apart():
         scale.copy_(w.fp8_scale)
         assert torch.equal(F8.fp8_linear(rows, LinearWeight(w.weight, fp8_scale=scale)), F8.fp8_linear(rows, w))
     tcgen05.check_errors(rows.device)
+
+
+# ---- the activation in a product's epilogue --------------------------------------------------------------------------------------------
+#
+# Against `fp8_silu_mul` of the fp32 product, which is the definition's nearest.  Codes may be the neighbour's where the two fp32 values lie on different sides of a
+# middle: both are within some 20 units of 2^-24 (gates of -16) of the value, middles are 2^-4 of a value apart or more, so that fewer than
+# 2 * 20 * 2^-24 * 2^4 = 4e-5 of evenly spread codes are; an exponent likewise where a group's largest value lies next to a limit, of which these cases have none.
+# Products of two codes are not evenly spread, many are a middle themselves: where sums are exact, the value of each code that differs is looked at.
+
+def fused_and_apart(rows, w, t, n, k):
+    assert F8._on_pairs(t, n, k)
+    return F8.fp8_gate_up(rows, w), F8.fp8_silu_mul(F8.fp8_linear(rows, w, out_f32=True))
+
+
+def agree(got, want, value=None):
+    tcgen05.check_errors(got.device)
+    a, b = held(got), held(want)
+    assert torch.equal(got.exps, want.exps) and torch.equal(a.isnan(), b.isnan())
+    step = torch.exp2(want.exps.double() - 127).repeat_interleave(128, 1)
+    off = (a - b).nan_to_num(0.0).abs()
+    assert (off <= torch.maximum(2.0 ** -3 * b.nan_to_num(0.0).abs(), 2.0 ** -9 * step)).all()
+    if value is None:
+        assert (off > 0).sum() <= 2 + 4e-5 * off.numel(), (off > 0).sum()
+    else:
+        middle = (a + b) / 2
+        assert ((off == 0) | ((value - middle).abs() <= 20 * 2.0 ** -24 * middle.abs())).all()
+
+
+def chosen(gate, up):
+    """Rows and weights whose product has column j of weight row i at [j, i]: gates and ups [t, inner] as they are given, up to a power of two."""
+    t, inner = gate.shape
+    k = -(-t // 128) * 128
+    codes = torch.zeros(2 * inner, k, dtype=torch.uint8, device="cuda")
+    codes[:inner, :t] = gate.t().to(torch.float8_e4m3fn).view(torch.uint8)
+    codes[inner:, :t] = up.t().to(torch.float8_e4m3fn).view(torch.uint8)
+    rows = F8.Fp8Rows.allocate(t, k, "cuda")
+    rows.codes.copy_(torch.nn.functional.pad(torch.eye(t, device="cuda") * 2.0, (0, k - t)).to(torch.float8_e4m3fn).view(torch.uint8))
+    rows.exps.fill_(126)                                  # 2 * 2^-1
+    return rows, LinearWeight(codes.view(torch.float8_e4m3fn), fp8_scale=torch.ones(2 * inner // 128, k // 128, device="cuda"))
+
+
+def test_gates_of_all_sizes_in_the_epilogue():
+    """Gates of every code (up to 448 either way: those below -87 are zeros), and around -16, -88 and 88, times ups of every code."""
+    t, inner = 254, 512
+    codes = torch.tensor([c for c in range(256) if c & 127 != 127], dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn).float()
+    gate = codes[:, None].expand(t, inner)
+    up = codes[torch.randint(0, 254, (t, inner), generator=gen(40), device="cuda")]
+    for g in (gate, gate[torch.randperm(254, generator=gen(41), device="cuda")], torch.tensor([-15., -16, -18, -80, -88, -96, 80, 88, 96, 448.], device="cuda")[
+            torch.randint(0, 10, (t, inner), generator=gen(42), device="cuda")]):
+        rows, w = chosen(g, up)
+        got, want = fused_and_apart(rows, w, t, 2 * inner, rows.shape[1])
+        value = silu_mul(torch.cat([g.to(torch.float8_e4m3fn).float(), up], 1))
+        assert same(want, value)
+        agree(got, want, value)
+
+
+@pytest.mark.parametrize("t,inner,k", [(129, 384, 400), (300, 512, 400), (700, 1024, 528)])
+def test_numbers_that_are_not_finite_in_the_epilogue(t, inner, k):
+    """A NaN code of a row spoils its row, one of a gate's or an up's weight its column, and no other value or exponent."""
+    (w, _), rows = weight(2 * inner, k, 43), some_rows(t, k, 44)
+    clean, _ = fused_and_apart(rows, w, t, 2 * inner, k)
+    rows.codes[t // 2, 3] = 0x7f
+    codes = w.weight.view(torch.uint8)
+    codes[5, 390], codes[inner + 130, 17] = 0xff, 0x7f
+    got, want = fused_and_apart(rows, w, t, 2 * inner, k)
+    agree(got, want)
+    bad = torch.zeros(t, inner, dtype=torch.bool, device="cuda")
+    bad[t // 2], bad[:, 5], bad[:, 130] = True, True, True
+    assert torch.equal(held(got).isnan(), bad) and (got.exps[t // 2] == 67).all()
+    assert (got.codes == clean.codes)[:, 256:][~bad[:, 256:]].all()
+
+
+@pytest.mark.parametrize("t,inner,k", [(129, 384, 400), (300, 512, 400), (700, 1024, 528)])
+def test_limits_of_the_format_in_the_epilogue(t, inner, k):
+    """Rows of zeros, products that saturate and that leave fp32, that lie below the smallest code, and scales far apart from block to block."""
+    for up, more, spread in ((0, 0, 6), (60, 30, 1), (60, 57, 1), (-50, -25, 1), (-50, -50, 1)):       # (powers of two of up's scales and of the rows)
+        (w, _), rows = weight(2 * inner, k, 45, spread=spread), some_rows(t, k, 46, spread=40 if spread > 1 else 1)
+        rows.codes[1::3] = 0
+        scale = w.fp8_scale.clone()
+        scale[inner // 128:] *= 2.0 ** up
+        rows.exps.add_(more)
+        got, want = fused_and_apart(rows, LinearWeight(w.weight, fp8_scale=scale), t, 2 * inner, k)
+        agree(got, want)
+        assert (got.codes[1::3] == 0).all() and (got.exps[1::3] == 67).all()
+        if (up, more) == (60, 30):
+            assert (got.exps == 187).any() and (got.codes & 127 == 126).any()
+        if more == 57:
+            assert held(got).isnan().any() and held(got).isfinite().any()
+        if more == -50:
+            assert (got.exps == 67).all()
