@@ -134,8 +134,9 @@ def check_memory_plan(args, ctx: ParallelContext, model_dir: str, model_type: st
         from ..models.dense import DenseConfig
         with open(os.path.join(model_dir, "config.json")) as f:
             dcfg = DenseConfig.from_hf_dict(json.load(f))
+        fp8 = False if _act_dtype(args) is None else set(_tensor_names(model_dir))
         p = plan_dense(dcfg, world=ctx.world, batch_size=args.batch_size, chunk_size=args.chunk_size, max_pages=args.max_pages,
-                       arena_gb=args.arena, device_gb=total / GIB, fp8=_act_dtype(args) is not None, kv_dtype=_kv_dtype(args))
+                       arena_gb=args.arena, device_gb=total / GIB, fp8=fp8, kv_dtype=_kv_dtype(args))
     if p.requested_fits:
         return None
     msg = (f"memory plan: {p.weights_bytes / GIB:.1f} GiB of weights per rank + about {p.workspace_bytes / GIB:.1f} GiB of "
@@ -156,6 +157,14 @@ def _act_dtype(args) -> Optional[str]:
     return None if name == "auto" else name
 
 
+def _tensor_names(model_dir: str):
+    """Names of a checkpoint's tensors."""
+    from ..checkpoint.safetensors_io import SafetensorsFile
+    for f in sorted(os.listdir(model_dir)):
+        if f.endswith(".safetensors"):
+            yield from SafetensorsFile(os.path.join(model_dir, f)).names()
+
+
 def _refuse_act_dtype(args, ctx: ParallelContext, reg, model_type: str, raw: dict, model_dir: str) -> None:
     """Ends with a line of text where a checkpoint's rows do not go to its projections in the type asked for."""
     act_dtype = _act_dtype(args)
@@ -163,15 +172,13 @@ def _refuse_act_dtype(args, ctx: ParallelContext, reg, model_type: str, raw: dic
         return
     if not reg.act8:
         raise SystemExit(f"{args.model}: {model_type} does not take activations in {act_dtype}")
-    from ..checkpoint.safetensors_io import SafetensorsFile
     from ..models.dense import DenseConfig, check_act_dtype, has_fp8_projections
     cfg = DenseConfig.from_hf_dict(raw)
     try:
         check_act_dtype(cfg, act_dtype, ctx.world, ctx.device.type == "cuda")
     except ValueError as e:
         raise SystemExit(f"{args.model}: {e}")
-    shards = (os.path.join(model_dir, f) for f in sorted(os.listdir(model_dir)) if f.endswith(".safetensors"))
-    if not any(has_fp8_projections(cfg, SafetensorsFile(f).names()) for f in shards):
+    if not has_fp8_projections(cfg, _tensor_names(model_dir)):
         raise SystemExit(f"{args.model}: activations in 8 bits go with FP8 projections, and this checkpoint has none")
 
 

@@ -297,7 +297,7 @@ def _on_pairs(tokens: int, n: int, k: int) -> bool:
 def fp8_linear(rows: Fp8Rows, w, out_f32: bool = False) -> torch.Tensor:
     """y = rows @ W^T [T, N], fp32 sums, in bf16 or fp32.  `w`: a :class:`~slopllm_b200.models.weights.LinearWeight` in FP8.  A NaN code spoils its row's (a
     weight's: its column's) results and no other.  A block's factor, its scale times 2^exponent, is an fp32 number: results are those of the values as
-    long as it is a normal one (scales of 2^67 and more, or below 2^-66, leave that range together with exponents at their limits)."""
+    long as it is a normal one (scales of 2^68 and more, or below 2^-66, leave that range together with exponents at their limits)."""
     codes, scale, device = _operands(rows, w)
     n, kind = codes.shape[0], torch.float32 if out_f32 else torch.bfloat16
     if device < 0:

@@ -149,27 +149,32 @@ def plan_memory(cfg: GlmMoeDsaConfig, world: int = 1, cp: bool = False, ep: bool
 
 # ---- dense families (Qwen3, Qwen3.5) -----------------------------------------------------------------------------------
 
-def dense_weight_bytes(cfg, tp: int = 1, elem: int = 2, fp8: bool = False) -> int:
+GROUP_OF = {p: "self_attn" for p in "qkvo"} | {p: "mlp" for p in ("gate", "up", "down")}       # where a layer keeps its projections
+
+
+def dense_weight_bytes(cfg, tp: int = 1, elem: int = 2, fp8=False) -> int:
     """Per-rank weight bytes of a Qwen3 / Qwen3.5 decoder: attention and Gated-DeltaNet projections head-sharded, MLP
-    column / row sharded, embedding whole, lm_head vocabulary-sharded.  `fp8`: the attention and MLP projections stay FP8
-    (one byte per weight + one fp32 scale per 128 x 128 block) where the loader keeps them: shards end on a block's edge, and so does each
+    column / row sharded, embedding whole, lm_head vocabulary-sharded.  `fp8`: the attention and MLP projections (those that
+    the checkpoint holds in FP8, where it is a set of its tensors' names) stay FP8 (one byte per weight + one fp32 scale per 128 x 128 block) where the loader keeps them: shards end on a block's edge, and so does each
     part of a fused matrix but the last.  (Where they do not, the last rank's may; rank 0's, which is counted, does not.)"""
     H, I, hd = cfg.hidden_size, cfg.intermediate_size, cfg.head_dim
 
     def lin(n, k, quant=False):
         return n * k + (-(-n // 128)) * (-(-k // 128)) * 4 if quant else n * k * elem
 
-    def whole(*parts):                                              # a rank's rows (or columns) of one matrix
-        return fp8 and all(n % 128 == 0 for n in (parts if tp > 1 else parts[:-1]))
+    def whole(i, **parts):                                          # a rank's rows (or columns) of one matrix, by projection
+        held = fp8 if isinstance(fp8, bool) else all(f"{cfg.weight_prefix}layers.{i}.{GROUP_OF[p]}.{p}_proj.weight_scale_inv" in fp8 for p in parts)
+        return held and all(n % 128 == 0 for n in (list(parts.values()) if tp > 1 else list(parts.values())[:-1]))
     b = cfg.vocab_size * H * elem + H * elem
     b += (cfg.vocab_size // tp) * H * elem                         # the head's shard is materialised even when it is tied
-    for kind in cfg.layer_types:
+    for i, kind in enumerate(cfg.layer_types):
         b += 2 * H * elem                                           # the two layer norms
-        b += lin(2 * (I // tp), H, whole(I // tp, I // tp)) + lin(H, I // tp, whole(I // tp))
+        b += lin(2 * (I // tp), H, whole(i, gate=I // tp, up=I // tp)) + lin(H, I // tp, whole(i, down=I // tp))
         if kind == "full_attention":
             qs = hd * (2 if cfg.attn_output_gate else 1)
             hq, hk = cfg.num_attention_heads // tp, max(1, cfg.num_key_value_heads // tp)
-            b += lin(hq * qs + 2 * hk * hd, H, whole(hq * qs, hk * hd, hk * hd)) + lin(H, hq * hd, whole(hq * hd)) + 2 * hd * elem      # qkv, o_proj, q/k norms
+            b += lin(hq * qs + 2 * hk * hd, H, whole(i, q=hq * qs, k=hk * hd, v=hk * hd)) + lin(H, hq * hd, whole(i, o=hq * hd))
+            b += 2 * hd * elem                                                                  # (qkv, o_proj,) q/k norms
         else:
             lh, dk, dv = cfg.linear_num_key_heads // tp, cfg.linear_key_head_dim, cfg.linear_value_head_dim
             conv_dim = lh * (2 * dk + dv)
@@ -187,7 +192,7 @@ def dense_kv_page_bytes(cfg, tp: int = 1, elem: int = 2, kv_dtype=None) -> int:
 
 
 def plan_dense(cfg, world: int = 1, batch_size: int = 8, chunk_size: int = 8192, max_pages: int = 0, arena_gb: float = 0.0,
-               device_gb: float = 180.0, fp8: bool = False, reserve_gb: float = 4.0, kv_dtype=None) -> MemoryPlan:
+               device_gb: float = 180.0, fp8=False, reserve_gb: float = 4.0, kv_dtype=None) -> MemoryPlan:
     """`plan_memory` for the dense families (tensor parallel only; the workspace estimate is the residual / activation rows
     plus the MLP's gate-up rows of one chunk, and the rows that prompts read back from an 8-bit cache)."""
     if kv_dtype is not None:

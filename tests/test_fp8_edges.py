@@ -160,3 +160,25 @@ def test_communicators_join_rows_in_8_bits():
         _, hid = eng.prefill([s], [[5, 6, 7]], chunk_size=32, want_hidden=True)
         logits.append(model.compute_logits(hid[0]))
     assert told == [8, 8, 8, 16] and not torch.equal(*logits)
+
+
+@pytest.mark.parametrize("keep", [("o_proj",), ("gate_proj", "up_proj"), ("q_proj", "k_proj", "down_proj"), ("q_proj", "k_proj", "v_proj", "o_proj", "gate_proj", "up_proj", "down_proj")])
+def test_plans_count_what_a_checkpoint_holds(tmp_path, keep):
+    """A checkpoint that is partly FP8: its loaded weights against the plan from its tensors' names."""
+    from slopllm_b200.cli.model_cli import _tensor_names
+    from slopllm_b200.models.dense import DenseConfig, load_dense_model
+    from slopllm_b200.parallel.dist import ParallelContext
+    from slopllm_b200.runtime.workspace import walk_tensors
+    from slopllm_b200.utils.sizing import dense_weight_bytes
+    cfg = DenseConfig(num_hidden_layers=2, vocab_size=512, hidden_size=256, intermediate_size=512, num_attention_heads=4, num_key_value_heads=4, head_dim=64)
+    path = fp8_checkpoint(tmp_path / "model", cfg, keep)
+    if keep != ("q_proj", "k_proj", "down_proj"):
+        cfg, model = load_dense_model(path, ParallelContext(device=torch.device("cpu")), act_dtype="e4m3")
+        w = model.w
+    else:                                                 # (q, k and v are one matrix: nothing takes rows in 8 bits, the plan counts it all the same)
+        from slopllm_b200.checkpoint.safetensors_io import load_dir
+        from slopllm_b200.models.dense import assemble_dense_weights
+        w = assemble_dense_weights(cfg, load_dir(path), "cpu", torch.bfloat16, keep_fp8=True)
+    seen = {}
+    walk_tensors(w, lambda t: seen.setdefault(t.data_ptr(), t.numel() * t.element_size()))
+    assert dense_weight_bytes(cfg, 1, fp8=set(_tensor_names(path))) == sum(seen.values())

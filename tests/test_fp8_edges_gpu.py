@@ -336,3 +336,23 @@ def test_limits_of_the_format_in_the_epilogue(t, inner, k):
             assert held(got).isnan().any() and held(got).isfinite().any()
         if more == -50:
             assert (got.exps == 67).all()
+
+
+def test_a_checkpoint_that_a_command_serves(tmp_path, capsys):
+    """Partly FP8: planned by its tensors' names, loaded, told about, and a token made."""
+    from slopllm_b200.cli import model_cli
+    from slopllm_b200.models.dense import DenseConfig
+    from test_fp8_edges import fp8_checkpoint
+    import argparse
+    cfg = DenseConfig(num_hidden_layers=2, vocab_size=512, hidden_size=256, intermediate_size=512, num_attention_heads=4, num_key_value_heads=4, head_dim=64)
+    path = fp8_checkpoint(tmp_path / "model", cfg, ("o_proj", "gate_proj", "up_proj", "down_proj"))
+    ap = argparse.ArgumentParser()
+    model_cli.add_model_args(ap)
+    args = ["--act-dtype", "e4m3", "--max-pages", "8", "--batch-size", "2", "--model", path]
+    rt = model_cli.build_runtime(ap.parse_args(args), with_scheduler=False)
+    assert "6 of 8 matrices" in capsys.readouterr().err and rt.engine.model.fp8_layers() == (6, 8)
+    s = rt.engine.kv.new_sequence()
+    last, _ = rt.engine.prefill([s], [list(range(2, 100))], chunk_size=64)
+    assert 0 <= last[0] < cfg.vocab_size and 0 <= rt.engine.decode_step([s], last)[0] < cfg.vocab_size
+    plan = model_cli.check_memory_plan(ap.parse_args([*args, "--max-pages", str(10 ** 8)]), rt.ctx, path, "qwen3")
+    assert "memory plan" in plan
