@@ -182,3 +182,37 @@ def test_plans_count_what_a_checkpoint_holds(tmp_path, keep):
     seen = {}
     walk_tensors(w, lambda t: seen.setdefault(t.data_ptr(), t.numel() * t.element_size()))
     assert dense_weight_bytes(cfg, 1, fp8=set(_tensor_names(path))) == sum(seen.values())
+
+
+def test_what_a_layer_calls(monkeypatch):
+    """Which operators a forward pass goes through, with which weights, epsilon and types of results: what a comparison of logits is too wide to see."""
+    from slopllm_b200.models.dense import DenseConfig, DenseModel, random_dense_model
+    from slopllm_b200.parallel.dist import ParallelContext
+    from slopllm_b200.runtime.engine import Engine
+    cfg = DenseConfig(num_hidden_layers=2, vocab_size=512, hidden_size=256, intermediate_size=512, num_attention_heads=4, num_key_value_heads=4, head_dim=64,
+                      rms_norm_eps=3e-3)
+    w, _ = random_dense_model(cfg, 0, "cpu", torch.float32, fp8=True)
+    told = []
+
+    def spy(name, which):
+        plain = getattr(F8, name)
+
+        def call(*args, **kw):
+            told.append((name, *which(*args, **kw)))
+            return plain(*args, **kw)
+        monkeypatch.setattr(F8, name, call)
+
+    at = {id(x): (i, n) for i, lw in enumerate(w.layers) for n in ("w_qkv", "o_proj", "mlp_w13", "mlp_w2", "input_norm", "post_attn_norm") for x in [getattr(lw, n)]}
+    spy("fp8_add_rmsnorm", lambda x, r, n, eps: (at[id(n)], eps, r is None))
+    spy("fp8_rows", lambda x: (tuple(x.shape),))
+    spy("fp8_linear", lambda rows, m, out_f32=False: (at[id(m)], out_f32))
+    spy("fp8_gate_up", lambda rows, m: (at[id(m)],))
+    eng = Engine(cfg, DenseModel(cfg, w, ParallelContext(device=torch.device("cpu")), act_dtype="e4m3"), num_pages=8, max_batch=2, max_seq_len=256)
+    s = eng.kv.new_sequence()
+    eng.prefill([s], [[5, 6, 7]], chunk_size=32)
+    want = []
+    for i in (0, 1):
+        want += [("fp8_add_rmsnorm", (i, "input_norm"), 3e-3, i == 0), ("fp8_linear", (i, "w_qkv"), True), ("fp8_rows", (3, 256)), ("fp8_linear", (i, "o_proj"), True),
+                 ("fp8_add_rmsnorm", (i, "post_attn_norm"), 3e-3, False), ("fp8_gate_up", (i, "mlp_w13")), ("fp8_linear", (i, "mlp_w13"), True),
+                 ("fp8_linear", (i, "mlp_w2"), True)]
+    assert told == want
