@@ -62,7 +62,7 @@ __device__ __forceinline__ uint32_t quantize_group(float (&v)[4], uint32_t withi
     const float most = max3(max3(0.f, fabsf(v[0]), fabsf(v[1])), fabsf(v[2]), fabsf(v[3]));
     uint32_t top = __reduce_max_sync(0xffffffffu, __float_as_uint(most));          // (max passes over NaN)
     if (within != 0) all |= top >= INFINITE - within - 1;    // (64 bits say which of them fp32 holds)
-    if (top == INFINITE) {                                // an infinity: a NaN from here on, and not the largest magnitude
+    if (top == INFINITE) {                                   // an infinity: a NaN from here on, and not the largest magnitude
         top = 0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {

@@ -155,8 +155,9 @@ GROUP_OF = {p: "self_attn" for p in "qkvo"} | {p: "mlp" for p in ("gate", "up", 
 def dense_weight_bytes(cfg, tp: int = 1, elem: int = 2, fp8=False) -> int:
     """Per-rank weight bytes of a Qwen3 / Qwen3.5 decoder: attention and Gated-DeltaNet projections head-sharded, MLP
     column / row sharded, embedding whole, lm_head vocabulary-sharded.  `fp8`: the attention and MLP projections (those that
-    the checkpoint holds in FP8, where it is a set of its tensors' names) stay FP8 (one byte per weight + one fp32 scale per 128 x 128 block) where the loader keeps them: shards end on a block's edge, and so does each
-    part of a fused matrix but the last.  (Where they do not, the last rank's may; rank 0's, which is counted, does not.)"""
+    the checkpoint holds in FP8, where it is a set of its tensors' names) stay FP8 (one byte per weight + one fp32 scale per
+    128 x 128 block) where the loader keeps them: shards end on a block's edge, and so does each part of a fused matrix but
+    the last.  (Where they do not, the last rank's may; rank 0's, which is counted, does not.)"""
     H, I, hd = cfg.hidden_size, cfg.intermediate_size, cfg.head_dim
 
     def lin(n, k, quant=False):
